@@ -1,0 +1,289 @@
+// Eviction from a cache of bounded size: of the rows that a sequence holds, `budget` stay.
+//
+// For every (sequence, kv head): n = lengths[s] rows; row j has gathered weights[j] and stands for the token at positions[j], or, for the rows
+// of the last step (j >= past[s]), at seen[s] - (n - j). With n <= budget all stay. Otherwise those stay that come first by
+//   (position < first or position >= seen - recent, before the others; then the larger weight, NaN last; then the lower row),
+// and the rows that stay but lie at budget or behind move, in ascending order, into the places below budget of those that go, in ascending
+// order: the least that has to be moved, and no place is read and written both. Rows of a cache are in no order of positions after that,
+// which attention over all rows does not ask for.
+//
+// A block takes one (sequence, kv head). The order is one 32-bit key a row (the weight's bits made ascending, all ones for protected rows),
+// kept in shared memory; a radix descent of four digits of eight bits finds the key of the last row that stays, and how many of the rows with
+// that very key stay (the lowest). Counts are whole numbers, so neither the blocks' nor the threads' order matters. Rows are dealt to the
+// threads in runs, so that ranks within a run are sums of a block-wide scan. Where a step can move a few rows only, the block moves them
+// itself; else it leaves the lists for a second kernel with a half warp a row.
+// Bound by latency: a block's descent; the bytes are the weights and positions once and the moved rows twice.
+#include "common.cuh"
+
+namespace slb {
+
+constexpr int kEvictThreads = 1024;
+constexpr int kFewMoves = 32;
+
+struct EvictArgs {
+  const float* weights;      // [slots, K, capacity]
+  float* weights_out;
+  const int* positions;
+  int* positions_out;
+  long long capacity;
+  char* k_pool;
+  char* v_pool;
+  const int* block_table;
+  const int* past;
+  const int* lengths;
+  const int* seen;
+  const int* slots;
+  int* scratch;              // with many moves: per (sequence, kv head) their number, the places, the rows
+  int table_stride, n_seqs, kv_heads, row_bytes, budget, first, recent, max_length, keys_fit, most_moves, vector;
+};
+
+__device__ __forceinline__ uint32_t order_key(float w, bool safe) {
+  if (safe) return 0xffffffffu;
+  if (w != w) return 0u;
+  const uint32_t b = __float_as_uint(w + 0.0f);      // -0 counts as 0
+  return (b & 0x80000000u) ? ~b : b | 0x80000000u;   // between 0x007fffff (-inf) and 0xff800000 (inf)
+}
+
+// Exclusive sum over the block's threads of two counts packed in one word (each below 2^32), and the totals.
+__device__ __forceinline__ unsigned long long block_scan(unsigned long long v, unsigned long long* warp_sums, unsigned long long& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  unsigned long long x = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const unsigned long long y = __shfl_up_sync(0xffffffffu, x, d);
+    if (lane >= d) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    unsigned long long w = lane < (int)(blockDim.x >> 5) ? warp_sums[lane] : 0ull;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const unsigned long long y = __shfl_up_sync(0xffffffffu, w, d);
+      if (lane >= d) w += y;
+    }
+    warp_sums[lane] = w;
+  }
+  __syncthreads();
+  total = warp_sums[31];
+  return x - v + (warp ? warp_sums[warp - 1] : 0ull);
+}
+
+__device__ __forceinline__ size_t pool_row(const EvictArgs& a, const int* table, int kh, int j) {
+  return ((size_t)table[j / kPageTokens] * a.kv_heads + kh) * kPageTokens + j % kPageTokens;
+}
+
+// `lanes` threads copy one row of each pool.
+__device__ __forceinline__ void move_row(const EvictArgs& a, const int* table, int kh, int to, int from, int lane, int lanes) {
+  const size_t src = pool_row(a, table, kh, from) * a.row_bytes, dst = pool_row(a, table, kh, to) * a.row_bytes;
+  if (a.vector) {
+    for (int c = lane * 16; c < a.row_bytes; c += lanes * 16) {
+      const uint4 k = *reinterpret_cast<const uint4*>(a.k_pool + src + c), v = *reinterpret_cast<const uint4*>(a.v_pool + src + c);
+      *reinterpret_cast<uint4*>(a.k_pool + dst + c) = k;
+      *reinterpret_cast<uint4*>(a.v_pool + dst + c) = v;
+    }
+  } else {
+    for (int c = lane * 4; c < a.row_bytes; c += lanes * 4) {
+      const uint32_t k = *reinterpret_cast<const uint32_t*>(a.k_pool + src + c), v = *reinterpret_cast<const uint32_t*>(a.v_pool + src + c);
+      *reinterpret_cast<uint32_t*>(a.k_pool + dst + c) = k;
+      *reinterpret_cast<uint32_t*>(a.v_pool + dst + c) = v;
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kEvictThreads) cache_evict_kernel(EvictArgs a) {
+  pdl_enter();
+  extern __shared__ uint32_t keys[];
+  __shared__ int hist[256];
+  __shared__ unsigned long long warp_sums[32];
+  __shared__ int few_to[kFewMoves], few_from[kFewMoves];
+  __shared__ uint32_t s_digit;
+  __shared__ int s_need;
+  const int tid = threadIdx.x, kh = blockIdx.x, seq = blockIdx.y;
+  const size_t row0 = ((size_t)(a.slots ? a.slots[seq] : seq) * a.kv_heads + kh) * a.capacity;
+  const float* weights = a.weights + row0;
+  const int* positions = a.positions + row0;
+  float* weights_out = a.weights_out + row0;
+  int* positions_out = a.positions_out + row0;
+  const int* table = a.block_table + (size_t)seq * a.table_stride;
+  int n = min(a.lengths[seq], a.max_length);
+  if ((long long)n > a.capacity) n = (int)a.capacity;
+  const int past = min(a.past[seq], n), seen = a.seen[seq];
+  const int left = min(n, a.budget);
+  auto position = [&](int j) { return j < past ? positions[j] : seen - (n - j); };
+  auto make_key = [&](int j) {
+    const int p = position(j);
+    return order_key(weights[j], p < a.first || p >= seen - a.recent);
+  };
+  int* lists = a.scratch ? a.scratch + ((size_t)seq * a.kv_heads + kh) * (2 * (size_t)a.most_moves + 1) : nullptr;
+  if (n <= a.budget) {       // all stay
+    for (int j = tid; j < n; j += kEvictThreads) {
+      if (positions_out != positions || j >= past) positions_out[j] = position(j);
+      if (weights_out != weights) weights_out[j] = weights[j];
+    }
+    if (lists && tid == 0) lists[0] = 0;
+    return;
+  }
+  if (a.keys_fit)
+    for (int j = tid; j < n; j += kEvictThreads) keys[j] = make_key(j);
+  __syncthreads();
+  auto key_of = [&](int j) { return a.keys_fit ? keys[j] : make_key(j); };
+
+  // the key of the last row that stays: digit by digit, the largest ones first
+  uint32_t prefix = 0, mask = 0;
+  int need = left;             // rows still to be chosen among those that agree with the prefix
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    if (tid < 256) hist[tid] = 0;
+    __syncthreads();
+    for (int j = tid; j < n; j += kEvictThreads) {
+      const uint32_t k = key_of(j);
+      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1);
+    }
+    __syncthreads();
+    if (tid < 32) {            // counts of the digits above each lane's eight
+      int own = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) own += hist[tid * 8 + i];
+      int above = own;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int y = __shfl_down_sync(0xffffffffu, above, d);
+        if (tid + d < 32) above += y;
+      }
+      above -= own;
+      if (above < need && above + own >= need) {
+        int i = 7;
+        for (; i > 0; --i) {
+          if (above + hist[tid * 8 + i] >= need) break;
+          above += hist[tid * 8 + i];
+        }
+        s_digit = (uint32_t)(tid * 8 + i);
+        s_need = need - above;
+      }
+    }
+    __syncthreads();
+    prefix |= s_digit << shift;
+    mask |= 0xffu << shift;
+    need = s_need;
+    __syncthreads();
+  }
+  const uint32_t last = prefix;
+
+  // runs of rows a thread: an odd number, so that the threads of a warp meet different banks
+  const int per = ((n + kEvictThreads - 1) / kEvictThreads) | 1, j0 = min(n, tid * per), j1 = min(n, j0 + per);
+  unsigned long long ties = 0, total;
+  for (int j = j0; j < j1; ++j) ties += key_of(j) == last;
+  const int tie0 = (int)block_scan(ties, warp_sums, total);
+  int tie = tie0;
+  unsigned long long counts = 0;           // low word: places that become free below the budget; high word: rows that move
+  for (int j = j0; j < j1; ++j) {
+    const uint32_t k = key_of(j);
+    const bool stays = k > last || (k == last && tie < need);
+    tie += k == last;
+    if (j < left) counts += !stays;
+    else if (stays) counts += 1ull << 32;
+  }
+  const unsigned long long before = block_scan(counts, warp_sums, total);
+  const int moves = (int)(total >> 32);
+  int hole = (int)(before & 0xffffffffu), mover = (int)(before >> 32);
+  const bool few = a.most_moves <= kFewMoves;
+  tie = tie0;
+  for (int j = j0; j < j1; ++j) {
+    const uint32_t k = key_of(j);
+    const bool stays = k > last || (k == last && tie < need);
+    tie += k == last;
+    if (j < left) {
+      if (stays) {
+        if (positions_out != positions || j >= past) positions_out[j] = position(j);
+        if (weights_out != weights) weights_out[j] = weights[j];
+      } else {
+        if (few) few_to[hole] = j;
+        else lists[1 + hole] = j;
+        ++hole;
+      }
+    } else if (stays) {
+      if (few) few_from[mover] = j;
+      else lists[1 + a.most_moves + mover] = j;
+      ++mover;
+    }
+  }
+  if (!few && tid == 0) lists[0] = moves;
+  __syncthreads();
+  for (int i = tid; i < moves; i += kEvictThreads) {      // (the block's own stores are visible to it after the barrier)
+    const int to = few ? few_to[i] : lists[1 + i], from = few ? few_from[i] : lists[1 + a.most_moves + i];
+    weights_out[to] = weights[from];
+    positions_out[to] = position(from);
+  }
+  if (few)
+    for (int i = tid >> 4; i < moves; i += kEvictThreads / 16) move_row(a, table, kh, few_to[i], few_from[i], tid & 15, 16);
+}
+
+// The moves of the lists: 16 threads a row of each pool.
+__global__ void __launch_bounds__(256) cache_move_kernel(EvictArgs a) {
+  pdl_enter();
+  const int kh = blockIdx.y, seq = blockIdx.z;
+  const int* lists = a.scratch + ((size_t)seq * a.kv_heads + kh) * (2 * (size_t)a.most_moves + 1);
+  const int* table = a.block_table + (size_t)seq * a.table_stride;
+  const int moves = lists[0];
+  for (int i = blockIdx.x * 16 + (threadIdx.x >> 4); i < moves; i += gridDim.x * 16)
+    move_row(a, table, kh, lists[1 + i], lists[1 + a.most_moves + i], threadIdx.x & 15, 16);
+}
+
+static int most_moves(int budget, int max_length) {
+  const int behind = max_length - budget;
+  return behind <= 0 ? 0 : behind < budget ? behind : budget;
+}
+
+constexpr int kMostKeysShared = 48 * 1024;      // 192 KB of keys
+
+}  // namespace slb
+
+using namespace slb;
+
+// 32-bit words of scratch that slb_cache_evict takes: the lists of moves, where a sequence may move more rows than a block does by itself.
+extern "C" long long slb_cache_evict_scratch(int n_seqs, int kv_heads, int budget, int max_length) {
+  const int moves = most_moves(budget, max_length);
+  if (n_seqs <= 0 || kv_heads <= 0 || moves <= kFewMoves) return 0;
+  return (long long)n_seqs * kv_heads * (2ll * moves + 1);
+}
+
+// See the head of the file. weights, positions and their targets [slots, kv_heads, capacity] (a target may be its source); pools
+// [pages, kv_heads, 64, row_bytes]; max_length: no sequence holds more rows (0: as many as its table takes).
+extern "C" int slb_cache_evict(const float* weights, float* weights_out, const int* positions, int* positions_out, long long capacity,
+                               void* k_pool, void* v_pool, const int* block_table, int table_stride, int n_seqs, int kv_heads, int row_bytes,
+                               const int* past, const int* lengths, const int* seen, const int* slots, int budget, int first, int recent,
+                               int max_length, int* scratch, long long scratch_words, void* stream) {
+  SLB_REQUIRE(n_seqs >= 0 && kv_heads > 0 && row_bytes > 0 && row_bytes % 4 == 0 && table_stride > 0 && capacity > 0 && n_seqs < 65536 && kv_heads < 65536,
+              "cache_evict: n_seqs=%d kv_heads=%d row_bytes=%d table_stride=%d", n_seqs, kv_heads, row_bytes, table_stride);
+  SLB_REQUIRE(budget > 0 && first >= 0 && recent >= 0 && (long long)first + recent <= budget,
+              "cache_evict: %d first and %d recent rows do not fit a budget of %d", first, recent, budget);
+  if (n_seqs == 0) return 0;
+  const long long table_rows = (long long)table_stride * kPageTokens;
+  if (max_length <= 0 || max_length > table_rows) max_length = (int)(table_rows < 0x7fffffffll ? table_rows : 0x7fffffffll);
+  if (max_length > capacity) max_length = (int)capacity;
+  const long long need = slb_cache_evict_scratch(n_seqs, kv_heads, budget, max_length);
+  SLB_REQUIRE(need == 0 || (scratch != nullptr && scratch_words >= need), "cache_evict: the step needs %lld words of scratch, %lld were given", need,
+              scratch ? scratch_words : 0ll);
+  EvictArgs a{};
+  a.weights = weights; a.weights_out = weights_out; a.positions = positions; a.positions_out = positions_out; a.capacity = capacity;
+  a.k_pool = (char*)k_pool; a.v_pool = (char*)v_pool; a.block_table = block_table; a.past = past; a.lengths = lengths; a.seen = seen;
+  a.slots = slots; a.scratch = need ? scratch : nullptr; a.table_stride = table_stride; a.n_seqs = n_seqs; a.kv_heads = kv_heads;
+  a.row_bytes = row_bytes; a.budget = budget; a.first = first; a.recent = recent; a.max_length = max_length;
+  a.most_moves = most_moves(budget, max_length);
+  a.keys_fit = max_length <= kMostKeysShared;
+  a.vector = row_bytes % 16 == 0 && (uintptr_t)k_pool % 16 == 0 && (uintptr_t)v_pool % 16 == 0;
+  const int smem = a.keys_fit ? max_length * 4 : 0;
+  static std::atomic<unsigned long long> allowed;
+  const cudaError_t e = allow_shared((const void*)cache_evict_kernel, kMostKeysShared * 4, allowed);
+  if (e != cudaSuccess) return fail(2, "cache_evict: cannot reserve shared memory: %s", cudaGetErrorString(e));
+  launch(cache_evict_kernel, dim3(kv_heads, n_seqs), dim3(kEvictThreads), smem, (cudaStream_t)stream, a);
+  int rc = check_launch("cache_evict");
+  if (rc || need == 0) return rc;
+  const long long pairs = (long long)n_seqs * kv_heads;
+  long long blocks = 8ll * sm_count() / pairs;
+  const long long most = (a.most_moves + 15) / 16;
+  blocks = blocks < 1 ? 1 : blocks < most ? blocks : most;
+  launch(cache_move_kernel, dim3((unsigned)blocks, kv_heads, n_seqs), dim3(256), 0, (cudaStream_t)stream, a);
+  return check_launch("cache_evict (moves)");
+}

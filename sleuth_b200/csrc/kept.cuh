@@ -1,0 +1,39 @@
+// What the kernels of a cache of bounded size share: which rows of the cache a query sees, and the arguments of a step.
+//
+// Rows of a sequence are counted from 0 in the order of its block table (64 rows a page). A step appends counts[s] rows behind the
+// past[s] rows that are there; the query of row p sees row j if j <= p and (window == 0, or j > p - window, or j < first): the latest
+// `window` rows, its own included, and the first `first` ones.
+#pragma once
+
+#include "common.cuh"
+
+namespace slb {
+
+constexpr float kKeptLog2e = 1.4426950408889634f;
+
+struct KeptArgs {
+  const void* q;            // [tokens, H, hd]
+  const void* k_pool;       // [pages, K, 64, hd]
+  const void* v_pool;
+  void* out;                // [tokens, H * hd]
+  const int* seq_start;     // [n] first token row of each sequence
+  const int* past;          // [n] rows before the step
+  const int* counts;        // [n] new rows
+  const int* block_table;   // [n, table_stride]
+  int table_stride, n_seqs, heads, kv_heads, head_dim, window, first;
+  float scale;
+  float* lse;               // [tokens, H] log of the softmax denominator, or null
+  float* scratch;
+  int splits;
+  const int* slots;         // [n] the row of `weights` of each sequence, or null: its own number
+  const float* weights;     // [slots, K, capacity] what the rows have gathered before
+  float* weights_out;
+  long long capacity;
+};
+
+// First row of the window of the query at row p.
+__host__ __device__ __forceinline__ int window_lo(int p, int window) { return window > 0 && p - window + 1 > 0 ? p - window + 1 : 0; }
+
+__device__ __forceinline__ bool sees(int key, int pos, int lo, int first) { return key <= pos && (key >= lo || key < first); }
+
+}  // namespace slb

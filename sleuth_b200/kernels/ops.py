@@ -1681,3 +1681,112 @@ def sigmoid_gate(y, gate, stream=None) -> None:
     gs = _rows_f32(gate, C, "sigmoid_gate")
     _need(y.dtype in DT and gate.shape[0] == T, "sigmoid_gate: shapes")
     lib().call("slb_sigmoid_gate", _p(y), _p(gate), gs, T, C, DT[y.dtype], _st(stream))
+
+
+# ---- a cache of bounded size: the first rows, the latest ones and those that queries look at most ----
+
+
+def _gathered_ok(t, kv_heads: int, dtype, what: str) -> None:
+    _need(t is not None and t.dtype == dtype and t.dim() == 3 and t.shape[1] == kv_heads and t.shape[2] > 0,
+          f"{what}: [slots, kv_heads, rows] of {dtype}")
+
+
+def _rows_ok(n: int, what: str, **tables) -> None:
+    for name, t in tables.items():
+        _need(t is None or (t.dtype == torch.int32 and t.numel() >= n), f"{what}: {name} is int32, one per sequence")
+
+
+def attention_kept_scratch_floats(tokens: int, n_seqs: int, max_count: int, heads: int, kv_heads: int, head_dim: int, max_keys: int,
+                                  dtype: torch.dtype, weights: bool = False) -> int:
+    """Floats of scratch that ``attention_kept`` takes for a step of ``tokens`` new tokens, at most ``max_count`` a sequence, with at
+    most ``max_keys`` rows a sequence after the step; ``weights``: the step gathers weights."""
+    _need(dtype in DT, "attention_kept: dtypes")
+    fn = lib().dll.slb_attention_kept_scratch
+    fn.argtypes = [ctypes.c_longlong] + [ctypes.c_int] * 8
+    fn.restype = ctypes.c_longlong
+    return fn(int(tokens), int(n_seqs), int(max_count), heads, kv_heads, head_dim, int(max_keys), DT[dtype], 1 if weights else 0)
+
+
+def attention_kept(q, k_pool, v_pool, out, seq_start, past, counts, block_table, max_count: int, heads: int, kv_heads: int,
+                   head_dim: int, window: int, first: int, scale: float, stream=None, scratch=None, max_keys: int = 0, lse=None,
+                   weights=None, weights_out=None, slots=None) -> None:
+    """Attention of a step's new tokens (any number a sequence) over a cache of bounded size.
+
+    The step has written its keys and values; the query of cache row p sees row j <= p if ``window`` is 0, or j > p - window, or
+    j < ``first``: the latest ``window`` rows, its own included, and the first ``first`` ones. Rows are counted in the order of the
+    block table, not in positions of tokens, so table entries of pages that no query sees may hold anything. float32 or bfloat16,
+    even ``head_dim`` up to 256; softmax and sums in float32.
+
+    ``lse`` [tokens, heads] float32 receives the logarithm of each softmax denominator. ``weights`` [slots, kv_heads, rows] float32
+    holds what every cache row has gathered; ``weights_out`` (default: ``weights`` itself) receives the same plus this step's softmax
+    weights, summed over the step's queries and the query heads of each kv head; rows of the step itself start from 0, whatever lay
+    there. ``slots`` [n] int32: the row of ``weights`` of each sequence (default: 0, 1, ...). ``max_keys``: a promise that no sequence
+    has more rows after the step (0: as many as its table holds). ``scratch``: ``attention_kept_scratch_floats`` floats. A row whose
+    scores are all -inf gives zeros and gathers nothing. Values of hidden rows never reach a result, whatever they are, except that in
+    bfloat16 an infinity or NaN among the values of a row that some query of the same tile of up to 128 (token, head) rows sees may
+    reach the tile's other rows."""
+    _cuda(q, k_pool, v_pool, out, seq_start, past, counts, block_table, scratch, lse, weights, weights_out, slots)
+    _need(block_table.dtype == torch.int32 and block_table.dim() == 2, "attention_kept: block table")
+    T, n = q.shape[0], block_table.shape[0]
+    _need(q.shape == (T, heads, head_dim) and out.shape == (T, heads * head_dim), "attention_kept: shapes disagree")
+    _need(q.dtype == out.dtype == k_pool.dtype == v_pool.dtype and q.dtype in DT, "attention_kept: dtypes")
+    _need(tuple(k_pool.shape[1:]) == (kv_heads, 64, head_dim) and k_pool.shape == v_pool.shape, "attention_kept: pool shape")
+    _rows_ok(n, "attention_kept", seq_start=seq_start, past=past, counts=counts, slots=slots)
+    _need(window >= 0 and first >= 0, "attention_kept: window and first are not negative")
+    _need(lse is None or (lse.dtype == torch.float32 and lse.shape == (T, heads)), "attention_kept: lse is float32 [tokens, heads]")
+    _need(scratch is None or scratch.dtype == torch.float32, "attention_kept: scratch is float32")
+    _need(weights is not None or weights_out is None, "attention_kept: weights_out goes with weights")
+    if weights is not None:
+        weights_out = weights if weights_out is None else weights_out
+        _gathered_ok(weights, kv_heads, torch.float32, "attention_kept: weights")
+        _need(weights_out.dtype == torch.float32 and weights_out.shape == weights.shape, "attention_kept: weights_out as weights")
+        _need(slots is not None or weights.shape[0] >= n, "attention_kept: weights hold a row of every sequence")
+        _need(weights.shape[2] >= (max_keys if 0 < max_keys <= 64 * block_table.shape[1] else 64 * block_table.shape[1]),
+              "attention_kept: weights are shorter than the cache")
+    lib().call("slb_attention_kept", _p(q), _p(k_pool), _p(v_pool), _p(out), _p(seq_start), _p(past), _p(counts), _p(block_table),
+               block_table.shape[1], n, T, int(max_count), int(max_keys), heads, kv_heads, head_dim, int(window), int(first), float(scale),
+               _p(lse), _p(slots), _p(weights), _p(weights_out), 0 if weights is None else weights.shape[2], _p(scratch),
+               0 if scratch is None else scratch.numel(), DT[q.dtype], stream if stream is not None else current_stream())
+
+
+def cache_evict_scratch_words(n_seqs: int, kv_heads: int, budget: int, max_length: int) -> int:
+    """int32 words of scratch that ``cache_evict`` takes for sequences of at most ``max_length`` rows."""
+    fn = lib().dll.slb_cache_evict_scratch
+    fn.argtypes = [ctypes.c_int] * 4
+    fn.restype = ctypes.c_longlong
+    return fn(int(n_seqs), kv_heads, int(budget), int(max_length))
+
+
+def cache_evict(weights, positions, k_pool, v_pool, block_table, past, lengths, seen, budget: int, first: int, recent: int,
+                weights_out=None, positions_out=None, slots=None, scratch=None, max_length: int = 0, stream=None) -> None:
+    """After a step: of the ``lengths`` [n] rows that a sequence holds, ``budget`` stay for each kv head.
+
+    ``weights`` / ``positions`` [slots, kv_heads, rows] float32 / int32: what each row has gathered (``attention_kept``) and the
+    position of its token. The rows of the step itself, from ``past`` [n] on, need no position yet: they end at ``seen`` [n] - 1, the
+    last token of the sequence so far. Of more than ``budget`` rows those stay whose position is below ``first`` or among the last
+    ``recent``, and of the others those with the largest weight (NaN counts as the least, equal weights keep the lower rows). Rows that
+    stay but lie at ``budget`` or behind move, keys, values, weight and position, into the places of those that go; a sequence then holds
+    min(length, ``budget``) rows, and the pages behind them are free. ``weights_out`` / ``positions_out``: where the rows' weights and
+    positions go (default: in place); places behind the last row are left alone. ``max_length``: a promise that no sequence
+    holds more rows (0: as many as its table takes); ``scratch``: ``cache_evict_scratch_words`` int32 words."""
+    _cuda(weights, positions, k_pool, v_pool, block_table, past, lengths, seen, weights_out, positions_out, slots, scratch)
+    _need(block_table.dtype == torch.int32 and block_table.dim() == 2, "cache_evict: block table")
+    n, kv_heads = block_table.shape[0], k_pool.shape[1]
+    _need(k_pool.dim() == 4 and k_pool.shape == v_pool.shape and k_pool.dtype == v_pool.dtype and k_pool.dtype in DT and k_pool.shape[2] == 64,
+          "cache_evict: pools [pages, kv_heads, 64, head_dim]")
+    row_bytes = k_pool.shape[3] * k_pool.element_size()
+    _need(row_bytes % 4 == 0, "cache_evict: a row's bytes are a multiple of four")
+    _gathered_ok(weights, kv_heads, torch.float32, "cache_evict: weights")
+    _gathered_ok(positions, kv_heads, torch.int32, "cache_evict: positions")
+    weights_out = weights if weights_out is None else weights_out
+    positions_out = positions if positions_out is None else positions_out
+    _need(positions.shape == weights.shape == weights_out.shape == positions_out.shape and weights_out.dtype == torch.float32
+          and positions_out.dtype == torch.int32, "cache_evict: weights, positions and their targets have one shape")
+    _need(slots is not None or weights.shape[0] >= n, "cache_evict: weights hold a row of every sequence")
+    _rows_ok(n, "cache_evict", past=past, lengths=lengths, seen=seen, slots=slots)
+    _need(budget > 0 and first >= 0 and recent >= 0 and first + recent <= budget, "cache_evict: first and recent rows fit the budget")
+    _need(scratch is None or scratch.dtype == torch.int32, "cache_evict: scratch is int32")
+    lib().call("slb_cache_evict", _p(weights), _p(weights_out), _p(positions), _p(positions_out), weights.shape[2], _p(k_pool), _p(v_pool),
+               _p(block_table), block_table.shape[1], n, kv_heads, row_bytes, _p(past), _p(lengths), _p(seen), _p(slots), int(budget),
+               int(first), int(recent), int(max_length), _p(scratch), 0 if scratch is None else scratch.numel(),
+               stream if stream is not None else current_stream())
