@@ -36,4 +36,9 @@ __host__ __device__ __forceinline__ int window_lo(int p, int window) { return wi
 
 __device__ __forceinline__ bool sees(int key, int pos, int lo, int first) { return key <= pos && (key >= lo || key < first); }
 
+// Steps of few tokens (kept_few.cu): which they take, the floats of scratch (the first ones 16-byte aligned), the launch.
+bool kept_few_takes(long long tokens, int max_count, int heads, int kv_heads, int head_dim, int max_keys, int dtype, bool weights);
+long long kept_few_floats(long long tokens, int n_seqs, int max_count, int heads, int kv_heads, int head_dim, int max_keys, bool weights);
+int kept_few(const KeptArgs& a, long long tokens, int max_count, int max_keys, long long pool_pages, int* status, cudaStream_t s);
+
 }  // namespace slb

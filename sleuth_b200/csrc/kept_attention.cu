@@ -343,22 +343,31 @@ static int general_splits(int n_seqs, int max_count, int heads, int kv_heads, in
 
 using namespace slb;
 
-// Floats of scratch that slb_attention_kept takes for a step of these sizes: the shares' results, and with weights the denominators.
+enum KeptForm : int { kKeptGeneral = 0, kKeptFew = 1 };
+static int kept_form(long long tokens, int max_count, int heads, int kv_heads, int head_dim, int max_keys, int dtype, bool weights) {
+  if (kept_few_takes(tokens, max_count, heads, kv_heads, head_dim, max_keys, dtype, weights)) return kKeptFew;
+  return kKeptGeneral;
+}
+
+// Floats of scratch that slb_attention_kept takes for a step of these sizes: shares of results, with weights denominators and scores.
 extern "C" long long slb_attention_kept_scratch(long long tokens, int n_seqs, int max_count, int heads, int kv_heads, int head_dim, int max_keys,
                                                 int dtype, int weights) {
   if (tokens <= 0 || n_seqs <= 0 || max_count <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || max_keys <= 0) return 0;
+  if (kept_form(tokens, max_count, heads, kv_heads, head_dim, max_keys, dtype, weights != 0) == kKeptFew)
+    return kept_few_floats(tokens, n_seqs, max_count, heads, kv_heads, head_dim, max_keys, weights != 0);
   const int splits = general_splits(n_seqs, max_count, heads, kv_heads, max_keys);
   return (weights ? tokens * heads : 0) + (splits > 1 ? (long long)splits * tokens * heads * (head_dim + 2) : 0);
 }
 
-// Attention of a step over a cache of bounded size (kept.cuh). lse [tokens, heads] float32 or null; weights and weights_out
-// [slots, kv_heads, capacity] float32 (the same memory or apart) or both null; slots [n_seqs] or null. max_keys: no sequence has more rows
-// after the step. Scratch as slb_attention_kept_scratch says.
+// Attention of a step over a cache of bounded size (kept.cuh). Pools of pool_pages pages; lse [tokens, heads] float32 or null; weights and
+// weights_out [slots, kv_heads, capacity] float32 (the same memory or apart) or both null; slots [n_seqs] or null. max_keys: no sequence has
+// more rows after the step (0: as many as its table takes). Scratch as slb_attention_kept_scratch says. `status`: a zeroed device word that
+// receives a code if a bounded wait inside a kernel gave up.
 extern "C" int slb_attention_kept(const void* q, const void* k_pool, const void* v_pool, void* out, const int* seq_start, const int* past,
                                   const int* counts, const int* block_table, int table_stride, int n_seqs, long long tokens, int max_count,
                                   int max_keys, int heads, int kv_heads, int head_dim, int window, int first, float scale, float* lse,
                                   const int* slots, const float* weights, float* weights_out, long long capacity, float* scratch,
-                                  long long scratch_floats, int dtype, void* stream) {
+                                  long long scratch_floats, long long pool_pages, int* status, int dtype, void* stream) {
   SLB_REQUIRE(n_seqs >= 0 && tokens >= 0 && max_count >= 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0,
               "attention_kept: n_seqs=%d heads=%d kv_heads=%d", n_seqs, heads, kv_heads);
   SLB_REQUIRE(head_dim > 0 && head_dim <= 256 && head_dim % 2 == 0, "attention_kept: head_dim %d is not supported (even, at most 256)", head_dim);
@@ -367,8 +376,12 @@ extern "C" int slb_attention_kept(const void* q, const void* k_pool, const void*
   SLB_REQUIRE((weights == nullptr) == (weights_out == nullptr) && (weights == nullptr || capacity > 0), "attention_kept: weights and their target go together");
   SLB_REQUIRE(n_seqs < 65536 && kv_heads < 65536 && tokens < (1ll << 31), "attention_kept: n_seqs=%d tokens=%lld", n_seqs, tokens);
   if (n_seqs == 0 || tokens == 0 || max_count == 0) return 0;
-  if (max_keys <= 0 || max_keys > table_stride * (long long)kPageTokens) max_keys = table_stride * kPageTokens;
-  const long long need = slb_attention_kept_scratch(tokens, n_seqs, max_count, heads, kv_heads, head_dim, max_keys, dtype, weights != nullptr && lse == nullptr);
+  if (max_keys <= 0 || max_keys > table_stride * (long long)kPageTokens) {
+    SLB_REQUIRE(table_stride < (1 << 25), "attention_kept: table_stride=%d", table_stride);
+    max_keys = table_stride * kPageTokens;
+  }
+  const bool gather = weights != nullptr;
+  const long long need = slb_attention_kept_scratch(tokens, n_seqs, max_count, heads, kv_heads, head_dim, max_keys, dtype, gather);
   SLB_REQUIRE(need == 0 || (scratch != nullptr && scratch_floats >= need), "attention_kept: the step needs %lld floats of scratch, %lld were given",
               need, scratch ? scratch_floats : 0ll);
   KeptArgs a{};
@@ -376,13 +389,15 @@ extern "C" int slb_attention_kept(const void* q, const void* k_pool, const void*
   a.block_table = block_table; a.table_stride = table_stride; a.n_seqs = n_seqs; a.heads = heads; a.kv_heads = kv_heads;
   a.head_dim = head_dim; a.window = window; a.first = window > 0 ? first : 0; a.scale = scale; a.slots = slots; a.weights = weights;
   a.weights_out = weights_out; a.capacity = capacity; a.lse = lse; a.scratch = scratch;
-  if (weights != nullptr && lse == nullptr) {
+  const cudaStream_t s = (cudaStream_t)stream;
+  if (kept_form(tokens, max_count, heads, kv_heads, head_dim, max_keys, dtype, gather) == kKeptFew)
+    return kept_few(a, tokens, max_count, max_keys, pool_pages, status, s);
+  if (gather && lse == nullptr) {
     a.lse = scratch;
     a.scratch = scratch + tokens * heads;
   }
   a.splits = general_splits(n_seqs, max_count, heads, kv_heads, max_keys);
-  const cudaStream_t s = (cudaStream_t)stream;
   int rc = dtype == kF32 ? general<float>(a, max_count, tokens, s) : general<__nv_bfloat16>(a, max_count, tokens, s);
-  if (rc || weights == nullptr) return rc;
+  if (rc || !gather) return rc;
   return dtype == kF32 ? general_weights<float>(a, max_keys, s) : general_weights<__nv_bfloat16>(a, max_keys, s);
 }

@@ -1,0 +1,622 @@
+// Attention over a cache of bounded size (kept.cuh) for steps of few tokens, bfloat16, heads of 64 and 128: single tokens, short turns.
+//
+// What such a step costs is the read of the keys and values that its queries see, so the work is the pages: every sequence has so many
+// (page, kv head, tile of rows) units, and each block takes an equal run of the list of all units, whatever the sequences' lengths. A
+// (sequence, kv head, tile) that lies in one run is finished by its block; the others' shares wait in scratch for a second kernel.
+//   * warp 8, one lane: asks TMA for the pages of the block's run, keys and values, into a ring (128 KB: 32 KB a stage at heads of 128, and
+//     more than the 43 KB an SM that hide a memory latency of a microsecond at full bandwidth);
+//   * warps 0 to 7: mma.sync on the pages as they land. A tile is R times 16 rows, row r being token r / G, query head r % G of the group;
+//     R = 1: two groups of four warps take pages in turn, a warp 16 keys; R = 2: four warps share a page for each 16 rows, 16 keys each;
+//     R = 4: two, 32 keys each. Each warp keeps a running maximum, sum and weighted values of its own keys; they are joined at the end of
+//     a (sequence, kv head, tile), in the order of the warps.
+// (tcgen05 has nothing to win here: its tiles are 128 rows high, and rows are 2 to 64.)
+// With weights wanted the scores go to scratch as they are formed (log2 units, 4 bytes for each row and key against 4 x head_dim for the
+// key and value: 1 to 4 per cent more bytes), because the denominators are known at the end only; the second kernel turns them into weights.
+// Keys that no row of the tile sees (stale rows of the last page, what lies between the first rows and the window) have their values
+// replaced by zeros in registers, so that infinities or NaN in them do not meet a zero weight.
+#include <math.h>
+
+#include "kept.cuh"
+#include "mma_sync.cuh"
+#include "tcgen05.cuh"
+
+namespace slb {
+
+constexpr int kFewThreads = 288;
+constexpr int kFewMostRows = 256;      // rows of a (sequence, kv head) that the second kernel takes
+
+struct FewArgs {
+  KeptArgs k;
+  float scale_log2;
+  int max_tiles;        // tiles of the longest share
+  int max_count;        // no sequence brings more tokens (the room below is made for that)
+  float* part;          // [blocks][2][16 R][HD] weighted values, then [blocks][2][16 R][2] maximum and sum
+  float* part_ml;
+  int2* info;           // [n, kv_heads, max_tiles] first block and number of blocks
+  float* lse2;          // [tokens, H] denominators in log2 units
+  float* scores;        // [tokens, H, score_stride] or null
+  long long score_stride;
+  int* status;
+};
+
+// The pages of a step of one sequence: the first ones and the window's, as one list.
+struct PageRun {
+  int nf, lo, count;      // pages 0 .. nf - 1, then lo ..
+  __device__ __forceinline__ PageRun(int past, int tokens, int window, int first) {
+    if (tokens <= 0) { nf = lo = count = 0; return; }
+    const int key_lo = window_lo(past, window);
+    nf = (min(first, key_lo) + 63) / 64;
+    lo = max(key_lo / 64, nf);
+    count = nf + (past + tokens - 1) / 64 - lo + 1;
+  }
+  __device__ __forceinline__ int page(int i) const { return i < nf ? i : lo + i - nf; }
+};
+
+__device__ __forceinline__ float few_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <int HD, int R>
+struct FewLayout {
+  static constexpr int PAGE = 64 * HD * 2;
+  static constexpr int STAGES = HD == 128 ? 4 : 8;
+  static constexpr int Q_OFF = 0;                               // [16 R][HD] bfloat16, swizzled
+  static constexpr int RING_OFF = Q_OFF + 4 * 16 * HD * 2;      // keys then values of a stage
+  static constexpr int MERGE_OFF = RING_OFF + STAGES * 2 * PAGE;      // [8 warps][16][HD] float
+  static constexpr int ML_OFF = MERGE_OFF + 8 * 16 * HD * 4;    // [8][16][2]
+  static constexpr int BAR_OFF = ML_OFF + 8 * 16 * 2 * 4;
+  static constexpr int TOTAL = BAR_OFF + 2 * STAGES * 8;
+  static_assert(TOTAL <= 226 * 1024, "the block must fit on an SM");
+};
+
+// 16-byte piece of channel `col` of row `row` in a tile of 64 rows as TMA leaves it: 64 channels a half, pieces exchanged by the row.
+template <int ROWS>
+__device__ __forceinline__ uint32_t tile_at(int row, int col) {
+  return (uint32_t)((col >> 6) * (ROWS * 128) + row * 128 + (((col >> 3) & 7) ^ (row & 7)) * 16);
+}
+
+template <int HD, int R>
+__global__ void __launch_bounds__(kFewThreads, 1)
+kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, FewArgs fa) {
+  using L = FewLayout<HD, R>;
+  constexpr int ROWS = 16 * R, KW = R == 4 ? 32 : 16, KB = KW / 16, GROUPS = 8 / R;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  __shared__ long long warp_units[9];
+  __shared__ long long s_first;
+  __shared__ int s_seq;
+  const KeptArgs& a = fa.k;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t base = smem_addr(smem);
+  if ((base & 1023u) != 0) {
+    if (tid == 0) atomicExch(fa.status, 81);
+    return;
+  }
+  const uint32_t bars = base + L::BAR_OFF;
+  if (tid == 0) {
+    for (int i = 0; i < L::STAGES; ++i) {
+      mbar_init(bars + 8 * i, 1);
+      mbar_init(bars + 8 * (L::STAGES + i), R == 1 ? 4 : 8);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  pdl_wait();
+
+  // units of the sequences, and where this block's run begins
+  const int G = a.heads / a.kv_heads;
+  auto tiles_of = [&](int count) { return (count * G + ROWS - 1) / ROWS; };
+  auto units_of = [&](int s) -> long long {
+    const int c = min(a.counts[s], fa.max_count);
+    return (long long)PageRun(a.past[s], c, a.window, a.first).count * a.kv_heads * tiles_of(c);
+  };
+  const int per = (a.n_seqs + kFewThreads - 1) / kFewThreads, q0 = min(a.n_seqs, tid * per), q1 = min(a.n_seqs, q0 + per);
+  long long own = 0;
+  for (int s = q0; s < q1; ++s) own += units_of(s);
+  long long incl = own;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += y;
+  }
+  if (lane == 31) warp_units[warp] = incl;
+  __syncthreads();
+  long long before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < 9; ++w) {
+    if (w < warp) before += warp_units[w];
+    total += warp_units[w];
+  }
+  const long long blocks = min((long long)gridDim.x, total);
+  if ((long long)blockIdx.x >= blocks) return;
+  const long long u_lo = blockIdx.x * total / blocks, u_hi = (blockIdx.x + 1) * total / blocks;
+  before += incl - own;
+  if (own > 0 && u_lo >= before && u_lo < before + own) {
+    for (int s = q0; s < q1; ++s) {
+      const long long u = units_of(s);
+      if (u_lo < before + u) {
+        s_seq = s;
+        s_first = before;
+        break;
+      }
+      before += u;
+    }
+  }
+  __syncthreads();
+  int seq = s_seq;
+  long long seq_first = s_first;      // units before this sequence
+  long long u = u_lo;
+
+  if (warp == 8) {
+    // ---- the ring's pages ----
+    int cnt = 0;
+    bool ok = true;
+    while (u < u_hi && ok) {
+      const int count = min(a.counts[seq], fa.max_count), past = a.past[seq];
+      const PageRun run(past, count, a.window, a.first);
+      const long long units = (long long)run.count * a.kv_heads * tiles_of(count);
+      const int* table = a.block_table + (size_t)seq * a.table_stride;
+      const int n_tiles = tiles_of(count);
+      const long long stop = min(u_hi, seq_first + units);
+      while (u < stop && ok) {
+        const int off = (int)((u - seq_first) % run.count), pair = (int)((u - seq_first) / run.count), kh = pair / n_tiles;
+        const int n = (int)min((long long)(run.count - off), stop - u);
+        for (int i0 = 0; i0 < n && ok; i0 += 32) {
+          const int mine = i0 + lane < n ? table[run.page(off + i0 + lane)] : 0;
+          for (int i = 0; i < min(32, n - i0); ++i, ++cnt) {
+            const int page = __shfl_sync(0xffffffffu, mine, i);
+            const int st = cnt % L::STAGES;
+            if (cnt >= L::STAGES && !mbar_wait(bars + 8 * (L::STAGES + st), ((cnt / L::STAGES) - 1) & 1)) {
+              if (lane == 0) atomicExch(fa.status, 82);
+              ok = false;
+              break;
+            }
+            if (elect_one()) {
+              const int row = (page * a.kv_heads + kh) * 64;
+              const uint32_t dst = base + L::RING_OFF + st * 2 * L::PAGE;
+              mbar_expect_tx(bars + 8 * st, 2 * L::PAGE);
+#pragma unroll
+              for (int h = 0; h < HD / 64; ++h) tma_load_2d(dst + h * 8192, &map_k, h * 64, row, bars + 8 * st);
+#pragma unroll
+              for (int h = 0; h < HD / 64; ++h) tma_load_2d(dst + L::PAGE + h * 8192, &map_v, h * 64, row, bars + 8 * st);
+            }
+            __syncwarp();
+          }
+        }
+        u += n;
+      }
+      seq_first += units;
+      ++seq;
+    }
+    pdl_launch_dependents();
+    return;
+  }
+
+  // ---- the products ----
+  const int g = lane >> 2, t4 = lane & 3;
+  const int rt = R == 1 ? 0 : warp % R, group = warp / R;      // 16 rows of the tile; which keys
+  const int key_in = R == 1 ? (warp & 3) * 16 : group * KW;
+  auto sync = [&]() { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+  int cnt = 0;
+  bool ok = true;
+  while (u < u_hi) {
+    const int count = min(a.counts[seq], fa.max_count), past = a.past[seq];
+    const PageRun run(past, count, a.window, a.first);
+    const int n_tiles = tiles_of(count);
+    const long long units = (long long)run.count * a.kv_heads * n_tiles;
+    const int tok0 = a.seq_start[seq];
+    const long long stop = min(u_hi, seq_first + units);
+    while (u < stop) {
+      const int off = (int)((u - seq_first) % run.count), pair = (int)((u - seq_first) / run.count), kh = pair / n_tiles, tile = pair % n_tiles;
+      const int n = (int)min((long long)(run.count - off), stop - u);
+      const int row0 = tile * ROWS, rows = min(ROWS, count * G - row0);
+      // queries (the previous tile's results have been read: every warp has passed its last barrier)
+      for (int e = tid; e < ROWS * (HD / 8); e += 256) {
+        const int r = e / (HD / 8), col = (e % (HD / 8)) * 8, Rr = row0 + r;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (r < rows) v = *reinterpret_cast<const uint4*>((const __nv_bfloat16*)a.q + ((size_t)(tok0 + Rr / G) * a.heads + kh * G + Rr % G) * HD + col);
+        *reinterpret_cast<uint4*>(smem + L::Q_OFF + tile_at<ROWS>(r, col)) = v;
+      }
+      sync();
+      uint32_t qf[HD / 16][4];
+#pragma unroll
+      for (int kb = 0; kb < HD / 16; ++kb) ldmatrix_x4(qf[kb], base + L::Q_OFF + tile_at<ROWS>(rt * 16 + (lane & 15), kb * 16 + ((lane >> 4) << 3)));
+      int pos[2], lo[2];
+      float* score_row[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = rt * 16 + g + 8 * h, Rr = row0 + r;
+        pos[h] = r < rows ? past + Rr / G : -1;
+        lo[h] = window_lo(pos[h], a.window);
+        score_row[h] = fa.scores && r < rows ? fa.scores + ((size_t)(tok0 + Rr / G) * a.heads + kh * G + Rr % G) * fa.score_stride : nullptr;
+      }
+      // what the 16 rows of this warp see: all of them from see_lo (or below `first`) to see_hi, none beyond any_hi or below any_lo
+      const int r_first = row0 + rt * 16, r_last = min(row0 + rows, r_first + 16) - 1;
+      const bool idle = r_first > r_last;
+      const int any_lo = window_lo(past + r_first / G, a.window), any_hi = past + r_last / G;
+      const int all_lo = window_lo(any_hi, a.window), all_hi = past + r_first / G;
+
+      float o[HD / 8][4];
+#pragma unroll
+      for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+      float m_r[2] = {-INFINITY, -INFINITY}, l_r[2] = {0.0f, 0.0f};
+      for (int i = 0; i < n; ++i, ++cnt) {
+        if (R == 1 && (i & 1) != (warp >> 2)) {
+          continue;
+        }
+        const int st = cnt % L::STAGES;
+        if (ok && !mbar_wait(bars + 8 * st, (cnt / L::STAGES) & 1)) {
+          ok = false;
+          if (lane == 0) atomicExch(fa.status, 83);
+        }
+        const int key0 = run.page(off + i) * 64 + key_in;
+        const bool none = idle || key0 > any_hi || (key0 + KW - 1 < any_lo && key0 >= a.first);
+        if (!none) {
+          const uint32_t kS = base + L::RING_OFF + st * 2 * L::PAGE, vS = kS + L::PAGE;
+          float s[2 * KB][4];
+#pragma unroll
+          for (int j = 0; j < 2 * KB; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
+#pragma unroll
+          for (int kb = 0; kb < HD / 16; ++kb) {
+#pragma unroll
+            for (int b = 0; b < KB; ++b) {
+              uint32_t kf[4];
+              ldmatrix_x4(kf, kS + tile_at<64>(key_in + b * 16 + (lane & 7) + ((lane >> 4) << 3), kb * 16 + (((lane >> 3) & 1) << 3)));
+              mma_bf16(s[2 * b], qf[kb], kf[0], kf[1]);
+              mma_bf16(s[2 * b + 1], qf[kb], kf[2], kf[3]);
+            }
+          }
+          const bool whole = key0 + KW - 1 <= all_hi && (key0 >= all_lo || key0 + KW <= a.first);
+#pragma unroll
+          for (int j = 0; j < 2 * KB; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int key = key0 + j * 8 + 2 * t4 + (e & 1);
+              s[j][e] *= fa.scale_log2;
+              if (!whole && !sees(key, pos[e >> 1], lo[e >> 1], a.first)) s[j][e] = -INFINITY;
+            }
+          if (fa.scores != nullptr) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (score_row[h] != nullptr) {
+#pragma unroll
+                for (int j = 0; j < 2 * KB; ++j) {
+                  const int key = key0 + j * 8 + 2 * t4;
+                  if (key < fa.score_stride) *reinterpret_cast<float2*>(score_row[h] + key) = make_float2(s[j][2 * h], s[j][2 * h + 1]);
+                }
+              }
+          }
+          float alpha[2], m_use[2];
+          bool moved = false;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 2 * KB; ++j) mx = fmaxf(mx, fmaxf(s[j][2 * h], s[j][2 * h + 1]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const float m_new = fmaxf(m_r[h], mx);
+            m_use[h] = m_new == -INFINITY ? 0.0f : m_new;
+            alpha[h] = few_ex2(m_r[h] - m_use[h]);
+            moved = moved || m_new > m_r[h];
+            m_r[h] = m_new;
+          }
+          uint32_t pf[KB][4];
+          float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+          for (int j = 0; j < 2 * KB; ++j) {
+            const float p0 = few_ex2(s[j][0] - m_use[0]), p1 = few_ex2(s[j][1] - m_use[0]);
+            const float p2 = few_ex2(s[j][2] - m_use[1]), p3 = few_ex2(s[j][3] - m_use[1]);
+            sum[0] += p0 + p1;
+            sum[1] += p2 + p3;
+            pf[j >> 1][(j & 1) * 2 + 0] = pack_bf16(p0, p1);
+            pf[j >> 1][(j & 1) * 2 + 1] = pack_bf16(p2, p3);
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) l_r[h] = l_r[h] * alpha[h] + sum[h];
+          if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+            for (int c = 0; c < HD / 8; ++c) {
+              o[c][0] *= alpha[0]; o[c][1] *= alpha[0];
+              o[c][2] *= alpha[1]; o[c][3] *= alpha[1];
+            }
+          }
+          if (whole) {
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+              for (int dp = 0; dp < HD / 16; ++dp) {
+                uint32_t vf[4];
+                ldmatrix_x4_trans(vf, vS + tile_at<64>(key_in + b * 16 + (lane & 15), dp * 16 + ((lane >> 4) << 3)));
+                mma_bf16(o[2 * dp], pf[b], vf[0], vf[1]);
+                mma_bf16(o[2 * dp + 1], pf[b], vf[2], vf[3]);
+              }
+          } else {
+#pragma unroll
+            for (int b = 0; b < KB; ++b) {
+              // a lane holds the values of keys 2 t4, 2 t4 + 1 (and + 8) in the halves of a register
+              uint32_t live[2];
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int key = key0 + b * 16 + h * 8 + 2 * t4;
+                live[h] = (sees(key, any_hi, any_lo, a.first) ? 0x0000ffffu : 0u) | (sees(key + 1, any_hi, any_lo, a.first) ? 0xffff0000u : 0u);
+              }
+#pragma unroll
+              for (int dp = 0; dp < HD / 16; ++dp) {
+                uint32_t vf[4];
+                ldmatrix_x4_trans(vf, vS + tile_at<64>(key_in + b * 16 + (lane & 15), dp * 16 + ((lane >> 4) << 3)));
+                mma_bf16(o[2 * dp], pf[b], vf[0] & live[0], vf[1] & live[1]);
+                mma_bf16(o[2 * dp + 1], pf[b], vf[2] & live[0], vf[3] & live[1]);
+              }
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bars + 8 * (L::STAGES + st));
+      }
+
+      // join the warps that share these rows
+      float* mo = reinterpret_cast<float*>(smem + L::MERGE_OFF);      // [8][16][HD]
+      float* ml = reinterpret_cast<float*>(smem + L::ML_OFF);         // [8][16][2]
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        l_r[h] += __shfl_xor_sync(0xffffffffu, l_r[h], 1);
+        l_r[h] += __shfl_xor_sync(0xffffffffu, l_r[h], 2);
+        const int r = g + 8 * h;
+        if (rt * 16 + r >= rows) continue;
+        if (t4 == 0) *reinterpret_cast<float2*>(ml + (warp * 16 + r) * 2) = make_float2(m_r[h], l_r[h]);
+        // (rows of a warp start 8 x 4-byte banks apart by the row, so that the eight rows of a store meet different banks)
+#pragma unroll
+        for (int c = 0; c < HD / 8; ++c)
+          *reinterpret_cast<float2*>(mo + (warp * 16 + r) * HD + ((c * 8 + 2 * t4) ^ ((r & 3) << 3))) = make_float2(o[c][2 * h], o[c][2 * h + 1]);
+      }
+      sync();
+      const bool begins = off == 0, complete = begins && n == run.count;
+      const long long pair_lo = seq_first + (long long)pair * run.count;
+      const int first_block = blockIdx.x;
+      if (begins && tid == 0) {
+        const long long last = pair_lo + run.count - 1;
+        const int last_block = (int)(((last + 1) * blocks - 1) / total);
+        fa.info[((size_t)seq * a.kv_heads + kh) * fa.max_tiles + tile] = make_int2(first_block, last_block - first_block + 1);
+      }
+      const size_t slot = ((size_t)blockIdx.x * 2 + (begins ? 1 : 0)) * ROWS;
+      for (int e = tid; e < rows * (HD / 4); e += 256) {
+        const int r = e / (HD / 4), d = (e % (HD / 4)) * 4, in = r & 15;
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < GROUPS; ++w) M = fmaxf(M, ml[((w * R + (r >> 4)) * 16 + in) * 2]);
+        const float top = M == -INFINITY ? 0.0f : M;
+        float sum = 0.0f;
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < GROUPS; ++w) {
+          const int at = (w * R + (r >> 4)) * 16 + in;
+          const float f = few_ex2(ml[at * 2] - top);
+          const float4 v = *reinterpret_cast<const float4*>(mo + at * HD + (d ^ ((in & 3) << 3)));
+          sum += ml[at * 2 + 1] * f;
+          acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+        }
+        const int Rr = row0 + r;
+        const size_t row = (size_t)(tok0 + Rr / G) * a.heads + kh * G + Rr % G;
+        if (complete) {
+          const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+          uint2 pk;
+          pk.x = pack_bf16(acc.x * inv, acc.y * inv);
+          pk.y = pack_bf16(acc.z * inv, acc.w * inv);
+          *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + row * HD + d) = pk;
+          if (d == 0) {
+            const float lse2 = sum == 0.0f ? -INFINITY : top + log2f(sum);
+            if (fa.lse2) fa.lse2[row] = lse2;
+            if (a.lse) a.lse[row] = lse2 * 0.6931471805599453f;
+          }
+        } else {
+          *reinterpret_cast<float4*>(fa.part + (slot + r) * HD + d) = acc;
+          if (d == 0) *reinterpret_cast<float2*>(fa.part_ml + (slot + r) * 2) = make_float2(M, sum);
+        }
+      }
+      sync();
+      u += n;
+    }
+    seq_first += units;
+    ++seq;
+  }
+}
+
+// Joins the shares of what no block finished alone, and turns scores into weights: a block takes some of the outputs and 1,024 keys of one
+// (sequence, kv head).
+template <int HD, int R>
+__global__ void __launch_bounds__(256) kept_few_finish_kernel(FewArgs fa) {
+  pdl_wait();
+  const KeptArgs& a = fa.k;
+  constexpr int ROWS = 16 * R;
+  __shared__ float lse_s[kFewMostRows];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int kh = blockIdx.y, seq = blockIdx.z, G = a.heads / a.kv_heads;
+  const int count = min(a.counts[seq], fa.max_count), past = a.past[seq], tok0 = a.seq_start[seq], rows_total = count * G;
+  if (count <= 0) return;
+  const int2* info = fa.info + ((size_t)seq * a.kv_heads + kh) * fa.max_tiles;
+  auto row_of = [&](int Rr) { return (size_t)(tok0 + Rr / G) * a.heads + kh * G + Rr % G; };
+  auto slot_of = [&](int2 in, int i) { return ((size_t)(in.x + i) * 2 + (i == 0 ? 1 : 0)) * ROWS; };
+  // denominators: a warp a row, its lanes along the shares
+  if (fa.scores != nullptr || a.lse != nullptr) {
+    for (int Rr = warp; Rr < rows_total; Rr += 8) {
+      const int2 in = info[Rr / ROWS];
+      float v;
+      if (in.y == 1) {
+        v = fa.lse2 ? fa.lse2[row_of(Rr)] : 0.0f;
+      } else {
+        float M = -INFINITY, L = 0.0f;
+        for (int i = lane; i < in.y; i += 32) {
+          const float2 p = *reinterpret_cast<const float2*>(fa.part_ml + (slot_of(in, i) + Rr % ROWS) * 2);
+          const float top = fmaxf(M, p.x), use = top == -INFINITY ? 0.0f : top;
+          L = L * few_ex2(M - use) + p.y * few_ex2(p.x - use);
+          M = top;
+        }
+        const float top = warp_max(M), use = top == -INFINITY ? 0.0f : top;
+        L = warp_sum(L * few_ex2(M - use));
+        v = L == 0.0f ? -INFINITY : use + log2f(L);
+        if (lane == 0 && blockIdx.x == 0 && a.lse) a.lse[row_of(Rr)] = v * 0.6931471805599453f;
+      }
+      if (lane == 0) lse_s[Rr] = v;
+    }
+  }
+  // outputs
+  for (int e = blockIdx.x * 256 + tid; e < rows_total * (HD / 4); e += gridDim.x * 256) {
+    const int Rr = e / (HD / 4), d = (e % (HD / 4)) * 4;
+    const int2 in = info[Rr / ROWS];
+    if (in.y == 1) continue;
+    float M = -INFINITY, L = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int i0 = 0; i0 < in.y; i0 += 8) {
+      float2 p[8];
+      float4 v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool live = i0 + i < in.y;
+        const size_t at = slot_of(in, live ? i0 + i : 0) + Rr % ROWS;
+        p[i] = *reinterpret_cast<const float2*>(fa.part_ml + at * 2);
+        v[i] = *reinterpret_cast<const float4*>(fa.part + at * HD + d);
+        if (!live) p[i] = make_float2(-INFINITY, 0.0f);
+      }
+      float top = M;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, p[i].x);
+      const float use = top == -INFINITY ? 0.0f : top, keep = few_ex2(M - use);
+      L *= keep;
+      acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float f = few_ex2(p[i].x - use);
+        if (i0 + i < in.y) {      // (a share whose scores were all NaN has maximum -inf and a sum of NaN)
+          L += p[i].y * f;
+          acc.x += v[i].x * f; acc.y += v[i].y * f; acc.z += v[i].z * f; acc.w += v[i].w * f;
+        }
+      }
+      M = top;
+    }
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    uint2 pk;
+    pk.x = pack_bf16(acc.x * inv, acc.y * inv);
+    pk.y = pack_bf16(acc.z * inv, acc.w * inv);
+    *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + row_of(Rr) * HD + d) = pk;
+  }
+  if (fa.scores == nullptr) return;
+  __syncthreads();
+  const int end = past + count;
+  const size_t at0 = ((size_t)(a.slots ? a.slots[seq] : seq) * a.kv_heads + kh) * a.capacity;
+  for (int c = 0; c < 4; ++c) {
+    const int key = blockIdx.x * 1024 + c * 256 + tid;
+    if (key >= end || key >= a.capacity) break;
+    float sum = 0.0f;
+    for (int i = 0; i < count; ++i) {
+      const int p = past + i;
+      if (!sees(key, p, window_lo(p, a.window), a.first)) continue;
+      const float* src = fa.scores + ((size_t)(tok0 + i) * a.heads + kh * G) * fa.score_stride + key;
+#pragma unroll 4
+      for (int h = 0; h < G; ++h) {
+        const float d = lse_s[i * G + h];
+        const float w = few_ex2(src[(size_t)h * fa.score_stride] - d);
+        if (d != -INFINITY) sum += w;
+      }
+    }
+    a.weights_out[at0 + key] = (key < past ? a.weights[at0 + key] : 0.0f) + sum;
+  }
+}
+
+static int few_row_tiles(int max_count, int G) { return max_count * G <= 16 ? 1 : max_count * G <= 32 ? 2 : 4; }
+
+// Where the pieces of scratch lie, in floats.
+struct FewScratch {
+  long long part, part_ml, info, lse2, scores, total, score_stride;
+  int max_tiles, blocks;
+};
+static FewScratch few_scratch(long long tokens, int n_seqs, int max_count, int heads, int kv_heads, int head_dim, int max_keys, bool weights) {
+  FewScratch f{};
+  const int G = heads / kv_heads, R = few_row_tiles(max_count, G);
+  f.max_tiles = (max_count * G + 16 * R - 1) / (16 * R);
+  const long long units = (long long)n_seqs * kv_heads * f.max_tiles * ((max_keys + 63) / 64);
+  f.blocks = (int)(units < sm_count() ? units : sm_count());      // a block an SM; none without a page
+  const long long slots = 2ll * f.blocks * 16 * R;
+  long long at = 0;
+  auto take = [&](long long n) { const long long o = at; at += (n + 3) & ~3ll; return o; };
+  f.part = take(slots * head_dim);
+  f.part_ml = take(slots * 2);
+  f.info = take(2ll * n_seqs * kv_heads * f.max_tiles);
+  f.lse2 = weights ? take(tokens * heads) : 0;
+  f.score_stride = (max_keys + 1) & ~1;
+  f.scores = weights ? take(tokens * heads * f.score_stride) : 0;
+  f.total = at;
+  return f;
+}
+
+template <int HD, int R>
+static int launch_few(const CUtensorMap& mk, const CUtensorMap& mv, const FewArgs& fa, int blocks, int max_keys, int max_count, cudaStream_t s) {
+  using L = FewLayout<HD, R>;
+  static std::atomic<unsigned long long> allowed;
+  const cudaError_t e = allow_shared((const void*)kept_few_kernel<HD, R>, L::TOTAL, allowed);
+  if (e != cudaSuccess) return fail(2, "attention_kept: cannot reserve %d bytes of shared memory: %s", L::TOTAL, cudaGetErrorString(e));
+  launch(kept_few_kernel<HD, R>, dim3(blocks), dim3(kFewThreads), (size_t)L::TOTAL, s, mk, mv, fa);
+  int rc = check_launch("attention_kept (few tokens)");
+  if (rc) return rc;
+  const int G = fa.k.heads / fa.k.kv_heads;
+  int gx = fa.scores ? (max_keys + 1023) / 1024 : 1;
+  const int outs = (max_count * G * (HD / 4) + 255) / 256;
+  gx = gx > outs ? gx : outs < 8 ? outs : 8 > gx ? 8 : gx;
+  launch_prefetching(kept_few_finish_kernel<HD, R>, dim3(gx, fa.k.kv_heads, fa.k.n_seqs), dim3(256), 0, s, fa);
+  return check_launch("attention_kept (few tokens, joined)");
+}
+
+static int encode_pool(CUtensorMap* map, const void* base, long long rows, int head_dim, const char* what) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(2, "attention_kept: the driver does not offer cuTensorMapEncodeTiled");
+  cuuint64_t dims[2] = {(cuuint64_t)head_dim, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)head_dim * 2};
+  cuuint32_t box[2] = {64, 64}, estr[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : fail(2, "attention_kept: cuTensorMapEncodeTiled failed for %s with code %d", what, (int)r);
+}
+
+constexpr long long kMostScores = 1ll << 28;      // floats of scratch for scores: a gigabyte
+
+bool kept_few_takes(long long tokens, int max_count, int heads, int kv_heads, int head_dim, int max_keys, int dtype, bool weights) {
+  return dtype == kBF16 && (head_dim == 64 || head_dim == 128) && (long long)max_count * (heads / kv_heads) <= 64 &&
+         (!weights || tokens * heads * max_keys <= kMostScores);
+}
+
+long long kept_few_floats(long long tokens, int n_seqs, int max_count, int heads, int kv_heads, int head_dim, int max_keys, bool weights) {
+  return few_scratch(tokens, n_seqs, max_count, heads, kv_heads, head_dim, max_keys, weights).total;
+}
+
+int kept_few(const KeptArgs& a, long long tokens, int max_count, int max_keys, long long pool_pages, int* status, cudaStream_t s) {
+  SLB_REQUIRE(pool_pages * a.kv_heads * 64 < (1ll << 31), "attention_kept: the pool has too many rows for one tensor map");
+  SLB_REQUIRE((uintptr_t)a.q % 16 == 0 && (uintptr_t)a.k_pool % 16 == 0 && (uintptr_t)a.v_pool % 16 == 0 && (uintptr_t)a.out % 16 == 0 &&
+              (uintptr_t)a.scratch % 16 == 0, "attention_kept: q, out, scratch and the pools must be 16-byte aligned");
+  SLB_REQUIRE(status != nullptr, "attention_kept: no status word");
+  CUtensorMap mk, mv;
+  int rc = encode_pool(&mk, a.k_pool, pool_pages * a.kv_heads * 64, a.head_dim, "the key pool");
+  if (rc == 0) rc = encode_pool(&mv, a.v_pool, pool_pages * a.kv_heads * 64, a.head_dim, "the value pool");
+  if (rc) return rc;
+  const bool weights = a.weights != nullptr;
+  const FewScratch f = few_scratch(tokens, a.n_seqs, max_count, a.heads, a.kv_heads, a.head_dim, max_keys, weights);
+  FewArgs fa{};
+  fa.k = a;
+  fa.scale_log2 = a.scale * kKeptLog2e;
+  fa.max_tiles = f.max_tiles;
+  fa.max_count = max_count;
+  fa.part = a.scratch + f.part;
+  fa.part_ml = a.scratch + f.part_ml;
+  fa.info = reinterpret_cast<int2*>(a.scratch + f.info);
+  fa.lse2 = weights ? a.scratch + f.lse2 : nullptr;
+  fa.scores = weights ? a.scratch + f.scores : nullptr;
+  fa.score_stride = f.score_stride;
+  fa.status = status;
+  const int R = few_row_tiles(max_count, a.heads / a.kv_heads);
+  if (a.head_dim == 128)
+    return R == 1 ? launch_few<128, 1>(mk, mv, fa, f.blocks, max_keys, max_count, s) : R == 2 ? launch_few<128, 2>(mk, mv, fa, f.blocks, max_keys, max_count, s)
+                                                                           : launch_few<128, 4>(mk, mv, fa, f.blocks, max_keys, max_count, s);
+  return R == 1 ? launch_few<64, 1>(mk, mv, fa, f.blocks, max_keys, max_count, s) : R == 2 ? launch_few<64, 2>(mk, mv, fa, f.blocks, max_keys, max_count, s)
+                                                                        : launch_few<64, 4>(mk, mv, fa, f.blocks, max_keys, max_count, s);
+}
+
+}  // namespace slb

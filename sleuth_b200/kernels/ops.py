@@ -799,7 +799,8 @@ def gemm_tc_check(device) -> None:
                            f"misaligned, 21-27 = producer and MMA waits, 28-32 = softmax waits; persistent single-token kernel: 40 = grid "
                            f"barrier, 41 = a ring slot that did not fill, 42 = a ring slot that did not empty; 32-bit product: 61 = free chunk, 62 = split "
                            f"chunk, 63 = loaded chunk, 64 = multiplied chunk, 65 = up values; streamed product: 71 = free slice, 72 = loaded slice, "
-                           f"73 = finished sums; 99 = the wait "
+                           f"73 = finished sums; attention over a bounded cache, few tokens: 81 = shared memory misaligned, 82 = a free stage, 83 = a "
+                           f"loaded stage; 99 = the wait "
                            f"probe of the tests); "
                            f"its results are not valid")
 
@@ -1746,7 +1747,8 @@ def attention_kept(q, k_pool, v_pool, out, seq_start, past, counts, block_table,
     lib().call("slb_attention_kept", _p(q), _p(k_pool), _p(v_pool), _p(out), _p(seq_start), _p(past), _p(counts), _p(block_table),
                block_table.shape[1], n, T, int(max_count), int(max_keys), heads, kv_heads, head_dim, int(window), int(first), float(scale),
                _p(lse), _p(slots), _p(weights), _p(weights_out), 0 if weights is None else weights.shape[2], _p(scratch),
-               0 if scratch is None else scratch.numel(), DT[q.dtype], stream if stream is not None else current_stream())
+               0 if scratch is None else scratch.numel(), k_pool.shape[0], _p(_tc_status(q.device)), DT[q.dtype],
+               stream if stream is not None else current_stream())
 
 
 def cache_evict_scratch_words(n_seqs: int, kv_heads: int, budget: int, max_length: int) -> int:
