@@ -34,6 +34,7 @@
 // frees its tensor memory and returns. TMA loads never use cluster multicast.
 #include <math.h>
 
+#include "kept.cuh"
 #include "tcgen05.cuh"
 
 namespace slb {
@@ -56,6 +57,22 @@ struct AttnTcArgs {
   // other score rules (off by default): score <- cap * tanh(score / cap), then score -= slopes[head] * (query position - key position)
   float softcap_log2;           // cap * log2(e), or 0
   const float* slopes;          // [H] or null
+  // a cache of bounded size (kept.cuh; only kernels instantiated for it read these): the first rows that every query sees beside its
+  // window, and where the rows' denominators go
+  int first;
+  float* lse;                   // [tokens, H] natural logarithm, or null
+  float* lse2;                  // [tokens, H] log2 units, or null
+};
+
+// The pages that a tile walks: the first ones (none without KEPT), then lo .. hi.
+struct TilePages {
+  int nf, lo, count;
+  __device__ __forceinline__ TilePages(bool kept, int key_lo, int page_hi, int first) {
+    nf = kept ? (min(first, key_lo) + 63) / 64 : 0;
+    lo = max(key_lo / 64, nf);
+    count = nf + page_hi - lo + 1;
+  }
+  __device__ __forceinline__ int page(int i) const { return i < nf ? i : lo + i - nf; }
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -109,6 +126,12 @@ __device__ __forceinline__ void store_rows(uint32_t sQ, int w, int lane, int r0,
   }
 }
 
+__device__ __forceinline__ void put_denominator(const AttnTcArgs& a, size_t row, float m, float l) {
+  const float lse2 = m + log2f(l);      // -inf for a row without weight (m = -inf, l = 0)
+  if (a.lse2) a.lse2[row] = lse2;
+  if (a.lse) a.lse[row] = lse2 * 0.6931471805599453f;
+}
+
 template <int HD>
 struct AttnTcLayout {
   static constexpr int Q_BYTES = kAtRows * HD * 2;
@@ -125,7 +148,7 @@ struct AttnTcLayout {
   static constexpr int TMEM_COLS = 256;              // S0, S1 (64 each; P_j takes the first 32 of S_j's) and O (HD <= 128)
 };
 
-template <int HD>
+template <int HD, bool KEPT>
 __global__ void __launch_bounds__(kAtThreads, 2)
 attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                const __grid_constant__ CUtensorMap map_v, AttnTcArgs a) {
@@ -159,8 +182,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   const int t_first = r0 / G;
   const int t_last = min(rows_total - 1, r0 + kAtRows - 1) / G;
   const int key_lo = first_key(past + t_first, a.window);
-  const int page_lo = key_lo / 64, page_hi = (past + t_last) / 64;
-  const int n_pages = page_hi - page_lo + 1;
+  const int page_hi = (past + t_last) / 64;
+  const TilePages pages(KEPT, key_lo, page_hi, a.first);
+  const int n_pages = pages.count;
   const int seq_len = past + count;
   const int* table = a.block_table + (size_t)seq * a.table_stride;
 
@@ -195,7 +219,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       // ---- scores: loads Q and the key pages, issues S_j = Q K_j^T one page ahead of the softmax. A page's keys are
       // asked for before the products of the page before are issued, its number a page earlier still ----
       constexpr uint32_t idesc_s = instr_desc(kAtRows, 64);
-      auto page_of = [&](int i) { return i < n_pages ? table[page_lo + i] : 0; };
+      auto page_of = [&](int i) { return i < n_pages ? table[pages.page(i)] : 0; };
       auto load_keys = [&](int j, int page) {
         const int s = j & 1;
         const int row0 = (page * a.kv_heads + kh) * 64;
@@ -238,7 +262,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     if (elect_one()) {
       // ---- values: loads the value pages, issues O += P_j V_j as soon as the softmax has written P_j ----
       constexpr uint32_t idesc_o = instr_desc(kAtRows, HD, true);
-      auto page_of = [&](int i) { return i < n_pages ? table[page_lo + i] : 0; };
+      auto page_of = [&](int i) { return i < n_pages ? table[pages.page(i)] : 0; };
       auto load_values = [&](int j, int page) {
         const int s = j & 1;
         const int row0 = (page * a.kv_heads + kh) * 64;
@@ -298,9 +322,12 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       if (lane == 0) mbar_arrive(bar);
     };
     auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory"); };
+    // KEPT: rows of a page that no row of the tile sees, whatever lies in them (values of other rows the causal mask hides are finite)
+    auto hidden = [&](int key) { return key > past + t_last || (key < key_lo && key >= a.first); };
+    auto hides = [&](int page) { return page * 64 + 63 > past + t_last || (page * 64 < key_lo && page * 64 + 63 >= a.first); };
     uint32_t s_ready = 0;
     for (int j = 0; j < n_pages; ++j) {
-      const int b = j & 1, key0 = (page_lo + j) * 64 + half * 32;
+      const int b = j & 1, page = pages.page(j), key0 = page * 64 + half * 32;
       if (!s_ready) wait_warp(s_full + 8 * b, (j >> 1) & 1, 28);
       tc_fence_after();
       uint32_t sr[32];
@@ -318,11 +345,11 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 
       // raw scores -> masked raw scores and their maximum; the mask costs two compares and a select per score, so
       // only warps with a row that needs it (the diagonal, a window's edge, padding) run it
-      if (__any_sync(0xffffffffu, key0 + 31 > pos || key0 < lo)) {
+      if (__any_sync(0xffffffffu, key0 + 31 > pos || (key0 < lo && !(KEPT && key0 + 31 < a.first)))) {
 #pragma unroll
         for (int c = 0; c < 32; ++c) {
           const int key = key0 + c;
-          if (key > pos || key < lo) sr[c] = 0xff800000u;     // -inf
+          if (key > pos || (key < lo && !(KEPT && key < a.first))) sr[c] = 0xff800000u;     // -inf
         }
       }
       float mx = -INFINITY;
@@ -375,10 +402,10 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       // P_j goes where S_j was: both threads of the row have read their scores (they met at the barrier above), and
       // the product that read P_{j-2} from these columns finished before S_j was written
       tmem_st16(lane_addr + (uint32_t)(b * 64 + half * 16), pk);
-      const int valid = seq_len - (page_lo + j) * 64;          // rows of this page that belong to the sequence
-      if (valid < 64) {
+      const int valid = seq_len - page * 64;          // rows of this page that belong to the sequence
+      if (KEPT ? hides(page) : valid < 64) {
         wait_warp(v_full + 8 * b, (j >> 1) & 1, 31);
-        if (r < 64 && r >= valid && half < HD / 64) {          // each half clears one 64-wide slab of the row
+        if (r < 64 && (KEPT ? hidden(page * 64 + r) : r >= valid) && half < HD / 64) {          // each half clears one 64-wide slab of the row
 #pragma unroll
           for (int ch = 0; ch < 8; ++ch) {
             const uint32_t dst = sV + (uint32_t)(b * L::KV_BYTES + half * 8192 + r * 128 + ch * 16);
@@ -399,6 +426,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       pair_sync();
       l += xl[(half ^ 1) * 128 + r];
       if (a.sinks) l += ex2(a.sinks[kh * G + (r0 + r) % G] * 1.4426950408889634f - m_used);     // both halves hold the same m_used
+      if (KEPT && half == 0 && ok && R < rows_total) put_denominator(a, (size_t)(tok0 + R / G) * a.heads + kh * G + R % G, m_used, l);
       const float inv = l > 0.0f ? 1.0f / l : 0.0f;
       // this thread's half of the accumulator row: all loads under way at once, one wait
       uint32_t o[HD / 2];
@@ -444,7 +472,7 @@ struct AttnWideLayout {
   static constexpr int TMEM_COLS = 512;                  // S0, S1 (128 each; P takes the first 64 of its S) and O (HD <= 128)
 };
 
-template <int HD>
+template <int HD, bool KEPT>
 __global__ void __launch_bounds__(kAwThreads, 1)
 attn_tc_wide_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                     const __grid_constant__ CUtensorMap map_v, AttnTcArgs a) {
@@ -476,8 +504,9 @@ attn_tc_wide_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   const int t_first = r0 / G;
   const int t_last = min(rows_total - 1, r0 + kAtRows - 1) / G;
   const int key_lo = first_key(past + t_first, a.window);
-  const int page_lo = key_lo / 64, page_hi = (past + t_last) / 64;
-  const int n_pages = page_hi - page_lo + 1;
+  const int page_hi = (past + t_last) / 64;
+  const TilePages pages(KEPT, key_lo, page_hi, a.first);
+  const int n_pages = pages.count;
   const int n_steps = (n_pages + 1) >> 1;
   const int seq_len = past + count;
   const int* table = a.block_table + (size_t)seq * a.table_stride;
@@ -515,7 +544,7 @@ attn_tc_wide_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       // cycles an instruction, two of N = 64 take 2 x 68); the page numbers of the step after next are asked for a
       // step early, and a step's keys are asked for before the products of the step before are issued ----
       constexpr uint32_t idesc_s2 = instr_desc(kAtRows, 128), idesc_s1 = instr_desc(kAtRows, 64);
-      auto page_of = [&](int i) { return i < n_pages ? table[page_lo + i] : 0; };
+      auto page_of = [&](int i) { return i < n_pages ? table[pages.page(i)] : 0; };
       auto load_keys = [&](int j, int pg0, int pg1) {
         const int s = j & 1, n = min(2, n_pages - 2 * j);
         mbar_expect_tx(k_full + 8 * s, (uint32_t)(n * L::PAGE_BYTES));
@@ -563,7 +592,7 @@ attn_tc_wide_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     if (elect_one()) {
       // ---- values: two value pages per step, O += P_j V_j as soon as the softmax has written P_j ----
       constexpr uint32_t idesc_o = instr_desc(kAtRows, HD, true);
-      auto page_of = [&](int i) { return i < n_pages ? table[page_lo + i] : 0; };
+      auto page_of = [&](int i) { return i < n_pages ? table[pages.page(i)] : 0; };
       auto load_values = [&](int j, int pg0, int pg1) {
         const int s = j & 1, n = min(2, n_pages - 2 * j);
         mbar_expect_tx(v_full + 8 * s, (uint32_t)(n * L::PAGE_BYTES));
@@ -625,9 +654,12 @@ attn_tc_wide_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       if (lane == 0) mbar_arrive(bar);
     };
     auto row_sync = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + quad) : "memory"); };
+    // KEPT: rows of a page that no row of the tile sees, whatever lies in them (values of other rows the causal mask hides are finite)
+    auto hidden = [&](int key) { return key > past + t_last || (key < key_lo && key >= a.first); };
+    auto hides = [&](int page) { return page * 64 + 63 > past + t_last || (page * 64 < key_lo && page * 64 + 63 >= a.first); };
     uint32_t s_ready = 0;
     for (int j = 0; j < n_steps; ++j) {
-      const int b = j & 1, page = page_lo + 2 * j + (part >> 1), key0 = page * 64 + (part & 1) * 32;
+      const int b = j & 1, page = pages.page(2 * j + (part >> 1)), key0 = page * 64 + (part & 1) * 32;
       if (!s_ready) wait_warp(s_full + 8 * b, (j >> 1) & 1, 28);
       tc_fence_after();
       uint32_t sr[32];
@@ -645,11 +677,11 @@ attn_tc_wide_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 
       // a page behind the tile's last one was never multiplied: what lies in its columns is masked like every key
       // behind the row's own position
-      if (__any_sync(0xffffffffu, key0 + 31 > pos || key0 < lo)) {
+      if (__any_sync(0xffffffffu, key0 + 31 > pos || (key0 < lo && !(KEPT && key0 + 31 < a.first)))) {
 #pragma unroll
         for (int c = 0; c < 32; ++c) {
           const int key = key0 + c;
-          if (key > pos || key < lo) sr[c] = 0xff800000u;     // -inf
+          if (key > pos || (key < lo && !(KEPT && key < a.first))) sr[c] = 0xff800000u;     // -inf
         }
       }
       float mx = -INFINITY;
@@ -698,9 +730,9 @@ attn_tc_wide_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       // P_j goes where S_j was: the four threads of the row have read their scores (they met at the barrier above)
       tmem_st16(lane_addr + (uint32_t)(b * 128 + part * 16), pk);
       const int valid = seq_len - page * 64;          // rows of this warp's page that belong to the sequence
-      if (page <= page_hi && valid < 64) {
+      if (page <= page_hi && (KEPT ? hides(page) : valid < 64)) {
         wait_warp(v_full + 8 * b, (j >> 1) & 1, 31);
-        if (r < 64 && r >= valid && (part & 1) < HD / 64) {          // each of the page's two warps-per-quad clears one 64-wide slab
+        if (r < 64 && (KEPT ? hidden(page * 64 + r) : r >= valid) && (part & 1) < HD / 64) {          // each of the page's two warps-per-quad clears one 64-wide slab
 #pragma unroll
           for (int ch = 0; ch < 8; ++ch) {
             const uint32_t dst = sV + (uint32_t)(b * L::STAGE_BYTES + (part >> 1) * L::PAGE_BYTES + (part & 1) * 8192 + r * 128 + ch * 16);
@@ -720,6 +752,7 @@ attn_tc_wide_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       row_sync();
       l = (xl[0] + xl[128]) + (xl[256] + xl[384]);
       if (a.sinks) l += ex2(a.sinks[kh * G + (r0 + r) % G] * 1.4426950408889634f - m_used);
+      if (KEPT && part == 0 && ok && R < rows_total) put_denominator(a, (size_t)(tok0 + R / G) * a.heads + kh * G + R % G, m_used, l);
       const float inv = l > 0.0f ? 1.0f / l : 0.0f;
       uint32_t o[HD / 4];      // this thread's quarter of the accumulator row
 #pragma unroll
@@ -753,7 +786,7 @@ static int encode(CUtensorMap* map, int rank, const void* base, const cuuint64_t
 // with one page a step, 0.6 with two) against the pages an SM has to walk in all (0.46 us a page with two blocks of
 // the first kernel on an SM, 0.6 with one of the second). `max_keys`: the most keys any sequence has after this
 // step (0 = not known: taken as max_count, sequences that start here).
-static bool wide_pays(int n_seqs, int max_count, int max_keys, int heads, int kv_heads, int window) {
+static bool wide_pays(int n_seqs, int max_count, int max_keys, int heads, int kv_heads, int window, int first = 0) {
   const int G = heads / kv_heads;
   const long long tiles = (max_count * (long long)G + kAtRows - 1) / kAtRows, blocks = tiles * kv_heads * n_seqs;
   const int sms = sm_count();
@@ -762,27 +795,63 @@ static bool wide_pays(int n_seqs, int max_count, int max_keys, int heads, int kv
   int longest = (max_keys + 63) / 64;      // pages of the last tile
   int mean = longest - (max_count / 64) / 2;      // tiles of a prompt grow from its first page to its last
   if (window != 0) {            // a window, or (negative) chunks
-    const int seen = (abs(window) + kAtRows / G + 63) / 64 + 1;
+    const int seen = (abs(window) + kAtRows / G + 63) / 64 + 1 + (first + 63) / 64;
     longest = min(longest, seen);
     mean = min(mean, seen);
   }
   return longest >= 16 && blocks * (long long)max(mean, 1) < (long long)sms * longest * 5 / 4;
 }
 
-template <int HD>
+template <int HD, bool KEPT>
 static int launch_attn_tc(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const AttnTcArgs& a,
                           int n_seqs, int max_count, bool wide, cudaStream_t s) {
   const int total = wide ? AttnWideLayout<HD>::TOTAL : AttnTcLayout<HD>::TOTAL;
   static std::atomic<unsigned long long> allowed[2];
-  const cudaError_t e = allow_shared(wide ? (const void*)attn_tc_wide_kernel<HD> : (const void*)attn_tc_kernel<HD>, total, allowed[wide]);
+  const cudaError_t e = allow_shared(wide ? (const void*)attn_tc_wide_kernel<HD, KEPT> : (const void*)attn_tc_kernel<HD, KEPT>, total, allowed[wide]);
   if (e != cudaSuccess) return fail(2, "attention (tcgen05): cannot reserve %d bytes of shared memory: %s", total, cudaGetErrorString(e));
   const int G = a.heads / a.kv_heads;
   const int tiles = (max_count * G + kAtRows - 1) / kAtRows;
   dim3 grid(tiles, a.kv_heads, n_seqs);
   // its prologue (barriers, tensor memory) runs while the kernel in front drains
-  if (wide) launch_prefetching(attn_tc_wide_kernel<HD>, grid, dim3(kAwThreads), (size_t)total, s, mq, mk, mv, a);
-  else launch_prefetching(attn_tc_kernel<HD>, grid, dim3(kAtThreads), (size_t)total, s, mq, mk, mv, a);
+  if (wide) launch_prefetching(attn_tc_wide_kernel<HD, KEPT>, grid, dim3(kAwThreads), (size_t)total, s, mq, mk, mv, a);
+  else launch_prefetching(attn_tc_kernel<HD, KEPT>, grid, dim3(kAtThreads), (size_t)total, s, mq, mk, mv, a);
   return check_launch("attention (tcgen05)");
+}
+
+// The maps of queries in tiles of `rows` (token, head) rows, and of a pool.
+static int encode_queries(CUtensorMap* map, const void* q, int heads, int kv_heads, int head_dim, long long tokens, int rows) {
+  const int G = heads / kv_heads;
+  cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)heads, (cuuint64_t)tokens};
+  cuuint64_t strides[2] = {(cuuint64_t)head_dim * 2, (cuuint64_t)heads * head_dim * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)(rows / G)};
+  return encode(map, 3, q, dims, strides, box, "q");
+}
+static int encode_rows(CUtensorMap* map, const void* pool, int head_dim, long long rows, const char* what) {
+  cuuint64_t dims[2] = {(cuuint64_t)head_dim, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)head_dim * 2};
+  cuuint32_t box[2] = {64, 64};
+  return encode(map, 2, pool, dims, strides, box, what);
+}
+
+// Many new tokens over a cache of bounded size (kept.cuh): the kernels above with the first rows' pages in front of the window's.
+int attention_tc_kept(const KeptArgs& k, float* lse2, long long tokens, int max_count, int max_keys, long long pool_pages, int* status,
+                      cudaStream_t stream) {
+  SLB_REQUIRE(pool_pages * k.kv_heads * 64 < (1ll << 31), "attention_kept: the pool has too many rows for one tensor map");
+  SLB_REQUIRE((uintptr_t)k.q % 16 == 0 && (uintptr_t)k.k_pool % 16 == 0 && (uintptr_t)k.v_pool % 16 == 0 && (uintptr_t)k.out % 16 == 0,
+              "attention_kept: q, out and the pools must be 16-byte aligned");
+  SLB_REQUIRE(status != nullptr && k.scale > 0.0f, "attention_kept: scale=%g, or no status word", (double)k.scale);
+  CUtensorMap mq, mk, mv;
+  int rc = encode_queries(&mq, k.q, k.heads, k.kv_heads, k.head_dim, tokens, kAtRows);
+  if (rc == 0) rc = encode_rows(&mk, k.k_pool, k.head_dim, pool_pages * k.kv_heads * 64, "the key pool");
+  if (rc == 0) rc = encode_rows(&mv, k.v_pool, k.head_dim, pool_pages * k.kv_heads * 64, "the value pool");
+  if (rc) return rc;
+  AttnTcArgs a{};
+  a.out = (__nv_bfloat16*)k.out; a.seq_start = k.seq_start; a.past = k.past; a.counts = k.counts; a.block_table = k.block_table;
+  a.table_stride = k.table_stride; a.heads = k.heads; a.kv_heads = k.kv_heads; a.window = k.window; a.scale_log2 = k.scale * kKeptLog2e;
+  a.status = status; a.first = k.first; a.lse = k.lse; a.lse2 = lse2;
+  const bool wide = wide_pays(k.n_seqs, max_count, max_keys, k.heads, k.kv_heads, k.window, k.first);
+  return k.head_dim == 64 ? launch_attn_tc<64, true>(mq, mk, mv, a, k.n_seqs, max_count, wide, stream)
+                          : launch_attn_tc<128, true>(mq, mk, mv, a, k.n_seqs, max_count, wide, stream);
 }
 
 }  // namespace slb
@@ -823,32 +892,19 @@ static int attention_tc_any(const void* q, const void* k_pool, const void* v_poo
   SLB_REQUIRE(((uintptr_t)q % 16 == 0) && ((uintptr_t)k_pool % 16 == 0) && ((uintptr_t)v_pool % 16 == 0) && ((uintptr_t)out % 16 == 0),
               "attention (tcgen05): q, pools and out must be 16-byte aligned");
   if (n_seqs == 0 || max_count == 0 || tokens == 0) return 0;
-  const int G = heads / kv_heads;
   CUtensorMap mq, mk, mv;
-  {
-    cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)heads, (cuuint64_t)tokens};
-    cuuint64_t strides[2] = {(cuuint64_t)head_dim * 2, (cuuint64_t)heads * head_dim * 2};
-    cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)(kAtRows / G)};
-    int rc = encode(&mq, 3, q, dims, strides, box, "q");
-    if (rc) return rc;
-  }
-  {
-    cuuint64_t dims[2] = {(cuuint64_t)head_dim, (cuuint64_t)(pool_pages * kv_heads * 64)};
-    cuuint64_t strides[1] = {(cuuint64_t)head_dim * 2};
-    cuuint32_t box[2] = {64, 64};
-    int rc = encode(&mk, 2, k_pool, dims, strides, box, "the key pool");
-    if (rc) return rc;
-    rc = encode(&mv, 2, v_pool, dims, strides, box, "the value pool");
-    if (rc) return rc;
-  }
-  AttnTcArgs a;
+  int rc = encode_queries(&mq, q, heads, kv_heads, head_dim, tokens, kAtRows);
+  if (rc == 0) rc = encode_rows(&mk, k_pool, head_dim, pool_pages * kv_heads * 64, "the key pool");
+  if (rc == 0) rc = encode_rows(&mv, v_pool, head_dim, pool_pages * kv_heads * 64, "the value pool");
+  if (rc) return rc;
+  AttnTcArgs a{};
   a.out = (__nv_bfloat16*)out; a.seq_start = seq_start; a.past = past; a.counts = counts; a.block_table = block_table;
   a.table_stride = table_stride; a.heads = heads; a.kv_heads = kv_heads; a.window = window;
   a.scale_log2 = scale * 1.4426950408889634f; a.status = status; a.sinks = sinks;
   a.slopes = slopes; a.softcap_log2 = softcap > 0.0f ? softcap * 1.4426950408889634f : 0.0f;
   const bool use_wide = wide < 0 ? wide_pays(n_seqs, max_count, max_keys, heads, kv_heads, window) : wide != 0;
-  return head_dim == 64 ? launch_attn_tc<64>(mq, mk, mv, a, n_seqs, max_count, use_wide, (cudaStream_t)stream)
-                        : launch_attn_tc<128>(mq, mk, mv, a, n_seqs, max_count, use_wide, (cudaStream_t)stream);
+  return head_dim == 64 ? launch_attn_tc<64, false>(mq, mk, mv, a, n_seqs, max_count, use_wide, (cudaStream_t)stream)
+                        : launch_attn_tc<128, false>(mq, mk, mv, a, n_seqs, max_count, use_wide, (cudaStream_t)stream);
 }
 
 extern "C" int slb_attention_tc(const void* q, const void* k_pool, const void* v_pool, void* out, const int* seq_start,

@@ -41,4 +41,9 @@ bool kept_few_takes(long long tokens, int max_count, int heads, int kv_heads, in
 long long kept_few_floats(long long tokens, int n_seqs, int max_count, int heads, int kv_heads, int head_dim, int max_keys, bool weights);
 int kept_few(const KeptArgs& a, long long tokens, int max_count, int max_keys, long long pool_pages, int* status, cudaStream_t s);
 
+// Steps of many tokens on the tcgen05 tensor cores: the attention (attention_tc.cu), which leaves the denominators in `lse2` (log2 units,
+// [tokens, H], may be null), and the weights from them (kept_weights.cu).
+int attention_tc_kept(const KeptArgs& a, float* lse2, long long tokens, int max_count, int max_keys, long long pool_pages, int* status, cudaStream_t s);
+int kept_weights_tc(const KeptArgs& a, const float* lse2, long long tokens, int max_count, int max_keys, long long pool_pages, int* status, cudaStream_t s);
+
 }  // namespace slb

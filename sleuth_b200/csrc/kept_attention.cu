@@ -343,9 +343,13 @@ static int general_splits(int n_seqs, int max_count, int heads, int kv_heads, in
 
 using namespace slb;
 
-enum KeptForm : int { kKeptGeneral = 0, kKeptFew = 1 };
+// Which kernels a step takes: few rows are cut along the keys (kept_few.cu), many go to the tcgen05 tensor cores, what neither takes to the
+// general kernels above.
+enum KeptForm : int { kKeptGeneral = 0, kKeptFew = 1, kKeptTc = 2 };
 static int kept_form(long long tokens, int max_count, int heads, int kv_heads, int head_dim, int max_keys, int dtype, bool weights) {
   if (kept_few_takes(tokens, max_count, heads, kv_heads, head_dim, max_keys, dtype, weights)) return kKeptFew;
+  const int G = heads / kv_heads;
+  if (dtype == kBF16 && (head_dim == 64 || head_dim == 128) && G <= 128 && 128 % G == 0) return kKeptTc;
   return kKeptGeneral;
 }
 
@@ -353,8 +357,9 @@ static int kept_form(long long tokens, int max_count, int heads, int kv_heads, i
 extern "C" long long slb_attention_kept_scratch(long long tokens, int n_seqs, int max_count, int heads, int kv_heads, int head_dim, int max_keys,
                                                 int dtype, int weights) {
   if (tokens <= 0 || n_seqs <= 0 || max_count <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || max_keys <= 0) return 0;
-  if (kept_form(tokens, max_count, heads, kv_heads, head_dim, max_keys, dtype, weights != 0) == kKeptFew)
-    return kept_few_floats(tokens, n_seqs, max_count, heads, kv_heads, head_dim, max_keys, weights != 0);
+  const int form = kept_form(tokens, max_count, heads, kv_heads, head_dim, max_keys, dtype, weights != 0);
+  if (form == kKeptFew) return kept_few_floats(tokens, n_seqs, max_count, heads, kv_heads, head_dim, max_keys, weights != 0);
+  if (form == kKeptTc) return weights ? tokens * heads : 0;
   const int splits = general_splits(n_seqs, max_count, heads, kv_heads, max_keys);
   return (weights ? tokens * heads : 0) + (splits > 1 ? (long long)splits * tokens * heads * (head_dim + 2) : 0);
 }
@@ -390,8 +395,14 @@ extern "C" int slb_attention_kept(const void* q, const void* k_pool, const void*
   a.head_dim = head_dim; a.window = window; a.first = window > 0 ? first : 0; a.scale = scale; a.slots = slots; a.weights = weights;
   a.weights_out = weights_out; a.capacity = capacity; a.lse = lse; a.scratch = scratch;
   const cudaStream_t s = (cudaStream_t)stream;
-  if (kept_form(tokens, max_count, heads, kv_heads, head_dim, max_keys, dtype, gather) == kKeptFew)
-    return kept_few(a, tokens, max_count, max_keys, pool_pages, status, s);
+  SLB_REQUIRE(scale > 0.0f, "attention_kept: the scale is positive, got %g", (double)scale);
+  const int form = kept_form(tokens, max_count, heads, kv_heads, head_dim, max_keys, dtype, gather);
+  if (form == kKeptFew) return kept_few(a, tokens, max_count, max_keys, pool_pages, status, s);
+  if (form == kKeptTc) {
+    float* lse2 = gather ? scratch : nullptr;
+    const int rc = attention_tc_kept(a, lse2, tokens, max_count, max_keys, pool_pages, status, s);
+    return rc || !gather ? rc : kept_weights_tc(a, lse2, tokens, max_count, max_keys, pool_pages, status, s);
+  }
   if (gather && lse == nullptr) {
     a.lse = scratch;
     a.scratch = scratch + tokens * heads;

@@ -1,0 +1,295 @@
+// The weights that the rows of a cache of bounded size gather in a step of many tokens (kept.cuh), on the tcgen05 tensor cores:
+//   weights_out[j] = (weights[j] if row j was there before, else 0) + sum over queries i, heads h of the group, of 2^(s_ihj - d_ih),
+// s = scale log2(e) q . k and d the rows' finished denominators in log2 units, which the attention has left.
+//
+// The scores are formed again with the keys as the instruction's rows, so that a thread of the epilogue owns one key and adds its
+// weights over the queries in registers: no sum crosses threads until the end. A block takes 128 keys (two pages) of one (sequence, kv
+// head) and walks over the (token, head) rows that see some of them, 256 at a time:
+//   * warp 0, one lane: TMA loads of the key tile (once) and of the queries (two stages), S^T = K Q^T (M = 128, N = 256: 160 cycles an
+//     instruction where two of N = 128 take 2 x 96) into one of two accumulators of 256 columns, all of tensor memory;
+//   * warp 1: the 256 denominators of the step into shared memory (infinity for rows that do not exist: their weight is 0);
+//   * warps 2 to 17: two sets of eight take the steps in turn, a warp 32 keys and 128 columns, a thread 128 scores: one FMA, one power of
+//     two, one addition each. Only steps with a key that some row does not see run a mask, a range of columns for each key.
+// A causal prompt's first keys have the longest walk; blocks start in the order of the keys. Where blocks are too few for the SMs,
+// a cluster shares a key tile: the steps are dealt to its blocks in turn, the first block adds the sums in the order of the ranks.
+// Bound by the powers of two (16 a cycle and SM: 2,048 cycles a step against 1,280 of the products).
+#include <math.h>
+
+#include "kept.cuh"
+#include "tcgen05.cuh"
+
+namespace slb {
+
+constexpr int kKwThreads = 576, kKwRows = 256, kKwKeys = 128;
+
+struct KeptWeightsArgs {
+  KeptArgs k;
+  const float* lse2;
+  float scale_log2;
+  int* status;
+};
+
+template <int HD>
+struct KwLayout {
+  static constexpr int K_BYTES = kKwKeys * HD * 2, Q_BYTES = kKwRows * HD * 2;
+  static constexpr int K_OFF = 0, Q_OFF = K_BYTES;              // two stages of queries
+  static constexpr int D_OFF = Q_OFF + 2 * Q_BYTES;             // denominators, [2][256]
+  static constexpr int SUM_OFF = D_OFF + 2 * kKwRows * 4;       // [4 parts][128 keys]
+  static constexpr int RANK_OFF = SUM_OFF + 4 * kKwKeys * 4;    // [8 ranks][128 keys] (the first block's)
+  static constexpr int BAR_OFF = RANK_OFF + 8 * kKwKeys * 4;
+  static constexpr int N_BARS = 11;
+  static constexpr int TOTAL = BAR_OFF + N_BARS * 8 + 8;
+  static_assert(TOTAL <= 226 * 1024, "the block must fit on an SM");
+};
+
+__device__ __forceinline__ float kw_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kKwThreads, 1)
+kept_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, KeptWeightsArgs w) {
+  using L = KwLayout<HD>;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  const KeptArgs& a = w.k;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t base = smem_addr(smem);
+  const int rank = (int)cluster_ctarank(), ranks = a.splits;
+  const int seq = blockIdx.z, kh = blockIdx.y, G = a.heads / a.kv_heads;
+  const int key0 = (int)(blockIdx.x / ranks) * kKwKeys;
+  const uint32_t bars = base + L::BAR_OFF;
+  const uint32_t k_full = bars, q_full = bars + 8, d_full = bars + 24, s_full = bars + 40, s_free = bars + 56, d_free = bars + 72;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::BAR_OFF + L::N_BARS * 8);
+  pdl_wait();
+  const int count = a.counts[seq], past = a.past[seq], end = past + count;
+  if (count <= 0 || key0 >= end) return;       // (the whole cluster)
+  const size_t tok0 = a.seq_start[seq];
+  const int last = min(end, key0 + kKwKeys) - 1;
+  const int t_lo = max(0, key0 - past);
+  const int t_hi = a.window > 0 && key0 >= a.first ? min(count - 1, last + a.window - 1 - past) : count - 1;
+  const int row_lo = t_lo * G, row_hi = (t_hi + 1) * G;
+  const int all_steps = t_lo <= t_hi ? (row_hi - row_lo + kKwRows - 1) / kKwRows : 0;
+  const int steps = all_steps > rank ? (all_steps - rank + ranks - 1) / ranks : 0;      // rank, rank + ranks, ...
+  const bool aligned = (base & 1023u) == 0;
+  float sum = 0.0f;
+  const int quad = warp & 3, part = (warp - 2) >> 2;      // lanes of tensor memory; part = 2 * set + half of the columns
+  if (all_steps > 0 && aligned) {
+    if (tid == 0) {
+      mbar_init(k_full, 1);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(q_full + 8 * i, 1);
+        mbar_init(d_full + 8 * i, 32);
+        mbar_init(s_full + 8 * i, 1);
+        mbar_init(s_free + 8 * i, 8);
+        mbar_init(d_free + 8 * i, 8);
+      }
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 2) {
+      __syncwarp();
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(tmem_slot)) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    if (warp == 0) {
+      if (elect_one() && steps > 0) {
+        constexpr uint32_t idesc = instr_desc(kKwKeys, kKwRows);
+        const int* table = a.block_table + (size_t)seq * a.table_stride;
+        int pages[2] = {-1, -1};
+        for (int i = 0; i < 2; ++i)
+          if (key0 + 64 * i < end) pages[i] = table[key0 / 64 + i];
+        const int held = (pages[0] >= 0) + (pages[1] >= 0);      // a page that no query sees may be gone: its rows are masked
+        mbar_expect_tx(k_full, held * (L::K_BYTES / 2));
+        for (int i = 0; i < 2; ++i)
+          if (pages[i] >= 0)
+#pragma unroll
+            for (int h = 0; h < HD / 64; ++h)
+              tma_load_2d(base + L::K_OFF + h * (kKwKeys * 128) + i * 8192, &map_k, h * 64, (pages[i] * a.kv_heads + kh) * 64, k_full);
+        auto load_queries = [&](int i) {
+          const int st = i & 1, token = t_lo + (rank + i * ranks) * (kKwRows / G);
+          mbar_expect_tx(q_full + 8 * st, L::Q_BYTES);
+#pragma unroll
+          for (int h = 0; h < HD / 64; ++h)
+            tma_load_3d(base + L::Q_OFF + st * L::Q_BYTES + h * (kKwRows * 128), &map_q, h * 64, kh * G, (int)tok0 + token, q_full + 8 * st);
+        };
+        load_queries(0);
+        bool ok = mbar_wait(k_full, 0);
+        if (!ok) atomicExch(w.status, 85);
+        for (int i = 0; i < steps && ok; ++i) {
+          const int st = i & 1;
+          if (i + 1 < steps) {
+            // the other stage was read by the products of step i - 1
+            if (i >= 1 && !mbar_wait(s_full + 8 * (st ^ 1), ((i - 1) >> 1) & 1)) { atomicExch(w.status, 86); break; }
+            load_queries(i + 1);
+          }
+          if (!mbar_wait(q_full + 8 * st, (i >> 1) & 1)) { atomicExch(w.status, 87); break; }
+          if (i >= 2 && !mbar_wait(s_free + 8 * st, ((i >> 1) - 1) & 1)) { atomicExch(w.status, 88); break; }
+          tc_fence_after();
+#pragma unroll
+          for (int h = 0; h < HD / 64; ++h) {
+            const uint64_t dk = smem_desc(base + L::K_OFF + h * (kKwKeys * 128)), dq = smem_desc(base + L::Q_OFF + st * L::Q_BYTES + h * (kKwRows * 128));
+#pragma unroll
+            for (int k4 = 0; k4 < 4; ++k4)
+              mma_bf16_ss(tmem + (uint32_t)(st * kKwRows), dk + (uint64_t)(k4 * 2), dq + (uint64_t)(k4 * 2), idesc, (h > 0 || k4 > 0) ? 1u : 0u);
+          }
+          mma_commit(s_full + 8 * st);
+        }
+      }
+    } else if (warp == 1) {
+      float* d = reinterpret_cast<float*>(smem + L::D_OFF);
+      for (int i = 0; i < steps; ++i) {
+        const int st = i & 1, R0 = row_lo + (rank + i * ranks) * kKwRows;
+        float v[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const int R = R0 + c * 32 + lane;
+          v[c] = -INFINITY;
+          if (R < row_hi) v[c] = w.lse2[(tok0 + R / G) * a.heads + kh * G + R % G];
+        }
+        if (i >= 2 && !mbar_wait(d_free + 8 * st, ((i >> 1) - 1) & 1)) {
+          if (lane == 0) atomicExch(w.status, 89);
+          break;
+        }
+        // the negative, to be added; a row without weight or behind the last gives none
+#pragma unroll
+        for (int c = 0; c < 8; ++c) d[st * kKwRows + c * 32 + lane] = v[c] == -INFINITY ? -INFINITY : -v[c];
+        mbar_arrive(d_full + 8 * st);
+      }
+    } else {
+      const int set = part >> 1, col0 = (part & 1) * 128;
+      const int key = key0 + quad * 32 + lane;
+      const float* d = reinterpret_cast<const float*>(smem + L::D_OFF);
+      // rows that see this key: [see_lo, see_hi)
+      const int see_lo = max(0, key - past) * G;
+      const int see_hi = key >= end ? 0 : a.window > 0 && key >= a.first ? (int)min((long long)row_hi, max(0ll, (long long)key + a.window - past) * G) : row_hi;
+      bool ok = true;
+      float s0 = 0.0f, s1 = 0.0f, s2 = 0.0f, s3 = 0.0f;
+      for (int i = set; i < steps; i += 2) {
+        const int st = set, R0 = row_lo + (rank + i * ranks) * kKwRows + col0;
+        if (ok && !(mbar_wait(s_full + 8 * st, (i >> 1) & 1) && mbar_wait(d_full + 8 * st, (i >> 1) & 1))) {
+          ok = false;
+          if (lane == 0) atomicExch(w.status, 90);
+        }
+        tc_fence_after();
+        const bool masked = __any_sync(0xffffffffu, R0 < see_lo || R0 + 128 > see_hi);
+        const float4* dd = reinterpret_cast<const float4*>(d + st * kKwRows + col0);
+        for (int c0 = 0; c0 < 128; c0 += 32) {
+          uint32_t sr[32];
+          tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(st * kKwRows + col0 + c0), sr);
+          if (masked) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (R0 + c0 + c < see_lo || R0 + c0 + c >= see_hi) sr[c] = 0xff800000u;
+          }
+#pragma unroll
+          for (int c = 0; c < 32; c += 4) {
+            const float4 n = dd[(c0 + c) >> 2];
+            s0 += kw_ex2(fmaf(__uint_as_float(sr[c]), w.scale_log2, n.x));
+            s1 += kw_ex2(fmaf(__uint_as_float(sr[c + 1]), w.scale_log2, n.y));
+            s2 += kw_ex2(fmaf(__uint_as_float(sr[c + 2]), w.scale_log2, n.z));
+            s3 += kw_ex2(fmaf(__uint_as_float(sr[c + 3]), w.scale_log2, n.w));
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(s_free + 8 * st);
+          mbar_arrive(d_free + 8 * st);
+        }
+      }
+      sum = (s0 + s1) + (s2 + s3);
+    }
+    if (warp >= 2) reinterpret_cast<float*>(smem + L::SUM_OFF)[part * kKwKeys + quad * 32 + lane] = sum;
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  } else if (!aligned && tid == 0) {
+    atomicExch(w.status, 84);
+  }
+  pdl_launch_dependents();
+  float total = 0.0f;
+  if (all_steps > 0 && aligned && tid < kKwKeys) {
+    const float* p = reinterpret_cast<const float*>(smem + L::SUM_OFF) + tid;
+    total = (p[0] + p[kKwKeys]) + (p[2 * kKwKeys] + p[3 * kKwKeys]);
+  }
+  if (ranks > 1) {
+    if (tid < kKwKeys) {
+      const uint32_t to = cluster_map(base + L::RANK_OFF + (rank * kKwKeys + tid) * 4, 0);
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(total) : "memory");
+    }
+    cluster_sync_all();
+    if (rank != 0) return;
+    if (tid < kKwKeys) {
+      const float* p = reinterpret_cast<const float*>(smem + L::RANK_OFF) + tid;
+      total = 0.0f;
+      for (int i = 0; i < ranks; ++i) total += p[i * kKwKeys];
+    }
+  }
+  const int key = key0 + tid;
+  if (tid < kKwKeys && key < end && key < a.capacity) {
+    const size_t at = ((size_t)(a.slots ? a.slots[seq] : seq) * a.kv_heads + kh) * a.capacity + key;
+    a.weights_out[at] = (key < past ? a.weights[at] : 0.0f) + total;
+  }
+}
+
+// Blocks that share a key tile: while blocks are fewer than two an SM, and a block keeps four steps of the longest walk.
+static int kw_ranks(int n_seqs, int kv_heads, int G, int max_count, int max_keys) {
+  const long long tiles = (long long)n_seqs * kv_heads * ((max_keys + kKwKeys - 1) / kKwKeys);
+  const int steps = (max_count * G + kKwRows - 1) / kKwRows;
+  int ranks = 1;
+  while (ranks < 8 && tiles * ranks < 2 * sm_count() && steps / (2 * ranks) >= 4) ranks *= 2;
+  return ranks;
+}
+
+static int kw_encode(CUtensorMap* map, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box, const char* what) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(2, "attention_kept: the driver does not offer cuTensorMapEncodeTiled");
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : fail(2, "attention_kept: cuTensorMapEncodeTiled failed for %s with code %d", what, (int)r);
+}
+
+template <int HD>
+static int launch_kw(const CUtensorMap& mq, const CUtensorMap& mk, const KeptWeightsArgs& w, int max_keys, cudaStream_t s) {
+  static std::atomic<unsigned long long> allowed;
+  const cudaError_t e = allow_shared((const void*)kept_weights_kernel<HD>, KwLayout<HD>::TOTAL, allowed);
+  if (e != cudaSuccess) return fail(2, "attention_kept: cannot reserve %d bytes of shared memory: %s", KwLayout<HD>::TOTAL, cudaGetErrorString(e));
+  const unsigned tiles = (unsigned)((max_keys + kKwKeys - 1) / kKwKeys);
+  const dim3 grid(tiles * w.k.splits, w.k.kv_heads, w.k.n_seqs);
+  launch_clusters(pdl_mode() != 0, (unsigned)w.k.splits, kept_weights_kernel<HD>, grid, dim3(kKwThreads), (size_t)KwLayout<HD>::TOTAL, s, mq, mk, w);
+  return check_launch("attention_kept (weights)");
+}
+
+int kept_weights_tc(const KeptArgs& k, const float* lse2, long long tokens, int max_count, int max_keys, long long pool_pages, int* status, cudaStream_t s) {
+  const int G = k.heads / k.kv_heads;
+  CUtensorMap mq, mk;
+  {
+    cuuint64_t dims[3] = {(cuuint64_t)k.head_dim, (cuuint64_t)k.heads, (cuuint64_t)tokens};
+    cuuint64_t strides[2] = {(cuuint64_t)k.head_dim * 2, (cuuint64_t)k.heads * k.head_dim * 2};
+    cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)(kKwRows / G)};
+    int rc = kw_encode(&mq, 3, k.q, dims, strides, box, "q");
+    if (rc) return rc;
+  }
+  {
+    cuuint64_t dims[2] = {(cuuint64_t)k.head_dim, (cuuint64_t)(pool_pages * k.kv_heads * 64)};
+    cuuint64_t strides[1] = {(cuuint64_t)k.head_dim * 2};
+    cuuint32_t box[2] = {64, 64};
+    int rc = kw_encode(&mk, 2, k.k_pool, dims, strides, box, "the key pool");
+    if (rc) return rc;
+  }
+  KeptWeightsArgs w{};
+  w.k = k;
+  w.k.splits = kw_ranks(k.n_seqs, k.kv_heads, G, max_count, max_keys);
+  w.lse2 = lse2;
+  w.scale_log2 = k.scale * kKeptLog2e;
+  w.status = status;
+  return k.head_dim == 64 ? launch_kw<64>(mq, mk, w, max_keys, s) : launch_kw<128>(mq, mk, w, max_keys, s);
+}
+
+}  // namespace slb

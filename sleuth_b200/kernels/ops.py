@@ -800,7 +800,7 @@ def gemm_tc_check(device) -> None:
                            f"barrier, 41 = a ring slot that did not fill, 42 = a ring slot that did not empty; 32-bit product: 61 = free chunk, 62 = split "
                            f"chunk, 63 = loaded chunk, 64 = multiplied chunk, 65 = up values; streamed product: 71 = free slice, 72 = loaded slice, "
                            f"73 = finished sums; attention over a bounded cache, few tokens: 81 = shared memory misaligned, 82 = a free stage, 83 = a "
-                           f"loaded stage; 99 = the wait "
+                           f"loaded stage; its weights: 84 = shared memory misaligned, 85-89 = producer and MMA waits, 90 = finished scores; 99 = the wait "
                            f"probe of the tests); "
                            f"its results are not valid")
 
@@ -1733,7 +1733,7 @@ def attention_kept(q, k_pool, v_pool, out, seq_start, past, counts, block_table,
     _need(q.dtype == out.dtype == k_pool.dtype == v_pool.dtype and q.dtype in DT, "attention_kept: dtypes")
     _need(tuple(k_pool.shape[1:]) == (kv_heads, 64, head_dim) and k_pool.shape == v_pool.shape, "attention_kept: pool shape")
     _rows_ok(n, "attention_kept", seq_start=seq_start, past=past, counts=counts, slots=slots)
-    _need(window >= 0 and first >= 0, "attention_kept: window and first are not negative")
+    _need(window >= 0 and first >= 0 and scale > 0, "attention_kept: window and first are not negative, the scale is positive")
     _need(lse is None or (lse.dtype == torch.float32 and lse.shape == (T, heads)), "attention_kept: lse is float32 [tokens, heads]")
     _need(scratch is None or scratch.dtype == torch.float32, "attention_kept: scratch is float32")
     _need(weights is not None or weights_out is None, "attention_kept: weights_out goes with weights")
