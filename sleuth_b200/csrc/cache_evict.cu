@@ -7,18 +7,19 @@
 // order: the least that has to be moved, and no place is read and written both. Rows of a cache are in no order of positions after that,
 // which attention over all rows does not ask for.
 //
-// A block takes one (sequence, kv head). The order is one 32-bit key a row (the weight's bits made ascending, all ones for protected rows),
-// kept in shared memory; a radix descent of four digits of eight bits finds the key of the last row that stays, and how many of the rows with
-// that very key stay (the lowest). Counts are whole numbers, so neither the blocks' nor the threads' order matters. Rows are dealt to the
-// threads in runs, so that ranks within a run are sums of a block-wide scan. Where a step can move a few rows only, the block moves them
-// itself; else it leaves the lists for a second kernel with a half warp a row.
-// Bound by latency: a block's descent; the bytes are the weights and positions once and the moved rows twice.
+// A block takes one (sequence, kv head). The order is one 32-bit key a row: the weight's bits made ascending, all ones for protected rows.
+//   * Few rows go (a token or a short turn a step): the keys stay in registers, and the rows that go are taken out one after the other, each
+//     a minimum over the block (the highest row among equals). The block moves the few rows itself.
+//   * Many go (after a prompt): the keys lie in shared memory; a radix descent of 11, 11 and 10 bits finds the key of the last row that stays, and how
+//     many of the rows with that very key stay (the lowest). Counts are whole numbers, so no order of threads matters. Rows are dealt to the threads in
+//     runs, so that ranks are sums of a block-wide scan; the lists of places and rows go to scratch, and a second kernel moves, 16 threads a row.
+// Bound by latency: loads, a descent, moves; the bytes are the weights and positions once and the moved rows twice.
 #include "common.cuh"
 
 namespace slb {
 
 constexpr int kEvictThreads = 1024;
-constexpr int kFewMoves = 32;
+constexpr int kFewGone = 16;       // rows that go one by one
 
 struct EvictArgs {
   const float* weights;      // [slots, K, capacity]
@@ -92,12 +93,106 @@ __device__ __forceinline__ void move_row(const EvictArgs& a, const int* table, i
   }
 }
 
+// ---- few rows go ----
+// THREADS threads with E keys each: row tid + e * THREADS.
+template <int THREADS, int E>
+__global__ void __launch_bounds__(THREADS) cache_evict_few_kernel(EvictArgs a) {
+  pdl_enter();
+  __shared__ unsigned long long mins[2][THREADS / 32];
+  __shared__ int gone[kFewGone], to_s[kFewGone], from_s[kFewGone];
+  __shared__ int s_moves;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kh = blockIdx.x, seq = blockIdx.y;
+  const size_t row0 = ((size_t)(a.slots ? a.slots[seq] : seq) * a.kv_heads + kh) * a.capacity;
+  const float* weights = a.weights + row0;
+  const int* positions = a.positions + row0;
+  float* weights_out = a.weights_out + row0;
+  int* positions_out = a.positions_out + row0;
+  const int* table = a.block_table + (size_t)seq * a.table_stride;
+  const int n = min(a.lengths[seq], a.max_length), past = min(a.past[seq], n), seen = a.seen[seq], left = min(n, a.budget);
+  auto position = [&](int j) { return j < past ? positions[j] : seen - (n - j); };
+  uint32_t key[E];
+  {
+    float w[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) w[e] = tid + e * THREADS < n ? weights[tid + e * THREADS] : 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int j = tid + e * THREADS, p = j < n ? position(j) : 0;
+      key[e] = j < n ? order_key(w[e], p < a.first || p >= seen - a.recent) : 0xffffffffu;
+    }
+  }
+  const int goes = n - left;           // 0 .. kFewGone
+  uint32_t live = 0;                   // rows of this thread that stay so far
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (tid + e * THREADS < n) live |= 1u << e;
+  // the least key of a thread, and its highest row: packed so that the smaller number goes first
+  auto least = [&]() {
+    unsigned long long best = ~0ull;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (live >> e & 1) {
+        const unsigned long long v = (unsigned long long)key[e] << 32 | (uint32_t)~(tid + e * THREADS);
+        best = v < best ? v : best;
+      }
+    return best;
+  };
+  unsigned long long mine = goes > 0 ? least() : 0ull;
+  for (int g = 0; g < goes; ++g) {
+    const uint32_t k = __reduce_min_sync(0xffffffffu, (uint32_t)(mine >> 32));
+    const uint32_t r = __reduce_min_sync(0xffffffffu, (uint32_t)(mine >> 32) == k ? (uint32_t)mine : 0xffffffffu);
+    if (lane == 0) mins[g & 1][warp] = (unsigned long long)k << 32 | r;
+    __syncthreads();
+    unsigned long long best = lane < THREADS / 32 ? mins[g & 1][lane] : ~0ull;
+    const uint32_t bk = __reduce_min_sync(0xffffffffu, (uint32_t)(best >> 32));
+    const uint32_t br = __reduce_min_sync(0xffffffffu, (uint32_t)(best >> 32) == bk ? (uint32_t)best : 0xffffffffu);
+    const int row = (int)~br;
+    if (tid == 0) gone[g] = row;
+    if (row % THREADS == tid) {
+      live &= ~(1u << (row / THREADS));
+      mine = least();
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int j = tid + e * THREADS;
+    if (j < left && (live >> e & 1)) {
+      if (positions_out != positions || j >= past) positions_out[j] = position(j);
+      if (weights_out != weights) weights_out[j] = weights[j];
+    }
+  }
+  if (goes == 0) return;
+  __syncthreads();
+  if (warp == 0) {       // lane i: the i-th row that went, and the i-th row behind the budget
+    const int out = lane < goes ? gone[lane] : 0x7fffffff, behind = left + lane;
+    int rank = 0;
+    bool stays = lane < goes;
+#pragma unroll
+    for (int i = 0; i < kFewGone; ++i) {
+      const int o = __shfl_sync(0xffffffffu, out, i);
+      rank += o < out;
+      if (o == behind) stays = false;
+    }
+    const unsigned holes = __ballot_sync(0xffffffffu, out < left), movers = __ballot_sync(0xffffffffu, stays);
+    if (out < left) to_s[rank] = out;          // (all rows below the budget come before those behind it)
+    if (stays) from_s[__popc(movers & ((1u << lane) - 1))] = behind;
+    if (lane == 0) s_moves = __popc(holes);
+  }
+  __syncthreads();
+  const int moves = s_moves;
+  if (tid < moves) {
+    weights_out[to_s[tid]] = weights[from_s[tid]];
+    positions_out[to_s[tid]] = position(from_s[tid]);
+  }
+  for (int i = tid >> 4; i < moves; i += THREADS / 16) move_row(a, table, kh, to_s[i], from_s[i], tid & 15, 16);
+}
+
+// ---- many rows go ----
 __global__ void __launch_bounds__(kEvictThreads) cache_evict_kernel(EvictArgs a) {
   pdl_enter();
   extern __shared__ uint32_t keys[];
-  __shared__ int hist[256];
+  __shared__ int hist[2048];
   __shared__ unsigned long long warp_sums[32];
-  __shared__ int few_to[kFewMoves], few_from[kFewMoves];
   __shared__ uint32_t s_digit;
   __shared__ int s_need;
   const int tid = threadIdx.x, kh = blockIdx.x, seq = blockIdx.y;
@@ -106,9 +201,7 @@ __global__ void __launch_bounds__(kEvictThreads) cache_evict_kernel(EvictArgs a)
   const int* positions = a.positions + row0;
   float* weights_out = a.weights_out + row0;
   int* positions_out = a.positions_out + row0;
-  const int* table = a.block_table + (size_t)seq * a.table_stride;
-  int n = min(a.lengths[seq], a.max_length);
-  if ((long long)n > a.capacity) n = (int)a.capacity;
+  const int n = min(a.lengths[seq], a.max_length);
   const int past = min(a.past[seq], n), seen = a.seen[seq];
   const int left = min(n, a.budget);
   auto position = [&](int j) { return j < past ? positions[j] : seen - (n - j); };
@@ -117,7 +210,7 @@ __global__ void __launch_bounds__(kEvictThreads) cache_evict_kernel(EvictArgs a)
     return order_key(weights[j], p < a.first || p >= seen - a.recent);
   };
   int* lists = a.scratch ? a.scratch + ((size_t)seq * a.kv_heads + kh) * (2 * (size_t)a.most_moves + 1) : nullptr;
-  if (n <= a.budget) {       // all stay
+  if (n <= a.budget) {       // all stay (the whole block leaves)
     for (int j = tid; j < n; j += kEvictThreads) {
       if (positions_out != positions || j >= past) positions_out[j] = position(j);
       if (weights_out != weights) weights_out[j] = weights[j];
@@ -133,38 +226,28 @@ __global__ void __launch_bounds__(kEvictThreads) cache_evict_kernel(EvictArgs a)
   // the key of the last row that stays: digit by digit, the largest ones first
   uint32_t prefix = 0, mask = 0;
   int need = left;             // rows still to be chosen among those that agree with the prefix
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
+#pragma unroll
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
+    hist[tid] = hist[tid + 1024] = 0;
     __syncthreads();
     for (int j = tid; j < n; j += kEvictThreads) {
       const uint32_t k = key_of(j);
-      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1);
+      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1);
     }
     __syncthreads();
-    if (tid < 32) {            // counts of the digits above each lane's eight
-      int own = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) own += hist[tid * 8 + i];
-      int above = own;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int y = __shfl_down_sync(0xffffffffu, above, d);
-        if (tid + d < 32) above += y;
-      }
-      above -= own;
-      if (above < need && above + own >= need) {
-        int i = 7;
-        for (; i > 0; --i) {
-          if (above + hist[tid * 8 + i] >= need) break;
-          above += hist[tid * 8 + i];
-        }
-        s_digit = (uint32_t)(tid * 8 + i);
-        s_need = need - above;
-      }
+    // a thread two digits, the largest first: how many keys lie above them
+    const int hi = hist[2047 - 2 * tid], lo = hist[2046 - 2 * tid];
+    unsigned long long all;
+    const int above = (int)block_scan((unsigned long long)(hi + lo), warp_sums, all);
+    if (above < need && above + hi + lo >= need) {
+      const bool in_hi = above + hi >= need;
+      s_digit = (uint32_t)(2047 - 2 * tid - (in_hi ? 0 : 1));
+      s_need = need - above - (in_hi ? 0 : hi);
     }
     __syncthreads();
     prefix |= s_digit << shift;
-    mask |= 0xffu << shift;
+    mask |= (uint32_t)(bins - 1) << shift;
     need = s_need;
     __syncthreads();
   }
@@ -187,7 +270,6 @@ __global__ void __launch_bounds__(kEvictThreads) cache_evict_kernel(EvictArgs a)
   const unsigned long long before = block_scan(counts, warp_sums, total);
   const int moves = (int)(total >> 32);
   int hole = (int)(before & 0xffffffffu), mover = (int)(before >> 32);
-  const bool few = a.most_moves <= kFewMoves;
   tie = tie0;
   for (int j = j0; j < j1; ++j) {
     const uint32_t k = key_of(j);
@@ -198,25 +280,21 @@ __global__ void __launch_bounds__(kEvictThreads) cache_evict_kernel(EvictArgs a)
         if (positions_out != positions || j >= past) positions_out[j] = position(j);
         if (weights_out != weights) weights_out[j] = weights[j];
       } else {
-        if (few) few_to[hole] = j;
-        else lists[1 + hole] = j;
+        lists[1 + hole] = j;
         ++hole;
       }
     } else if (stays) {
-      if (few) few_from[mover] = j;
-      else lists[1 + a.most_moves + mover] = j;
+      lists[1 + a.most_moves + mover] = j;
       ++mover;
     }
   }
-  if (!few && tid == 0) lists[0] = moves;
+  if (tid == 0) lists[0] = moves;
   __syncthreads();
   for (int i = tid; i < moves; i += kEvictThreads) {      // (the block's own stores are visible to it after the barrier)
-    const int to = few ? few_to[i] : lists[1 + i], from = few ? few_from[i] : lists[1 + a.most_moves + i];
+    const int to = lists[1 + i], from = lists[1 + a.most_moves + i];
     weights_out[to] = weights[from];
     positions_out[to] = position(from);
   }
-  if (few)
-    for (int i = tid >> 4; i < moves; i += kEvictThreads / 16) move_row(a, table, kh, few_to[i], few_from[i], tid & 15, 16);
 }
 
 // The moves of the lists: 16 threads a row of each pool.
@@ -237,6 +315,20 @@ static int most_moves(int budget, int max_length) {
 
 constexpr int kMostKeysShared = 48 * 1024;      // 192 KB of keys
 
+// Whether no sequence loses more rows than the kernel for that takes, nor holds more than its registers do.
+static bool few_go(int budget, int max_length) { return max_length - budget <= kFewGone && max_length <= 32 * 1024; }
+
+static int launch_evict_few(const EvictArgs& a, cudaStream_t s) {
+  const dim3 grid(a.kv_heads, a.n_seqs);
+  // a block of 256 threads up to 16 keys each, so that several share an SM; 1,024 beyond
+  if (a.max_length <= 256 * 4) launch(cache_evict_few_kernel<256, 4>, grid, dim3(256), 0, s, a);
+  else if (a.max_length <= 256 * 10) launch(cache_evict_few_kernel<256, 10>, grid, dim3(256), 0, s, a);
+  else if (a.max_length <= 512 * 10) launch(cache_evict_few_kernel<512, 10>, grid, dim3(512), 0, s, a);
+  else if (a.max_length <= 1024 * 10) launch(cache_evict_few_kernel<1024, 10>, grid, dim3(1024), 0, s, a);
+  else launch(cache_evict_few_kernel<1024, 32>, grid, dim3(1024), 0, s, a);
+  return check_launch("cache_evict (few rows)");
+}
+
 }  // namespace slb
 
 using namespace slb;
@@ -244,7 +336,7 @@ using namespace slb;
 // 32-bit words of scratch that slb_cache_evict takes: the lists of moves, where a sequence may move more rows than a block does by itself.
 extern "C" long long slb_cache_evict_scratch(int n_seqs, int kv_heads, int budget, int max_length) {
   const int moves = most_moves(budget, max_length);
-  if (n_seqs <= 0 || kv_heads <= 0 || moves <= kFewMoves) return 0;
+  if (n_seqs <= 0 || kv_heads <= 0 || few_go(budget, max_length)) return 0;
   return (long long)n_seqs * kv_heads * (2ll * moves + 1);
 }
 
@@ -273,17 +365,18 @@ extern "C" int slb_cache_evict(const float* weights, float* weights_out, const i
   a.most_moves = most_moves(budget, max_length);
   a.keys_fit = max_length <= kMostKeysShared;
   a.vector = row_bytes % 16 == 0 && (uintptr_t)k_pool % 16 == 0 && (uintptr_t)v_pool % 16 == 0;
+  if (few_go(budget, max_length)) return launch_evict_few(a, (cudaStream_t)stream);
   const int smem = a.keys_fit ? max_length * 4 : 0;
   static std::atomic<unsigned long long> allowed;
   const cudaError_t e = allow_shared((const void*)cache_evict_kernel, kMostKeysShared * 4, allowed);
   if (e != cudaSuccess) return fail(2, "cache_evict: cannot reserve shared memory: %s", cudaGetErrorString(e));
   launch(cache_evict_kernel, dim3(kv_heads, n_seqs), dim3(kEvictThreads), smem, (cudaStream_t)stream, a);
-  int rc = check_launch("cache_evict");
-  if (rc || need == 0) return rc;
+  const int rc = check_launch("cache_evict");
+  if (rc) return rc;
   const long long pairs = (long long)n_seqs * kv_heads;
   long long blocks = 8ll * sm_count() / pairs;
   const long long most = (a.most_moves + 15) / 16;
   blocks = blocks < 1 ? 1 : blocks < most ? blocks : most;
-  launch(cache_move_kernel, dim3((unsigned)blocks, kv_heads, n_seqs), dim3(256), 0, (cudaStream_t)stream, a);
+  launch_prefetching(cache_move_kernel, dim3((unsigned)blocks, kv_heads, n_seqs), dim3(256), 0, (cudaStream_t)stream, a);
   return check_launch("cache_evict (moves)");
 }

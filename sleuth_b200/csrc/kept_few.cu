@@ -3,12 +3,12 @@
 // What such a step costs is the read of the keys and values that its queries see, so the work is the pages: every sequence has so many
 // (page, kv head, tile of rows) units, and each block takes an equal run of the list of all units, whatever the sequences' lengths. A
 // (sequence, kv head, tile) that lies in one run is finished by its block; the others' shares wait in scratch for a second kernel.
-//   * warp 8, one lane: asks TMA for the pages of the block's run, keys and values, into a ring (128 KB: 32 KB a stage at heads of 128, and
-//     more than the 43 KB an SM that hide a memory latency of a microsecond at full bandwidth);
-//   * warps 0 to 7: mma.sync on the pages as they land. A tile is R times 16 rows, row r being token r / G, query head r % G of the group;
-//     R = 1: two groups of four warps take pages in turn, a warp 16 keys; R = 2: four warps share a page for each 16 rows, 16 keys each;
-//     R = 4: two, 32 keys each. Each warp keeps a running maximum, sum and weighted values of its own keys; they are joined at the end of
-//     a (sequence, kv head, tile), in the order of the warps.
+//   * the last warp: asks TMA for the pages of the block's run, keys and values, into a ring (32 KB a stage at heads of 128; about 190 KB an SM,
+//     where 43 KB hide a memory latency of a microsecond at full bandwidth);
+//   * the other warps: mma.sync on the pages as they land. A tile is R times 16 rows, row r being token r / G, query head r % G of the group.
+//     R = 1: four warps, a warp 16 of a page's keys, and two blocks an SM, so that one reads while the other joins its warps' results;
+//     R = 2 and 4: eight warps, four or two for each 16 rows, a block an SM. Each warp keeps a running maximum, sum and weighted values of its own
+//     keys; they are joined at the end of a (sequence, kv head, tile), in the order of the warps.
 // (tcgen05 has nothing to win here: its tiles are 128 rows high, and rows are 2 to 64.)
 // With weights wanted the scores go to scratch as they are formed (log2 units, 4 bytes for each row and key against 4 x head_dim for the
 // key and value: 1 to 4 per cent more bytes), because the denominators are known at the end only; the second kernel turns them into weights.
@@ -22,8 +22,32 @@
 
 namespace slb {
 
-constexpr int kFewThreads = 288;
+constexpr int few_warps(int R) { return R == 1 ? 4 : 8; }
+constexpr int few_blocks_an_sm(int R) { return R == 1 ? 2 : 1; }
 constexpr int kFewMostRows = 256;      // rows of a (sequence, kv head) that the second kernel takes
+
+// Shared memory: the ring (keys then values of a stage), queries [16 R][HD] as the ring's tiles lie, the warps' results [warps][rows][HD] float
+// and [warps][rows][2], barriers. As many stages as fit.
+struct FewLayout {
+  int stages, q_off, merge_off, ml_off, bar_off, total, merge_rows;
+};
+// (228 KB an SM; a block has 1 KB of static shared memory and 1 KB that the driver takes)
+constexpr int few_room(int R) { return (R == 1 ? 112 : 226) * 1024; }
+static FewLayout few_layout(int HD, int R, int rows) {
+  FewLayout l;
+  const int stage = 2 * 64 * HD * 2;
+  l.merge_rows = rows < 16 ? rows : 16;
+  const int rest = 16 * R * HD * 2 + few_warps(R) * l.merge_rows * (HD * 4 + 8) + 2 * 8 * 8;
+  const int room = few_room(R);
+  l.stages = (room - rest) / stage;
+  if (l.stages > 8) l.stages = 8;
+  l.q_off = l.stages * stage;
+  l.merge_off = l.q_off + 16 * R * HD * 2;
+  l.ml_off = l.merge_off + few_warps(R) * l.merge_rows * HD * 4;
+  l.bar_off = (l.ml_off + few_warps(R) * l.merge_rows * 8 + 7) & ~7;
+  l.total = l.bar_off + 2 * l.stages * 8;
+  return l;
+}
 
 struct FewArgs {
   KeptArgs k;
@@ -37,6 +61,8 @@ struct FewArgs {
   float* scores;        // [tokens, H, score_stride] or null
   long long score_stride;
   int* status;
+  FewLayout lay;
+  int out_blocks, keys_a_block;      // the second kernel's blocks of a (sequence, kv head): some for outputs, one for so many keys
 };
 
 // The pages of a step of one sequence: the first ones and the window's, as one list.
@@ -58,19 +84,6 @@ __device__ __forceinline__ float few_ex2(float x) {
   return y;
 }
 
-template <int HD, int R>
-struct FewLayout {
-  static constexpr int PAGE = 64 * HD * 2;
-  static constexpr int STAGES = HD == 128 ? 4 : 8;
-  static constexpr int Q_OFF = 0;                               // [16 R][HD] bfloat16, swizzled
-  static constexpr int RING_OFF = Q_OFF + 4 * 16 * HD * 2;      // keys then values of a stage
-  static constexpr int MERGE_OFF = RING_OFF + STAGES * 2 * PAGE;      // [8 warps][16][HD] float
-  static constexpr int ML_OFF = MERGE_OFF + 8 * 16 * HD * 4;    // [8][16][2]
-  static constexpr int BAR_OFF = ML_OFF + 8 * 16 * 2 * 4;
-  static constexpr int TOTAL = BAR_OFF + 2 * STAGES * 8;
-  static_assert(TOTAL <= 226 * 1024, "the block must fit on an SM");
-};
-
 // 16-byte piece of channel `col` of row `row` in a tile of 64 rows as TMA leaves it: 64 channels a half, pieces exchanged by the row.
 template <int ROWS>
 __device__ __forceinline__ uint32_t tile_at(int row, int col) {
@@ -78,12 +91,12 @@ __device__ __forceinline__ uint32_t tile_at(int row, int col) {
 }
 
 template <int HD, int R>
-__global__ void __launch_bounds__(kFewThreads, 1)
+__global__ void __launch_bounds__((few_warps(R) + 1) * 32, few_blocks_an_sm(R))
 kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, FewArgs fa) {
-  using L = FewLayout<HD, R>;
-  constexpr int ROWS = 16 * R, KW = R == 4 ? 32 : 16, KB = KW / 16, GROUPS = 8 / R;
+  constexpr int ROWS = 16 * R, KW = R == 4 ? 32 : 16, KB = KW / 16, WARPS = few_warps(R), GROUPS = WARPS / R, THREADS = (WARPS + 1) * 32, PAGE = 64 * HD * 2;
+  const FewLayout& L = fa.lay;
   extern __shared__ __align__(1024) unsigned char smem[];
-  __shared__ long long warp_units[9];
+  __shared__ long long warp_units[WARPS + 1];
   __shared__ long long s_first;
   __shared__ int s_seq;
   const KeptArgs& a = fa.k;
@@ -93,11 +106,11 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     if (tid == 0) atomicExch(fa.status, 81);
     return;
   }
-  const uint32_t bars = base + L::BAR_OFF;
+  const uint32_t bars = base + L.bar_off;
   if (tid == 0) {
-    for (int i = 0; i < L::STAGES; ++i) {
+    for (int i = 0; i < L.stages; ++i) {
       mbar_init(bars + 8 * i, 1);
-      mbar_init(bars + 8 * (L::STAGES + i), R == 1 ? 4 : 8);
+      mbar_init(bars + 8 * (L.stages + i), WARPS);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -110,7 +123,7 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     const int c = min(a.counts[s], fa.max_count);
     return (long long)PageRun(a.past[s], c, a.window, a.first).count * a.kv_heads * tiles_of(c);
   };
-  const int per = (a.n_seqs + kFewThreads - 1) / kFewThreads, q0 = min(a.n_seqs, tid * per), q1 = min(a.n_seqs, q0 + per);
+  const int per = (a.n_seqs + THREADS - 1) / THREADS, q0 = min(a.n_seqs, tid * per), q1 = min(a.n_seqs, q0 + per);
   long long own = 0;
   for (int s = q0; s < q1; ++s) own += units_of(s);
   long long incl = own;
@@ -123,7 +136,7 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   __syncthreads();
   long long before = 0, total = 0;
 #pragma unroll
-  for (int w = 0; w < 9; ++w) {
+  for (int w = 0; w <= WARPS; ++w) {
     if (w < warp) before += warp_units[w];
     total += warp_units[w];
   }
@@ -147,9 +160,9 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   long long seq_first = s_first;      // units before this sequence
   long long u = u_lo;
 
-  if (warp == 8) {
+  if (warp == WARPS) {
     // ---- the ring's pages ----
-    int cnt = 0;
+    int st = 0, lap = 0;
     bool ok = true;
     while (u < u_hi && ok) {
       const int count = min(a.counts[seq], fa.max_count), past = a.past[seq];
@@ -163,24 +176,24 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         const int n = (int)min((long long)(run.count - off), stop - u);
         for (int i0 = 0; i0 < n && ok; i0 += 32) {
           const int mine = i0 + lane < n ? table[run.page(off + i0 + lane)] : 0;
-          for (int i = 0; i < min(32, n - i0); ++i, ++cnt) {
+          for (int i = 0; i < min(32, n - i0); ++i) {
             const int page = __shfl_sync(0xffffffffu, mine, i);
-            const int st = cnt % L::STAGES;
-            if (cnt >= L::STAGES && !mbar_wait(bars + 8 * (L::STAGES + st), ((cnt / L::STAGES) - 1) & 1)) {
+            if (lap > 0 && !mbar_wait(bars + 8 * (L.stages + st), (lap - 1) & 1)) {
               if (lane == 0) atomicExch(fa.status, 82);
               ok = false;
               break;
             }
             if (elect_one()) {
               const int row = (page * a.kv_heads + kh) * 64;
-              const uint32_t dst = base + L::RING_OFF + st * 2 * L::PAGE;
-              mbar_expect_tx(bars + 8 * st, 2 * L::PAGE);
+              const uint32_t dst = base + st * 2 * PAGE;
+              mbar_expect_tx(bars + 8 * st, 2 * PAGE);
 #pragma unroll
               for (int h = 0; h < HD / 64; ++h) tma_load_2d(dst + h * 8192, &map_k, h * 64, row, bars + 8 * st);
 #pragma unroll
-              for (int h = 0; h < HD / 64; ++h) tma_load_2d(dst + L::PAGE + h * 8192, &map_v, h * 64, row, bars + 8 * st);
+              for (int h = 0; h < HD / 64; ++h) tma_load_2d(dst + PAGE + h * 8192, &map_v, h * 64, row, bars + 8 * st);
             }
             __syncwarp();
+            if (++st == L.stages) { st = 0; ++lap; }
           }
         }
         u += n;
@@ -194,10 +207,9 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 
   // ---- the products ----
   const int g = lane >> 2, t4 = lane & 3;
-  const int rt = R == 1 ? 0 : warp % R, group = warp / R;      // 16 rows of the tile; which keys
-  const int key_in = R == 1 ? (warp & 3) * 16 : group * KW;
-  auto sync = [&]() { asm volatile("bar.sync 1, 256;" ::: "memory"); };
-  int cnt = 0;
+  const int rt = warp % R, key_in = warp / R * KW;      // 16 rows of the tile; which keys of a page
+  auto sync = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory"); };
+  int st = 0, lap = 0;
   bool ok = true;
   while (u < u_hi) {
     const int count = min(a.counts[seq], fa.max_count), past = a.past[seq];
@@ -211,16 +223,16 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       const int n = (int)min((long long)(run.count - off), stop - u);
       const int row0 = tile * ROWS, rows = min(ROWS, count * G - row0);
       // queries (the previous tile's results have been read: every warp has passed its last barrier)
-      for (int e = tid; e < ROWS * (HD / 8); e += 256) {
+      for (int e = tid; e < ROWS * (HD / 8); e += WARPS * 32) {
         const int r = e / (HD / 8), col = (e % (HD / 8)) * 8, Rr = row0 + r;
         uint4 v = make_uint4(0, 0, 0, 0);
         if (r < rows) v = *reinterpret_cast<const uint4*>((const __nv_bfloat16*)a.q + ((size_t)(tok0 + Rr / G) * a.heads + kh * G + Rr % G) * HD + col);
-        *reinterpret_cast<uint4*>(smem + L::Q_OFF + tile_at<ROWS>(r, col)) = v;
+        *reinterpret_cast<uint4*>(smem + L.q_off + tile_at<ROWS>(r, col)) = v;
       }
       sync();
       uint32_t qf[HD / 16][4];
 #pragma unroll
-      for (int kb = 0; kb < HD / 16; ++kb) ldmatrix_x4(qf[kb], base + L::Q_OFF + tile_at<ROWS>(rt * 16 + (lane & 15), kb * 16 + ((lane >> 4) << 3)));
+      for (int kb = 0; kb < HD / 16; ++kb) ldmatrix_x4(qf[kb], base + L.q_off + tile_at<ROWS>(rt * 16 + (lane & 15), kb * 16 + ((lane >> 4) << 3)));
       int pos[2], lo[2];
       float* score_row[2];
 #pragma unroll
@@ -240,19 +252,15 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 #pragma unroll
       for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
       float m_r[2] = {-INFINITY, -INFINITY}, l_r[2] = {0.0f, 0.0f};
-      for (int i = 0; i < n; ++i, ++cnt) {
-        if (R == 1 && (i & 1) != (warp >> 2)) {
-          continue;
-        }
-        const int st = cnt % L::STAGES;
-        if (ok && !mbar_wait(bars + 8 * st, (cnt / L::STAGES) & 1)) {
+      for (int i = 0; i < n; ++i) {
+        if (ok && !mbar_wait(bars + 8 * st, lap & 1)) {
           ok = false;
           if (lane == 0) atomicExch(fa.status, 83);
         }
         const int key0 = run.page(off + i) * 64 + key_in;
         const bool none = idle || key0 > any_hi || (key0 + KW - 1 < any_lo && key0 >= a.first);
         if (!none) {
-          const uint32_t kS = base + L::RING_OFF + st * 2 * L::PAGE, vS = kS + L::PAGE;
+          const uint32_t kS = base + st * 2 * PAGE, vS = kS + PAGE;
           float s[2 * KB][4];
 #pragma unroll
           for (int j = 0; j < 2 * KB; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
@@ -352,23 +360,24 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
           }
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(bars + 8 * (L::STAGES + st));
+        if (lane == 0) mbar_arrive(bars + 8 * (L.stages + st));
+        if (++st == L.stages) { st = 0; ++lap; }
       }
 
       // join the warps that share these rows
-      float* mo = reinterpret_cast<float*>(smem + L::MERGE_OFF);      // [8][16][HD]
-      float* ml = reinterpret_cast<float*>(smem + L::ML_OFF);         // [8][16][2]
+      float* mo = reinterpret_cast<float*>(smem + L.merge_off);      // [warps][rows][HD]
+      float* ml = reinterpret_cast<float*>(smem + L.ml_off);         // [warps][rows][2]
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         l_r[h] += __shfl_xor_sync(0xffffffffu, l_r[h], 1);
         l_r[h] += __shfl_xor_sync(0xffffffffu, l_r[h], 2);
         const int r = g + 8 * h;
         if (rt * 16 + r >= rows) continue;
-        if (t4 == 0) *reinterpret_cast<float2*>(ml + (warp * 16 + r) * 2) = make_float2(m_r[h], l_r[h]);
+        if (t4 == 0) *reinterpret_cast<float2*>(ml + (warp * L.merge_rows + r) * 2) = make_float2(m_r[h], l_r[h]);
         // (rows of a warp start 8 x 4-byte banks apart by the row, so that the eight rows of a store meet different banks)
 #pragma unroll
         for (int c = 0; c < HD / 8; ++c)
-          *reinterpret_cast<float2*>(mo + (warp * 16 + r) * HD + ((c * 8 + 2 * t4) ^ ((r & 3) << 3))) = make_float2(o[c][2 * h], o[c][2 * h + 1]);
+          *reinterpret_cast<float2*>(mo + (warp * L.merge_rows + r) * HD + ((c * 8 + 2 * t4) ^ ((r & 3) << 3))) = make_float2(o[c][2 * h], o[c][2 * h + 1]);
       }
       sync();
       const bool begins = off == 0, complete = begins && n == run.count;
@@ -380,17 +389,17 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         fa.info[((size_t)seq * a.kv_heads + kh) * fa.max_tiles + tile] = make_int2(first_block, last_block - first_block + 1);
       }
       const size_t slot = ((size_t)blockIdx.x * 2 + (begins ? 1 : 0)) * ROWS;
-      for (int e = tid; e < rows * (HD / 4); e += 256) {
+      for (int e = tid; e < rows * (HD / 4); e += WARPS * 32) {
         const int r = e / (HD / 4), d = (e % (HD / 4)) * 4, in = r & 15;
         float M = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < GROUPS; ++w) M = fmaxf(M, ml[((w * R + (r >> 4)) * 16 + in) * 2]);
+        for (int w = 0; w < GROUPS; ++w) M = fmaxf(M, ml[((w * R + (r >> 4)) * L.merge_rows + in) * 2]);
         const float top = M == -INFINITY ? 0.0f : M;
         float sum = 0.0f;
         float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
         for (int w = 0; w < GROUPS; ++w) {
-          const int at = (w * R + (r >> 4)) * 16 + in;
+          const int at = (w * R + (r >> 4)) * L.merge_rows + in;
           const float f = few_ex2(ml[at * 2] - top);
           const float4 v = *reinterpret_cast<const float4*>(mo + at * HD + (d ^ ((in & 3) << 3)));
           sum += ml[at * 2 + 1] * f;
@@ -422,104 +431,118 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   }
 }
 
-// Joins the shares of what no block finished alone, and turns scores into weights: a block takes some of the outputs and 1,024 keys of one
-// (sequence, kv head).
+// Joins the shares of what no block finished alone, and turns scores into weights: of the blocks of a (sequence, kv head) the first few take
+// outputs, the others `keys_a_block` keys each.
 template <int HD, int R>
 __global__ void __launch_bounds__(256) kept_few_finish_kernel(FewArgs fa) {
   pdl_wait();
   const KeptArgs& a = fa.k;
   constexpr int ROWS = 16 * R;
   __shared__ float lse_s[kFewMostRows];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  __shared__ int pos_s[kFewMostRows];
+  __shared__ long long row_s[kFewMostRows];
+  const int tid = threadIdx.x;
   const int kh = blockIdx.y, seq = blockIdx.z, G = a.heads / a.kv_heads;
   const int count = min(a.counts[seq], fa.max_count), past = a.past[seq], tok0 = a.seq_start[seq], rows_total = count * G;
   if (count <= 0) return;
   const int2* info = fa.info + ((size_t)seq * a.kv_heads + kh) * fa.max_tiles;
   auto row_of = [&](int Rr) { return (size_t)(tok0 + Rr / G) * a.heads + kh * G + Rr % G; };
   auto slot_of = [&](int2 in, int i) { return ((size_t)(in.x + i) * 2 + (i == 0 ? 1 : 0)) * ROWS; };
-  // denominators: a warp a row, its lanes along the shares
-  if (fa.scores != nullptr || a.lse != nullptr) {
-    for (int Rr = warp; Rr < rows_total; Rr += 8) {
+  const bool outputs = (int)blockIdx.x < fa.out_blocks;
+  const int key_begin = ((int)blockIdx.x - fa.out_blocks) * fa.keys_a_block, end = past + count;
+  if (!outputs && key_begin >= end) return;
+  if (outputs) {
+    for (int e = blockIdx.x * 256 + tid; e < rows_total * (HD / 4); e += fa.out_blocks * 256) {
+      const int Rr = e / (HD / 4), d = (e % (HD / 4)) * 4;
       const int2 in = info[Rr / ROWS];
-      float v;
-      if (in.y == 1) {
-        v = fa.lse2 ? fa.lse2[row_of(Rr)] : 0.0f;
-      } else {
-        float M = -INFINITY, L = 0.0f;
-        for (int i = lane; i < in.y; i += 32) {
-          const float2 p = *reinterpret_cast<const float2*>(fa.part_ml + (slot_of(in, i) + Rr % ROWS) * 2);
-          const float top = fmaxf(M, p.x), use = top == -INFINITY ? 0.0f : top;
-          L = L * few_ex2(M - use) + p.y * few_ex2(p.x - use);
-          M = top;
+      if (in.y == 1) continue;
+      float M = -INFINITY, L = 0.0f;
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int i0 = 0; i0 < in.y; i0 += 8) {
+        float2 p[8];
+        float4 v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const size_t at = slot_of(in, i0 + i < in.y ? i0 + i : 0) + Rr % ROWS;
+          p[i] = *reinterpret_cast<const float2*>(fa.part_ml + at * 2);
+          v[i] = *reinterpret_cast<const float4*>(fa.part + at * HD + d);
+          if (i0 + i >= in.y) p[i].x = -INFINITY;
         }
-        const float top = warp_max(M), use = top == -INFINITY ? 0.0f : top;
-        L = warp_sum(L * few_ex2(M - use));
-        v = L == 0.0f ? -INFINITY : use + log2f(L);
-        if (lane == 0 && blockIdx.x == 0 && a.lse) a.lse[row_of(Rr)] = v * 0.6931471805599453f;
-      }
-      if (lane == 0) lse_s[Rr] = v;
-    }
-  }
-  // outputs
-  for (int e = blockIdx.x * 256 + tid; e < rows_total * (HD / 4); e += gridDim.x * 256) {
-    const int Rr = e / (HD / 4), d = (e % (HD / 4)) * 4;
-    const int2 in = info[Rr / ROWS];
-    if (in.y == 1) continue;
-    float M = -INFINITY, L = 0.0f;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int i0 = 0; i0 < in.y; i0 += 8) {
-      float2 p[8];
-      float4 v[8];
+        float top = M;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const bool live = i0 + i < in.y;
-        const size_t at = slot_of(in, live ? i0 + i : 0) + Rr % ROWS;
-        p[i] = *reinterpret_cast<const float2*>(fa.part_ml + at * 2);
-        v[i] = *reinterpret_cast<const float4*>(fa.part + at * HD + d);
-        if (!live) p[i] = make_float2(-INFINITY, 0.0f);
-      }
-      float top = M;
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, p[i].x);
+        const float use = top == -INFINITY ? 0.0f : top, keep = few_ex2(M - use);
+        L *= keep;
+        acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = fmaxf(top, p[i].x);
-      const float use = top == -INFINITY ? 0.0f : top, keep = few_ex2(M - use);
-      L *= keep;
-      acc.x *= keep; acc.y *= keep; acc.z *= keep; acc.w *= keep;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float f = few_ex2(p[i].x - use);
-        if (i0 + i < in.y) {      // (a share whose scores were all NaN has maximum -inf and a sum of NaN)
-          L += p[i].y * f;
-          acc.x += v[i].x * f; acc.y += v[i].y * f; acc.z += v[i].z * f; acc.w += v[i].w * f;
+        for (int i = 0; i < 8; ++i) {
+          const float f = few_ex2(p[i].x - use);
+          if (i0 + i < in.y) {      // (a share whose scores were all NaN has maximum -inf and a sum of NaN)
+            L += p[i].y * f;
+            acc.x += v[i].x * f; acc.y += v[i].y * f; acc.z += v[i].z * f; acc.w += v[i].w * f;
+          }
         }
+        M = top;
       }
-      M = top;
+      const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+      uint2 pk;
+      pk.x = pack_bf16(acc.x * inv, acc.y * inv);
+      pk.y = pack_bf16(acc.z * inv, acc.w * inv);
+      *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + row_of(Rr) * HD + d) = pk;
+      if (d == 0 && a.lse) a.lse[row_of(Rr)] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
     }
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    uint2 pk;
-    pk.x = pack_bf16(acc.x * inv, acc.y * inv);
-    pk.y = pack_bf16(acc.z * inv, acc.w * inv);
-    *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + row_of(Rr) * HD + d) = pk;
+    return;
   }
-  if (fa.scores == nullptr) return;
+  // denominators, a thread a row
+  if (tid < rows_total) {
+    const int2 in = info[tid / ROWS];
+    const size_t row = row_of(tid);
+    float v;
+    if (in.y == 1) {
+      v = fa.lse2[row];
+    } else {
+      float M = -INFINITY, L = 0.0f;
+      for (int i0 = 0; i0 < in.y; i0 += 8) {
+        float2 p[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          p[i] = *reinterpret_cast<const float2*>(fa.part_ml + (slot_of(in, i0 + i < in.y ? i0 + i : 0) + tid % ROWS) * 2);
+          if (i0 + i >= in.y) p[i] = make_float2(-INFINITY, 0.0f);
+        }
+        float top = M;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, p[i].x);
+        const float use = top == -INFINITY ? 0.0f : top;
+        L *= few_ex2(M - use);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) L += p[i].y * few_ex2(p[i].x - use);
+        M = top;
+      }
+      v = L == 0.0f ? -INFINITY : M + log2f(L);
+    }
+    lse_s[tid] = v == -INFINITY ? INFINITY : v;      // a row without weight gives none
+    pos_s[tid] = past + tid / G;
+    row_s[tid] = (long long)row * fa.score_stride;
+  }
   __syncthreads();
-  const int end = past + count;
   const size_t at0 = ((size_t)(a.slots ? a.slots[seq] : seq) * a.kv_heads + kh) * a.capacity;
-  for (int c = 0; c < 4; ++c) {
-    const int key = blockIdx.x * 1024 + c * 256 + tid;
-    if (key >= end || key >= a.capacity) break;
-    float sum = 0.0f;
-    for (int i = 0; i < count; ++i) {
-      const int p = past + i;
-      if (!sees(key, p, window_lo(p, a.window), a.first)) continue;
-      const float* src = fa.scores + ((size_t)(tok0 + i) * a.heads + kh * G) * fa.score_stride + key;
-#pragma unroll 4
-      for (int h = 0; h < G; ++h) {
-        const float d = lse_s[i * G + h];
-        const float w = few_ex2(src[(size_t)h * fa.score_stride] - d);
-        if (d != -INFINITY) sum += w;
+  const int key_end = (int)min((long long)min(end, key_begin + fa.keys_a_block), a.capacity);
+  for (int key = key_begin + tid; key < key_end; key += 256) {
+    float sum = key < past ? a.weights[at0 + key] : 0.0f;
+    float gained = 0.0f;
+    for (int r0 = 0; r0 < rows_total; r0 += 8) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = r0 + i;
+        v[i] = -INFINITY;
+        if (r < rows_total && sees(key, pos_s[r], window_lo(pos_s[r], a.window), a.first)) v[i] = fa.scores[row_s[r] + key];
       }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (r0 + i < rows_total) gained += few_ex2(v[i] - lse_s[r0 + i]);
     }
-    a.weights_out[at0 + key] = (key < past ? a.weights[at0 + key] : 0.0f) + sum;
+    a.weights_out[at0 + key] = sum + gained;
   }
 }
 
@@ -535,7 +558,8 @@ static FewScratch few_scratch(long long tokens, int n_seqs, int max_count, int h
   const int G = heads / kv_heads, R = few_row_tiles(max_count, G);
   f.max_tiles = (max_count * G + 16 * R - 1) / (16 * R);
   const long long units = (long long)n_seqs * kv_heads * f.max_tiles * ((max_keys + 63) / 64);
-  f.blocks = (int)(units < sm_count() ? units : sm_count());      // a block an SM; none without a page
+  const long long most = (long long)sm_count() * few_blocks_an_sm(R);
+  f.blocks = (int)(units < most ? units : most);      // as many as run at once; none without a page
   const long long slots = 2ll * f.blocks * 16 * R;
   long long at = 0;
   auto take = [&](long long n) { const long long o = at; at += (n + 3) & ~3ll; return o; };
@@ -550,19 +574,24 @@ static FewScratch few_scratch(long long tokens, int n_seqs, int max_count, int h
 }
 
 template <int HD, int R>
-static int launch_few(const CUtensorMap& mk, const CUtensorMap& mv, const FewArgs& fa, int blocks, int max_keys, int max_count, cudaStream_t s) {
-  using L = FewLayout<HD, R>;
+static int launch_few(const CUtensorMap& mk, const CUtensorMap& mv, FewArgs fa, int blocks, int max_keys, int max_count, cudaStream_t s) {
+  const int rows = max_count * (fa.k.heads / fa.k.kv_heads);
+  fa.lay = few_layout(HD, R, rows);
   static std::atomic<unsigned long long> allowed;
-  const cudaError_t e = allow_shared((const void*)kept_few_kernel<HD, R>, L::TOTAL, allowed);
-  if (e != cudaSuccess) return fail(2, "attention_kept: cannot reserve %d bytes of shared memory: %s", L::TOTAL, cudaGetErrorString(e));
-  launch(kept_few_kernel<HD, R>, dim3(blocks), dim3(kFewThreads), (size_t)L::TOTAL, s, mk, mv, fa);
-  int rc = check_launch("attention_kept (few tokens)");
+  const cudaError_t e = allow_shared((const void*)kept_few_kernel<HD, R>, few_room(R), allowed);
+  if (e != cudaSuccess) return fail(2, "attention_kept: cannot reserve shared memory: %s", cudaGetErrorString(e));
+  launch(kept_few_kernel<HD, R>, dim3(blocks), dim3((few_warps(R) + 1) * 32), (size_t)fa.lay.total, s, mk, mv, fa);
+  const int rc = check_launch("attention_kept (few tokens)");
   if (rc) return rc;
-  const int G = fa.k.heads / fa.k.kv_heads;
-  int gx = fa.scores ? (max_keys + 1023) / 1024 : 1;
-  const int outs = (max_count * G * (HD / 4) + 255) / 256;
-  gx = gx > outs ? gx : outs < 8 ? outs : 8 > gx ? 8 : gx;
-  launch_prefetching(kept_few_finish_kernel<HD, R>, dim3(gx, fa.k.kv_heads, fa.k.n_seqs), dim3(256), 0, s, fa);
+  const long long pairs = (long long)fa.k.n_seqs * fa.k.kv_heads;
+  fa.out_blocks = (rows * (HD / 4) + 255) / 256;
+  long long key_blocks = 0;
+  if (fa.scores) {      // about eight blocks an SM in all; each works out the denominators for itself
+    const long long wanted = 8ll * sm_count() / pairs;
+    fa.keys_a_block = (int)((max_keys / (wanted < 1 ? 1 : wanted) + 256) / 256 * 256);
+    key_blocks = (max_keys + fa.keys_a_block - 1) / fa.keys_a_block;
+  }
+  launch_prefetching(kept_few_finish_kernel<HD, R>, dim3((unsigned)(fa.out_blocks + key_blocks), fa.k.kv_heads, fa.k.n_seqs), dim3(256), 0, s, fa);
   return check_launch("attention_kept (few tokens, joined)");
 }
 

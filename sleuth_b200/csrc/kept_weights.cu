@@ -8,8 +8,9 @@
 //   * warp 0, one lane: TMA loads of the key tile (once) and of the queries (two stages), S^T = K Q^T (M = 128, N = 256: 160 cycles an
 //     instruction where two of N = 128 take 2 x 96) into one of two accumulators of 256 columns, all of tensor memory;
 //   * warp 1: the 256 denominators of the step into shared memory (infinity for rows that do not exist: their weight is 0);
-//   * warps 2 to 17: two sets of eight take the steps in turn, a warp 32 keys and 128 columns, a thread 128 scores: one FMA, one power of
-//     two, one addition each. Only steps with a key that some row does not see run a mask, a range of columns for each key.
+//   * warps 2 to 17: a warp 32 keys and 64 columns of every step, a thread 64 scores, which it takes into registers at once so that the next
+//     product may begin: one FMA, one power of two, one addition each. Only steps with a key that some row does not see run a mask, a
+//     range of columns for each key. (Two sets of warps that took the steps in turn each waited for their own product: 2.4 us a step.)
 // A causal prompt's first keys have the longest walk; blocks start in the order of the keys. Where blocks are too few for the SMs,
 // a cluster shares a key tile: the steps are dealt to its blocks in turn, the first block adds the sums in the order of the ranks.
 // Bound by the powers of two (16 a cycle and SM: 2,048 cycles a step against 1,280 of the products).
@@ -74,7 +75,7 @@ kept_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   const int steps = all_steps > rank ? (all_steps - rank + ranks - 1) / ranks : 0;      // rank, rank + ranks, ...
   const bool aligned = (base & 1023u) == 0;
   float sum = 0.0f;
-  const int quad = warp & 3, part = (warp - 2) >> 2;      // lanes of tensor memory; part = 2 * set + half of the columns
+  const int quad = warp & 3, part = (warp - 2) >> 2;      // lanes of tensor memory; 64 of a step's columns
   if (all_steps > 0 && aligned) {
     if (tid == 0) {
       mbar_init(k_full, 1);
@@ -82,8 +83,8 @@ kept_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         mbar_init(q_full + 8 * i, 1);
         mbar_init(d_full + 8 * i, 32);
         mbar_init(s_full + 8 * i, 1);
-        mbar_init(s_free + 8 * i, 8);
-        mbar_init(d_free + 8 * i, 8);
+        mbar_init(s_free + 8 * i, 16);
+        mbar_init(d_free + 8 * i, 16);
       }
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -161,7 +162,7 @@ kept_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         mbar_arrive(d_full + 8 * st);
       }
     } else {
-      const int set = part >> 1, col0 = (part & 1) * 128;
+      const int col0 = part * 64;
       const int key = key0 + quad * 32 + lane;
       const float* d = reinterpret_cast<const float*>(smem + L::D_OFF);
       // rows that see this key: [see_lo, see_hi)
@@ -169,38 +170,36 @@ kept_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       const int see_hi = key >= end ? 0 : a.window > 0 && key >= a.first ? (int)min((long long)row_hi, max(0ll, (long long)key + a.window - past) * G) : row_hi;
       bool ok = true;
       float s0 = 0.0f, s1 = 0.0f, s2 = 0.0f, s3 = 0.0f;
-      for (int i = set; i < steps; i += 2) {
-        const int st = set, R0 = row_lo + (rank + i * ranks) * kKwRows + col0;
+      for (int i = 0; i < steps; ++i) {
+        const int st = i & 1, R0 = row_lo + (rank + i * ranks) * kKwRows + col0;
         if (ok && !(mbar_wait(s_full + 8 * st, (i >> 1) & 1) && mbar_wait(d_full + 8 * st, (i >> 1) & 1))) {
           ok = false;
           if (lane == 0) atomicExch(w.status, 90);
         }
         tc_fence_after();
-        const bool masked = __any_sync(0xffffffffu, R0 < see_lo || R0 + 128 > see_hi);
-        const float4* dd = reinterpret_cast<const float4*>(d + st * kKwRows + col0);
-        for (int c0 = 0; c0 < 128; c0 += 32) {
-          uint32_t sr[32];
-          tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(st * kKwRows + col0 + c0), sr);
-          if (masked) {
+        uint32_t sr[64];
 #pragma unroll
-            for (int c = 0; c < 32; ++c)
-              if (R0 + c0 + c < see_lo || R0 + c0 + c >= see_hi) sr[c] = 0xff800000u;
-          }
-#pragma unroll
-          for (int c = 0; c < 32; c += 4) {
-            const float4 n = dd[(c0 + c) >> 2];
-            s0 += kw_ex2(fmaf(__uint_as_float(sr[c]), w.scale_log2, n.x));
-            s1 += kw_ex2(fmaf(__uint_as_float(sr[c + 1]), w.scale_log2, n.y));
-            s2 += kw_ex2(fmaf(__uint_as_float(sr[c + 2]), w.scale_log2, n.z));
-            s3 += kw_ex2(fmaf(__uint_as_float(sr[c + 3]), w.scale_log2, n.w));
-          }
-        }
+        for (int c0 = 0; c0 < 64; c0 += 16) tmem_ld16_nowait(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(st * kKwRows + col0 + c0), sr + c0);
+        tmem_wait_ld();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(s_free + 8 * st);
-          mbar_arrive(d_free + 8 * st);
+        if (lane == 0) mbar_arrive(s_free + 8 * st);      // the next product may overwrite the scores
+        if (__any_sync(0xffffffffu, R0 < see_lo || R0 + 64 > see_hi)) {
+#pragma unroll
+          for (int c = 0; c < 64; ++c)
+            if (R0 + c < see_lo || R0 + c >= see_hi) sr[c] = 0xff800000u;
         }
+        const float4* dd = reinterpret_cast<const float4*>(d + st * kKwRows + col0);
+#pragma unroll
+        for (int c = 0; c < 64; c += 4) {
+          const float4 n = dd[c >> 2];
+          s0 += kw_ex2(fmaf(__uint_as_float(sr[c]), w.scale_log2, n.x));
+          s1 += kw_ex2(fmaf(__uint_as_float(sr[c + 1]), w.scale_log2, n.y));
+          s2 += kw_ex2(fmaf(__uint_as_float(sr[c + 2]), w.scale_log2, n.z));
+          s3 += kw_ex2(fmaf(__uint_as_float(sr[c + 3]), w.scale_log2, n.w));
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(d_free + 8 * st);
       }
       sum = (s0 + s1) + (s2 + s3);
     }

@@ -27,7 +27,8 @@ def lib() -> library.KernelLibrary:
 
 
 def current_stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    # (the handle itself: building torch's stream object costs 2 us of a call's 10)
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _p(t):
@@ -1687,14 +1688,24 @@ def sigmoid_gate(y, gate, stream=None) -> None:
 # ---- a cache of bounded size: the first rows, the latest ones and those that queries look at most ----
 
 
-def _gathered_ok(t, kv_heads: int, dtype, what: str) -> None:
-    _need(t is not None and t.dtype == dtype and t.dim() == 3 and t.shape[1] == kv_heads and t.shape[2] > 0,
-          f"{what}: [slots, kv_heads, rows] of {dtype}")
+def _kept_refusal(what: str, tensors: dict, checks) -> None:
+    """Says which of an operator's conditions does not hold (worked out only when one does not: a call's checks cost the host 2 us this
+    way, 8 us one by one)."""
+    for name, t in tensors.items():
+        if t is not None:
+            _need(t.is_cuda, f"{what}: {name} must be a CUDA tensor; the kernels of sleuth_b200 run on CUDA tensors only")
+            _need(t.is_contiguous(), f"{what}: {name} of shape {tuple(t.shape)} must be contiguous")
+    for cond, msg in checks:
+        try:
+            ok = cond()
+        except (AttributeError, IndexError, TypeError):
+            ok = False
+        _need(ok, f"{what}: {msg}")
+    _need(False, f"{what}: the arguments do not fit together")
 
 
-def _rows_ok(n: int, what: str, **tables) -> None:
-    for name, t in tables.items():
-        _need(t is None or (t.dtype == torch.int32 and t.numel() >= n), f"{what}: {name} is int32, one per sequence")
+def _plain_cuda(t) -> bool:
+    return t is None or (t.is_cuda and t.is_contiguous())
 
 
 def attention_kept_scratch_floats(tokens: int, n_seqs: int, max_count: int, heads: int, kv_heads: int, head_dim: int, max_keys: int,
@@ -1726,29 +1737,50 @@ def attention_kept(q, k_pool, v_pool, out, seq_start, past, counts, block_table,
     scores are all -inf gives zeros and gathers nothing. Values of hidden rows never reach a result, whatever they are, except that in
     bfloat16 an infinity or NaN among the values of a row that some query of the same tile of up to 128 (token, head) rows sees may
     reach the tile's other rows."""
-    _cuda(q, k_pool, v_pool, out, seq_start, past, counts, block_table, scratch, lse, weights, weights_out, slots)
-    _need(block_table.dtype == torch.int32 and block_table.dim() == 2, "attention_kept: block table")
-    T, n = q.shape[0], block_table.shape[0]
-    _need(q.shape == (T, heads, head_dim) and out.shape == (T, heads * head_dim), "attention_kept: shapes disagree")
-    _need(q.dtype == out.dtype == k_pool.dtype == v_pool.dtype and q.dtype in DT, "attention_kept: dtypes")
-    _need(tuple(k_pool.shape[1:]) == (kv_heads, 64, head_dim) and k_pool.shape == v_pool.shape, "attention_kept: pool shape")
-    _rows_ok(n, "attention_kept", seq_start=seq_start, past=past, counts=counts, slots=slots)
-    _need(window >= 0 and first >= 0 and scale > 0, "attention_kept: window and first are not negative, the scale is positive")
-    _need(lse is None or (lse.dtype == torch.float32 and lse.shape == (T, heads)), "attention_kept: lse is float32 [tokens, heads]")
-    _need(scratch is None or scratch.dtype == torch.float32, "attention_kept: scratch is float32")
-    _need(weights is not None or weights_out is None, "attention_kept: weights_out goes with weights")
+    dt, i32, f32 = q.dtype, torch.int32, torch.float32
+    q_shape, k_shape, (n, stride) = q.shape, k_pool.shape, block_table.shape
+    T, capacity = q_shape[0], 0
     if weights is not None:
-        weights_out = weights if weights_out is None else weights_out
-        _gathered_ok(weights, kv_heads, torch.float32, "attention_kept: weights")
-        _need(weights_out.dtype == torch.float32 and weights_out.shape == weights.shape, "attention_kept: weights_out as weights")
-        _need(slots is not None or weights.shape[0] >= n, "attention_kept: weights hold a row of every sequence")
-        _need(weights.shape[2] >= (max_keys if 0 < max_keys <= 64 * block_table.shape[1] else 64 * block_table.shape[1]),
-              "attention_kept: weights are shorter than the cache")
-    lib().call("slb_attention_kept", _p(q), _p(k_pool), _p(v_pool), _p(out), _p(seq_start), _p(past), _p(counts), _p(block_table),
-               block_table.shape[1], n, T, int(max_count), int(max_keys), heads, kv_heads, head_dim, int(window), int(first), float(scale),
-               _p(lse), _p(slots), _p(weights), _p(weights_out), 0 if weights is None else weights.shape[2], _p(scratch),
-               0 if scratch is None else scratch.numel(), k_pool.shape[0], _p(_tc_status(q.device)), DT[q.dtype],
-               stream if stream is not None else current_stream())
+        if weights_out is None:
+            weights_out = weights
+        capacity = weights.shape[-1]
+    if not (q.is_cuda and q.is_contiguous() and k_pool.is_cuda and k_pool.is_contiguous() and v_pool.is_cuda and v_pool.is_contiguous()
+            and out.is_cuda and out.is_contiguous() and seq_start.is_cuda and seq_start.is_contiguous() and past.is_cuda and past.is_contiguous()
+            and counts.is_cuda and counts.is_contiguous() and block_table.is_cuda and block_table.is_contiguous()
+            and _plain_cuda(scratch) and _plain_cuda(lse) and _plain_cuda(slots)
+            and q_shape == (T, heads, head_dim) and out.shape == (T, heads * head_dim) and dt in DT
+            and dt == out.dtype == k_pool.dtype == v_pool.dtype and k_shape == (k_shape[0], kv_heads, 64, head_dim) and k_shape == v_pool.shape
+            and i32 == block_table.dtype == seq_start.dtype == past.dtype == counts.dtype
+            and seq_start.numel() >= n and past.numel() >= n and counts.numel() >= n
+            and window >= 0 and first >= 0 and scale > 0
+            and (lse is None or (lse.dtype == f32 and lse.shape == (T, heads))) and (scratch is None or scratch.dtype == f32)
+            and (slots is None or (slots.dtype == i32 and slots.numel() >= n))
+            and (weights_out is None if weights is None else (
+                weights.is_cuda and weights.is_contiguous() and weights_out.is_cuda and weights_out.is_contiguous()
+                and f32 == weights.dtype == weights_out.dtype and weights.dim() == 3 and weights.shape == weights_out.shape
+                and weights.shape[1] == kv_heads and (slots is not None or weights.shape[0] >= n)
+                and capacity >= (max_keys if 0 < max_keys <= 64 * stride else 64 * stride)))):
+        _kept_refusal("attention_kept", dict(q=q, k_pool=k_pool, v_pool=v_pool, out=out, seq_start=seq_start, past=past, counts=counts,
+                                             block_table=block_table, scratch=scratch, lse=lse, weights=weights, weights_out=weights_out, slots=slots), (
+            (lambda: q_shape == (T, heads, head_dim) and out.shape == (T, heads * head_dim), "q is [tokens, heads, head_dim], out [tokens, heads * head_dim]"),
+            (lambda: dt in DT and dt == out.dtype == k_pool.dtype == v_pool.dtype, "q, out and the pools are float32 or bfloat16 alike"),
+            (lambda: k_shape == (k_shape[0], kv_heads, 64, head_dim) and k_shape == v_pool.shape, "pools are [pages, kv_heads, 64, head_dim]"),
+            (lambda: i32 == block_table.dtype == seq_start.dtype == past.dtype == counts.dtype and min(x.numel() for x in (seq_start, past, counts)) >= n,
+             "block_table, seq_start, past and counts are int32, one row a sequence"),
+            (lambda: window >= 0 and first >= 0 and scale > 0, "window and first are not negative, the scale is positive"),
+            (lambda: lse is None or (lse.dtype == f32 and lse.shape == (T, heads)), "lse is float32 [tokens, heads]"),
+            (lambda: scratch is None or scratch.dtype == f32, "scratch is float32"),
+            (lambda: slots is None or (slots.dtype == i32 and slots.numel() >= n), "slots are int32, one a sequence"),
+            (lambda: weights is not None or weights_out is None, "weights_out goes with weights"),
+            (lambda: f32 == weights.dtype == weights_out.dtype and weights.dim() == 3 and weights.shape == weights_out.shape and weights.shape[1] == kv_heads,
+             "weights and weights_out are float32 [slots, kv_heads, rows]"),
+            (lambda: slots is not None or weights.shape[0] >= n, "weights hold a row of every sequence"),
+            (lambda: capacity >= (max_keys if 0 < max_keys <= 64 * stride else 64 * stride), "weights are shorter than the cache")))
+    status = _TC_STATUS.get(q.device)
+    lib().call("slb_attention_kept", q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), seq_start.data_ptr(), past.data_ptr(),
+               counts.data_ptr(), block_table.data_ptr(), stride, n, T, int(max_count), int(max_keys), heads, kv_heads, head_dim, int(window), int(first), float(scale),
+               _p(lse), _p(slots), _p(weights), _p(weights_out), capacity, _p(scratch), 0 if scratch is None else scratch.numel(), k_shape[0],
+               (status if status is not None else _tc_status(q.device)).data_ptr(), DT[dt], stream if stream is not None else current_stream())
 
 
 def cache_evict_scratch_words(n_seqs: int, kv_heads: int, budget: int, max_length: int) -> int:
@@ -1771,24 +1803,41 @@ def cache_evict(weights, positions, k_pool, v_pool, block_table, past, lengths, 
     min(length, ``budget``) rows, and the pages behind them are free. ``weights_out`` / ``positions_out``: where the rows' weights and
     positions go (default: in place); places behind the last row are left alone. ``max_length``: a promise that no sequence
     holds more rows (0: as many as its table takes); ``scratch``: ``cache_evict_scratch_words`` int32 words."""
-    _cuda(weights, positions, k_pool, v_pool, block_table, past, lengths, seen, weights_out, positions_out, slots, scratch)
-    _need(block_table.dtype == torch.int32 and block_table.dim() == 2, "cache_evict: block table")
-    n, kv_heads = block_table.shape[0], k_pool.shape[1]
-    _need(k_pool.dim() == 4 and k_pool.shape == v_pool.shape and k_pool.dtype == v_pool.dtype and k_pool.dtype in DT and k_pool.shape[2] == 64,
-          "cache_evict: pools [pages, kv_heads, 64, head_dim]")
-    row_bytes = k_pool.shape[3] * k_pool.element_size()
-    _need(row_bytes % 4 == 0, "cache_evict: a row's bytes are a multiple of four")
-    _gathered_ok(weights, kv_heads, torch.float32, "cache_evict: weights")
-    _gathered_ok(positions, kv_heads, torch.int32, "cache_evict: positions")
-    weights_out = weights if weights_out is None else weights_out
-    positions_out = positions if positions_out is None else positions_out
-    _need(positions.shape == weights.shape == weights_out.shape == positions_out.shape and weights_out.dtype == torch.float32
-          and positions_out.dtype == torch.int32, "cache_evict: weights, positions and their targets have one shape")
-    _need(slots is not None or weights.shape[0] >= n, "cache_evict: weights hold a row of every sequence")
-    _rows_ok(n, "cache_evict", past=past, lengths=lengths, seen=seen, slots=slots)
-    _need(budget > 0 and first >= 0 and recent >= 0 and first + recent <= budget, "cache_evict: first and recent rows fit the budget")
-    _need(scratch is None or scratch.dtype == torch.int32, "cache_evict: scratch is int32")
-    lib().call("slb_cache_evict", _p(weights), _p(weights_out), _p(positions), _p(positions_out), weights.shape[2], _p(k_pool), _p(v_pool),
-               _p(block_table), block_table.shape[1], n, kv_heads, row_bytes, _p(past), _p(lengths), _p(seen), _p(slots), int(budget),
-               int(first), int(recent), int(max_length), _p(scratch), 0 if scratch is None else scratch.numel(),
+    i32, f32 = torch.int32, torch.float32
+    k_shape, w_shape, (n, stride) = k_pool.shape, weights.shape, block_table.shape
+    if weights_out is None:
+        weights_out = weights
+    if positions_out is None:
+        positions_out = positions
+    kv_heads, row_bytes = k_shape[1], k_shape[-1] * k_pool.element_size()
+    if not (weights.is_cuda and weights.is_contiguous() and positions.is_cuda and positions.is_contiguous() and k_pool.is_cuda
+            and k_pool.is_contiguous() and v_pool.is_cuda and v_pool.is_contiguous() and block_table.is_cuda and block_table.is_contiguous()
+            and past.is_cuda and past.is_contiguous() and lengths.is_cuda and lengths.is_contiguous() and seen.is_cuda and seen.is_contiguous()
+            and weights_out.is_cuda and weights_out.is_contiguous() and positions_out.is_cuda and positions_out.is_contiguous()
+            and _plain_cuda(slots) and _plain_cuda(scratch)
+            and k_pool.dtype in DT and k_pool.dtype == v_pool.dtype and len(k_shape) == 4 and k_shape == v_pool.shape and k_shape[2] == 64
+            and row_bytes % 4 == 0 and i32 == block_table.dtype == past.dtype == lengths.dtype == seen.dtype
+            and past.numel() >= n and lengths.numel() >= n and seen.numel() >= n
+            and f32 == weights.dtype == weights_out.dtype and i32 == positions.dtype == positions_out.dtype
+            and len(w_shape) == 3 and w_shape[1] == kv_heads and w_shape[2] > 0 and w_shape == positions.shape == weights_out.shape == positions_out.shape
+            and (slots is None and w_shape[0] >= n or slots is not None and slots.dtype == i32 and slots.numel() >= n)
+            and (scratch is None or scratch.dtype == i32) and budget > 0 and first >= 0 and recent >= 0 and first + recent <= budget):
+        _kept_refusal("cache_evict", dict(weights=weights, positions=positions, k_pool=k_pool, v_pool=v_pool, block_table=block_table, past=past,
+                                          lengths=lengths, seen=seen, weights_out=weights_out, positions_out=positions_out, slots=slots, scratch=scratch), (
+            (lambda: k_pool.dtype in DT and k_pool.dtype == v_pool.dtype and len(k_shape) == 4 and k_shape == v_pool.shape and k_shape[2] == 64,
+             "pools are [pages, kv_heads, 64, head_dim], float32 or bfloat16"),
+            (lambda: row_bytes % 4 == 0, "a row's bytes are a multiple of four"),
+            (lambda: i32 == block_table.dtype == past.dtype == lengths.dtype == seen.dtype and min(x.numel() for x in (past, lengths, seen)) >= n,
+             "block_table, past, lengths and seen are int32, one row a sequence"),
+            (lambda: f32 == weights.dtype == weights_out.dtype and len(w_shape) == 3 and w_shape[1] == kv_heads and w_shape[2] > 0,
+             "weights are float32 [slots, kv_heads, rows]"),
+            (lambda: i32 == positions.dtype == positions_out.dtype and w_shape == positions.shape == weights_out.shape == positions_out.shape,
+             "positions are int32, and all four have one shape"),
+            (lambda: slots is None and w_shape[0] >= n or slots is not None and slots.dtype == i32 and slots.numel() >= n,
+             "slots are int32, one a sequence; without them weights hold a row of every sequence"),
+            (lambda: scratch is None or scratch.dtype == i32, "scratch is int32"),
+            (lambda: budget > 0 and first >= 0 and recent >= 0 and first + recent <= budget, "first and recent rows fit the budget")))
+    lib().call("slb_cache_evict", weights.data_ptr(), weights_out.data_ptr(), positions.data_ptr(), positions_out.data_ptr(), w_shape[2],
+               k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(), stride, n, kv_heads, row_bytes, past.data_ptr(), lengths.data_ptr(),
+               seen.data_ptr(), _p(slots), int(budget), int(first), int(recent), int(max_length), _p(scratch), 0 if scratch is None else scratch.numel(),
                stream if stream is not None else current_stream())
