@@ -75,6 +75,9 @@ struct TilePages {
   __device__ __forceinline__ int page(int i) const { return i < nf ? i : lo + i - nf; }
 };
 
+// The n lowest of 32 bits (n below 0 counts as 0, above 32 as 32).
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -346,10 +349,17 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       // raw scores -> masked raw scores and their maximum; the mask costs two compares and a select per score, so
       // only warps with a row that needs it (the diagonal, a window's edge, padding) run it
       if (__any_sync(0xffffffffu, key0 + 31 > pos || (key0 < lo && !(KEPT && key0 + 31 < a.first)))) {
+        if constexpr (KEPT) {      // one bit a key: two tests of a score less
+          const uint32_t seen = bits_below(pos + 1 - key0) & (~bits_below(lo - key0) | bits_below(a.first - key0));
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          const int key = key0 + c;
-          if (key > pos || (key < lo && !(KEPT && key < a.first))) sr[c] = 0xff800000u;     // -inf
+          for (int c = 0; c < 32; ++c)
+            if (!(seen >> c & 1u)) sr[c] = 0xff800000u;     // -inf
+        } else {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            const int key = key0 + c;
+            if (key > pos || key < lo) sr[c] = 0xff800000u;
+          }
         }
       }
       float mx = -INFINITY;
@@ -678,10 +688,17 @@ attn_tc_wide_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       // a page behind the tile's last one was never multiplied: what lies in its columns is masked like every key
       // behind the row's own position
       if (__any_sync(0xffffffffu, key0 + 31 > pos || (key0 < lo && !(KEPT && key0 + 31 < a.first)))) {
+        if constexpr (KEPT) {      // one bit a key: two tests of a score less
+          const uint32_t seen = bits_below(pos + 1 - key0) & (~bits_below(lo - key0) | bits_below(a.first - key0));
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          const int key = key0 + c;
-          if (key > pos || (key < lo && !(KEPT && key < a.first))) sr[c] = 0xff800000u;     // -inf
+          for (int c = 0; c < 32; ++c)
+            if (!(seen >> c & 1u)) sr[c] = 0xff800000u;     // -inf
+        } else {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            const int key = key0 + c;
+            if (key > pos || key < lo) sr[c] = 0xff800000u;
+          }
         }
       }
       float mx = -INFINITY;

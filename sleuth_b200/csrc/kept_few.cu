@@ -441,6 +441,7 @@ __global__ void __launch_bounds__(256) kept_few_finish_kernel(FewArgs fa) {
   __shared__ float lse_s[kFewMostRows];
   __shared__ int pos_s[kFewMostRows];
   __shared__ long long row_s[kFewMostRows];
+  __shared__ float sum_s[4][256];
   const int tid = threadIdx.x;
   const int kh = blockIdx.y, seq = blockIdx.z, G = a.heads / a.kv_heads;
   const int count = min(a.counts[seq], fa.max_count), past = a.past[seq], tok0 = a.seq_start[seq], rows_total = count * G;
@@ -527,22 +528,45 @@ __global__ void __launch_bounds__(256) kept_few_finish_kernel(FewArgs fa) {
   __syncthreads();
   const size_t at0 = ((size_t)(a.slots ? a.slots[seq] : seq) * a.kv_heads + kh) * a.capacity;
   const int key_end = (int)min((long long)min(end, key_begin + fa.keys_a_block), a.capacity);
-  for (int key = key_begin + tid; key < key_end; key += 256) {
-    float sum = key < past ? a.weights[at0 + key] : 0.0f;
-    float gained = 0.0f;
-    for (int r0 = 0; r0 < rows_total; r0 += 8) {
-      float v[8];
+  // four keys a thread, four groups of threads for the rows r = group, group + 4, ...; the groups' sums are added in their order
+  const int quad = tid & 63, group = tid >> 6;
+  for (int key0 = key_begin; key0 < key_end; key0 += 256) {
+    const int key = key0 + 4 * quad;
+    float4 gained = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (key < key_end) {
+      for (int r0 = group; r0 < rows_total; r0 += 16) {
+        float4 v[4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = r0 + i;
-        v[i] = -INFINITY;
-        if (r < rows_total && sees(key, pos_s[r], window_lo(pos_s[r], a.window), a.first)) v[i] = fa.scores[row_s[r] + key];
+        for (int i = 0; i < 4; ++i) {
+          const int r = r0 + 4 * i;
+          v[i] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+          if (r >= rows_total) continue;
+          const int pos = pos_s[r], lo = window_lo(pos, a.window);
+          const bool s0 = sees(key, pos, lo, a.first), s1 = sees(key + 1, pos, lo, a.first), s2 = sees(key + 2, pos, lo, a.first), s3 = sees(key + 3, pos, lo, a.first);
+          if (s0 || s1 || s2 || s3) {
+            const float4 x = *reinterpret_cast<const float4*>(fa.scores + row_s[r] + key);
+            if (s0) v[i].x = x.x;
+            if (s1) v[i].y = x.y;
+            if (s2) v[i].z = x.z;
+            if (s3) v[i].w = x.w;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (r0 + 4 * i >= rows_total) continue;
+          const float d = lse_s[r0 + 4 * i];
+          gained.x += few_ex2(v[i].x - d); gained.y += few_ex2(v[i].y - d);
+          gained.z += few_ex2(v[i].z - d); gained.w += few_ex2(v[i].w - d);
+        }
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (r0 + i < rows_total) gained += few_ex2(v[i] - lse_s[r0 + i]);
     }
-    a.weights_out[at0 + key] = sum + gained;
+    __syncthreads();
+    *reinterpret_cast<float4*>(&sum_s[group][4 * quad]) = gained;
+    __syncthreads();
+    if (key0 + tid < key_end) {
+      const float before = key0 + tid < past ? a.weights[at0 + key0 + tid] : 0.0f;
+      a.weights_out[at0 + key0 + tid] = before + ((sum_s[0][tid] + sum_s[1][tid]) + (sum_s[2][tid] + sum_s[3][tid]));
+    }
   }
 }
 
@@ -567,7 +591,7 @@ static FewScratch few_scratch(long long tokens, int n_seqs, int max_count, int h
   f.part_ml = take(slots * 2);
   f.info = take(2ll * n_seqs * kv_heads * f.max_tiles);
   f.lse2 = weights ? take(tokens * heads) : 0;
-  f.score_stride = (max_keys + 1) & ~1;
+  f.score_stride = (max_keys + 3) & ~3;
   f.scores = weights ? take(tokens * heads * f.score_stride) : 0;
   f.total = at;
   return f;

@@ -17,6 +17,7 @@
 #include <math.h>
 
 #include "kept.cuh"
+#include "packed_f32.cuh"
 #include "tcgen05.cuh"
 
 namespace slb {
@@ -39,7 +40,8 @@ struct KwLayout {
   static constexpr int RANK_OFF = SUM_OFF + 4 * kKwKeys * 4;    // [8 ranks][128 keys] (the first block's)
   static constexpr int BAR_OFF = RANK_OFF + 8 * kKwKeys * 4;
   static constexpr int N_BARS = 11;
-  static constexpr int TOTAL = BAR_OFF + N_BARS * 8 + 8;
+  static constexpr int ODD_OFF = BAR_OFF + N_BARS * 8 + 8;     // [2] whether a denominator of the step is NaN or infinite
+  static constexpr int TOTAL = ODD_OFF + 8;
   static_assert(TOTAL <= 226 * 1024, "the block must fit on an SM");
 };
 
@@ -47,6 +49,22 @@ __device__ __forceinline__ float kw_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// 2^x for two x of at most a little above 0, on the FMA pipe: x = n + f with f in [-1/2, 1/2] (adding 1.5 * 2^23 leaves n in the low bits), 2^f
+// by the polynomial of degree 5 with the least largest relative error (7.5e-8, by the Remez exchange), n added to the exponent. Below
+// 2^-126 the result is 2^-126, nothing beside a weight that counts; NaN would come out as that too, so rows whose denominator is NaN or
+// infinite (any such score among the keys that they see makes it that) do not come here.
+__device__ __forceinline__ f32x2 kw_ex2_pair(f32x2 x) {
+  x = pair_of(fmaxf(low_half(x), -126.0f), fmaxf(high_half(x), -126.0f));
+  const f32x2 t = add2(x, both(12582912.0f)), f = add2(x, mul2(add2(t, both(-12582912.0f)), both(-1.0f)));
+  f32x2 p = fma2(f, both(0.0013276472454890609f), both(0.009675540961325169f));
+  p = fma2(p, f, both(0.05550713092088699f));
+  p = fma2(p, f, both(0.24022120237350464f));
+  p = fma2(p, f, both(0.6931469440460205f));
+  p = fma2(p, f, both(1.0000001192092896f));
+  return pair_of(__uint_as_float(__float_as_uint(low_half(p)) + (__float_as_uint(low_half(t)) << 23)),
+                 __uint_as_float(__float_as_uint(high_half(p)) + (__float_as_uint(high_half(t)) << 23)));
 }
 
 template <int HD>
@@ -58,8 +76,10 @@ kept_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t base = smem_addr(smem);
   const int rank = (int)cluster_ctarank(), ranks = a.splits;
-  const int seq = blockIdx.z, kh = blockIdx.y, G = a.heads / a.kv_heads;
-  const int key0 = (int)(blockIdx.x / ranks) * kKwKeys;
+  // clusters start in the order of their number: the first keys of all sequences and heads, whose walk is the longest, before the next
+  const int G = a.heads / a.kv_heads, pairs = (int)(gridDim.y * gridDim.z);
+  const int lin = (int)(blockIdx.x / ranks + gridDim.x / ranks * (blockIdx.y + gridDim.y * blockIdx.z));
+  const int seq = (lin % pairs) / (int)gridDim.y, kh = (lin % pairs) % (int)gridDim.y, key0 = lin / pairs * kKwKeys;
   const uint32_t bars = base + L::BAR_OFF;
   const uint32_t k_full = bars, q_full = bars + 8, d_full = bars + 24, s_full = bars + 40, s_free = bars + 56, d_free = bars + 72;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::BAR_OFF + L::N_BARS * 8);
@@ -156,6 +176,11 @@ kept_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           if (lane == 0) atomicExch(w.status, 89);
           break;
         }
+        bool odd = false;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) odd = odd || !(v[c] < INFINITY);
+        odd = __any_sync(0xffffffffu, odd);
+        if (lane == 0) reinterpret_cast<int*>(smem + L::ODD_OFF)[st] = odd;
         // the negative, to be added; a row without weight or behind the last gives none
 #pragma unroll
         for (int c = 0; c < 8; ++c) d[st * kKwRows + c * 32 + lane] = v[c] == -INFINITY ? -INFINITY : -v[c];
@@ -169,7 +194,8 @@ kept_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       const int see_lo = max(0, key - past) * G;
       const int see_hi = key >= end ? 0 : a.window > 0 && key >= a.first ? (int)min((long long)row_hi, max(0ll, (long long)key + a.window - past) * G) : row_hi;
       bool ok = true;
-      float s0 = 0.0f, s1 = 0.0f, s2 = 0.0f, s3 = 0.0f;
+      f32x2 s0 = 0, s1 = 0;
+      const f32x2 scale2 = both(w.scale_log2);
       for (int i = 0; i < steps; ++i) {
         const int st = i & 1, R0 = row_lo + (rank + i * ranks) * kKwRows + col0;
         if (ok && !(mbar_wait(s_full + 8 * st, (i >> 1) & 1) && mbar_wait(d_full + 8 * st, (i >> 1) & 1))) {
@@ -189,19 +215,32 @@ kept_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           for (int c = 0; c < 64; ++c)
             if (R0 + c < see_lo || R0 + c >= see_hi) sr[c] = 0xff800000u;
         }
-        const float4* dd = reinterpret_cast<const float4*>(d + st * kKwRows + col0);
+        const bool odd = reinterpret_cast<const int*>(smem + L::ODD_OFF)[st] != 0;
+        const ulonglong2* dd = reinterpret_cast<const ulonglong2*>(d + st * kKwRows + col0);
+        if (odd) {
+#pragma unroll
+          for (int c = 0; c < 64; c += 4) {
+            const ulonglong2 n = dd[c >> 2];
+            const f32x2 x0 = fma2(pair_of(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), scale2, n.x);
+            const f32x2 x1 = fma2(pair_of(__uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3])), scale2, n.y);
+            s0 = add2(s0, pair_of(kw_ex2(low_half(x0)), kw_ex2(high_half(x0))));
+            s1 = add2(s1, pair_of(kw_ex2(low_half(x1)), kw_ex2(high_half(x1))));
+          }
+        } else {
 #pragma unroll
         for (int c = 0; c < 64; c += 4) {
-          const float4 n = dd[c >> 2];
-          s0 += kw_ex2(fmaf(__uint_as_float(sr[c]), w.scale_log2, n.x));
-          s1 += kw_ex2(fmaf(__uint_as_float(sr[c + 1]), w.scale_log2, n.y));
-          s2 += kw_ex2(fmaf(__uint_as_float(sr[c + 2]), w.scale_log2, n.z));
-          s3 += kw_ex2(fmaf(__uint_as_float(sr[c + 3]), w.scale_log2, n.w));
+          const ulonglong2 n = dd[c >> 2];
+          const f32x2 x0 = fma2(pair_of(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), scale2, n.x);
+          const f32x2 x1 = fma2(pair_of(__uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3])), scale2, n.y);
+          // three pairs of eight by the polynomial: 5 cycles a score on either pipe where the powers of two alone take 8
+          s0 = add2(s0, pair_of(kw_ex2(low_half(x0)), kw_ex2(high_half(x0))));
+          s1 = add2(s1, (c >> 2) % 4 != 3 ? kw_ex2_pair(x1) : pair_of(kw_ex2(low_half(x1)), kw_ex2(high_half(x1))));
+        }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(d_free + 8 * st);
       }
-      sum = (s0 + s1) + (s2 + s3);
+      sum = halves_sum(s0) + halves_sum(s1);
     }
     if (warp >= 2) reinterpret_cast<float*>(smem + L::SUM_OFF)[part * kKwKeys + quad * 32 + lane] = sum;
     tc_fence_before();

@@ -22,6 +22,18 @@ __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
   return d;
 }
 
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+__device__ __forceinline__ f32x2 pair_of(float low, float high) {
+  f32x2 d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(low), "f"(high));
+  return d;
+}
+
 __device__ __forceinline__ f32x2 both(float v) {
   f32x2 d;
   asm("mov.b64 %0, {%1, %1};" : "=l"(d) : "f"(v));
