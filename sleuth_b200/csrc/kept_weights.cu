@@ -4,17 +4,20 @@
 //
 // The scores are formed again with the keys as the instruction's rows, so that a thread of the epilogue owns one key and adds its
 // weights over the queries in registers: no sum crosses threads until the end. A block takes 128 keys (two pages) of one (sequence, kv
-// head) and walks over the (token, head) rows that see some of them, 256 at a time:
-//   * warp 0, one lane: TMA loads of the key tile (once) and of the queries (two stages), S^T = K Q^T (M = 128, N = 256: 160 cycles an
-//     instruction where two of N = 128 take 2 x 96) into one of two accumulators of 256 columns, all of tensor memory;
-//   * warp 1: the 256 denominators of the step into shared memory (infinity for rows that do not exist: their weight is 0);
-//   * warps 2 to 17: a warp 32 keys and 64 columns of every step, a thread 64 scores, which it takes into registers at once so that the next
-//     product may begin: one FMA, one power of two, one addition each. Only steps with a key that some row does not see run a mask, a
-//     range of columns for each key. (Two sets of warps that took the steps in turn each waited for their own product: 2.4 us a step.)
-// A causal prompt's first keys have the longest walk; blocks start in the order of the keys. Where blocks are too few for the SMs,
-// a cluster shares a key tile: the steps are dealt to its blocks in turn, the first block adds the sums in the order of the ranks.
-// Bound by the powers of two (16 a cycle and SM: 2,048 cycles a step against 1,280 of the products).
+// head) and walks over the (token, head) rows that see some of them, 128 at a time:
+//   * warp 0, one lane: TMA loads of the key tile (once) and of the queries, a ring of five stages (eight at heads of 64): what a step reads from L2, 32
+//     KB, takes about as long as its products, and arrives late with two;
+//   * warp 1, one lane: S^T = K Q^T (M = 128, N = 128) into one of four accumulators of 128 columns, all of tensor memory;
+//   * warp 2: the 128 denominators of a step into shared memory, asked for a step early;
+//   * warps 3 to 18: two sets of eight take the steps in turn, a warp 32 keys and 64 columns, a thread 64 scores, which it takes into registers at
+//     once so that the accumulator is free again. Per score one FMA, one power of two, one addition; three powers of eight are worked out on the
+//     FMA pipe, five cycles a score on either pipe. Only steps with a key that some row does not see run a mask, a range of columns for each key.
+// Clusters start in the order of their number: the first keys of all sequences and heads, whose walk is the longest, before the next ones. Where
+// blocks are too few for the SMs, a cluster shares a key tile: the steps are dealt to its blocks in turn, the first block adds the sums in the
+// order of the ranks.
 #include <math.h>
+
+#include <type_traits>
 
 #include "kept.cuh"
 #include "packed_f32.cuh"
@@ -22,7 +25,7 @@
 
 namespace slb {
 
-constexpr int kKwThreads = 576, kKwRows = 256, kKwKeys = 128;
+constexpr int kKwThreads = 608, kKwRows = 128, kKwKeys = 128, kKwBuffers = 4;
 
 struct KeptWeightsArgs {
   KeptArgs k;
@@ -33,15 +36,15 @@ struct KeptWeightsArgs {
 
 template <int HD>
 struct KwLayout {
-  static constexpr int K_BYTES = kKwKeys * HD * 2, Q_BYTES = kKwRows * HD * 2;
-  static constexpr int K_OFF = 0, Q_OFF = K_BYTES;              // two stages of queries
-  static constexpr int D_OFF = Q_OFF + 2 * Q_BYTES;             // denominators, [2][256]
-  static constexpr int SUM_OFF = D_OFF + 2 * kKwRows * 4;       // [4 parts][128 keys]
-  static constexpr int RANK_OFF = SUM_OFF + 4 * kKwKeys * 4;    // [8 ranks][128 keys] (the first block's)
+  static constexpr int K_BYTES = kKwKeys * HD * 2, Q_BYTES = kKwRows * HD * 2, STAGES = HD == 128 ? 5 : 8;
+  static constexpr int K_OFF = 0, Q_OFF = K_BYTES;
+  static constexpr int D_OFF = Q_OFF + STAGES * Q_BYTES;                // denominators, [4 buffers][128]
+  static constexpr int SUM_OFF = D_OFF + kKwBuffers * kKwRows * 4;      // [4 parts][128 keys]
+  static constexpr int RANK_OFF = SUM_OFF + 4 * kKwKeys * 4;            // [8 ranks][128 keys] (the first block's)
   static constexpr int BAR_OFF = RANK_OFF + 8 * kKwKeys * 4;
-  static constexpr int N_BARS = 11;
-  static constexpr int ODD_OFF = BAR_OFF + N_BARS * 8 + 8;     // [2] whether a denominator of the step is NaN or infinite
-  static constexpr int TOTAL = ODD_OFF + 8;
+  static constexpr int N_BARS = 1 + 2 * STAGES + 4 * kKwBuffers;
+  static constexpr int ODD_OFF = BAR_OFF + N_BARS * 8 + 8;              // [4] whether a denominator of the step is NaN or infinite
+  static constexpr int TOTAL = ODD_OFF + 4 * kKwBuffers;
   static_assert(TOTAL <= 226 * 1024, "the block must fit on an SM");
 };
 
@@ -76,12 +79,12 @@ kept_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t base = smem_addr(smem);
   const int rank = (int)cluster_ctarank(), ranks = a.splits;
-  // clusters start in the order of their number: the first keys of all sequences and heads, whose walk is the longest, before the next
   const int G = a.heads / a.kv_heads, pairs = (int)(gridDim.y * gridDim.z);
   const int lin = (int)(blockIdx.x / ranks + gridDim.x / ranks * (blockIdx.y + gridDim.y * blockIdx.z));
   const int seq = (lin % pairs) / (int)gridDim.y, kh = (lin % pairs) % (int)gridDim.y, key0 = lin / pairs * kKwKeys;
   const uint32_t bars = base + L::BAR_OFF;
-  const uint32_t k_full = bars, q_full = bars + 8, d_full = bars + 24, s_full = bars + 40, s_free = bars + 56, d_free = bars + 72;
+  const uint32_t k_full = bars, q_full = bars + 8, q_free = q_full + 8 * L::STAGES, s_full = q_free + 8 * L::STAGES, s_free = s_full + 8 * kKwBuffers,
+                 d_full = s_free + 8 * kKwBuffers, d_free = d_full + 8 * kKwBuffers;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::BAR_OFF + L::N_BARS * 8);
   pdl_wait();
   const int count = a.counts[seq], past = a.past[seq], end = past + count;
@@ -95,16 +98,19 @@ kept_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   const int steps = all_steps > rank ? (all_steps - rank + ranks - 1) / ranks : 0;      // rank, rank + ranks, ...
   const bool aligned = (base & 1023u) == 0;
   float sum = 0.0f;
-  const int quad = warp & 3, part = (warp - 2) >> 2;      // lanes of tensor memory; 64 of a step's columns
+  const int quad = warp & 3, part = (warp - 3) >> 2;      // lanes of tensor memory; part = 2 * set + half of the columns
   if (all_steps > 0 && aligned) {
     if (tid == 0) {
       mbar_init(k_full, 1);
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < L::STAGES; ++i) {
         mbar_init(q_full + 8 * i, 1);
-        mbar_init(d_full + 8 * i, 32);
+        mbar_init(q_free + 8 * i, 1);
+      }
+      for (int i = 0; i < kKwBuffers; ++i) {
         mbar_init(s_full + 8 * i, 1);
-        mbar_init(s_free + 8 * i, 16);
-        mbar_init(d_free + 8 * i, 16);
+        mbar_init(s_free + 8 * i, 8);
+        mbar_init(d_full + 8 * i, 32);
+        mbar_init(d_free + 8 * i, 8);
       }
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -119,7 +125,6 @@ kept_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     const uint32_t tmem = *tmem_slot;
     if (warp == 0) {
       if (elect_one() && steps > 0) {
-        constexpr uint32_t idesc = instr_desc(kKwKeys, kKwRows);
         const int* table = a.block_table + (size_t)seq * a.table_stride;
         int pages[2] = {-1, -1};
         for (int i = 0; i < 2; ++i)
@@ -131,63 +136,74 @@ kept_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 #pragma unroll
             for (int h = 0; h < HD / 64; ++h)
               tma_load_2d(base + L::K_OFF + h * (kKwKeys * 128) + i * 8192, &map_k, h * 64, (pages[i] * a.kv_heads + kh) * 64, k_full);
-        auto load_queries = [&](int i) {
-          const int st = i & 1, token = t_lo + (rank + i * ranks) * (kKwRows / G);
+        for (int i = 0, st = 0, lap = 0; i < steps; ++i) {
+          if (lap > 0 && !mbar_wait(q_free + 8 * st, (lap - 1) & 1)) { atomicExch(w.status, 85); break; }
+          const int token = t_lo + (rank + i * ranks) * (kKwRows / G);
           mbar_expect_tx(q_full + 8 * st, L::Q_BYTES);
 #pragma unroll
           for (int h = 0; h < HD / 64; ++h)
             tma_load_3d(base + L::Q_OFF + st * L::Q_BYTES + h * (kKwRows * 128), &map_q, h * 64, kh * G, (int)tok0 + token, q_full + 8 * st);
-        };
-        load_queries(0);
+          if (++st == L::STAGES) { st = 0; ++lap; }
+        }
+      }
+    } else if (warp == 1) {
+      if (elect_one() && steps > 0) {
+        constexpr uint32_t idesc = instr_desc(kKwKeys, kKwRows);
         bool ok = mbar_wait(k_full, 0);
-        if (!ok) atomicExch(w.status, 85);
-        for (int i = 0; i < steps && ok; ++i) {
-          const int st = i & 1;
-          if (i + 1 < steps) {
-            // the other stage was read by the products of step i - 1
-            if (i >= 1 && !mbar_wait(s_full + 8 * (st ^ 1), ((i - 1) >> 1) & 1)) { atomicExch(w.status, 86); break; }
-            load_queries(i + 1);
-          }
-          if (!mbar_wait(q_full + 8 * st, (i >> 1) & 1)) { atomicExch(w.status, 87); break; }
-          if (i >= 2 && !mbar_wait(s_free + 8 * st, ((i >> 1) - 1) & 1)) { atomicExch(w.status, 88); break; }
+        if (!ok) atomicExch(w.status, 86);
+        for (int i = 0, st = 0, lap = 0; i < steps && ok; ++i) {
+          const int b = i % kKwBuffers;
+          if (!mbar_wait(q_full + 8 * st, lap & 1)) { atomicExch(w.status, 87); break; }
+          if (i >= kKwBuffers && !mbar_wait(s_free + 8 * b, (i / kKwBuffers - 1) & 1)) { atomicExch(w.status, 88); break; }
           tc_fence_after();
 #pragma unroll
           for (int h = 0; h < HD / 64; ++h) {
             const uint64_t dk = smem_desc(base + L::K_OFF + h * (kKwKeys * 128)), dq = smem_desc(base + L::Q_OFF + st * L::Q_BYTES + h * (kKwRows * 128));
 #pragma unroll
             for (int k4 = 0; k4 < 4; ++k4)
-              mma_bf16_ss(tmem + (uint32_t)(st * kKwRows), dk + (uint64_t)(k4 * 2), dq + (uint64_t)(k4 * 2), idesc, (h > 0 || k4 > 0) ? 1u : 0u);
+              mma_bf16_ss(tmem + (uint32_t)(b * kKwRows), dk + (uint64_t)(k4 * 2), dq + (uint64_t)(k4 * 2), idesc, (h > 0 || k4 > 0) ? 1u : 0u);
           }
-          mma_commit(s_full + 8 * st);
+          mma_commit(q_free + 8 * st);
+          mma_commit(s_full + 8 * b);
+          if (++st == L::STAGES) { st = 0; ++lap; }
         }
       }
-    } else if (warp == 1) {
+    } else if (warp == 2) {
       float* d = reinterpret_cast<float*>(smem + L::D_OFF);
-      for (int i = 0; i < steps; ++i) {
-        const int st = i & 1, R0 = row_lo + (rank + i * ranks) * kKwRows;
-        float v[8];
+      const int shift = 31 - __clz(G);      // (a divisor of 128)
+      float v[4], next[4];
+      auto ask = [&](int i, float (&x)[4]) {
+        const int R0 = row_lo + (rank + i * ranks) * kKwRows;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
+        for (int c = 0; c < 4; ++c) {
           const int R = R0 + c * 32 + lane;
-          v[c] = -INFINITY;
-          if (R < row_hi) v[c] = w.lse2[(tok0 + R / G) * a.heads + kh * G + R % G];
+          x[c] = -INFINITY;
+          if (i < steps && R < row_hi) x[c] = w.lse2[(tok0 + (R >> shift)) * a.heads + kh * G + (R & (G - 1))];
         }
-        if (i >= 2 && !mbar_wait(d_free + 8 * st, ((i >> 1) - 1) & 1)) {
+      };
+      ask(0, v);
+      for (int i = 0; i < steps; ++i) {
+        const int b = i % kKwBuffers;
+        ask(i + 1, next);
+        if (i >= kKwBuffers && !mbar_wait(d_free + 8 * b, (i / kKwBuffers - 1) & 1)) {
           if (lane == 0) atomicExch(w.status, 89);
           break;
         }
         bool odd = false;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) odd = odd || !(v[c] < INFINITY);
+        for (int c = 0; c < 4; ++c) odd = odd || !(v[c] < INFINITY);
         odd = __any_sync(0xffffffffu, odd);
-        if (lane == 0) reinterpret_cast<int*>(smem + L::ODD_OFF)[st] = odd;
+        if (lane == 0) reinterpret_cast<int*>(smem + L::ODD_OFF)[b] = odd;
         // the negative, to be added; a row without weight or behind the last gives none
 #pragma unroll
-        for (int c = 0; c < 8; ++c) d[st * kKwRows + c * 32 + lane] = v[c] == -INFINITY ? -INFINITY : -v[c];
-        mbar_arrive(d_full + 8 * st);
+        for (int c = 0; c < 4; ++c) {
+          d[b * kKwRows + c * 32 + lane] = v[c] == -INFINITY ? -INFINITY : -v[c];
+          v[c] = next[c];
+        }
+        mbar_arrive(d_full + 8 * b);
       }
     } else {
-      const int col0 = part * 64;
+      const int set = part >> 1, col0 = (part & 1) * 64;
       const int key = key0 + quad * 32 + lane;
       const float* d = reinterpret_cast<const float*>(smem + L::D_OFF);
       // rows that see this key: [see_lo, see_hi)
@@ -196,53 +212,46 @@ kept_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       bool ok = true;
       f32x2 s0 = 0, s1 = 0;
       const f32x2 scale2 = both(w.scale_log2);
-      for (int i = 0; i < steps; ++i) {
-        const int st = i & 1, R0 = row_lo + (rank + i * ranks) * kKwRows + col0;
-        if (ok && !(mbar_wait(s_full + 8 * st, (i >> 1) & 1) && mbar_wait(d_full + 8 * st, (i >> 1) & 1))) {
+      for (int i = set; i < steps; i += 2) {
+        const int b = i % kKwBuffers, R0 = row_lo + (rank + i * ranks) * kKwRows + col0;
+        if (ok && !(mbar_wait(s_full + 8 * b, (i / kKwBuffers) & 1) && mbar_wait(d_full + 8 * b, (i / kKwBuffers) & 1))) {
           ok = false;
           if (lane == 0) atomicExch(w.status, 90);
         }
         tc_fence_after();
         uint32_t sr[64];
 #pragma unroll
-        for (int c0 = 0; c0 < 64; c0 += 16) tmem_ld16_nowait(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(st * kKwRows + col0 + c0), sr + c0);
+        for (int c0 = 0; c0 < 64; c0 += 16) tmem_ld16_nowait(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(b * kKwRows + col0 + c0), sr + c0);
         tmem_wait_ld();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(s_free + 8 * st);      // the next product may overwrite the scores
+        if (lane == 0) mbar_arrive(s_free + 8 * b);      // the next product may overwrite the scores
         if (__any_sync(0xffffffffu, R0 < see_lo || R0 + 64 > see_hi)) {
 #pragma unroll
           for (int c = 0; c < 64; ++c)
             if (R0 + c < see_lo || R0 + c >= see_hi) sr[c] = 0xff800000u;
         }
-        const bool odd = reinterpret_cast<const int*>(smem + L::ODD_OFF)[st] != 0;
-        const ulonglong2* dd = reinterpret_cast<const ulonglong2*>(d + st * kKwRows + col0);
-        if (odd) {
+        const bool odd = reinterpret_cast<const int*>(smem + L::ODD_OFF)[b] != 0;
+        const ulonglong2* dd = reinterpret_cast<const ulonglong2*>(d + b * kKwRows + col0);
+        auto add_up = [&](auto both_pipes) {
 #pragma unroll
           for (int c = 0; c < 64; c += 4) {
             const ulonglong2 n = dd[c >> 2];
             const f32x2 x0 = fma2(pair_of(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), scale2, n.x);
             const f32x2 x1 = fma2(pair_of(__uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3])), scale2, n.y);
+            // three pairs of eight by the polynomial: 5 cycles a score on either pipe where the powers of two alone take 8
             s0 = add2(s0, pair_of(kw_ex2(low_half(x0)), kw_ex2(high_half(x0))));
-            s1 = add2(s1, pair_of(kw_ex2(low_half(x1)), kw_ex2(high_half(x1))));
+            s1 = add2(s1, (c >> 2) % 4 != 3 && decltype(both_pipes)::value ? kw_ex2_pair(x1) : pair_of(kw_ex2(low_half(x1)), kw_ex2(high_half(x1))));
           }
-        } else {
-#pragma unroll
-        for (int c = 0; c < 64; c += 4) {
-          const ulonglong2 n = dd[c >> 2];
-          const f32x2 x0 = fma2(pair_of(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), scale2, n.x);
-          const f32x2 x1 = fma2(pair_of(__uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3])), scale2, n.y);
-          // three pairs of eight by the polynomial: 5 cycles a score on either pipe where the powers of two alone take 8
-          s0 = add2(s0, pair_of(kw_ex2(low_half(x0)), kw_ex2(high_half(x0))));
-          s1 = add2(s1, (c >> 2) % 4 != 3 ? kw_ex2_pair(x1) : pair_of(kw_ex2(low_half(x1)), kw_ex2(high_half(x1))));
-        }
-        }
+        };
+        if (odd) add_up(std::false_type());
+        else add_up(std::true_type());
         __syncwarp();
-        if (lane == 0) mbar_arrive(d_free + 8 * st);
+        if (lane == 0) mbar_arrive(d_free + 8 * b);
       }
       sum = halves_sum(s0) + halves_sum(s1);
     }
-    if (warp >= 2) reinterpret_cast<float*>(smem + L::SUM_OFF)[part * kKwKeys + quad * 32 + lane] = sum;
+    if (warp >= 3) reinterpret_cast<float*>(smem + L::SUM_OFF)[part * kKwKeys + quad * 32 + lane] = sum;
     tc_fence_before();
     __syncthreads();
     if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
