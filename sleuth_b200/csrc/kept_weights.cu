@@ -60,7 +60,7 @@ __device__ __forceinline__ float kw_ex2(float x) {
 // infinite (any such score among the keys that they see makes it that) do not come here.
 __device__ __forceinline__ f32x2 kw_ex2_pair(f32x2 x) {
   x = pair_of(fmaxf(low_half(x), -126.0f), fmaxf(high_half(x), -126.0f));
-  const f32x2 t = add2(x, both(12582912.0f)), f = add2(x, mul2(add2(t, both(-12582912.0f)), both(-1.0f)));
+  const f32x2 t = add2(x, both(12582912.0f)), f = fma2(add2(t, both(-12582912.0f)), both(-1.0f), x);
   f32x2 p = fma2(f, both(0.0013276472454890609f), both(0.009675540961325169f));
   p = fma2(p, f, both(0.05550713092088699f));
   p = fma2(p, f, both(0.24022120237350464f));
@@ -219,33 +219,38 @@ kept_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           if (lane == 0) atomicExch(w.status, 90);
         }
         tc_fence_after();
-        uint32_t sr[64];
-#pragma unroll
-        for (int c0 = 0; c0 < 64; c0 += 16) tmem_ld16_nowait(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(b * kKwRows + col0 + c0), sr + c0);
-        tmem_wait_ld();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(s_free + 8 * b);      // the next product may overwrite the scores
-        if (__any_sync(0xffffffffu, R0 < see_lo || R0 + 64 > see_hi)) {
-#pragma unroll
-          for (int c = 0; c < 64; ++c)
-            if (R0 + c < see_lo || R0 + c >= see_hi) sr[c] = 0xff800000u;
-        }
+        const bool masked = __any_sync(0xffffffffu, R0 < see_lo || R0 + 64 > see_hi);
         const bool odd = reinterpret_cast<const int*>(smem + L::ODD_OFF)[b] != 0;
-        const ulonglong2* dd = reinterpret_cast<const ulonglong2*>(d + b * kKwRows + col0);
-        auto add_up = [&](auto both_pipes) {
+        // 32 columns at a time: with 64 in registers the polynomial's constants are loaded anew for every use
 #pragma unroll
-          for (int c = 0; c < 64; c += 4) {
-            const ulonglong2 n = dd[c >> 2];
-            const f32x2 x0 = fma2(pair_of(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), scale2, n.x);
-            const f32x2 x1 = fma2(pair_of(__uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3])), scale2, n.y);
-            // three pairs of eight by the polynomial: 5 cycles a score on either pipe where the powers of two alone take 8
-            s0 = add2(s0, pair_of(kw_ex2(low_half(x0)), kw_ex2(high_half(x0))));
-            s1 = add2(s1, (c >> 2) % 4 != 3 && decltype(both_pipes)::value ? kw_ex2_pair(x1) : pair_of(kw_ex2(low_half(x1)), kw_ex2(high_half(x1))));
+        for (int c0 = 0; c0 < 64; c0 += 32) {
+          uint32_t sr[32];
+          tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + (uint32_t)(b * kKwRows + col0 + c0), sr);
+          if (c0 == 32) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(s_free + 8 * b);      // the next product may overwrite the scores
           }
-        };
-        if (odd) add_up(std::false_type());
-        else add_up(std::true_type());
+          if (masked) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (R0 + c0 + c < see_lo || R0 + c0 + c >= see_hi) sr[c] = 0xff800000u;
+          }
+          const ulonglong2* dd = reinterpret_cast<const ulonglong2*>(d + b * kKwRows + col0 + c0);
+          auto add_up = [&](auto both_pipes) {
+#pragma unroll
+            for (int c = 0; c < 32; c += 4) {
+              const ulonglong2 n = dd[c >> 2];
+              const f32x2 x0 = fma2(pair_of(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), scale2, n.x);
+              const f32x2 x1 = fma2(pair_of(__uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3])), scale2, n.y);
+              // three pairs of eight by the polynomial: 5 cycles a score on either pipe where the powers of two alone take 8
+              s0 = add2(s0, pair_of(kw_ex2(low_half(x0)), kw_ex2(high_half(x0))));
+              s1 = add2(s1, (c >> 2) % 4 != 3 && decltype(both_pipes)::value ? kw_ex2_pair(x1) : pair_of(kw_ex2(low_half(x1)), kw_ex2(high_half(x1))));
+            }
+          };
+          if (odd) add_up(std::false_type());
+          else add_up(std::true_type());
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive(d_free + 8 * b);
       }
