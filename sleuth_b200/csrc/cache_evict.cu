@@ -275,21 +275,26 @@ __global__ void __launch_bounds__(kEvictThreads) cache_evict_kernel(EvictArgs a)
     const uint32_t k = key_of(j);
     const bool stays = k > last || (k == last && tie < need);
     tie += k == last;
-    if (j < left) {
-      if (stays) {
-        if (positions_out != positions || j >= past) positions_out[j] = position(j);
-        if (weights_out != weights) weights_out[j] = weights[j];
-      } else {
-        lists[1 + hole] = j;
-        ++hole;
-      }
-    } else if (stays) {
-      lists[1 + a.most_moves + mover] = j;
-      ++mover;
+    if (j < left && !stays) lists[1 + hole++] = j;
+    if (j >= left && stays) lists[1 + a.most_moves + mover++] = j;
+    if (a.keys_fit) keys[j] = stays;      // (a row of this thread's own run)
+    else if (j < left && stays) {
+      if (positions_out != positions || j >= past) positions_out[j] = position(j);
+      if (weights_out != weights) weights_out[j] = weights[j];
     }
   }
   if (tid == 0) lists[0] = moves;
   __syncthreads();
+  // what stays in its place, a warp whole lines (in the loop above each copy would wait for the one before)
+  if (a.keys_fit && (positions_out != positions || weights_out != weights || past < left))
+#pragma unroll 4
+    for (int j = tid; j < left; j += kEvictThreads) {
+      if (!keys[j]) continue;
+      const float w = weights[j];
+      const int p = position(j);
+      if (positions_out != positions || j >= past) positions_out[j] = p;
+      if (weights_out != weights) weights_out[j] = w;
+    }
   for (int i = tid; i < moves; i += kEvictThreads) {      // (the block's own stores are visible to it after the barrier)
     const int to = lists[1 + i], from = lists[1 + a.most_moves + i];
     weights_out[to] = weights[from];

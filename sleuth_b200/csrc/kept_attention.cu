@@ -19,7 +19,7 @@
 
 namespace slb {
 
-constexpr int kGenThreads = 256, kGenRows = 16, kGenKeys = 64;
+constexpr int kGenThreads = 256, kGenRows = 16, kGenKeys = 64, kGenWeightRows = 64;
 
 __host__ __device__ constexpr int padded_dim(int hd) { return (hd + 3) & ~3; }
 
@@ -60,11 +60,11 @@ __device__ __forceinline__ void load_rows(float* dst, const T* pool, const KeptA
   }
 }
 
-// 16 rows of queries, times scale * log2(e), zeros behind the last row.
-template <typename T>
+// ROWS rows of queries, times the scale, zeros behind the last row.
+template <typename T, int ROWS>
 __device__ __forceinline__ void load_queries(float* dst, const KeptArgs& a, size_t token0, int kh, int G, int r0, int rows_total) {
   const int hd = a.head_dim, hdp = padded_dim(hd);
-  for (int e = threadIdx.x; e < kGenRows * hdp; e += kGenThreads) {
+  for (int e = threadIdx.x; e < ROWS * hdp; e += kGenThreads) {
     const int r = e / hdp, c = e - r * hdp, R = r0 + r;
     float v = 0.0f;
     if (R < rows_total && c < hd) v = to_f32(((const T*)a.q)[((token0 + R / G) * a.heads + kh * G + R % G) * hd + c]) * a.scale;
@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(kGenThreads) kept_general_kernel(KeptArgs a, l
   const int steps = (run.total + kGenKeys - 1) / kGenKeys, per = (steps + a.splits - 1) / a.splits;
   const int v_begin = split * per * kGenKeys, v_end = min(run.total, v_begin + per * kGenKeys);
 
-  load_queries<T>(q_s, a, token0, kh, G, r0, rows_total);
+  load_queries<T, kGenRows>(q_s, a, token0, kh, G, r0, rows_total);
   const int key_i = tid & 63, rg = tid >> 6;             // scores: a key, rows 4 rg .. 4 rg + 3
   int row_pos[4], row_lo[4];
 #pragma unroll
@@ -241,7 +241,7 @@ __global__ void kept_join_kernel(KeptArgs a, long long tokens) {
   if (c == 0 && a.lse) a.lse[token * a.heads + head] = L == 0.0f ? -INFINITY : M + logf(L);
 }
 
-__host__ __device__ constexpr int weights_smem(int hd) { return (kGenKeys * (padded_dim(hd) + 4) + kGenRows * padded_dim(hd) + kGenRows + kGenThreads) * 4; }
+__host__ __device__ constexpr int weights_smem(int hd) { return (kGenKeys * (padded_dim(hd) + 4) + kGenWeightRows * (padded_dim(hd) + 1) + kGenThreads) * 4; }
 
 template <typename T>
 __global__ void __launch_bounds__(kGenThreads) kept_weights_general_kernel(KeptArgs a) {
@@ -249,9 +249,9 @@ __global__ void __launch_bounds__(kGenThreads) kept_weights_general_kernel(KeptA
   extern __shared__ __align__(16) float smem[];
   const int hd = a.head_dim, hdp = padded_dim(hd);
   float* rows_s = smem;                                  // [64][hdp + 4]
-  float* q_s = rows_s + kGenKeys * (hdp + 4);            // [16][hdp]
-  float* lse_s = q_s + kGenRows * hdp;                   // [16]
-  float* part_s = lse_s + kGenRows;                      // [4][64]
+  float* q_s = rows_s + kGenKeys * (hdp + 4);            // [64][hdp]
+  float* lse_s = q_s + kGenWeightRows * hdp;             // [64]
+  float* part_s = lse_s + kGenWeightRows;                // [4][64]
   const int tid = threadIdx.x, key_i = tid & 63, rg = tid >> 6;
   const int seq = blockIdx.z, kh = blockIdx.y, G = a.heads / a.kv_heads;
   const int count = a.counts[seq], past = a.past[seq], end = past + count;
@@ -269,21 +269,24 @@ __global__ void __launch_bounds__(kGenThreads) kept_weights_general_kernel(KeptA
     run.lo = key0;       // 64 keys as they lie
     load_rows<T>(rows_s, (const T*)a.k_pool, a, table, kh, run, 0, last - key0 + 1);
     const int r_hi = (t_hi + 1) * G;
-    for (int r0 = t_lo * G; r0 < r_hi; r0 += kGenRows) {
+    for (int r0 = t_lo * G; r0 < r_hi; r0 += kGenWeightRows) {
       __syncthreads();
-      load_queries<T>(q_s, a, token0, kh, G, r0, r_hi);
-      if (tid < kGenRows) {
+      load_queries<T, kGenWeightRows>(q_s, a, token0, kh, G, r0, r_hi);
+      if (tid < kGenWeightRows) {
         const int R = r0 + tid;
-        lse_s[tid] = R < r_hi ? a.lse[(token0 + R / G) * a.heads + kh * G + R % G] : 0.0f;
+        lse_s[tid] = R < r_hi ? a.lse[(token0 + R / G) * a.heads + kh * G + R % G] : -INFINITY;
       }
       __syncthreads();
-      float s[4];
-      dots(rows_s + key_i * (hdp + 4), q_s + 4 * rg * hdp, hdp, s);
+      const int n = min(kGenWeightRows, r_hi - r0);
+      for (int q0 = 4 * rg; q0 < n; q0 += 16) {      // a thread's group of four rows, then the next but three
+        float s[4];
+        dots(rows_s + key_i * (hdp + 4), q_s + q0 * hdp, hdp, s);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int R = r0 + 4 * rg + i, pos = R < r_hi ? past + R / G : -1;
-        const float d = lse_s[4 * rg + i];
-        if (sees(key, pos, window_lo(pos, a.window), a.first) && d != -INFINITY) sum += expf(s[i] - d);
+        for (int i = 0; i < 4; ++i) {
+          const int R = r0 + q0 + i, pos = R < r_hi ? past + R / G : -1;
+          const float d = lse_s[q0 + i];
+          if (sees(key, pos, window_lo(pos, a.window), a.first) && d != -INFINITY) sum += expf(s[i] - d);
+        }
       }
     }
   }
@@ -330,11 +333,12 @@ static int general_weights(const KeptArgs& a, int max_keys, cudaStream_t s) {
   return check_launch("attention_kept (weights, general kernel)");
 }
 
-// Shares of the keys: as many as give every SM about four blocks, of at least four steps of 64 keys each.
+// Shares of the keys: as many as give every SM about four blocks, of at least one step of 64 keys (a step takes a block 3 us, a share more takes
+// the joining kernel 0.1: five sequences of 33 to 700 rows in shares of 256 keys 20 us).
 static int general_splits(int n_seqs, int max_count, int heads, int kv_heads, int max_keys) {
   const long long tiles = ((long long)max_count * (heads / kv_heads) + kGenRows - 1) / kGenRows * kv_heads * n_seqs;
   long long splits = 4ll * sm_count() / (tiles > 0 ? tiles : 1);
-  const long long most = (max_keys + 4 * kGenKeys - 1) / (4 * kGenKeys);
+  const long long most = (max_keys + kGenKeys - 1) / kGenKeys;
   splits = splits < most ? splits : most;
   return splits < 1 ? 1 : splits > 64 ? 64 : (int)splits;
 }

@@ -434,7 +434,7 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 // Joins the shares of what no block finished alone, and turns scores into weights: of the blocks of a (sequence, kv head) the first few take
 // outputs, the others `keys_a_block` keys each.
 template <int HD, int R>
-__global__ void __launch_bounds__(256) kept_few_finish_kernel(FewArgs fa) {
+__global__ void __launch_bounds__(256, 4) kept_few_finish_kernel(FewArgs fa) {
   pdl_wait();
   const KeptArgs& a = fa.k;
   constexpr int ROWS = 16 * R;
@@ -528,44 +528,54 @@ __global__ void __launch_bounds__(256) kept_few_finish_kernel(FewArgs fa) {
   __syncthreads();
   const size_t at0 = ((size_t)(a.slots ? a.slots[seq] : seq) * a.kv_heads + kh) * a.capacity;
   const int key_end = (int)min((long long)min(end, key_begin + fa.keys_a_block), a.capacity);
-  // four keys a thread, four groups of threads for the rows r = group, group + 4, ...; the groups' sums are added in their order
-  const int quad = tid & 63, group = tid >> 6;
-  for (int key0 = key_begin; key0 < key_end; key0 += 256) {
+  // Four keys a thread. Up to eight rows a thread takes them all, their loads under way together; with more, four groups of threads take the rows
+  // r = group, group + 4, ..., and the groups' sums are added in their order.
+  const bool alone = rows_total <= 8;
+  const int quads = alone ? 256 : 64, quad = tid & (quads - 1), group = alone ? 0 : tid >> 6, step = alone ? 1 : 4;
+  for (int key0 = key_begin; key0 < key_end; key0 += 4 * quads) {
     const int key = key0 + 4 * quad;
     float4 gained = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (key < key_end) {
-      for (int r0 = group; r0 < rows_total; r0 += 16) {
-        float4 v[4];
+    float before[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = r0 + 4 * i;
+    for (int i = 0; i < 4; ++i) before[i] = alone && key + i < min(past, key_end) ? a.weights[at0 + key + i] : 0.0f;
+    if (key < key_end) {
+      for (int r0 = group; r0 < rows_total; r0 += 8 * step) {
+        float4 v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = r0 + i * step;
           v[i] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
           if (r >= rows_total) continue;
           const int pos = pos_s[r], lo = window_lo(pos, a.window);
-          const bool s0 = sees(key, pos, lo, a.first), s1 = sees(key + 1, pos, lo, a.first), s2 = sees(key + 2, pos, lo, a.first), s3 = sees(key + 3, pos, lo, a.first);
-          if (s0 || s1 || s2 || s3) {
-            const float4 x = *reinterpret_cast<const float4*>(fa.scores + row_s[r] + key);
-            if (s0) v[i].x = x.x;
-            if (s1) v[i].y = x.y;
-            if (s2) v[i].z = x.z;
-            if (s3) v[i].w = x.w;
-          }
+          if (key > pos || (key + 3 < lo && key >= a.first)) continue;
+          v[i] = *reinterpret_cast<const float4*>(fa.scores + row_s[r] + key);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (r0 + 4 * i >= rows_total) continue;
-          const float d = lse_s[r0 + 4 * i];
-          gained.x += few_ex2(v[i].x - d); gained.y += few_ex2(v[i].y - d);
-          gained.z += few_ex2(v[i].z - d); gained.w += few_ex2(v[i].w - d);
+        for (int i = 0; i < 8; ++i) {
+          const int r = r0 + i * step;
+          if (r >= rows_total) continue;
+          const int pos = pos_s[r], lo = window_lo(pos, a.window);
+          const float d = lse_s[r];
+          gained.x += sees(key, pos, lo, a.first) ? few_ex2(v[i].x - d) : 0.0f;
+          gained.y += sees(key + 1, pos, lo, a.first) ? few_ex2(v[i].y - d) : 0.0f;
+          gained.z += sees(key + 2, pos, lo, a.first) ? few_ex2(v[i].z - d) : 0.0f;
+          gained.w += sees(key + 3, pos, lo, a.first) ? few_ex2(v[i].w - d) : 0.0f;
         }
       }
+    }
+    if (alone) {
+      const float sum[4] = {before[0] + gained.x, before[1] + gained.y, before[2] + gained.z, before[3] + gained.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (key + i < key_end) a.weights_out[at0 + key + i] = sum[i];
+      continue;
     }
     __syncthreads();
     *reinterpret_cast<float4*>(&sum_s[group][4 * quad]) = gained;
     __syncthreads();
     if (key0 + tid < key_end) {
-      const float before = key0 + tid < past ? a.weights[at0 + key0 + tid] : 0.0f;
-      a.weights_out[at0 + key0 + tid] = before + ((sum_s[0][tid] + sum_s[1][tid]) + (sum_s[2][tid] + sum_s[3][tid]));
+      const float w = key0 + tid < past ? a.weights[at0 + key0 + tid] : 0.0f;
+      a.weights_out[at0 + key0 + tid] = w + ((sum_s[0][tid] + sum_s[1][tid]) + (sum_s[2][tid] + sum_s[3][tid]));
     }
   }
 }
