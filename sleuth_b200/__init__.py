@@ -8,6 +8,7 @@ Importing the package needs no GPU; loading a model does.
 """
 
 from .config import ConfigError, Qwen3Config, parse_config, register_architecture
+from .cache.keep import KeepPolicy
 from .sampling.config import SamplingConfig
 
 __version__ = "0.1.0"
@@ -28,5 +29,5 @@ def write_random_model(*args, **kwargs):
     return _w(*args, **kwargs)
 
 
-__all__ = ["ConfigError", "Qwen3Config", "parse_config", "register_architecture", "SamplingConfig", "load",
+__all__ = ["ConfigError", "Qwen3Config", "parse_config", "register_architecture", "KeepPolicy", "SamplingConfig", "load",
            "generate", "write_random_model", "__version__"]

@@ -13,6 +13,11 @@ kept here.
   long the sequence grows. Positions still map to table entries the same way. Windows are signed numbers: w > 0 means the
   w most recent positions, w < 0 chunks of -w positions counted from position 0 (a query sees its own chunk only), 0 every
   earlier position (``first_visible``; csrc/common.cuh first_key is the same rule for the kernels).
+* A windowed group may keep the first ``first`` positions beside its window (``cache/keep.py``): the pages that hold them are never given
+  back before the sequence ends.
+* Under a ``budget`` a sequence holds at most so many rows after a step (which ones, the device decides for each layer and key/value head:
+  csrc/cache_evict.cu); rows are then no longer positions, and ``seen[slot]`` counts the tokens that went through. Without a budget
+  ``seen`` equals ``lengths``.
 * ``lengths[slot]`` is the number of tokens the sequence holds. Stale contents of a reused page are
   never read: every kernel reads positions below the length only (the reference relies on the same
   idea: entries past ``pos`` are simply overwritten, sleuth/forge/infer/kv_cache.py:52-64).
@@ -89,7 +94,8 @@ class GroupBook:
     window: int                 # signed, see above; 0 = keep every position
     pool: PagePool
     table: np.ndarray           # [max_slots, stride] int32, -1 = no page
-    first_page: np.ndarray      # [max_slots] index of the first table entry still held
+    first_page: np.ndarray      # [max_slots] index of the first table entry still held (behind the kept ones, if something was given back)
+    kept: int = 0               # pages of the first positions, which stay
 
 
 class CacheBook:
@@ -99,15 +105,18 @@ class CacheBook:
     stride: entries per block-table row = pages of the longest sequence allowed.
     """
 
-    def __init__(self, windows: list[int], n_pages: int, max_slots: int, stride: int):
+    def __init__(self, windows: list[int], n_pages: int, max_slots: int, stride: int, firsts: list[int] | None = None, budget: int = 0):
         self.max_slots = max_slots
         self.stride = stride
         self.max_len = stride * PAGE_TOKENS
         self.lengths = np.zeros(max_slots, dtype=np.int32)
+        self.seen = np.zeros(max_slots, dtype=np.int32)
+        self.budget = int(budget)
         self._free_slots = list(range(max_slots - 1, -1, -1))
         self._live = np.zeros(max_slots, dtype=bool)
         self.groups = [GroupBook(w, PagePool(n_pages), np.full((max_slots, stride), -1, dtype=np.int32),
-                                 np.zeros(max_slots, dtype=np.int64)) for w in windows]
+                                 np.zeros(max_slots, dtype=np.int64), pages_for(f) if w else 0)
+                       for w, f in zip(windows, firsts or [0] * len(windows))]
 
     # ---- slots ----
     @property
@@ -123,7 +132,7 @@ class CacheBook:
         slots = [self._free_slots.pop() for _ in range(n)]
         for s in slots:
             self._live[s] = True
-            self.lengths[s] = 0
+            self.lengths[s] = self.seen[s] = 0
             for g in self.groups:
                 g.first_page[s] = 0
         return slots
@@ -136,7 +145,7 @@ class CacheBook:
                 held = row[row >= 0]
                 g.pool.give(held.tolist())
                 row[:] = -1
-            self.lengths[s] = 0
+            self.lengths[s] = self.seen[s] = 0
             self._live[s] = False
             self._free_slots.append(s)
 
@@ -152,7 +161,7 @@ class CacheBook:
             for gi, g in enumerate(self.groups):
                 have = int((g.table[s] >= 0).sum())
                 lo = int(g.first_page[s])
-                need[gi] += max(0, pages_for(n) - lo - have)
+                need[gi] += max(0, pages_for(n) - lo + (g.kept if lo else 0) - have)
         return need
 
     def peak_pages_needed(self, chunks) -> list[int]:
@@ -170,18 +179,24 @@ class CacheBook:
                     if s not in first:
                         first[s] = int(g.first_page[s])
                         have[s] = int((g.table[s] >= 0).sum())
-                    take = max(0, pages_for(n) - first[s] - have[s])
+                    take = max(0, pages_for(n) - first[s] + (g.kept if first[s] else 0) - have[s])
                     have[s] += take
                     out += take
                 peak = max(peak, out)
                 if g.window:
                     for s, n in zip(slots, new_lengths):
                         keep_from = first_visible(n, g.window) // PAGE_TOKENS
-                        if keep_from > first[s]:
-                            back = min(have[s], keep_from - first[s])
+                        lo = max(first[s], g.kept)
+                        if keep_from > lo:
+                            back = min(have[s], keep_from - lo)
                             have[s] -= back
                             out -= back
                             first[s] = keep_from
+                if self.budget:
+                    for s, n in zip(slots, new_lengths):
+                        back = max(0, have[s] - pages_for(min(n, self.budget)))
+                        have[s] -= back
+                        out -= back
             peaks.append(peak)
         return peaks
 
@@ -208,12 +223,20 @@ class CacheBook:
     def commit(self, slots, new_lengths) -> None:
         """The step has been issued: set the lengths and let windowed groups give pages back."""
         for s, n in zip(slots, new_lengths):
+            self.seen[s] += n - int(self.lengths[s])
+            if self.budget and n > self.budget:
+                n = self.budget
+                for g in self.groups:
+                    row = g.table[s]
+                    behind = row[pages_for(n):]
+                    g.pool.give(behind[behind >= 0].tolist())
+                    behind[:] = -1
             self.lengths[s] = n
             for g in self.groups:
                 if g.window:
                     # the next query sits at position >= n; what it sees never begins earlier for later ones
                     keep_from = first_visible(n, g.window) // PAGE_TOKENS
-                    lo = int(g.first_page[s])
+                    lo = max(int(g.first_page[s]), g.kept)
                     if keep_from > lo:
                         row = g.table[s]
                         g.pool.give(row[lo:keep_from].tolist())

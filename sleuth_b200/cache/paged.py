@@ -43,6 +43,7 @@ class KVRequest:
     head_dim: int
     window: int = 0
     value_dim: int = 0          # width of a value row when it is not head_dim (0 = head_dim)
+    first: int = 0              # first positions that stay visible beside a window (cache/keep.py)
 
 
 @dataclass(frozen=True)
@@ -102,8 +103,8 @@ class PagedCache:
     DEFAULT_SEQUENCES_WITH_STATE = 256
 
     def __init__(self, requests: list, max_tokens: int, max_seq_len: int, dtype: torch.dtype, device,
-                 max_sequences: int | None = None):
-        """max_tokens: tokens all live sequences may hold together (pages of 64). max_sequences: how many
+                 max_sequences: int | None = None, budget: int = 0):
+        """budget: rows that a sequence keeps after a step (0: all; see cache/keep.py). max_tokens: tokens all live sequences may hold together (pages of 64). max_sequences: how many
         sequences may be live at once (slots). Default: one per page, the most that can ever hold a token, unless
         some entry keeps a per-sequence state, which is allocated for every slot: then 256 at most."""
         self.dtype = dtype
@@ -149,7 +150,7 @@ class PagedCache:
             else:
                 raise TypeError(f"cache entry {e}: unknown request {r!r}")
         self.group_requests = keys
-        self.book = CacheBook([k.window for k in keys], self.n_pages, self.max_slots, self.stride)
+        self.book = CacheBook([k.window for k in keys], self.n_pages, self.max_slots, self.stride, [getattr(k, "first", 0) for k in keys], budget)
         self.pools = [torch.zeros(self._pool_shape(k, len(m)), dtype=dtype, device=self.device) for k, m in zip(keys, members)]
         self.states = {e: torch.zeros((self.max_slots, *r.shape), dtype=r.dtype, device=self.device)
                        for e, r in enumerate(self.requests) if isinstance(r, StateRequest)}

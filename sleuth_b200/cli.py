@@ -66,6 +66,12 @@ def build_parser() -> argparse.ArgumentParser:
     s.add_argument("--stop-id", type=int, action="append", default=None,
                    help="stop at this token id (repeatable; default: eos_token_id of config.json)")
     s.add_argument("--max-seq-len", type=int, default=4096, help="longest sequence, prompt plus new tokens")
+    s.add_argument("--keep-window", type=int, default=0, metavar="N",
+                   help="the cache keeps the latest N tokens and the first ones (see --keep-first); 0 = everything")
+    s.add_argument("--keep-budget", type=int, default=0, metavar="N",
+                   help="the cache keeps N tokens for each key/value head: the first, the latest, and those that were looked at most")
+    s.add_argument("--keep-first", type=int, default=4, metavar="N", help="first tokens that stay (default 4)")
+    s.add_argument("--keep-recent", type=int, default=None, metavar="N", help="latest tokens that stay under a budget (default: half of it)")
     s.set_defaults(fn=cmd_generate)
 
     r = sub.add_parser("replay", help="feed token traces through a model and write logits (see bin/trace_run)")
@@ -105,8 +111,13 @@ def cmd_generate(a) -> int:
               "this library goes from tokens to tokens and ships no tokenizer", file=sys.stderr)
         return 2
     device = "cuda:0" if a.device == "auto" else a.device
+    keep = None
+    if a.keep_window or a.keep_budget:
+        from .cache.keep import KeepPolicy
+        keep = KeepPolicy(budget=a.keep_budget, window=a.keep_window, first=a.keep_first, recent=a.keep_recent)
+    per_prompt = min(a.max_seq_len, keep.most_rows) if keep is not None and keep.budget else a.max_seq_len
     engine = load(a.path, dtype=_dtype_name(a.dtype), max_seq_len=a.max_seq_len, device=device,
-                  max_tokens=max(1, len(prompts)) * a.max_seq_len)
+                  max_tokens=max(1, len(prompts)) * (-(-per_prompt // 64) * 64 if keep is not None else per_prompt), keep=keep)
     sampling = SamplingConfig(a.temperature, a.top_k, a.top_p, a.min_p, a.repetition_penalty, a.repeat_last_n,
                               a.no_repeat_ngram)
     n_params = sum(int(torch.tensor(d.shape).prod()) for d in engine.model.expected().values())

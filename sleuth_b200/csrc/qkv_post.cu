@@ -28,6 +28,7 @@ struct QkvPostArgs {
   void* v_pool;
   const int* tok_seq;       // [tokens]
   const int* tok_pos;       // [tokens]
+  const int* tok_rot;       // [tokens] the position by which a token is rotated, when tok_pos is its row of the cache only
   const int* block_table;   // [seqs, table_stride]
   int table_stride;
   int tokens, heads, kv_heads, head_dim, rot_dim;
@@ -89,7 +90,7 @@ __global__ void qkv_post_kernel(QkvPostArgs a) {
         if (c < hd) stage[c] = v[i];
       }
       __syncwarp();
-      const int pos = a.tok_pos[t];
+      const int pos = a.tok_rot[t];
       const float* cs = a.cos_table + (size_t)pos * half;
       const float* sn = a.sin_table + (size_t)pos * half;
 #pragma unroll
@@ -167,8 +168,9 @@ __global__ void qkv_post_vec_kernel(QkvPostArgs a) {
       for (int e = 0; e < EPL; ++e) v[e] = (v[e] * inv) * gain[c0 + e];
     }
     if (a.cos_table) {
-      const float* cs = a.cos_table + (size_t)pos * (HD / 2) + (lane & 15) * EPL;
-      const float* sn = a.sin_table + (size_t)pos * (HD / 2) + (lane & 15) * EPL;
+      const int turn = a.tok_rot[t];
+      const float* cs = a.cos_table + (size_t)turn * (HD / 2) + (lane & 15) * EPL;
+      const float* sn = a.sin_table + (size_t)turn * (HD / 2) + (lane & 15) * EPL;
 #pragma unroll
       for (int e = 0; e < EPL; ++e) {
         const float partner = __shfl_xor_sync(0xffffffffu, v[e], 16);
@@ -482,11 +484,12 @@ __global__ void __launch_bounds__(256) qkv_post_span_quad_kernel(QkvSpanArgs a) 
 
 using namespace slb;
 
-extern "C" int slb_qkv_post(const void* qkv, const float* bias, const float* q_gain, const float* k_gain,
-                            const float* cos_table, const float* sin_table, void* q_out, void* k_pool, void* v_pool,
-                            const int* tok_seq, const int* tok_pos, const int* block_table, int table_stride,
-                            int tokens, int heads, int kv_heads, int head_dim, int rot_dim, float eps, int dtype,
-                            void* stream) {
+// As slb_qkv_post below; tok_pos gives a token's row of the cache, tok_rot the position by which its query and key are rotated.
+extern "C" int slb_qkv_post_rows(const void* qkv, const float* bias, const float* q_gain, const float* k_gain,
+                                 const float* cos_table, const float* sin_table, void* q_out, void* k_pool, void* v_pool,
+                                 const int* tok_seq, const int* tok_pos, const int* tok_rot, const int* block_table, int table_stride,
+                                 int tokens, int heads, int kv_heads, int head_dim, int rot_dim, float eps, int dtype,
+                                 void* stream) {
   SLB_REQUIRE(tokens >= 0 && heads > 0 && kv_heads >= 0, "qkv_post: tokens=%d heads=%d kv_heads=%d", tokens, heads,
               kv_heads);
   SLB_REQUIRE(head_dim > 0 && head_dim <= 256 && head_dim % 2 == 0,
@@ -501,13 +504,22 @@ extern "C" int slb_qkv_post(const void* qkv, const float* bias, const float* q_g
   a.qkv = qkv; a.bias = bias; a.q_gain = q_gain; a.k_gain = k_gain;
   a.cos_table = rot_dim > 0 ? cos_table : nullptr; a.sin_table = sin_table;
   a.q_out = q_out; a.k_pool = k_pool; a.v_pool = v_pool;
-  a.tok_seq = tok_seq; a.tok_pos = tok_pos; a.block_table = block_table; a.table_stride = table_stride;
+  a.tok_seq = tok_seq; a.tok_pos = tok_pos; a.tok_rot = tok_rot; a.block_table = block_table; a.table_stride = table_stride;
   a.tokens = tokens; a.heads = heads; a.kv_heads = kv_heads; a.head_dim = head_dim; a.rot_dim = rot_dim;
   a.eps = eps;
   cudaStream_t s = (cudaStream_t)stream;
   if (dtype == kF32) return launch_qkv_post<float>(a, s);
   if (dtype == kBF16) return launch_qkv_post<__nv_bfloat16>(a, s);
   return fail(1, "qkv_post: unknown dtype %d", dtype);
+}
+
+extern "C" int slb_qkv_post(const void* qkv, const float* bias, const float* q_gain, const float* k_gain,
+                            const float* cos_table, const float* sin_table, void* q_out, void* k_pool, void* v_pool,
+                            const int* tok_seq, const int* tok_pos, const int* block_table, int table_stride,
+                            int tokens, int heads, int kv_heads, int head_dim, int rot_dim, float eps, int dtype,
+                            void* stream) {
+  return slb_qkv_post_rows(qkv, bias, q_gain, k_gain, cos_table, sin_table, q_out, k_pool, v_pool, tok_seq, tok_pos, tok_pos, block_table,
+                           table_stride, tokens, heads, kv_heads, head_dim, rot_dim, eps, dtype, stream);
 }
 
 extern "C" int slb_qkv_post_span(const float* qkv, long long row_stride, const float* bias, const float* q_gain, const float* k_gain, const float* cos_table,

@@ -7,6 +7,8 @@ A step runs ``n`` sequences with ``counts[i]`` new tokens each (unequal), append
   (its absolute position), ``seq_start[n + 1]``, ``past[n]``, ``counts[n]``, ``slots[n]``
 * ``rows[W]``: the token rows whose logits are wanted
 * per cache group a block table ``[n, stride]``
+* under a budget (cache/keep.py), where ``tok_pos``, ``past`` and ``counts`` speak of rows of the cache: ``tok_rot[T]`` (the tokens' positions in
+  their texts, by which they are rotated), ``lengths[n]`` (rows after the step, before its eviction), ``seen[n]`` (tokens of the text so far)
 
 All of it is packed into one pinned host buffer and sent with one copy. The host buffers form a
 ring guarded by events, because a copy from pinned memory reads the buffer when it executes, not
@@ -49,6 +51,9 @@ class StepBatch:
     # the weight matrix that is read right after the part now running has finished (the next part's first product),
     # or None: the last kernel of a part may ask the L2 cache for it
     next_read: torch.Tensor | None = None
+    tok_rot: torch.Tensor | None = None
+    lengths: torch.Tensor | None = None
+    seen: torch.Tensor | None = None
 
 
 def _round(n: int) -> int:
@@ -61,8 +66,10 @@ class MetaStager:
     RING = 4
     FEED = 1024      # int32 slots at the start of the buffer where decode steps find their tokens
 
-    def __init__(self, device, n_groups: int, stride: int, capacity: int = 1 << 16):
+    def __init__(self, device, n_groups: int, stride: int, capacity: int = 1 << 16, rows_apart: bool = False):
+        """rows_apart: rows of the cache are not the tokens' positions (a budget), so both go up."""
         self.device = torch.device(device)
+        self.rows_apart = rows_apart
         self.n_groups, self.stride = n_groups, stride
         self.cap = 0
         self.dev = None
@@ -95,7 +102,8 @@ class MetaStager:
         """Offsets (in int32 elements) of every region for a batch of these sizes."""
         off, o = {}, self.FEED
         for name, size in (("token_ids", T), ("tok_seq", T), ("tok_pos", T), ("seq_start", n + 1), ("past", n),
-                           ("counts", n), ("slots", n), ("rows", W), ("floats", n_floats), ("ids_map", n)):
+                           ("counts", n), ("slots", n), ("rows", W), ("floats", n_floats), ("ids_map", n),
+                           *((("tok_rot", T), ("lengths", n), ("seen", n)) if self.rows_apart else ())):
             off[name] = (o, size)
             o += _round(max(size, 1))
         for g in range(self.n_groups):
@@ -117,7 +125,8 @@ class MetaStager:
             view = {name: self.dev[o:o + size] for name, (o, size) in off.items()}
             fixed = dict(token_ids=self.feed if via_feed else view["token_ids"], ids_map=view["ids_map"] if via_feed else None,
                          floats=view["floats"].view(torch.float32) if nf else None,
-                         **{name: view[name] for name in ("tok_seq", "tok_pos", "seq_start", "past", "counts", "slots", "rows")})
+                         **{name: view[name] for name in ("tok_seq", "tok_pos", "seq_start", "past", "counts", "slots", "rows",
+                                                          *(("tok_rot", "lengths", "seen") if self.rows_apart else ()))})
             tables = [view[f"table{g}"].view(n, self.stride) for g in range(self.n_groups)]
             copies = {first: (self.dev[first:total], [h[first:total] for h in self.hosts]) for first in (0, self.FEED)}
             plan = self._plans[key] = (off, total, fixed, tables, copies)
@@ -131,7 +140,7 @@ class MetaStager:
 
     def upload(self, slots, pasts, counts, tokens: np.ndarray | None, rows: np.ndarray, tables: list[np.ndarray],
                floats: np.ndarray | None = None, stream: torch.cuda.Stream | None = None,
-               feed_map: np.ndarray | None = None) -> StepBatch:
+               feed_map: np.ndarray | None = None, seen=None) -> StepBatch:
         """tokens: this step's token ids from the host. For a decode step (one token per sequence, at most FEED
         sequences) they go to the feed region; with ``tokens=None`` the feed is left as the sampler filled it and
         ``feed_map[i]`` says which feed slot holds sequence i's token."""
@@ -174,6 +183,11 @@ class MetaStager:
         put("past", pasts_a)
         put("counts", counts_a)
         put("slots", np.asarray(slots, dtype=np.int32))
+        if self.rows_apart:
+            seen_a = np.asarray(seen, dtype=np.int32)
+            put("tok_rot", pos_of + (seen_a - pasts_a)[seq_of])
+            put("lengths", pasts_a + counts_a)
+            put("seen", seen_a + counts_a)
         put("rows", rows)
         if nf:
             o, size = off["floats"]

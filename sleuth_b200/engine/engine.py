@@ -20,6 +20,7 @@ from typing import Callable, Sequence
 import numpy as np
 import torch
 
+from ..cache.keep import KeepPolicy
 from ..cache.paged import PagedCache
 from ..config.base import read_config_json
 from ..config.registry import parse_config
@@ -47,17 +48,40 @@ def resolve_dtype(dtype) -> torch.dtype:
                          f"(or 'float32')") from None
 
 
+def _check_keep(keep: KeepPolicy | None, spec) -> None:
+    """A bounded cache is built for models whose every mixer is grouped-query attention over a cache entry of its own."""
+    if keep is None:
+        return
+    if not isinstance(keep, KeepPolicy):
+        raise TypeError(f"keep is a KeepPolicy or None, got {type(keep).__name__}")
+    kinds = sorted({layer.mixer.kind for layer in spec.layers if layer.mixer.kind != "gqa_attention"})
+    if kinds:
+        raise ValueError(f"keep: not built for mixers of kind {', '.join(kinds)}")
+    if len({e.cache for e in spec.schedule}) != len(spec.schedule) or any(e.borrow >= 0 for e in spec.schedule):
+        raise ValueError("keep: not built for layer applications that share a cache entry")
+
+
+def _cache_for(model, keep: KeepPolicy | None, max_tokens, max_seq_len: int, dtype, device, max_sequences) -> PagedCache:
+    if keep is not None and keep.budget:
+        rows = keep.most_rows
+        return PagedCache(model.cache_requests, 8 * rows if max_tokens is None else max_tokens, rows, dtype, device, max_sequences, keep.budget)
+    return PagedCache(model.cache_requests, 8 * max_seq_len if max_tokens is None else max_tokens, max_seq_len, dtype, device, max_sequences)
+
+
 class Engine:
     """A loaded model with its cache, step function, sampler and generation loop."""
 
     def __init__(self, config, spec, model: Model, cache: PagedCache, device, dtype, max_seq_len: int,
-                 unread_keys=(), use_graphs: bool = True, max_step_tokens: int = 8192):
+                 unread_keys=(), use_graphs: bool = True, max_step_tokens: int = 8192, keep: KeepPolicy | None = None):
         self.config, self.spec, self.model, self.cache = config, spec, model, cache
         self.device, self.dtype = torch.device(device), dtype
         self.unread_keys = list(unread_keys)
         self.max_len = int(max_seq_len)
+        self.keep = keep
+        budget = keep is not None and keep.budget > 0
+        self.max_rows = keep.most_rows if budget else None       # rows of the cache that a sequence holds at most, if the policy bounds them
         self.stepper = Stepper(model, cache, device, max_len=self.max_len, max_step_tokens=max_step_tokens,
-                               use_graphs=use_graphs)
+                               use_graphs=use_graphs, portion=keep.portion if budget else 0)
         self.sampler = Sampler(device, model.vocab)
         self.vocab = model.vocab
         self.total_pages = cache.n_pages
@@ -66,14 +90,15 @@ class Engine:
     @classmethod
     def from_pretrained(cls, folder, dtype="bf16", max_seq_len: int = 4096, max_tokens: int | None = None,
                         device="cuda:0", use_graphs: bool = True, max_step_tokens: int = 8192,
-                        max_sequences: int | None = None) -> "Engine":
+                        max_sequences: int | None = None, keep: KeepPolicy | None = None) -> "Engine":
         """Load ``folder`` (``config.json`` + safetensors).
 
         max_seq_len: the longest sequence (prompt plus new tokens); capped by the model's
         ``max_position_embeddings`` (sleuth/formats/hf.py:96). max_tokens: how many tokens all live
         sequences may hold together (each rounded up to 64); sizes the cache. Default: 8 sequences
         of ``max_seq_len``. max_sequences: how many sequences may be live at once (sizes the slot tables and
-        any per-sequence state; see ``PagedCache``)."""
+        any per-sequence state; see ``PagedCache``). keep: bounds what the cache holds of each sequence (``cache/keep.py``);
+        under a budget ``max_tokens`` counts the rows that are kept, and ``max_seq_len`` may be far above what the cache holds."""
         if not torch.cuda.is_available():
             raise RuntimeError("sleuth_b200 runs on an NVIDIA GPU only; torch.cuda.is_available() is False")
         run_dtype = resolve_dtype(dtype)
@@ -85,20 +110,20 @@ class Engine:
             # name -> shape: a description may ask which tensors the files hold, and read a size that only a shape gives
             spec = arch.model_spec(cfg, tensor_names={n: tuple(ckpt.describe(n)[1]) for n in ckpt.names()})
             max_seq_len = max(1, min(int(max_seq_len), spec.max_positions))
-            ctx = BuildContext(device=device, dtype=run_dtype, max_positions=-(-max_seq_len // 64) * 64)
+            _check_keep(keep, spec)
+            ctx = BuildContext(device=device, dtype=run_dtype, max_positions=-(-max_seq_len // 64) * 64, keep=keep)
             model = Model(spec, ctx)
             tensors = load_into(model.expected(), ckpt, run_dtype, device, ignored=spec.ignored_tensors)
             model.bind(tensors)
             del tensors
-        if max_tokens is None:
-            max_tokens = 8 * max_seq_len
-        cache = PagedCache(model.cache_requests, max_tokens, max_seq_len, run_dtype, device, max_sequences)
-        return cls(cfg, spec, model, cache, device, run_dtype, max_seq_len, unread, use_graphs, max_step_tokens)
+        cache = _cache_for(model, keep, max_tokens, max_seq_len, run_dtype, device, max_sequences)
+        return cls(cfg, spec, model, cache, device, run_dtype, max_seq_len, unread, use_graphs, max_step_tokens, keep)
 
     @classmethod
     def from_config(cls, config_json: dict, seed: int = 0, dtype="bf16", max_seq_len: int = 4096,
                     max_tokens: int | None = None, device="cuda:0", use_graphs: bool = True,
-                    max_step_tokens: int = 8192, std: float = 0.02, max_sequences: int | None = None) -> "Engine":
+                    max_step_tokens: int = 8192, std: float = 0.02, max_sequences: int | None = None,
+                    keep: KeepPolicy | None = None) -> "Engine":
         """A model with random weights drawn on the device from a ``config.json`` dictionary and a
         seed: matrices and biases ~ N(0, std), norm gains ~ 1 + N(0, std). Nothing is written to disk
         (``weights.write_random_model`` writes a folder instead, with a generator that is the same on
@@ -111,7 +136,8 @@ class Engine:
         arch, cfg, unread = parse_config(config_json)
         spec = arch.model_spec(cfg)
         max_seq_len = max(1, min(int(max_seq_len), spec.max_positions))
-        ctx = BuildContext(device=device, dtype=run_dtype, max_positions=-(-max_seq_len // 64) * 64)
+        _check_keep(keep, spec)
+        ctx = BuildContext(device=device, dtype=run_dtype, max_positions=-(-max_seq_len // 64) * 64, keep=keep)
         model = Model(spec, ctx)
         gen = torch.Generator(device=device)
         gen.manual_seed(int(seed))
@@ -128,10 +154,8 @@ class Engine:
             tensors[name] = t.to(run_dtype) if d.role == "matrix" else t
         model.bind(tensors)
         del tensors
-        if max_tokens is None:
-            max_tokens = 8 * max_seq_len
-        cache = PagedCache(model.cache_requests, max_tokens, max_seq_len, run_dtype, device, max_sequences)
-        return cls(cfg, spec, model, cache, device, run_dtype, max_seq_len, unread, use_graphs, max_step_tokens)
+        cache = _cache_for(model, keep, max_tokens, max_seq_len, run_dtype, device, max_sequences)
+        return cls(cfg, spec, model, cache, device, run_dtype, max_seq_len, unread, use_graphs, max_step_tokens, keep)
 
     # ------------------------------------------------------------------ stepping ----
     def open(self, n: int) -> list[int]:
@@ -173,11 +197,14 @@ class Engine:
         return min(g.pool.free for g in self.cache.book.groups) if self.cache.book.groups else 1 << 30
 
     def pages_needed(self, slots, new_lengths) -> int:
-        need = self.cache.book.pages_needed(slots, new_lengths)
+        # (tokens of the texts -> rows of the cache: the same numbers unless a budget took rows out)
+        book = self.cache.book
+        need = book.pages_needed(slots, [n - int(book.seen[s]) + int(book.lengths[s]) for s, n in zip(slots, new_lengths)])
         return max(need) if need else 0
 
     def length(self, slot: int) -> int:
-        return int(self.cache.book.lengths[slot])
+        """Tokens of the sequence so far."""
+        return int(self.cache.book.seen[slot])
 
     def sync(self) -> None:
         torch.cuda.synchronize(self.device)

@@ -76,13 +76,13 @@ class _Live:
 
 
 def plan_batches(prompt_lengths: Sequence[int], max_new_tokens: int, max_len: int, total_pages: int,
-                 max_batch: int) -> list[list[int]]:
+                 max_batch: int, max_rows: int | None = None) -> list[list[int]]:
     """Split request indices, in order, into batches. A batch holds at most ``max_batch`` requests and
     only as many as the cache can hold at their longest (prompt plus new tokens, capped by the
-    context); a request too long for that on its own still gets a batch to itself."""
+    context, and by ``max_rows`` where the cache keeps no more); a request too long for that on its own still gets a batch to itself."""
     batches, cur, pages = [], [], 0
     for i, n in enumerate(prompt_lengths):
-        need = pages_for(min(n + max_new_tokens, max_len))
+        need = pages_for(min(n + max_new_tokens, max_len, max_len if max_rows is None else max_rows))
         if cur and (len(cur) >= max_batch or pages + need > total_pages):
             batches.append(cur)
             cur, pages = [], 0
@@ -120,7 +120,7 @@ def generate_batches(backend: Backend, prompts: Sequence[Sequence[int]], max_new
     pipelined = getattr(backend, "pipelined", False) and not sampling.needs_context
     run = _run_batch_pipelined if pipelined else _run_batch
     for batch in plan_batches([len(p) for p in cleaned], max_new_tokens, backend.max_len, backend.total_pages,
-                              max_batch):
+                              max_batch, getattr(backend, "max_rows", None)):
         run(backend, batch, cleaned, results, max_new_tokens, sampling, stop_ids, vocab_limit, seed, on_token)
     return results  # type: ignore[return-value]
 

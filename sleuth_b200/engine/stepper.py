@@ -45,15 +45,19 @@ class Stepper:
     STATUS_EVERY = 16
 
     def __init__(self, model, cache, device, max_len: int | None = None, max_step_tokens: int = 8192,
-                 use_graphs: bool = True, max_graph_batch: int = 256):
+                 use_graphs: bool = True, max_graph_batch: int = 256, portion: int = 0):
+        """portion: the most tokens one sequence may bring in a chunk (0: no limit), which a cache with a budget needs: its
+        rows are bounded by the budget and one portion, whatever the length of the texts."""
         self.model, self.cache = model, cache
-        self.max_len = cache.book.max_len if max_len is None else min(int(max_len), cache.book.max_len)
+        self.portion = int(portion)
+        budget = cache.book.budget
+        self.max_len = cache.book.max_len if max_len is None else int(max_len) if budget else min(int(max_len), cache.book.max_len)
         self.device = torch.device(device)
         self.max_step_tokens = max_step_tokens
         self.use_graphs = use_graphs
         self.max_graph_batch = max_graph_batch
         self.ws = Workspace(self.device)
-        self.meta = MetaStager(self.device, cache.n_groups, cache.stride)
+        self.meta = MetaStager(self.device, cache.n_groups, cache.stride, rows_apart=budget > 0)
         self._graphs: dict = {}
         self._seen_decode: set = set()
         self._seen_chunk: set = set()
@@ -91,7 +95,7 @@ class Stepper:
         slots = [int(e.slot) for e in entries]
         if len(set(slots)) != len(slots):
             raise ValueError("a step names a slot twice")
-        finals = [int(book.lengths[s]) + int(t.size) for s, t in zip(slots, toks)]
+        finals = [int(book.seen[s]) + int(t.size) for s, t in zip(slots, toks)]
         for s, n in zip(slots, finals):
             if n > self.max_len:
                 raise CacheFull(f"slot {s} would hold {n} tokens; the longest sequence allowed is {self.max_len}")
@@ -109,6 +113,9 @@ class Stepper:
             for (i, _, take), s in zip(chunk, c_slots):
                 lens[s] += take
             plan.append((c_slots, [lens[s] for s in c_slots]))
+            if book.budget:
+                for s in c_slots:
+                    lens[s] = min(lens[s], book.budget)
         for g, need in zip(book.groups, book.peak_pages_needed(plan)):
             if need > g.pool.free:
                 raise CacheFull(f"the step needs {need} more pages of 64 tokens and {g.pool.free} of {g.pool.n_pages} "
@@ -134,7 +141,7 @@ class Stepper:
             for i, t in enumerate(toks):
                 left = t.size - done[i]
                 if left and room:
-                    take = min(left, room)
+                    take = min(left, room, self.portion or room)
                     chunk.append((i, done[i], take))
                     room -= take
             if not chunk:
@@ -206,7 +213,7 @@ class Stepper:
         order = np.argsort(np.asarray(dest, dtype=np.int64), kind="stable") if dest else np.zeros(0, dtype=np.int64)
         rows_a = np.asarray(rows, dtype=np.int32)[order] if rows else np.zeros(0, dtype=np.int32)
         dest_a = np.asarray(dest, dtype=np.int64)[order] if dest else np.zeros(0, dtype=np.int64)
-        b = self.meta.upload(c_slots, c_past, c_counts, tokens, rows_a, book.tables_for(c_slots))
+        b = self.meta.upload(c_slots, c_past, c_counts, tokens, rows_a, book.tables_for(c_slots), seen=book.seen[c_slots])
         W = rows_a.shape[0]
         if self._chunk_by_graph(b, W, out, dest_a):
             pass
@@ -289,8 +296,8 @@ class Stepper:
         if len(slots) > self.meta.FEED:
             raise ValueError(f"a device-fed step takes at most {self.meta.FEED} sequences")
         for s in slots:
-            if int(book.lengths[s]) + 1 > self.max_len:
-                raise CacheFull(f"slot {s} would hold {int(book.lengths[s]) + 1} tokens; the longest sequence allowed "
+            if int(book.seen[s]) + 1 > self.max_len:
+                raise CacheFull(f"slot {s} would hold {int(book.seen[s]) + 1} tokens; the longest sequence allowed "
                                 f"is {self.max_len}")
         return self._decode_core(slots, None, np.asarray(feed_map, dtype=np.int32), None)
 
@@ -308,7 +315,7 @@ class Stepper:
         if floats is None:
             floats = np.zeros(n, dtype=np.float32)
         b = self.meta.upload(slots, past, [1] * n, tokens, rows, book.tables_for(slots), floats=floats,
-                             feed_map=feed_map)
+                             feed_map=feed_map, seen=book.seen[slots])
         self.last_batch = b
         if self._decode_logits is None or self._decode_logits.shape[0] < n:
             cap = max(n, 8 if self._decode_logits is None else 2 * self._decode_logits.shape[0])

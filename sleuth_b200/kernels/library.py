@@ -201,6 +201,7 @@ _SIGNATURES = {
     "slb_streams_sum": [P, P, L, I, I, P],
     "slb_pair_combine": [P, P, P, P, F, F, F, P, L, I, I, P],
     "slb_row_gate": [P, P, P, P, L, I, I, I, I, P],
+    "slb_qkv_post_rows": [P, P, P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, F, I, P],
     "slb_attention_kept": [P, P, P, P, P, P, P, P, I, I, L, I, I, I, I, I, I, I, F, P, P, P, P, L, P, L, L, P, I, P],
     "slb_cache_evict": [P, P, P, P, L, P, P, P, I, I, I, I, P, P, P, P, I, I, I, I, P, L, P],
 }

@@ -234,8 +234,9 @@ def mingru(p, bz, bu, state, slots, seq_start, y, max_count: int, scratch=None, 
 
 
 def qkv_post(qkv, bias, q_gain, k_gain, cos, sin, q_out, k_pool, v_pool, tok_seq, tok_pos, block_table,
-             heads: int, kv_heads: int, head_dim: int, rot_dim: int, eps: float, stream=None) -> None:
-    _cuda(qkv, bias, q_gain, k_gain, cos, sin, q_out, k_pool, v_pool, tok_seq, tok_pos, block_table)
+             heads: int, kv_heads: int, head_dim: int, rot_dim: int, eps: float, stream=None, tok_rot=None) -> None:
+    """``tok_rot`` [tokens] int32: the positions by which queries and keys are rotated, when ``tok_pos`` speaks of rows of the cache only."""
+    _cuda(qkv, bias, q_gain, k_gain, cos, sin, q_out, k_pool, v_pool, tok_seq, tok_pos, block_table, tok_rot)
     T = q_out.shape[0]
     rows = heads + 2 * kv_heads
     _need(qkv.shape == (T, rows * head_dim) and q_out.shape[1:] == (heads, head_dim), "qkv_post: shapes disagree")
@@ -253,6 +254,12 @@ def qkv_post(qkv, bias, q_gain, k_gain, cos, sin, q_out, k_pool, v_pool, tok_seq
         _need(block_table.dtype == torch.int32 and block_table.dim() == 2, "qkv_post: block table")
         stride = block_table.shape[1]
     _need(tok_seq.dtype == torch.int32 and tok_pos.dtype == torch.int32, "qkv_post: token tables are int32")
+    if tok_rot is not None:
+        _need(tok_rot.dtype == torch.int32 and tok_rot.numel() >= T, "qkv_post: tok_rot is int32, one a token")
+        lib().call("slb_qkv_post_rows", _p(qkv), _p(bias), _p(q_gain), _p(k_gain), _p(cos), _p(sin), _p(q_out), _p(k_pool), _p(v_pool),
+                   _p(tok_seq), _p(tok_pos), _p(tok_rot), _p(block_table), stride, T, heads, kv_heads, head_dim, rot_dim, float(eps),
+                   DT[qkv.dtype], stream if stream is not None else current_stream())
+        return
     lib().call("slb_qkv_post", _p(qkv), _p(bias), _p(q_gain), _p(k_gain), _p(cos), _p(sin), _p(q_out), _p(k_pool),
                _p(v_pool), _p(tok_seq), _p(tok_pos), _p(block_table), stride, T, heads, kv_heads, head_dim, rot_dim,
                float(eps), DT[qkv.dtype], stream if stream is not None else current_stream())

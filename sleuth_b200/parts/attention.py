@@ -27,7 +27,8 @@ import os
 
 import torch
 
-from ..cache.paged import KVRequest
+from ..cache.book import pages_for
+from ..cache.paged import BundleRequest, KVRequest, StateRequest
 from ..kernels import ops
 from .base import BuildContext, Normed, ParamDecl, Part, build_position, register_mixer, result_target
 from .linear import Linear, use_tc
@@ -75,6 +76,7 @@ class GQAAttention(Part):
         # the signed window of the cache and the kernels (a chunk longer than any sequence is as good as 2^29 positions)
         self.reach = -min(spec.chunk, 1 << 29) if spec.chunk else spec.window
         self.gated = spec.gate == "channel"
+        self.keep = ctx.keep
         self.wide = (self.value_dim != spec.head_dim or self.whole_norm or getattr(self.position, "neighbours", False) or self.gated)
         # The tensor-core attention kernels take keys and values of one width, 64 or 128. A bfloat16 run of the wide form
         # with other widths up to 128 gives every head zero channels at its end until it has such a width (zero rows in
@@ -83,6 +85,9 @@ class GQAAttention(Part):
         self.key_run, self.value_run = spec.head_dim, self.value_dim
         if self.wide and ctx.dtype == torch.bfloat16 and max(spec.head_dim, self.value_dim) <= 128:
             self.key_run = self.value_run = 64 if max(spec.head_dim, self.value_dim) <= 64 else 128
+        if self.keep is not None and (self.wide or spec.sinks or spec.unit_sink or spec.chunk or spec.window or spec.reads_shared_kv):
+            raise ValueError("keep: not built for attention with a window, chunks or sinks of its own, values of another width, whole-projection "
+                             "norms, neighbour pairing, a gate or a borrowed cache entry")
         if self.wide and spec.reads_shared_kv:
             raise ValueError("attention: a borrowed cache entry is not built for values of another width, whole-projection "
                              "norms, neighbour pairing or a gate")
@@ -161,6 +166,12 @@ class GQAAttention(Part):
 
     def cache_request(self):
         s = self.spec
+        if self.keep is not None and self.keep.window:
+            return KVRequest(s.kv_heads, s.head_dim, self.keep.window, first=self.keep.first)
+        if self.keep is not None:      # beside keys and values, for every row what it has gathered and the position of its token
+            shape = (s.kv_heads, 64 * pages_for(self.keep.most_rows))
+            return BundleRequest((("kv", KVRequest(s.kv_heads, s.head_dim)), ("gathered", StateRequest(shape)),
+                                  ("positions", StateRequest(shape, torch.int32))))
         return KVRequest(s.kv_heads, self.key_run, self.reach, 0 if self.value_run == self.key_run else self.value_run)
 
     # ---- one step ----
@@ -204,7 +215,7 @@ class GQAAttention(Part):
     def fused_decode(self):
         s = self.spec
         rot = self.position.rot_dim
-        if (self.wide or self.sinks is not None or s.chunk or self.ctx.dtype != torch.bfloat16 or self.qkv is None or s.reads_shared_kv or s.head_dim not in (64, 128)
+        if (self.keep is not None or self.wide or self.sinks is not None or s.chunk or self.ctx.dtype != torch.bfloat16 or self.qkv is None or s.reads_shared_kv or s.head_dim not in (64, 128)
                 or rot not in (0, s.head_dim) or s.heads // s.kv_heads > 8 or s.hidden % 128
                 or (s.qk_norm and (self.q_gain is None or self.k_gain is None))):
             return None
@@ -214,7 +225,40 @@ class GQAAttention(Part):
                 "sin": tables[1] if tables else None, "heads": s.heads, "kv_heads": s.kv_heads, "head_dim": s.head_dim,
                 "window": s.window, "qk_eps": s.qk_norm_eps, "scale": self.scale, "hidden": s.hidden}
 
+    def _forward_kept(self, h, x, b, view, ws):
+        """A cache of bounded size (cache/keep.py). Under a window: the latest tokens and the first ones. Under a budget: all rows that are
+        held; the step's weights are gathered, and rows beyond the budget evicted."""
+        s, keep, T = self.spec, self.keep, h.shape[0]
+        mark = ws.mark()
+        gathered = positions = None
+        if keep.budget:
+            gathered, positions, view = view["gathered"].state, view["positions"].state, view["kv"]
+        table = b.tables[view.group]
+        tables = self.position.tables()
+        cos, sin = tables if tables is not None else (None, None)
+        qkv = self.qkv.forward(h, ws=ws, stream=b.stream)
+        q = ws.take((T, s.heads, s.head_dim), self.ctx.dtype)
+        ops.qkv_post(qkv, self.bias, self.q_gain, self.k_gain, cos, sin, q, view.k_pool, view.v_pool, b.tok_seq, b.tok_pos, table, s.heads,
+                     s.kv_heads, s.head_dim, self.position.rot_dim, s.qk_norm_eps, b.stream, tok_rot=b.tok_rot)
+        y = ws.take((T, s.heads * s.head_dim), self.ctx.dtype)
+        # (a recorded step serves later ones of its shape, so sizes go by what the cache may hold, not by what it holds now)
+        rows = 64 * table.shape[1]
+        floats = ops.attention_kept_scratch_floats(T, b.n, b.max_count, s.heads, s.kv_heads, s.head_dim, rows, self.ctx.dtype, weights=keep.budget > 0)
+        scratch = ws.take((floats,), torch.float32) if floats else None
+        ops.attention_kept(q, view.k_pool, view.v_pool, y, b.seq_start, b.past, b.counts, table, b.max_count, s.heads, s.kv_heads, s.head_dim,
+                           keep.window, keep.first, self.scale, b.stream, scratch=scratch, weights=gathered, slots=b.slots if keep.budget else None)
+        self.o.forward(y, ws=ws, stream=b.stream, next_read=getattr(b, "next_read", None), **result_target(b, x))
+        if keep.budget:
+            most = min(rows, keep.budget + b.max_count)
+            words = ops.cache_evict_scratch_words(b.n, s.kv_heads, keep.budget, most)
+            ops.cache_evict(gathered, positions, view.k_pool, view.v_pool, table, b.past, b.lengths, b.seen, keep.budget, keep.first, keep.latest,
+                            slots=b.slots, scratch=ws.take((words,), torch.int32) if words else None, max_length=most, stream=b.stream)
+        ws.release(mark)
+
     def forward(self, h, x, b, view, ws):
+        if self.keep is not None:
+            self._forward_kept(h, x, b, view, ws)
+            return
         s = self.spec
         T = h.shape[0]
         writes = view.writes and not s.reads_shared_kv

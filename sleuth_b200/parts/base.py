@@ -57,6 +57,7 @@ class BuildContext:
     dtype: torch.dtype          # run dtype: torch.bfloat16 or torch.float32
     max_positions: int          # longest sequence the engine will hold
     shared: dict = field(default_factory=dict)   # parts that several layers share (position tables)
+    keep: object = None         # a KeepPolicy: the cache holds a bounded number of tokens (cache/keep.py)
 
 
 class Normed:
