@@ -35,7 +35,7 @@ struct EvictArgs {
   const int* seen;
   const int* slots;
   int* scratch;              // with many moves: per (sequence, kv head) their number, the places, the rows
-  int table_stride, n_seqs, kv_heads, row_bytes, budget, first, recent, max_length, keys_fit, most_moves, vector;
+  int table_stride, n_seqs, kv_heads, row_bytes, budget, first, recent, max_length, keys_fit, most_moves, vector, moves_here;
 };
 
 __device__ __forceinline__ uint32_t order_key(float w, bool safe) {
@@ -188,7 +188,8 @@ __global__ void __launch_bounds__(THREADS) cache_evict_few_kernel(EvictArgs a) {
 }
 
 // ---- many rows go ----
-__global__ void __launch_bounds__(kEvictThreads) cache_evict_kernel(EvictArgs a) {
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) cache_evict_kernel(EvictArgs a) {
   pdl_enter();
   extern __shared__ uint32_t keys[];
   __shared__ int hist[2048];
@@ -209,9 +210,10 @@ __global__ void __launch_bounds__(kEvictThreads) cache_evict_kernel(EvictArgs a)
     const int p = position(j);
     return order_key(weights[j], p < a.first || p >= seen - a.recent);
   };
+  const int* table = a.block_table + (size_t)seq * a.table_stride;
   int* lists = a.scratch ? a.scratch + ((size_t)seq * a.kv_heads + kh) * (2 * (size_t)a.most_moves + 1) : nullptr;
   if (n <= a.budget) {       // all stay (the whole block leaves)
-    for (int j = tid; j < n; j += kEvictThreads) {
+    for (int j = tid; j < n; j += THREADS) {
       if (positions_out != positions || j >= past) positions_out[j] = position(j);
       if (weights_out != weights) weights_out[j] = weights[j];
     }
@@ -219,7 +221,7 @@ __global__ void __launch_bounds__(kEvictThreads) cache_evict_kernel(EvictArgs a)
     return;
   }
   if (a.keys_fit)
-    for (int j = tid; j < n; j += kEvictThreads) keys[j] = make_key(j);
+    for (int j = tid; j < n; j += THREADS) keys[j] = make_key(j);
   __syncthreads();
   auto key_of = [&](int j) { return a.keys_fit ? keys[j] : make_key(j); };
 
@@ -229,21 +231,30 @@ __global__ void __launch_bounds__(kEvictThreads) cache_evict_kernel(EvictArgs a)
 #pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
-    hist[tid] = hist[tid + 1024] = 0;
+#pragma unroll
+    for (int i = 0; i < 2048 / THREADS; ++i) hist[tid + i * THREADS] = 0;
     __syncthreads();
-    for (int j = tid; j < n; j += kEvictThreads) {
+    for (int j = tid; j < n; j += THREADS) {
       const uint32_t k = key_of(j);
       if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1);
     }
     __syncthreads();
-    // a thread two digits, the largest first: how many keys lie above them
-    const int hi = hist[2047 - 2 * tid], lo = hist[2046 - 2 * tid];
+    // a thread a run of digits, the largest first: how many keys lie above them
+    constexpr int RUN = 2048 / THREADS;
+    int own = 0;
+#pragma unroll
+    for (int i = 0; i < RUN; ++i) own += hist[2047 - RUN * tid - i];
     unsigned long long all;
-    const int above = (int)block_scan((unsigned long long)(hi + lo), warp_sums, all);
-    if (above < need && above + hi + lo >= need) {
-      const bool in_hi = above + hi >= need;
-      s_digit = (uint32_t)(2047 - 2 * tid - (in_hi ? 0 : 1));
-      s_need = need - above - (in_hi ? 0 : hi);
+    int above = (int)block_scan((unsigned long long)own, warp_sums, all);
+    if (above < need && above + own >= need) {
+      int i = 0;
+      for (; i < RUN - 1; ++i) {
+        const int c = hist[2047 - RUN * tid - i];
+        if (above + c >= need) break;
+        above += c;
+      }
+      s_digit = (uint32_t)(2047 - RUN * tid - i);
+      s_need = need - above;
     }
     __syncthreads();
     prefix |= s_digit << shift;
@@ -254,7 +265,7 @@ __global__ void __launch_bounds__(kEvictThreads) cache_evict_kernel(EvictArgs a)
   const uint32_t last = prefix;
 
   // runs of rows a thread: an odd number, so that the threads of a warp meet different banks
-  const int per = ((n + kEvictThreads - 1) / kEvictThreads) | 1, j0 = min(n, tid * per), j1 = min(n, j0 + per);
+  const int per = ((n + THREADS - 1) / THREADS) | 1, j0 = min(n, tid * per), j1 = min(n, j0 + per);
   unsigned long long ties = 0, total;
   for (int j = j0; j < j1; ++j) ties += key_of(j) == last;
   const int tie0 = (int)block_scan(ties, warp_sums, total);
@@ -288,18 +299,20 @@ __global__ void __launch_bounds__(kEvictThreads) cache_evict_kernel(EvictArgs a)
   // what stays in its place, a warp whole lines (in the loop above each copy would wait for the one before)
   if (a.keys_fit && (positions_out != positions || weights_out != weights || past < left))
 #pragma unroll 4
-    for (int j = tid; j < left; j += kEvictThreads) {
+    for (int j = tid; j < left; j += THREADS) {
       if (!keys[j]) continue;
       const float w = weights[j];
       const int p = position(j);
       if (positions_out != positions || j >= past) positions_out[j] = p;
       if (weights_out != weights) weights_out[j] = w;
     }
-  for (int i = tid; i < moves; i += kEvictThreads) {      // (the block's own stores are visible to it after the barrier)
+  for (int i = tid; i < moves; i += THREADS) {      // (the block's own stores are visible to it after the barrier)
     const int to = lists[1 + i], from = lists[1 + a.most_moves + i];
     weights_out[to] = weights[from];
     positions_out[to] = position(from);
   }
+  if (a.moves_here)
+    for (int i = tid >> 4; i < moves; i += THREADS / 16) move_row(a, table, kh, lists[1 + i], lists[1 + a.most_moves + i], tid & 15, 16);
 }
 
 // The moves of the lists: 16 threads a row of each pool.
@@ -330,6 +343,7 @@ static int launch_evict_few(const EvictArgs& a, cudaStream_t s) {
   else if (a.max_length <= 256 * 10) launch(cache_evict_few_kernel<256, 10>, grid, dim3(256), 0, s, a);
   else if (a.max_length <= 512 * 10) launch(cache_evict_few_kernel<512, 10>, grid, dim3(512), 0, s, a);
   else if (a.max_length <= 1024 * 10) launch(cache_evict_few_kernel<1024, 10>, grid, dim3(1024), 0, s, a);
+  else if (a.max_length <= 1024 * 16) launch(cache_evict_few_kernel<1024, 16>, grid, dim3(1024), 0, s, a);
   else launch(cache_evict_few_kernel<1024, 32>, grid, dim3(1024), 0, s, a);
   return check_launch("cache_evict (few rows)");
 }
@@ -373,11 +387,17 @@ extern "C" int slb_cache_evict(const float* weights, float* weights_out, const i
   if (few_go(budget, max_length)) return launch_evict_few(a, (cudaStream_t)stream);
   const int smem = a.keys_fit ? max_length * 4 : 0;
   static std::atomic<unsigned long long> allowed;
-  const cudaError_t e = allow_shared((const void*)cache_evict_kernel, kMostKeysShared * 4, allowed);
-  if (e != cudaSuccess) return fail(2, "cache_evict: cannot reserve shared memory: %s", cudaGetErrorString(e));
-  launch(cache_evict_kernel, dim3(kv_heads, n_seqs), dim3(kEvictThreads), smem, (cudaStream_t)stream, a);
+  // few moves are made by the block that found them: a second kernel costs 3 us, 64 rows of 512 bytes a block less than one
+  a.moves_here = a.most_moves * (long long)row_bytes <= 32 * 1024;
+  if (max_length <= 2048) {      // small blocks, so that many share an SM
+    launch(cache_evict_kernel<256>, dim3(kv_heads, n_seqs), dim3(256), smem, (cudaStream_t)stream, a);
+  } else {
+    const cudaError_t e = allow_shared((const void*)cache_evict_kernel<kEvictThreads>, kMostKeysShared * 4, allowed);
+    if (e != cudaSuccess) return fail(2, "cache_evict: cannot reserve shared memory: %s", cudaGetErrorString(e));
+    launch(cache_evict_kernel<kEvictThreads>, dim3(kv_heads, n_seqs), dim3(kEvictThreads), smem, (cudaStream_t)stream, a);
+  }
   const int rc = check_launch("cache_evict");
-  if (rc) return rc;
+  if (rc || a.moves_here) return rc;
   const long long pairs = (long long)n_seqs * kv_heads;
   long long blocks = 8ll * sm_count() / pairs;
   const long long most = (a.most_moves + 15) / 16;

@@ -310,7 +310,7 @@ static int launch_general(const KeptArgs& a, int max_count, long long tokens, cu
   launch(kept_general_kernel<T, RPT>, dim3((unsigned)(tiles * a.splits), a.kv_heads, a.n_seqs), dim3(kGenThreads), smem, s, a, tokens);
   int rc = check_launch("attention_kept (general kernel)");
   if (rc || a.splits == 1) return rc;
-  launch(kept_join_kernel<T>, dim3(a.heads, (unsigned)(tokens < 65535 ? tokens : 65535), (unsigned)((tokens + 65534) / 65535)),
+  launch_prefetching(kept_join_kernel<T>, dim3(a.heads, (unsigned)(tokens < 65535 ? tokens : 65535), (unsigned)((tokens + 65534) / 65535)),
          dim3((a.head_dim + 31) / 32 * 32), 0, s, a, tokens);
   return check_launch("attention_kept (join)");
 }
@@ -328,7 +328,7 @@ static int general_weights(const KeptArgs& a, int max_keys, cudaStream_t s) {
   static std::atomic<unsigned long long> allowed;
   const cudaError_t e = allow_shared((const void*)kept_weights_general_kernel<T>, weights_smem(256), allowed);
   if (e != cudaSuccess) return fail(2, "attention_kept: cannot reserve shared memory: %s", cudaGetErrorString(e));
-  launch(kept_weights_general_kernel<T>, dim3((max_keys + kGenKeys - 1) / kGenKeys, a.kv_heads, a.n_seqs), dim3(kGenThreads),
+  launch_prefetching(kept_weights_general_kernel<T>, dim3((max_keys + kGenKeys - 1) / kGenKeys, a.kv_heads, a.n_seqs), dim3(kGenThreads),
          weights_smem(a.head_dim), s, a);
   return check_launch("attention_kept (weights, general kernel)");
 }

@@ -17,6 +17,7 @@
 // order of the ranks.
 #include <math.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "kept.cuh"
@@ -32,6 +33,7 @@ struct KeptWeightsArgs {
   const float* lse2;
   float scale_log2;
   int* status;
+  int tile0;            // the first key tile of the launch
 };
 
 template <int HD>
@@ -81,7 +83,7 @@ kept_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   const int rank = (int)cluster_ctarank(), ranks = a.splits;
   const int G = a.heads / a.kv_heads, pairs = (int)(gridDim.y * gridDim.z);
   const int lin = (int)(blockIdx.x / ranks + gridDim.x / ranks * (blockIdx.y + gridDim.y * blockIdx.z));
-  const int seq = (lin % pairs) / (int)gridDim.y, kh = (lin % pairs) % (int)gridDim.y, key0 = lin / pairs * kKwKeys;
+  const int seq = (lin % pairs) / (int)gridDim.y, kh = (lin % pairs) % (int)gridDim.y, key0 = (w.tile0 + lin / pairs) * kKwKeys;
   const uint32_t bars = base + L::BAR_OFF;
   const uint32_t k_full = bars, q_full = bars + 8, q_free = q_full + 8 * L::STAGES, s_full = q_free + 8 * L::STAGES, s_free = s_full + 8 * kKwBuffers,
                  d_full = s_free + 8 * kKwBuffers, d_free = d_full + 8 * kKwBuffers;
@@ -289,12 +291,12 @@ kept_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   }
 }
 
-// Blocks that share a key tile: while blocks are fewer than two an SM, and a block keeps four steps of the longest walk.
-static int kw_ranks(int n_seqs, int kv_heads, int G, int max_count, int max_keys) {
-  const long long tiles = (long long)n_seqs * kv_heads * ((max_keys + kKwKeys - 1) / kKwKeys);
-  const int steps = (max_count * G + kKwRows - 1) / kKwRows;
+// Blocks that share each of `tiles` key tiles whose walks are at most `longest` steps and `total` in all: while the longest walk is longer than an SM's
+// share of all, or blocks are fewer than two an SM; a block keeps four steps of the longest.
+static int kw_ranks(long long tiles, long long longest, long long total) {
+  const long long sms = sm_count();
   int ranks = 1;
-  while (ranks < 8 && tiles * ranks < 2 * sm_count() && steps / (2 * ranks) >= 4) ranks *= 2;
+  while (ranks < 8 && longest / (2 * ranks) >= 4 && (longest * sms > total * ranks || tiles * ranks < 2 * sms)) ranks *= 2;
   return ranks;
 }
 
@@ -308,14 +310,34 @@ static int kw_encode(CUtensorMap* map, int rank, const void* base, const cuuint6
 }
 
 template <int HD>
-static int launch_kw(const CUtensorMap& mq, const CUtensorMap& mk, const KeptWeightsArgs& w, int max_keys, cudaStream_t s) {
+static int launch_kw(const CUtensorMap& mq, const CUtensorMap& mk, KeptWeightsArgs w, int tile0, int tiles, int ranks, cudaStream_t s) {
   static std::atomic<unsigned long long> allowed;
   const cudaError_t e = allow_shared((const void*)kept_weights_kernel<HD>, KwLayout<HD>::TOTAL, allowed);
   if (e != cudaSuccess) return fail(2, "attention_kept: cannot reserve %d bytes of shared memory: %s", KwLayout<HD>::TOTAL, cudaGetErrorString(e));
-  const unsigned tiles = (unsigned)((max_keys + kKwKeys - 1) / kKwKeys);
-  const dim3 grid(tiles * w.k.splits, w.k.kv_heads, w.k.n_seqs);
-  launch_clusters(pdl_mode() != 0, (unsigned)w.k.splits, kept_weights_kernel<HD>, grid, dim3(kKwThreads), (size_t)KwLayout<HD>::TOTAL, s, mq, mk, w);
+  w.tile0 = tile0;
+  w.k.splits = ranks;
+  const dim3 grid((unsigned)(tiles * ranks), w.k.kv_heads, w.k.n_seqs);
+  launch_clusters(pdl_mode() != 0, (unsigned)ranks, kept_weights_kernel<HD>, grid, dim3(kKwThreads), (size_t)KwLayout<HD>::TOTAL, s, mq, mk, w);
   return check_launch("attention_kept (weights)");
+}
+
+template <int HD>
+static int launch_all(const CUtensorMap& mq, const CUtensorMap& mk, const KeptWeightsArgs& w, int max_count, int max_keys, cudaStream_t s) {
+  const KeptArgs& k = w.k;
+  const int G = k.heads / k.kv_heads, tiles = (max_keys + kKwKeys - 1) / kKwKeys;
+  const long long pairs = (long long)k.n_seqs * k.kv_heads, longest = ((long long)max_count * G + kKwRows - 1) / kKwRows;
+  if (k.window == 0) return launch_kw<HD>(mq, mk, w, 0, tiles, kw_ranks(pairs * tiles, longest, pairs * tiles * ((longest + 1) / 2)), s);
+  // Under a window most keys are seen by a few steps' queries, the first ones by all: launches of their own where that is far apart (two prompts of 875
+  // and 2,626 tokens, 32 / 8 heads, a window of 8, 4 first: one launch 102 us, with eight blocks a tile or one)
+  const long long usual = std::min(longest, ((long long)(k.window + kKwKeys) * G + kKwRows - 1) / kKwRows + 1);
+  const int all = std::min(tiles, (k.first + kKwKeys - 1) / kKwKeys);
+  const int apart = all < tiles && longest > 2 * usual ? all : 0;
+  if (apart) {
+    const int rc = launch_kw<HD>(mq, mk, w, 0, apart, kw_ranks(pairs * apart, longest, pairs * apart * longest), s);
+    if (rc) return rc;
+  }
+  const long long rest = pairs * (tiles - apart), walk = apart ? usual : longest;
+  return launch_kw<HD>(mq, mk, w, apart, tiles - apart, kw_ranks(rest, walk, rest * usual), s);
 }
 
 int kept_weights_tc(const KeptArgs& k, const float* lse2, long long tokens, int max_count, int max_keys, long long pool_pages, int* status, cudaStream_t s) {
@@ -337,11 +359,10 @@ int kept_weights_tc(const KeptArgs& k, const float* lse2, long long tokens, int 
   }
   KeptWeightsArgs w{};
   w.k = k;
-  w.k.splits = kw_ranks(k.n_seqs, k.kv_heads, G, max_count, max_keys);
   w.lse2 = lse2;
   w.scale_log2 = k.scale * kKeptLog2e;
   w.status = status;
-  return k.head_dim == 64 ? launch_kw<64>(mq, mk, w, max_keys, s) : launch_kw<128>(mq, mk, w, max_keys, s);
+  return k.head_dim == 64 ? launch_all<64>(mq, mk, w, max_count, max_keys, s) : launch_all<128>(mq, mk, w, max_count, max_keys, s);
 }
 
 }  // namespace slb

@@ -22,8 +22,14 @@ ACTIVATIONS = {"silu": 0, "relu": 1, "clamped_swish": 2, "gelu_tanh": 3}
 ROUTE_SCORINGS = {"softmax_top": 0, "sigmoid": 1, "softmax": 2, "softmax_norm": 3}
 
 
+_LIBRARY = None
+
+
 def lib() -> library.KernelLibrary:
-    return library.load()
+    global _LIBRARY
+    if _LIBRARY is None:
+        _LIBRARY = library.load()
+    return _LIBRARY
 
 
 def current_stream() -> int:
