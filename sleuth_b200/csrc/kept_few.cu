@@ -16,6 +16,8 @@
 // replaced by zeros in registers, so that infinities or NaN in them do not meet a zero weight.
 #include <math.h>
 
+#include <algorithm>
+
 #include "kept.cuh"
 #include "mma_sync.cuh"
 #include "tcgen05.cuh"
@@ -30,22 +32,28 @@ constexpr int kFewMostRows = 256;      // rows of a (sequence, kv head) that the
 // and [warps][rows][2], barriers. As many stages as fit.
 struct FewLayout {
   int stages, q_off, merge_off, ml_off, bar_off, total, merge_rows;
+  int part_off, score_off, score_pitch;      // clusters: the block's joined results [rows][HD], [rows][2], and its scores [rows][pitch]
 };
 // (228 KB an SM; a block has 1 KB of static shared memory and 1 KB that the driver takes)
 constexpr int few_room(int R) { return (R == 1 ? 112 : 226) * 1024; }
-static FewLayout few_layout(int HD, int R, int rows) {
+static FewLayout few_layout(int HD, int R, int rows, int cluster_pages = 0, bool weights = false) {
   FewLayout l;
   const int stage = 2 * 64 * HD * 2;
   l.merge_rows = rows < 16 ? rows : 16;
-  const int rest = 16 * R * HD * 2 + few_warps(R) * l.merge_rows * (HD * 4 + 8) + 2 * 8 * 8;
+  l.score_pitch = cluster_pages * 64 + 8;
+  const int shared = cluster_pages ? rows * (HD * 4 + 16) + (weights ? rows * l.score_pitch * 4 : 0) + 32 : 0;
+  const int rest = 16 * R * HD * 2 + few_warps(R) * l.merge_rows * (HD * 4 + 8) + 2 * 8 * 8 + shared;
   const int room = few_room(R);
   l.stages = (room - rest) / stage;
   if (l.stages > 8) l.stages = 8;
+  if (cluster_pages && l.stages > cluster_pages) l.stages = cluster_pages;
   l.q_off = l.stages * stage;
   l.merge_off = l.q_off + 16 * R * HD * 2;
   l.ml_off = l.merge_off + few_warps(R) * l.merge_rows * HD * 4;
   l.bar_off = (l.ml_off + few_warps(R) * l.merge_rows * 8 + 7) & ~7;
-  l.total = l.bar_off + 2 * l.stages * 8;
+  l.part_off = (l.bar_off + 2 * l.stages * 8 + 15) & ~15;
+  l.score_off = l.part_off + rows * (HD * 4 + 16);      // (the last 8 bytes a row: its denominator)
+  l.total = l.part_off + shared;
   return l;
 }
 
@@ -62,6 +70,7 @@ struct FewArgs {
   long long score_stride;
   int* status;
   FewLayout lay;
+  int cluster, cluster_pages;        // blocks that share a (sequence, kv head), and the pages that each takes at most; 0: runs of all units
   int out_blocks, keys_a_block;      // the second kernel's blocks of a (sequence, kv head): some for outputs, one for so many keys
 };
 
@@ -84,13 +93,24 @@ __device__ __forceinline__ float few_ex2(float x) {
   return y;
 }
 
+__device__ __forceinline__ float2 peer_ld2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 peer_ld4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
 // 16-byte piece of channel `col` of row `row` in a tile of 64 rows as TMA leaves it: 64 channels a half, pieces exchanged by the row.
 template <int ROWS>
 __device__ __forceinline__ uint32_t tile_at(int row, int col) {
   return (uint32_t)((col >> 6) * (ROWS * 128) + row * 128 + (((col >> 3) & 7) ^ (row & 7)) * 16);
 }
 
-template <int HD, int R>
+template <int HD, int R, bool CLUSTER>
 __global__ void __launch_bounds__((few_warps(R) + 1) * 32, few_blocks_an_sm(R))
 kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, FewArgs fa) {
   constexpr int ROWS = 16 * R, KW = R == 4 ? 32 : 16, KB = KW / 16, WARPS = few_warps(R), GROUPS = WARPS / R, THREADS = (WARPS + 1) * 32, PAGE = 64 * HD * 2;
@@ -123,42 +143,58 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     const int c = min(a.counts[s], fa.max_count);
     return (long long)PageRun(a.past[s], c, a.window, a.first).count * a.kv_heads * tiles_of(c);
   };
-  const int per = (a.n_seqs + THREADS - 1) / THREADS, q0 = min(a.n_seqs, tid * per), q1 = min(a.n_seqs, q0 + per);
-  long long own = 0;
-  for (int s = q0; s < q1; ++s) own += units_of(s);
-  long long incl = own;
+  // CLUSTER: the blocks of a cluster share the pages of one (sequence, kv head); `u` counts the pages of that pair alone
+  int seq, rank = 0;
+  long long seq_first, u, u_hi, blocks = 1, total = 0;
+  const int pair_kh = CLUSTER ? (int)(blockIdx.x / fa.cluster) % a.kv_heads : 0;
+  if constexpr (CLUSTER) {
+    rank = (int)cluster_ctarank();
+    seq = (int)(blockIdx.x / fa.cluster) / a.kv_heads;
+    const int pages = PageRun(a.past[seq], min(a.counts[seq], fa.max_count), a.window, a.first).count;
+    if (pages == 0) return;      // (the whole cluster)
+    const int share = min((pages + fa.cluster - 1) / fa.cluster, fa.cluster_pages);
+    seq_first = -(long long)pair_kh * pages;      // as if the kv head's units were the first
+    u = min(pages, rank * share);
+    u_hi = min(pages, (int)u + share);
+    __syncthreads();
+  } else {
+    const int per = (a.n_seqs + THREADS - 1) / THREADS, q0 = min(a.n_seqs, tid * per), q1 = min(a.n_seqs, q0 + per);
+    long long own = 0;
+    for (int s = q0; s < q1; ++s) own += units_of(s);
+    long long incl = own;
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, incl, d);
-    if (lane >= d) incl += y;
-  }
-  if (lane == 31) warp_units[warp] = incl;
-  __syncthreads();
-  long long before = 0, total = 0;
-#pragma unroll
-  for (int w = 0; w <= WARPS; ++w) {
-    if (w < warp) before += warp_units[w];
-    total += warp_units[w];
-  }
-  const long long blocks = min((long long)gridDim.x, total);
-  if ((long long)blockIdx.x >= blocks) return;
-  const long long u_lo = blockIdx.x * total / blocks, u_hi = (blockIdx.x + 1) * total / blocks;
-  before += incl - own;
-  if (own > 0 && u_lo >= before && u_lo < before + own) {
-    for (int s = q0; s < q1; ++s) {
-      const long long u = units_of(s);
-      if (u_lo < before + u) {
-        s_seq = s;
-        s_first = before;
-        break;
-      }
-      before += u;
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += y;
     }
+    if (lane == 31) warp_units[warp] = incl;
+    __syncthreads();
+    long long before = 0;
+#pragma unroll
+    for (int w = 0; w <= WARPS; ++w) {
+      if (w < warp) before += warp_units[w];
+      total += warp_units[w];
+    }
+    blocks = min((long long)gridDim.x, total);
+    if ((long long)blockIdx.x >= blocks) return;
+    u = blockIdx.x * total / blocks;
+    u_hi = (blockIdx.x + 1) * total / blocks;
+    before += incl - own;
+    if (own > 0 && u >= before && u < before + own) {
+      for (int s = q0; s < q1; ++s) {
+        const long long units = units_of(s);
+        if (u < before + units) {
+          s_seq = s;
+          s_first = before;
+          break;
+        }
+        before += units;
+      }
+    }
+    __syncthreads();
+    seq = s_seq;
+    seq_first = s_first;      // units before this sequence
   }
-  __syncthreads();
-  int seq = s_seq;
-  long long seq_first = s_first;      // units before this sequence
-  long long u = u_lo;
 
   if (warp == WARPS) {
     // ---- the ring's pages ----
@@ -198,12 +234,13 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         }
         u += n;
       }
+      if (CLUSTER) break;
       seq_first += units;
       ++seq;
     }
     pdl_launch_dependents();
-    return;
-  }
+    if (!CLUSTER) return;
+  } else {
 
   // ---- the products ----
   const int g = lane >> 2, t4 = lane & 3;
@@ -211,6 +248,12 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   auto sync = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory"); };
   int st = 0, lap = 0;
   bool ok = true;
+  if constexpr (CLUSTER) {
+    // a block without pages leaves an empty share
+    if (u >= u_hi)
+      for (int r = tid; r < min(16 * R, min(a.counts[seq], fa.max_count) * G); r += WARPS * 32)
+        *reinterpret_cast<float2*>(smem + L.part_off + r * (HD * 4 + 16) + HD * 4) = make_float2(-INFINITY, 0.0f);
+  }
   while (u < u_hi) {
     const int count = min(a.counts[seq], fa.max_count), past = a.past[seq];
     const PageRun run(past, count, a.window, a.first);
@@ -240,7 +283,8 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         const int r = rt * 16 + g + 8 * h, Rr = row0 + r;
         pos[h] = r < rows ? past + Rr / G : -1;
         lo[h] = window_lo(pos[h], a.window);
-        score_row[h] = fa.scores && r < rows ? fa.scores + ((size_t)(tok0 + Rr / G) * a.heads + kh * G + Rr % G) * fa.score_stride : nullptr;
+        if (CLUSTER) score_row[h] = a.weights && r < rows ? reinterpret_cast<float*>(smem + L.score_off) + r * L.score_pitch : nullptr;
+        else score_row[h] = fa.scores && r < rows ? fa.scores + ((size_t)(tok0 + Rr / G) * a.heads + kh * G + Rr % G) * fa.score_stride : nullptr;
       }
       // what the 16 rows of this warp see: all of them from see_lo (or below `first`) to see_hi, none beyond any_hi or below any_lo
       const int r_first = row0 + rt * 16, r_last = min(row0 + rows, r_first + 16) - 1;
@@ -283,14 +327,14 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
               s[j][e] *= fa.scale_log2;
               if (!whole && !sees(key, pos[e >> 1], lo[e >> 1], a.first)) s[j][e] = -INFINITY;
             }
-          if (fa.scores != nullptr) {
+          if (CLUSTER ? a.weights != nullptr : fa.scores != nullptr) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
               if (score_row[h] != nullptr) {
 #pragma unroll
                 for (int j = 0; j < 2 * KB; ++j) {
-                  const int key = key0 + j * 8 + 2 * t4;
-                  if (key < fa.score_stride) *reinterpret_cast<float2*>(score_row[h] + key) = make_float2(s[j][2 * h], s[j][2 * h + 1]);
+                  const int key = (CLUSTER ? i * 64 + key_in : key0) + j * 8 + 2 * t4;      // (clusters: by the page's place in the block)
+                  if (CLUSTER || key < fa.score_stride) *reinterpret_cast<float2*>(score_row[h] + key) = make_float2(s[j][2 * h], s[j][2 * h + 1]);
                 }
               }
           }
@@ -383,7 +427,7 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       const bool begins = off == 0, complete = begins && n == run.count;
       const long long pair_lo = seq_first + (long long)pair * run.count;
       const int first_block = blockIdx.x;
-      if (begins && tid == 0) {
+      if (!CLUSTER && begins && tid == 0) {
         const long long last = pair_lo + run.count - 1;
         const int last_block = (int)(((last + 1) * blocks - 1) / total);
         fa.info[((size_t)seq * a.kv_heads + kh) * fa.max_tiles + tile] = make_int2(first_block, last_block - first_block + 1);
@@ -407,7 +451,11 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         }
         const int Rr = row0 + r;
         const size_t row = (size_t)(tok0 + Rr / G) * a.heads + kh * G + Rr % G;
-        if (complete) {
+        if (CLUSTER) {
+          float* slot = reinterpret_cast<float*>(smem + L.part_off + r * (HD * 4 + 16));
+          *reinterpret_cast<float4*>(slot + d) = acc;
+          if (d == 0) *reinterpret_cast<float2*>(slot + HD) = make_float2(M, sum);
+        } else if (complete) {
           const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
           uint2 pk;
           pk.x = pack_bf16(acc.x * inv, acc.y * inv);
@@ -426,8 +474,75 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       sync();
       u += n;
     }
+    if (CLUSTER) break;
     seq_first += units;
     ++seq;
+  }
+  }
+  if constexpr (CLUSTER) {
+    const int count = min(a.counts[seq], fa.max_count), past = a.past[seq], tok0 = a.seq_start[seq], rows = min(ROWS, count * G);
+    const PageRun run(past, count, a.window, a.first);
+    const int share = min((run.count + fa.cluster - 1) / fa.cluster, fa.cluster_pages), first_page = min(run.count, rank * share);
+    const int my_pages = min(run.count, first_page + share) - first_page;
+    __syncthreads();         // (the cluster's barrier counts warps: they have to come to it whole)
+    cluster_sync_all();
+    auto peer = [&](int c, int r, int word) { return cluster_map(base + L.part_off + r * (HD * 4 + 16) + word * 4, c); };
+    // denominators: a thread a row
+    for (int r = tid; r < rows; r += THREADS) {
+      float M = -INFINITY, D = 0.0f;
+      for (int c = 0; c < fa.cluster; ++c) {
+        const float2 p = peer_ld2(peer(c, r, HD));
+        const float top = fmaxf(M, p.x), use = top == -INFINITY ? 0.0f : top;
+        D = D * few_ex2(M - use) + p.y * few_ex2(p.x - use);
+        M = top;
+      }
+      const float lse2 = D == 0.0f ? -INFINITY : M + log2f(D);
+      float* slot = reinterpret_cast<float*>(smem + L.part_off + r * (HD * 4 + 16));
+      *reinterpret_cast<float2*>(slot + HD + 2) = make_float2(M, lse2 == -INFINITY ? INFINITY : lse2);
+      if (rank == 0 && a.lse) a.lse[(size_t)(tok0 + r / G) * a.heads + pair_kh * G + r % G] = lse2 * 0.6931471805599453f;
+    }
+    __syncthreads();
+    for (int e = rank * THREADS + tid; e < rows * (HD / 4); e += fa.cluster * THREADS) {
+      const int r = e / (HD / 4), d = (e % (HD / 4)) * 4;
+      const float M = reinterpret_cast<const float*>(smem + L.part_off + r * (HD * 4 + 16))[HD + 2], use = M == -INFINITY ? 0.0f : M;
+      float D = 0.0f;
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (int c = 0; c < fa.cluster; ++c) {
+        const float2 p = peer_ld2(peer(c, r, HD));
+        const float f = few_ex2(p.x - use);
+        if (p.x == -INFINITY && p.y == 0.0f) continue;      // a share without keys (its values were never written)
+        const float4 v = peer_ld4(peer(c, r, d));
+        D += p.y * f;
+        acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
+      }
+      const float inv = D == 0.0f ? 0.0f : 1.0f / D;
+      uint2 pk;
+      pk.x = pack_bf16(acc.x * inv, acc.y * inv);
+      pk.y = pack_bf16(acc.z * inv, acc.w * inv);
+      *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + ((size_t)(tok0 + r / G) * a.heads + pair_kh * G + r % G) * HD + d) = pk;
+    }
+    if (a.weights) {
+      const int end = past + count;
+      const size_t at0 = ((size_t)(a.slots ? a.slots[seq] : seq) * a.kv_heads + pair_kh) * a.capacity;
+      const float* scores = reinterpret_cast<const float*>(smem + L.score_off);
+      for (int k = tid; k < my_pages * 64; k += THREADS) {
+        const int key = run.page(first_page + (k >> 6)) * 64 + (k & 63);
+        if (key >= end || key >= a.capacity) continue;
+        float w = key < past ? a.weights[at0 + key] : 0.0f, gained = 0.0f;
+        for (int r = 0; r < rows; ++r) {
+          const int pos = past + r / G;
+          const float d = reinterpret_cast<const float*>(smem + L.part_off + r * (HD * 4 + 16))[HD + 3];
+          if (sees(key, pos, window_lo(pos, a.window), a.first)) gained += few_ex2(scores[r * L.score_pitch + k] - d);
+        }
+        a.weights_out[at0 + key] = w + gained;
+      }
+      // rows that no query of the step sees: nothing is gathered
+      if (a.weights_out != a.weights)
+        for (int key = run.nf * 64 + rank * THREADS + tid; key < min(run.lo * 64, end); key += fa.cluster * THREADS)
+          if (key < a.capacity) a.weights_out[at0 + key] = a.weights[at0 + key];
+    }
+    __syncthreads();
+    cluster_sync_all();      // the others may still be reading this block's results
   }
 }
 
@@ -585,11 +700,33 @@ static int few_row_tiles(int max_count, int G) { return max_count * G <= 16 ? 1 
 // Where the pieces of scratch lie, in floats.
 struct FewScratch {
   long long part, part_ml, info, lse2, scores, total, score_stride;
-  int max_tiles, blocks;
+  int max_tiles, blocks, cluster, cluster_pages;
 };
-static FewScratch few_scratch(long long tokens, int n_seqs, int max_count, int heads, int kv_heads, int head_dim, int max_keys, bool weights) {
+
+// Whether blocks of a cluster share each (sequence, kv head), and how many: then no second kernel and no scratch is needed (a chat's token on 17 pages:
+// 10.1 us by runs of units, TIME1 by clusters), but a cluster waits for its longest sequence alone, so only where all clusters run at once and
+// no block takes more than ten pages (8 KB of scores a row at most).
+static void few_cluster(int n_seqs, int max_count, int heads, int kv_heads, int head_dim, int max_keys, bool weights, int window, int first, FewScratch& f) {
+  const int G = heads / kv_heads, R = few_row_tiles(max_count, G);
+  f.cluster = f.cluster_pages = 0;
+  if (R > 2) return;
+  long long pages = (max_keys + 63) / 64;
+  if (window > 0) pages = std::min(pages, (long long)(window + max_count - 2) / 64 + 2 + (first + 63) / 64);
+  const long long pairs = (long long)n_seqs * kv_heads, resident = (long long)sm_count() * few_blocks_an_sm(R);
+  if (pairs > resident) return;
+  int c = 8;
+  while (c > 1 && (pairs * c > resident || c >= 2 * pages)) c /= 2;
+  const int each = (int)((pages + c - 1) / c);
+  if (each > 10 || few_layout(head_dim, R, max_count * G, each, weights).stages < std::min(2, each)) return;
+  f.cluster = c;
+  f.cluster_pages = each;
+}
+
+static FewScratch few_scratch(long long tokens, int n_seqs, int max_count, int heads, int kv_heads, int head_dim, int max_keys, bool weights, int window, int first) {
   FewScratch f{};
   const int G = heads / kv_heads, R = few_row_tiles(max_count, G);
+  few_cluster(n_seqs, max_count, heads, kv_heads, head_dim, max_keys, weights, window, first, f);
+  if (f.cluster) return f;
   f.max_tiles = (max_count * G + 16 * R - 1) / (16 * R);
   const long long units = (long long)n_seqs * kv_heads * f.max_tiles * ((max_keys + 63) / 64);
   const long long most = (long long)sm_count() * few_blocks_an_sm(R);
@@ -608,13 +745,25 @@ static FewScratch few_scratch(long long tokens, int n_seqs, int max_count, int h
 }
 
 template <int HD, int R>
+static int launch_few_cluster(const CUtensorMap& mk, const CUtensorMap& mv, const FewArgs& fa, cudaStream_t s) {
+  static std::atomic<unsigned long long> allowed;
+  const cudaError_t e = allow_shared((const void*)kept_few_kernel<HD, R, true>, few_room(R), allowed);
+  if (e != cudaSuccess) return fail(2, "attention_kept: cannot reserve shared memory: %s", cudaGetErrorString(e));
+  launch_clusters(false, (unsigned)fa.cluster, kept_few_kernel<HD, R, true>, dim3(fa.cluster * fa.k.kv_heads * fa.k.n_seqs), dim3((few_warps(R) + 1) * 32),
+                  (size_t)fa.lay.total, s, mk, mv, fa);
+  return check_launch("attention_kept (few tokens, clusters)");
+}
+
+template <int HD, int R>
 static int launch_few(const CUtensorMap& mk, const CUtensorMap& mv, FewArgs fa, int blocks, int max_keys, int max_count, cudaStream_t s) {
   const int rows = max_count * (fa.k.heads / fa.k.kv_heads);
-  fa.lay = few_layout(HD, R, rows);
+  fa.lay = few_layout(HD, R, rows, fa.cluster_pages, fa.k.weights != nullptr);
+  if constexpr (R <= 2)
+    if (fa.cluster) return launch_few_cluster<HD, R>(mk, mv, fa, s);
   static std::atomic<unsigned long long> allowed;
-  const cudaError_t e = allow_shared((const void*)kept_few_kernel<HD, R>, few_room(R), allowed);
+  const cudaError_t e = allow_shared((const void*)kept_few_kernel<HD, R, false>, few_room(R), allowed);
   if (e != cudaSuccess) return fail(2, "attention_kept: cannot reserve shared memory: %s", cudaGetErrorString(e));
-  launch(kept_few_kernel<HD, R>, dim3(blocks), dim3((few_warps(R) + 1) * 32), (size_t)fa.lay.total, s, mk, mv, fa);
+  launch(kept_few_kernel<HD, R, false>, dim3(blocks), dim3((few_warps(R) + 1) * 32), (size_t)fa.lay.total, s, mk, mv, fa);
   const int rc = check_launch("attention_kept (few tokens)");
   if (rc) return rc;
   const long long pairs = (long long)fa.k.n_seqs * fa.k.kv_heads;
@@ -648,7 +797,9 @@ bool kept_few_takes(long long tokens, int max_count, int heads, int kv_heads, in
 }
 
 long long kept_few_floats(long long tokens, int n_seqs, int max_count, int heads, int kv_heads, int head_dim, int max_keys, bool weights) {
-  return few_scratch(tokens, n_seqs, max_count, heads, kv_heads, head_dim, max_keys, weights).total;
+  // (asked without the window: what a step without one takes is enough for every other, by runs of units or by clusters)
+  FewScratch runs = few_scratch(tokens, n_seqs, max_count, heads, kv_heads, head_dim, max_keys, weights, 0, 0);
+  return runs.total;
 }
 
 int kept_few(const KeptArgs& a, long long tokens, int max_count, int max_keys, long long pool_pages, int* status, cudaStream_t s) {
@@ -661,17 +812,19 @@ int kept_few(const KeptArgs& a, long long tokens, int max_count, int max_keys, l
   if (rc == 0) rc = encode_pool(&mv, a.v_pool, pool_pages * a.kv_heads * 64, a.head_dim, "the value pool");
   if (rc) return rc;
   const bool weights = a.weights != nullptr;
-  const FewScratch f = few_scratch(tokens, a.n_seqs, max_count, a.heads, a.kv_heads, a.head_dim, max_keys, weights);
+  const FewScratch f = few_scratch(tokens, a.n_seqs, max_count, a.heads, a.kv_heads, a.head_dim, max_keys, weights, a.window, a.first);
   FewArgs fa{};
   fa.k = a;
   fa.scale_log2 = a.scale * kKeptLog2e;
   fa.max_tiles = f.max_tiles;
   fa.max_count = max_count;
+  fa.cluster = f.cluster;
+  fa.cluster_pages = f.cluster_pages;
   fa.part = a.scratch + f.part;
   fa.part_ml = a.scratch + f.part_ml;
   fa.info = reinterpret_cast<int2*>(a.scratch + f.info);
-  fa.lse2 = weights ? a.scratch + f.lse2 : nullptr;
-  fa.scores = weights ? a.scratch + f.scores : nullptr;
+  fa.lse2 = weights && !f.cluster ? a.scratch + f.lse2 : nullptr;
+  fa.scores = weights && !f.cluster ? a.scratch + f.scores : nullptr;
   fa.score_stride = f.score_stride;
   fa.status = status;
   const int R = few_row_tiles(max_count, a.heads / a.kv_heads);

@@ -91,6 +91,8 @@ kept_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   pdl_wait();
   const int count = a.counts[seq], past = a.past[seq], end = past + count;
   if (count <= 0 || key0 >= end) return;       // (the whole cluster)
+  // that all blocks of the cluster have begun is waited for before the first store into another's shared memory
+  if (ranks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   const size_t tok0 = a.seq_start[seq];
   const int last = min(end, key0 + kKwKeys) - 1;
   const int t_lo = max(0, key0 - past);
@@ -272,10 +274,13 @@ kept_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     total = (p[0] + p[kKwKeys]) + (p[2 * kKwKeys] + p[3 * kKwKeys]);
   }
   if (ranks > 1) {
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     if (tid < kKwKeys) {
       const uint32_t to = cluster_map(base + L::RANK_OFF + (rank * kKwKeys + tid) * 4, 0);
       asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(total) : "memory");
     }
+    __syncthreads();
     cluster_sync_all();
     if (rank != 0) return;
     if (tid < kKwKeys) {

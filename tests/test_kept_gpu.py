@@ -322,8 +322,8 @@ def test_refusals():
                dict(weights=w, weights_out=w[:, :, :-1].contiguous()), dict(slots=t["past"].long()), dict(v_pool=t["v"].transpose(1, 2))):
         with pytest.raises(ValueError):
             call(**kw)
-    with pytest.raises(RuntimeError):
-        call(weights=w, scratch=None)
+    with pytest.raises(RuntimeError):       # (float32 keeps the denominators in scratch, whatever the step)
+        call(weights=w, scratch=None, q=t["q"].float(), out=out.float(), k_pool=t["k"].float(), v_pool=t["v"].float())
     with pytest.raises(RuntimeError):
         call(q=t["q"][:, :3].contiguous(), heads=3, out=out[:, :192].contiguous())
     pos = torch.zeros((1, 2, step.stride * 64), dtype=torch.int32, device=DEV)
