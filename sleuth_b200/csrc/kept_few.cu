@@ -273,7 +273,10 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         *reinterpret_cast<uint4*>(smem + L.q_off + tile_at<ROWS>(r, col)) = v;
       }
       sync();
-      uint32_t qf[HD / 16][4];
+      // (with 64 rows the fragments are read anew for every page: held they push others out of 168 registers, four turns of 3 to 13 tokens 31.0 us against 29.8)
+      constexpr bool HOLD = R != 4;
+      uint32_t qf[HOLD ? HD / 16 : 1][4];
+      if constexpr (HOLD)
 #pragma unroll
       for (int kb = 0; kb < HD / 16; ++kb) ldmatrix_x4(qf[kb], base + L.q_off + tile_at<ROWS>(rt * 16 + (lane & 15), kb * 16 + ((lane >> 4) << 3)));
       int pos[2], lo[2];
@@ -310,12 +313,14 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
           for (int j = 0; j < 2 * KB; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
 #pragma unroll
           for (int kb = 0; kb < HD / 16; ++kb) {
+            if constexpr (!HOLD) ldmatrix_x4(qf[0], base + L.q_off + tile_at<ROWS>(rt * 16 + (lane & 15), kb * 16 + ((lane >> 4) << 3)));
+            const uint32_t (&q)[4] = qf[HOLD ? kb : 0];
 #pragma unroll
             for (int b = 0; b < KB; ++b) {
               uint32_t kf[4];
               ldmatrix_x4(kf, kS + tile_at<64>(key_in + b * 16 + (lane & 7) + ((lane >> 4) << 3), kb * 16 + (((lane >> 3) & 1) << 3)));
-              mma_bf16(s[2 * b], qf[kb], kf[0], kf[1]);
-              mma_bf16(s[2 * b + 1], qf[kb], kf[2], kf[3]);
+              mma_bf16(s[2 * b], q, kf[0], kf[1]);
+              mma_bf16(s[2 * b + 1], q, kf[2], kf[3]);
             }
           }
           const bool whole = key0 + KW - 1 <= all_hi && (key0 >= all_lo || key0 + KW <= a.first);
@@ -704,7 +709,7 @@ struct FewScratch {
 };
 
 // Whether blocks of a cluster share each (sequence, kv head), and how many: then no second kernel and no scratch is needed (a chat's token on 17 pages:
-// 10.1 us by runs of units, TIME1 by clusters), but a cluster waits for its longest sequence alone, so only where all clusters run at once and
+// 10.1 us by runs of units, 7.9 by clusters; eight tokens on 2,049 rows 19.4 / 15.6), but a cluster waits for its longest sequence alone, so only where all clusters run at once and
 // no block takes more than ten pages (8 KB of scores a row at most).
 static void few_cluster(int n_seqs, int max_count, int heads, int kv_heads, int head_dim, int max_keys, bool weights, int window, int first, FewScratch& f) {
   const int G = heads / kv_heads, R = few_row_tiles(max_count, G);
