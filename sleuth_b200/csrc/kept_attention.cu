@@ -5,17 +5,20 @@
 //   weights_out[j] = (weights[j] where row j was there before the step, else 0) + sum over the step's queries, and over the query heads
 //                    of the key/value head, of exp(scale q . k_j - lse)
 //
-// A block of the first kernel takes 16 rows (row r is token r / G, query head r % G of the group) of one (sequence, kv head) and a share
-// of the keys that some of them sees, 64 at a time: keys as float32 in shared memory, a thread a key and four rows; one pass with a running
-// maximum and sum per row; values the same way, a thread four channels. Rows that are seen come in two runs, the first ones and the
-// window; keys between them are not read. Shares are joined by a second kernel, in order. A key that a row does not see is left out of its sum,
-// not multiplied by zero, so what lies in such a row of the pool (infinities, NaN) never reaches it.
+// Few rows (up to 16 of a sequence and kv head): a block takes 16 rows (row r is token r / G, query head r % G of the group) and a share of the keys
+// that some of them sees, 64 at a time, keys as float32 in shared memory, a thread a key and four rows. Many rows: tiles of 64 rows, a thread 4 x 4
+// scores, so that eight 16-byte reads of shared memory feed 64 FMAs. Both make one pass with a running maximum and sum per row; values come the
+// same way. Rows that are seen come in two runs, the first ones and the window; keys between them are not read. Shares are joined by a second
+// kernel, in order. A key that a row does not see is left out of its sum, not multiplied by zero, so what lies in such a row of the pool
+// (infinities, NaN) never reaches it.
 // The weights need the finished denominators, so their kernel forms the scores again: a block takes 64 keys of one (sequence, kv head)
-// and walks over the rows that see some of them, a thread a key; every sum has one order, and no two blocks add to the same place.
+// and walks over the rows that see some of them, 64 at a time, a thread 4 x 4 scores; where such blocks are few a cluster shares the rows and its first
+// block adds the sums in the order of the ranks. Every sum has one order, and no two blocks add to the same place.
 // Bound by the FMA pipe and shared memory.
 #include <math.h>
 
 #include "kept.cuh"
+#include "tcgen05.cuh"      // clusters
 
 namespace slb {
 
@@ -34,41 +37,71 @@ struct KeyRun {
   __device__ __forceinline__ int key(int v) const { return v < nf ? v : lo + v - nf; }
 };
 
-// 64 rows of a pool as float32 in shared memory, rows of hdp + 4 floats (16-byte reads of 8 lanes then meet 32 banks). Rows beyond the
-// run are zeros.
+// Four channels of a row as float32; `whole`: rows start where 16 bytes (bfloat16: 8) may be read at once, and end with a whole group of four.
+template <typename T>
+__device__ __forceinline__ float4 load_quad(const T* src, int left, bool whole) {
+  if constexpr (sizeof(T) == 4) {
+    if (whole) return *reinterpret_cast<const float4*>(src);
+  } else if (whole) {
+    const uint2 p = *reinterpret_cast<const uint2*>(src);
+    const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&p.x)), b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&p.y));
+    return make_float4(a.x, a.y, b.x, b.y);
+  }
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  v.x = to_f32(src[0]);
+  if (left > 1) v.y = to_f32(src[1]);
+  if (left > 2) v.z = to_f32(src[2]);
+  if (left > 3) v.w = to_f32(src[3]);
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ bool whole_quads(const T* base, int hd) { return hd % 4 == 0 && (reinterpret_cast<uintptr_t>(base) & (4 * sizeof(T) - 1)) == 0; }
+
+// 64 rows of a pool as float32 in shared memory, rows of hdp + 4 floats (16-byte reads of 8 lanes then meet 32 banks); zeros beyond the run. Sixteen
+// threads a row and four rows a thread: no division, and a thread's loads are under way together.
 template <typename T>
 __device__ __forceinline__ void load_rows(float* dst, const T* pool, const KeptArgs& a, const int* table, int kh, const KeyRun& run, int v0, int v1) {
-  const int hd = a.head_dim, hdp = padded_dim(hd);
-  for (int e = threadIdx.x; e < kGenKeys * (hdp / 2); e += kGenThreads) {
-    const int r = e / (hdp / 2), c = (e - r * (hdp / 2)) * 2;
-    float x = 0.0f, y = 0.0f;
-    if (v0 + r < v1 && c < hd) {
-      const int key = run.key(v0 + r);
-      const size_t row = ((size_t)table[key / kPageTokens] * a.kv_heads + kh) * kPageTokens + key % kPageTokens;
-      const T* src = pool + row * hd + c;
-      if constexpr (sizeof(T) == 4) {
-        const float2 p = *reinterpret_cast<const float2*>(src);
-        x = p.x;
-        y = p.y;
-      } else {
-        const float2 p = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(src));
-        x = p.x;
-        y = p.y;
-      }
+  const int hd = a.head_dim, hdp = padded_dim(hd), r0 = threadIdx.x >> 4;
+  const bool whole = whole_quads(pool, hd);
+  const T* src[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int v = v0 + r0 + 16 * i;
+    src[i] = nullptr;
+    if (v < v1) {
+      const int key = run.key(v);
+      src[i] = pool + (((size_t)table[key / kPageTokens] * a.kv_heads + kh) * kPageTokens + key % kPageTokens) * hd;
     }
-    *reinterpret_cast<float2*>(dst + r * (hdp + 4) + c) = make_float2(x, y);
+  }
+#pragma unroll 2
+  for (int c = 4 * (threadIdx.x & 15); c < hdp; c += 64) {
+    float4 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = src[i] ? load_quad(src[i] + c, hd - c, whole) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(dst + (r0 + 16 * i) * (hdp + 4) + c) = x[i];
   }
 }
 
 // ROWS rows of queries, times the scale, zeros behind the last row.
 template <typename T, int ROWS>
-__device__ __forceinline__ void load_queries(float* dst, const KeptArgs& a, size_t token0, int kh, int G, int r0, int rows_total) {
-  const int hd = a.head_dim, hdp = padded_dim(hd);
-  for (int e = threadIdx.x; e < ROWS * hdp; e += kGenThreads) {
-    const int r = e / hdp, c = e - r * hdp, R = r0 + r;
-    float v = 0.0f;
-    if (R < rows_total && c < hd) v = to_f32(((const T*)a.q)[((token0 + R / G) * a.heads + kh * G + R % G) * hd + c]) * a.scale;
-    dst[e] = v;
+__device__ __forceinline__ void load_queries(float* dst, const KeptArgs& a, size_t token0, int kh, int G, int r0, int rows_total, int pitch) {
+  const int hd = a.head_dim, hdp = padded_dim(hd), first = threadIdx.x >> 4;
+  const bool whole = whole_quads((const T*)a.q, hd);
+  const T* src[ROWS / 16];
+#pragma unroll
+  for (int i = 0; i < ROWS / 16; ++i) {
+    const int R = r0 + first + 16 * i;
+    src[i] = R < rows_total ? (const T*)a.q + ((token0 + R / G) * a.heads + kh * G + R % G) * hd : nullptr;
+  }
+#pragma unroll 2
+  for (int c = 4 * (threadIdx.x & 15); c < hdp; c += 64) {
+    float4 x[ROWS / 16];
+#pragma unroll
+    for (int i = 0; i < ROWS / 16; ++i) x[i] = src[i] ? load_quad(src[i] + c, hd - c, whole) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < ROWS / 16; ++i)
+      *reinterpret_cast<float4*>(dst + (first + 16 * i) * pitch + c) = make_float4(x[i].x * a.scale, x[i].y * a.scale, x[i].z * a.scale, x[i].w * a.scale);
   }
 }
 
@@ -117,7 +150,7 @@ __global__ void __launch_bounds__(kGenThreads) kept_general_kernel(KeptArgs a, l
   const int steps = (run.total + kGenKeys - 1) / kGenKeys, per = (steps + a.splits - 1) / a.splits;
   const int v_begin = split * per * kGenKeys, v_end = min(run.total, v_begin + per * kGenKeys);
 
-  load_queries<T, kGenRows>(q_s, a, token0, kh, G, r0, rows_total);
+  load_queries<T, kGenRows>(q_s, a, token0, kh, G, r0, rows_total, hdp);
   const int key_i = tid & 63, rg = tid >> 6;             // scores: a key, rows 4 rg .. 4 rg + 3
   int row_pos[4], row_lo[4];
 #pragma unroll
@@ -220,6 +253,210 @@ __global__ void __launch_bounds__(kGenThreads) kept_general_kernel(KeptArgs a, l
   }
 }
 
+// Scores of 64 rows and 64 keys: rows 4 ry .. + 3, keys kx + 16 j; q_s and rows_s in rows of hdp + 4 floats.
+__device__ __forceinline__ void dots_tile(const float* rows_s, const float* q_s, int hdp, int kx, int ry, float (&s)[4][4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[i][j] = 0.0f;
+  const float* k0 = rows_s + kx * (hdp + 4);
+  const float* q0 = q_s + 4 * ry * (hdp + 4);
+#pragma unroll 2
+  for (int c = 0; c < hdp; c += 4) {
+    float4 k[4], q[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) k[j] = *reinterpret_cast<const float4*>(k0 + 16 * j * (hdp + 4) + c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const float4*>(q0 + i * (hdp + 4) + c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[i][j] = fmaf(q[i].x, k[j].x, s[i][j]);
+        s[i][j] = fmaf(q[i].y, k[j].y, s[i][j]);
+        s[i][j] = fmaf(q[i].z, k[j].z, s[i][j]);
+        s[i][j] = fmaf(q[i].w, k[j].w, s[i][j]);
+      }
+  }
+}
+
+constexpr int kTileRows = 64, kTilePitch = kGenKeys + 4;
+__host__ __device__ constexpr int tile_smem(int hd) { return (2 * 64 * (padded_dim(hd) + 4) + kTileRows * kTilePitch + 2 * kTileRows) * 4; }
+
+// Tiles of 64 rows. CH: groups of 64 channels.
+template <typename T, int CH>
+__global__ void __launch_bounds__(kGenThreads, CH <= 2 ? 2 : 1) kept_tile_kernel(KeptArgs a, long long tokens) {
+  pdl_enter();
+  extern __shared__ __align__(16) float smem[];
+  const int hd = a.head_dim, hdp = padded_dim(hd);
+  float* rows_s = smem;                                  // [64][hdp + 4]
+  float* q_s = rows_s + kGenKeys * (hdp + 4);            // [64][hdp + 4]
+  float* p_s = q_s + kTileRows * (hdp + 4);              // [64][68]
+  float* alpha_s = p_s + kTileRows * kTilePitch;         // [64]
+  float* l_s = alpha_s + kTileRows;                      // [64]
+  const int tid = threadIdx.x, kx = tid & 15, ry = tid >> 4;
+  // the longest walks first: tiles of the highest rows of all sequences and heads
+  const int seq = blockIdx.x % a.n_seqs, kh = blockIdx.y, G = a.heads / a.kv_heads;
+  const int tiles = gridDim.x / a.n_seqs / a.splits, part = blockIdx.x / a.n_seqs;
+  const int tile = tiles - 1 - part / a.splits, split = part % a.splits;
+  const int count = a.counts[seq], past = a.past[seq], rows_total = count * G, r0 = tile * kTileRows;
+  if (r0 >= rows_total) return;
+  const size_t token0 = a.seq_start[seq];
+  const int* table = a.block_table + (size_t)seq * a.table_stride;
+  const int pos_first = past + r0 / G, pos_last = past + min(rows_total - 1, r0 + kTileRows - 1) / G;
+  const KeyRun run(pos_first, pos_last, a.window, a.first);
+  const int steps = (run.total + kGenKeys - 1) / kGenKeys, per = (steps + a.splits - 1) / a.splits;
+  const int v_begin = split * per * kGenKeys, v_end = min(run.total, v_begin + per * kGenKeys);
+  const int all_lo = window_lo(pos_last, a.window);      // keys from here to pos_first, and the first ones, are seen by every row
+
+  load_queries<T, kTileRows>(q_s, a, token0, kh, G, r0, rows_total, hdp + 4);
+  int row_pos[4], row_lo[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int R = r0 + 4 * ry + i;
+    row_pos[i] = R < rows_total ? past + R / G : -1;
+    row_lo[i] = window_lo(row_pos[i], a.window);
+  }
+  float acc[4][CH][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int h = 0; h < CH; ++h) acc[i][h][0] = acc[i][h][1] = acc[i][h][2] = acc[i][h][3] = 0.0f;
+  float m = -INFINITY, l = 0.0f;                         // row tid / 4, its keys 16 (tid % 4) .. + 15
+  const int sr = tid >> 2, sq = tid & 3;
+  for (int v0 = v_begin; v0 < v_end; v0 += kGenKeys) {
+    __syncthreads();
+    load_rows<T>(rows_s, (const T*)a.k_pool, a, table, kh, run, v0, v_end);
+    __syncthreads();
+    const int k_first = run.key(v0), k_last = run.key(min(v0 + kGenKeys, v_end) - 1), n = min(kGenKeys, v_end - v0);
+    const bool whole = n == kGenKeys && k_last <= pos_first && (k_first >= all_lo || k_last < a.first) && r0 + kTileRows <= rows_total;
+    {
+      float s[4][4];
+      dots_tile(rows_s, q_s, hdp, kx, ry, s);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int c = kx + 16 * j, key = run.key(v0 + c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          p_s[(4 * ry + i) * kTilePitch + c] = whole || (v0 + c < v_end && sees(key, row_pos[i], row_lo[i], a.first)) ? s[i][j] : -INFINITY;
+      }
+    }
+    __syncthreads();
+    load_rows<T>(rows_s, (const T*)a.v_pool, a, table, kh, run, v0, v_end);
+    {
+      float4 x[4];
+      float* row = p_s + sr * kTilePitch + 16 * sq;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) x[g] = *reinterpret_cast<const float4*>(row + 4 * g);
+      float top = -INFINITY;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) top = fmaxf(top, fmaxf(fmaxf(x[g].x, x[g].y), fmaxf(x[g].z, x[g].w)));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const float m_new = fmaxf(m, top), use = m_new == -INFINITY ? 0.0f : m_new, alpha = expf(m - use);
+      float sum = 0.0f;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        x[g].x = expf(x[g].x - use); x[g].y = expf(x[g].y - use);
+        x[g].z = expf(x[g].z - use); x[g].w = expf(x[g].w - use);
+        sum += (x[g].x + x[g].y) + (x[g].z + x[g].w);
+        *reinterpret_cast<float4*>(row + 4 * g) = x[g];
+      }
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      l = l * alpha + sum;
+      m = m_new;
+      if (sq == 0) alpha_s[sr] = alpha;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float f = alpha_s[4 * ry + i];
+#pragma unroll
+      for (int h = 0; h < CH; ++h)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[i][h][c] *= f;
+    }
+    const float* v_at = rows_s + 4 * kx;
+    if (whole) {
+#pragma unroll 2
+      for (int j = 0; j < kGenKeys; j += 4) {
+        float4 p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = *reinterpret_cast<const float4*>(p_s + (4 * ry + i) * kTilePitch + j);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int h = 0; h < CH; ++h) {
+            if (64 * h + 4 * kx >= hdp) continue;
+            const float4 v = *reinterpret_cast<const float4*>(v_at + (j + u) * (hdp + 4) + 64 * h);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float w = u == 0 ? p[i].x : u == 1 ? p[i].y : u == 2 ? p[i].z : p[i].w;
+              acc[i][h][0] = fmaf(w, v.x, acc[i][h][0]);
+              acc[i][h][1] = fmaf(w, v.y, acc[i][h][1]);
+              acc[i][h][2] = fmaf(w, v.z, acc[i][h][2]);
+              acc[i][h][3] = fmaf(w, v.w, acc[i][h][3]);
+            }
+          }
+      }
+    } else {
+      for (int j = 0; j < n; ++j) {
+        float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = p_s[(4 * ry + i) * kTilePitch + j];
+#pragma unroll
+        for (int h = 0; h < CH; ++h) {
+          if (64 * h + 4 * kx >= hdp) continue;
+          const float4 v = *reinterpret_cast<const float4*>(v_at + j * (hdp + 4) + 64 * h);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (w[i] != 0.0f) {
+              acc[i][h][0] = fmaf(w[i], v.x, acc[i][h][0]);
+              acc[i][h][1] = fmaf(w[i], v.y, acc[i][h][1]);
+              acc[i][h][2] = fmaf(w[i], v.z, acc[i][h][2]);
+              acc[i][h][3] = fmaf(w[i], v.w, acc[i][h][3]);
+            }
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (sq == 0) {
+    l_s[sr] = l;
+    const int R = r0 + sr;
+    if (R < rows_total) {
+      const size_t token = token0 + R / G;
+      const int head = kh * G + R % G;
+      if (a.splits > 1) {
+        float* slot = share_slot(a, split, token, head, tokens);
+        slot[hd] = m;
+        slot[hd + 1] = l;
+      } else if (a.lse) {
+        a.lse[token * a.heads + head] = l == 0.0f ? -INFINITY : m + logf(l);
+      }
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = 4 * ry + i, R = r0 + r;
+    if (R >= rows_total) continue;
+    const size_t token = token0 + R / G;
+    const int head = kh * G + R % G;
+    const float inv = a.splits > 1 ? 1.0f : l_s[r] == 0.0f ? 0.0f : 1.0f / l_s[r];
+#pragma unroll
+    for (int h = 0; h < CH; ++h)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int ch = 64 * h + 4 * kx + c;
+        if (ch >= hd) continue;
+        if (a.splits > 1) share_slot(a, split, token, head, tokens)[ch] = acc[i][h][c];
+        else ((T*)a.out)[(token * a.heads + head) * hd + ch] = from_f32<T>(acc[i][h][c] * inv);
+      }
+  }
+}
+
 // The shares of one (token, head), in order; a thread a channel.
 template <typename T>
 __global__ void kept_join_kernel(KeptArgs a, long long tokens) {
@@ -241,7 +478,7 @@ __global__ void kept_join_kernel(KeptArgs a, long long tokens) {
   if (c == 0 && a.lse) a.lse[token * a.heads + head] = L == 0.0f ? -INFINITY : M + logf(L);
 }
 
-__host__ __device__ constexpr int weights_smem(int hd) { return (kGenKeys * (padded_dim(hd) + 4) + kGenWeightRows * (padded_dim(hd) + 1) + kGenThreads) * 4; }
+__host__ __device__ constexpr int weights_smem(int hd) { return ((kGenKeys + kGenWeightRows) * (padded_dim(hd) + 4) + kGenWeightRows + (16 + 8) * kGenKeys) * 4; }
 
 template <typename T>
 __global__ void __launch_bounds__(kGenThreads) kept_weights_general_kernel(KeptArgs a) {
@@ -249,54 +486,79 @@ __global__ void __launch_bounds__(kGenThreads) kept_weights_general_kernel(KeptA
   extern __shared__ __align__(16) float smem[];
   const int hd = a.head_dim, hdp = padded_dim(hd);
   float* rows_s = smem;                                  // [64][hdp + 4]
-  float* q_s = rows_s + kGenKeys * (hdp + 4);            // [64][hdp]
-  float* lse_s = q_s + kGenWeightRows * hdp;             // [64]
-  float* part_s = lse_s + kGenWeightRows;                // [4][64]
-  const int tid = threadIdx.x, key_i = tid & 63, rg = tid >> 6;
+  float* q_s = rows_s + kGenKeys * (hdp + 4);            // [64][hdp + 4]
+  float* lse_s = q_s + kGenWeightRows * (hdp + 4);       // [64]
+  float* part_s = lse_s + kGenWeightRows;                // [16 groups of rows][64]
+  float* rank_s = part_s + 16 * kGenKeys;                // [8 ranks][64] (the first block's)
+  const int tid = threadIdx.x, kx = tid & 15, ry = tid >> 4;
+  const int ranks = a.splits, rank = (int)cluster_ctarank();
   const int seq = blockIdx.z, kh = blockIdx.y, G = a.heads / a.kv_heads;
   const int count = a.counts[seq], past = a.past[seq], end = past + count;
-  const int key0 = blockIdx.x * kGenKeys, key = key0 + key_i;
-  if (count <= 0 || key0 >= end) return;
+  const int key0 = (int)(blockIdx.x / ranks) * kGenKeys;
+  if (count <= 0 || key0 >= end) return;                 // (the whole cluster)
   const size_t token0 = a.seq_start[seq];
   const int* table = a.block_table + (size_t)seq * a.table_stride;
   // the queries that see some key of the tile: from the tile's own rows on, and while the window reaches back to it (or all of them)
   const int last = min(end, key0 + kGenKeys) - 1;
   const int t_lo = max(0, key0 - past);
   const int t_hi = a.window > 0 && key0 >= a.first ? min(count - 1, last + a.window - 1 - past) : count - 1;
-  float sum = 0.0f;
+  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   if (t_lo <= t_hi) {
     KeyRun run(0, 0, 0, 0);
     run.lo = key0;       // 64 keys as they lie
     load_rows<T>(rows_s, (const T*)a.k_pool, a, table, kh, run, 0, last - key0 + 1);
     const int r_hi = (t_hi + 1) * G;
-    for (int r0 = t_lo * G; r0 < r_hi; r0 += kGenWeightRows) {
+    for (int r0 = t_lo * G + rank * kGenWeightRows; r0 < r_hi; r0 += ranks * kGenWeightRows) {
       __syncthreads();
-      load_queries<T, kGenWeightRows>(q_s, a, token0, kh, G, r0, r_hi);
+      load_queries<T, kGenWeightRows>(q_s, a, token0, kh, G, r0, r_hi, hdp + 4);
       if (tid < kGenWeightRows) {
         const int R = r0 + tid;
         lse_s[tid] = R < r_hi ? a.lse[(token0 + R / G) * a.heads + kh * G + R % G] : -INFINITY;
       }
       __syncthreads();
-      const int n = min(kGenWeightRows, r_hi - r0);
-      for (int q0 = 4 * rg; q0 < n; q0 += 16) {      // a thread's group of four rows, then the next but three
-        float s[4];
-        dots(rows_s + key_i * (hdp + 4), q_s + q0 * hdp, hdp, s);
+      float s[4][4];
+      dots_tile(rows_s, q_s, hdp, kx, ry, s);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int R = r0 + q0 + i, pos = R < r_hi ? past + R / G : -1;
-          const float d = lse_s[q0 + i];
-          if (sees(key, pos, window_lo(pos, a.window), a.first) && d != -INFINITY) sum += expf(s[i] - d);
-        }
+      for (int i = 0; i < 4; ++i) {
+        const int R = r0 + 4 * ry + i, pos = R < r_hi ? past + R / G : -1, lo = window_lo(pos, a.window);
+        const float d = lse_s[4 * ry + i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (sees(key0 + kx + 16 * j, pos, lo, a.first) && d != -INFINITY) sum[j] += expf(s[i][j] - d);
       }
     }
   }
-  part_s[tid] = sum;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) part_s[ry * kGenKeys + kx + 16 * j] = sum[j];
   __syncthreads();
+  float total = 0.0f;
+  if (tid < kGenKeys)
+#pragma unroll
+    for (int g = 0; g < 16; ++g) total += part_s[g * kGenKeys + tid];
+  if (ranks > 1) {
+    cluster_sync_all();      // (the first block has begun; whole warps come here)
+    if (tid < kGenKeys)
+      asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_map(smem_addr(rank_s + rank * kGenKeys + tid), 0)), "f"(total) : "memory");
+    __syncthreads();
+    cluster_sync_all();
+    if (rank != 0) return;
+    total = 0.0f;
+    if (tid < kGenKeys)
+      for (int i = 0; i < ranks; ++i) total += rank_s[i * kGenKeys + tid];
+  }
+  const int key = key0 + tid;
   if (tid < kGenKeys && key < end && key < a.capacity) {
     const size_t at = ((size_t)(a.slots ? a.slots[seq] : seq) * a.kv_heads + kh) * a.capacity + key;
-    const float before = key < past ? a.weights[at] : 0.0f;
-    a.weights_out[at] = before + ((part_s[tid] + part_s[64 + tid]) + (part_s[128 + tid] + part_s[192 + tid]));
+    a.weights_out[at] = (key < past ? a.weights[at] : 0.0f) + total;
   }
+}
+
+template <typename T>
+static int launch_join(const KeptArgs& a, long long tokens, cudaStream_t s) {
+  if (a.splits == 1) return 0;
+  launch_prefetching(kept_join_kernel<T>, dim3(a.heads, (unsigned)(tokens < 65535 ? tokens : 65535), (unsigned)((tokens + 65534) / 65535)),
+                     dim3((a.head_dim + 31) / 32 * 32), 0, s, a, tokens);
+  return check_launch("attention_kept (join)");
 }
 
 template <typename T, int RPT>
@@ -306,17 +568,32 @@ static int launch_general(const KeptArgs& a, int max_count, long long tokens, cu
   const cudaError_t e = allow_shared((const void*)kept_general_kernel<T, RPT>, general_smem(256), allowed);
   if (e != cudaSuccess) return fail(2, "attention_kept: cannot reserve shared memory: %s", cudaGetErrorString(e));
   const long long tiles = ((long long)max_count * G + kGenRows - 1) / kGenRows;
-  SLB_REQUIRE(tiles * a.splits < (1ll << 31), "attention_kept: too many tiles (%lld)", tiles);
   launch(kept_general_kernel<T, RPT>, dim3((unsigned)(tiles * a.splits), a.kv_heads, a.n_seqs), dim3(kGenThreads), smem, s, a, tokens);
-  int rc = check_launch("attention_kept (general kernel)");
-  if (rc || a.splits == 1) return rc;
-  launch_prefetching(kept_join_kernel<T>, dim3(a.heads, (unsigned)(tokens < 65535 ? tokens : 65535), (unsigned)((tokens + 65534) / 65535)),
-         dim3((a.head_dim + 31) / 32 * 32), 0, s, a, tokens);
-  return check_launch("attention_kept (join)");
+  const int rc = check_launch("attention_kept (general kernel)");
+  return rc ? rc : launch_join<T>(a, tokens, s);
 }
+
+template <typename T, int CH>
+static int launch_tiles(const KeptArgs& a, int max_count, long long tokens, cudaStream_t s) {
+  const int smem = tile_smem(a.head_dim), G = a.heads / a.kv_heads;
+  static std::atomic<unsigned long long> allowed;
+  const cudaError_t e = allow_shared((const void*)kept_tile_kernel<T, CH>, tile_smem(64 * CH), allowed);
+  if (e != cudaSuccess) return fail(2, "attention_kept: cannot reserve shared memory: %s", cudaGetErrorString(e));
+  const long long blocks = ((long long)max_count * G + kTileRows - 1) / kTileRows * a.splits * a.n_seqs;
+  SLB_REQUIRE(blocks < (1ll << 31), "attention_kept: too many tiles (%lld)", blocks);
+  launch(kept_tile_kernel<T, CH>, dim3((unsigned)blocks, a.kv_heads), dim3(kGenThreads), smem, s, a, tokens);
+  const int rc = check_launch("attention_kept (tiles)");
+  return rc ? rc : launch_join<T>(a, tokens, s);
+}
+
+// Tiles of 64 rows from 17 rows on.
+static int general_rows(int max_count, int G) { return (long long)max_count * G <= kGenRows ? kGenRows : kTileRows; }
 
 template <typename T>
 static int general(const KeptArgs& a, int max_count, long long tokens, cudaStream_t s) {
+  if (general_rows(max_count, a.heads / a.kv_heads) == kTileRows)
+    return a.head_dim <= 64 ? launch_tiles<T, 1>(a, max_count, tokens, s) : a.head_dim <= 128 ? launch_tiles<T, 2>(a, max_count, tokens, s)
+                                                                                             : launch_tiles<T, 4>(a, max_count, tokens, s);
   const int groups = kGenThreads / (padded_dim(a.head_dim) / 4);
   if (groups >= 16) return launch_general<T, 1>(a, max_count, tokens, s);
   if (groups >= 8) return launch_general<T, 2>(a, max_count, tokens, s);
@@ -324,20 +601,26 @@ static int general(const KeptArgs& a, int max_count, long long tokens, cudaStrea
 }
 
 template <typename T>
-static int general_weights(const KeptArgs& a, int max_keys, cudaStream_t s) {
+static int general_weights(KeptArgs a, int max_count, int max_keys, cudaStream_t s) {
   static std::atomic<unsigned long long> allowed;
   const cudaError_t e = allow_shared((const void*)kept_weights_general_kernel<T>, weights_smem(256), allowed);
   if (e != cudaSuccess) return fail(2, "attention_kept: cannot reserve shared memory: %s", cudaGetErrorString(e));
-  launch_prefetching(kept_weights_general_kernel<T>, dim3((max_keys + kGenKeys - 1) / kGenKeys, a.kv_heads, a.n_seqs), dim3(kGenThreads),
-         weights_smem(a.head_dim), s, a);
+  // blocks that share 64 keys: up to two an SM in all, and no more than there are steps of rows
+  const int tiles = (max_keys + kGenKeys - 1) / kGenKeys;
+  const long long blocks = (long long)tiles * a.kv_heads * a.n_seqs, steps = ((long long)max_count * (a.heads / a.kv_heads) + kGenWeightRows - 1) / kGenWeightRows;
+  a.splits = 1;
+  while (a.splits < 8 && a.splits < steps && blocks * a.splits < 2 * sm_count()) a.splits *= 2;
+  launch_clusters(pdl_mode() != 0, (unsigned)a.splits, kept_weights_general_kernel<T>, dim3(tiles * a.splits, a.kv_heads, a.n_seqs), dim3(kGenThreads),
+                  weights_smem(a.head_dim), s, a);
   return check_launch("attention_kept (weights, general kernel)");
 }
 
-// Shares of the keys: as many as give every SM about four blocks, of at least one step of 64 keys (a step takes a block 3 us, a share more takes
-// the joining kernel 0.1: five sequences of 33 to 700 rows in shares of 256 keys 20 us).
+// Shares of the keys: as many as give every SM about four blocks of 16 rows or two of 64, of at least one step of 64 keys (a step takes a block 3 us, a
+// share more takes the joining kernel 0.1: five sequences of 33 to 700 rows in shares of 256 keys 20 us).
 static int general_splits(int n_seqs, int max_count, int heads, int kv_heads, int max_keys) {
-  const long long tiles = ((long long)max_count * (heads / kv_heads) + kGenRows - 1) / kGenRows * kv_heads * n_seqs;
-  long long splits = 4ll * sm_count() / (tiles > 0 ? tiles : 1);
+  const int G = heads / kv_heads, rows = general_rows(max_count, G);
+  const long long tiles = ((long long)max_count * G + rows - 1) / rows * kv_heads * n_seqs;
+  long long splits = (rows == kGenRows ? 4ll : 2ll) * sm_count() / (tiles > 0 ? tiles : 1);
   const long long most = (max_keys + kGenKeys - 1) / kGenKeys;
   splits = splits < most ? splits : most;
   return splits < 1 ? 1 : splits > 64 ? 64 : (int)splits;
@@ -414,5 +697,5 @@ extern "C" int slb_attention_kept(const void* q, const void* k_pool, const void*
   a.splits = general_splits(n_seqs, max_count, heads, kv_heads, max_keys);
   int rc = dtype == kF32 ? general<float>(a, max_count, tokens, s) : general<__nv_bfloat16>(a, max_count, tokens, s);
   if (rc || !gather) return rc;
-  return dtype == kF32 ? general_weights<float>(a, max_keys, s) : general_weights<__nv_bfloat16>(a, max_keys, s);
+  return dtype == kF32 ? general_weights<float>(a, max_count, max_keys, s) : general_weights<__nv_bfloat16>(a, max_count, max_keys, s);
 }
