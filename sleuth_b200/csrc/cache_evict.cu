@@ -362,12 +362,28 @@ extern "C" long long slb_cache_evict_scratch(int n_seqs, int kv_heads, int budge
   return (long long)n_seqs * kv_heads * (2ll * moves + 1);
 }
 
-// See the head of the file. weights, positions and their targets [slots, kv_heads, capacity] (a target may be its source); pools
-// [pages, kv_heads, 64, row_bytes]; max_length: no sequence holds more rows (0: as many as its table takes).
-extern "C" int slb_cache_evict(const float* weights, float* weights_out, const int* positions, int* positions_out, long long capacity,
-                               void* k_pool, void* v_pool, const int* block_table, int table_stride, int n_seqs, int kv_heads, int row_bytes,
-                               const int* past, const int* lengths, const int* seen, const int* slots, int budget, int first, int recent,
-                               int max_length, int* scratch, long long scratch_words, void* stream) {
+// What a caller says, in one piece of memory (as KeptCall, kept.cuh).
+struct EvictCall {
+  const float* weights;                 // [slots, kv_heads, capacity]; a target may be its source
+  float* weights_out;
+  const int* positions;
+  int* positions_out;
+  void *k_pool, *v_pool;                // [pages, kv_heads, 64, row_bytes]
+  const int *block_table, *past, *lengths, *seen, *slots;
+  int* scratch;
+  void* stream;
+  long long capacity, scratch_words;
+  int table_stride, n_seqs, kv_heads, row_bytes, budget, first, recent, max_length;
+};
+static_assert(sizeof(EvictCall) == 13 * 8 + 2 * 8 + 8 * 4, "as packed in kernels/ops.py");
+
+// See the head of the file. max_length: no sequence holds more rows (0: as many as its table takes).
+extern "C" int slb_cache_evict(const EvictCall* call) {
+  SLB_REQUIRE(call != nullptr, "cache_evict: no call");
+  const EvictCall c = *call;
+  const int table_stride = c.table_stride, n_seqs = c.n_seqs, kv_heads = c.kv_heads, row_bytes = c.row_bytes, budget = c.budget, first = c.first, recent = c.recent;
+  const long long capacity = c.capacity;
+  int max_length = c.max_length;
   SLB_REQUIRE(n_seqs >= 0 && kv_heads > 0 && row_bytes > 0 && row_bytes % 4 == 0 && table_stride > 0 && capacity > 0 && n_seqs < 65536 && kv_heads < 65536,
               "cache_evict: n_seqs=%d kv_heads=%d row_bytes=%d table_stride=%d", n_seqs, kv_heads, row_bytes, table_stride);
   SLB_REQUIRE(budget > 0 && first >= 0 && recent >= 0 && (long long)first + recent <= budget,
@@ -377,27 +393,27 @@ extern "C" int slb_cache_evict(const float* weights, float* weights_out, const i
   if (max_length <= 0 || max_length > table_rows) max_length = (int)(table_rows < 0x7fffffffll ? table_rows : 0x7fffffffll);
   if (max_length > capacity) max_length = (int)capacity;
   const long long need = slb_cache_evict_scratch(n_seqs, kv_heads, budget, max_length);
-  SLB_REQUIRE(need == 0 || (scratch != nullptr && scratch_words >= need), "cache_evict: the step needs %lld words of scratch, %lld were given", need,
-              scratch ? scratch_words : 0ll);
+  SLB_REQUIRE(need == 0 || (c.scratch != nullptr && c.scratch_words >= need), "cache_evict: the step needs %lld words of scratch, %lld were given", need,
+              c.scratch ? c.scratch_words : 0ll);
   EvictArgs a{};
-  a.weights = weights; a.weights_out = weights_out; a.positions = positions; a.positions_out = positions_out; a.capacity = capacity;
-  a.k_pool = (char*)k_pool; a.v_pool = (char*)v_pool; a.block_table = block_table; a.past = past; a.lengths = lengths; a.seen = seen;
-  a.slots = slots; a.scratch = need ? scratch : nullptr; a.table_stride = table_stride; a.n_seqs = n_seqs; a.kv_heads = kv_heads;
+  a.weights = c.weights; a.weights_out = c.weights_out; a.positions = c.positions; a.positions_out = c.positions_out; a.capacity = capacity;
+  a.k_pool = (char*)c.k_pool; a.v_pool = (char*)c.v_pool; a.block_table = c.block_table; a.past = c.past; a.lengths = c.lengths; a.seen = c.seen;
+  a.slots = c.slots; a.scratch = need ? c.scratch : nullptr; a.table_stride = table_stride; a.n_seqs = n_seqs; a.kv_heads = kv_heads;
   a.row_bytes = row_bytes; a.budget = budget; a.first = first; a.recent = recent; a.max_length = max_length;
   a.most_moves = most_moves(budget, max_length);
   a.keys_fit = max_length <= kMostKeysShared;
-  a.vector = row_bytes % 16 == 0 && (uintptr_t)k_pool % 16 == 0 && (uintptr_t)v_pool % 16 == 0;
-  if (few_go(budget, max_length)) return launch_evict_few(a, (cudaStream_t)stream);
+  a.vector = row_bytes % 16 == 0 && (uintptr_t)c.k_pool % 16 == 0 && (uintptr_t)c.v_pool % 16 == 0;
+  if (few_go(budget, max_length)) return launch_evict_few(a, (cudaStream_t)c.stream);
   const int smem = a.keys_fit ? max_length * 4 : 0;
   static std::atomic<unsigned long long> allowed;
   // few moves are made by the block that found them: a second kernel costs 3 us, 64 rows of 512 bytes a block less than one
   a.moves_here = a.most_moves * (long long)row_bytes <= 32 * 1024;
   if (max_length <= 2048) {      // small blocks, so that many share an SM
-    launch(cache_evict_kernel<256>, dim3(kv_heads, n_seqs), dim3(256), smem, (cudaStream_t)stream, a);
+    launch(cache_evict_kernel<256>, dim3(kv_heads, n_seqs), dim3(256), smem, (cudaStream_t)c.stream, a);
   } else {
     const cudaError_t e = allow_shared((const void*)cache_evict_kernel<kEvictThreads>, kMostKeysShared * 4, allowed);
     if (e != cudaSuccess) return fail(2, "cache_evict: cannot reserve shared memory: %s", cudaGetErrorString(e));
-    launch(cache_evict_kernel<kEvictThreads>, dim3(kv_heads, n_seqs), dim3(kEvictThreads), smem, (cudaStream_t)stream, a);
+    launch(cache_evict_kernel<kEvictThreads>, dim3(kv_heads, n_seqs), dim3(kEvictThreads), smem, (cudaStream_t)c.stream, a);
   }
   const int rc = check_launch("cache_evict");
   if (rc || a.moves_here) return rc;
@@ -405,6 +421,6 @@ extern "C" int slb_cache_evict(const float* weights, float* weights_out, const i
   long long blocks = 8ll * sm_count() / pairs;
   const long long most = (a.most_moves + 15) / 16;
   blocks = blocks < 1 ? 1 : blocks < most ? blocks : most;
-  launch_prefetching(cache_move_kernel, dim3((unsigned)blocks, kv_heads, n_seqs), dim3(256), 0, (cudaStream_t)stream, a);
+  launch_prefetching(cache_move_kernel, dim3((unsigned)blocks, kv_heads, n_seqs), dim3(256), 0, (cudaStream_t)c.stream, a);
   return check_launch("cache_evict (moves)");
 }

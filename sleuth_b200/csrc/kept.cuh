@@ -31,6 +31,23 @@ struct KeptArgs {
   long long capacity;
 };
 
+// What a caller of slb_attention_kept says, in one piece of memory (thirty arguments cost a call through ctypes 4 us, one 1).
+struct KeptCall {
+  const void *q, *k_pool, *v_pool;      // [tokens, heads, head_dim]; [pool_pages, kv_heads, 64, head_dim]
+  void* out;                            // [tokens, heads * head_dim]
+  const int *seq_start, *past, *counts, *block_table;
+  float* lse;                           // [tokens, heads] or null
+  const int* slots;                     // [n_seqs] or null
+  const float* weights;                 // [slots, kv_heads, capacity]; with its target (the same memory or apart), or both null
+  float *weights_out, *scratch;
+  int* status;                          // a zeroed device word that receives a code if a bounded wait inside a kernel gave up
+  void* stream;
+  long long tokens, capacity, scratch_floats, pool_pages;
+  int table_stride, n_seqs, max_count, max_keys, heads, kv_heads, head_dim, window, first, dtype;
+  float scale;
+};
+static_assert(sizeof(KeptCall) == 15 * 8 + 4 * 8 + 11 * 4 + 4, "as packed in kernels/ops.py");
+
 // First row of the window of the query at row p.
 __host__ __device__ __forceinline__ int window_lo(int p, int window) { return window > 0 && p - window + 1 > 0 ? p - window + 1 : 0; }
 

@@ -654,48 +654,49 @@ extern "C" long long slb_attention_kept_scratch(long long tokens, int n_seqs, in
   return (weights ? tokens * heads : 0) + (splits > 1 ? (long long)splits * tokens * heads * (head_dim + 2) : 0);
 }
 
-// Attention of a step over a cache of bounded size (kept.cuh). Pools of pool_pages pages; lse [tokens, heads] float32 or null; weights and
-// weights_out [slots, kv_heads, capacity] float32 (the same memory or apart) or both null; slots [n_seqs] or null. max_keys: no sequence has
-// more rows after the step (0: as many as its table takes). Scratch as slb_attention_kept_scratch says. `status`: a zeroed device word that
-// receives a code if a bounded wait inside a kernel gave up.
-extern "C" int slb_attention_kept(const void* q, const void* k_pool, const void* v_pool, void* out, const int* seq_start, const int* past,
-                                  const int* counts, const int* block_table, int table_stride, int n_seqs, long long tokens, int max_count,
-                                  int max_keys, int heads, int kv_heads, int head_dim, int window, int first, float scale, float* lse,
-                                  const int* slots, const float* weights, float* weights_out, long long capacity, float* scratch,
-                                  long long scratch_floats, long long pool_pages, int* status, int dtype, void* stream) {
+// Attention of a step over a cache of bounded size (kept.cuh). max_keys: no sequence has more rows after the step (0: as many as its table
+// takes). Scratch as slb_attention_kept_scratch says.
+extern "C" int slb_attention_kept(const KeptCall* call) {
+  SLB_REQUIRE(call != nullptr, "attention_kept: no call");
+  const KeptCall c = *call;
+  const int n_seqs = c.n_seqs, max_count = c.max_count, heads = c.heads, kv_heads = c.kv_heads, head_dim = c.head_dim, window = c.window, first = c.first,
+            table_stride = c.table_stride, dtype = c.dtype;
+  const long long tokens = c.tokens;
+  const float scale = c.scale;
+  int max_keys = c.max_keys;
   SLB_REQUIRE(n_seqs >= 0 && tokens >= 0 && max_count >= 0 && heads > 0 && kv_heads > 0 && heads % kv_heads == 0,
               "attention_kept: n_seqs=%d heads=%d kv_heads=%d", n_seqs, heads, kv_heads);
   SLB_REQUIRE(head_dim > 0 && head_dim <= 256 && head_dim % 2 == 0, "attention_kept: head_dim %d is not supported (even, at most 256)", head_dim);
   SLB_REQUIRE(window >= 0 && first >= 0 && table_stride > 0, "attention_kept: window=%d first=%d table_stride=%d", window, first, table_stride);
   SLB_REQUIRE(dtype == kF32 || dtype == kBF16, "attention_kept: unknown dtype %d", dtype);
-  SLB_REQUIRE((weights == nullptr) == (weights_out == nullptr) && (weights == nullptr || capacity > 0), "attention_kept: weights and their target go together");
+  SLB_REQUIRE((c.weights == nullptr) == (c.weights_out == nullptr) && (c.weights == nullptr || c.capacity > 0), "attention_kept: weights and their target go together");
   SLB_REQUIRE(n_seqs < 65536 && kv_heads < 65536 && tokens < (1ll << 31), "attention_kept: n_seqs=%d tokens=%lld", n_seqs, tokens);
   if (n_seqs == 0 || tokens == 0 || max_count == 0) return 0;
   if (max_keys <= 0 || max_keys > table_stride * (long long)kPageTokens) {
     SLB_REQUIRE(table_stride < (1 << 25), "attention_kept: table_stride=%d", table_stride);
     max_keys = table_stride * kPageTokens;
   }
-  const bool gather = weights != nullptr;
+  const bool gather = c.weights != nullptr;
   const long long need = slb_attention_kept_scratch(tokens, n_seqs, max_count, heads, kv_heads, head_dim, max_keys, dtype, gather);
-  SLB_REQUIRE(need == 0 || (scratch != nullptr && scratch_floats >= need), "attention_kept: the step needs %lld floats of scratch, %lld were given",
-              need, scratch ? scratch_floats : 0ll);
+  SLB_REQUIRE(need == 0 || (c.scratch != nullptr && c.scratch_floats >= need), "attention_kept: the step needs %lld floats of scratch, %lld were given",
+              need, c.scratch ? c.scratch_floats : 0ll);
   KeptArgs a{};
-  a.q = q; a.k_pool = k_pool; a.v_pool = v_pool; a.out = out; a.seq_start = seq_start; a.past = past; a.counts = counts;
-  a.block_table = block_table; a.table_stride = table_stride; a.n_seqs = n_seqs; a.heads = heads; a.kv_heads = kv_heads;
-  a.head_dim = head_dim; a.window = window; a.first = window > 0 ? first : 0; a.scale = scale; a.slots = slots; a.weights = weights;
-  a.weights_out = weights_out; a.capacity = capacity; a.lse = lse; a.scratch = scratch;
-  const cudaStream_t s = (cudaStream_t)stream;
+  a.q = c.q; a.k_pool = c.k_pool; a.v_pool = c.v_pool; a.out = c.out; a.seq_start = c.seq_start; a.past = c.past; a.counts = c.counts;
+  a.block_table = c.block_table; a.table_stride = table_stride; a.n_seqs = n_seqs; a.heads = heads; a.kv_heads = kv_heads;
+  a.head_dim = head_dim; a.window = window; a.first = window > 0 ? first : 0; a.scale = scale; a.slots = c.slots; a.weights = c.weights;
+  a.weights_out = c.weights_out; a.capacity = c.capacity; a.lse = c.lse; a.scratch = c.scratch;
+  const cudaStream_t s = (cudaStream_t)c.stream;
   SLB_REQUIRE(scale > 0.0f, "attention_kept: the scale is positive, got %g", (double)scale);
   const int form = kept_form(tokens, max_count, heads, kv_heads, head_dim, max_keys, dtype, gather);
-  if (form == kKeptFew) return kept_few(a, tokens, max_count, max_keys, pool_pages, status, s);
+  if (form == kKeptFew) return kept_few(a, tokens, max_count, max_keys, c.pool_pages, c.status, s);
   if (form == kKeptTc) {
-    float* lse2 = gather ? scratch : nullptr;
-    const int rc = attention_tc_kept(a, lse2, tokens, max_count, max_keys, pool_pages, status, s);
-    return rc || !gather ? rc : kept_weights_tc(a, lse2, tokens, max_count, max_keys, pool_pages, status, s);
+    float* lse2 = gather ? c.scratch : nullptr;
+    const int rc = attention_tc_kept(a, lse2, tokens, max_count, max_keys, c.pool_pages, c.status, s);
+    return rc || !gather ? rc : kept_weights_tc(a, lse2, tokens, max_count, max_keys, c.pool_pages, c.status, s);
   }
-  if (gather && lse == nullptr) {
-    a.lse = scratch;
-    a.scratch = scratch + tokens * heads;
+  if (gather && c.lse == nullptr) {
+    a.lse = c.scratch;
+    a.scratch = c.scratch + tokens * heads;
   }
   a.splits = general_splits(n_seqs, max_count, heads, kv_heads, max_keys);
   int rc = dtype == kF32 ? general<float>(a, max_count, tokens, s) : general<__nv_bfloat16>(a, max_count, tokens, s);

@@ -17,7 +17,7 @@
 // order of the ranks.
 // Measured: a prompt of 6,000 tokens, 32 / 8 heads of 128, 180 us = 0.82 PFLOP/s (576 M scores; the powers of two alone would take 139 on their unit); four
 // earlier steps: two stages of 256 rows 333, three of eight powers on the FMA pipe 284, the ring of stages 228, 32 columns at a time 180. What bounds it:
-// the issue slots of the epilogue (63 % busy) and the waits between its stages; tensor cores 37 %, L2 23 % (profiles/kept_kernels.md).
+// the issue slots of the epilogue (63 % busy) and the waits between its stages; tensor cores 37 %, L2 23 %.
 #include <math.h>
 
 #include <algorithm>

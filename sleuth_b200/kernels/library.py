@@ -202,8 +202,8 @@ _SIGNATURES = {
     "slb_pair_combine": [P, P, P, P, F, F, F, P, L, I, I, P],
     "slb_row_gate": [P, P, P, P, L, I, I, I, I, P],
     "slb_qkv_post_rows": [P, P, P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, F, I, P],
-    "slb_attention_kept": [P, P, P, P, P, P, P, P, I, I, L, I, I, I, I, I, I, I, F, P, P, P, P, L, P, L, L, P, I, P],
-    "slb_cache_evict": [P, P, P, P, L, P, P, P, I, I, I, I, P, P, P, P, I, I, I, I, P, L, P],
+    "slb_attention_kept": [ctypes.c_char_p],
+    "slb_cache_evict": [ctypes.c_char_p],
 }
 
 

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 import torch
 
@@ -1717,6 +1718,10 @@ def _kept_refusal(what: str, tensors: dict, checks) -> None:
     _need(False, f"{what}: the arguments do not fit together")
 
 
+_KEPT_CALL = struct.Struct("15Q4q10if4x")    # KeptCall in csrc/kept.cuh (to its whole size)
+_EVICT_CALL = struct.Struct("13Q2q8i")       # EvictCall in csrc/cache_evict.cu
+
+
 def _plain_cuda(t) -> bool:
     return t is None or (t.is_cuda and t.is_contiguous())
 
@@ -1790,10 +1795,18 @@ def attention_kept(q, k_pool, v_pool, out, seq_start, past, counts, block_table,
             (lambda: slots is not None or weights.shape[0] >= n, "weights hold a row of every sequence"),
             (lambda: capacity >= (max_keys if 0 < max_keys <= 64 * stride else 64 * stride), "weights are shorter than the cache")))
     status = _TC_STATUS.get(q.device)
-    lib().call("slb_attention_kept", q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), seq_start.data_ptr(), past.data_ptr(),
-               counts.data_ptr(), block_table.data_ptr(), stride, n, T, int(max_count), int(max_keys), heads, kv_heads, head_dim, int(window), int(first), float(scale),
-               _p(lse), _p(slots), _p(weights), _p(weights_out), capacity, _p(scratch), 0 if scratch is None else scratch.numel(), k_shape[0],
-               (status if status is not None else _tc_status(q.device)).data_ptr(), DT[dt], stream if stream is not None else current_stream())
+    if status is None:
+        status = _tc_status(q.device)
+    try:
+        call = _KEPT_CALL.pack(q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), seq_start.data_ptr(), past.data_ptr(), counts.data_ptr(),
+                               block_table.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if slots is None else slots.data_ptr(),
+                               0 if weights is None else weights.data_ptr(), 0 if weights is None else weights_out.data_ptr(),
+                               0 if scratch is None else scratch.data_ptr(), status.data_ptr(), stream if stream is not None else current_stream(),
+                               T, capacity, 0 if scratch is None else scratch.numel(), k_shape[0], stride, n, max_count, max_keys, heads, kv_heads, head_dim,
+                               window, first, DT[dt], scale)
+    except struct.error as e:
+        raise ValueError(f"attention_kept: a number is out of range ({e})") from None
+    lib().call("slb_attention_kept", call)
 
 
 def cache_evict_scratch_words(n_seqs: int, kv_heads: int, budget: int, max_length: int) -> int:
@@ -1850,7 +1863,12 @@ def cache_evict(weights, positions, k_pool, v_pool, block_table, past, lengths, 
              "slots are int32, one a sequence; without them weights hold a row of every sequence"),
             (lambda: scratch is None or scratch.dtype == i32, "scratch is int32"),
             (lambda: budget > 0 and first >= 0 and recent >= 0 and first + recent <= budget, "first and recent rows fit the budget")))
-    lib().call("slb_cache_evict", weights.data_ptr(), weights_out.data_ptr(), positions.data_ptr(), positions_out.data_ptr(), w_shape[2],
-               k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(), stride, n, kv_heads, row_bytes, past.data_ptr(), lengths.data_ptr(),
-               seen.data_ptr(), _p(slots), int(budget), int(first), int(recent), int(max_length), _p(scratch), 0 if scratch is None else scratch.numel(),
-               stream if stream is not None else current_stream())
+    try:
+        call = _EVICT_CALL.pack(weights.data_ptr(), weights_out.data_ptr(), positions.data_ptr(), positions_out.data_ptr(), k_pool.data_ptr(),
+                                v_pool.data_ptr(), block_table.data_ptr(), past.data_ptr(), lengths.data_ptr(), seen.data_ptr(),
+                                0 if slots is None else slots.data_ptr(), 0 if scratch is None else scratch.data_ptr(),
+                                stream if stream is not None else current_stream(), w_shape[2], 0 if scratch is None else scratch.numel(), stride, n, kv_heads,
+                                row_bytes, budget, first, recent, max_length)
+    except struct.error as e:
+        raise ValueError(f"cache_evict: a number is out of range ({e})") from None
+    lib().call("slb_cache_evict", call)
