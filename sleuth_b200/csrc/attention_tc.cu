@@ -30,7 +30,7 @@
 // product) is what bounds a single long prompt; many sequences or heads fill the GPU.
 //
 // With KEPT the same kernels serve a cache of bounded size (kept.cuh): the pages of the first rows come before the window's, as one list (TilePages),
-// and the rows' denominators are left for the kernel that gathers weights. Measured there: a prompt of 6,000 tokens, 32 / 8 heads of 128, 303 us = 0.97
+// and the rows' denominators are left for the kernel that gathers weights. Measured there: a prompt of 6,000 tokens, 32 / 8 heads of 128, 285 us = 1.03
 // PFLOP/s; seven portions of 349 to 1,500 tokens on up to 3,000 rows, heads of 64, a window of 1,000 and 100 first rows, 182 us (20 pages a tile, of
 // which five run the mask); 2,048 tokens under a window of 512, 16 / 8 heads, 19 us, mostly a tile's way in and out (10 pages).
 //

@@ -9,19 +9,17 @@
 //     KB, takes about as long as its products, and arrives late with two;
 //   * warp 1, one lane: S^T = K Q^T (M = 128, N = 128) into one of four accumulators of 128 columns, all of tensor memory;
 //   * warp 2: the 128 denominators of a step into shared memory, asked for a step early;
-//   * warps 3 to 18: two sets of eight take the steps in turn, a warp 32 keys and 64 columns, a thread 64 scores, which it takes into registers at
-//     once so that the accumulator is free again. Per score one FMA, one power of two, one addition; three powers of eight are worked out on the
-//     FMA pipe, five cycles a score on either pipe. Only steps with a key that some row does not see run a mask, a range of columns for each key.
+//   * warps 3 to 18: two sets of eight take the steps in turn, a warp 32 keys and 64 columns, a thread 64 scores, 32 at a time. Per score one FMA,
+//     one power of two, one addition (in pairs). Only steps with a key that some row does not see run a mask, a range of columns for each key.
 // Clusters start in the order of their number: the first keys of all sequences and heads, whose walk is the longest, before the next ones. Where
 // blocks are too few for the SMs, a cluster shares a key tile: the steps are dealt to its blocks in turn, the first block adds the sums in the
 // order of the ranks.
-// Measured: a prompt of 6,000 tokens, 32 / 8 heads of 128, 180 us = 0.82 PFLOP/s (576 M scores; the powers of two alone would take 139 on their unit); four
-// earlier steps: two stages of 256 rows 333, three of eight powers on the FMA pipe 284, the ring of stages 228, 32 columns at a time 180. What bounds it:
-// the issue slots of the epilogue (63 % busy) and the waits between its stages; tensor cores 37 %, L2 23 %.
+// Measured: a prompt of 6,000 tokens, 32 / 8 heads of 128, 205 us = 0.72 PFLOP/s. What bounds it: the powers of two (576 M scores at 16 a cycle and SM: 139 us), then
+// the epilogue's waits between its stages; tensor cores 37 %. Tried: 256 queries a step with two stages of them 333 us; three powers of eight by a
+// polynomial on the FMA pipe 215, two of eight 201 (issue slots take what the unit gives back); 64 scores at once 211; 24 warps 201.
 #include <math.h>
 
 #include <algorithm>
-#include <type_traits>
 
 #include "kept.cuh"
 #include "packed_f32.cuh"
@@ -48,8 +46,7 @@ struct KwLayout {
   static constexpr int RANK_OFF = SUM_OFF + 4 * kKwKeys * 4;            // [8 ranks][128 keys] (the first block's)
   static constexpr int BAR_OFF = RANK_OFF + 8 * kKwKeys * 4;
   static constexpr int N_BARS = 1 + 2 * STAGES + 4 * kKwBuffers;
-  static constexpr int ODD_OFF = BAR_OFF + N_BARS * 8 + 8;              // [4] whether a denominator of the step is NaN or infinite
-  static constexpr int TOTAL = ODD_OFF + 4 * kKwBuffers;
+  static constexpr int TOTAL = BAR_OFF + N_BARS * 8 + 8;
   static_assert(TOTAL <= 226 * 1024, "the block must fit on an SM");
 };
 
@@ -57,22 +54,6 @@ __device__ __forceinline__ float kw_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-
-// 2^x for two x of at most a little above 0, on the FMA pipe: x = n + f with f in [-1/2, 1/2] (adding 1.5 * 2^23 leaves n in the low bits), 2^f
-// by the polynomial of degree 5 with the least largest relative error (7.5e-8, by the Remez exchange), n added to the exponent. Below
-// 2^-126 the result is 2^-126, nothing beside a weight that counts; NaN would come out as that too, so rows whose denominator is NaN or
-// infinite (any such score among the keys that they see makes it that) do not come here.
-__device__ __forceinline__ f32x2 kw_ex2_pair(f32x2 x) {
-  x = pair_of(fmaxf(low_half(x), -126.0f), fmaxf(high_half(x), -126.0f));
-  const f32x2 t = add2(x, both(12582912.0f)), f = fma2(add2(t, both(-12582912.0f)), both(-1.0f), x);
-  f32x2 p = fma2(f, both(0.0013276472454890609f), both(0.009675540961325169f));
-  p = fma2(p, f, both(0.05550713092088699f));
-  p = fma2(p, f, both(0.24022120237350464f));
-  p = fma2(p, f, both(0.6931469440460205f));
-  p = fma2(p, f, both(1.0000001192092896f));
-  return pair_of(__uint_as_float(__float_as_uint(low_half(p)) + (__float_as_uint(low_half(t)) << 23)),
-                 __uint_as_float(__float_as_uint(high_half(p)) + (__float_as_uint(high_half(t)) << 23)));
 }
 
 template <int HD>
@@ -196,11 +177,6 @@ kept_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           if (lane == 0) atomicExch(w.status, 89);
           break;
         }
-        bool odd = false;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) odd = odd || !(v[c] < INFINITY);
-        odd = __any_sync(0xffffffffu, odd);
-        if (lane == 0) reinterpret_cast<int*>(smem + L::ODD_OFF)[b] = odd;
         // the negative, to be added; a row without weight or behind the last gives none
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -227,8 +203,6 @@ kept_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
         }
         tc_fence_after();
         const bool masked = __any_sync(0xffffffffu, R0 < see_lo || R0 + 64 > see_hi);
-        const bool odd = reinterpret_cast<const int*>(smem + L::ODD_OFF)[b] != 0;
-        // 32 columns at a time: with 64 in registers the polynomial's constants are loaded anew for every use
 #pragma unroll
         for (int c0 = 0; c0 < 64; c0 += 32) {
           uint32_t sr[32];
@@ -244,19 +218,14 @@ kept_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
               if (R0 + c0 + c < see_lo || R0 + c0 + c >= see_hi) sr[c] = 0xff800000u;
           }
           const ulonglong2* dd = reinterpret_cast<const ulonglong2*>(d + b * kKwRows + col0 + c0);
-          auto add_up = [&](auto both_pipes) {
 #pragma unroll
-            for (int c = 0; c < 32; c += 4) {
-              const ulonglong2 n = dd[c >> 2];
-              const f32x2 x0 = fma2(pair_of(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), scale2, n.x);
-              const f32x2 x1 = fma2(pair_of(__uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3])), scale2, n.y);
-              // three pairs of eight by the polynomial: 5 cycles a score on either pipe where the powers of two alone take 8
-              s0 = add2(s0, pair_of(kw_ex2(low_half(x0)), kw_ex2(high_half(x0))));
-              s1 = add2(s1, (c >> 2) % 4 != 3 && decltype(both_pipes)::value ? kw_ex2_pair(x1) : pair_of(kw_ex2(low_half(x1)), kw_ex2(high_half(x1))));
-            }
-          };
-          if (odd) add_up(std::false_type());
-          else add_up(std::true_type());
+          for (int c = 0; c < 32; c += 4) {
+            const ulonglong2 n = dd[c >> 2];
+            const f32x2 x0 = fma2(pair_of(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), scale2, n.x);
+            const f32x2 x1 = fma2(pair_of(__uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3])), scale2, n.y);
+            s0 = add2(s0, pair_of(kw_ex2(low_half(x0)), kw_ex2(high_half(x0))));
+            s1 = add2(s1, pair_of(kw_ex2(low_half(x1)), kw_ex2(high_half(x1))));
+          }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(d_free + 8 * b);
