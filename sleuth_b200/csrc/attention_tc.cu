@@ -30,8 +30,8 @@
 // product) is what bounds a single long prompt; many sequences or heads fill the GPU.
 //
 // With KEPT the same kernels serve a cache of bounded size (kept.cuh): the pages of the first rows come before the window's, as one list (TilePages),
-// and the rows' denominators are left for the kernel that gathers weights. Measured there: a prompt of 6,000 tokens, 32 / 8 heads of 128, 285 us = 1.03
-// PFLOP/s; seven portions of 349 to 1,500 tokens on up to 3,000 rows, heads of 64, a window of 1,000 and 100 first rows, 182 us (20 pages a tile, of
+// and the rows' denominators are left for the kernel that gathers weights. Measured there: a prompt of 6,000 tokens, 32 / 8 heads of 128, 290 us = 1.02
+// PFLOP/s; seven portions of 349 to 1,500 tokens on up to 3,000 rows, heads of 64, a window of 1,000 and 100 first rows, 186 us (20 pages a tile, of
 // which five run the mask); 2,048 tokens under a window of 512, 16 / 8 heads, 19 us, mostly a tile's way in and out (10 pages).
 //
 // Every wait on an mbarrier is bounded; a wait that gives up writes a code into `status`, the thread stops waiting
@@ -40,6 +40,7 @@
 #include <math.h>
 
 #include "kept.cuh"
+#include "packed_f32.cuh"
 #include "tcgen05.cuh"
 
 namespace slb {
@@ -311,6 +312,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16);
     unsigned short* xch = reinterpret_cast<unsigned short*>(smem + L::XCH_OFF);     // [2 pages][2 halves][128 rows]
     float m_used = -INFINITY, l = 0.0f;
+    // KEPT: the sum of the weights as they are rounded for the product, by which the result is divided: what rounds the one key that a peaked row looks at
+    // then cancels (error against 64 bits 2.3e-3 -> 2.1e-3 for 2 per cent of the time); the denominator that others get is the sum of the weights themselves
+    float l_rounded = 0.0f;
     // with a soft cap or a distance penalty the raw scores are turned into final ones (log2 units) right after they are read
     const bool scored = a.softcap_log2 > 0.0f || a.slopes != nullptr;
     const float sl2 = scored ? 1.0f : a.scale_log2;
@@ -397,21 +401,33 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
           tmem_st16(lane_addr + 128 + half * (HD / 2) + c0, o);
         }
         l *= alpha;
+        l_rounded *= alpha;
       }
       if (grow) m_used = m_new;
       const float neg_m = m_used == -INFINITY ? 0.0f : -m_used;
       uint32_t pk[16];
       float l0 = 0.0f, l1 = 0.0f;
+      f32x2 sums = 0, rounded = 0;
 #pragma unroll
       for (int c = 0; c < 32; c += 2) {
         const float p0 = ex2(fmaf(__uint_as_float(sr[c]), sl2, neg_m));
         const float p1 = ex2(fmaf(__uint_as_float(sr[c + 1]), sl2, neg_m));
-        l0 += p0;
-        l1 += p1;
         __nv_bfloat162 h2 = __floats2bfloat162_rn(p0, p1);
         pk[c >> 1] = *reinterpret_cast<uint32_t*>(&h2);
+        if constexpr (KEPT) {
+          sums = add2(sums, pair_of(p0, p1));
+          rounded = add2(rounded, pair_of(__uint_as_float(pk[c >> 1] << 16), __uint_as_float(pk[c >> 1] & 0xffff0000u)));
+        } else {
+          l0 += p0;
+          l1 += p1;
+        }
       }
-      l += l0 + l1;
+      if constexpr (KEPT) {
+        l += halves_sum(sums);
+        l_rounded += halves_sum(rounded);
+      } else {
+        l += l0 + l1;
+      }
       // asked now, needed at the top of the next page: are its scores complete?
       s_ready = j + 1 < n_pages ? mbar_test(s_full + 8 * (b ^ 1), ((j + 1) >> 1) & 1) : 0u;
       // P_j goes where S_j was: both threads of the row have read their scores (they met at the barrier above), and
@@ -442,6 +458,12 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       l += xl[(half ^ 1) * 128 + r];
       if (a.sinks) l += ex2(a.sinks[kh * G + (r0 + r) % G] * 1.4426950408889634f - m_used);     // both halves hold the same m_used
       if (KEPT && half == 0 && ok && R < rows_total) put_denominator(a, (size_t)(tok0 + R / G) * a.heads + kh * G + R % G, m_used, l);
+      if constexpr (KEPT) {
+        pair_sync();
+        xl[half * 128 + r] = l_rounded;
+        pair_sync();
+        l = l_rounded + xl[(half ^ 1) * 128 + r];
+      }
       const float inv = l > 0.0f ? 1.0f / l : 0.0f;
       // this thread's half of the accumulator row: all loads under way at once, one wait
       uint32_t o[HD / 2];
@@ -653,6 +675,9 @@ attn_tc_wide_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16);
     unsigned short* xch = reinterpret_cast<unsigned short*>(smem + L::XCH_OFF);     // [2 steps][4 parts][128 rows]
     float m_used = -INFINITY, l = 0.0f;
+    // KEPT: the sum of the weights as they are rounded for the product, by which the result is divided: what rounds the one key that a peaked row looks at
+    // then cancels (error against 64 bits 2.3e-3 -> 2.1e-3 for 2 per cent of the time); the denominator that others get is the sum of the weights themselves
+    float l_rounded = 0.0f;
     // with a soft cap or a distance penalty the raw scores are turned into final ones (log2 units) right after they are read
     const bool scored = a.softcap_log2 > 0.0f || a.slopes != nullptr;
     const float sl2 = scored ? 1.0f : a.scale_log2;
@@ -733,21 +758,33 @@ attn_tc_wide_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
           tmem_st16(lane_addr + 256 + part * (HD / 4) + c0, o);
         }
         l *= alpha;
+        l_rounded *= alpha;
       }
       if (grow) m_used = m_new;
       const float neg_m = m_used == -INFINITY ? 0.0f : -m_used;
       uint32_t pk[16];
       float l0 = 0.0f, l1 = 0.0f;
+      f32x2 sums = 0, rounded = 0;
 #pragma unroll
       for (int c = 0; c < 32; c += 2) {
         const float p0 = ex2(fmaf(__uint_as_float(sr[c]), sl2, neg_m));
         const float p1 = ex2(fmaf(__uint_as_float(sr[c + 1]), sl2, neg_m));
-        l0 += p0;
-        l1 += p1;
         __nv_bfloat162 h2 = __floats2bfloat162_rn(p0, p1);
         pk[c >> 1] = *reinterpret_cast<uint32_t*>(&h2);
+        if constexpr (KEPT) {
+          sums = add2(sums, pair_of(p0, p1));
+          rounded = add2(rounded, pair_of(__uint_as_float(pk[c >> 1] << 16), __uint_as_float(pk[c >> 1] & 0xffff0000u)));
+        } else {
+          l0 += p0;
+          l1 += p1;
+        }
       }
-      l += l0 + l1;
+      if constexpr (KEPT) {
+        l += halves_sum(sums);
+        l_rounded += halves_sum(rounded);
+      } else {
+        l += l0 + l1;
+      }
       s_ready = j + 1 < n_steps ? mbar_test(s_full + 8 * (b ^ 1), ((j + 1) >> 1) & 1) : 0u;
       // P_j goes where S_j was: the four threads of the row have read their scores (they met at the barrier above)
       tmem_st16(lane_addr + (uint32_t)(b * 128 + part * 16), pk);
@@ -775,6 +812,12 @@ attn_tc_wide_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
       l = (xl[0] + xl[128]) + (xl[256] + xl[384]);
       if (a.sinks) l += ex2(a.sinks[kh * G + (r0 + r) % G] * 1.4426950408889634f - m_used);
       if (KEPT && part == 0 && ok && R < rows_total) put_denominator(a, (size_t)(tok0 + R / G) * a.heads + kh * G + R % G, m_used, l);
+      if constexpr (KEPT) {
+        row_sync();
+        xl[part * 128] = l_rounded;
+        row_sync();
+        l = (xl[0] + xl[128]) + (xl[256] + xl[384]);
+      }
       const float inv = l > 0.0f ? 1.0f / l : 0.0f;
       uint32_t o[HD / 4];      // this thread's quarter of the accumulator row
 #pragma unroll
