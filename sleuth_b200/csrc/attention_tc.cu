@@ -30,7 +30,7 @@
 // product) is what bounds a single long prompt; many sequences or heads fill the GPU.
 //
 // With KEPT the same kernels serve a cache of bounded size (kept.cuh): the pages of the first rows come before the window's, as one list (TilePages),
-// and the rows' denominators are left for the kernel that gathers weights. Measured there: a prompt of 6,000 tokens, 32 / 8 heads of 128, 290 us = 1.02
+// and the rows' denominators are left for the kernel that gathers weights. Measured there: a prompt of 6,000 tokens, 32 / 8 heads of 128, 320 us = 0.92
 // PFLOP/s; seven portions of 349 to 1,500 tokens on up to 3,000 rows, heads of 64, a window of 1,000 and 100 first rows, 186 us (20 pages a tile, of
 // which five run the mask); 2,048 tokens under a window of 512, 16 / 8 heads, 19 us, mostly a tile's way in and out (10 pages).
 //
@@ -313,7 +313,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     unsigned short* xch = reinterpret_cast<unsigned short*>(smem + L::XCH_OFF);     // [2 pages][2 halves][128 rows]
     float m_used = -INFINITY, l = 0.0f;
     // KEPT: the sum of the weights as they are rounded for the product, by which the result is divided: what rounds the one key that a peaked row looks at
-    // then cancels (error against 64 bits 2.3e-3 -> 2.1e-3 for 2 per cent of the time); the denominator that others get is the sum of the weights themselves
+    // then cancels (error against 64 bits 2.2e-3 to 2.3e-3 -> 2.1e-3 to 2.2e-3 for 2 to 4 per cent of the time); the denominator that others get is the sum of the weights themselves
     float l_rounded = 0.0f;
     // with a soft cap or a distance penalty the raw scores are turned into final ones (log2 units) right after they are read
     const bool scored = a.softcap_log2 > 0.0f || a.slopes != nullptr;
@@ -676,7 +676,7 @@ attn_tc_wide_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     unsigned short* xch = reinterpret_cast<unsigned short*>(smem + L::XCH_OFF);     // [2 steps][4 parts][128 rows]
     float m_used = -INFINITY, l = 0.0f;
     // KEPT: the sum of the weights as they are rounded for the product, by which the result is divided: what rounds the one key that a peaked row looks at
-    // then cancels (error against 64 bits 2.3e-3 -> 2.1e-3 for 2 per cent of the time); the denominator that others get is the sum of the weights themselves
+    // then cancels (error against 64 bits 2.2e-3 to 2.3e-3 -> 2.1e-3 to 2.2e-3 for 2 to 4 per cent of the time); the denominator that others get is the sum of the weights themselves
     float l_rounded = 0.0f;
     // with a soft cap or a distance penalty the raw scores are turned into final ones (log2 units) right after they are read
     const bool scored = a.softcap_log2 > 0.0f || a.slopes != nullptr;
