@@ -15,8 +15,8 @@
 //     runs, so that ranks are sums of a block-wide scan; the lists of places and rows go to scratch. The block, or where the rows are many a second
 //     kernel, moves them, 16 threads a row.
 // Bound by latency: loads, a descent, moves; the bytes are the weights and positions once and the moved rows twice. Measured: a row of 2,049 goes in each
-// of 512 (sequence, kv head) pairs 7.6 us (17 MB, 2.3 TB/s; by the descent 37); 64 pairs of 2,500 to 8,192 rows come down to 1,024 in 24 us, of which the
-// descent is 14 and the moves, 59 MB, 10.
+// of 512 (sequence, kv head) pairs 7.6 us (17 MB, 2.3 TB/s; by the descent 37); 64 pairs of 2,500 to 8,192 rows come down to 1,024: the
+// descent 15 us (18 with one row a thread in flight while the keys are made), the moves, 59 MB, 14 (4.2 TB/s; the same with four rows in flight a thread).
 #include "common.cuh"
 
 namespace slb {
@@ -223,9 +223,35 @@ __global__ void __launch_bounds__(THREADS) cache_evict_kernel(EvictArgs a) {
     if (lists && tid == 0) lists[0] = 0;
     return;
   }
-  if (a.keys_fit)
-    for (int j = tid; j < n; j += THREADS) keys[j] = make_key(j);
+#pragma unroll
+  for (int i = 0; i < 2048 / THREADS; ++i) hist[tid + i * THREADS] = 0;
   __syncthreads();
+  if (a.keys_fit) {
+    // the keys and the counts of their first digit; kBatch rows a thread in flight (one after the other each would wait for the memory's answer)
+    constexpr int kBatch = 8;
+    for (int base = 0; base < n; base += kBatch * THREADS) {
+      float w[kBatch];
+      int p[kBatch];
+#pragma unroll
+      for (int e = 0; e < kBatch; ++e) {
+        const int j = base + e * THREADS + tid;
+        w[e] = j < n ? weights[j] : 0.0f;
+        p[e] = j < past ? positions[j] : seen - (n - j);
+      }
+#pragma unroll
+      for (int e = 0; e < kBatch; ++e) {
+        const int j = base + e * THREADS + tid;
+        const bool safe = p[e] < a.first || p[e] >= seen - a.recent;
+        const uint32_t k = order_key(w[e], safe);
+        const unsigned protect = __ballot_sync(0xffffffffu, safe && j < n);
+        if (j < n) {
+          keys[j] = k;
+          if (!safe) atomicAdd(&hist[k >> 21], 1);
+        }
+        if (protect && (tid & 31) == 0) atomicAdd(&hist[2047], __popc(protect));      // (protected rows stand together: one addition a warp)
+      }
+    }
+  }
   auto key_of = [&](int j) { return a.keys_fit ? keys[j] : make_key(j); };
 
   // the key of the last row that stays: digit by digit, the largest ones first
@@ -234,13 +260,16 @@ __global__ void __launch_bounds__(THREADS) cache_evict_kernel(EvictArgs a) {
 #pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
+    if (pass) {
 #pragma unroll
-    for (int i = 0; i < 2048 / THREADS; ++i) hist[tid + i * THREADS] = 0;
-    __syncthreads();
-    for (int j = tid; j < n; j += THREADS) {
-      const uint32_t k = key_of(j);
-      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1);
+      for (int i = 0; i < 2048 / THREADS; ++i) hist[tid + i * THREADS] = 0;
+      __syncthreads();
     }
+    if (pass || !a.keys_fit)
+      for (int j = tid; j < n; j += THREADS) {
+        const uint32_t k = key_of(j);
+        if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1);
+      }
     __syncthreads();
     // a thread a run of digits, the largest first: how many keys lie above them
     constexpr int RUN = 2048 / THREADS;
