@@ -295,6 +295,13 @@ def test_evict_after_prompts(kind, in_place):
     _evict_case(torch.float32, 2, 16, [300, 260], [256, 256], 256, 1, 3, seed=6, kind=kind, gone=5, in_place=in_place, promise=False)
 
 
+@pytest.mark.parametrize("kind", ["plain", "ties", "same", "odd"])
+@pytest.mark.parametrize("in_place", [True, False])
+def test_evict_around_and_beyond_the_rows_a_block_reads_at_once(kind, in_place):
+    _evict_case(torch.bfloat16, 2, 16, [8191, 8192, 8193, 20011], [8000, 8192, 0, 16385], 700, 5, 300, seed=9, kind=kind, gone=33, in_place=in_place)
+    _evict_case(torch.bfloat16, 1, 16, [2047, 2048, 33], [2000, 0, 33], 1500, 0, 1500, seed=10, kind=kind, in_place=in_place)
+
+
 def test_evict_more_rows_than_shared_memory_holds():
     _evict_case(torch.bfloat16, 1, 16, [50001, 100], [50000, 100], 50000, 4, 100, seed=7, kind="ties", gone=9)
     _evict_case(torch.bfloat16, 1, 16, [60000], [100], 3000, 4, 100, seed=8, kind="plain", gone=9)
