@@ -18,6 +18,8 @@
 // tiles 425); five tokens on 33 to 700 rows, 8 / 4 heads of 64, with weights 22.7 us, three launches of which each waits for the one before.
 #include <math.h>
 
+#include <algorithm>
+
 #include "kept.cuh"
 #include "tcgen05.cuh"      // clusters
 
@@ -643,10 +645,14 @@ static int kept_form(long long tokens, int max_count, int heads, int kv_heads, i
   return kKeptGeneral;
 }
 
+// No sequence brings more tokens than the step has, or than it has rows afterwards.
+static int least_count(int max_count, long long tokens, int max_keys) { return (int)std::min({(long long)max_count, tokens, (long long)max_keys}); }
+
 // Floats of scratch that slb_attention_kept takes for a step of these sizes: shares of results, with weights denominators and scores.
 extern "C" long long slb_attention_kept_scratch(long long tokens, int n_seqs, int max_count, int heads, int kv_heads, int head_dim, int max_keys,
                                                 int dtype, int weights) {
   if (tokens <= 0 || n_seqs <= 0 || max_count <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || max_keys <= 0) return 0;
+  max_count = least_count(max_count, tokens, max_keys);
   const int form = kept_form(tokens, max_count, heads, kv_heads, head_dim, max_keys, dtype, weights != 0);
   if (form == kKeptFew) return kept_few_floats(tokens, n_seqs, max_count, heads, kv_heads, head_dim, max_keys, weights != 0);
   if (form == kKeptTc) return weights ? tokens * heads : 0;
@@ -659,8 +665,8 @@ extern "C" long long slb_attention_kept_scratch(long long tokens, int n_seqs, in
 extern "C" int slb_attention_kept(const KeptCall* call) {
   SLB_REQUIRE(call != nullptr, "attention_kept: no call");
   const KeptCall c = *call;
-  const int n_seqs = c.n_seqs, max_count = c.max_count, heads = c.heads, kv_heads = c.kv_heads, head_dim = c.head_dim, window = c.window, first = c.first,
-            table_stride = c.table_stride, dtype = c.dtype;
+  const int n_seqs = c.n_seqs, heads = c.heads, kv_heads = c.kv_heads, head_dim = c.head_dim, table_stride = c.table_stride, dtype = c.dtype;
+  int max_count = c.max_count, window = c.window, first = c.first;
   const long long tokens = c.tokens;
   const float scale = c.scale;
   int max_keys = c.max_keys;
@@ -676,6 +682,12 @@ extern "C" int slb_attention_kept(const KeptCall* call) {
     SLB_REQUIRE(table_stride < (1 << 25), "attention_kept: table_stride=%d", table_stride);
     max_keys = table_stride * kPageTokens;
   }
+  // What hides nothing is taken out and what is beyond the last row is cut, so that sums of these numbers stay within 32 bits whatever a caller
+  // says for "no limit": a window as long as the longest sequence is none, first rows behind it are all.
+  SLB_REQUIRE(max_keys <= (1 << 30), "attention_kept: a sequence of %d rows", max_keys);
+  if (window >= max_keys) window = 0;
+  first = window > 0 ? std::min(first, max_keys) : 0;
+  max_count = least_count(max_count, tokens, max_keys);
   const bool gather = c.weights != nullptr;
   const long long need = slb_attention_kept_scratch(tokens, n_seqs, max_count, heads, kv_heads, head_dim, max_keys, dtype, gather);
   SLB_REQUIRE(need == 0 || (c.scratch != nullptr && c.scratch_floats >= need), "attention_kept: the step needs %lld floats of scratch, %lld were given",
@@ -683,7 +695,7 @@ extern "C" int slb_attention_kept(const KeptCall* call) {
   KeptArgs a{};
   a.q = c.q; a.k_pool = c.k_pool; a.v_pool = c.v_pool; a.out = c.out; a.seq_start = c.seq_start; a.past = c.past; a.counts = c.counts;
   a.block_table = c.block_table; a.table_stride = table_stride; a.n_seqs = n_seqs; a.heads = heads; a.kv_heads = kv_heads;
-  a.head_dim = head_dim; a.window = window; a.first = window > 0 ? first : 0; a.scale = scale; a.slots = c.slots; a.weights = c.weights;
+  a.head_dim = head_dim; a.window = window; a.first = first; a.scale = scale; a.slots = c.slots; a.weights = c.weights;
   a.weights_out = c.weights_out; a.capacity = c.capacity; a.lse = c.lse; a.scratch = c.scratch;
   const cudaStream_t s = (cudaStream_t)c.stream;
   SLB_REQUIRE(scale > 0.0f, "attention_kept: the scale is positive, got %g", (double)scale);
