@@ -53,6 +53,14 @@ __host__ __device__ __forceinline__ int window_lo(int p, int window) { return wi
 
 __device__ __forceinline__ bool sees(int key, int pos, int lo, int first) { return key <= pos && (key >= lo || key < first); }
 
+// A sequence that brings no token keeps what its rows have gathered: where the target lies apart, rows lo .. hi - 1 of it go over. `t` of `threads` threads.
+__device__ __forceinline__ void carry_weights(const KeptArgs& a, int seq, int kh, long long lo, long long hi, int t, int threads) {
+  if (a.weights == nullptr || a.weights_out == a.weights) return;
+  const size_t at0 = ((size_t)(a.slots ? a.slots[seq] : seq) * a.kv_heads + kh) * a.capacity;
+  hi = min(hi, min((long long)a.past[seq], a.capacity));
+  for (long long key = lo + t; key < hi; key += threads) a.weights_out[at0 + key] = a.weights[at0 + key];
+}
+
 // Steps of few tokens (kept_few.cu): which they take, the floats of scratch (the first ones 16-byte aligned), the launch.
 bool kept_few_takes(long long tokens, int max_count, int heads, int kv_heads, int head_dim, int max_keys, int dtype, bool weights);
 long long kept_few_floats(long long tokens, int n_seqs, int max_count, int heads, int kv_heads, int head_dim, int max_keys, bool weights);

@@ -499,7 +499,10 @@ __global__ void __launch_bounds__(kGenThreads) kept_weights_general_kernel(KeptA
   const int seq = blockIdx.z, kh = blockIdx.y, G = a.heads / a.kv_heads;
   const int count = a.counts[seq], past = a.past[seq], end = past + count;
   const int key0 = (int)(blockIdx.x / ranks) * kGenKeys;
-  if (count <= 0 || key0 >= end) return;                 // (the whole cluster)
+  if (count <= 0 || key0 >= end) {                       // (the whole cluster)
+    if (count <= 0 && rank == 0) carry_weights(a, seq, kh, key0, key0 + kGenKeys, tid, kGenThreads);
+    return;
+  }
   const size_t token0 = a.seq_start[seq];
   const int* table = a.block_table + (size_t)seq * a.table_stride;
   // the queries that see some key of the tile: from the tile's own rows on, and while the window reaches back to it (or all of them)
@@ -555,6 +558,12 @@ __global__ void __launch_bounds__(kGenThreads) kept_weights_general_kernel(KeptA
     const size_t at = ((size_t)(a.slots ? a.slots[seq] : seq) * a.kv_heads + kh) * a.capacity + key;
     a.weights_out[at] = (key < past ? a.weights[at] : 0.0f) + total;
   }
+}
+
+// A step without any token, whose weights go elsewhere.
+__global__ void __launch_bounds__(256) kept_carry_kernel(KeptArgs a) {
+  pdl_enter();
+  carry_weights(a, blockIdx.z, blockIdx.y, 0, a.capacity, blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
 }
 
 template <typename T>
@@ -677,7 +686,18 @@ extern "C" int slb_attention_kept(const KeptCall* call) {
   SLB_REQUIRE(dtype == kF32 || dtype == kBF16, "attention_kept: unknown dtype %d", dtype);
   SLB_REQUIRE((c.weights == nullptr) == (c.weights_out == nullptr) && (c.weights == nullptr || c.capacity > 0), "attention_kept: weights and their target go together");
   SLB_REQUIRE(n_seqs < 65536 && kv_heads < 65536 && tokens < (1ll << 31), "attention_kept: n_seqs=%d tokens=%lld", n_seqs, tokens);
-  if (n_seqs == 0 || tokens == 0 || max_count == 0) return 0;
+  if (n_seqs == 0) return 0;
+  KeptArgs a{};
+  a.q = c.q; a.k_pool = c.k_pool; a.v_pool = c.v_pool; a.out = c.out; a.seq_start = c.seq_start; a.past = c.past; a.counts = c.counts;
+  a.block_table = c.block_table; a.table_stride = table_stride; a.n_seqs = n_seqs; a.heads = heads; a.kv_heads = kv_heads;
+  a.head_dim = head_dim; a.scale = scale; a.slots = c.slots; a.weights = c.weights; a.weights_out = c.weights_out; a.capacity = c.capacity; a.lse = c.lse;
+  a.scratch = c.scratch;
+  const cudaStream_t s = (cudaStream_t)c.stream;
+  if (tokens == 0 || max_count == 0) {
+    if (c.weights == nullptr || c.weights_out == c.weights) return 0;
+    launch(kept_carry_kernel, dim3((unsigned)std::min((c.capacity + 255) / 256, 8ll), kv_heads, n_seqs), dim3(256), 0, s, a);
+    return check_launch("attention_kept (no tokens)");
+  }
   if (max_keys <= 0 || max_keys > table_stride * (long long)kPageTokens) {
     SLB_REQUIRE(table_stride < (1 << 25), "attention_kept: table_stride=%d", table_stride);
     max_keys = table_stride * kPageTokens;
@@ -692,12 +712,8 @@ extern "C" int slb_attention_kept(const KeptCall* call) {
   const long long need = slb_attention_kept_scratch(tokens, n_seqs, max_count, heads, kv_heads, head_dim, max_keys, dtype, gather);
   SLB_REQUIRE(need == 0 || (c.scratch != nullptr && c.scratch_floats >= need), "attention_kept: the step needs %lld floats of scratch, %lld were given",
               need, c.scratch ? c.scratch_floats : 0ll);
-  KeptArgs a{};
-  a.q = c.q; a.k_pool = c.k_pool; a.v_pool = c.v_pool; a.out = c.out; a.seq_start = c.seq_start; a.past = c.past; a.counts = c.counts;
-  a.block_table = c.block_table; a.table_stride = table_stride; a.n_seqs = n_seqs; a.heads = heads; a.kv_heads = kv_heads;
-  a.head_dim = head_dim; a.window = window; a.first = first; a.scale = scale; a.slots = c.slots; a.weights = c.weights;
-  a.weights_out = c.weights_out; a.capacity = c.capacity; a.lse = c.lse; a.scratch = c.scratch;
-  const cudaStream_t s = (cudaStream_t)c.stream;
+  a.window = window;
+  a.first = first;
   SLB_REQUIRE(scale > 0.0f, "attention_kept: the scale is positive, got %g", (double)scale);
   const int form = kept_form(tokens, max_count, heads, kv_heads, head_dim, max_keys, dtype, gather);
   if (form == kKeptFew) return kept_few(a, tokens, max_count, max_keys, c.pool_pages, c.status, s);

@@ -156,7 +156,10 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     rank = (int)cluster_ctarank();
     seq = (int)(blockIdx.x / fa.cluster) / a.kv_heads;
     const int pages = PageRun(a.past[seq], min(a.counts[seq], fa.max_count), a.window, a.first).count;
-    if (pages == 0) return;      // (the whole cluster)
+    if (pages == 0) {      // (the whole cluster)
+      carry_weights(a, seq, pair_kh, 0, a.capacity, rank * THREADS + tid, fa.cluster * THREADS);
+      return;
+    }
     const int share = min((pages + fa.cluster - 1) / fa.cluster, fa.cluster_pages);
     seq_first = -(long long)pair_kh * pages;      // as if the kv head's units were the first
     u = min(pages, rank * share);
@@ -570,7 +573,13 @@ __global__ void __launch_bounds__(256, 4) kept_few_finish_kernel(FewArgs fa) {
   const int tid = threadIdx.x;
   const int kh = blockIdx.y, seq = blockIdx.z, G = a.heads / a.kv_heads;
   const int count = min(a.counts[seq], fa.max_count), past = a.past[seq], tok0 = a.seq_start[seq], rows_total = count * G;
-  if (count <= 0) return;
+  if (count <= 0) {
+    if ((int)blockIdx.x >= fa.out_blocks) {
+      const long long lo = (long long)((int)blockIdx.x - fa.out_blocks) * fa.keys_a_block;
+      carry_weights(a, seq, kh, lo, lo + fa.keys_a_block, tid, 256);
+    }
+    return;
+  }
   const int2* info = fa.info + ((size_t)seq * a.kv_heads + kh) * fa.max_tiles;
   auto row_of = [&](int Rr) { return (size_t)(tok0 + Rr / G) * a.heads + kh * G + Rr % G; };
   auto slot_of = [&](int2 in, int i) { return ((size_t)(in.x + i) * 2 + (i == 0 ? 1 : 0)) * ROWS; };

@@ -74,7 +74,10 @@ kept_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::BAR_OFF + L::N_BARS * 8);
   pdl_wait();
   const int count = a.counts[seq], past = a.past[seq], end = past + count;
-  if (count <= 0 || key0 >= end) return;       // (the whole cluster)
+  if (count <= 0 || key0 >= end) {             // (the whole cluster)
+    if (count <= 0 && rank == 0) carry_weights(a, seq, kh, key0, key0 + kKwKeys, tid, kKwThreads);
+    return;
+  }
   // that all blocks of the cluster have begun is waited for before the first store into another's shared memory
   if (ranks > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   const size_t tok0 = a.seq_start[seq];

@@ -42,3 +42,37 @@ def test_largest_promise_of_new_tokens(dtype, heads, kv_heads, dim, counts):
     assert bool(((out.cpu().view(want.shape).double() - want).abs() <= rel * size + 1e-12).all())
     for s, (p, c) in enumerate(zip(step.past, step.counts)):
         assert bool(((w[s, :, :p + c].cpu().double() - want_w[s, :, :p + c]).abs() <= 5e-5 * want_w[s, :, :p + c].abs() + 1e-7).all())
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim", KINDS, ids=KIND_IDS)
+@pytest.mark.parametrize("past,counts", [([40, 700, 9], [1, 0, 1]), ([0, 130], [0, 1]), ([70, 300, 0, 64], [3, 0, 0, 2]), ([500, 20], [0, 150]),
+                                         ([3000, 10, 65], [0, 300, 0])])
+@pytest.mark.parametrize("window,first", [(0, 0), (50, 5)])
+def test_sequences_without_new_tokens_keep_what_they_gathered(dtype, heads, kv_heads, dim, past, counts, window, first):
+    step = Step(dtype, heads, kv_heads, dim, past, counts, window, first, seed=13)
+    for slots in (None, [len(past) - i for i in range(len(past))]):
+        for in_place in (True, False):
+            _, _, got = step.run(weights=True, in_place=in_place, slots=slots)
+            for s, (p, c) in enumerate(zip(past, counts)):
+                if c == 0:
+                    assert torch.equal(got[s, :, :p], step.weights[s, :, :p])
+                    rest = step.weights[s, :, p:] if in_place else torch.full_like(got[s, :, p:], -5.0)
+                    assert torch.equal(got[s, :, p:], rest)
+
+
+@pytest.mark.parametrize("slots", [None, [2, 0]])
+def test_a_step_without_any_token_keeps_what_was_gathered(slots):
+    from sleuth_b200.kernels import ops
+    past, K, cap = [200, 3], 2, 5 * 64
+    w = torch.rand((3, K, cap), device=DEV)
+    target = torch.full_like(w, -5.0)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    pool = torch.zeros((10, K, 64, 64), dtype=torch.bfloat16, device=DEV)
+    q, out = torch.empty((0, 4, 64), dtype=torch.bfloat16, device=DEV), torch.empty((0, 256), dtype=torch.bfloat16, device=DEV)
+    ops.attention_kept(q, pool, pool, out, i32([0, 0, 0]), i32(past), i32([0, 0]), torch.zeros((2, 5), dtype=torch.int32, device=DEV), 0, 4, K, 64, 0, 0, 0.1,
+                       weights=w, weights_out=target, slots=None if slots is None else i32(slots))
+    want = torch.full_like(w, -5.0)
+    for s, p in enumerate(past):
+        at = s if slots is None else slots[s]
+        want[at, :, :p] = w[at, :, :p]
+    assert torch.equal(target, want)
