@@ -420,7 +420,7 @@ extern "C" int slb_cache_evict(const EvictCall* call) {
   if (n_seqs == 0) return 0;
   const long long table_rows = (long long)table_stride * kPageTokens;
   if (max_length <= 0 || max_length > table_rows) max_length = (int)(table_rows < 0x7fffffffll ? table_rows : 0x7fffffffll);
-  if (max_length > capacity) max_length = (int)capacity;
+  SLB_REQUIRE(capacity >= max_length, "cache_evict: weights and positions of %lld rows are shorter than the cache (%d)", capacity, max_length);
   const long long need = slb_cache_evict_scratch(n_seqs, kv_heads, budget, max_length);
   SLB_REQUIRE(need == 0 || (c.scratch != nullptr && c.scratch_words >= need), "cache_evict: the step needs %lld words of scratch, %lld were given", need,
               c.scratch ? c.scratch_words : 0ll);

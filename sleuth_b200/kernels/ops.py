@@ -1828,7 +1828,7 @@ def cache_evict(weights, positions, k_pool, v_pool, block_table, past, lengths, 
     stay but lie at ``budget`` or behind move, keys, values, weight and position, into the places of those that go; a sequence then holds
     min(length, ``budget``) rows, and the pages behind them are free. ``weights_out`` / ``positions_out``: where the rows' weights and
     positions go (default: in place); places behind the last row are left alone. ``max_length``: a promise that no sequence
-    holds more rows (0: as many as its table takes); ``scratch``: ``cache_evict_scratch_words`` int32 words."""
+    holds more rows (0: as many as its table takes), and weights and positions are at least as long; ``scratch``: ``cache_evict_scratch_words`` int32 words."""
     i32, f32 = torch.int32, torch.float32
     k_shape, w_shape, (n, stride) = k_pool.shape, weights.shape, block_table.shape
     if weights_out is None:
@@ -1847,6 +1847,7 @@ def cache_evict(weights, positions, k_pool, v_pool, block_table, past, lengths, 
             and f32 == weights.dtype == weights_out.dtype and i32 == positions.dtype == positions_out.dtype
             and len(w_shape) == 3 and w_shape[1] == kv_heads and w_shape[2] > 0 and w_shape == positions.shape == weights_out.shape == positions_out.shape
             and (slots is None and w_shape[0] >= n or slots is not None and slots.dtype == i32 and slots.numel() >= n)
+            and w_shape[2] >= (max_length if 0 < max_length <= 64 * stride else 64 * stride)
             and (scratch is None or scratch.dtype == i32) and budget > 0 and first >= 0 and recent >= 0 and first + recent <= budget):
         _kept_refusal("cache_evict", dict(weights=weights, positions=positions, k_pool=k_pool, v_pool=v_pool, block_table=block_table, past=past,
                                           lengths=lengths, seen=seen, weights_out=weights_out, positions_out=positions_out, slots=slots, scratch=scratch), (
@@ -1861,6 +1862,7 @@ def cache_evict(weights, positions, k_pool, v_pool, block_table, past, lengths, 
              "positions are int32, and all four have one shape"),
             (lambda: slots is None and w_shape[0] >= n or slots is not None and slots.dtype == i32 and slots.numel() >= n,
              "slots are int32, one a sequence; without them weights hold a row of every sequence"),
+            (lambda: w_shape[2] >= (max_length if 0 < max_length <= 64 * stride else 64 * stride), "weights and positions are shorter than the cache"),
             (lambda: scratch is None or scratch.dtype == i32, "scratch is int32"),
             (lambda: budget > 0 and first >= 0 and recent >= 0 and first + recent <= budget, "first and recent rows fit the budget")))
     try:

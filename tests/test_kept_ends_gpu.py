@@ -76,3 +76,24 @@ def test_a_step_without_any_token_keeps_what_was_gathered(slots):
         at = s if slots is None else slots[s]
         want[at, :, :p] = w[at, :, :p]
     assert torch.equal(target, want)
+
+
+def _evict_call(cap, stride=4, **kw):
+    from sleuth_b200.kernels import ops
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+    pool = torch.zeros((stride, 2, 64, 16), device=DEV)
+    a = dict(weights=torch.rand((1, 2, cap), device=DEV), positions=torch.zeros((1, 2, cap), dtype=torch.int32, device=DEV), k_pool=pool, v_pool=pool.clone(),
+             block_table=torch.arange(stride, dtype=torch.int32, device=DEV).view(1, -1), past=i32([50]), lengths=i32([90]), seen=i32([90]), budget=60, first=2,
+             recent=3, scratch=torch.empty(10000, dtype=torch.int32, device=DEV))
+    a.update(kw)
+    ops.cache_evict(**a)
+
+
+def test_evictions_refuse_weights_that_are_shorter_than_the_cache():
+    """A row that weights and positions have no place for cannot be ranked, and no position behind it can be told."""
+    _evict_call(256)
+    _evict_call(100, max_length=100)
+    _evict_call(300, max_length=5000)
+    for cap, kw in ((255, {}), (80, {}), (99, dict(max_length=100)), (80, dict(max_length=90)), (255, dict(max_length=5000))):
+        with pytest.raises(ValueError):
+            _evict_call(cap, **kw)
