@@ -215,12 +215,21 @@ kept_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
             __syncwarp();
             if (lane == 0) mbar_arrive(s_free + 8 * b);      // the next product may overwrite the scores
           }
-          if (masked) {
-#pragma unroll
-            for (int c = 0; c < 32; ++c)
-              if (R0 + c0 + c < see_lo || R0 + c0 + c >= see_hi) sr[c] = 0xff800000u;
-          }
           const ulonglong2* dd = reinterpret_cast<const ulonglong2*>(d + b * kKwRows + col0 + c0);
+          if (masked) {
+            // what a row does not give is left out of the sum, not added as 2^(-inf - d): d is NaN where a query is
+            const int first_c = see_lo - R0 - c0, end_c = see_hi - R0 - c0;
+#pragma unroll
+            for (int c = 0; c < 32; c += 4) {
+              const ulonglong2 n = dd[c >> 2];
+              const f32x2 x0 = fma2(pair_of(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), scale2, n.x);
+              const f32x2 x1 = fma2(pair_of(__uint_as_float(sr[c + 2]), __uint_as_float(sr[c + 3])), scale2, n.y);
+              auto given = [&](int i, float p) { return i >= first_c && i < end_c ? p : 0.0f; };
+              s0 = add2(s0, pair_of(given(c, kw_ex2(low_half(x0))), given(c + 1, kw_ex2(high_half(x0)))));
+              s1 = add2(s1, pair_of(given(c + 2, kw_ex2(low_half(x1))), given(c + 3, kw_ex2(high_half(x1)))));
+            }
+            continue;
+          }
 #pragma unroll
           for (int c = 0; c < 32; c += 4) {
             const ulonglong2 n = dd[c >> 2];

@@ -97,3 +97,22 @@ def test_evictions_refuse_weights_that_are_shorter_than_the_cache():
     for cap, kw in ((255, {}), (80, {}), (99, dict(max_length=100)), (80, dict(max_length=90)), (255, dict(max_length=5000))):
         with pytest.raises(ValueError):
             _evict_call(cap, **kw)
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim", KINDS, ids=KIND_IDS)
+@pytest.mark.parametrize("past,counts,token", [([30, 200], [1, 1], 0), ([30, 200], [5, 3], 6), ([0, 90], [200, 70], 60), ([64, 10], [150, 140], 149)])
+@pytest.mark.parametrize("window,first", [(0, 0), (40, 6)])
+def test_a_query_that_is_not_a_number_spoils_only_what_it_sees(dtype, heads, kv_heads, dim, past, counts, token, window, first):
+    step = Step(dtype, heads, kv_heads, dim, past, counts, window, first, seed=14, hole=False)
+    step.q[token, heads - 1, 0] = math.nan
+    out, lse, got = step.run(weights=True, lse=True)
+    want, want_lse, size, want_w = plain.attention(step.q, step.k, step.v, step.seq_start, past, counts, step.table, heads, kv_heads, window, first, step.scale,
+                                                   step.weights)
+    # (the same bounds as in the tests of finite queries)
+    rel = 2.0 ** -7 if dtype == torch.bfloat16 else 5e-5
+    assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(torch.isnan(lse), torch.isnan(want_lse))
+    assert bool(((out - want).abs() <= rel * size + 1e-12)[~torch.isnan(want)].all())
+    for s, (p, c) in enumerate(zip(past, counts)):
+        a, b = got[s, :, :p + c].double(), want_w[s, :, :p + c]
+        assert torch.equal(torch.isnan(a), torch.isnan(b)), (s, torch.isnan(a).sum(-1).tolist(), torch.isnan(b).sum(-1).tolist())
+        assert bool(((a - b).abs() <= 5e-5 * b.abs() + 1e-7)[~torch.isnan(b)].all())
