@@ -630,12 +630,15 @@ static int general_weights(KeptArgs a, int max_count, int max_keys, cudaStream_t
 
 // Shares of the keys: as many as give every SM about four blocks (a prompt's tiles grow with their rows: 176 tiles of 1 to 11 steps, whole, 239 us,
 // in three shares 152), of at least one step of 64 keys (a step takes a block 3 us, a
-// share more takes the joining kernel 0.1: five sequences of 33 to 700 rows in shares of 256 keys 20 us).
-static int general_splits(int n_seqs, int max_count, int heads, int kv_heads, int max_keys) {
+// share more takes the joining kernel 0.1: five sequences of 33 to 700 rows in shares of 256 keys 20 us). A tile walks the first rows and its
+// tokens' windows at most, however long the cache is.
+static int general_splits(int n_seqs, int max_count, int heads, int kv_heads, int max_keys, int window, int first) {
   const int G = heads / kv_heads, rows = general_rows(max_count, G);
   const long long tiles = ((long long)max_count * G + rows - 1) / rows * kv_heads * n_seqs;
   long long splits = 4ll * sm_count() / (tiles > 0 ? tiles : 1);
-  const long long most = (max_keys + kGenKeys - 1) / kGenKeys;
+  long long keys = max_keys;
+  if (window > 0) keys = std::min(keys, (long long)first + window + std::min(max_count, (rows + G - 2) / G + 1) - 1);
+  const long long most = (keys + kGenKeys - 1) / kGenKeys;
   splits = splits < most ? splits : most;
   return splits < 1 ? 1 : splits > 64 ? 64 : (int)splits;
 }
@@ -665,7 +668,7 @@ extern "C" long long slb_attention_kept_scratch(long long tokens, int n_seqs, in
   const int form = kept_form(tokens, max_count, heads, kv_heads, head_dim, max_keys, dtype, weights != 0);
   if (form == kKeptFew) return kept_few_floats(tokens, n_seqs, max_count, heads, kv_heads, head_dim, max_keys, weights != 0);
   if (form == kKeptTc) return weights ? tokens * heads : 0;
-  const int splits = general_splits(n_seqs, max_count, heads, kv_heads, max_keys);
+  const int splits = general_splits(n_seqs, max_count, heads, kv_heads, max_keys, 0, 0);      // (under a window no more)
   return (weights ? tokens * heads : 0) + (splits > 1 ? (long long)splits * tokens * heads * (head_dim + 2) : 0);
 }
 
@@ -726,7 +729,7 @@ extern "C" int slb_attention_kept(const KeptCall* call) {
     a.lse = c.scratch;
     a.scratch = c.scratch + tokens * heads;
   }
-  a.splits = general_splits(n_seqs, max_count, heads, kv_heads, max_keys);
+  a.splits = general_splits(n_seqs, max_count, heads, kv_heads, max_keys, window, first);
   int rc = dtype == kF32 ? general<float>(a, max_count, tokens, s) : general<__nv_bfloat16>(a, max_count, tokens, s);
   if (rc || !gather) return rc;
   return dtype == kF32 ? general_weights<float>(a, max_count, max_keys, s) : general_weights<__nv_bfloat16>(a, max_count, max_keys, s);

@@ -116,3 +116,12 @@ def test_a_query_that_is_not_a_number_spoils_only_what_it_sees(dtype, heads, kv_
         a, b = got[s, :, :p + c].double(), want_w[s, :, :p + c]
         assert torch.equal(torch.isnan(a), torch.isnan(b)), (s, torch.isnan(a).sum(-1).tolist(), torch.isnan(b).sum(-1).tolist())
         assert bool(((a - b).abs() <= 5e-5 * b.abs() + 1e-7)[~torch.isnan(b)].all())
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim", [KINDS[0], KINDS[1], KINDS[4]], ids=[KIND_IDS[0], KIND_IDS[1], KIND_IDS[4]])
+@pytest.mark.parametrize("window,first", [(1, 0), (63, 1), (64, 64), (65, 3), (300, 130)])
+@pytest.mark.parametrize("count", [1, 4, 23, 70])
+def test_short_windows_on_a_long_table(dtype, heads, kv_heads, dim, window, first, count):
+    """Shares of the keys go by what a tile sees, not by the table's length (no promise of a length is made)."""
+    step = Step(dtype, heads, kv_heads, dim, [1500, 0, 64], [count, 1, max(1, count - 1)], window, first, seed=15)
+    step.check(weights=True, lse=True, promise=False)
