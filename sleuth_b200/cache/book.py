@@ -17,7 +17,7 @@ kept here.
   back before the sequence ends.
 * Under a ``budget`` a sequence holds at most so many rows after a step (which ones, the device decides for each layer and key/value head:
   csrc/cache_evict.cu); rows are then no longer positions, and ``seen[slot]`` counts the tokens that went through. Without a budget
-  ``seen`` equals ``lengths``.
+  ``seen`` is ``lengths``.
 * ``lengths[slot]`` is the number of tokens the sequence holds. Stale contents of a reused page are
   never read: every kernel reads positions below the length only (the reference relies on the same
   idea: entries past ``pos`` are simply overwritten, sleuth/forge/infer/kv_cache.py:52-64).
@@ -110,8 +110,9 @@ class CacheBook:
         self.stride = stride
         self.max_len = stride * PAGE_TOKENS
         self.lengths = np.zeros(max_slots, dtype=np.int32)
-        self.seen = np.zeros(max_slots, dtype=np.int32)
         self.budget = int(budget)
+        # (one and the same without a budget: nothing is to be counted twice then)
+        self.seen = np.zeros(max_slots, dtype=np.int32) if self.budget else self.lengths
         self._free_slots = list(range(max_slots - 1, -1, -1))
         self._live = np.zeros(max_slots, dtype=bool)
         self.groups = [GroupBook(w, PagePool(n_pages), np.full((max_slots, stride), -1, dtype=np.int32),
@@ -223,14 +224,15 @@ class CacheBook:
     def commit(self, slots, new_lengths) -> None:
         """The step has been issued: set the lengths and let windowed groups give pages back."""
         for s, n in zip(slots, new_lengths):
-            self.seen[s] += n - int(self.lengths[s])
-            if self.budget and n > self.budget:
-                n = self.budget
-                for g in self.groups:
-                    row = g.table[s]
-                    behind = row[pages_for(n):]
-                    g.pool.give(behind[behind >= 0].tolist())
-                    behind[:] = -1
+            if self.budget:
+                self.seen[s] += n - int(self.lengths[s])
+                if n > self.budget:
+                    n = self.budget
+                    for g in self.groups:
+                        row = g.table[s]
+                        behind = row[pages_for(n):]
+                        g.pool.give(behind[behind >= 0].tolist())
+                        behind[:] = -1
             self.lengths[s] = n
             for g in self.groups:
                 if g.window:

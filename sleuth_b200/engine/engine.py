@@ -197,9 +197,10 @@ class Engine:
         return min(g.pool.free for g in self.cache.book.groups) if self.cache.book.groups else 1 << 30
 
     def pages_needed(self, slots, new_lengths) -> int:
-        # (tokens of the texts -> rows of the cache: the same numbers unless a budget took rows out)
         book = self.cache.book
-        need = book.pages_needed(slots, [n - int(book.seen[s]) + int(book.lengths[s]) for s, n in zip(slots, new_lengths)])
+        if book.budget:      # tokens of the texts -> rows of the cache
+            new_lengths = [n - int(book.seen[s]) + int(book.lengths[s]) for s, n in zip(slots, new_lengths)]
+        need = book.pages_needed(slots, new_lengths)
         return max(need) if need else 0
 
     def length(self, slot: int) -> int:

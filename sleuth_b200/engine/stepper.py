@@ -213,7 +213,7 @@ class Stepper:
         order = np.argsort(np.asarray(dest, dtype=np.int64), kind="stable") if dest else np.zeros(0, dtype=np.int64)
         rows_a = np.asarray(rows, dtype=np.int32)[order] if rows else np.zeros(0, dtype=np.int32)
         dest_a = np.asarray(dest, dtype=np.int64)[order] if dest else np.zeros(0, dtype=np.int64)
-        b = self.meta.upload(c_slots, c_past, c_counts, tokens, rows_a, book.tables_for(c_slots), seen=book.seen[c_slots])
+        b = self.meta.upload(c_slots, c_past, c_counts, tokens, rows_a, book.tables_for(c_slots), seen=book.seen[c_slots] if book.budget else None)
         W = rows_a.shape[0]
         if self._chunk_by_graph(b, W, out, dest_a):
             pass
@@ -315,7 +315,7 @@ class Stepper:
         if floats is None:
             floats = np.zeros(n, dtype=np.float32)
         b = self.meta.upload(slots, past, [1] * n, tokens, rows, book.tables_for(slots), floats=floats,
-                             feed_map=feed_map, seen=book.seen[slots])
+                             feed_map=feed_map, seen=book.seen[slots] if book.budget else None)
         self.last_batch = b
         if self._decode_logits is None or self._decode_logits.shape[0] < n:
             cap = max(n, 8 if self._decode_logits is None else 2 * self._decode_logits.shape[0])
