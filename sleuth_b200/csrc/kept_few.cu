@@ -1,14 +1,16 @@
 // Attention over a cache of bounded size (kept.cuh) for steps of few tokens, bfloat16, heads of 64 and 128: single tokens, short turns.
 //
 // What such a step costs is the read of the keys and values that its queries see, so the work is the pages: every sequence has so many
-// (page, kv head, tile of rows) units, and each block takes an equal run of the list of all units, whatever the sequences' lengths. A
-// (sequence, kv head, tile) that lies in one run is finished by its block; the others' shares wait in scratch for a second kernel.
+// (kv head, page) units, and each block takes an equal run of the list of all units, whatever the sequences' lengths. A
+// (sequence, kv head) that lies in one run is finished by its block; the others' shares wait in scratch for a second kernel.
 //   * the last warp: asks TMA for the pages of the block's run, keys and values, into a ring (32 KB a stage at heads of 128; about 190 KB an SM,
 //     where 43 KB hide a memory latency of a microsecond at full bandwidth);
-//   * the other warps: mma.sync on the pages as they land. A tile is R times 16 rows, row r being token r / G, query head r % G of the group.
+//   * the other warps: mma.sync on the pages as they land. A (sequence, kv head) has up to R times 16 rows, row r being token r / G, query head r % G of
+//     the group; R is 1, 2 or 4, by the longest share of a sequence, and all rows meet a page at once.
 //     R = 1: four warps, a warp 16 of a page's keys, and two blocks an SM, so that one reads while the other joins its warps' results;
 //     R = 2 and 4: eight warps, four or two for each 16 rows, a block an SM. Each warp keeps a running maximum, sum and weighted values of its own
-//     keys; they are joined at the end of a (sequence, kv head, tile), in the order of the warps.
+//     keys; they are joined at the end of a (sequence, kv head), in the order of the warps. The weights of the softmax are rounded to bfloat16
+//     for their product, as in the prompt kernels (the instruction takes no wider ones beside bfloat16 values); sums and maxima stay in 32 bits.
 // (tcgen05 has nothing to win here: its tiles are 128 rows high, and rows are 2 to 64.)
 // With weights wanted the scores go to scratch as they are formed (log2 units, 4 bytes for each row and key against 4 x head_dim for the
 // key and value: 1 to 4 per cent more bytes), because the denominators are known at the end only; the second kernel turns them into weights.
@@ -17,7 +19,7 @@
 // Measured (device time): 64 sequences of 150 to 4,096 rows, a window of 2,048, 32 / 8 heads of 128, 79 us = 5.2 TB/s of 6.46; six of 9,000 to 30,000
 // 78 us = 5.8 TB/s, with weights 94; eight of 2,049 with weights, 16 / 8 heads, by clusters 15.6 us = 4.4 TB/s (rows that L2 holds); a token on 1,028
 // rows 7.9 us: launch, tables, one page, two meetings.
-// Keys that no row of the tile sees (stale rows of the last page, what lies between the first rows and the window) have their values
+// Keys that no row of the 16 sees (stale rows of the last page, what lies between the first rows and the window) have their values
 // replaced by zeros in registers, so that infinities or NaN in them do not meet a zero weight.
 #include <math.h>
 
@@ -31,7 +33,7 @@ namespace slb {
 
 constexpr int few_warps(int R) { return R == 1 ? 4 : 8; }
 constexpr int few_blocks_an_sm(int R) { return R == 1 ? 2 : 1; }
-constexpr int kFewMostRows = 256;      // rows of a (sequence, kv head) that the second kernel takes
+constexpr int kFewMostRows = 64;      // rows of a (sequence, kv head)
 
 // Shared memory: the ring (keys then values of a stage), queries [16 R][HD] as the ring's tiles lie, the warps' results [warps][rows][HD] float
 // and [warps][rows][2], barriers, in clusters what the blocks exchange. As many stages as fit.
@@ -65,11 +67,10 @@ static FewLayout few_layout(int HD, int R, int rows, int cluster_pages = 0, bool
 struct FewArgs {
   KeptArgs k;
   float scale_log2;
-  int max_tiles;        // tiles of the longest share
   int max_count;        // no sequence brings more tokens (the room below is made for that)
   float* part;          // [blocks][2][16 R][HD] weighted values, then [blocks][2][16 R][2] maximum and sum
   float* part_ml;
-  int2* info;           // [n, kv_heads, max_tiles] first block and number of blocks
+  int2* info;           // [n, kv_heads] first block and number of blocks
   float* lse2;          // [tokens, H] denominators in log2 units
   float* scores;        // [tokens, H, score_stride] or null
   long long score_stride;
@@ -143,11 +144,7 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 
   // units of the sequences, and where this block's run begins
   const int G = a.heads / a.kv_heads;
-  auto tiles_of = [&](int count) { return (count * G + ROWS - 1) / ROWS; };
-  auto units_of = [&](int s) -> long long {
-    const int c = min(a.counts[s], fa.max_count);
-    return (long long)PageRun(a.past[s], c, a.window, a.first).count * a.kv_heads * tiles_of(c);
-  };
+  auto units_of = [&](int s) -> long long { return (long long)PageRun(a.past[s], min(a.counts[s], fa.max_count), a.window, a.first).count * a.kv_heads; };
   // CLUSTER: the blocks of a cluster share the pages of one (sequence, kv head); `u` counts the pages of that pair alone
   int seq, rank = 0;
   long long seq_first, u, u_hi, blocks = 1, total = 0;
@@ -211,12 +208,11 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     while (u < u_hi && ok) {
       const int count = min(a.counts[seq], fa.max_count), past = a.past[seq];
       const PageRun run(past, count, a.window, a.first);
-      const long long units = (long long)run.count * a.kv_heads * tiles_of(count);
+      const long long units = (long long)run.count * a.kv_heads;
       const int* table = a.block_table + (size_t)seq * a.table_stride;
-      const int n_tiles = tiles_of(count);
       const long long stop = min(u_hi, seq_first + units);
       while (u < stop && ok) {
-        const int off = (int)((u - seq_first) % run.count), pair = (int)((u - seq_first) / run.count), kh = pair / n_tiles;
+        const int off = (int)((u - seq_first) % run.count), kh = (int)((u - seq_first) / run.count);
         const int n = (int)min((long long)(run.count - off), stop - u);
         for (int i0 = 0; i0 < n && ok; i0 += 32) {
           const int mine = i0 + lane < n ? table[run.page(off + i0 + lane)] : 0;
@@ -252,7 +248,7 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 
   // ---- the products ----
   const int g = lane >> 2, t4 = lane & 3;
-  const int rt = warp % R, key_in = warp / R * KW;      // 16 rows of the tile; which keys of a page
+  const int rt = warp % R, key_in = warp / R * KW;      // which 16 of the rows; which keys of a page
   auto sync = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory"); };
   int st = 0, lap = 0;
   bool ok = true;
@@ -265,19 +261,18 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   while (u < u_hi) {
     const int count = min(a.counts[seq], fa.max_count), past = a.past[seq];
     const PageRun run(past, count, a.window, a.first);
-    const int n_tiles = tiles_of(count);
-    const long long units = (long long)run.count * a.kv_heads * n_tiles;
+    const long long units = (long long)run.count * a.kv_heads;
     const int tok0 = a.seq_start[seq];
     const long long stop = min(u_hi, seq_first + units);
     while (u < stop) {
-      const int off = (int)((u - seq_first) % run.count), pair = (int)((u - seq_first) / run.count), kh = pair / n_tiles, tile = pair % n_tiles;
+      const int off = (int)((u - seq_first) % run.count), kh = (int)((u - seq_first) / run.count);
       const int n = (int)min((long long)(run.count - off), stop - u);
-      const int row0 = tile * ROWS, rows = min(ROWS, count * G - row0);
-      // queries (the previous tile's results have been read: every warp has passed its last barrier)
+      const int rows = min(ROWS, count * G);
+      // queries (the previous kv head's results have been read: every warp has passed its last barrier)
       for (int e = tid; e < ROWS * (HD / 8); e += WARPS * 32) {
-        const int r = e / (HD / 8), col = (e % (HD / 8)) * 8, Rr = row0 + r;
+        const int r = e / (HD / 8), col = (e % (HD / 8)) * 8;
         uint4 v = make_uint4(0, 0, 0, 0);
-        if (r < rows) v = *reinterpret_cast<const uint4*>((const __nv_bfloat16*)a.q + ((size_t)(tok0 + Rr / G) * a.heads + kh * G + Rr % G) * HD + col);
+        if (r < rows) v = *reinterpret_cast<const uint4*>((const __nv_bfloat16*)a.q + ((size_t)(tok0 + r / G) * a.heads + kh * G + r % G) * HD + col);
         *reinterpret_cast<uint4*>(smem + L.q_off + tile_at<ROWS>(r, col)) = v;
       }
       sync();
@@ -291,14 +286,14 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       float* score_row[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int r = rt * 16 + g + 8 * h, Rr = row0 + r;
-        pos[h] = r < rows ? past + Rr / G : -1;
+        const int r = rt * 16 + g + 8 * h;
+        pos[h] = r < rows ? past + r / G : -1;
         lo[h] = window_lo(pos[h], a.window);
         if (CLUSTER) score_row[h] = a.weights && r < rows ? reinterpret_cast<float*>(smem + L.score_off) + r * L.score_pitch : nullptr;
-        else score_row[h] = fa.scores && r < rows ? fa.scores + ((size_t)(tok0 + Rr / G) * a.heads + kh * G + Rr % G) * fa.score_stride : nullptr;
+        else score_row[h] = fa.scores && r < rows ? fa.scores + ((size_t)(tok0 + r / G) * a.heads + kh * G + r % G) * fa.score_stride : nullptr;
       }
       // what the 16 rows of this warp see: all of them from see_lo (or below `first`) to see_hi, none beyond any_hi or below any_lo
-      const int r_first = row0 + rt * 16, r_last = min(row0 + rows, r_first + 16) - 1;
+      const int r_first = rt * 16, r_last = min(rows, r_first + 16) - 1;
       const bool idle = r_first > r_last;
       const int any_lo = window_lo(past + r_first / G, a.window), any_hi = past + r_last / G;
       const int all_lo = window_lo(any_hi, a.window), all_hi = past + r_first / G;
@@ -438,12 +433,12 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       }
       sync();
       const bool begins = off == 0, complete = begins && n == run.count;
-      const long long pair_lo = seq_first + (long long)pair * run.count;
+      const long long pair_lo = seq_first + (long long)kh * run.count;
       const int first_block = blockIdx.x;
       if (!CLUSTER && begins && tid == 0) {
         const long long last = pair_lo + run.count - 1;
         const int last_block = (int)(((last + 1) * blocks - 1) / total);
-        fa.info[((size_t)seq * a.kv_heads + kh) * fa.max_tiles + tile] = make_int2(first_block, last_block - first_block + 1);
+        fa.info[(size_t)seq * a.kv_heads + kh] = make_int2(first_block, last_block - first_block + 1);
       }
       const size_t slot = ((size_t)blockIdx.x * 2 + (begins ? 1 : 0)) * ROWS;
       for (int e = tid; e < rows * (HD / 4); e += WARPS * 32) {
@@ -462,8 +457,7 @@ kept_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
           sum += ml[at * 2 + 1] * f;
           acc.x += v.x * f; acc.y += v.y * f; acc.z += v.z * f; acc.w += v.w * f;
         }
-        const int Rr = row0 + r;
-        const size_t row = (size_t)(tok0 + Rr / G) * a.heads + kh * G + Rr % G;
+        const size_t row = (size_t)(tok0 + r / G) * a.heads + kh * G + r % G;
         if (CLUSTER) {
           float* slot = reinterpret_cast<float*>(smem + L.part_off + r * (HD * 4 + 16));
           *reinterpret_cast<float4*>(slot + d) = acc;
@@ -580,17 +574,16 @@ __global__ void __launch_bounds__(256, 4) kept_few_finish_kernel(FewArgs fa) {
     }
     return;
   }
-  const int2* info = fa.info + ((size_t)seq * a.kv_heads + kh) * fa.max_tiles;
-  auto row_of = [&](int Rr) { return (size_t)(tok0 + Rr / G) * a.heads + kh * G + Rr % G; };
-  auto slot_of = [&](int2 in, int i) { return ((size_t)(in.x + i) * 2 + (i == 0 ? 1 : 0)) * ROWS; };
+  const int2 in = fa.info[(size_t)seq * a.kv_heads + kh];
+  auto row_of = [&](int r) { return (size_t)(tok0 + r / G) * a.heads + kh * G + r % G; };
+  auto slot_of = [&](int i) { return ((size_t)(in.x + i) * 2 + (i == 0 ? 1 : 0)) * ROWS; };
   const bool outputs = (int)blockIdx.x < fa.out_blocks;
   const int key_begin = ((int)blockIdx.x - fa.out_blocks) * fa.keys_a_block, end = past + count;
   if (!outputs && key_begin >= end) return;
   if (outputs) {
+    if (in.y == 1) return;      // its block has finished it
     for (int e = blockIdx.x * 256 + tid; e < rows_total * (HD / 4); e += fa.out_blocks * 256) {
-      const int Rr = e / (HD / 4), d = (e % (HD / 4)) * 4;
-      const int2 in = info[Rr / ROWS];
-      if (in.y == 1) continue;
+      const int r = e / (HD / 4), d = (e % (HD / 4)) * 4;
       float M = -INFINITY, L = 0.0f;
       float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       for (int i0 = 0; i0 < in.y; i0 += 8) {
@@ -598,7 +591,7 @@ __global__ void __launch_bounds__(256, 4) kept_few_finish_kernel(FewArgs fa) {
         float4 v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const size_t at = slot_of(in, i0 + i < in.y ? i0 + i : 0) + Rr % ROWS;
+          const size_t at = slot_of(i0 + i < in.y ? i0 + i : 0) + r;
           p[i] = *reinterpret_cast<const float2*>(fa.part_ml + at * 2);
           v[i] = *reinterpret_cast<const float4*>(fa.part + at * HD + d);
           if (i0 + i >= in.y) p[i].x = -INFINITY;
@@ -623,14 +616,13 @@ __global__ void __launch_bounds__(256, 4) kept_few_finish_kernel(FewArgs fa) {
       uint2 pk;
       pk.x = pack_bf16(acc.x * inv, acc.y * inv);
       pk.y = pack_bf16(acc.z * inv, acc.w * inv);
-      *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + row_of(Rr) * HD + d) = pk;
-      if (d == 0 && a.lse) a.lse[row_of(Rr)] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+      *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + row_of(r) * HD + d) = pk;
+      if (d == 0 && a.lse) a.lse[row_of(r)] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
     }
     return;
   }
   // denominators, a thread a row
   if (tid < rows_total) {
-    const int2 in = info[tid / ROWS];
     const size_t row = row_of(tid);
     float v;
     if (in.y == 1) {
@@ -641,7 +633,7 @@ __global__ void __launch_bounds__(256, 4) kept_few_finish_kernel(FewArgs fa) {
         float2 p[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          p[i] = *reinterpret_cast<const float2*>(fa.part_ml + (slot_of(in, i0 + i < in.y ? i0 + i : 0) + tid % ROWS) * 2);
+          p[i] = *reinterpret_cast<const float2*>(fa.part_ml + (slot_of(i0 + i < in.y ? i0 + i : 0) + tid) * 2);
           if (i0 + i >= in.y) p[i] = make_float2(-INFINITY, 0.0f);
         }
         float top = M;
@@ -714,12 +706,13 @@ __global__ void __launch_bounds__(256, 4) kept_few_finish_kernel(FewArgs fa) {
   }
 }
 
+// R: kept_few_takes admits 64 rows.
 static int few_row_tiles(int max_count, int G) { return max_count * G <= 16 ? 1 : max_count * G <= 32 ? 2 : 4; }
 
 // Where the pieces of scratch lie, in floats.
 struct FewScratch {
   long long part, part_ml, info, lse2, scores, total, score_stride;
-  int max_tiles, blocks, cluster, cluster_pages;
+  int blocks, cluster, cluster_pages;
 };
 
 // Whether blocks of a cluster share each (sequence, kv head), and how many: then no second kernel and no scratch is needed (a chat's token on 17 pages:
@@ -746,8 +739,7 @@ static FewScratch few_scratch(long long tokens, int n_seqs, int max_count, int h
   const int G = heads / kv_heads, R = few_row_tiles(max_count, G);
   few_cluster(n_seqs, max_count, heads, kv_heads, head_dim, max_keys, weights, window, first, f);
   if (f.cluster) return f;
-  f.max_tiles = (max_count * G + 16 * R - 1) / (16 * R);
-  const long long units = (long long)n_seqs * kv_heads * f.max_tiles * ((max_keys + 63) / 64);
+  const long long units = (long long)n_seqs * kv_heads * ((max_keys + 63) / 64);
   const long long most = (long long)sm_count() * few_blocks_an_sm(R);
   f.blocks = (int)(units < most ? units : most);      // as many as run at once; none without a page
   const long long slots = 2ll * f.blocks * 16 * R;
@@ -755,7 +747,7 @@ static FewScratch few_scratch(long long tokens, int n_seqs, int max_count, int h
   auto take = [&](long long n) { const long long o = at; at += (n + 3) & ~3ll; return o; };
   f.part = take(slots * head_dim);
   f.part_ml = take(slots * 2);
-  f.info = take(2ll * n_seqs * kv_heads * f.max_tiles);
+  f.info = take(2ll * n_seqs * kv_heads);
   f.lse2 = weights ? take(tokens * heads) : 0;
   f.score_stride = (max_keys + 3) & ~3;
   f.scores = weights ? take(tokens * heads * f.score_stride) : 0;
@@ -811,7 +803,7 @@ static int encode_pool(CUtensorMap* map, const void* base, long long rows, int h
 constexpr long long kMostScores = 1ll << 28;      // floats of scratch for scores: a gigabyte
 
 bool kept_few_takes(long long tokens, int max_count, int heads, int kv_heads, int head_dim, int max_keys, int dtype, bool weights) {
-  return dtype == kBF16 && (head_dim == 64 || head_dim == 128) && (long long)max_count * (heads / kv_heads) <= 64 &&
+  return dtype == kBF16 && (head_dim == 64 || head_dim == 128) && (long long)max_count * (heads / kv_heads) <= kFewMostRows &&
          (!weights || tokens * heads * max_keys <= kMostScores);
 }
 
@@ -835,7 +827,6 @@ int kept_few(const KeptArgs& a, long long tokens, int max_count, int max_keys, l
   FewArgs fa{};
   fa.k = a;
   fa.scale_log2 = a.scale * kKeptLog2e;
-  fa.max_tiles = f.max_tiles;
   fa.max_count = max_count;
   fa.cluster = f.cluster;
   fa.cluster_pages = f.cluster_pages;
