@@ -6,7 +6,9 @@ given back (attention with a sliding window and first tokens that stay visible).
 ``KeepPolicy(budget=B, first=f, recent=r)``: a query sees all that its layer still holds. After every step each key/value head of each
 layer keeps at most ``B`` tokens of a sequence: the first ``f``, the latest ``r`` (half of ``B`` when not given) and, of the others, those to
 which the queries so far have given the largest sum of softmax weights. A prompt goes in portions of ``portion`` tokens, with an
-eviction after each, so a sequence never holds more than ``B + portion`` rows. Tokens keep the rotation of their own position.
+eviction after each, so a sequence never holds more than ``B + portion`` rows, nor more than the longest text has tokens. Tokens keep the rotation
+of their own position. Beside the cache's pages every slot (``max_sequences``) takes 8 bytes a row, key/value head and layer for what its rows have
+gathered and their positions; the number of slots goes by the pages when none is named, so a program that knows how many texts it serves at once names it.
 
 ``Engine.from_pretrained(folder, keep=KeepPolicy(...))``, ``sleuth_b200.load(folder, keep=...)`` or ``generate --keep-window/--keep-budget``.
 """
@@ -49,3 +51,7 @@ class KeepPolicy:
     def most_rows(self) -> int:
         """Rows that a sequence holds at most under a budget."""
         return self.budget + self.portion
+
+    def rows_for(self, longest: int) -> int:
+        """The same where no text is longer than ``longest`` tokens."""
+        return min(self.most_rows, longest)

@@ -115,7 +115,7 @@ def cmd_generate(a) -> int:
     if a.keep_window or a.keep_budget:
         from .cache.keep import KeepPolicy
         keep = KeepPolicy(budget=a.keep_budget, window=a.keep_window, first=a.keep_first, recent=a.keep_recent)
-    per_prompt = min(a.max_seq_len, keep.most_rows) if keep is not None and keep.budget else a.max_seq_len
+    per_prompt = keep.rows_for(a.max_seq_len) if keep is not None and keep.budget else a.max_seq_len
     engine = load(a.path, dtype=_dtype_name(a.dtype), max_seq_len=a.max_seq_len, device=device,
                   max_tokens=max(1, len(prompts)) * (-(-per_prompt // 64) * 64 if keep is not None else per_prompt), keep=keep)
     sampling = SamplingConfig(a.temperature, a.top_k, a.top_p, a.min_p, a.repetition_penalty, a.repeat_last_n,

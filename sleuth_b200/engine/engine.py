@@ -63,7 +63,7 @@ def _check_keep(keep: KeepPolicy | None, spec) -> None:
 
 def _cache_for(model, keep: KeepPolicy | None, max_tokens, max_seq_len: int, dtype, device, max_sequences) -> PagedCache:
     if keep is not None and keep.budget:
-        rows = keep.most_rows
+        rows = keep.rows_for(max_seq_len)
         return PagedCache(model.cache_requests, 8 * rows if max_tokens is None else max_tokens, rows, dtype, device, max_sequences, keep.budget)
     return PagedCache(model.cache_requests, 8 * max_seq_len if max_tokens is None else max_tokens, max_seq_len, dtype, device, max_sequences)
 
@@ -79,7 +79,7 @@ class Engine:
         self.max_len = int(max_seq_len)
         self.keep = keep
         budget = keep is not None and keep.budget > 0
-        self.max_rows = keep.most_rows if budget else None       # rows of the cache that a sequence holds at most, if the policy bounds them
+        self.max_rows = keep.rows_for(self.max_len) if budget else None       # rows of the cache that a sequence holds at most, if the policy bounds them
         self.stepper = Stepper(model, cache, device, max_len=self.max_len, max_step_tokens=max_step_tokens,
                                use_graphs=use_graphs, portion=keep.portion if budget else 0)
         self.sampler = Sampler(device, model.vocab)

@@ -169,7 +169,7 @@ class GQAAttention(Part):
         if self.keep is not None and self.keep.window:
             return KVRequest(s.kv_heads, s.head_dim, self.keep.window, first=self.keep.first)
         if self.keep is not None:      # beside keys and values, for every row what it has gathered and the position of its token
-            shape = (s.kv_heads, 64 * pages_for(self.keep.most_rows))
+            shape = (s.kv_heads, 64 * pages_for(self.keep.rows_for(self.ctx.max_positions)))
             return BundleRequest((("kv", KVRequest(s.kv_heads, s.head_dim)), ("gathered", StateRequest(shape)),
                                   ("positions", StateRequest(shape, torch.int32))))
         return KVRequest(s.kv_heads, self.key_run, self.reach, 0 if self.value_run == self.key_run else self.value_run)

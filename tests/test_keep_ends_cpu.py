@@ -1,8 +1,15 @@
 """What a cache of bounded size asks of the host where its policy does not apply, and at the ends of its numbers (no GPU)."""
 
 import numpy as np
+import torch
 
+import tiny
 from sleuth_b200.cache.book import CacheBook
+from sleuth_b200.cache.keep import KeepPolicy
+from sleuth_b200.config.registry import parse_config
+from sleuth_b200.engine.engine import _cache_for
+from sleuth_b200.engine.model import Model
+from sleuth_b200.parts.base import BuildContext
 
 
 def test_without_a_budget_tokens_and_rows_are_counted_once():
@@ -24,3 +31,19 @@ def test_without_a_budget_tokens_and_rows_are_counted_once():
         assert (int(bounded.seen[s]), int(bounded.lengths[s])) == (seen, min(rows, 70))
     bounded.close([s])
     assert not np.any(bounded.seen) and not np.any(bounded.lengths)
+
+
+def test_a_sequence_holds_no_more_rows_than_its_text_has_tokens():
+    """``portion`` without a limit, a budget above every text: what the cache reserves goes by the longest text then."""
+    most = 2 ** 31 - 1
+    assert KeepPolicy(budget=2048).rows_for(32768) == 2560
+    assert KeepPolicy(budget=2048).rows_for(1000) == 1000
+    assert KeepPolicy(budget=100, portion=most).rows_for(4096) == 4096
+    assert KeepPolicy(budget=most).rows_for(4096) == 4096
+    arch, cfg, _ = parse_config(tiny.CONFIGS["A"])
+    spec = arch.model_spec(cfg)
+    for policy, longest, rows in ((KeepPolicy(budget=most, portion=most), 320, 320), (KeepPolicy(budget=70, portion=60), 4096, 192), (KeepPolicy(budget=70, portion=60), 100, 128)):
+        model = Model(spec, BuildContext(device="cpu", dtype=torch.float32, max_positions=-(-longest // 64) * 64, keep=policy))
+        shapes = {name: getattr(r, "shape", None) for name, r in model.cache_requests[0].parts}
+        cache = _cache_for(model, policy, None, longest, torch.float32, "cpu", 2)
+        assert shapes["gathered"] == shapes["positions"] == (cfg.kv_heads, rows) and cache.stride * 64 == rows

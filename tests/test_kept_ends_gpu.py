@@ -125,3 +125,27 @@ def test_short_windows_on_a_long_table(dtype, heads, kv_heads, dim, window, firs
     """Shares of the keys go by what a tile sees, not by the table's length (no promise of a length is made)."""
     step = Step(dtype, heads, kv_heads, dim, [1500, 0, 64], [count, 1, max(1, count - 1)], window, first, seed=15)
     step.check(weights=True, lse=True, promise=False)
+
+
+def test_an_engine_with_the_largest_policies(tmp_path):
+    """A budget, a portion, a window or first tokens without a limit are the whole cache."""
+    import numpy as np
+
+    import sleuth_b200 as sb
+    import tiny
+    cfg = tiny.CONFIGS["D"]
+    sb.write_random_model(tmp_path, cfg, seed=9, dtype=torch.float32)
+    prompts = [np.random.default_rng(1).integers(0, cfg["vocab_size"], n).tolist() for n in (150, 9)]
+    rows = []
+    for keep in (None, sb.KeepPolicy(budget=MOST, portion=MOST), sb.KeepPolicy(budget=MOST, first=MOST, recent=0, portion=40), sb.KeepPolicy(window=MOST, first=4),
+                 sb.KeepPolicy(window=7, first=MOST)):
+        engine = sb.load(tmp_path, dtype="fp32", max_seq_len=300, device="cuda:0", keep=keep)
+        assert engine.cache.stride == 5
+        slots = engine.open(2)
+        out = [engine.step([(s, p, (len(p) - 1,)) for s, p in zip(slots, prompts)]).cpu()]
+        for turn in ([3], [4, 5, 6], [7]):
+            out.append(engine.step([(s, turn, (len(turn) - 1,)) for s in slots]).cpu().clone())
+        rows.append(torch.cat(out))
+        engine.stepper.check_status()
+    for r in rows[1:]:      # (sums of at most a few hundred terms in another order)
+        assert float((r - rows[0]).abs().max()) <= 1e-5 * float(rows[0].abs().max())
