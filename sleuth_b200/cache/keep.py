@@ -31,6 +31,8 @@ class KeepPolicy:
             v = getattr(self, name)
             if not isinstance(v, int) or isinstance(v, bool) or v < 0:
                 raise ValueError(f"keep: {name} must be a whole number, not negative, got {v!r}")
+            if v >= 1 << 31:
+                raise ValueError(f"keep: {name} must be below 2^31, got {v}")
         if (self.budget > 0) == (self.window > 0):
             raise ValueError(f"keep: give a budget or a window, one of them (budget {self.budget}, window {self.window})")
         if self.recent is not None and (not isinstance(self.recent, int) or isinstance(self.recent, bool) or self.recent < 0):

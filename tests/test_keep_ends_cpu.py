@@ -1,6 +1,7 @@
 """What a cache of bounded size asks of the host where its policy does not apply, and at the ends of its numbers (no GPU)."""
 
 import numpy as np
+import pytest
 import torch
 
 import tiny
@@ -47,3 +48,12 @@ def test_a_sequence_holds_no_more_rows_than_its_text_has_tokens():
         shapes = {name: getattr(r, "shape", None) for name, r in model.cache_requests[0].parts}
         cache = _cache_for(model, policy, None, longest, torch.float32, "cpu", 2)
         assert shapes["gathered"] == shapes["positions"] == (cfg.kv_heads, rows) and cache.stride * 64 == rows
+
+
+@pytest.mark.parametrize("name", ["budget", "window", "first", "portion"])
+def test_numbers_that_no_row_can_have_are_refused_at_once(name):
+    kw = dict(budget=50) if name in ("first", "portion") else {}
+    with pytest.raises(ValueError):
+        KeepPolicy(**{**kw, name: 2 ** 31})
+    with pytest.raises(ValueError):
+        KeepPolicy(budget=50, recent=2 ** 31)
