@@ -117,7 +117,9 @@ def cmd_generate(a) -> int:
         keep = KeepPolicy(budget=a.keep_budget, window=a.keep_window, first=a.keep_first, recent=a.keep_recent)
     per_prompt = keep.rows_for(a.max_seq_len) if keep is not None and keep.budget else a.max_seq_len
     engine = load(a.path, dtype=_dtype_name(a.dtype), max_seq_len=a.max_seq_len, device=device,
-                  max_tokens=max(1, len(prompts)) * (-(-per_prompt // 64) * 64 if keep is not None else per_prompt), keep=keep)
+                  max_tokens=max(1, len(prompts)) * (-(-per_prompt // 64) * 64 if keep is not None else per_prompt), keep=keep,
+                  # (a policy's state is kept for every slot)
+                  max_sequences=None if keep is None else max(1, len(prompts)))
     sampling = SamplingConfig(a.temperature, a.top_k, a.top_p, a.min_p, a.repetition_penalty, a.repeat_last_n,
                               a.no_repeat_ngram)
     n_params = sum(int(torch.tensor(d.shape).prod()) for d in engine.model.expected().values())

@@ -57,3 +57,26 @@ def test_numbers_that_no_row_can_have_are_refused_at_once(name):
         KeepPolicy(**{**kw, name: 2 ** 31})
     with pytest.raises(ValueError):
         KeepPolicy(budget=50, recent=2 ** 31)
+
+
+def test_the_command_line_reserves_state_for_its_prompts_alone(monkeypatch):
+    from sleuth_b200 import cli
+    from sleuth_b200.engine import engine
+
+    class Loaded(Exception):
+        pass
+
+    def load(path, **kw):
+        raise Loaded(kw)
+
+    monkeypatch.setattr(engine, "load", load)
+
+    def asked(*options):
+        with pytest.raises(Loaded) as e:
+            cli.main(["generate", "m", "--prompt-ids", "1 2; 3 4 5", *options])
+        return e.value.args[0]
+
+    kw = asked("--keep-budget", "2048")
+    assert kw["max_sequences"] == 2 and kw["max_tokens"] == 2 * 2560 and kw["keep"].budget == 2048
+    assert asked("--keep-window", "100")["max_sequences"] == 2
+    assert asked()["max_sequences"] is None and asked()["keep"] is None

@@ -149,3 +149,14 @@ def test_an_engine_with_the_largest_policies(tmp_path):
         engine.stepper.check_status()
     for r in rows[1:]:      # (sums of at most a few hundred terms in another order)
         assert float((r - rows[0]).abs().max()) <= 1e-5 * float(rows[0].abs().max())
+
+
+def test_the_command_line_generates_beyond_its_budget(tmp_path, capsys):
+    import sleuth_b200 as sb
+    import tiny
+    from sleuth_b200.cli import main
+    sb.write_random_model(tmp_path, tiny.CONFIGS["D"], seed=9, dtype=torch.float32)
+    assert main(["generate", str(tmp_path), "--prompt-ids", "1 2 3; 7 8", "--max-new-tokens", "150", "--temperature", "0", "--max-seq-len", "300",
+                 "--keep-budget", "64", "--samples", "2"]) == 0
+    lines = [[int(t) for t in x.split()] for x in capsys.readouterr().out.splitlines() if x and x[0].isdigit()]
+    assert len(lines) == 4 and lines[0] == lines[2] and lines[1] == lines[3] and all(lines)
