@@ -112,7 +112,7 @@ def cmd_generate(a) -> int:
         return 2
     device = "cuda:0" if a.device == "auto" else a.device
     keep = None
-    if a.keep_window or a.keep_budget:
+    if a.keep_window or a.keep_budget or a.keep_recent is not None:
         from .cache.keep import KeepPolicy
         keep = KeepPolicy(budget=a.keep_budget, window=a.keep_window, first=a.keep_first, recent=a.keep_recent)
     per_prompt = keep.rows_for(a.max_seq_len) if keep is not None and keep.budget else a.max_seq_len

@@ -80,3 +80,9 @@ def test_the_command_line_reserves_state_for_its_prompts_alone(monkeypatch):
     assert kw["max_sequences"] == 2 and kw["max_tokens"] == 2 * 2560 and kw["keep"].budget == 2048
     assert asked("--keep-window", "100")["max_sequences"] == 2
     assert asked()["max_sequences"] is None and asked()["keep"] is None
+
+
+def test_the_command_line_does_not_ignore_half_a_policy():
+    from sleuth_b200 import cli
+    with pytest.raises(ValueError):
+        cli.main(["generate", "m", "--prompt-ids", "1 2", "--keep-recent", "100"])
