@@ -1756,8 +1756,10 @@ def attention_kept(q, k_pool, v_pool, out, seq_start, past, counts, block_table,
     bfloat16 an infinity or NaN among the values of a row that some query of the same tile of up to 128 (token, head) rows sees may
     reach the tile's other rows."""
     dt, i32, f32 = q.dtype, torch.int32, torch.float32
-    q_shape, k_shape, (n, stride) = q.shape, k_pool.shape, block_table.shape
-    T, capacity = q_shape[0], 0
+    q_shape, k_shape, t_shape = q.shape, k_pool.shape, block_table.shape
+    _need(len(q_shape) == 3 and len(k_shape) == 4 and len(t_shape) == 2 and (weights is None or weights.dim() == 3),
+          "attention_kept: q is [tokens, heads, head_dim], pools are [pages, kv_heads, 64, head_dim], block_table is [n, pages], weights are [slots, kv_heads, rows]")
+    (n, stride), T, capacity = t_shape, q_shape[0], 0
     if weights is not None:
         if weights_out is None:
             weights_out = weights
@@ -1830,7 +1832,10 @@ def cache_evict(weights, positions, k_pool, v_pool, block_table, past, lengths, 
     positions go (default: in place); places behind the last row are left alone. ``max_length``: a promise that no sequence
     holds more rows (0: as many as its table takes), and weights and positions are at least as long; ``scratch``: ``cache_evict_scratch_words`` int32 words."""
     i32, f32 = torch.int32, torch.float32
-    k_shape, w_shape, (n, stride) = k_pool.shape, weights.shape, block_table.shape
+    k_shape, w_shape, t_shape = k_pool.shape, weights.shape, block_table.shape
+    _need(len(k_shape) == 4 and len(t_shape) == 2 and len(w_shape) == 3,
+          "cache_evict: pools are [pages, kv_heads, 64, head_dim], block_table is [n, pages], weights are [slots, kv_heads, rows]")
+    n, stride = t_shape
     if weights_out is None:
         weights_out = weights
     if positions_out is None:

@@ -86,3 +86,21 @@ def test_the_command_line_does_not_ignore_half_a_policy():
     from sleuth_b200 import cli
     with pytest.raises(ValueError):
         cli.main(["generate", "m", "--prompt-ids", "1 2", "--keep-recent", "100"])
+
+
+@pytest.mark.parametrize("name", ["q", "k_pool", "block_table", "weights"])
+@pytest.mark.parametrize("rank", [0, 1])
+def test_operators_name_arguments_of_another_rank(name, rank):
+    """Told before anything is launched or asked of a device."""
+    from sleuth_b200.kernels import ops
+    odd = torch.zeros(()) if rank == 0 else torch.zeros(8)
+    i32 = torch.zeros(1, dtype=torch.int32)
+    pool, table, w = torch.zeros((2, 2, 64, 16)), torch.zeros((1, 2), dtype=torch.int32), torch.zeros((1, 2, 128))
+    attend = {**dict(q=torch.zeros((1, 4, 16)), k_pool=pool, block_table=table, weights=w), name: odd}
+    with pytest.raises(ValueError, match="attention_kept"):
+        ops.attention_kept(v_pool=pool, out=torch.zeros((1, 64)), seq_start=i32, past=i32, counts=i32, max_count=1, heads=4, kv_heads=2, head_dim=16, window=0,
+                           first=0, scale=1.0, **attend)
+    if name != "q":
+        evict = {**dict(k_pool=pool, block_table=table, weights=w), name: odd}
+        with pytest.raises(ValueError, match="cache_evict"):
+            ops.cache_evict(positions=w.int(), v_pool=pool, past=i32, lengths=i32, seen=i32, budget=3, first=0, recent=0, **evict)
