@@ -15,8 +15,10 @@
 //     runs, so that ranks are sums of a block-wide scan; the lists of places and rows go to scratch. The block, or where the rows are many a second
 //     kernel, moves them, 16 threads a row.
 // Bound by latency: loads, a descent, moves; the bytes are the weights and positions once and the moved rows twice. Measured: a row of 2,049 goes in each
-// of 512 (sequence, kv head) pairs 7.6 us (17 MB, 2.3 TB/s; by the descent 37); 64 pairs of 2,500 to 8,192 rows come down to 1,024: the
-// descent 15 us (18 with one row a thread in flight while the keys are made), the moves, 59 MB, 14 (4.2 TB/s; the same with four rows in flight a thread).
+// of 512 (sequence, kv head) pairs 7.6 us (17 MB, 2.3 TB/s; by the descent 37), of 16,000 in each of 32 pairs 11.5, of 16,386 18.8 and of 30,001 27.6 (32 keys a thread
+// do not fit 64 registers: 504 bytes are spilled); 64 pairs of 2,500 to 8,192 rows come down to 1,024: the
+// descent 15 us (18 with one row a thread in flight while the keys are made), the moves, 59 MB, 14 (4.2 TB/s; the same with four rows in flight a thread). 16 pairs of
+// 40,000 rows to 3,000: 44 us, of 60,000: 114 (the keys do not fit shared memory and are made anew in every pass).
 #include "common.cuh"
 
 namespace slb {

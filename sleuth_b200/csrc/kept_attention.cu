@@ -13,9 +13,12 @@
 // (infinities, NaN) never reaches it.
 // The weights need the finished denominators, so their kernel forms the scores again: a block takes 64 keys of one (sequence, kv head)
 // and walks over the rows that see some of them, 64 at a time, a thread 4 x 4 scores; where such blocks are few a cluster shares the rows and its first
-// block adds the sums in the order of the ranks. Every sum has one order, and no two blocks add to the same place.
-// Bound by the FMA pipe and shared memory. Measured, float32: a prompt of 700 tokens, 16 / 8 heads of 128, 152 us, with weights 226 (one pass of 16-row
-// tiles 425); five tokens on 33 to 700 rows, 8 / 4 heads of 64, with weights 22.7 us, three launches of which each waits for the one before.
+// block adds the sums in the order of the ranks. For one cut every sum has one order, and no two blocks add to the same place; the cut goes by the step (how many
+// sequences, the longest share, the rows that the table holds, the window), so a token's bits may differ between batches.
+// Bound by the FMA pipe (39 per cent busy) and shared memory. Measured (device time): float32, a prompt of 700 tokens, 16 / 8 heads of 128, 144 us, with weights 215
+// (one pass of 16-row tiles 425); five tokens on 33 to 700 rows, 8 / 4 heads of 64, 12 us, with weights 20, three launches of which each waits for the one before.
+// bfloat16 prompts come here where the tensor-core kernels do not take them: other head sizes (2,000 tokens, 8 / 8 heads of 96, 445 us, with weights 647), and groups
+// that do not divide their tiles of 128 rows (6,000 tokens, 28 / 4 heads of 128, 8.8 ms, with weights 15.5; 40 / 8 heads 12.8 and 21.3; 32 / 8 heads there 0.32 and 0.48).
 #include <math.h>
 
 #include <algorithm>

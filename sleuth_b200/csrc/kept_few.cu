@@ -16,9 +16,9 @@
 // key and value: 1 to 4 per cent more bytes), because the denominators are known at the end only; the second kernel turns them into weights.
 // Where the units are few (few_cluster) a cluster of blocks shares one (sequence, kv head) instead: the shares meet in distributed shared memory, the
 // scores stay in shared memory, and there is neither a second kernel nor scratch.
-// Measured (device time): 64 sequences of 150 to 4,096 rows, a window of 2,048, 32 / 8 heads of 128, 79 us = 5.2 TB/s of 6.46; six of 9,000 to 30,000
-// 78 us = 5.8 TB/s, with weights 94; eight of 2,049 with weights, 16 / 8 heads, by clusters 15.6 us = 4.4 TB/s (rows that L2 holds); a token on 1,028
-// rows 7.9 us: launch, tables, one page, two meetings.
+// Measured (device time): 64 sequences of 150 to 4,096 rows, a window of 2,048, 32 / 8 heads of 128, 76 us = 5.4 TB/s of 6.46; six of 9,000 to 30,000
+// 76 us = 5.9 TB/s, with weights 90; eight of 2,049 with weights, 16 / 8 heads, by clusters 15.8 us = 4.3 TB/s (rows that L2 holds); four turns of 3 to 13
+// tokens on 1,024 to 2,048 rows, 32 / 8 heads, 23 us, with weights 29; a token on 1,028 rows 7.8 us: launch, tables, one page, two meetings.
 // Keys that no row of the 16 sees (stale rows of the last page, what lies between the first rows and the window) have their values
 // replaced by zeros in registers, so that infinities or NaN in them do not meet a zero weight.
 #include <math.h>
@@ -800,7 +800,9 @@ static int encode_pool(CUtensorMap* map, const void* base, long long rows, int h
   return r == CUDA_SUCCESS ? 0 : fail(2, "attention_kept: cuTensorMapEncodeTiled failed for %s with code %d", what, (int)r);
 }
 
-constexpr long long kMostScores = 1ll << 28;      // floats of scratch for scores: a gigabyte
+// Floats of scratch for scores: a gigabyte (64 sequences of 32 heads in a table of 131,072 rows). Single tokens and turns with weights beyond it take the
+// prompt kernels, whose tiles of 128 rows they leave mostly empty.
+constexpr long long kMostScores = 1ll << 28;
 
 bool kept_few_takes(long long tokens, int max_count, int heads, int kv_heads, int head_dim, int max_keys, int dtype, bool weights) {
   return dtype == kBF16 && (head_dim == 64 || head_dim == 128) && (long long)max_count * (heads / kv_heads) <= kFewMostRows &&

@@ -14,8 +14,9 @@
 // Clusters start in the order of their number: the first keys of all sequences and heads, whose walk is the longest, before the next ones. Where
 // blocks are too few for the SMs, a cluster shares a key tile: the steps are dealt to its blocks in turn, the first block adds the sums in the
 // order of the ranks.
-// Measured: a prompt of 6,000 tokens, 32 / 8 heads of 128, 205 to 213 us (two ways of timing it) = 0.69 to 0.72 PFLOP/s. What bounds it: the powers of two (576 M scores at 16 a cycle and SM: 139 us), then
-// the epilogue's waits between its stages. Tried: 256 queries a step with two stages of them 333 us; three powers of eight by a
+// Measured: a prompt of 6,000 tokens, 32 / 8 heads of 128, 192 us by itself (0.77 PFLOP/s at 1.84 GHz), 160 to 170 added to the attention in front of it back to
+// back. What bounds it: the powers of two (576 M scores at 16 a cycle and SM: 132 us at that clock, their unit 81 per cent busy), then
+// the epilogue's waits between its stages. Tried, at 205 us then: 256 queries a step with two stages of them 333 us; three powers of eight by a
 // polynomial on the FMA pipe 215, two of eight 201 (issue slots take what the unit gives back); 64 scores at once 211; 24 warps 201.
 #include <math.h>
 
