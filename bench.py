@@ -35,7 +35,7 @@ import time
 ROOT = os.path.dirname(os.path.abspath(__file__))
 sys.path.insert(0, ROOT)
 
-CONFIG = {  # BASELINE.json configs[2]: Qwen3-0.6B-shaped
+CONFIG = {  # Qwen3-0.6B-shaped
     "architectures": ["Qwen3ForCausalLM"], "model_type": "qwen3", "vocab_size": 151936, "hidden_size": 1024,
     "intermediate_size": 3072, "num_hidden_layers": 28, "num_attention_heads": 16, "num_key_value_heads": 8,
     "head_dim": 128, "rope_theta": 1000000.0, "rms_norm_eps": 1e-6, "attention_bias": False,
@@ -229,9 +229,9 @@ def e2e_run(engine, batch: int, steps: int, seed: int, windows=None):
 
 
 CONFIG4 = dict(CONFIG, hidden_size=2560, num_hidden_layers=36, num_attention_heads=32, num_key_value_heads=8,
-               intermediate_size=9728)                                    # BASELINE.json configs[3]: Qwen3-4B-shaped
+               intermediate_size=9728)                                    # Qwen3-4B-shaped
 CONFIG5 = dict(CONFIG, hidden_size=4096, num_hidden_layers=36, num_attention_heads=32, num_key_value_heads=8,
-               intermediate_size=12288, tie_word_embeddings=False)        # configs[4]: Qwen3-8B-shaped, untied
+               intermediate_size=12288, tie_word_embeddings=False)        # Qwen3-8B-shaped, untied
 
 
 def release(engine) -> None:
@@ -246,7 +246,7 @@ def release(engine) -> None:
 
 
 def config4_points(windows, new_tokens: int = 257) -> dict:
-    """4B-shaped, a ragged batch of 16 prompts with seeded lengths in [64, 2048], then 256
+    """4B-shaped: a ragged batch of 16 prompts with seeded lengths in [64, 2048], then 256
     decode steps each, greedy and at temperature 0.8, through ``Engine.generate`` (host tokens in and out)."""
     import numpy as np
 
@@ -274,7 +274,7 @@ def config4_points(windows, new_tokens: int = 257) -> dict:
 
 
 def config5_points(windows, steps: int, warmup: int, layers: int) -> dict:
-    """8B-shaped, untied, batch 64, 4,096-token prompts, decode steps from there on."""
+    """8B-shaped, untied: batch 64, 4,096-token prompts, decode steps from there on."""
     from sleuth_b200.engine.engine import Engine
     cfg = dict(CONFIG5, num_hidden_layers=layers)
     engine = Engine.from_config(cfg, seed=5, dtype="bf16", max_seq_len=8192, max_tokens=64 * (4096 + 128))
