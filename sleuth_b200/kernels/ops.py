@@ -1879,3 +1879,179 @@ def cache_evict(weights, positions, k_pool, v_pool, block_table, past, lengths, 
     except struct.error as e:
         raise ValueError(f"cache_evict: a number is out of range ({e})") from None
     lib().call("slb_cache_evict", call)
+
+
+# ---- drafted tokens: steps whose new rows form trees, their judgement, and the cache after it ----
+
+MOST_NODES = 256                             # of a sequence in a step (kMostNodes in csrc/tree.cuh)
+_TREE_CALL = struct.Struct("13Q3q10if4x")    # TreeCall in csrc/tree.cuh (to its whole size)
+_VERIFY_CALL = struct.Struct("13Q4qd4i")     # VerifyCall in csrc/verify_drafts.cu
+
+
+def _fits_int(what: str, *values: int) -> None:
+    _need(all(-(1 << 31) <= int(v) < 1 << 31 for v in values), f"{what}: a number is out of range")
+
+
+def draft_tree(parents, seq_start, past, counts, seen, positions, max_count: int, window: int = 0, stream=None) -> None:
+    """What each drafted node sees of its step, and its position, from the nodes' parents.
+
+    ``parents`` [tokens] int32: the node that a node continues, counted within its sequence, and before it in the step; anything else
+    (-1) makes it a first node. ``counts`` [n] nodes of each sequence, at most ``max_count`` (up to 256), its first at row ``seq_start``; ``past`` [n]: tokens
+    before the step. ``seen`` [tokens, words] int32, 32 nodes a word, receives bit b of a node where it sees node b: itself and
+    those that it continues, under a ``window`` the last ``window`` of them. ``positions`` [tokens] int32 receives ``past`` plus the number of nodes above."""
+    i32 = torch.int32
+    _cuda(parents, seq_start, past, counts, seen, positions)
+    n, T = past.numel(), parents.numel()
+    _need(all(t.dtype == i32 for t in (parents, seq_start, past, counts, seen, positions)), "draft_tree: all tensors are int32")
+    _need(seq_start.numel() >= n and counts.numel() == n, "draft_tree: seq_start, past and counts have one row a sequence")
+    _need(seen.dim() == 2 and seen.shape[0] >= T and seen.shape[1] * 32 >= max_count and positions.numel() >= T,
+          "draft_tree: seen is [tokens, words] with a bit for each of max_count nodes, positions is [tokens]")
+    _need(0 < max_count <= MOST_NODES, f"draft_tree: {max_count} nodes of a sequence; 1 to {MOST_NODES} are taken")
+    _need(window >= 0, "draft_tree: the window is not negative")
+    _fits_int("draft_tree", window)
+    lib().call("slb_draft_tree", _p(parents), _p(seq_start), _p(past), _p(counts), _p(seen), _p(positions), T, n, int(max_count), seen.shape[1], int(window),
+               stream if stream is not None else current_stream())
+
+
+def attention_tree_scratch_floats(tokens: int, n_seqs: int, max_count: int, heads: int, kv_heads: int, head_dim: int, max_keys: int,
+                                  dtype: torch.dtype) -> int:
+    """Floats of scratch that ``attention_tree`` takes for a step of ``tokens`` nodes, at most ``max_count`` a sequence, with at most
+    ``max_keys`` rows a sequence after the step."""
+    _need(dtype in DT, "attention_tree: dtypes")
+    fn = lib().dll.slb_attention_tree_scratch
+    fn.argtypes = [ctypes.c_longlong] + [ctypes.c_int] * 7
+    fn.restype = ctypes.c_longlong
+    _fits_int("attention_tree", n_seqs, max_count, heads, kv_heads, head_dim, max_keys)
+    floats = fn(int(tokens), int(n_seqs), int(max_count), int(heads), int(kv_heads), int(head_dim), int(max_keys), DT[dtype])
+    _need(floats >= 0, "attention_tree: sizes")
+    return floats
+
+
+def attention_tree(q, k_pool, v_pool, out, seq_start, past, counts, seen, positions, block_table, max_count: int, heads: int, kv_heads: int,
+                   head_dim: int, window: int, scale: float, scratch=None, max_keys: int = 0, stream=None) -> None:
+    """Attention of a step whose new rows are drafted nodes, over the paged cache that already holds their keys and values.
+
+    Sequence s brings ``counts[s]`` nodes (at most ``max_count``, up to 256), rows ``past[s]`` on of its cache. A node sees the rows before the step, with a
+    ``window`` those above ``positions`` [tokens] - window alone (without one ``positions`` may be None), and of the step's rows the
+    ones whose bit is set in its row of ``seen`` [tokens, words] int32 (``draft_tree`` makes both; any bits are taken). float32 or bfloat16, even
+    ``head_dim`` up to 256; softmax and sums in float32. ``max_keys``: a promise that no sequence has more rows after the step (0: as many as its table
+    holds). ``scratch``: ``attention_tree_scratch_floats`` floats. A node that sees nothing gives zeros. Rows that a node does not see never reach its result, whatever they hold."""
+    dt, i32 = q.dtype, torch.int32
+    q_shape, k_shape, t_shape = q.shape, k_pool.shape, block_table.shape
+    _need(len(q_shape) == 3 and len(k_shape) == 4 and len(t_shape) == 2 and seen.dim() == 2,
+          "attention_tree: q is [tokens, heads, head_dim], pools are [pages, kv_heads, 64, head_dim], block_table is [n, pages], seen is [tokens, words]")
+    (n, stride), T = t_shape, q_shape[0]
+    if not (q.is_cuda and q.is_contiguous() and k_pool.is_cuda and k_pool.is_contiguous() and v_pool.is_cuda and v_pool.is_contiguous()
+            and out.is_cuda and out.is_contiguous() and seq_start.is_cuda and seq_start.is_contiguous() and past.is_cuda and past.is_contiguous()
+            and counts.is_cuda and counts.is_contiguous() and seen.is_cuda and seen.is_contiguous() and block_table.is_cuda and block_table.is_contiguous()
+            and _plain_cuda(positions) and _plain_cuda(scratch)
+            and q_shape == (T, heads, head_dim) and out.shape == (T, heads * head_dim) and dt in DT
+            and dt == out.dtype == k_pool.dtype == v_pool.dtype and k_shape == (k_shape[0], kv_heads, 64, head_dim) and k_shape == v_pool.shape
+            and i32 == block_table.dtype == seq_start.dtype == past.dtype == counts.dtype == seen.dtype
+            and seq_start.numel() >= n and past.numel() >= n and counts.numel() >= n
+            and seen.shape[0] >= T and seen.shape[1] * 32 >= max_count > 0 and max_count <= MOST_NODES
+            and window >= 0 and scale > 0 and (scratch is None or scratch.dtype == torch.float32)
+            and (positions is None and window == 0 or positions is not None and positions.dtype == i32 and positions.numel() >= T)):
+        _kept_refusal("attention_tree", dict(q=q, k_pool=k_pool, v_pool=v_pool, out=out, seq_start=seq_start, past=past, counts=counts, seen=seen,
+                                             positions=positions, block_table=block_table, scratch=scratch), (
+            (lambda: q_shape == (T, heads, head_dim) and out.shape == (T, heads * head_dim), "q is [tokens, heads, head_dim], out [tokens, heads * head_dim]"),
+            (lambda: dt in DT and dt == out.dtype == k_pool.dtype == v_pool.dtype, "q, out and the pools are float32 or bfloat16 alike"),
+            (lambda: k_shape == (k_shape[0], kv_heads, 64, head_dim) and k_shape == v_pool.shape, "pools are [pages, kv_heads, 64, head_dim]"),
+            (lambda: i32 == block_table.dtype == seq_start.dtype == past.dtype == counts.dtype and min(x.numel() for x in (seq_start, past, counts)) >= n,
+             "block_table, seq_start, past and counts are int32, one row a sequence"),
+            (lambda: 0 < max_count <= MOST_NODES, f"{max_count} nodes of a sequence; 1 to {MOST_NODES} are taken"),
+            (lambda: seen.dtype == i32 and seen.shape[0] >= T and seen.shape[1] * 32 >= max_count, "seen is int32 [tokens, words] with a bit for each of max_count nodes"),
+            (lambda: window >= 0 and scale > 0, "the window is not negative, the scale is positive"),
+            (lambda: scratch is None or scratch.dtype == torch.float32, "scratch is float32"),
+            (lambda: positions is not None or window == 0, "a window needs the nodes' positions"),
+            (lambda: positions is None or positions.dtype == i32 and positions.numel() >= T, "positions are int32, one a token")))
+    status = _TC_STATUS.get(q.device)
+    if status is None:
+        status = _tc_status(q.device)
+    try:
+        call = _TREE_CALL.pack(q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), seq_start.data_ptr(), past.data_ptr(), counts.data_ptr(),
+                               seen.data_ptr(), 0 if positions is None else positions.data_ptr(), block_table.data_ptr(),
+                               0 if scratch is None else scratch.data_ptr(), status.data_ptr(), stream if stream is not None else current_stream(),
+                               T, 0 if scratch is None else scratch.numel(), k_shape[0], stride, n, max_count, max_keys, heads, kv_heads, head_dim,
+                               window, seen.shape[1], DT[dt], scale)
+    except struct.error as e:
+        raise ValueError(f"attention_tree: a number is out of range ({e})") from None
+    lib().call("slb_attention_tree", call)
+
+
+def verify_drafts_scratch_words(n_seqs: int, tokens: int, limit: int, drawn: bool) -> int:
+    """int32 words of scratch that ``verify_drafts`` takes; ``drawn``: with ``probs``."""
+    fn = lib().dll.slb_verify_drafts_scratch
+    fn.argtypes, fn.restype = [ctypes.c_int, ctypes.c_longlong, ctypes.c_int, ctypes.c_int], ctypes.c_longlong
+    _fits_int("verify_drafts", n_seqs, limit)
+    return fn(int(n_seqs), int(tokens), int(limit), 1 if drawn else 0)
+
+
+def verify_drafts(logits, limit: int, tokens, parents, seq_start, counts, uniforms, temperature: float, path, lengths, chosen, max_count: int,
+                  probs=None, floors=None, scratch=None, stream=None) -> None:
+    """Which drafted nodes the target accepts, and the token behind the last of them.
+
+    ``logits`` [tokens, vocab] float32: row t is what the target says behind node t, of which the first ``limit`` tokens count. Sequence s brings ``counts[s]``
+    nodes (at most ``max_count``, up to 256) from row ``seq_start[s]`` on; node 0 is its newest certain token, ``tokens`` / ``parents`` [tokens] int32 the drafted token
+    of each other node and the node that it continues, which lies before it (a node with another parent is never reached). p is softmax(logits / ``temperature``)
+    over the tokens whose logit is not below the row's ``floors`` [tokens] float32, if given. At an accepted node its children are
+    tried in their order with ``uniforms`` [tokens] float32 in [0, 1), one a node: child x is accepted with probability min(1, p(x) / q(x)), q being row
+    t of ``probs`` [tokens, vocab] float32, from which the children of node t were drawn one by one; after a refusal p becomes max(p - q, 0) over its sum. Without
+    ``probs`` drafts are certain: q(x) = 1, and p loses the refused token. Where no child is left, the next token is drawn from p with node 0's number, the first in the order of token numbers
+    where the running sum passes it. Temperature 0 (or below): the child that is the first largest logit, and in the end that token; ``uniforms`` may be None.
+
+    Outputs, int32: ``path`` [n, places] the accepted nodes from node 0 on, then -1; ``lengths`` [n] their number (at least 1; 0 for a sequence without nodes); ``chosen``
+    [n] the next token (-1 without nodes; 0 where the row has no number above -inf). ``scratch``: ``verify_drafts_scratch_words`` int32 words. Rows may be apart (a stride)."""
+    i32, f32 = torch.int32, torch.float32
+    _cuda(tokens, parents, seq_start, counts, uniforms, path, lengths, chosen, floors, scratch)
+    for name, t in (("logits", logits), ("probs", probs)):
+        _need(t is None or t.is_cuda and t.dtype == f32 and t.dim() == 2 and t.stride(1) == 1, f"verify_drafts: {name} are float32 CUDA rows of unit column stride")
+    n, T = counts.numel(), logits.shape[0]
+    _need(0 < limit <= logits.shape[1] and (probs is None or probs.shape[0] >= T and probs.shape[1] >= limit), "verify_drafts: limit tokens of a row of logits and of probs")
+    _need(all(t.dtype == i32 for t in (tokens, parents, seq_start, counts, path, lengths, chosen)), "verify_drafts: tables and outputs are int32")
+    _need(tokens.numel() >= T and parents.numel() >= T, "verify_drafts: tokens and parents have a value for each row of logits")
+    _need(seq_start.numel() >= n and lengths.numel() >= n and chosen.numel() >= n and path.dim() == 2 and path.shape[0] >= n and path.shape[1] >= max_count,
+          "verify_drafts: path is [n, places] for max_count nodes; seq_start, lengths and chosen have one value a sequence")
+    _need(0 < max_count <= MOST_NODES, f"verify_drafts: {max_count} nodes of a sequence; 1 to {MOST_NODES} are taken")
+    temperature = float(temperature)
+    _need(temperature == temperature and temperature < float("inf"), "verify_drafts: the temperature must be a finite number")
+    _need(uniforms is None and temperature <= 0 or uniforms is not None and uniforms.dtype == f32 and uniforms.numel() >= T,
+          "verify_drafts: uniforms are float32, one a node, and needed above temperature 0")
+    _need(floors is None or floors.dtype == f32 and floors.numel() >= T, "verify_drafts: floors are float32, one a node")
+    _need(scratch is None or scratch.dtype == i32, "verify_drafts: scratch is int32")
+    try:
+        call = _VERIFY_CALL.pack(logits.data_ptr(), 0 if probs is None else probs.data_ptr(), 0 if floors is None else floors.data_ptr(),
+                                 0 if uniforms is None else uniforms.data_ptr(), tokens.data_ptr(), parents.data_ptr(), seq_start.data_ptr(), counts.data_ptr(),
+                                 path.data_ptr(), lengths.data_ptr(), chosen.data_ptr(), 0 if scratch is None else scratch.data_ptr(),
+                                 stream if stream is not None else current_stream(), T, logits.stride(0) if T > 1 else logits.shape[1],
+                                 0 if probs is None else probs.stride(0) if probs.shape[0] > 1 else probs.shape[1], 0 if scratch is None else scratch.numel(),
+                                 temperature, n, limit, max_count, path.shape[1])
+    except struct.error as e:
+        raise ValueError(f"verify_drafts: a number is out of range ({e})") from None
+    lib().call("slb_verify_drafts", call)
+
+
+def cache_compact(k_pool, block_table, past, path, lengths, v_pool=None, stream=None) -> None:
+    """The rows of the nodes that stay move together behind the rows from before the step, in every layer.
+
+    For each sequence, i = 0 .. ``lengths`` - 1: the row ``past`` + ``path[i]`` becomes row ``past`` + i. ``path`` [n, places] int32 (at most 256 places) rises, from 0 or
+    above (``verify_drafts`` gives such); it ends in front of the first entry that does not. ``k_pool`` [..., pages, kv_heads, 64, width]: any number of layers,
+    or keys and values, in front, all with one block table; ``v_pool``: more layers, perhaps of another width. A sequence then holds ``past`` + ``lengths`` rows; what lies behind them is left as it was."""
+    i32 = torch.int32
+    _cuda(k_pool, v_pool, block_table, past, path, lengths)
+    shape = k_pool.shape
+    _need(k_pool.dim() >= 4 and shape[-2] == 64 and k_pool.dtype in DT, "cache_compact: pools are [..., pages, kv_heads, 64, width], float32 or bfloat16")
+    _need(v_pool is None or v_pool.dim() >= 4 and v_pool.dtype == k_pool.dtype and v_pool.shape[-4:-1] == shape[-4:-1], "cache_compact: v_pool has the pages and heads of k_pool")
+    _need(block_table.dim() == 2 and path.dim() == 2, "cache_compact: block_table is [n, pages], path is [n, places]")
+    n = block_table.shape[0]
+    _need(all(t.dtype == i32 for t in (block_table, past, path, lengths)) and past.numel() >= n and lengths.numel() >= n and path.shape[0] >= n,
+          "cache_compact: block_table, past, path and lengths are int32, one row a sequence")
+    _need(path.shape[1] <= MOST_NODES, f"cache_compact: paths of {path.shape[1]} nodes; at most {MOST_NODES} are taken")
+    size, rows = k_pool.element_size(), shape[-4] * shape[-3] * 64
+    k_row, v_row = shape[-1] * size, 0 if v_pool is None else v_pool.shape[-1] * size
+    _need(k_row > 0 and k_row % 4 == 0 and v_row % 4 == 0, "cache_compact: a row's bytes are a multiple of four")
+    if rows == 0 or path.shape[1] == 0 or n == 0:
+        return
+    lib().call("slb_cache_compact", _p(k_pool), _p(v_pool), _p(block_table), _p(past), _p(path), _p(lengths), k_pool.numel() // (rows * shape[-1]),
+               0 if v_row == 0 else v_pool.numel() // (rows * v_pool.shape[-1]), shape[-4], block_table.shape[1], n, shape[-3], k_row, v_row, path.shape[1],
+               stream if stream is not None else current_stream())
