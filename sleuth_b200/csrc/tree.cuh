@@ -1,7 +1,7 @@
 // What the kernels of drafted tokens share: the arguments of a step whose new rows form trees, and what its queries see.
 //
 // Rows of a sequence are counted from 0 in the order of its block table (64 rows a page). A step appends counts[s] rows, the nodes of
-// a tree, behind the past[s] rows that are there. The query of a node sees the row j < past[s] if window == 0 or j > positions[node] - window,
+// a tree, behind the past[s] rows that are there. The query of a node sees the row j < past[s] if window == 0 or j > max(positions[node], past[s]) - window,
 // and the row past[s] + b of the step if bit b of its words of `seen` is set; a bit at counts[s] or behind says nothing.
 #pragma once
 
@@ -58,7 +58,7 @@ struct TreeSeq {
 // First row of those before the step that a node sees.
 __device__ __forceinline__ int tree_lo(const TreeArgs& a, int token, int past) {
   if (a.window <= 0) return 0;
-  const long long lo = (long long)a.positions[token] - a.window + 1;
+  const long long lo = (long long)max(a.positions[token], past) - a.window + 1;
   return lo <= 0 ? 0 : lo >= past ? past : (int)lo;
 }
 
@@ -73,5 +73,10 @@ __device__ __forceinline__ unsigned long long tree_bits(const uint32_t* words, i
   if (left < 64) v &= (1ull << left) - 1ull;
   return v;
 }
+
+// On the tensor cores (tree_attention_tc.cu): which calls it takes, the floats of scratch (the first ones 16-byte aligned), the launch.
+bool tree_tc_takes(int n_seqs, int max_count, int heads, int kv_heads, int head_dim, int max_keys, int dtype);
+long long tree_tc_floats(int n_seqs, int max_count, int heads, int kv_heads, int head_dim, int max_keys);
+int tree_tc(const TreeArgs& a, long long pool_pages, int* status, cudaStream_t s);
 
 }  // namespace slb

@@ -251,6 +251,7 @@ static int launch_tree_general(TreeArgs a, cudaStream_t s) {
 extern "C" long long slb_attention_tree_scratch(long long tokens, int n_seqs, int max_count, int heads, int kv_heads, int head_dim, int max_keys, int dtype) {
   if (tokens < 0 || n_seqs < 0 || max_count <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || head_dim <= 0 || max_keys <= 0) return -1;
   if (tokens == 0 || n_seqs == 0) return 0;
+  if (tree_tc_takes(n_seqs, max_count, heads, kv_heads, head_dim, max_keys, dtype)) return tree_tc_floats(n_seqs, max_count, heads, kv_heads, head_dim, max_keys);
   return general_tree_floats(tokens, n_seqs, max_count, heads, kv_heads, head_dim, max_keys);
 }
 
@@ -277,6 +278,7 @@ extern "C" int slb_attention_tree(const TreeCall* call) {
   const long long need = slb_attention_tree_scratch(c.tokens, c.n_seqs, c.max_count, c.heads, c.kv_heads, c.head_dim, a.max_keys, c.dtype);
   SLB_REQUIRE(need == 0 || (c.scratch != nullptr && c.scratch_floats >= need), "attention_tree: the step needs %lld floats of scratch, %lld were given", need,
               c.scratch ? c.scratch_floats : 0ll);
+  if (tree_tc_takes(c.n_seqs, c.max_count, c.heads, c.kv_heads, c.head_dim, a.max_keys, c.dtype)) return tree_tc(a, c.pool_pages, c.status, (cudaStream_t)c.stream);
   return c.dtype == kF32 ? launch_tree_general<float>(a, (cudaStream_t)c.stream) : launch_tree_general<__nv_bfloat16>(a, (cudaStream_t)c.stream);
 }
 

@@ -1932,7 +1932,7 @@ def attention_tree(q, k_pool, v_pool, out, seq_start, past, counts, seen, positi
     """Attention of a step whose new rows are drafted nodes, over the paged cache that already holds their keys and values.
 
     Sequence s brings ``counts[s]`` nodes (at most ``max_count``, up to 256), rows ``past[s]`` on of its cache. A node sees the rows before the step, with a
-    ``window`` those above ``positions`` [tokens] - window alone (without one ``positions`` may be None), and of the step's rows the
+    ``window`` those above ``positions`` [tokens] - window alone (without one ``positions`` may be None; a position below ``past`` counts as ``past``), and of the step's rows the
     ones whose bit is set in its row of ``seen`` [tokens, words] int32 (``draft_tree`` makes both; any bits are taken). float32 or bfloat16, even
     ``head_dim`` up to 256; softmax and sums in float32. ``max_keys``: a promise that no sequence has more rows after the step (0: as many as its table
     holds). ``scratch``: ``attention_tree_scratch_floats`` floats. A node that sees nothing gives zeros. Rows that a node does not see never reach its result, whatever they hold."""
