@@ -1,14 +1,17 @@
 // Attention of drafted nodes (tree.cuh) on the tcgen05 tensor cores: bfloat16, heads of 64 and 128, any number of query heads a key/value head.
 //
 // What such a step costs is the read of the keys and values (up to 256 rows of queries meet each: 512 FLOP a byte at most), so the work is the pages: every sequence has
-// (kv head, tile of 128 rows, page) units, and each block takes an equal run of the list of all units, whatever the sequences' lengths. A (sequence, kv head, tile) that
-// lies in one run is finished by its block; the others' shares wait in scratch for a second kernel that joins them in their order.
-//   warp 0      asks TMA for the run's pages of keys, into a ring, and issues S = Q K^T, 128 x 64, one page ahead of the softmax (two score buffers in tensor memory);
-//   warp 1      the same for the values, and O += P V as soon as P is written, P read from tensor memory where S was;
-//   warps 2..9  the softmax, two threads a row (32 keys of a page each) that agree on the row's running maximum; P is rounded to bfloat16 (the instruction takes no wider
-//                one beside bfloat16 values), the sum is of the unrounded weights, in 32 bits.
-// Rows are row r = node r / G, query head r % G of the group. Fewer than 128 rows leave the tile's other rows to whatever lies behind the queries in shared memory: a row of
-// A reaches that row of the result alone, and nobody reads it. Two blocks an SM, so that one loads and multiplies while the other stands in its chain of load, maximum, powers and store.
+// (kv head, tile of 256 rows, page) units, and each block, one an SM, takes an equal run of the list of all units, whatever the sequences' lengths. What a run holds of one (sequence, kv head,
+// tile) is a segment. A (sequence, kv head, tile) that is one segment is finished by its block; the others' shares wait in scratch for a second kernel that joins them in their order.
+//   warp 0       asks TMA for the pages of the run, keys and values, each into a ring of its own (128 KB on the way at most: 43 KB an SM hide a microsecond of latency, and it is more under load);
+//   warp 1       S = Q K^T, 128 x 64, ahead of the softmax; two score buffers a group in tensor memory;
+//   warp 2       O += P V as soon as P is written, P read from tensor memory where S was;
+//   warp 3       walks the segments ahead of the others, leaves their descriptions and brings their queries, into the other of two buffers where they fit;
+//   warps 4..19  the softmax: two groups of 256 threads, two threads a row (32 keys of a page each), that take the pages in turn where the tile has up to 128 rows (each with a maximum, a sum
+//                and an accumulator of its own, joined at the segment's end), or every page for 128 rows each where it has more. P is rounded to bfloat16 (the instruction takes no wider one
+//                beside bfloat16 values), the sum is of the unrounded weights, in 32 bits.
+// Rows are row r = node r / G, query head r % G of the group. Fewer than 128 rows leave the instruction's other rows to whatever lies behind the queries in shared memory: a row of
+// A reaches that row of the result alone, and nobody reads it.
 // Rows that a node does not see are masked by a bit each. Their values meet a zero weight in the product, which an infinity or a NaN among them would survive: so in pages that
 // not all rows see alike (the step's own and those at a window's edge) values that are not finite are taken out in shared memory, and nodes that do see them get them back at the end, a bit pair for each (row, channel).
 #include <math.h>
@@ -20,7 +23,7 @@
 
 namespace slb {
 
-constexpr int kTtRows = 128, kTtThreads = 10 * 32, kTtSoft = 256;
+constexpr int kTtRows = 128, kTtTile = 256, kTtThreads = 20 * 32;
 constexpr float kTtRescale = 8.0f;      // log2 units by which a maximum may be stale
 
 __device__ __forceinline__ float tt_ex2(float x) {
@@ -33,22 +36,25 @@ __device__ __forceinline__ float tt_max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
   return y;
 }
+__device__ __forceinline__ void tt_copy16(uint32_t dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src)); }
 
 struct TtLayout {
-  int rows, stages, k_off, v_off, poison_off, xch_off, sum_off, bar_off, total;
+  int rows, queries, stages, q_bytes, k_off, v_off, poison_off, ml_off, xch_off, bar_off, total;      // queries: buffers for them
 };
 static TtLayout tt_layout(int HD, int rows) {
   TtLayout l;
-  l.rows = std::min(kTtRows, (rows + 31) & ~31);
-  const int page = 64 * HD * 2, q = l.rows * HD * 2, rest = l.rows * HD / 4 + 2 * 2 * kTtRows * 2 + 2 * kTtRows * 4 + 32 * 8;
-  l.stages = std::min(4, (112 * 1024 - q - rest) / (2 * page));      // (113 KB a block, 1 KB of it static)
-  l.k_off = q;
+  l.rows = std::min(kTtTile, (rows + 31) & ~31);
+  l.queries = l.rows <= kTtRows ? 2 : 1;
+  l.q_bytes = l.rows * HD * 2;
+  const int page = 64 * HD * 2, rest = 2 * kTtRows * HD / 4 + 2 * 2 * kTtRows * 16 + 2 * 2 * 2 * kTtRows * 2 + 64 * 8;
+  l.stages = std::min(8, (225 * 1024 - l.queries * l.q_bytes - rest) / (2 * page));      // (227 KB a block, 2 KB of it static)
+  l.k_off = l.queries * l.q_bytes;
   l.v_off = l.k_off + l.stages * page;
   l.poison_off = l.v_off + l.stages * page;
-  l.xch_off = l.poison_off + l.rows * HD / 4;
-  l.sum_off = l.xch_off + 2 * 2 * kTtRows * 2;
-  l.bar_off = l.sum_off + 2 * kTtRows * 4;
-  l.total = l.bar_off + 32 * 8;
+  l.ml_off = l.poison_off + 2 * kTtRows * HD / 4;
+  l.xch_off = l.ml_off + 2 * 2 * kTtRows * 16;
+  l.bar_off = l.xch_off + 2 * 2 * 2 * kTtRows * 2;
+  l.total = l.bar_off + 64 * 8;
   return l;
 }
 
@@ -60,84 +66,79 @@ struct TtArgs {
   int2* info;           // [n, kv_heads, tiles] first block and number of blocks
   int* status;
   int tiles;            // most tiles of a sequence
+  int q_by_tma;         // queries come by TMA: a group divides 32
   TtLayout lay;
 };
 
-// The pages of a sequence that some node may see: those from the window of a node at `past` on.
+// The pages of a sequence that some node may see: those from the window of a node at `past` on. A (sequence, kv head, tile) counts kTtEntry units more than it has
+// pages: what a segment's beginning and end cost (runs of equal pages left blocks with many short segments behind: 64 sequences of 150 to 4,096 rows, of 148 blocks the median 99 us, the last 136).
+constexpr int kTtEntry = 3;
 struct TtSeq {
-  int page_lo, pages, tiles, rows, units;
-  __device__ __forceinline__ TtSeq(const TreeArgs& a, const TreeSeq& s) {
-    const int G = a.heads / a.kv_heads;
-    const long long lo = a.window > 0 ? (long long)s.past - a.window + 1 : 0;
+  int past, count, tok0, page_lo, pages, tiles, units;
+  __device__ __forceinline__ void read(const TreeArgs& a, int seq) {
+    const TreeSeq s(a, seq);
+    past = s.past; count = s.count; tok0 = s.tok0;
+    const long long lo = a.window > 0 ? (long long)past - a.window + 1 : 0;
     page_lo = lo > 0 ? (int)(lo / 64) : 0;
-    pages = s.count > 0 ? (s.past + s.count - 1) / 64 - page_lo + 1 : 0;
-    rows = s.count * G;
-    tiles = (rows + kTtRows - 1) / kTtRows;
-    units = pages * tiles * a.kv_heads;      // (the launcher has seen that all units of a call stay below 2^31)
+    pages = count > 0 ? (past + count - 1) / 64 - page_lo + 1 : 0;
+    tiles = (count * (a.heads / a.kv_heads) + kTtTile - 1) / kTtTile;
+    units = (pages + kTtEntry) * tiles * a.kv_heads;      // (the launcher has seen that all units of a call stay below 2^31)
   }
 };
 
-// A block's run of units, segment by segment: a segment is what the run holds of one (sequence, kv head, tile).
+// How units go to blocks: the first `more` blocks take each + 1 of them, the others each.
+struct TtShare {
+  int each, more;
+  __device__ __forceinline__ TtShare(int total, int blocks) { each = total / blocks; more = total - each * blocks; }
+  __device__ __forceinline__ int begin(int block) const { return block * each + min(block, more); }
+  __device__ __forceinline__ int block_of(int unit) const {
+    const int at = more * (each + 1);
+    return unit < at ? unit / (each + 1) : more + (unit - at) / each;
+  }
+};
+
+// A block's run of units, segment by segment.
 struct TtWalk {
   int u, u_hi, seq, seq_first;      // the next unit, the run's end; the sequence and its first unit
-  int kh, tile, off, n;             // the segment: its first page within the sequence, its pages
-  int past, count, tok0, page_lo, pages, rows;
+  TtSeq s;
+  int kh, tile, off, n, rows;       // the segment: its first page within the sequence, its pages, its rows
+  int first;                        // the unit of its (sequence, kv head, tile)'s first page
   __device__ __forceinline__ bool next(const TreeArgs& a) {
-    if (u >= u_hi) return false;
-    while (true) {
-      const TreeSeq s(a, seq);
-      const TtSeq t(a, s);
-      if (u < seq_first + t.units) {
-        const int rel = u - seq_first, at = rel / t.pages;
-        off = rel - at * t.pages;
-        kh = at / t.tiles;
-        tile = at - kh * t.tiles;
-        n = min(t.pages - off, u_hi - u);
-        past = s.past; count = s.count; tok0 = s.tok0;
-        page_lo = t.page_lo; pages = t.pages; rows = t.rows;
-        u += n;
-        return true;
+    n = 0;
+    while (u < u_hi) {
+      const int rel = u - seq_first;
+      if (rel >= s.units) {
+        seq_first += s.units;
+        s.read(a, ++seq);
+        continue;
       }
-      seq_first += t.units;
-      ++seq;
+      const int long_pages = s.pages + kTtEntry, at = rel / long_pages, place = rel - at * long_pages;
+      kh = at / s.tiles;
+      tile = at - kh * s.tiles;
+      first = u - place + kTtEntry;
+      const int end = min(first + s.pages, u_hi), begin = max(u, first);
+      u = end;
+      if (end <= begin) continue;      // the run ends before the first page
+      off = begin - first;
+      n = end - begin;
+      rows = min(kTtTile, s.count * (a.heads / a.kv_heads) - tile * kTtTile);
+      return true;
     }
-  }
-};
-
-// The same run page by page, for loads that go ahead of the products: rows of a tensor map's pool.
-struct TtPages {
-  TtWalk w;
-  int i, ahead;      // pages taken of the segment; the number of the next page, read one page early
-  const int* table;
-  __device__ __forceinline__ void segment(const TreeArgs& a) {
-    i = 0;
-    if (w.next(a)) {
-      table = a.block_table + (size_t)w.seq * a.table_stride + w.page_lo + w.off;
-      ahead = table[0];
-    } else {
-      w.n = 0;
-    }
-  }
-  __device__ __forceinline__ TtPages(const TtWalk& from, const TreeArgs& a) : w(from) { segment(a); }
-  __device__ __forceinline__ bool next(const TreeArgs& a, int& row) {
-    if (w.n == 0) return false;
-    row = (ahead * a.kv_heads + w.kh) * 64;
-    if (++i == w.n) segment(a);
-    else ahead = table[i];
-    return true;
+    return false;
   }
 };
 
 template <int HD>
-__global__ void __launch_bounds__(kTtThreads, 2)
-tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TtArgs ta) {
-  constexpr int PAGE = 64 * HD * 2;
+__global__ void __launch_bounds__(kTtThreads, 1)
+tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TtArgs ta) {
+  constexpr int PAGE = 64 * HD * 2, WORDS = HD / 16;      // words of a row's poison
   const TreeArgs& a = ta.t;
   const TtLayout& L = ta.lay;
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ int warp_units[kTtThreads / 32];
-  __shared__ int s_first, s_seq, s_lo, s_poison;
-  __shared__ uint32_t s_odd[2], tmem_slot;
+  __shared__ int s_lo[2];
+  __shared__ uint32_t s_odd[3][2][2], tmem_slot;      // rows of a page with values that are not finite: of either group's page, of a page of both; two places used in turn
+  __shared__ TtWalk desc[2], s_run;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t base = smem_addr(smem);
   if ((base & 1023u) != 0) {
@@ -145,37 +146,33 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
     return;
   }
   const uint32_t sK = base + L.k_off, sV = base + L.v_off, bars = base + L.bar_off;
-  const uint32_t k_full = bars, k_free = bars + 32, v_full = bars + 64, v_free = bars + 96, s_full = bars + 128, p_full = bars + 144, pv_done = bars + 160,
-                 q_full = bars + 176, o_free = bars + 184;
-  if (tid == 0) {
-    for (int i = 0; i < L.stages; ++i) {
-      mbar_init(k_full + 8 * i, 1);
-      mbar_init(k_free + 8 * i, 1);
-      mbar_init(v_full + 8 * i, 1);
-      mbar_init(v_free + 8 * i, 1);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(s_full + 8 * i, 1);
-      mbar_init(p_full + 8 * i, 8);
-      mbar_init(pv_done + 8 * i, 1);
-    }
-    mbar_init(q_full, 8);
-    mbar_init(o_free, 8);
+  const uint32_t k_full = bars, k_free = bars + 64, v_full = bars + 128, v_free = bars + 192, s_full = bars + 256, p_full = bars + 288, pv_done = bars + 320,
+                 q_full = bars + 352, q_free = bars + 368, o_free = bars + 384;      // (s_full, p_full, pv_done: [group][buffer])
+  if (warp == 0) {
+    // one arrival each, but for p_full (eight softmax warps), q_free (all sixteen, the scores' and the values' thread) and o_free (sixteen)
+    for (int i = lane; i < 49; i += 32) mbar_init(bars + 8 * i, i >= 36 && i < 40 ? 8 : i == 46 || i == 47 ? 18 : i == 48 ? 16 : 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    s_lo = s_poison = 0;
-    s_odd[0] = s_odd[1] = 0u;
+    if (lane < 12) (&s_odd[0][0][0])[lane] = 0u;
+    if (lane < 2) s_lo[lane] = 0;
+  }
+  if (warp == 2) {
+    __syncwarp();
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   pdl_wait();
 
   // where this block's run of units begins
   const int G = a.heads / a.kv_heads;
-  TtWalk run;
-  int total = 0, blocks;
+  int total = 0;
   {
     const int per = (a.n_seqs + kTtThreads - 1) / kTtThreads, q0 = min(a.n_seqs, tid * per), q1 = min(a.n_seqs, q0 + per);
-    auto units_of = [&](int s) { return TtSeq(a, TreeSeq(a, s)).units; };
+    TtSeq one;
     int own = 0;
-    for (int s = q0; s < q1; ++s) own += units_of(s);
+    for (int s = q0; s < q1; ++s) {
+      one.read(a, s);
+      own += one.units;
+    }
     int incl = own;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -190,132 +187,194 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
       if (w < warp) before += warp_units[w];
       total += warp_units[w];
     }
-    blocks = min((int)gridDim.x, total);
-    if ((int)blockIdx.x >= blocks) return;
-    run.u = (int)((long long)blockIdx.x * total / blocks);
-    run.u_hi = (int)((long long)(blockIdx.x + 1) * total / blocks);
-    before += incl - own;
-    if (own > 0 && run.u >= before && run.u < before + own) {
-      for (int s = q0; s < q1; ++s) {
-        const int units = units_of(s);
-        if (run.u < before + units) {
-          s_seq = s;
-          s_first = before;
-          break;
+    const int blocks = min((int)gridDim.x, total);
+    if ((int)blockIdx.x < blocks) {
+      const TtShare share(total, blocks);
+      const int u = share.begin(blockIdx.x);
+      before += incl - own;
+      if (own > 0 && u >= before && u < before + own) {
+        int s = q0;
+        if (per > 1) one.read(a, s);
+        while (u >= before + one.units) {
+          before += one.units;
+          one.read(a, ++s);
         }
-        before += units;
+        s_run.u = u;
+        s_run.u_hi = share.begin(blockIdx.x + 1);
+        s_run.seq = s;
+        s_run.seq_first = before;
+        s_run.s = one;
       }
+    } else if (tid == 0) {
+      s_run.u = s_run.u_hi = 0;
     }
-  }
-  if (warp == 1) {
-    __syncwarp();
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"(256) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   pdl_launch_dependents();      // (only now: a successor that also wants tensor memory must not take it before this block has its own)
-  const uint32_t tmem = tmem_slot, tO = tmem + 128;
-  run.seq = s_seq;
-  run.seq_first = s_first;
+  const uint32_t tmem = tmem_slot;
 
   if (warp == 0) {
-    if (elect_one()) {
-      // ---- scores ----
-      constexpr uint32_t idesc = instr_desc(kTtRows, 64);
-      TtPages pages(run, a);
-      int st = 0, lap = 0, jj = 0, seg = 0, lst = 0, loaded = 0;      // lst: the stage of the next load
-      auto load = [&]() {      // (a stage is free once S of the page that lay there is complete; the caller has seen to it)
-        int row;
-        if (!pages.next(a, row)) return;
-        mbar_expect_tx(k_full + 8 * lst, PAGE);
+    // ---- pages ----
+    TtWalk run = s_run;
+    int st = 0, lap = 0;
+    bool ok = true;
+    while (ok && run.next(a)) {
+      const int* table = a.block_table + (size_t)run.seq * a.table_stride + run.s.page_lo + run.off;
+      for (int i0 = 0; i0 < run.n && ok; i0 += 32) {
+        const int mine = i0 + lane < run.n ? table[i0 + lane] : 0;
+        for (int i = 0; i < min(32, run.n - i0) && ok; ++i) {
+          const int row = (__shfl_sync(0xffffffffu, mine, i) * a.kv_heads + run.kh) * 64;
+          if (lap > 0 && !mbar_wait(k_free + 8 * st, (lap - 1) & 1)) { ok = false; break; }
+          if (elect_one()) {
+            mbar_expect_tx(k_full + 8 * st, PAGE);
 #pragma unroll
-        for (int h = 0; h < HD / 64; ++h) tma_load_2d(sK + lst * PAGE + h * 8192, &map_k, h * 64, row, k_full + 8 * lst);
-        if (++lst == L.stages) lst = 0;
-        ++loaded;
-      };
-      for (int i = 0; i + 1 < L.stages; ++i) load();
-      bool ok = true;
-      while (ok && run.next(a)) {
-        if (!mbar_wait(q_full, seg & 1)) { atomicExch(ta.status, 93); break; }
-        ++seg;
-        for (int i = 0; i < run.n; ++i, ++jj) {
-          const int b = jj & 1, before = st ? st - 1 : L.stages - 1;
-          if (jj >= 1 && !mbar_wait(k_free + 8 * before, (st ? lap : lap - 1) & 1)) { atomicExch(ta.status, 92); ok = false; break; }
-          load();      // into the stage of page jj - 1
-          if (!mbar_wait(k_full + 8 * st, lap & 1)) { atomicExch(ta.status, 94); ok = false; break; }
-          // S lands where S and then P of two pages ago lay: the product that read that P must be through
-          if (jj >= 2 && !mbar_wait(pv_done + 8 * b, ((jj >> 1) - 1) & 1)) { atomicExch(ta.status, 95); ok = false; break; }
-          tc_fence_after();
-#pragma unroll
-          for (int h = 0; h < HD / 64; ++h) {
-            const uint64_t dq = smem_desc(base + h * L.rows * 128), dk = smem_desc(sK + st * PAGE + h * 8192);
-#pragma unroll
-            for (int k4 = 0; k4 < 4; ++k4)
-              mma_bf16_ss(tmem + (uint32_t)(b * 64), dq + (uint64_t)(k4 * 2), dk + (uint64_t)(k4 * 2), idesc, (h > 0 || k4 > 0) ? 1u : 0u);
+            for (int h = 0; h < HD / 64; ++h) tma_load_2d(sK + st * PAGE + h * 8192, &map_k, h * 64, row, k_full + 8 * st);
           }
-          mma_commit(s_full + 8 * b);
-          mma_commit(k_free + 8 * st);
+          __syncwarp();
+          if (lap > 0 && !mbar_wait(v_free + 8 * st, (lap - 1) & 1)) {
+            mbar_wait(k_full + 8 * st, lap & 1);      // (the copy under way lands before the block goes)
+            ok = false;
+            break;
+          }
+          if (elect_one()) {
+            mbar_expect_tx(v_full + 8 * st, PAGE);
+#pragma unroll
+            for (int h = 0; h < HD / 64; ++h) tma_load_2d(sV + st * PAGE + h * 8192, &map_v, h * 64, row, v_full + 8 * st);
+          }
+          __syncwarp();
           if (++st == L.stages) { st = 0; ++lap; }
         }
       }
-      // copies under way land before the block goes
-      for (; jj < loaded; ++jj) {
-        mbar_wait(k_full + 8 * st, lap & 1);
-        if (++st == L.stages) { st = 0; ++lap; }
-      }
+    }
+    if (!ok && lane == 0) atomicExch(ta.status, 92);
+    // copies under way land before the block goes
+    for (int i = 0; i < L.stages; ++i) {
+      if (st == 0) { st = L.stages; --lap; }
+      if (lap < 0) break;
+      --st;
+      mbar_wait(k_full + 8 * st, lap & 1);
+      mbar_wait(v_full + 8 * st, lap & 1);
     }
   } else if (warp == 1) {
     if (elect_one()) {
+      // ---- scores: item x is a page of one group, x & 1, whose item x >> 1 it is ----
+      constexpr uint32_t idesc = instr_desc(kTtRows, 64);
+      int st = 0, lap = 0, x = 0;
+      for (int seg = 0;; ++seg) {
+        const int qb = L.queries == 2 ? seg & 1 : 0, q_lap = L.queries == 2 ? seg >> 1 : seg;
+        if (!mbar_wait(q_full + 8 * qb, q_lap & 1)) { atomicExch(ta.status, 93); break; }
+        const int n = desc[qb].n;
+        const bool dual = desc[qb].rows > kTtRows;
+        if (n == 0) break;
+        bool ok = true;
+        for (int i = 0; i < n && ok; ++i) {
+          if (!mbar_wait(k_full + 8 * st, lap & 1)) { atomicExch(ta.status, 94); ok = false; break; }
+          for (int d = 0; d < (dual ? 2 : 1); ++d, ++x) {
+            const int g = x & 1, c = x >> 1, b = c & 1;
+            // S lands where S and then P of two items ago lay: the product that read that P must be through
+            if (c >= 2 && !mbar_wait(pv_done + 8 * (2 * g + b), ((c >> 1) - 1) & 1)) { atomicExch(ta.status, 95); ok = false; break; }
+            tc_fence_after();
+            const uint32_t q = base + qb * L.q_bytes + (dual ? g * (kTtRows * 128) : 0);
+#pragma unroll
+            for (int h = 0; h < HD / 64; ++h) {
+              const uint64_t dq = smem_desc(q + h * L.rows * 128), dk = smem_desc(sK + st * PAGE + h * 8192);
+#pragma unroll
+              for (int k4 = 0; k4 < 4; ++k4)
+                mma_bf16_ss(tmem + (uint32_t)(g * 256 + b * 64), dq + (uint64_t)(k4 * 2), dk + (uint64_t)(k4 * 2), idesc, (h > 0 || k4 > 0) ? 1u : 0u);
+            }
+            mma_commit(s_full + 8 * (2 * g + b));
+          }
+          if (!ok) break;
+          mma_commit(k_free + 8 * st);
+          if (++st == L.stages) { st = 0; ++lap; }
+        }
+        if (!ok) break;
+        mma_commit(q_free + 8 * qb);
+      }
+    }
+  } else if (warp == 2) {
+    if (elect_one()) {
       // ---- values ----
       constexpr uint32_t idesc = instr_desc(kTtRows, HD, true);
-      TtPages pages(run, a);
-      int st = 0, lap = 0, jj = 0, seg = 0, lst = 0, loaded = 0;
-      auto load = [&]() {
-        int row;
-        if (!pages.next(a, row)) return;
-        mbar_expect_tx(v_full + 8 * lst, PAGE);
-#pragma unroll
-        for (int h = 0; h < HD / 64; ++h) tma_load_2d(sV + lst * PAGE + h * 8192, &map_v, h * 64, row, v_full + 8 * lst);
-        if (++lst == L.stages) lst = 0;
-        ++loaded;
-      };
-      for (int i = 0; i + 1 < L.stages; ++i) load();
-      bool ok = true;
-      while (ok && run.next(a)) {
+      int st = 0, lap = 0, x = 0;
+      for (int seg = 0;; ++seg) {
+        const int qb = L.queries == 2 ? seg & 1 : 0, q_lap = L.queries == 2 ? seg >> 1 : seg;
+        if (!mbar_wait(q_full + 8 * qb, q_lap & 1)) { atomicExch(ta.status, 96); break; }
+        const int n = desc[qb].n;
+        const bool dual = desc[qb].rows > kTtRows;
+        if (n == 0) break;
+        mbar_arrive(q_free + 8 * qb);
         if (seg > 0 && !mbar_wait(o_free, (seg - 1) & 1)) { atomicExch(ta.status, 96); break; }
-        ++seg;
-        for (int i = 0; i < run.n; ++i, ++jj) {
-          const int b = jj & 1, before = st ? st - 1 : L.stages - 1;
-          if (jj >= 1 && !mbar_wait(v_free + 8 * before, (st ? lap : lap - 1) & 1)) { atomicExch(ta.status, 92); ok = false; break; }
-          load();
+        uint32_t fresh = 3u;      // groups without a product in this segment
+        bool ok = true;
+        for (int i = 0; i < n && ok; ++i) {
           if (!mbar_wait(v_full + 8 * st, lap & 1)) { atomicExch(ta.status, 97); ok = false; break; }
-          if (!mbar_wait(p_full + 8 * b, (jj >> 1) & 1)) { atomicExch(ta.status, 98); ok = false; break; }
-          tc_fence_after();
+          for (int d = 0; d < (dual ? 2 : 1); ++d, ++x) {
+            const int g = x & 1, c = x >> 1, b = c & 1;
+            if (!mbar_wait(p_full + 8 * (2 * g + b), (c >> 1) & 1)) { atomicExch(ta.status, 98); ok = false; break; }
+            tc_fence_after();
 #pragma unroll
-          for (int k4 = 0; k4 < 4; ++k4) {
-            const uint64_t dv = smem_desc_mn(sV + st * PAGE + k4 * 2048, 8192, 1024);
-            mma_bf16_ts(tO, tmem + (uint32_t)(b * 64 + k4 * 8), dv, idesc, (i > 0 || k4 > 0) ? 1u : 0u);
+            for (int k4 = 0; k4 < 4; ++k4) {
+              const uint64_t dv = smem_desc_mn(sV + st * PAGE + k4 * 2048, 8192, 1024);
+              mma_bf16_ts(tmem + (uint32_t)(g * 256 + 128), tmem + (uint32_t)(g * 256 + b * 64 + k4 * 8), dv, idesc, k4 > 0 || !(fresh >> g & 1u) ? 1u : 0u);
+            }
+            fresh &= ~(1u << g);
+            mma_commit(pv_done + 8 * (2 * g + b));
           }
-          mma_commit(pv_done + 8 * b);
+          if (!ok) break;
           mma_commit(v_free + 8 * st);
           if (++st == L.stages) { st = 0; ++lap; }
         }
+        if (!ok) break;
       }
-      for (; jj < loaded; ++jj) {
-        mbar_wait(v_full + 8 * st, lap & 1);
-        if (++st == L.stages) { st = 0; ++lap; }
+    }
+  } else if (warp == 3) {
+    // ---- segments and their queries, as a tile that TMA would have left: 64 channels a half, 16-byte pieces exchanged by the row ----
+    TtWalk run = s_run;
+    for (int seg = 0;; ++seg) {
+      const int qb = L.queries == 2 ? seg & 1 : 0, q_lap = L.queries == 2 ? seg >> 1 : seg;
+      const bool more = run.next(a);
+      if (q_lap > 0 && !mbar_wait(q_free + 8 * qb, (q_lap - 1) & 1)) {
+        if (lane == 0) atomicExch(ta.status, 103);
+        break;
       }
+      const uint32_t q = base + qb * L.q_bytes;
+      if (more && !ta.q_by_tma) {
+        constexpr int PIECES = HD / 8, AT_ONCE = 32 / PIECES;
+        const int piece = lane % PIECES;
+        int r = lane / PIECES, node = (run.tile * kTtTile + r) / G, head = run.tile * kTtTile + r - node * G;
+        for (; r < run.rows; r += AT_ONCE) {
+          tt_copy16(q + (piece >> 3) * (L.rows * 128) + r * 128 + (((piece & 7) ^ (r & 7)) << 4),
+                    (const __nv_bfloat16*)a.q + ((size_t)(run.s.tok0 + node) * a.heads + run.kh * G + head) * HD + piece * 8);
+          for (head += AT_ONCE; head >= G; head -= G) ++node;
+        }
+      }
+      if (lane == 0) desc[qb] = run;
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      fence_smem_to_async();
+      __syncwarp();
+      if (elect_one()) {
+        if (more && ta.q_by_tma) {      // a tile that begins with a whole group, zeros or another sequence's queries behind its rows
+          mbar_expect_tx(q_full + 8 * qb, L.q_bytes);
+#pragma unroll
+          for (int h = 0; h < HD / 64; ++h) tma_load_3d(q + h * (L.rows * 128), &map_q, h * 64, run.kh * G, run.s.tok0 + run.tile * kTtTile / G, q_full + 8 * qb);
+        } else {
+          mbar_arrive(q_full + 8 * qb);
+        }
+      }
+      if (!more) break;
     }
   } else {
     // ---- softmax: tensor-memory lanes 32 (warp % 4) .. + 31 hold the rows; two warps share them, keys 0..31 and 32..63 of a page ----
-    const int quad = warp & 3, half = (warp - 2) >> 2, r = quad * 32 + lane, stid = tid - 64;
-    const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16);
-    unsigned short* xch = reinterpret_cast<unsigned short*>(smem + L.xch_off);      // [2 pages][2 halves][128 rows]
-    float* xl = reinterpret_cast<float*>(smem + L.sum_off);                          // [2 halves][128 rows]
-    uint32_t* poison = reinterpret_cast<uint32_t*>(smem + L.poison_off);             // [rows][HD / 16]
-    // A wait that gives up ends nothing here: the warp notes it and walks on to the end, because others meet it at barriers; the status word says so.
+    const int quad = warp & 3, g = (warp - 4) >> 3, half = (warp - 4) >> 2 & 1, r = quad * 32 + lane, stid = tid - 128, gtid = stid & 255;
+    const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16), own = lane_addr + g * 256;
+    uint32_t* poison = reinterpret_cast<uint32_t*>(smem + L.poison_off) + (g * kTtRows + r) * WORDS;      // [2 groups][128 rows][WORDS]; of the other group: other_poison words on
+    const int other_poison = g ? -kTtRows * WORDS : kTtRows * WORDS;
+    float4* ml = reinterpret_cast<float4*>(smem + L.ml_off);                  // [2 groups][2 halves][128 rows] maximum, sum, whether there is poison
+    unsigned short* xch = reinterpret_cast<unsigned short*>(smem + L.xch_off) + g * 512 + r;      // [2 groups][2 buffers][2 halves][128 rows]
+    // A wait that gives up ends nothing here: the warp notes it and walks on to the segment's end, because others meet it at barriers; the status word says so.
     bool ok = true;
     auto wait_warp = [&](uint32_t bar, uint32_t parity, int code) {
       if (ok && !mbar_wait(bar, parity)) {
@@ -327,264 +386,308 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant_
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
     };
-    auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory"); };
-    auto all_sync = [&]() { asm volatile("bar.sync 5, 256;" ::: "memory"); };
-    int st = 0, lap = 0, jj = 0;
-    while (run.next(a)) {
-      const int kh = run.kh, R0 = run.tile * kTtRows, rows = min(kTtRows, run.rows - R0), R = R0 + r, n = run.n;
-      // queries, as a tile that TMA would have left: 64 channels a half, 16-byte pieces exchanged by the row
-      for (int e = stid; e < L.rows * (HD / 8); e += kTtSoft) {
-        const int qr = e / (HD / 8), col = e % (HD / 8) * 8;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (qr < rows) v = *reinterpret_cast<const uint4*>((const __nv_bfloat16*)a.q + ((size_t)(run.tok0 + (R0 + qr) / G) * a.heads + kh * G + (R0 + qr) % G) * HD + col);
-        *reinterpret_cast<uint4*>(smem + (col >> 6) * (L.rows * 128) + qr * 128 + ((((col >> 3) & 7) ^ (qr & 7)) << 4)) = v;
+    auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(1 + 4 * g + quad) : "memory"); };
+    auto look_sync = [&](bool both) {      // of a group, or of both
+      asm volatile("bar.sync %0, %1;" ::"r"(both ? 11 : 9 + g), "r"(both ? 512 : 256) : "memory");
+    };
+    int page_no = 0, x = 0;      // pages and items so far, over all segments
+    int looked[2] = {0, 0};      // pages whose values were looked through: of this group's, of both groups'
+    for (int seg = 0;; ++seg) {
+      const int qb = L.queries == 2 ? seg & 1 : 0, q_lap = L.queries == 2 ? seg >> 1 : seg;
+      {
+        const uint32_t lost = mbar_wait(q_full + 8 * qb, q_lap & 1) ? 0u : 1u;      // all or none go on
+        uint32_t any;
+        __syncwarp();
+        asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 11, 512, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(any) : "r"(lost) : "memory");
+        if (any) {
+          if (stid == 0) atomicExch(ta.status, 104);
+          break;
+        }
       }
-      for (int e = stid; e < L.rows * (HD / 16); e += kTtSoft) poison[e] = 0u;
-      fence_smem_to_async();
-      arrive_warp(q_full);
-      const bool live = r < rows, warp_live = quad * 32 < rows;
-      const uint32_t* words = a.seen + (size_t)(run.tok0 + (live ? R / G : 0)) * a.words;
+      const TtWalk& w = desc[qb];
+      const int n = w.n;
+      if (n == 0) break;
+      const int past = w.s.past, key_first = (w.s.page_lo + w.off) * 64;
+      const bool dual = w.rows > kTtRows;
+      const int in_tile = dual ? g * kTtRows + r : r;
+      const bool live = in_tile < w.rows, warp_live = in_tile - lane < w.rows;
+      const int node = w.s.tok0 + (live ? (w.tile * kTtTile + in_tile) / G : 0);
+      const uint32_t* words = a.seen + (size_t)node * a.words;
       int lo = 0, lo_most = 0;
       if (a.window > 0) {      // the latest beginning of a window in the tile
-        lo = live ? tree_lo(a, run.tok0 + R / G, run.past) : 0;
-        if (live) atomicMax(&s_lo, lo);
-        all_sync();
-        lo_most = s_lo;
+        lo = live ? tree_lo(a, node, past) : 0;
+        if (live && half == 0) atomicMax(&s_lo[seg & 1], lo);
+        look_sync(true);
+        lo_most = s_lo[seg & 1];
+        if (stid == 0) s_lo[(seg + 1) & 1] = 0;      // (read for the last time before the barrier above)
       }
       float m_used = -INFINITY, l = 0.0f;
-      for (int i = 0; i < n; ++i, ++jj) {
-        const int b = jj & 1, key_page = (run.page_lo + run.off + i) * 64, key0 = key_page + half * 32;
-        wait_warp(s_full + 8 * b, (jj >> 1) & 1, 99);
-        const bool mixed = key_page + 63 >= run.past || key_page < lo_most;      // not all rows see all of the page
+      bool poisoned = false;
+      int done = 0;      // this group's items in the segment
+      for (int i = 0; i < n; ++i, ++page_no) {
+        if (dual) {
+          x += 2;
+        } else if ((x++ & 1) != g) {
+          continue;
+        }
+        const int c = (dual ? x - 2 + ((x & 1) != g) : x - 1) >> 1, b = c & 1;      // the item's number among the group's
+        const int key_page = key_first + i * 64, key0 = key_page + half * 32;
+        wait_warp(s_full + 8 * (2 * g + b), (c >> 1) & 1, 99);
+        const bool mixed = key_page + 63 >= past || key_page < lo_most;      // not all rows see all of the page
         uint32_t seen = 0xffffffffu;
         if (warp_live) {
           tc_fence_after();
           uint32_t sr[32];
-          tmem_ld32(lane_addr + (uint32_t)(b * 64 + half * 32), sr);
+          tmem_ld32(own + (uint32_t)(b * 64 + half * 32), sr);
           if (mixed) {
-            const int to = run.past - key0, from = lo - key0;
+            const int to = past - key0, from = lo - key0;
             seen = (to >= 32 ? 0xffffffffu : to <= 0 ? 0u : (1u << to) - 1u) & (from <= 0 ? 0xffffffffu : from >= 32 ? 0u : 0xffffffffu << from);
-            if (key0 + 31 >= run.past) seen |= (uint32_t)tree_bits(words, a.words, key0 - run.past, run.count);
+            if (key0 + 31 >= past) seen |= (uint32_t)tree_bits(words, a.words, key0 - past, w.s.count);
             if (!live) seen = 0u;
 #pragma unroll
-            for (int c = 0; c < 32; ++c)
-              if (!(seen >> c & 1u)) sr[c] = 0xff800000u;     // -inf
+            for (int k = 0; k < 32; ++k)
+              if (!(seen >> k & 1u)) sr[k] = 0xff800000u;     // -inf
           }
-          float mx = -INFINITY;
+          float mx = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
-          for (int c = 0; c < 32; c += 2) mx = tt_max3(mx, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
+          for (int k = 0; k < 32; k += 4) {
+            mx = tt_max3(mx, __uint_as_float(sr[k]), __uint_as_float(sr[k + 1]));
+            mx1 = tt_max3(mx1, __uint_as_float(sr[k + 2]), __uint_as_float(sr[k + 3]));
+          }
           // The row's maximum is the larger of the two halves'. They are exchanged rounded up to 16 bits (any common reference at or above the maximum serves a
           // softmax), so both threads of a row take the same decisions.
           {
-            const uint32_t bits = __float_as_uint(mx);
+            const uint32_t bits = __float_as_uint(fmaxf(mx, mx1));
             const unsigned short up = (unsigned short)(((bits & 0x80000000u) ? bits : bits + 0xffffu) >> 16);
-            xch[b * 256 + half * 128 + r] = up;      // (a place per parity: the partner passes the barrier of the next page only after reading this one)
+            xch[b * 256 + half * 128] = up;      // (a place per buffer: the partner passes the barrier of the next item only after reading this one)
             pair_sync();
-            const unsigned short other = xch[b * 256 + (half ^ 1) * 128 + r];
+            const unsigned short other = xch[b * 256 + (half ^ 1) * 128];
             mx = fmaxf(__uint_as_float((uint32_t)up << 16), __uint_as_float((uint32_t)other << 16));
           }
           const float m_new = fmaxf(m_used, mx * ta.scale_log2);      // the scale is positive
           const bool grow = m_new > m_used + kTtRescale;              // also true for the first finite maximum
-          if (i > 0 && __any_sync(0xffffffffu, grow)) {
-            wait_warp(pv_done + 8 * ((jj - 1) & 1), ((jj - 1) >> 1) & 1, 100);      // O must hold all of the last product
+          if (done > 0 && __any_sync(0xffffffffu, grow)) {
+            wait_warp(pv_done + 8 * (2 * g + (b ^ 1)), ((c - 1) >> 1) & 1, 100);      // O must hold all of the last product
             tc_fence_after();
             const float alpha = grow ? tt_ex2(m_used - m_new) : 1.0f;
-#pragma unroll
+#pragma unroll 1
             for (int c0 = 0; c0 < HD / 2; c0 += 16) {      // this thread's half of the accumulator row
               uint32_t o[16];
-              tmem_ld16(lane_addr + 128 + half * (HD / 2) + c0, o);
+              tmem_ld16(own + 128 + half * (HD / 2) + c0, o);
 #pragma unroll
-              for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
-              tmem_st16(lane_addr + 128 + half * (HD / 2) + c0, o);
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+              tmem_st16(own + 128 + half * (HD / 2) + c0, o);
             }
             l *= alpha;
           }
           if (grow) m_used = m_new;
           const float neg_m = m_used == -INFINITY ? 0.0f : -m_used;
-          uint32_t pk[16];
           float l0 = 0.0f, l1 = 0.0f;
+          uint32_t pk[16];
 #pragma unroll
-          for (int c = 0; c < 32; c += 2) {
-            const float p0 = tt_ex2(fmaf(__uint_as_float(sr[c]), ta.scale_log2, neg_m)), p1 = tt_ex2(fmaf(__uint_as_float(sr[c + 1]), ta.scale_log2, neg_m));
+          for (int k = 0; k < 32; k += 2) {
+            const float p0 = tt_ex2(fmaf(__uint_as_float(sr[k]), ta.scale_log2, neg_m)), p1 = tt_ex2(fmaf(__uint_as_float(sr[k + 1]), ta.scale_log2, neg_m));
             __nv_bfloat162 h2 = __floats2bfloat162_rn(p0, p1);
-            pk[c >> 1] = *reinterpret_cast<uint32_t*>(&h2);
+            pk[k >> 1] = *reinterpret_cast<uint32_t*>(&h2);
             l0 += p0;
             l1 += p1;
           }
+          tmem_st16(own + (uint32_t)(b * 64 + half * 16), pk);
           l += l0 + l1;
-          tmem_st16(lane_addr + (uint32_t)(b * 64 + half * 16), pk);
         }
+        ++done;
         if (mixed) {
-          // values that are not finite go; rows that see one remember it
+          // values that are not finite go; rows that see one remember it. Two groups on one page look together, since what one has taken out the other would miss
+          const int st = page_no % L.stages, lap = page_no / L.stages;
           wait_warp(v_full + 8 * st, lap & 1, 101);
-          const int held = run.past + run.count - key_page;      // rows of the page that belong to the sequence
-#pragma unroll
-          for (int e = stid; e < 64 * HD / 8; e += kTtSoft) {
-            const int row = e & 63, slab = e >> 6;           // a 16-byte piece of a row, in any order
-            const uint32_t at = sV + st * PAGE + (slab >> 3) * 8192 + row * 128 + (slab & 7) * 16;
+          const int held = past + w.s.count - key_page;      // rows of the page that belong to the sequence
+          uint32_t* odd = dual ? s_odd[2][looked[1]++ & 1] : s_odd[g][looked[0]++ & 1];
+          bool wrote = false;
+#pragma unroll 1
+          for (int e = dual ? stid : gtid; e < 64 * HD / 8; e += dual ? 512 : 256) {
+            const int row = e >> 3 & 63;                 // a 16-byte piece of a row, as the pieces lie
+            const uint32_t at = sV + st * PAGE + e * 16;
             uint4 v;
             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
-            auto bad = [](uint32_t x) { return ((x & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((x & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u); };
-            const uint32_t b0 = bad(v.x), b1 = bad(v.y), b2 = bad(v.z), b3 = bad(v.w);
-            if (b0 | b1 | b2 | b3) {
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x & ~b0), "r"(v.y & ~b1), "r"(v.z & ~b2), "r"(v.w & ~b3) : "memory");
-              if (row < held) atomicOr(&s_odd[row >> 5], 1u << (row & 31));
+            auto carry = [](uint32_t y) { return (y & 0x7fff7fffu) + 0x00800080u; };      // bit 15 and 31: an exponent of all ones
+            if ((carry(v.x) | carry(v.y) | carry(v.z) | carry(v.w)) & 0x80008000u) {
+              auto bad = [](uint32_t y) { return ((y & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((y & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u); };
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x & ~bad(v.x)), "r"(v.y & ~bad(v.y)), "r"(v.z & ~bad(v.z)), "r"(v.w & ~bad(v.w)) : "memory");
+              if (row < held) atomicOr(&odd[row >> 5], 1u << (row & 31));
+              wrote = true;
             }
           }
-          fence_smem_to_async();
-          all_sync();
-          const uint32_t odd0 = s_odd[0], odd1 = s_odd[1];
-          if (odd0 | odd1) {
-            const int page = a.block_table[(size_t)run.seq * a.table_stride + key_page / 64];
-            for (uint32_t left = live ? (half ? odd1 : odd0) & seen : 0u; left; left &= left - 1) {
-              const uint32_t* v = reinterpret_cast<const uint32_t*>((const __nv_bfloat16*)a.v_pool + (((size_t)page * a.kv_heads + kh) * 64 + half * 32 + __ffs(left) - 1) * HD);
-              for (int c = 0; c < HD; ++c) {
-                const uint32_t x = v[c >> 1] >> (c & 1) * 16 & 0xffffu;
-                if ((x & 0x7f80u) == 0x7f80u) {
-                  atomicOr(&poison[r * (HD / 16) + c / 16], ((x & 0x7fu) ? 3u : x >> 15 ? 2u : 1u) << (c % 16 * 2));
-                  s_poison = 1;
-                }
+          if (wrote) fence_smem_to_async();
+          look_sync(dual);
+          if (odd[0] | odd[1]) {
+            uint32_t left = live ? odd[half] & seen : 0u;
+            look_sync(dual);
+            if (gtid < 2 && (g == 0 || !dual)) odd[gtid] = 0u;
+            // the row's two threads one after the other: they share its words
+            if (half == 0 && live && !poisoned)
+              for (int k = 0; k < WORDS; ++k) poison[k] = 0u;
+            poisoned = true;
+            look_sync(dual);
+            const int page = a.block_table[(size_t)w.seq * a.table_stride + key_page / 64];
+            for (; left; left &= left - 1) {
+              const uint32_t* v = reinterpret_cast<const uint32_t*>((const __nv_bfloat16*)a.v_pool + (((size_t)page * a.kv_heads + w.kh) * 64 + half * 32 + __ffs(left) - 1) * HD);
+#pragma unroll 1
+              for (int k = 0; k < HD; ++k) {
+                const uint32_t y = v[k >> 1] >> (k & 1) * 16 & 0xffffu;
+                if ((y & 0x7f80u) == 0x7f80u) atomicOr(&poison[k / 16], ((y & 0x7fu) ? 3u : y >> 15 ? 2u : 1u) << (k % 16 * 2));
               }
             }
-            all_sync();
-            if (stid < 2) s_odd[stid] = 0u;
-            all_sync();
           }
         }
         tc_fence_before();
-        arrive_warp(p_full + 8 * b);
-        if (++st == L.stages) { st = 0; ++lap; }
+        arrive_warp(p_full + 8 * (2 * g + b));
       }
-      // ---- the segment's results ----
-      wait_warp(pv_done + 8 * ((jj - 1) & 1), ((jj - 1) >> 1) & 1, 102);
-      const bool begins = run.off == 0, complete = begins && n == run.pages;
-      if (begins && stid == 0) {      // (the segment's first unit is u - n)
-        const long long last = run.u - n + run.pages - 1;
-        ta.info[((long long)run.seq * a.kv_heads + kh) * ta.tiles + run.tile] = make_int2((int)blockIdx.x, (int)(((last + 1) * blocks - 1) / total) - (int)blockIdx.x + 1);
-      }
+      // ---- the segment's results: of a tile of up to 128 rows the groups join theirs, a quarter of the channels a thread; else half ----
+      const int first_item = x - (dual ? 2 * n : n);
+      auto items = [&](int group) { return dual ? n : (n + (((first_item & 1) == group) ? 1 : 0)) / 2; };      // of a group in the segment
+      auto wait_done = [&](int group) {      // its last one
+        const int last = (x - 1 - (((x - 1) & 1) != group)) >> 1;
+        wait_warp(pv_done + 8 * (2 * group + (last & 1)), (last >> 1) & 1, 102);
+      };
+      if (live) ml[(g * 2 + half) * kTtRows + r] = make_float4(m_used, l, poisoned ? 1.0f : 0.0f, 0.0f);
+      look_sync(true);
+      const bool begins = w.off == 0, complete = begins && n == w.s.pages;
+      if (begins && stid == 0)
+        ta.info[((long long)w.seq * a.kv_heads + w.kh) * ta.tiles + w.tile] =
+            make_int2((int)blockIdx.x, complete ? 1 : TtShare(total, min((int)gridDim.x, total)).block_of(w.first + w.s.pages - 1) - (int)blockIdx.x + 1);
+      const bool mine_here = items(g) > 0, other_here = !dual && items(g ^ 1) > 0;
       if (warp_live) {
-        xl[half * 128 + r] = l;
-        pair_sync();
-        l += xl[(half ^ 1) * 128 + r];
+        if (mine_here) wait_done(g);
+        if (other_here) wait_done(g ^ 1);
         tc_fence_after();
-      }
-      all_sync();      // (poison is complete)
-      const float inv = !complete ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-      const size_t slot = (size_t)blockIdx.x * 2 + (begins ? 1 : 0);
-#pragma unroll
-      for (int c0 = 0; c0 < HD / 2; c0 += 16) {      // this thread's half of the accumulator row
-        if (!warp_live) break;
-        uint32_t o[16];
-        __syncwarp();
-        tmem_ld16(lane_addr + 128 + half * (HD / 2) + c0, o);
-        if (!live) continue;
-        const int ch = half * (HD / 2) + c0;
-        const uint32_t x = s_poison ? poison[r * (HD / 16) + ch / 16] : 0u;
-#pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          float v = l == 0.0f ? 0.0f : __uint_as_float(o[c]) * inv;      // (0: nothing seen)
-          if (x >> (2 * c) & 3u) v += (x >> (2 * c) & 3u) == 1u ? INFINITY : (x >> (2 * c) & 3u) == 2u ? -INFINITY : NAN;
-          o[c] = __float_as_uint(v);
+        float4 me = ml[(g * 2 + half) * kTtRows + r], them = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+        me.y += ml[(g * 2 + (half ^ 1)) * kTtRows + r].y;
+        if (other_here) {
+          them = ml[((g ^ 1) * 2 + half) * kTtRows + r];
+          them.y += ml[((g ^ 1) * 2 + (half ^ 1)) * kTtRows + r].y;
         }
+        const float M = fmaxf(me.x, them.x), use = M == -INFINITY ? 0.0f : M;
+        float f = mine_here ? tt_ex2(me.x - use) : 0.0f, fo = other_here ? tt_ex2(them.x - use) : 0.0f;
+        const float sum = me.y * f + them.y * fo;
         if (complete) {
-#pragma unroll
-          for (int c = 0; c < 16; c += 8) {
-            uint32_t w[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              __nv_bfloat162 h2 = __floats2bfloat162_rn(__uint_as_float(o[c + 2 * k]), __uint_as_float(o[c + 2 * k + 1]));
-              w[k] = *reinterpret_cast<uint32_t*>(&h2);
-            }
-            const int piece = (ch + c) >> 3;      // (rows in the queries' place, pieces exchanged so that a warp's rows meet different banks)
-            *reinterpret_cast<uint4*>(smem + r * (HD * 2) + (((piece & ~7) | ((piece ^ r) & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        } else {
-          float* part = ta.part + (slot * HD + ch) * L.rows + r;
-#pragma unroll
-          for (int c = 0; c < 16; ++c) part[(size_t)c * L.rows] = __uint_as_float(o[c]);
+          const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+          f *= inv;
+          fo *= inv;
         }
+        // (a share that saw nothing, whose products are of nothing but zeros, stays out; one whose scores were all NaN has a sum of NaN)
+        const bool take = mine_here && me.y != 0.0f, take_other = other_here && them.y != 0.0f;
+        const size_t slot = (size_t)blockIdx.x * 2 + (begins ? 1 : 0);
+        const int width = dual ? HD / 2 : HD / 4, ch0 = dual ? half * width : (2 * g + half) * width;
+#pragma unroll 1
+        for (int ch = ch0; ch < ch0 + width; ch += 16) {
+          float v[16];
+          uint32_t o[16];
+          __syncwarp();
+          if (mine_here) tmem_ld16(own + 128 + ch, o);
+#pragma unroll
+          for (int k = 0; k < 16; ++k) v[k] = take ? __uint_as_float(o[k]) * f : 0.0f;
+          if (other_here) {
+            __syncwarp();
+            tmem_ld16(lane_addr + (g ^ 1) * 256 + 128 + ch, o);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) v[k] = take_other ? fmaf(__uint_as_float(o[k]), fo, v[k]) : v[k];
+          }
+          if (live) {
+            if (me.z != 0.0f || them.z != 0.0f) {
+              const uint32_t bad = (me.z != 0.0f ? poison[ch / 16] : 0u) | (them.z != 0.0f ? poison[other_poison + ch / 16] : 0u);
+#pragma unroll
+              for (int k = 0; k < 16; ++k) {
+                const uint32_t y = bad >> (2 * k) & 3u;
+                if (y) v[k] += y == 1u ? INFINITY : y == 2u ? -INFINITY : NAN;
+              }
+            }
+            if (complete) {
+              uint32_t y[8];
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                __nv_bfloat162 h2 = __floats2bfloat162_rn(v[2 * k], v[2 * k + 1]);
+                y[k] = *reinterpret_cast<uint32_t*>(&h2);
+              }
+              uint4* out = reinterpret_cast<uint4*>((__nv_bfloat16*)a.out + ((size_t)node * a.heads + w.kh * G + (w.tile * kTtTile + in_tile) % G) * HD + ch);
+              if (ok) {
+                out[0] = make_uint4(y[0], y[1], y[2], y[3]);
+                out[1] = make_uint4(y[4], y[5], y[6], y[7]);
+              }
+            } else {
+              float* part = ta.part + (slot * HD + ch) * L.rows + in_tile;
+#pragma unroll
+              for (int k = 0; k < 16; ++k) part[(size_t)k * L.rows] = v[k];
+            }
+          }
+        }
+        if (live && !complete && half == 0 && (dual || g == 0)) ta.part_ml[slot * L.rows + in_tile] = make_float2(M, sum);
       }
       tc_fence_before();
       arrive_warp(o_free);
-      if (complete) {
-        all_sync();
-        for (int e = stid; e < rows * (HD / 8); e += kTtSoft) {
-          const int rr = e / (HD / 8), piece = e % (HD / 8);
-          const uint4 v = *reinterpret_cast<const uint4*>(smem + rr * (HD * 2) + (((piece & ~7) | ((piece ^ rr) & 7)) << 4));
-          if (ok) *reinterpret_cast<uint4*>((__nv_bfloat16*)a.out + ((size_t)(run.tok0 + (R0 + rr) / G) * a.heads + kh * G + (R0 + rr) % G) * HD + piece * 8) = v;
-        }
-      } else if (live && half == 0) {
-        ta.part_ml[slot * L.rows + r] = make_float2(m_used, l);
-      }
-      all_sync();
-      if (stid == 0) s_lo = s_poison = 0;
-      all_sync();
+      arrive_warp(q_free + 8 * qb);
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256) : "memory");
+  if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
-// Joins the shares of what no block finished alone: a block takes 8 or more channels of a (sequence, kv head, tile), a thread a row and eight channels.
+// Joins the shares of what no block finished alone: a thread a row and four channels, eight shares on the way at once.
 template <int HD>
 __global__ void __launch_bounds__(256) tree_tc_join_kernel(TtArgs ta) {
   pdl_wait();
   const TreeArgs& a = ta.t;
   const int rows_pad = ta.lay.rows, seq = blockIdx.z, kh = blockIdx.y / ta.tiles, tile = blockIdx.y % ta.tiles, G = a.heads / a.kv_heads;
   const TreeSeq s(a, seq);
-  const int rows = min(kTtRows, s.count * G - tile * kTtRows);
+  const int rows = min(kTtTile, s.count * G - tile * kTtTile);
   if (rows <= 0) return;
   const int2 in = ta.info[((size_t)seq * a.kv_heads + kh) * ta.tiles + tile];
   if (in.y == 1) return;      // its block has finished it
-  const int e = blockIdx.x * 256 + threadIdx.x, r = e % rows_pad, c0 = e / rows_pad * 8;
+  const int e = blockIdx.x * 256 + threadIdx.x, r = e % rows_pad, c0 = e / rows_pad * 4;
   if (r >= rows || c0 >= HD) return;
   auto slot_of = [&](int i) { return (size_t)(in.x + i) * 2 + (i == 0 ? 1 : 0); };
-  float M = -INFINITY, l = 0.0f, acc[8];
+  float M = -INFINITY, l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int i0 = 0; i0 < in.y; i0 += 8) {
+    float2 ml[8];
+    float v[8][4];
 #pragma unroll
-  for (int c = 0; c < 8; ++c) acc[c] = 0.0f;
-  for (int i0 = 0; i0 < in.y; i0 += 4) {
-    float2 ml[4];
-    float v[4][8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
       const size_t slot = slot_of(min(i0 + i, in.y - 1));
       ml[i] = ta.part_ml[slot * rows_pad + r];
-      if (i0 + i >= in.y) ml[i] = make_float2(-INFINITY, 0.0f);
 #pragma unroll
-      for (int c = 0; c < 8; ++c) v[i][c] = ta.part[(slot * HD + c0 + c) * rows_pad + r];
+      for (int c = 0; c < 4; ++c) v[i][c] = ta.part[(slot * HD + c0 + c) * rows_pad + r];
     }
     float top = M;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) top = fmaxf(top, ml[i].x);
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, ml[i].x);      // (a share may be looked at twice here)
     const float use = top == -INFINITY ? 0.0f : top, keep = tt_ex2(M - use);
     l *= keep;
 #pragma unroll
-    for (int c = 0; c < 8; ++c) acc[c] *= keep;
+    for (int c = 0; c < 4; ++c) acc[c] *= keep;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 8; ++i) {
       if (i0 + i >= in.y || ml[i].y == 0.0f) continue;      // (a share that saw nothing; one whose scores were all NaN has a sum of NaN)
       const float f = tt_ex2(ml[i].x - use);
       l += ml[i].y * f;
 #pragma unroll
-      for (int c = 0; c < 8; ++c) acc[c] += v[i][c] * f;
+      for (int c = 0; c < 4; ++c) acc[c] += v[i][c] * f;
     }
     M = top;
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  uint32_t w[4];
+  uint32_t w[2];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < 2; ++k) {
     __nv_bfloat162 h2 = __floats2bfloat162_rn(acc[2 * k] * inv, acc[2 * k + 1] * inv);
     w[k] = *reinterpret_cast<uint32_t*>(&h2);
   }
-  const int R = tile * kTtRows + r;
-  *reinterpret_cast<uint4*>((__nv_bfloat16*)a.out + ((size_t)(s.tok0 + R / G) * a.heads + kh * G + R % G) * HD + c0) = make_uint4(w[0], w[1], w[2], w[3]);
+  const int R = tile * kTtTile + r;
+  *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + ((size_t)(s.tok0 + R / G) * a.heads + kh * G + R % G) * HD + c0) = make_uint2(w[0], w[1]);
 }
 
 bool tree_tc_takes(int n_seqs, int max_count, int heads, int kv_heads, int head_dim, int max_keys, int dtype) {
-  const long long tiles = ((long long)max_count * (heads / kv_heads) + kTtRows - 1) / kTtRows;
-  return dtype == kBF16 && (head_dim == 64 || head_dim == 128) && n_seqs * tiles * kv_heads * (max_keys / 64 + 2ll) < (1ll << 31);
+  const long long tiles = ((long long)max_count * (heads / kv_heads) + kTtTile - 1) / kTtTile;
+  return dtype == kBF16 && (head_dim == 64 || head_dim == 128) && n_seqs * tiles * kv_heads * (max_keys / 64 + 2ll + kTtEntry) < (1ll << 31);
 }
 
 struct TtScratch {
@@ -594,10 +697,10 @@ struct TtScratch {
 static TtScratch tt_scratch(int n_seqs, int max_count, int heads, int kv_heads, int head_dim, int max_keys) {
   TtScratch f{};
   const long long rows = (long long)max_count * (heads / kv_heads);
-  f.tiles = (int)((rows + kTtRows - 1) / kTtRows);
-  const long long units = (long long)n_seqs * kv_heads * f.tiles * ((max_keys + 63) / 64 + 1), most = 2ll * sm_count();
-  f.blocks = (int)std::min(units, most);      // as many as run at once
-  const int rows_pad = tt_layout(head_dim, (int)std::min(rows, (long long)kTtRows)).rows;
+  f.tiles = (int)((rows + kTtTile - 1) / kTtTile);
+  const long long units = (long long)n_seqs * kv_heads * f.tiles * (((long long)max_keys + 63) / 64 + 1), most = sm_count();
+  f.blocks = (int)std::min(units, most);      // one an SM
+  const int rows_pad = tt_layout(head_dim, (int)std::min(rows, (long long)kTtTile)).rows;
   long long at = 0;
   auto take = [&](long long n) { const long long o = at; at += (n + 3) & ~3ll; return o; };
   f.part = take(2ll * f.blocks * rows_pad * head_dim);
@@ -623,14 +726,14 @@ static int encode_tree_pool(CUtensorMap* map, const void* base, long long rows, 
 }
 
 template <int HD>
-static int launch_tree_tc(const CUtensorMap& mk, const CUtensorMap& mv, const TtArgs& ta, int blocks, cudaStream_t s) {
+static int launch_tree_tc(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const TtArgs& ta, int blocks, cudaStream_t s) {
   static std::atomic<unsigned long long> allowed;
-  const cudaError_t e = allow_shared((const void*)tree_tc_kernel<HD>, 113 * 1024, allowed);
+  const cudaError_t e = allow_shared((const void*)tree_tc_kernel<HD>, 225 * 1024, allowed);
   if (e != cudaSuccess) return fail(2, "attention_tree: cannot reserve shared memory: %s", cudaGetErrorString(e));
-  launch(tree_tc_kernel<HD>, dim3(blocks), dim3(kTtThreads), (size_t)ta.lay.total, s, mk, mv, ta);
+  launch(tree_tc_kernel<HD>, dim3(blocks), dim3(kTtThreads), (size_t)ta.lay.total, s, mq, mk, mv, ta);
   const int rc = check_launch("attention_tree (tensor cores)");
   if (rc) return rc;
-  launch_prefetching(tree_tc_join_kernel<HD>, dim3((ta.lay.rows * (HD / 8) + 255) / 256, ta.t.kv_heads * ta.tiles, ta.t.n_seqs), dim3(256), 0, s, ta);
+  launch_prefetching(tree_tc_join_kernel<HD>, dim3((ta.lay.rows * (HD / 4) + 255) / 256, ta.t.kv_heads * ta.tiles, ta.t.n_seqs), dim3(256), 0, s, ta);
   return check_launch("attention_tree (tensor cores, joined)");
 }
 
@@ -639,7 +742,7 @@ int tree_tc(const TreeArgs& a, long long pool_pages, int* status, cudaStream_t s
   SLB_REQUIRE((uintptr_t)a.q % 16 == 0 && (uintptr_t)a.k_pool % 16 == 0 && (uintptr_t)a.v_pool % 16 == 0 && (uintptr_t)a.out % 16 == 0 &&
               (uintptr_t)a.scratch % 16 == 0, "attention_tree: q, out, scratch and the pools must be 16-byte aligned");
   SLB_REQUIRE(status != nullptr, "attention_tree: no status word");
-  CUtensorMap mk, mv;
+  CUtensorMap mq{}, mk, mv;
   int rc = encode_tree_pool(&mk, a.k_pool, pool_pages * a.kv_heads * 64, a.head_dim, "the key pool");
   if (rc == 0) rc = encode_tree_pool(&mv, a.v_pool, pool_pages * a.kv_heads * 64, a.head_dim, "the value pool");
   if (rc) return rc;
@@ -653,8 +756,20 @@ int tree_tc(const TreeArgs& a, long long pool_pages, int* status, cudaStream_t s
   ta.info = reinterpret_cast<int2*>(a.scratch + f.info);
   ta.status = status;
   ta.tiles = f.tiles;
-  ta.lay = tt_layout(a.head_dim, (int)std::min((long long)a.max_count * (a.heads / a.kv_heads), (long long)kTtRows));
-  return a.head_dim == 128 ? launch_tree_tc<128>(mk, mv, ta, f.blocks, s) : launch_tree_tc<64>(mk, mv, ta, f.blocks, s);
+  ta.lay = tt_layout(a.head_dim, (int)std::min((long long)a.max_count * (a.heads / a.kv_heads), (long long)kTtTile));
+  const int G = a.heads / a.kv_heads;
+  ta.q_by_tma = 32 % G == 0 && a.tokens < (1ll << 31);
+  if (ta.q_by_tma) {
+    EncodeTiledFn fn = encode_fn();
+    const int nodes = ta.lay.rows / G;
+    cuuint64_t dims[3] = {(cuuint64_t)a.head_dim, (cuuint64_t)a.heads, (cuuint64_t)a.tokens};
+    cuuint64_t strides[2] = {(cuuint64_t)a.head_dim * 2, (cuuint64_t)a.heads * a.head_dim * 2};
+    cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)nodes}, estr[3] = {1, 1, 1};
+    const CUresult r = fn(&mq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(a.q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(2, "attention_tree: cuTensorMapEncodeTiled failed for the queries with code %d", (int)r);
+  }
+  return a.head_dim == 128 ? launch_tree_tc<128>(mq, mk, mv, ta, f.blocks, s) : launch_tree_tc<64>(mq, mk, mv, ta, f.blocks, s);
 }
 
 }  // namespace slb
