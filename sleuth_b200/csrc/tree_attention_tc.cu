@@ -10,6 +10,8 @@
 //   warps 4..19  the softmax: two groups of 256 threads, two threads a row (32 keys of a page each), that take the pages in turn where the tile has up to 128 rows (each with a maximum, a sum
 //                and an accumulator of its own, joined at the segment's end), or every page for 128 rows each where it has more. P is rounded to bfloat16 (the instruction takes no wider one
 //                beside bfloat16 values), the sum is of the unrounded weights, in 32 bits.
+// Where the sequences are few (tt_cluster) the blocks of a cluster share one (sequence, kv head, tile) instead: the shares meet in distributed shared memory, and there is neither a second
+// kernel nor scratch.
 // Rows are row r = node r / G, query head r % G of the group. Fewer than 128 rows leave the instruction's other rows to whatever lies behind the queries in shared memory: a row of
 // A reaches that row of the result alone, and nobody reads it.
 // Rows that a node does not see are masked by a bit each. Their values meet a zero weight in the product, which an infinity or a NaN among them would survive: so in pages that
@@ -18,6 +20,7 @@
 
 #include <algorithm>
 
+#include "packed_f32.cuh"
 #include "tcgen05.cuh"
 #include "tree.cuh"
 
@@ -47,7 +50,7 @@ static TtLayout tt_layout(int HD, int rows) {
   l.queries = l.rows <= kTtRows ? 2 : 1;
   l.q_bytes = l.rows * HD * 2;
   const int page = 64 * HD * 2, rest = 2 * kTtRows * HD / 4 + 2 * 2 * kTtRows * 16 + 2 * 2 * 2 * kTtRows * 2 + 64 * 8;
-  l.stages = std::min(8, (225 * 1024 - l.queries * l.q_bytes - rest) / (2 * page));      // (227 KB a block, 2 KB of it static)
+  l.stages = std::min(8, (223 * 1024 - l.queries * l.q_bytes - rest) / (2 * page));      // (227 KB a block, up to 3 KB of it static)
   l.k_off = l.queries * l.q_bytes;
   l.v_off = l.k_off + l.stages * page;
   l.poison_off = l.v_off + l.stages * page;
@@ -65,6 +68,7 @@ struct TtArgs {
   float2* part_ml;      // [blocks][2][rows] maximum (log2 units) and sum
   int2* info;           // [n, kv_heads, tiles] first block and number of blocks
   int* status;
+  int cluster;          // blocks that share a (sequence, kv head, tile), or 0: runs of all units
   int tiles;            // most tiles of a sequence
   int q_by_tma;         // queries come by TMA: a group divides 32
   TtLayout lay;
@@ -72,7 +76,7 @@ struct TtArgs {
 
 // The pages of a sequence that some node may see: those from the window of a node at `past` on. A (sequence, kv head, tile) counts kTtEntry units more than it has
 // pages: what a segment's beginning and end cost (runs of equal pages left blocks with many short segments behind: 64 sequences of 150 to 4,096 rows, of 148 blocks the median 99 us, the last 136).
-constexpr int kTtEntry = 3;
+constexpr int kTtEntry = 5;
 struct TtSeq {
   int past, count, tok0, page_lo, pages, tiles, units;
   __device__ __forceinline__ void read(const TreeArgs& a, int seq) {
@@ -128,7 +132,18 @@ struct TtWalk {
   }
 };
 
-template <int HD>
+__device__ __forceinline__ float2 tt_peer2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float tt_peer(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+template <int HD, bool CLUSTER>
 __global__ void __launch_bounds__(kTtThreads, 1)
 tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TtArgs ta) {
   constexpr int PAGE = 64 * HD * 2, WORDS = HD / 16;      // words of a row's poison
@@ -139,6 +154,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   __shared__ int s_lo[2];
   __shared__ uint32_t s_odd[3][2][2], tmem_slot;      // rows of a page with values that are not finite: of either group's page, of a page of both; two places used in turn
   __shared__ TtWalk desc[2], s_run;
+  __shared__ float2 s_ml[CLUSTER ? kTtTile : 1];      // a cluster's blocks: maximum and sum of each row
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t base = smem_addr(smem);
   if ((base & 1023u) != 0) {
@@ -165,7 +181,19 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   // where this block's run of units begins
   const int G = a.heads / a.kv_heads;
   int total = 0;
-  {
+  if constexpr (CLUSTER) {
+    if (tid == 0) {      // the block's share of its cluster's pages, as units that begin with this (sequence, kv head, tile)
+      const int pair = (int)blockIdx.x / ta.cluster, rank = (int)blockIdx.x % ta.cluster, at = pair % (a.kv_heads * ta.tiles);
+      s_run.seq = pair / (a.kv_heads * ta.tiles);
+      s_run.s.read(a, s_run.seq);
+      const int kh = at / ta.tiles, tile = at % ta.tiles, share = (s_run.s.pages + ta.cluster - 1) / ta.cluster;
+      s_run.kh = kh;
+      s_run.tile = tile;
+      s_run.seq_first = -(kh * s_run.s.tiles + tile) * (s_run.s.pages + kTtEntry);
+      s_run.u = kTtEntry + min(s_run.s.pages, rank * share);
+      s_run.u_hi = tile < s_run.s.tiles ? kTtEntry + min(s_run.s.pages, (rank + 1) * share) : 0;
+    }
+  } else {
     const int per = (a.n_seqs + kTtThreads - 1) / kTtThreads, q0 = min(a.n_seqs, tid * per), q1 = min(a.n_seqs, q0 + per);
     TtSeq one;
     int own = 0;
@@ -481,19 +509,19 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             l *= alpha;
           }
           if (grow) m_used = m_new;
-          const float neg_m = m_used == -INFINITY ? 0.0f : -m_used;
-          float l0 = 0.0f, l1 = 0.0f;
+          const f32x2 refs = both(m_used == -INFINITY ? 0.0f : -m_used), scales = both(ta.scale_log2);
+          f32x2 sums = 0ull;
           uint32_t pk[16];
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
-            const float p0 = tt_ex2(fmaf(__uint_as_float(sr[k]), ta.scale_log2, neg_m)), p1 = tt_ex2(fmaf(__uint_as_float(sr[k + 1]), ta.scale_log2, neg_m));
+            const f32x2 e = fma2(pair_of(__uint_as_float(sr[k]), __uint_as_float(sr[k + 1])), scales, refs);
+            const float p0 = tt_ex2(__uint_as_float((uint32_t)e)), p1 = tt_ex2(__uint_as_float((uint32_t)(e >> 32)));
             __nv_bfloat162 h2 = __floats2bfloat162_rn(p0, p1);
             pk[k >> 1] = *reinterpret_cast<uint32_t*>(&h2);
-            l0 += p0;
-            l1 += p1;
+            sums = add2(sums, pair_of(p0, p1));
           }
           tmem_st16(own + (uint32_t)(b * 64 + half * 16), pk);
-          l += l0 + l1;
+          l += __uint_as_float((uint32_t)sums) + __uint_as_float((uint32_t)(sums >> 32));
         }
         ++done;
         if (mixed) {
@@ -552,13 +580,13 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       if (live) ml[(g * 2 + half) * kTtRows + r] = make_float4(m_used, l, poisoned ? 1.0f : 0.0f, 0.0f);
       look_sync(true);
       const bool begins = w.off == 0, complete = begins && n == w.s.pages;
-      if (begins && stid == 0)
+      if (!CLUSTER && begins && stid == 0)
         ta.info[((long long)w.seq * a.kv_heads + w.kh) * ta.tiles + w.tile] =
             make_int2((int)blockIdx.x, complete ? 1 : TtShare(total, min((int)gridDim.x, total)).block_of(w.first + w.s.pages - 1) - (int)blockIdx.x + 1);
       const bool mine_here = items(g) > 0, other_here = !dual && items(g ^ 1) > 0;
       if (warp_live) {
         if (mine_here) wait_done(g);
-        if (other_here) wait_done(g ^ 1);
+        if (other_here || (CLUSTER && dual)) wait_done(g ^ 1);      // (a cluster's share goes where the other group's values lay)
         tc_fence_after();
         float4 me = ml[(g * 2 + half) * kTtRows + r], them = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
         me.y += ml[(g * 2 + (half ^ 1)) * kTtRows + r].y;
@@ -569,7 +597,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         const float M = fmaxf(me.x, them.x), use = M == -INFINITY ? 0.0f : M;
         float f = mine_here ? tt_ex2(me.x - use) : 0.0f, fo = other_here ? tt_ex2(them.x - use) : 0.0f;
         const float sum = me.y * f + them.y * fo;
-        if (complete) {
+        if (!CLUSTER && complete) {
           const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
           f *= inv;
           fo *= inv;
@@ -601,7 +629,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 if (y) v[k] += y == 1u ? INFINITY : y == 2u ? -INFINITY : NAN;
               }
             }
-            if (complete) {
+            if (!CLUSTER && complete) {
               uint32_t y[8];
 #pragma unroll
               for (int k = 0; k < 8; ++k) {
@@ -613,14 +641,17 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 out[0] = make_uint4(y[0], y[1], y[2], y[3]);
                 out[1] = make_uint4(y[4], y[5], y[6], y[7]);
               }
-            } else {
-              float* part = ta.part + (slot * HD + ch) * L.rows + in_tile;
+            } else {      // (in a cluster where the ring was: its pages have been multiplied)
+              float* part = (CLUSTER ? reinterpret_cast<float*>(smem + L.k_off) + (size_t)ch * L.rows : ta.part + (slot * HD + ch) * L.rows) + in_tile;
 #pragma unroll
               for (int k = 0; k < 16; ++k) part[(size_t)k * L.rows] = v[k];
             }
           }
         }
-        if (live && !complete && half == 0 && (dual || g == 0)) ta.part_ml[slot * L.rows + in_tile] = make_float2(M, sum);
+        if (live && half == 0 && (dual || g == 0)) {
+          if (CLUSTER) s_ml[in_tile] = make_float2(M, sum);
+          else if (!complete) ta.part_ml[slot * L.rows + in_tile] = make_float2(M, sum);
+        }
       }
       tc_fence_before();
       arrive_warp(o_free);
@@ -630,59 +661,115 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   tc_fence_before();
   __syncthreads();
   if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  if constexpr (CLUSTER) {
+    // the shares meet: every block adds up its part of the (row, four channels)
+    const int kh = s_run.kh, tile = s_run.tile, rank = (int)cluster_ctarank();
+    const TtSeq& s = s_run.s;
+    const int rows = min(kTtTile, s.count * G - tile * kTtTile);
+    if (s_run.u >= s_run.u_hi)      // (a block without pages)
+      for (int r = tid; r < kTtTile; r += kTtThreads) s_ml[r] = make_float2(-INFINITY, 0.0f);
+    __syncthreads();
+    cluster_sync_all();
+    const uint32_t ml_at = smem_addr(s_ml), part_at = base + L.k_off;
+    for (int e = rank * kTtThreads + tid; e < L.rows * (HD / 4); e += ta.cluster * kTtThreads) {
+      const int r = e % L.rows, c0 = e / L.rows * 4;
+      if (r >= rows) continue;
+      float2 p[8];
+      float v[8][4], M = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        p[i] = make_float2(-INFINITY, 0.0f);
+        if (i >= ta.cluster) continue;
+        p[i] = tt_peer2(cluster_map(ml_at + r * 8, i));
+        const uint32_t at = cluster_map(part_at + (c0 * L.rows + r) * 4, i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[i][k] = tt_peer(at + k * L.rows * 4);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) M = fmaxf(M, p[i].x);
+      const float use = M == -INFINITY ? 0.0f : M;
+      float l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i >= ta.cluster || p[i].y == 0.0f) continue;      // (a share that saw nothing, or has no pages)
+        const float f = tt_ex2(p[i].x - use);
+        l += p[i].y * f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[k] += v[i][k] * f;
+      }
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      uint32_t w[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        __nv_bfloat162 h2 = __floats2bfloat162_rn(acc[2 * k] * inv, acc[2 * k + 1] * inv);
+        w[k] = *reinterpret_cast<uint32_t*>(&h2);
+      }
+      const int R = tile * kTtTile + r;
+      *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + ((size_t)(s.tok0 + R / G) * a.heads + kh * G + R % G) * HD + c0) = make_uint2(w[0], w[1]);
+    }
+    __syncthreads();
+    cluster_sync_all();      // the others may still be reading this block's share
+  }
 }
 
-// Joins the shares of what no block finished alone: a thread a row and four channels, eight shares on the way at once.
+// Joins the shares of what no block finished alone: a thread a row and four channels of a quarter of the shares, four of them on the way at once.
 template <int HD>
 __global__ void __launch_bounds__(256) tree_tc_join_kernel(TtArgs ta) {
-  pdl_wait();
   const TreeArgs& a = ta.t;
   const int rows_pad = ta.lay.rows, seq = blockIdx.z, kh = blockIdx.y / ta.tiles, tile = blockIdx.y % ta.tiles, G = a.heads / a.kv_heads;
-  const TreeSeq s(a, seq);
+  const TreeSeq s(a, seq);      // (in front of the wait: what the kernel before this one has waited for is there)
   const int rows = min(kTtTile, s.count * G - tile * kTtTile);
   if (rows <= 0) return;
+  pdl_wait();
   const int2 in = ta.info[((size_t)seq * a.kv_heads + kh) * ta.tiles + tile];
   if (in.y == 1) return;      // its block has finished it
-  const int e = blockIdx.x * 256 + threadIdx.x, r = e % rows_pad, c0 = e / rows_pad * 4;
-  if (r >= rows || c0 >= HD) return;
+  __shared__ float4 acc_s[3][64];
+  __shared__ float2 ml_s[3][64];
+  const int lane = threadIdx.x & 63, part = threadIdx.x >> 6;
+  const int e = blockIdx.x * 64 + lane, r = e % rows_pad, c0 = e / rows_pad * 4;
+  const bool live = r < rows && c0 < HD;
   auto slot_of = [&](int i) { return (size_t)(in.x + i) * 2 + (i == 0 ? 1 : 0); };
-  float M = -INFINITY, l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int i0 = 0; i0 < in.y; i0 += 8) {
-    float2 ml[8];
-    float v[8][4];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const size_t slot = slot_of(min(i0 + i, in.y - 1));
-      ml[i] = ta.part_ml[slot * rows_pad + r];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) v[i][c] = ta.part[(slot * HD + c0 + c) * rows_pad + r];
-    }
-    float top = M;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = fmaxf(top, ml[i].x);      // (a share may be looked at twice here)
-    const float use = top == -INFINITY ? 0.0f : top, keep = tt_ex2(M - use);
-    l *= keep;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) acc[c] *= keep;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (i0 + i >= in.y || ml[i].y == 0.0f) continue;      // (a share that saw nothing; one whose scores were all NaN has a sum of NaN)
-      const float f = tt_ex2(ml[i].x - use);
-      l += ml[i].y * f;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) acc[c] += v[i][c] * f;
-    }
+  const int per = (in.y + 3) / 4, i1 = min(in.y, (part + 1) * per);
+  float M = -INFINITY, l = 0.0f;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  auto join = [&](float2 ml, float4 v) {
+    if (ml.y == 0.0f) return;      // (a share that saw nothing; one whose scores were all NaN has a sum of NaN)
+    const float top = fmaxf(M, ml.x), use = top == -INFINITY ? 0.0f : top, keep = tt_ex2(M - use), f = tt_ex2(ml.x - use);
+    l = l * keep + ml.y * f;
+    acc.x = acc.x * keep + v.x * f;
+    acc.y = acc.y * keep + v.y * f;
+    acc.z = acc.z * keep + v.z * f;
+    acc.w = acc.w * keep + v.w * f;
     M = top;
-  }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  uint32_t w[2];
+  };
+  if (live)
+    for (int i0 = part * per; i0 < i1; i0 += 4) {
+      float2 ml[4];
+      float4 v[4];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    __nv_bfloat162 h2 = __floats2bfloat162_rn(acc[2 * k] * inv, acc[2 * k + 1] * inv);
-    w[k] = *reinterpret_cast<uint32_t*>(&h2);
+      for (int i = 0; i < 4; ++i) {
+        const size_t slot = slot_of(min(i0 + i, i1 - 1));
+        ml[i] = ta.part_ml[slot * rows_pad + r];
+        const float* p = ta.part + (slot * HD + c0) * rows_pad + r;
+        v[i] = make_float4(p[0], p[rows_pad], p[2 * rows_pad], p[3 * rows_pad]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i0 + i < i1) join(ml[i], v[i]);
+    }
+  if (part > 0) {
+    acc_s[part - 1][lane] = acc;
+    ml_s[part - 1][lane] = make_float2(M, l);
   }
+  __syncthreads();
+  if (part > 0 || !live) return;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) join(ml_s[i][lane], acc_s[i][lane]);
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), hi = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
   const int R = tile * kTtTile + r;
-  *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + ((size_t)(s.tok0 + R / G) * a.heads + kh * G + R % G) * HD + c0) = make_uint2(w[0], w[1]);
+  *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + ((size_t)(s.tok0 + R / G) * a.heads + kh * G + R % G) * HD + c0) =
+      make_uint2(*reinterpret_cast<uint32_t*>(&lo), *reinterpret_cast<uint32_t*>(&hi));
 }
 
 bool tree_tc_takes(int n_seqs, int max_count, int heads, int kv_heads, int head_dim, int max_keys, int dtype) {
@@ -690,14 +777,27 @@ bool tree_tc_takes(int n_seqs, int max_count, int heads, int kv_heads, int head_
   return dtype == kBF16 && (head_dim == 64 || head_dim == 128) && n_seqs * tiles * kv_heads * (max_keys / 64 + 2ll + kTtEntry) < (1ll << 31);
 }
 
+// Whether blocks of a cluster share each (sequence, kv head, tile), and how many. A cluster waits for its longest sequence alone, so only where all clusters run at once (128 of the 148 blocks:
+// clusters of eight lie within one of the GPU's partitions each) and no block takes more than ten pages.
+static int tt_cluster(int n_seqs, int kv_heads, int tiles, int max_count, int max_keys, int window) {
+  long long pages = ((long long)max_keys + 63) / 64;
+  if (window > 0) pages = std::min(pages, ((long long)window + max_count + 62) / 64 + 1);
+  const long long pairs = (long long)n_seqs * kv_heads * tiles;
+  int c = 8;
+  while (c > 1 && (pairs * c > 128 || c > pages)) c /= 2;
+  return pairs * c <= 128 && pages <= 10ll * c ? c : 0;
+}
+
 struct TtScratch {
   long long part, part_ml, info, total;
-  int blocks, tiles;
+  int blocks, tiles, cluster;
 };
-static TtScratch tt_scratch(int n_seqs, int max_count, int heads, int kv_heads, int head_dim, int max_keys) {
+static TtScratch tt_scratch(int n_seqs, int max_count, int heads, int kv_heads, int head_dim, int max_keys, int window) {
   TtScratch f{};
   const long long rows = (long long)max_count * (heads / kv_heads);
   f.tiles = (int)((rows + kTtTile - 1) / kTtTile);
+  f.cluster = tt_cluster(n_seqs, kv_heads, f.tiles, max_count, max_keys, window);
+  if (f.cluster) return f;
   const long long units = (long long)n_seqs * kv_heads * f.tiles * (((long long)max_keys + 63) / 64 + 1), most = sm_count();
   f.blocks = (int)std::min(units, most);      // one an SM
   const int rows_pad = tt_layout(head_dim, (int)std::min(rows, (long long)kTtTile)).rows;
@@ -711,7 +811,7 @@ static TtScratch tt_scratch(int n_seqs, int max_count, int heads, int kv_heads, 
 }
 
 long long tree_tc_floats(int n_seqs, int max_count, int heads, int kv_heads, int head_dim, int max_keys) {
-  return tt_scratch(n_seqs, max_count, heads, kv_heads, head_dim, max_keys).total;
+  return tt_scratch(n_seqs, max_count, heads, kv_heads, head_dim, max_keys, 0).total;      // (a window makes no share longer: what a step without one takes is enough)
 }
 
 static int encode_tree_pool(CUtensorMap* map, const void* base, long long rows, int head_dim, const char* what) {
@@ -727,13 +827,17 @@ static int encode_tree_pool(CUtensorMap* map, const void* base, long long rows, 
 
 template <int HD>
 static int launch_tree_tc(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const TtArgs& ta, int blocks, cudaStream_t s) {
-  static std::atomic<unsigned long long> allowed;
-  const cudaError_t e = allow_shared((const void*)tree_tc_kernel<HD>, 225 * 1024, allowed);
+  static std::atomic<unsigned long long> allowed, allowed_clusters;
+  cudaError_t e = ta.cluster ? allow_shared((const void*)tree_tc_kernel<HD, true>, 224 * 1024, allowed_clusters) : allow_shared((const void*)tree_tc_kernel<HD, false>, 224 * 1024, allowed);
   if (e != cudaSuccess) return fail(2, "attention_tree: cannot reserve shared memory: %s", cudaGetErrorString(e));
-  launch(tree_tc_kernel<HD>, dim3(blocks), dim3(kTtThreads), (size_t)ta.lay.total, s, mq, mk, mv, ta);
+  if (ta.cluster) {
+    launch_clusters(pdl_mode() == 1, (unsigned)ta.cluster, tree_tc_kernel<HD, true>, dim3(ta.cluster * ta.t.kv_heads * ta.tiles * ta.t.n_seqs), dim3(kTtThreads), (size_t)ta.lay.total, s, mq, mk, mv, ta);
+    return check_launch("attention_tree (tensor cores, clusters)");
+  }
+  launch(tree_tc_kernel<HD, false>, dim3(blocks), dim3(kTtThreads), (size_t)ta.lay.total, s, mq, mk, mv, ta);
   const int rc = check_launch("attention_tree (tensor cores)");
   if (rc) return rc;
-  launch_prefetching(tree_tc_join_kernel<HD>, dim3((ta.lay.rows * (HD / 4) + 255) / 256, ta.t.kv_heads * ta.tiles, ta.t.n_seqs), dim3(256), 0, s, ta);
+  launch_prefetching(tree_tc_join_kernel<HD>, dim3((ta.lay.rows * (HD / 4) + 63) / 64, ta.t.kv_heads * ta.tiles, ta.t.n_seqs), dim3(256), 0, s, ta);
   return check_launch("attention_tree (tensor cores, joined)");
 }
 
@@ -746,14 +850,17 @@ int tree_tc(const TreeArgs& a, long long pool_pages, int* status, cudaStream_t s
   int rc = encode_tree_pool(&mk, a.k_pool, pool_pages * a.kv_heads * 64, a.head_dim, "the key pool");
   if (rc == 0) rc = encode_tree_pool(&mv, a.v_pool, pool_pages * a.kv_heads * 64, a.head_dim, "the value pool");
   if (rc) return rc;
-  const TtScratch f = tt_scratch(a.n_seqs, a.max_count, a.heads, a.kv_heads, a.head_dim, a.max_keys);
+  const TtScratch f = tt_scratch(a.n_seqs, a.max_count, a.heads, a.kv_heads, a.head_dim, a.max_keys, a.window);
   SLB_REQUIRE((long long)a.kv_heads * f.tiles < 65536, "attention_tree: too many heads for one launch");
   TtArgs ta{};
   ta.t = a;
   ta.scale_log2 = a.scale * 1.4426950408889634f;
-  ta.part = a.scratch + f.part;
-  ta.part_ml = reinterpret_cast<float2*>(a.scratch + f.part_ml);
-  ta.info = reinterpret_cast<int2*>(a.scratch + f.info);
+  if (!f.cluster) {
+    ta.part = a.scratch + f.part;
+    ta.part_ml = reinterpret_cast<float2*>(a.scratch + f.part_ml);
+    ta.info = reinterpret_cast<int2*>(a.scratch + f.info);
+  }
+  ta.cluster = f.cluster;
   ta.status = status;
   ta.tiles = f.tiles;
   ta.lay = tt_layout(a.head_dim, (int)std::min((long long)a.max_count * (a.heads / a.kv_heads), (long long)kTtTile));
