@@ -66,7 +66,7 @@ struct TtArgs {
   float scale_log2;
   float* part;          // [blocks][2][HD][rows] weighted values
   float2* part_ml;      // [blocks][2][rows] maximum (log2 units) and sum
-  int2* info;           // [n, kv_heads, tiles] first block and number of blocks
+  int2* info;           // [blocks] the (sequence, kv head, tile) whose first pages this block has and whose last ones it has not, and the blocks that share it (0: none)
   int* status;
   int cluster;          // blocks that share a (sequence, kv head, tile), or 0: runs of all units
   int tiles;            // most tiles of a sequence
@@ -170,6 +170,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (lane < 12) (&s_odd[0][0][0])[lane] = 0u;
     if (lane < 2) s_lo[lane] = 0;
+    if (!CLUSTER && lane == 0) ta.info[blockIdx.x] = make_int2(0, 0);
   }
   if (warp == 2) {
     __syncwarp();
@@ -580,9 +581,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       if (live) ml[(g * 2 + half) * kTtRows + r] = make_float4(m_used, l, poisoned ? 1.0f : 0.0f, 0.0f);
       look_sync(true);
       const bool begins = w.off == 0, complete = begins && n == w.s.pages;
-      if (!CLUSTER && begins && stid == 0)
-        ta.info[((long long)w.seq * a.kv_heads + w.kh) * ta.tiles + w.tile] =
-            make_int2((int)blockIdx.x, complete ? 1 : TtShare(total, min((int)gridDim.x, total)).block_of(w.first + w.s.pages - 1) - (int)blockIdx.x + 1);
+      if (!CLUSTER && begins && !complete && stid == 0)
+        ta.info[blockIdx.x] = make_int2((w.seq * a.kv_heads + w.kh) * ta.tiles + w.tile,
+                                        TtShare(total, min((int)gridDim.x, total)).block_of(w.first + w.s.pages - 1) - (int)blockIdx.x + 1);
       const bool mine_here = items(g) > 0, other_here = !dual && items(g ^ 1) > 0;
       if (warp_live) {
         if (mine_here) wait_done(g);
@@ -712,64 +713,75 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   }
 }
 
-// Joins the shares of what no block finished alone: a thread a row and four channels of a quarter of the shares, four of them on the way at once.
+// Joins the shares of what no block finished alone, of each block of the kernel before at most one (sequence, kv head, tile): the blocks make a list of them and go over its pieces of
+// 256 (row, four channels), a thread each, eight shares on the way at once.
+constexpr int kTtMostBlocks = 256;
 template <int HD>
-__global__ void __launch_bounds__(256) tree_tc_join_kernel(TtArgs ta) {
+__global__ void __launch_bounds__(256) tree_tc_join_kernel(TtArgs ta, int blocks) {
   const TreeArgs& a = ta.t;
-  const int rows_pad = ta.lay.rows, seq = blockIdx.z, kh = blockIdx.y / ta.tiles, tile = blockIdx.y % ta.tiles, G = a.heads / a.kv_heads;
-  const TreeSeq s(a, seq);      // (in front of the wait: what the kernel before this one has waited for is there)
-  const int rows = min(kTtTile, s.count * G - tile * kTtTile);
-  if (rows <= 0) return;
+  __shared__ int2 info_s[kTtMostBlocks];
+  __shared__ int block_s[kTtMostBlocks], warp_s[8];
+  const int rows_pad = ta.lay.rows, G = a.heads / a.kv_heads, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, chunks = rows_pad * (HD / 4) / 256;
   pdl_wait();
-  const int2 in = ta.info[((size_t)seq * a.kv_heads + kh) * ta.tiles + tile];
-  if (in.y == 1) return;      // its block has finished it
-  __shared__ float4 acc_s[3][64];
-  __shared__ float2 ml_s[3][64];
-  const int lane = threadIdx.x & 63, part = threadIdx.x >> 6;
-  const int e = blockIdx.x * 64 + lane, r = e % rows_pad, c0 = e / rows_pad * 4;
-  const bool live = r < rows && c0 < HD;
-  auto slot_of = [&](int i) { return (size_t)(in.x + i) * 2 + (i == 0 ? 1 : 0); };
-  const int per = (in.y + 3) / 4, i1 = min(in.y, (part + 1) * per);
-  float M = -INFINITY, l = 0.0f;
-  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  auto join = [&](float2 ml, float4 v) {
-    if (ml.y == 0.0f) return;      // (a share that saw nothing; one whose scores were all NaN has a sum of NaN)
-    const float top = fmaxf(M, ml.x), use = top == -INFINITY ? 0.0f : top, keep = tt_ex2(M - use), f = tt_ex2(ml.x - use);
-    l = l * keep + ml.y * f;
-    acc.x = acc.x * keep + v.x * f;
-    acc.y = acc.y * keep + v.y * f;
-    acc.z = acc.z * keep + v.z * f;
-    acc.w = acc.w * keep + v.w * f;
-    M = top;
-  };
-  if (live)
-    for (int i0 = part * per; i0 < i1; i0 += 4) {
-      float2 ml[4];
-      float4 v[4];
+  const int2 mine = tid < blocks ? ta.info[tid] : make_int2(0, 0);
+  const uint32_t has = __ballot_sync(0xffffffffu, mine.y > 1);
+  if (lane == 0) warp_s[warp] = __popc(has);
+  __syncthreads();
+  int before = 0, found = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const size_t slot = slot_of(min(i0 + i, i1 - 1));
-        ml[i] = ta.part_ml[slot * rows_pad + r];
-        const float* p = ta.part + (slot * HD + c0) * rows_pad + r;
-        v[i] = make_float4(p[0], p[rows_pad], p[2 * rows_pad], p[3 * rows_pad]);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (i0 + i < i1) join(ml[i], v[i]);
-    }
-  if (part > 0) {
-    acc_s[part - 1][lane] = acc;
-    ml_s[part - 1][lane] = make_float2(M, l);
+  for (int w = 0; w < 8; ++w) {
+    before += w < warp ? warp_s[w] : 0;
+    found += warp_s[w];
+  }
+  if (mine.y > 1) {
+    const int at = before + __popc(has & ((1u << lane) - 1u));
+    info_s[at] = mine;
+    block_s[at] = tid;
   }
   __syncthreads();
-  if (part > 0 || !live) return;
+  for (int task = blockIdx.x; task < found * chunks; task += gridDim.x) {
+    const int2 in = info_s[task / chunks];
+    const int first = block_s[task / chunks], tile = in.x % ta.tiles, kh = in.x / ta.tiles % a.kv_heads, seq = in.x / ta.tiles / a.kv_heads;
+    const TreeSeq s(a, seq);
+    const int rows = min(kTtTile, s.count * G - tile * kTtTile), e = task % chunks * 256 + tid, r = e % rows_pad, c0 = e / rows_pad * 4;
+    if (r >= rows) continue;
+    auto slot_of = [&](int i) { return (size_t)(first + i) * 2 + (i == 0 ? 1 : 0); };
+    float M = -INFINITY, l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i0 = 0; i0 < in.y; i0 += 8) {
+      float2 ml[8];
+      float v[8][4];
 #pragma unroll
-  for (int i = 0; i < 3; ++i) join(ml_s[i][lane], acc_s[i][lane]);
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * inv, acc.y * inv), hi = __floats2bfloat162_rn(acc.z * inv, acc.w * inv);
-  const int R = tile * kTtTile + r;
-  *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + ((size_t)(s.tok0 + R / G) * a.heads + kh * G + R % G) * HD + c0) =
-      make_uint2(*reinterpret_cast<uint32_t*>(&lo), *reinterpret_cast<uint32_t*>(&hi));
+      for (int i = 0; i < 8; ++i) {
+        ml[i] = make_float2(-INFINITY, 0.0f);
+        if (i0 + i >= in.y) continue;
+        const size_t slot = slot_of(i0 + i);
+        ml[i] = ta.part_ml[slot * rows_pad + r];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[i][c] = ta.part[(slot * HD + c0 + c) * rows_pad + r];
+      }
+      float top = M;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = fmaxf(top, ml[i].x);
+      const float use = top == -INFINITY ? 0.0f : top, keep = tt_ex2(M - use);
+      l *= keep;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[c] *= keep;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i0 + i >= in.y || ml[i].y == 0.0f) continue;      // (a share that saw nothing; one whose scores were all NaN has a sum of NaN)
+        const float f = tt_ex2(ml[i].x - use);
+        l += ml[i].y * f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[c] += v[i][c] * f;
+      }
+      M = top;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    __nv_bfloat162 lo = __floats2bfloat162_rn(acc[0] * inv, acc[1] * inv), hi = __floats2bfloat162_rn(acc[2] * inv, acc[3] * inv);
+    const int R = tile * kTtTile + r;
+    *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + ((size_t)(s.tok0 + R / G) * a.heads + kh * G + R % G) * HD + c0) =
+        make_uint2(*reinterpret_cast<uint32_t*>(&lo), *reinterpret_cast<uint32_t*>(&hi));
+  }
 }
 
 bool tree_tc_takes(int n_seqs, int max_count, int heads, int kv_heads, int head_dim, int max_keys, int dtype) {
@@ -798,14 +810,14 @@ static TtScratch tt_scratch(int n_seqs, int max_count, int heads, int kv_heads, 
   f.tiles = (int)((rows + kTtTile - 1) / kTtTile);
   f.cluster = tt_cluster(n_seqs, kv_heads, f.tiles, max_count, max_keys, window);
   if (f.cluster) return f;
-  const long long units = (long long)n_seqs * kv_heads * f.tiles * (((long long)max_keys + 63) / 64 + 1), most = sm_count();
+  const long long units = (long long)n_seqs * kv_heads * f.tiles * (((long long)max_keys + 63) / 64 + 1), most = std::min(sm_count(), kTtMostBlocks);
   f.blocks = (int)std::min(units, most);      // one an SM
   const int rows_pad = tt_layout(head_dim, (int)std::min(rows, (long long)kTtTile)).rows;
   long long at = 0;
   auto take = [&](long long n) { const long long o = at; at += (n + 3) & ~3ll; return o; };
   f.part = take(2ll * f.blocks * rows_pad * head_dim);
   f.part_ml = take(4ll * f.blocks * rows_pad);
-  f.info = take(2ll * n_seqs * kv_heads * f.tiles);
+  f.info = take(2ll * f.blocks);
   f.total = at;
   return f;
 }
@@ -837,7 +849,8 @@ static int launch_tree_tc(const CUtensorMap& mq, const CUtensorMap& mk, const CU
   launch(tree_tc_kernel<HD, false>, dim3(blocks), dim3(kTtThreads), (size_t)ta.lay.total, s, mq, mk, mv, ta);
   const int rc = check_launch("attention_tree (tensor cores)");
   if (rc) return rc;
-  launch_prefetching(tree_tc_join_kernel<HD>, dim3((ta.lay.rows * (HD / 4) + 63) / 64, ta.t.kv_heads * ta.tiles, ta.t.n_seqs), dim3(256), 0, s, ta);
+  if (blocks == 1) return 0;
+  launch_prefetching(tree_tc_join_kernel<HD>, dim3(std::min(4 * blocks, blocks * (ta.lay.rows * (HD / 4) / 256))), dim3(256), 0, s, ta, blocks);
   return check_launch("attention_tree (tensor cores, joined)");
 }
 
