@@ -9,10 +9,13 @@
 // drawn from what p has become: the first token, in the order of their numbers, where the running sum passes u of the whole. Temperature 0: the child that is
 // the row's first largest logit, and in the end that token.
 //
-// A cluster of eight blocks walks a sequence's way, an eighth of a row each, a run of it a warp, so that only rows on the way are read. Results are whole numbers and have to be
-// the definition's: what decides about a child (Z, p) comes from 32-bit powers summed in 64 bits, off by some 1e-8, which is the chance that a random number falls
-// between; but a draw compares one number with 150,000 running sums, so sums for draws and refusals are of 64-bit powers of two (a table of 32 and five
-// terms of the series, off by 3e-15).
+// Two kernels: the first leaves the largest logit and the sum Z of every node that has children, the whole GPU over all of them; the second walks the sequences' ways,
+// a cluster of up to sixteen blocks each, a run of the row a warp, and reads whole rows only where a draft is refused or the next token is drawn. (Where the rows of all nodes would be too much
+// to read, kMostStatsBytes, the second finds Z by itself, row by row.) Results are whole numbers and have to be the definition's: what decides about a child (Z, p) comes from
+// 32-bit powers summed in 64 bits, off by some 1e-8, which is the chance that a random number falls between; but a draw compares one number with 150,000 running sums, so sums
+// for draws and refusals are of powers in pairs of 32-bit numbers, off by some 1e-12 (a table of 64 and four terms of the series; in 64 bits, of which an SM does 16 operations a clock, a pass over a row
+// took 7.5 us in eight blocks, four fifths of them waiting for that unit). A refusal takes one pass: the sums of exp, and of exp and of q over the tokens where exp / Z > c q as far as 32 bits tell, make
+// both the exact Z and F (a token on the wrong side is off by 1e-7 of itself, and one in a million is).
 #include <float.h>
 #include <math.h>
 
@@ -21,7 +24,15 @@
 
 namespace slb {
 
-constexpr int kVerifyTeam = 8, kVerifyThreads = 512, kVerifyWarps = kVerifyThreads / 32, kVerifyRuns = kVerifyTeam * kVerifyWarps;
+constexpr int kVerifyTeam = 16, kVerifyThreads = 512, kVerifyWarps = kVerifyThreads / 32, kVerifyRuns = kVerifyTeam * kVerifyWarps;
+constexpr long long kMostStatsBytes = 512ll << 20;
+
+// Of a piece of a row of logits: the largest kept one, its first place, and the sum of exp((l - top) / T).
+struct VerifyStat {
+  float top;
+  int best;
+  double z;
+};
 
 // What a caller says, in one piece of memory (as KeptCall, kept.cuh).
 struct VerifyCall {
@@ -40,13 +51,15 @@ struct VerifyArgs {
   const int *tokens, *parents, *seq_start, *counts;
   int *path, *lengths, *chosen;
   long long rows, ld, ldp;
-  double scale;               // log2 e / T; 0: the largest logit alone counts
+  double scale, unscale;      // log2 e / T, and one over it; 0: the largest logit alone counts
   float scale_hi, scale_lo;
+  VerifyStat* stats;          // [rows, pieces], or null
   int limit, max_count, path_width, run, vec;      // run: tokens of a warp, a multiple of 4
+  int team, pieces, steps;    // blocks of a sequence; pieces of a row in the first kernel, and their steps
 };
 
 struct VerifyExchange {
-  double sum[2][kVerifyWarps];      // two copies, used in turn: a block may write its next share while a slower one still reads the last
+  double sum[2][3][kVerifyWarps];      // two copies, used in turn: a block may write its next share while a slower one still reads the last
   double z[2];
   float max[2];
   int best[2];
@@ -54,13 +67,16 @@ struct VerifyExchange {
 
 struct VerifyShared {
   VerifyExchange x;
-  double table[32];                 // 2^(j / 32)
+  float2 table[64];                 // 2^(j / 64), in two parts
   double runs[kVerifyRuns];         // sums before and with each run
   double red_z[kVerifyWarps];
   double scan[kVerifyWarps];
   float red_m[kVerifyWarps];
   int red_i[kVerifyWarps];
+  VerifyStat stat[kMostNodes];
+  int inner[kMostNodes];            // whether a node has children
   int parent[kMostNodes], token[kMostNodes], refused[kMostNodes];
+  double p[kMostNodes];
   float logit[kMostNodes], prob[kMostNodes], u[kMostNodes];
   double total_z;
   float top;
@@ -83,19 +99,239 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
   return v;
 }
 
-// 2^y for y <= 0: y = n + j / 32 + r with |r| <= 1 / 64, and 2^r from the series of exp(r ln 2), whose sixth power is below 3e-15.
-__device__ __forceinline__ double pow2_f64(double y, const double* table) {
-  if (!(y > -1000.0)) return y == y ? 0.0 : y;
-  const double t = y * 32.0 + 6755399441055744.0;      // 1.5 * 2^52: the nearest whole number in the low bits
-  const int k = __double2loint(t);
-  const double x = (y - (t - 6755399441055744.0) * 0.03125) * 0.6931471805599453;
-  double p = fma(x, 1.0 / 120.0, 1.0 / 24.0);
-  p = fma(x, p, 1.0 / 6.0);
-  p = fma(x, p, 0.5);
-  p = fma(x, p, 1.0);
-  p = fma(x, p, 1.0);
-  p *= table[k & 31];
-  return __hiloint2double(__double2hiint(p) + ((k >> 5) << 20), __double2loint(p));      // (p is in [0.98, 2), k >> 5 >= -1000: no underflow)
+// A sum of numbers from 0 to 1 in two parts: each addition's error is kept. It begins at 4 so that no number is larger than the sum.
+struct PairSum {
+  float hi = 4.0f, lo = 0.0f;
+  __device__ __forceinline__ void add(float x, float rest) {
+    const float t = hi + x;
+    lo += (x - (t - hi)) + rest;
+    hi = t;
+  }
+  __device__ __forceinline__ double value() const { return ((double)hi - 4.0) + (double)lo; }
+};
+
+// 2^y scaled so that the row's largest logit has between 1/2 and 1, y = l * log2 e / T in two parts (the product's error is an FMA away): y = m + j / 64 + r with |r| <= 1 / 128, 2^r = 1 + a + b with
+// a = r ln 2 rounded and b its error and the series' other terms up to the fourth, 2^(j / 64) from the table in two parts. Off by 1e-12 or less. Logits are counted from `base`: 0, or the
+// largest where its y is beyond 1,000 (all that counts then lies so near that the difference is exact).
+struct PairPower {
+  float scale_hi, scale_lo, base, cap, least;      // below `least` nothing counts; from `base` no logit lies further up than `cap`
+  int bias;                                   // what makes a power of two of the whole part
+  bool none;                                  // nothing counts
+  __device__ __forceinline__ PairPower() {}
+  __device__ __forceinline__ PairPower(const VerifyArgs& a, float top, float floor) {
+    const double y = (double)top * a.scale;
+    scale_hi = a.scale_hi;
+    scale_lo = a.scale_lo;
+    const bool near = fabs(y) <= 1000.0;
+    base = near ? 0.0f : top;
+    cap = near ? FLT_MAX : 0.0f;
+    bias = (127 - (near ? (int)ceil(y) : 0)) << 23;
+    none = floor != floor || !(top > -INFINITY);
+    least = top < INFINITY ? fmaxf(floor, (float)(top - 120.0 * a.unscale)) : INFINITY;
+  }
+  __device__ __forceinline__ float2 of(float l, const float2* table) const {
+    constexpr double kLn2 = 0.6931471805599453;
+    constexpr float kHi = (float)kLn2, kLo = (float)(kLn2 - (double)kHi);
+    const bool counts = l >= least && !none;
+    const float x = fminf(fmaxf(l, least) - base, cap);      // (inf - inf, beside an infinite logit, is no number and becomes `cap`: 0)
+    const float p = __fmul_rn(x, scale_hi), e = fmaf(x, scale_lo, fmaf(x, scale_hi, -p));
+    const float t = fmaf(p, 64.0f, 12582912.0f);      // 1.5 * 2^23: the nearest whole number in the low bits
+    const uint32_t bits = __float_as_uint(t);
+    const float r = fmaf(t - 12582912.0f, -0.015625f, p), r1 = r + e;
+    const float a = __fmul_rn(r, kHi);
+    float g = fmaf(r1, (float)(kLn2 * kLn2 * kLn2 * kLn2 / 24.0), (float)(kLn2 * kLn2 * kLn2 / 6.0));
+    g = fmaf(r1, g, (float)(kLn2 * kLn2 / 2.0));
+    const float b = fmaf(r1 * r1, g, fmaf(e, kHi, fmaf(r, kLo, fmaf(r, kHi, -a))));
+    const float2 f = table[bits & 63u];
+    const float h = __fmul_rn(f.x, a);                // (products that are also parts: never joined with a sum)
+    float lo = fmaf(f.x, b, fmaf(f.x, a, -h)) + fmaf(f.y, a, f.y);
+    const float s = f.x + h;
+    lo += h - (s - f.x);
+    const float two = counts ? __uint_as_float(((bits & ~63u) << 17) + (uint32_t)bias) : 0.0f;      // (from 2^-122 on; the magic number's own bits leave at the top)
+    return make_float2(s * two, lo * two);
+  }
+};
+
+// f(token, logit, q) for tokens lo .. hi - 1 of a row of logits and, if there is one, a row of q (else 0), by the lanes of a warp; `vec`: 16-byte reads, lo a multiple of 4. The next
+// eight tokens of a lane are on their way while f works on four: loops that fetch their instructions once (unrolled twice as far every pass waited for instructions more than for anything else).
+template <bool PAIR, typename F>
+__device__ __forceinline__ void each_logit(const float* row, const float* other, int lo, int hi, int lane, bool vec, F f) {
+  if (vec) {
+    const int last = hi - 4;      // the last place of a whole 16-byte read
+    int i = lo + 4 * lane;
+    float4 v[2], q[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (i + 128 * k <= last) {
+        v[k] = *reinterpret_cast<const float4*>(row + i + 128 * k);
+        if (PAIR) q[k] = *reinterpret_cast<const float4*>(other + i + 128 * k);
+      }
+#pragma unroll 1
+    for (; i <= last; i += 128) {
+      const float4 x = v[0], y = PAIR ? q[0] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      v[0] = v[1];
+      if (PAIR) q[0] = q[1];
+      if (i + 256 <= last) {
+        v[1] = *reinterpret_cast<const float4*>(row + i + 256);
+        if (PAIR) q[1] = *reinterpret_cast<const float4*>(other + i + 256);
+      }
+      f(i, x.x, y.x);
+      f(i + 1, x.y, y.y);
+      f(i + 2, x.z, y.z);
+      f(i + 3, x.w, y.w);
+    }
+    // what is left of four
+    const int tail = lo + ((hi - lo) & ~3) + lane;
+    if (hi > lo && tail < hi) f(tail, row[tail], PAIR ? other[tail] : 0.0f);
+  } else {
+    int i = lo + lane;
+#pragma unroll 1
+    for (; i + 3 * 32 < hi; i += 4 * 32) {
+      float v[4], q[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v[k] = row[i + 32 * k];
+        q[k] = PAIR ? other[i + 32 * k] : 0.0f;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) f(i + 32 * k, v[k], q[k]);
+    }
+#pragma unroll 1
+    for (; i < hi; i += 32) f(i, row[i], PAIR ? other[i] : 0.0f);
+  }
+}
+
+// exp((l - m) / T) from the 32-bit unit, l <= m
+__device__ __forceinline__ float rough_exp(const VerifyArgs& a, float l, float m) {
+  const float x = l - m, t = x * a.scale_hi;
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaf(x, a.scale_hi, x * a.scale_lo)));
+  return l == m ? 1.0f : t > -1e4f ? y : 0.0f;      // (infinities end here)
+}
+
+__device__ __forceinline__ float ex2_f32(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// What counts as a logit of row t: at or above its floor; -inf has no probability, nor has NaN.
+__device__ __forceinline__ float floor_of(const VerifyArgs& a, size_t t) {
+  if (a.floors == nullptr) return -FLT_MAX;
+  const float f = a.floors[t];
+  return f != f ? f : fmaxf(f, -FLT_MAX);
+}
+
+constexpr int kStatsThreads = 256, kStatsStep = 4096;      // tokens that a block holds at once, the next ones on their way
+// A piece of the row of a node that has children: `steps` steps. A thread's sum is relative to its own largest logit, in units of log2 after the temperature.
+__global__ void __launch_bounds__(kStatsThreads) verify_stats_kernel(VerifyArgs a) {
+  pdl_enter();
+  __shared__ float top_s[kStatsThreads / 32];
+  __shared__ int best_s[kStatsThreads / 32];
+  __shared__ double z_s[kStatsThreads / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, seq = blockIdx.y, node = blockIdx.z;
+  const int tok0 = a.seq_start[seq], count = min(max(a.counts[seq], 0), a.max_count);
+  if (node >= count || tok0 < 0 || (long long)tok0 + count > a.rows) return;
+  bool child = false;
+  for (int j = node + 1 + tid; j < count; j += kStatsThreads) child = child || a.parents[tok0 + j] == node;
+  if (!__syncthreads_or(child)) return;
+  const size_t t = (size_t)tok0 + node;
+  const float* row = a.logits + t * a.ld;
+  const float floor = floor_of(a, t);
+  const long long piece = (long long)a.steps * kStatsStep;
+  const int begin = (int)min((long long)a.limit, blockIdx.x * piece), end = (int)min((long long)a.limit, begin + piece);
+  constexpr int PER = kStatsStep / kStatsThreads;
+  // (vec: thread tid has tokens at + 4 tid + 1024 k .. + 3, else at + tid + 256 k)
+  auto token = [&](int at, int k) { return a.vec ? at + 4 * tid + 4 * kStatsThreads * (k >> 2) + (k & 3) : at + tid + kStatsThreads * k; };
+  auto load = [&](int at, float (&v)[PER]) {
+    if (a.vec) {
+#pragma unroll
+      for (int k = 0; k < PER; k += 4) {
+        const int i = at + 4 * tid + kStatsThreads * k;
+        if (i + 3 < end) {
+          const float4 x = *reinterpret_cast<const float4*>(row + i);
+          v[k] = x.x; v[k + 1] = x.y; v[k + 2] = x.z; v[k + 3] = x.w;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[k + e] = i + e < end ? row[i + e] : -INFINITY;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < PER; ++k) v[k] = token(at, k) < end ? row[token(at, k)] : -INFINITY;
+    }
+  };
+  const bool greedy = a.scale == 0.0;
+  float top = -INFINITY, v[PER];
+  int best = 0x7fffffff;
+  double z = 0.0;
+  load(begin, v);
+#pragma unroll 1
+  for (int at = begin; at < end; at += kStatsStep) {
+    float next[PER];
+    if (at + kStatsStep < end) load(at + kStatsStep, next);
+    if (greedy) {
+#pragma unroll
+      for (int k = 0; k < PER; ++k)
+        if (token(at, k) < end && (v[k] > top || (v[k] == top && token(at, k) < best))) { top = v[k]; best = token(at, k); }
+    } else {
+      float high = top;
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        v[k] = v[k] >= floor ? v[k] : -INFINITY;
+        high = fmaxf(high, v[k]);
+      }
+      if (high > top) {
+        z = top > -INFINITY ? z * rough_exp(a, top, high) : 0.0;
+        top = high;
+      }
+      float part = 0.0f;
+      const float ref = top * a.scale_hi;
+      if (fabsf(ref) < 4096.0f) {      // (its rounding is then nothing beside 1)
+        const float shift = ex2_f32(fmaf(top, a.scale_hi, fmaf(top, a.scale_lo, -ref)));      // (the largest logit's own power: near 1)
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+          const float y = ex2_f32(fmaf(v[k], a.scale_hi, fmaf(v[k], a.scale_lo, -ref)));
+          part += v[k] > -INFINITY ? y : 0.0f;
+        }
+        part /= shift;
+      } else if (top > -INFINITY) {      // (infinite, the type's lowest value, almost no temperature)
+#pragma unroll 1
+        for (int k = 0; k < PER; ++k) {
+          float x = v[0];
+#pragma unroll
+          for (int e = 1; e < PER; ++e) x = e == k ? v[e] : x;
+          part += x > -INFINITY ? rough_exp(a, x, top) : 0.0f;
+        }
+      }
+      z += part;
+    }
+#pragma unroll
+    for (int k = 0; k < PER; ++k) v[k] = next[k];
+  }
+  if (greedy) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const float x = __shfl_xor_sync(0xffffffffu, top, o);
+      const int i = __shfl_xor_sync(0xffffffffu, best, o);
+      if (x > top || (x == top && i < best)) { top = x; best = i; }
+    }
+  } else {
+    const float all = warp_max(top);
+    z = top > -INFINITY ? z * rough_exp(a, top, all) : 0.0;
+    top = all;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+  }
+  if (lane == 0) { top_s[warp] = top; best_s[warp] = best; z_s[warp] = z; }
+  __syncthreads();
+  if (tid != 0) return;
+  VerifyStat out{-INFINITY, 0x7fffffff, 0.0};
+  for (int w = 0; w < kStatsThreads / 32; ++w)
+    if (top_s[w] > out.top || (top_s[w] == out.top && best_s[w] < out.best)) { out.top = top_s[w]; out.best = best_s[w]; }
+  for (int w = 0; w < kStatsThreads / 32; ++w)
+    if (top_s[w] > -INFINITY) out.z += z_s[w] * rough_exp(a, top_s[w], out.top);
+  a.stats[t * a.pieces + blockIdx.x] = out;
 }
 
 struct Verifier {
@@ -106,6 +342,9 @@ struct Verifier {
   const float* row = nullptr;       // logits of the node reached
   const float* probs = nullptr;     // what its children were drawn from
   float floor = -FLT_MAX, top = 0.0f;
+  PairPower power;
+  double inv_e = 0.0;               // one over the row's sum of powers, where sums() has formed it
+  int node_at = 0;
 
   __device__ Verifier(const VerifyArgs& a_, VerifyShared& s_) : a(a_), s(s_), tid(threadIdx.x), lane(threadIdx.x & 31), warp(threadIdx.x >> 5), rank((int)cluster_ctarank()) {}
 
@@ -114,52 +353,45 @@ struct Verifier {
 
   __device__ void at_node(int seq_row, int node) {
     const size_t t = (size_t)seq_row + node;
+    node_at = node;
     row = a.logits + t * a.ld;
     probs = a.probs ? a.probs + t * a.ldp : nullptr;
-    floor = -FLT_MAX;             // -inf has no probability, nor has NaN
-    if (a.floors) {
-      const float f = a.floors[t];
-      floor = f != f ? f : fmaxf(f, -FLT_MAX);
-    }
+    floor = floor_of(a, t);
   }
   __device__ __forceinline__ bool kept(float l) const { return l >= floor; }
 
-  // f(token, logit) for this warp's run, four tokens of a lane at a time where rows are aligned
   template <typename F>
   __device__ __forceinline__ void each(F f) const {
-    const int lo = begin(rank, warp), hi = begin(rank, warp + 1);
-    if (a.vec) {
-      int i = lo + 4 * lane;
-      for (; i + 3 * 128 + 3 < hi; i += 4 * 128) {
-        float4 v[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const float4*>(row + i + 128 * k);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          f(i + 128 * k, v[k].x);
-          f(i + 128 * k + 1, v[k].y);
-          f(i + 128 * k + 2, v[k].z);
-          f(i + 128 * k + 3, v[k].w);
-        }
+    each_logit<false>(row, nullptr, begin(rank, warp), begin(rank, warp + 1), lane, a.vec, [&](int i, float l, float) { f(i, l); });
+  }
+
+  // which nodes have children, and the first kernel's findings of those, a warp a node
+  __device__ void find(int tok0, int count) {
+    for (int node = warp; node < count; node += kVerifyWarps) {
+      bool child = false;
+      for (int j = node + 1 + lane; j < count; j += 32) child = child || s.parent[j] == node;
+      const bool inner = __any_sync(0xffffffffu, child);
+      if (lane == 0) s.inner[node] = inner ? 1 : 0;
+      if (!inner || a.stats == nullptr) continue;
+      VerifyStat mine{-INFINITY, 0x7fffffff, 0.0};
+      for (int i = lane; i < a.pieces; i += 32) {
+        const VerifyStat x = a.stats[(size_t)(tok0 + node) * a.pieces + i];
+        const float top = fmaxf(mine.top, x.top);
+        if (x.top > mine.top || (x.top == mine.top && x.best < mine.best)) mine.best = x.best;
+        if (top > -INFINITY)
+          mine.z = (mine.top > -INFINITY ? mine.z * rough_exp(a, mine.top, top) : 0.0) + (x.top > -INFINITY ? x.z * rough_exp(a, x.top, top) : 0.0);
+        mine.top = top;
       }
-      for (; i < hi; i += 128)
-        for (int k = 0; k < 4; ++k)
-          if (i + k < hi) f(i + k, row[i + k]);
-    } else {
-      int i = lo + lane;
-      for (; i + 3 * 32 < hi; i += 4 * 32) {
-        float v[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = row[i + 32 * k];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) f(i + 32 * k, v[k]);
-      }
-      for (; i < hi; i += 32) f(i, row[i]);
+      const float top = warp_max(mine.top);
+      const double z = warp_sum_f64(mine.top > -INFINITY ? mine.z * rough_exp(a, mine.top, top) : 0.0);
+      const int best = __reduce_min_sync(0xffffffffu, mine.top == top ? mine.best : 0x7fffffff);
+      if (lane == 0) s.stat[node] = VerifyStat{top, best == 0x7fffffff ? 0 : best, z};
     }
   }
 
   // first largest logit of the row (0 where there is none), the same in all blocks
-  __device__ int argmax() {
+  __device__ int argmax(bool have) {
+    if (have) return s.stat[node_at].best;
     float bv = -INFINITY;
     int bi = 0x7fffffff;
     each([&](int i, float l) {
@@ -182,7 +414,7 @@ struct Verifier {
     if (tid == 0) {
       bv = -INFINITY;
       bi = 0x7fffffff;
-      for (int r = 0; r < kVerifyTeam; ++r) better(peer_f32(peer(&s.x.max[flip], r)), __float_as_int(peer_f32(peer(&s.x.best[flip], r))));
+      for (int r = 0; r < a.team; ++r) better(peer_f32(peer(&s.x.max[flip], r)), __float_as_int(peer_f32(peer(&s.x.best[flip], r))));
       s.best = bi == 0x7fffffff ? 0 : bi;
     }
     __syncthreads();
@@ -190,11 +422,10 @@ struct Verifier {
     return s.best;
   }
 
-  __device__ __forceinline__ float rough(float l, float m) const {      // exp((l - m) / T), l <= m
-    const float x = l - m, t = x * a.scale_hi;
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaf(x, a.scale_hi, x * a.scale_lo)));
-    return l == m ? 1.0f : t > -1e4f ? y : 0.0f;      // (infinities end here)
+  __device__ __forceinline__ float rough(float l, float m) const { return rough_exp(a, l, m); }
+  __device__ __forceinline__ void set_top(float m) {
+    top = m;
+    power = PairPower(a, m, floor);
   }
 
   // largest kept logit (into `top`) and the sum Z of exp((l - top) / T)
@@ -222,41 +453,78 @@ struct Verifier {
     __syncthreads();
     cluster_sync_all();
     if (warp == 0) {
-      const float mr = lane < kVerifyTeam ? peer_f32(peer(&s.x.max[flip], lane)) : -INFINITY, mc = warp_max(mr);
-      const double zr = lane < kVerifyTeam && mr > -INFINITY ? peer_f64(peer(&s.x.z[flip], lane)) * rough(mr, mc) : 0.0, zc = warp_sum_f64(zr);
+      const float mr = lane < a.team ? peer_f32(peer(&s.x.max[flip], lane)) : -INFINITY, mc = warp_max(mr);
+      const double zr = lane < a.team && mr > -INFINITY ? peer_f64(peer(&s.x.z[flip], lane)) * rough(mr, mc) : 0.0, zc = warp_sum_f64(zr);
       if (lane == 0) { s.top = mc; s.total_z = zc; }
     }
     __syncthreads();
     flip ^= 1;
-    top = s.top;
-    return s.total_z;
+    set_top(s.top);
+    const double all = s.total_z;
+    __syncthreads();
+    return all;
   }
 
-  __device__ __forceinline__ double fine(float l) const {      // exp((l - top) / T) in 64 bits
-    return !kept(l) ? 0.0 : l == top ? 1.0 : pow2_f64(((double)l - (double)top) * a.scale, s.table);
+  __device__ __forceinline__ double fine(float l) const {      // the power in 64 bits
+    const float2 x = power.of(l, s.table);
+    return (double)x.x + (double)x.y;
   }
-  __device__ __forceinline__ double rest(double e, double inv_z, double c, int i) const { return fmax(fma(e, inv_z, -c * (double)probs[i]), 0.0); }
 
-  // sums over the runs: of exp (inv_z 0) or of max(exp * inv_z - c q, 0), without the refused tokens of certain drafts; s.runs: sums up to and with each run
-  __device__ double sums(double inv_z, double c, int n_refused) {
-    double w = 0.0;
-    if (inv_z == 0.0) each([&](int, float l) { w += fine(l); });
-    else each([&](int i, float l) { w += rest(fine(l), inv_z, c, i); });
-    w = warp_sum_f64(w);
+  // Sums over the runs, into s.runs up to and with each run; returns the last. Without `pair` of the powers, less those of the refused tokens of certain drafts; with it of
+  // max(p - c q, 0), `cz` being c times the rough Z in the unit of the powers.
+  __device__ double sums(bool pair, double c, float cz, int n_refused) {
     const int lo = begin(rank, warp), hi = begin(rank, warp + 1);
+    PairSum all, over, drawn;
+    if (!pair) {
+      each_logit<false>(row, nullptr, lo, hi, lane, a.vec, [&](int, float l, float) {
+        const float2 x = power.of(l, s.table);
+        all.add(x.x, x.y);
+      });
+    } else {
+      each_logit<true>(row, probs, lo, hi, lane, a.vec, [&](int, float l, float q) {
+        const float2 x = power.of(l, s.table);
+        all.add(x.x, x.y);
+        const bool more = x.x > cz * q;
+        over.add(more ? x.x : 0.0f, more ? x.y : 0.0f);
+        drawn.add(more ? q : 0.0f, 0.0f);
+      });
+    }
+    double w = warp_sum_f64(all.value());
+    const double wo = pair ? warp_sum_f64(over.value()) : 0.0, wq = pair ? warp_sum_f64(drawn.value()) : 0.0;
     for (int r = 0; r < n_refused; ++r) {
       const int x = s.refused[r];
       if (x >= lo && x < hi) w -= fine(row[x]);
     }
-    if (lane == 0) s.x.sum[flip][warp] = fmax(w, 0.0);
+    if (lane == 0) {
+      s.x.sum[flip][0][warp] = fmax(w, 0.0);
+      s.x.sum[flip][1][warp] = wo;
+      s.x.sum[flip][2][warp] = wq;
+    }
     __syncthreads();
     cluster_sync_all();
     if (warp == 0) {
-      double v[4], before = 0.0;
+      constexpr int N = kVerifyRuns / 32;
+      double v[N], vo[N], vq[N], before = 0.0;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int g = lane * 4 + k;
-        v[k] = peer_f64(peer(&s.x.sum[flip][g % kVerifyWarps], g / kVerifyWarps));
+      for (int k = 0; k < N; ++k) {
+        const int g = lane * N + k, r = g / kVerifyWarps, i = g % kVerifyWarps;
+        const bool here = r < a.team;
+        v[k] = here ? peer_f64(peer(&s.x.sum[flip][0][i], r)) : 0.0;
+        vo[k] = here && pair ? peer_f64(peer(&s.x.sum[flip][1][i], r)) : 0.0;
+        vq[k] = here && pair ? peer_f64(peer(&s.x.sum[flip][2][i], r)) : 0.0;
+      }
+      if (pair) {
+        double e = 0.0;
+#pragma unroll
+        for (int k = 0; k < N; ++k) e += v[k];
+        e = warp_sum_f64(e);
+        const double inv = e > 0.0 ? 1.0 / e : 0.0;
+        if (lane == 0) s.total_z = inv;
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = fmax(vo[k] * inv - c * vq[k], 0.0);
+      }
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
         before += v[k];
         v[k] = before;
       }
@@ -268,15 +536,16 @@ struct Verifier {
       }
       const double off = __shfl_up_sync(0xffffffffu, incl, 1);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) s.runs[lane * 4 + k] = (lane ? off : 0.0) + v[k];
+      for (int k = 0; k < N; ++k) s.runs[lane * N + k] = (lane ? off : 0.0) + v[k];
     }
     __syncthreads();
     flip ^= 1;
+    if (pair) inv_e = s.total_z;
     return s.runs[kVerifyRuns - 1];
   }
 
   // the token where the running sum passes `target`; in the block that has its run, else -1
-  __device__ int draw(double target, double inv_z, double c, int n_refused) {
+  __device__ int draw(double target, bool pair, double c, int n_refused) {
     int first = kVerifyRuns, last = -1;      // the first run whose sum passes it, else the last that adds something
 #pragma unroll
     for (int k = kVerifyRuns / 32 - 1; k >= 0; --k) {
@@ -294,7 +563,7 @@ struct Verifier {
     const int lo = begin(rank, g % kVerifyWarps), hi = begin(rank, g % kVerifyWarps + 1);
     auto weight = [&](int i) {
       const double e = fine(row[i]);
-      if (inv_z != 0.0) return rest(e, inv_z, c, i);
+      if (pair) return fmax(e * inv_e - c * (double)probs[i], 0.0);
       for (int r = 0; r < n_refused; ++r)
         if (s.refused[r] == i) return 0.0;
       return e;
@@ -327,11 +596,11 @@ struct Verifier {
   }
 };
 
-__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(VerifyArgs a) {
+__global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(VerifyArgs a) {
   pdl_enter();
   __shared__ VerifyShared s;
   Verifier v(a, s);
-  const int tid = threadIdx.x, seq = blockIdx.x / kVerifyTeam;
+  const int tid = threadIdx.x, seq = blockIdx.x / a.team;
   const int tok0 = a.seq_start[seq];
   int count = min(max(a.counts[seq], 0), a.max_count);
   if (tok0 < 0 || (long long)tok0 + count > a.rows) count = 0;      // (never read behind the given rows)
@@ -343,7 +612,10 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(VerifyArgs a) {
     return;
   }
   const bool greedy = a.scale == 0.0;
-  if (tid < 32) s.table[tid] = exp2(tid * 0.03125);
+  if (tid < 64) {
+    const double x = exp2(tid * 0.015625);
+    s.table[tid] = make_float2((float)x, (float)(x - (double)(float)x));
+  }
   if (tid < count) {
     const int p = a.parents[tok0 + tid], x = a.tokens[tok0 + tid];
     const bool child = p >= 0 && p < tid, inside = x >= 0 && x < a.limit;
@@ -357,69 +629,87 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(VerifyArgs a) {
     for (int i = tid; i < a.path_width; i += kVerifyThreads)
       if (i > 0) a.path[(size_t)seq * a.path_width + i] = -1;
   __syncthreads();
+  v.find(tok0, count);
+  __syncthreads();
+  // the children's probabilities at their parents, where the first kernel has been over those
+  auto child_p = [&](int j, const PairPower& power, float top, double z) {
+    if (s.token[j] < 0 || !(z > 0.0)) return 0.0;
+    const float2 x = power.of(s.logit[j], s.table), one = power.of(top, s.table);
+    return ((double)x.x + (double)x.y) / (((double)one.x + (double)one.y) * z);
+  };
+  if (a.stats && !greedy && tid < count && s.parent[tid] >= 0) {
+    const VerifyStat& x = s.stat[s.parent[tid]];
+    s.p[tid] = child_p(tid, PairPower(a, x.top, floor_of(a, (size_t)tok0 + s.parent[tid])), x.top, x.z);
+  }
+  __syncthreads();
   int node = 0, length = 1, n_refused = 0, best = 0;
-  double inv_z = 0.0, c = 0.0, total = -1.0;      // inv_z, c: of what s.runs holds the sums; total < 0: not formed yet
+  double c = 0.0, total = -1.0;      // c: of what s.runs holds the sums; total < 0: not formed yet
+  bool pair = false;
   while (true) {
     v.at_node(tok0, node);
     int taken = -1;
     n_refused = 0;
-    inv_z = c = 0.0;
+    c = 0.0;
     total = -1.0;
+    pair = false;
+    const bool inner = s.inner[node] != 0, have = inner && a.stats != nullptr;
     if (greedy) {
-      best = v.argmax();
+      best = v.argmax(have);
       for (int j = node + 1; j < count && taken < 0; ++j)
         if (s.parent[j] == node && s.token[j] == best) taken = j;
     } else {
-      const double z = v.denominator();
+      double z = have ? s.stat[node].z : 0.0;
+      bool set = false;      // v's powers are the node's
+      if (!have) {
+        z = v.denominator();
+        set = true;
+        if (inner) {
+          if (tid > node && tid < count && s.parent[tid] == node) s.p[tid] = child_p(tid, v.power, v.top, z);
+          __syncthreads();
+        }
+      }
       double f = 1.0, gone = 0.0;
-      for (int j = node + 1; j < count; ++j) {
+      for (int j = inner ? node + 1 : count; j < count; ++j) {
         if (s.parent[j] != node) continue;
-        const double p = s.token[j] >= 0 && z > 0.0 ? v.fine(s.logit[j]) / z : 0.0, u = s.u[j];
-        if (a.probs ? p > (c + u * f) * (double)s.prob[j] : p > u * (1.0 - gone)) {
-          bool again = false;      // a certain draft that was refused before has no probability left
-          for (int r = 0; r < n_refused; ++r) again = again || s.refused[r] == s.token[j];
-          if (!again) {
-            taken = j;
-            break;
-          }
+        const double p = s.p[j], u = s.u[j];
+        bool again = false;      // a certain draft that was refused before has no probability left
+        for (int r = 0; r < n_refused; ++r) again = again || s.refused[r] == s.token[j];
+        if (!again && (a.probs ? p > (c + u * f) * (double)s.prob[j] : p > u * (1.0 - gone))) {
+          taken = j;
+          break;
         }
         if (a.probs) {
-          if (inv_z == 0.0) {
-            const double fine_z = v.sums(0.0, 0.0, 0);
-            if (!(fine_z > 0.0)) break;      // a row without probabilities: nothing to refuse
-            inv_z = 1.0 / fine_z;
-          }
+          if (!(z > 0.0)) continue;      // a row without probabilities: nothing to refuse
           c += f;
-          f = total = v.sums(inv_z, c, 0);
-        } else if (s.token[j] >= 0) {
-          bool again = false;
-          for (int r = 0; r < n_refused; ++r) again = again || s.refused[r] == s.token[j];
-          if (!again) {
-            __syncthreads();
-            if (tid == 0) s.refused[n_refused] = s.token[j];
-            ++n_refused;
-            gone += p;
-            __syncthreads();
-          }
+          if (!set) v.set_top(s.stat[node].top);
+          set = pair = true;
+          f = total = v.sums(true, c, (float)(c * z * v.fine(v.top)), 0);
+        } else if (s.token[j] >= 0 && !again) {
+          __syncthreads();
+          if (tid == 0) s.refused[n_refused] = s.token[j];
+          ++n_refused;
+          gone += p;
+          __syncthreads();
         }
       }
     }
-    if (taken < 0) break;
+    if (taken < 0) {
+      if (!greedy && have && !pair) v.set_top(s.stat[node].top);
+      break;
+    }
     node = taken;
     if (writer && length < a.path_width) a.path[(size_t)seq * a.path_width + length] = node;
     ++length;
+    __syncthreads();      // (s.p is written anew)
   }
   if (!greedy) {
-    if (total < 0.0) {
-      inv_z = 0.0;
-      total = v.sums(0.0, 0.0, n_refused);
-    }
+    if (total < 0.0) total = v.sums(false, 0.0, 0.0f, n_refused);
     if (!(total > 0.0)) {      // refusals that had no probability have left nothing: all of p again
-      inv_z = 0.0;
+      pair = false;
       n_refused = 0;
-      total = v.sums(0.0, 0.0, 0);
+      total = v.sums(false, 0.0, 0.0f, 0);
     }
-    const int x = v.draw((double)s.u[0] * total, inv_z, c, n_refused);
+    const int x = v.draw((double)s.u[0] * total, pair, c, n_refused);
     if (x >= 0 && tid == 0) a.chosen[seq] = x;
   }
   if (writer) {
@@ -432,7 +722,19 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(VerifyArgs a) {
 }
 
 // 32-bit words of scratch that slb_verify_drafts takes.
-extern "C" long long slb_verify_drafts_scratch(int n_seqs, long long rows, int limit, int drawn) { return 0; }
+// Pieces of a row in the first kernel: small ones where the rows are few, else as many blocks as run at once twice over.
+static int stats_steps(long long rows, int limit) {
+  const long long steps = ((long long)limit + kStatsStep - 1) / kStatsStep, pieces = 1184 / rows + 1;
+  return (int)(pieces >= steps ? 1 : (steps + pieces - 1) / pieces);
+}
+static int stats_pieces(long long rows, int limit) {
+  const long long piece = (long long)stats_steps(rows, limit) * kStatsStep;
+  return (int)((limit + piece - 1) / piece);
+}
+static bool stats_first(long long rows, int limit) { return rows * limit * 4 <= kMostStatsBytes; }
+extern "C" long long slb_verify_drafts_scratch(int n_seqs, long long rows, int limit, int drawn) {
+  return n_seqs > 0 && n_seqs < 65536 && rows > 0 && limit > 0 && stats_first(rows, limit) ? rows * stats_pieces(rows, limit) * (long long)(sizeof(VerifyStat) / 4) : 0;
+}
 
 extern "C" int slb_verify_drafts(const VerifyCall* call) {
   SLB_REQUIRE(call != nullptr, "verify_drafts: no call");
@@ -449,13 +751,55 @@ extern "C" int slb_verify_drafts(const VerifyCall* call) {
   a.counts = c.counts; a.path = c.path; a.lengths = c.lengths; a.chosen = c.chosen; a.rows = c.rows; a.ld = c.ld; a.ldp = c.ldp;
   a.limit = c.limit; a.max_count = c.max_count; a.path_width = c.path_width;
   if (c.temperature > 0.0) {
-    a.scale = 1.4426950408889634 / c.temperature;
-    a.scale_hi = a.scale < 1e30 ? (float)a.scale : 1e30f;      // (colder than that only the largest logit is left either way)
-    a.scale_lo = a.scale < 1e30 ? (float)(a.scale - (double)a.scale_hi) : 0.0f;
+    a.scale = fmin(1.4426950408889634 / c.temperature, 1e30);      // (colder than that only the largest logit is left either way)
+    a.unscale = 1.0 / a.scale;
+    a.scale_hi = (float)a.scale;
+    a.scale_lo = (float)(a.scale - (double)a.scale_hi);
   }
-  a.run = (int)((((long long)c.limit + kVerifyRuns - 1) / kVerifyRuns + 3) / 4 * 4);
-  a.vec = (uintptr_t)c.logits % 16 == 0 && c.ld % 4 == 0;
-  launch_clusters(pdl_mode() == 1, kVerifyTeam, verify_kernel, dim3(c.n_seqs * kVerifyTeam), dim3(kVerifyThreads), 0, (cudaStream_t)c.stream, a);
+  const long long need = slb_verify_drafts_scratch(c.n_seqs, c.rows, c.limit, c.probs != nullptr);
+  SLB_REQUIRE(need == 0 || (c.scratch != nullptr && c.scratch_words >= need), "verify_drafts: the call needs %lld words of scratch, %lld were given", need,
+              c.scratch ? c.scratch_words : 0ll);
+  SLB_REQUIRE((uintptr_t)c.scratch % 16 == 0, "verify_drafts: scratch must be 16-byte aligned");
+  a.team = kVerifyTeam;      // all blocks at once, one an SM or, of up to eight a sequence, two
+  while (a.team > 1 && (long long)c.n_seqs * a.team > (a.team > 8 ? 1ll : 2ll) * sm_count()) a.team /= 2;
+  if (a.team > 8) {      // clusters of sixteen are to be allowed, and lie within one of the GPU's partitions
+    static std::atomic<unsigned long long> asked, works;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const unsigned long long bit = dev >= 0 && dev < 64 ? 1ull << dev : 0ull;
+    if (!(asked.load(std::memory_order_acquire) & bit)) {
+      int clusters = 0;
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(kVerifyTeam);
+      cfg.blockDim = dim3(kVerifyThreads);
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = kVerifyTeam;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      const bool good = cudaFuncSetAttribute((const void*)verify_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                        cudaOccupancyMaxActiveClusters(&clusters, verify_kernel, &cfg) == cudaSuccess && clusters > 0;
+      if (!good) cudaGetLastError();
+      if (good) works.fetch_or(bit, std::memory_order_release);
+      asked.fetch_or(bit, std::memory_order_release);
+    }
+    if (!(works.load(std::memory_order_acquire) & bit)) a.team = 8;
+  }
+  const int runs = a.team * kVerifyWarps;
+  a.run = (int)((((long long)c.limit + runs - 1) / runs + 3) / 4 * 4);
+  a.vec = (uintptr_t)c.logits % 16 == 0 && c.ld % 4 == 0 && (c.probs == nullptr || ((uintptr_t)c.probs % 16 == 0 && c.ldp % 4 == 0));
+  if (need > 0) {
+    a.steps = stats_steps(c.rows, c.limit);
+    a.pieces = stats_pieces(c.rows, c.limit);
+  }
+  if (need > 0) {
+    a.stats = reinterpret_cast<VerifyStat*>(c.scratch);
+    launch(verify_stats_kernel, dim3(a.pieces, c.n_seqs, c.max_count), dim3(kStatsThreads), 0, (cudaStream_t)c.stream, a);
+    const int rc = check_launch("verify_drafts (sums)");
+    if (rc) return rc;
+  }
+  launch_clusters(need > 0 ? pdl_mode() != 0 : pdl_mode() == 1, a.team, verify_kernel, dim3(c.n_seqs * a.team), dim3(kVerifyThreads), 0, (cudaStream_t)c.stream, a);
   return check_launch("verify_drafts");
 }
 

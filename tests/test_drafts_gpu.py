@@ -390,6 +390,26 @@ def test_verification_of_odd_logits(temperature):
     assert int(lengths[0]) >= 2 and int(chosen[1]) == 0 and int(lengths[2]) == 4 and int(lengths[3]) == 1
 
 
+@pytest.mark.parametrize("temperature", [0.0, 0.7])
+@pytest.mark.parametrize("drawn", [True, False])
+def test_verification_of_masked_rows(temperature, drawn):
+    """Rows most of whose tokens carry the type's lowest value, one of them all; a floor above every logit leaves nothing."""
+    j = Judged([5, 5, 3, 4], "random", 20000, 20000, temperature, drawn, seed=11)
+    lowest = torch.finfo(torch.float32).min
+    allowed = torch.zeros(20000, dtype=torch.bool)
+    allowed[torch.randperm(20000, generator=torch.Generator().manual_seed(3))[:40]] = True
+    allowed[j.tokens[1:3].long()] = True
+    j.logits[:5, ~allowed] = lowest
+    j.logits[5:10, 12000:] = lowest
+    j.logits[10:13] = lowest
+    if temperature:
+        j.floors = torch.full((17,), -50.0)
+        j.floors[10:13] = -math.inf
+        j.floors[13:] = 1e9
+    path, lengths, chosen = j.check()
+    assert bool(allowed[int(chosen[0])]) and (not temperature or (int(lengths[3]) == 1 and int(chosen[3]) == 0))
+
+
 def test_verification_streams_graphs_widths():
     j = Judged([6, 3, 9], "random", 2000, 2000, 0.9, True, seed=10)
     first = j.check()
