@@ -24,7 +24,7 @@
 
 namespace slb {
 
-constexpr int kVerifyTeam = 16, kVerifyThreads = 512, kVerifyWarps = kVerifyThreads / 32, kVerifyRuns = kVerifyTeam * kVerifyWarps;
+constexpr int kVerifyTeam = 16, kVerifyThreads = 1024, kVerifyWarps = kVerifyThreads / 32, kVerifyRuns = kVerifyTeam * kVerifyWarps;
 constexpr long long kMostStatsBytes = 512ll << 20;
 
 // Of a piece of a row of logits: the largest kept one, its first place, and the sum of exp((l - top) / T).
@@ -68,7 +68,7 @@ struct VerifyExchange {
 struct VerifyShared {
   VerifyExchange x;
   float2 table[64];                 // 2^(j / 64), in two parts
-  double runs[kVerifyRuns];         // sums before and with each run
+  double runs[kVerifyRuns];         // sums up to and with each run
   double red_z[kVerifyWarps];
   double scan[kVerifyWarps];
   float red_m[kVerifyWarps];
@@ -159,9 +159,10 @@ __device__ __forceinline__ void each_logit(const float* row, const float* other,
   if (vec) {
     const int last = hi - 4;      // the last place of a whole 16-byte read
     int i = lo + 4 * lane;
-    float4 v[2], q[2];
+    constexpr int AHEAD = 2;
+    float4 v[AHEAD], q[AHEAD];
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int k = 0; k < AHEAD; ++k)
       if (i + 128 * k <= last) {
         v[k] = *reinterpret_cast<const float4*>(row + i + 128 * k);
         if (PAIR) q[k] = *reinterpret_cast<const float4*>(other + i + 128 * k);
@@ -169,11 +170,14 @@ __device__ __forceinline__ void each_logit(const float* row, const float* other,
 #pragma unroll 1
     for (; i <= last; i += 128) {
       const float4 x = v[0], y = PAIR ? q[0] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      v[0] = v[1];
-      if (PAIR) q[0] = q[1];
-      if (i + 256 <= last) {
-        v[1] = *reinterpret_cast<const float4*>(row + i + 256);
-        if (PAIR) q[1] = *reinterpret_cast<const float4*>(other + i + 256);
+#pragma unroll
+      for (int k = 0; k + 1 < AHEAD; ++k) {
+        v[k] = v[k + 1];
+        if (PAIR) q[k] = q[k + 1];
+      }
+      if (i + 128 * AHEAD <= last) {
+        v[AHEAD - 1] = *reinterpret_cast<const float4*>(row + i + 128 * AHEAD);
+        if (PAIR) q[AHEAD - 1] = *reinterpret_cast<const float4*>(other + i + 128 * AHEAD);
       }
       f(i, x.x, y.x);
       f(i + 1, x.y, y.y);
@@ -428,8 +432,8 @@ struct Verifier {
     power = PairPower(a, m, floor);
   }
 
-  // largest kept logit (into `top`) and the sum Z of exp((l - top) / T)
-  __device__ double denominator() {
+  // largest kept logit (into `top`) and, unless that is all, the sum Z of exp((l - top) / T)
+  __device__ double denominator(bool top_alone) {
     float m = -INFINITY;
     each([&](int, float l) {
       if (kept(l)) m = fmaxf(m, l);
@@ -438,10 +442,11 @@ struct Verifier {
     double z = 0.0;
     float part = 0.0f;
     int n = 0;
-    each([&](int, float l) {
-      if (kept(l)) part += rough(l, m);
-      if ((++n & 15) == 0) { z += part; part = 0.0f; }
-    });
+    if (!top_alone)
+      each([&](int, float l) {
+        if (kept(l)) part += rough(l, m);
+        if ((++n & 15) == 0) { z += part; part = 0.0f; }
+      });
     z = warp_sum_f64(z + part);
     if (lane == 0) { s.red_m[warp] = m; s.red_z[warp] = z; }
     __syncthreads();
@@ -502,58 +507,59 @@ struct Verifier {
     }
     __syncthreads();
     cluster_sync_all();
-    if (warp == 0) {
-      constexpr int N = kVerifyRuns / 32;
-      double v[N], vo[N], vq[N], before = 0.0;
-#pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const int g = lane * N + k, r = g / kVerifyWarps, i = g % kVerifyWarps;
-        const bool here = r < a.team;
-        v[k] = here ? peer_f64(peer(&s.x.sum[flip][0][i], r)) : 0.0;
-        vo[k] = here && pair ? peer_f64(peer(&s.x.sum[flip][1][i], r)) : 0.0;
-        vq[k] = here && pair ? peer_f64(peer(&s.x.sum[flip][2][i], r)) : 0.0;
-      }
+    // a thread a run
+    static_assert(kVerifyRuns <= kVerifyThreads && kVerifyWarps == 32, "a thread a run, a warp a block's runs");
+    const int runs = a.team * kVerifyWarps;
+    double own = 0.0, own_over = 0.0, own_drawn = 0.0, inv = 0.0;
+    if (warp < a.team) {
+      own = peer_f64(peer(&s.x.sum[flip][0][lane], warp));
       if (pair) {
-        double e = 0.0;
-#pragma unroll
-        for (int k = 0; k < N; ++k) e += v[k];
-        e = warp_sum_f64(e);
-        const double inv = e > 0.0 ? 1.0 / e : 0.0;
-        if (lane == 0) s.total_z = inv;
-#pragma unroll
-        for (int k = 0; k < N; ++k) v[k] = fmax(vo[k] * inv - c * vq[k], 0.0);
+        own_over = peer_f64(peer(&s.x.sum[flip][1][lane], warp));
+        own_drawn = peer_f64(peer(&s.x.sum[flip][2][lane], warp));
+        const double e = warp_sum_f64(own);
+        if (lane == 0) s.red_z[warp] = e;
       }
-#pragma unroll
-      for (int k = 0; k < N; ++k) {
-        before += v[k];
-        v[k] = before;
+    }
+    if (pair) {
+      __syncthreads();
+      if (warp == 0) {
+        const double e = warp_sum_f64(lane < a.team ? s.red_z[lane] : 0.0);
+        if (lane == 0) s.total_z = e > 0.0 ? 1.0 / e : 0.0;
       }
-      double incl = before;
+      __syncthreads();
+      inv = s.total_z;
+      own = fmax(own_over * inv - c * own_drawn, 0.0);
+    }
+    if (warp < a.team) {
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
-        const double y = __shfl_up_sync(0xffffffffu, incl, d);
-        if (lane >= d) incl += y;
+        const double y = __shfl_up_sync(0xffffffffu, own, d);
+        if (lane >= d) own += y;
       }
-      const double off = __shfl_up_sync(0xffffffffu, incl, 1);
-#pragma unroll
-      for (int k = 0; k < N; ++k) s.runs[lane * N + k] = (lane ? off : 0.0) + v[k];
+      if (lane == 31) s.scan[warp] = own;
+    }
+    __syncthreads();
+    if (warp < a.team) {
+      double off = 0.0;
+      for (int w = 0; w < warp; ++w) off += s.scan[w];
+      s.runs[tid] = off + own;
     }
     __syncthreads();
     flip ^= 1;
-    if (pair) inv_e = s.total_z;
-    return s.runs[kVerifyRuns - 1];
+    if (pair) inv_e = inv;
+    return s.runs[runs - 1];
   }
 
   // the token where the running sum passes `target`; in the block that has its run, else -1
   __device__ int draw(double target, bool pair, double c, int n_refused) {
+    const int runs = a.team * kVerifyWarps;
     int first = kVerifyRuns, last = -1;      // the first run whose sum passes it, else the last that adds something
-#pragma unroll
-    for (int k = kVerifyRuns / 32 - 1; k >= 0; --k) {
-      const int i = 32 * k + lane;
+    for (int i0 = runs - 32; i0 >= 0; i0 -= 32) {
+      const int i = i0 + lane;
       const bool adds = s.runs[i] > (i ? s.runs[i - 1] : 0.0);
       const uint32_t hits = __ballot_sync(0xffffffffu, adds && s.runs[i] > target), any = __ballot_sync(0xffffffffu, adds);
-      if (hits) first = 32 * k + __ffs(hits) - 1;
-      if (any && last < 0) last = 32 * k + 31 - __clz(any);
+      if (hits) first = i0 + __ffs(hits) - 1;
+      if (any && last < 0) last = i0 + 31 - __clz(any);
     }
     const int g = first < kVerifyRuns ? first : max(last, 0);
     double at = g ? s.runs[g - 1] : 0.0;
@@ -596,7 +602,7 @@ struct Verifier {
   }
 };
 
-__global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(VerifyArgs a) {
+__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(VerifyArgs a) {
   pdl_enter();
   __shared__ VerifyShared s;
   Verifier v(a, s);
@@ -661,7 +667,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(VerifyArgs a)
       double z = have ? s.stat[node].z : 0.0;
       bool set = false;      // v's powers are the node's
       if (!have) {
-        z = v.denominator();
+        z = v.denominator(!inner);
         set = true;
         if (inner) {
           if (tid > node && tid < count && s.parent[tid] == node) s.p[tid] = child_p(tid, v.power, v.top, z);
@@ -724,7 +730,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_kernel(VerifyArgs a)
 // 32-bit words of scratch that slb_verify_drafts takes.
 // Pieces of a row in the first kernel: small ones where the rows are few, else as many blocks as run at once twice over.
 static int stats_steps(long long rows, int limit) {
-  const long long steps = ((long long)limit + kStatsStep - 1) / kStatsStep, pieces = 1184 / rows + 1;
+  const long long steps = ((long long)limit + kStatsStep - 1) / kStatsStep, pieces = 2368 / rows + 1;
   return (int)(pieces >= steps ? 1 : (steps + pieces - 1) / pieces);
 }
 static int stats_pieces(long long rows, int limit) {
@@ -734,6 +740,32 @@ static int stats_pieces(long long rows, int limit) {
 static bool stats_first(long long rows, int limit) { return rows * limit * 4 <= kMostStatsBytes; }
 extern "C" long long slb_verify_drafts_scratch(int n_seqs, long long rows, int limit, int drawn) {
   return n_seqs > 0 && n_seqs < 65536 && rows > 0 && limit > 0 && stats_first(rows, limit) ? rows * stats_pieces(rows, limit) * (long long)(sizeof(VerifyStat) / 4) : 0;
+}
+
+// How many clusters of sixteen blocks, an SM each, run at once on the current device: such clusters are to be allowed, and lie within one of the GPU's partitions.
+static int wide_clusters() {
+  static std::atomic<int> known[64];      // one more than the number; 0: not asked yet
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  int n = known[dev].load(std::memory_order_acquire);
+  if (n > 0) return n - 1;
+  int clusters = 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(kVerifyTeam);
+  cfg.blockDim = dim3(kVerifyThreads);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kVerifyTeam;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaFuncSetAttribute((const void*)verify_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&clusters, verify_kernel, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    clusters = 0;
+  }
+  known[dev].store(clusters + 1, std::memory_order_release);
+  return clusters;
 }
 
 extern "C" int slb_verify_drafts(const VerifyCall* call) {
@@ -760,32 +792,10 @@ extern "C" int slb_verify_drafts(const VerifyCall* call) {
   SLB_REQUIRE(need == 0 || (c.scratch != nullptr && c.scratch_words >= need), "verify_drafts: the call needs %lld words of scratch, %lld were given", need,
               c.scratch ? c.scratch_words : 0ll);
   SLB_REQUIRE((uintptr_t)c.scratch % 16 == 0, "verify_drafts: scratch must be 16-byte aligned");
-  a.team = kVerifyTeam;      // all blocks at once, one an SM or, of up to eight a sequence, two
-  while (a.team > 1 && (long long)c.n_seqs * a.team > (a.team > 8 ? 1ll : 2ll) * sm_count()) a.team /= 2;
-  if (a.team > 8) {      // clusters of sixteen are to be allowed, and lie within one of the GPU's partitions
-    static std::atomic<unsigned long long> asked, works;
-    int dev = 0;
-    cudaGetDevice(&dev);
-    const unsigned long long bit = dev >= 0 && dev < 64 ? 1ull << dev : 0ull;
-    if (!(asked.load(std::memory_order_acquire) & bit)) {
-      int clusters = 0;
-      cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3(kVerifyTeam);
-      cfg.blockDim = dim3(kVerifyThreads);
-      cudaLaunchAttribute attr[1];
-      attr[0].id = cudaLaunchAttributeClusterDimension;
-      attr[0].val.clusterDim.x = kVerifyTeam;
-      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-      cfg.attrs = attr;
-      cfg.numAttrs = 1;
-      const bool good = cudaFuncSetAttribute((const void*)verify_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
-                        cudaOccupancyMaxActiveClusters(&clusters, verify_kernel, &cfg) == cudaSuccess && clusters > 0;
-      if (!good) cudaGetLastError();
-      if (good) works.fetch_or(bit, std::memory_order_release);
-      asked.fetch_or(bit, std::memory_order_release);
-    }
-    if (!(works.load(std::memory_order_acquire) & bit)) a.team = 8;
-  }
+  a.team = kVerifyTeam;      // as many as give every block an SM of its own
+  while (a.team > 1 && (long long)c.n_seqs * a.team > sm_count()) a.team /= 2;
+  if (a.team > 8 && c.n_seqs > wide_clusters()) a.team = 8;
+  if (a.team == 8 && c.n_seqs > 16) a.team = 4;      // (a cluster lies within one of the GPU's partitions: eighteen of eight may not run at once)
   const int runs = a.team * kVerifyWarps;
   a.run = (int)((((long long)c.limit + runs - 1) / runs + 3) / 4 * 4);
   a.vec = (uintptr_t)c.logits % 16 == 0 && c.ld % 4 == 0 && (c.probs == nullptr || ((uintptr_t)c.probs % 16 == 0 && c.ldp % 4 == 0));
