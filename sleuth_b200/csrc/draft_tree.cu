@@ -70,14 +70,28 @@ __global__ void __launch_bounds__(kMostNodes) draft_tree_kernel(DraftTreeArgs a)
   a.positions[token] = a.past[seq] + depth;
 }
 
-extern "C" int slb_draft_tree(const int* parents, const int* seq_start, const int* past, const int* counts, void* seen, int* positions, long long tokens,
-                              int n_seqs, int max_count, int words, int window, void* stream) {
+// What a caller says, in one piece of memory (as KeptCall, kept.cuh).
+struct DraftTreeCall {
+  const int *parents, *seq_start, *past, *counts;
+  void* seen;
+  int* positions;
+  void* stream;
+  long long tokens;
+  int n_seqs, max_count, words, window;
+};
+static_assert(sizeof(DraftTreeCall) == 7 * 8 + 8 + 4 * 4, "as packed in kernels/ops.py");
+
+extern "C" int slb_draft_tree(const DraftTreeCall* call) {
+  SLB_REQUIRE(call != nullptr, "draft_tree: no call");
+  const DraftTreeCall c = *call;
+  const int n_seqs = c.n_seqs, max_count = c.max_count, words = c.words, window = c.window;
+  const long long tokens = c.tokens;
   SLB_REQUIRE(n_seqs >= 0 && tokens >= 0 && window >= 0, "draft_tree: n_seqs=%d tokens=%lld window=%d", n_seqs, tokens, window);
   SLB_REQUIRE(max_count > 0 && max_count <= kMostNodes, "draft_tree: %d nodes of a sequence; 1 to %d are taken", max_count, kMostNodes);
   SLB_REQUIRE(words >= 1 && (long long)words * 32 >= max_count, "draft_tree: %d words of bits do not hold %d nodes", words, max_count);
   if (n_seqs == 0 || tokens == 0) return 0;
-  const DraftTreeArgs a{parents, seq_start, past, counts, (uint32_t*)seen, positions, tokens, n_seqs, max_count, words, window};
-  const cudaStream_t s = (cudaStream_t)stream;
+  const DraftTreeArgs a{c.parents, c.seq_start, c.past, c.counts, (uint32_t*)c.seen, c.positions, tokens, n_seqs, max_count, words, window};
+  const cudaStream_t s = (cudaStream_t)c.stream;
   if (max_count <= 32) launch(draft_tree_kernel<1>, dim3(n_seqs), dim3(32), 0, s, a);
   else if (max_count <= 64) launch(draft_tree_kernel<2>, dim3(n_seqs), dim3(64), 0, s, a);
   else if (max_count <= 128) launch(draft_tree_kernel<4>, dim3(n_seqs), dim3(128), 0, s, a);
@@ -143,8 +157,21 @@ __global__ void __launch_bounds__(kCompactThreads) cache_compact_kernel(CompactA
   }
 }
 
-extern "C" int slb_cache_compact(void* k_pool, void* v_pool, const int* block_table, const int* past, const int* path, const int* lengths, long long layers,
-                                 long long v_layers, long long pages, int table_stride, int n_seqs, int kv_heads, int k_row, int v_row, int path_width, void* stream) {
+struct CompactCall {
+  void *k_pool, *v_pool;                 // [layers, pages, kv_heads, 64, k_row]; [v_layers, pages, kv_heads, 64, v_row] or null
+  const int *block_table, *past, *path, *lengths;
+  void* stream;
+  long long layers, v_layers, pages;
+  int table_stride, n_seqs, kv_heads, k_row, v_row, path_width;      // bytes of a row
+};
+static_assert(sizeof(CompactCall) == 7 * 8 + 3 * 8 + 6 * 4, "as packed in kernels/ops.py");
+
+extern "C" int slb_cache_compact(const CompactCall* call) {
+  SLB_REQUIRE(call != nullptr, "cache_compact: no call");
+  const CompactCall c = *call;
+  void *k_pool = c.k_pool, *v_pool = c.v_pool;
+  const long long layers = c.layers, v_layers = c.v_layers, pages = c.pages;
+  const int table_stride = c.table_stride, n_seqs = c.n_seqs, kv_heads = c.kv_heads, k_row = c.k_row, v_row = c.v_row, path_width = c.path_width;
   SLB_REQUIRE(n_seqs >= 0 && n_seqs < 65536 && layers >= 0 && v_layers >= 0 && pages > 0 && table_stride > 0 && kv_heads > 0 && path_width > 0,
               "cache_compact: n_seqs=%d layers=%lld pages=%lld table_stride=%d kv_heads=%d path_width=%d", n_seqs, layers, pages, table_stride, kv_heads, path_width);
   SLB_REQUIRE(path_width <= kMostNodes, "cache_compact: paths of %d nodes; at most %d are taken", path_width, kMostNodes);
@@ -153,7 +180,7 @@ extern "C" int slb_cache_compact(void* k_pool, void* v_pool, const int* block_ta
   SLB_REQUIRE((long long)table_stride * kPageTokens < (1ll << 31) - kMostNodes, "cache_compact: a block table of %d pages is too long", table_stride);
   if (n_seqs == 0 || layers + v_layers == 0) return 0;
   CompactArgs a{};
-  a.k_pool = (char*)k_pool; a.v_pool = (char*)v_pool; a.block_table = block_table; a.past = past; a.path = path; a.lengths = lengths;
+  a.k_pool = (char*)k_pool; a.v_pool = (char*)v_pool; a.block_table = c.block_table; a.past = c.past; a.path = c.path; a.lengths = c.lengths;
   a.table_stride = table_stride; a.kv_heads = kv_heads; a.k_row = k_row; a.v_row = v_row; a.path_width = path_width;
   a.k_layer = pages * kv_heads * kPageTokens * k_row;
   a.v_layer = pages * kv_heads * kPageTokens * v_row;
@@ -163,8 +190,8 @@ extern "C" int slb_cache_compact(void* k_pool, void* v_pool, const int* block_ta
   a.pieces = a.k_pieces + v_layers * kv_heads * (v_row / piece);
   const long long blocks = (a.pieces + kCompactThreads - 1) / kCompactThreads;
   SLB_REQUIRE(blocks < (1ll << 31), "cache_compact: too many layers for one launch");
-  if (wide) launch(cache_compact_kernel<uint4>, dim3((unsigned)blocks, n_seqs), dim3(kCompactThreads), 0, (cudaStream_t)stream, a);
-  else launch(cache_compact_kernel<uint32_t>, dim3((unsigned)blocks, n_seqs), dim3(kCompactThreads), 0, (cudaStream_t)stream, a);
+  if (wide) launch(cache_compact_kernel<uint4>, dim3((unsigned)blocks, n_seqs), dim3(kCompactThreads), 0, (cudaStream_t)c.stream, a);
+  else launch(cache_compact_kernel<uint32_t>, dim3((unsigned)blocks, n_seqs), dim3(kCompactThreads), 0, (cudaStream_t)c.stream, a);
   return check_launch("cache_compact");
 }
 

@@ -204,10 +204,10 @@ _SIGNATURES = {
     "slb_qkv_post_rows": [P, P, P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, F, I, P],
     "slb_attention_kept": [ctypes.c_char_p],
     "slb_cache_evict": [ctypes.c_char_p],
-    "slb_draft_tree": [P, P, P, P, P, P, L, I, I, I, I, P],
+    "slb_draft_tree": [ctypes.c_char_p],
     "slb_attention_tree": [ctypes.c_char_p],
     "slb_verify_drafts": [ctypes.c_char_p],
-    "slb_cache_compact": [P, P, P, P, P, P, L, L, L, I, I, I, I, I, I, P],
+    "slb_cache_compact": [ctypes.c_char_p],
 }
 
 

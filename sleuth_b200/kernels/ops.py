@@ -11,6 +11,7 @@ is (sleuth/forge/model/attention.py:106-108,157; mlp.py:38-41; transformer.py:30
 from __future__ import annotations
 
 import ctypes
+import math
 import os
 import struct
 
@@ -1886,6 +1887,8 @@ def cache_evict(weights, positions, k_pool, v_pool, block_table, past, lengths, 
 MOST_NODES = 256                             # of a sequence in a step (kMostNodes in csrc/tree.cuh)
 _TREE_CALL = struct.Struct("13Q3q10if4x")    # TreeCall in csrc/tree.cuh (to its whole size)
 _VERIFY_CALL = struct.Struct("13Q4qd4i")     # VerifyCall in csrc/verify_drafts.cu
+_DRAFT_TREE_CALL = struct.Struct("7Qq4i")    # DraftTreeCall in csrc/draft_tree.cu
+_COMPACT_CALL = struct.Struct("7Q3q6i")      # CompactCall there
 
 
 def _fits_int(what: str, *values: int) -> None:
@@ -1900,17 +1903,26 @@ def draft_tree(parents, seq_start, past, counts, seen, positions, max_count: int
     before the step. ``seen`` [tokens, words] int32, 32 nodes a word, receives bit b of a node where it sees node b: itself and
     those that it continues, under a ``window`` the last ``window`` of them. ``positions`` [tokens] int32 receives ``past`` plus the number of nodes above."""
     i32 = torch.int32
-    _cuda(parents, seq_start, past, counts, seen, positions)
     n, T = past.numel(), parents.numel()
-    _need(all(t.dtype == i32 for t in (parents, seq_start, past, counts, seen, positions)), "draft_tree: all tensors are int32")
-    _need(seq_start.numel() >= n and counts.numel() == n, "draft_tree: seq_start, past and counts have one row a sequence")
-    _need(seen.dim() == 2 and seen.shape[0] >= T and seen.shape[1] * 32 >= max_count and positions.numel() >= T,
-          "draft_tree: seen is [tokens, words] with a bit for each of max_count nodes, positions is [tokens]")
-    _need(0 < max_count <= MOST_NODES, f"draft_tree: {max_count} nodes of a sequence; 1 to {MOST_NODES} are taken")
-    _need(window >= 0, "draft_tree: the window is not negative")
-    _fits_int("draft_tree", window)
-    lib().call("slb_draft_tree", _p(parents), _p(seq_start), _p(past), _p(counts), _p(seen), _p(positions), T, n, int(max_count), seen.shape[1], int(window),
-               stream if stream is not None else current_stream())
+    _need(seen.dim() == 2, "draft_tree: seen is [tokens, words]")
+    rows, words = seen.shape
+    if not (parents.is_cuda and parents.is_contiguous() and seq_start.is_cuda and seq_start.is_contiguous() and past.is_cuda and past.is_contiguous()
+            and counts.is_cuda and counts.is_contiguous() and seen.is_cuda and seen.is_contiguous() and positions.is_cuda and positions.is_contiguous()
+            and i32 == parents.dtype == seq_start.dtype == past.dtype == counts.dtype == seen.dtype == positions.dtype
+            and seq_start.numel() >= n and counts.numel() == n and rows >= T and positions.numel() >= T and words * 32 >= max_count
+            and 0 < max_count <= MOST_NODES and window >= 0):
+        _kept_refusal("draft_tree", dict(parents=parents, seq_start=seq_start, past=past, counts=counts, seen=seen, positions=positions), (
+            (lambda: i32 == parents.dtype == seq_start.dtype == past.dtype == counts.dtype == seen.dtype == positions.dtype, "all tensors are int32"),
+            (lambda: seq_start.numel() >= n and counts.numel() == n, "seq_start, past and counts have one row a sequence"),
+            (lambda: 0 < max_count <= MOST_NODES, f"{max_count} nodes of a sequence; 1 to {MOST_NODES} are taken"),
+            (lambda: rows >= T and positions.numel() >= T and words * 32 >= max_count, "seen is [tokens, words] with a bit for each of max_count nodes, positions is [tokens]"),
+            (lambda: window >= 0, "the window is not negative")))
+    try:
+        call = _DRAFT_TREE_CALL.pack(parents.data_ptr(), seq_start.data_ptr(), past.data_ptr(), counts.data_ptr(), seen.data_ptr(), positions.data_ptr(),
+                                     stream if stream is not None else current_stream(), T, n, max_count, words, window)
+    except struct.error as e:
+        raise ValueError(f"draft_tree: a number is out of range ({e})") from None
+    lib().call("slb_draft_tree", call)
 
 
 def attention_tree_scratch_floats(tokens: int, n_seqs: int, max_count: int, heads: int, kv_heads: int, head_dim: int, max_keys: int,
@@ -2003,29 +2015,39 @@ def verify_drafts(logits, limit: int, tokens, parents, seq_start, counts, unifor
     Outputs, int32: ``path`` [n, places] the accepted nodes from node 0 on, then -1; ``lengths`` [n] their number (at least 1; 0 for a sequence without nodes); ``chosen``
     [n] the next token (-1 without nodes; 0 where the row has no number above -inf). ``scratch``: ``verify_drafts_scratch_words`` int32 words. Rows may be apart (a stride)."""
     i32, f32 = torch.int32, torch.float32
-    _cuda(tokens, parents, seq_start, counts, uniforms, path, lengths, chosen, floors, scratch)
-    for name, t in (("logits", logits), ("probs", probs)):
-        _need(t is None or t.is_cuda and t.dtype == f32 and t.dim() == 2 and t.stride(1) == 1, f"verify_drafts: {name} are float32 CUDA rows of unit column stride")
-    n, T = counts.numel(), logits.shape[0]
-    _need(0 < limit <= logits.shape[1] and (probs is None or probs.shape[0] >= T and probs.shape[1] >= limit), "verify_drafts: limit tokens of a row of logits and of probs")
-    _need(all(t.dtype == i32 for t in (tokens, parents, seq_start, counts, path, lengths, chosen)), "verify_drafts: tables and outputs are int32")
-    _need(tokens.numel() >= T and parents.numel() >= T, "verify_drafts: tokens and parents have a value for each row of logits")
-    _need(seq_start.numel() >= n and lengths.numel() >= n and chosen.numel() >= n and path.dim() == 2 and path.shape[0] >= n and path.shape[1] >= max_count,
-          "verify_drafts: path is [n, places] for max_count nodes; seq_start, lengths and chosen have one value a sequence")
-    _need(0 < max_count <= MOST_NODES, f"verify_drafts: {max_count} nodes of a sequence; 1 to {MOST_NODES} are taken")
-    temperature = float(temperature)
-    _need(temperature == temperature and temperature < float("inf"), "verify_drafts: the temperature must be a finite number")
-    _need(uniforms is None and temperature <= 0 or uniforms is not None and uniforms.dtype == f32 and uniforms.numel() >= T,
-          "verify_drafts: uniforms are float32, one a node, and needed above temperature 0")
-    _need(floors is None or floors.dtype == f32 and floors.numel() >= T, "verify_drafts: floors are float32, one a node")
-    _need(scratch is None or scratch.dtype == i32, "verify_drafts: scratch is int32")
+    _need(logits.dim() == 2 and path.dim() == 2 and (probs is None or probs.dim() == 2), "verify_drafts: logits, probs and path have two dimensions")
+    n, (T, vocab), places = counts.numel(), logits.shape, path.shape[1]
+    if not (logits.is_cuda and logits.dtype == f32 and logits.stride(1) == 1 and 0 < limit <= vocab
+            and (probs is None or probs.is_cuda and probs.dtype == f32 and probs.stride(1) == 1 and probs.shape[0] >= T and probs.shape[1] >= limit)
+            and tokens.is_cuda and tokens.is_contiguous() and parents.is_cuda and parents.is_contiguous() and seq_start.is_cuda and seq_start.is_contiguous()
+            and counts.is_cuda and counts.is_contiguous() and path.is_cuda and path.is_contiguous() and lengths.is_cuda and lengths.is_contiguous()
+            and chosen.is_cuda and chosen.is_contiguous() and _plain_cuda(uniforms) and _plain_cuda(floors) and _plain_cuda(scratch)
+            and i32 == tokens.dtype == parents.dtype == seq_start.dtype == counts.dtype == path.dtype == lengths.dtype == chosen.dtype
+            and tokens.numel() >= T and parents.numel() >= T and seq_start.numel() >= n and lengths.numel() >= n and chosen.numel() >= n
+            and path.shape[0] >= n and places >= max_count and 0 < max_count <= MOST_NODES and temperature < math.inf
+            and (uniforms.dtype == f32 and uniforms.numel() >= T if uniforms is not None else temperature <= 0)
+            and (floors is None or floors.dtype == f32 and floors.numel() >= T) and (scratch is None or scratch.dtype == i32)):
+        for name, t in (("logits", logits), ("probs", probs)):
+            _need(t is None or t.is_cuda and t.dtype == f32 and t.stride(1) == 1, f"verify_drafts: {name} are float32 CUDA rows of unit column stride")
+        _kept_refusal("verify_drafts", dict(tokens=tokens, parents=parents, seq_start=seq_start, counts=counts, path=path, lengths=lengths, chosen=chosen, uniforms=uniforms,
+                                            floors=floors, scratch=scratch), (
+            (lambda: 0 < limit <= vocab and (probs is None or probs.shape[0] >= T and probs.shape[1] >= limit), "limit tokens of a row of logits and of probs, one row a node"),
+            (lambda: i32 == tokens.dtype == parents.dtype == seq_start.dtype == counts.dtype == path.dtype == lengths.dtype == chosen.dtype, "tables and outputs are int32"),
+            (lambda: tokens.numel() >= T and parents.numel() >= T, "tokens and parents have a value for each row of logits"),
+            (lambda: 0 < max_count <= MOST_NODES, f"{max_count} nodes of a sequence; 1 to {MOST_NODES} are taken"),
+            (lambda: min(seq_start.numel(), lengths.numel(), chosen.numel(), path.shape[0]) >= n and places >= max_count,
+             "path is [n, places] for max_count nodes; seq_start, lengths and chosen have one value a sequence"),
+            (lambda: temperature < math.inf, "the temperature must be a finite number"),
+            (lambda: uniforms.dtype == f32 and uniforms.numel() >= T if uniforms is not None else temperature <= 0, "uniforms are float32, one a node, and needed above temperature 0"),
+            (lambda: floors is None or floors.dtype == f32 and floors.numel() >= T, "floors are float32, one a node"),
+            (lambda: scratch is None or scratch.dtype == i32, "scratch is int32")))
     try:
         call = _VERIFY_CALL.pack(logits.data_ptr(), 0 if probs is None else probs.data_ptr(), 0 if floors is None else floors.data_ptr(),
                                  0 if uniforms is None else uniforms.data_ptr(), tokens.data_ptr(), parents.data_ptr(), seq_start.data_ptr(), counts.data_ptr(),
                                  path.data_ptr(), lengths.data_ptr(), chosen.data_ptr(), 0 if scratch is None else scratch.data_ptr(),
-                                 stream if stream is not None else current_stream(), T, logits.stride(0) if T > 1 else logits.shape[1],
+                                 stream if stream is not None else current_stream(), T, logits.stride(0) if T > 1 else vocab,
                                  0 if probs is None else probs.stride(0) if probs.shape[0] > 1 else probs.shape[1], 0 if scratch is None else scratch.numel(),
-                                 temperature, n, limit, max_count, path.shape[1])
+                                 temperature, n, limit, max_count, places)
     except struct.error as e:
         raise ValueError(f"verify_drafts: a number is out of range ({e})") from None
     lib().call("slb_verify_drafts", call)
@@ -2038,20 +2060,30 @@ def cache_compact(k_pool, block_table, past, path, lengths, v_pool=None, stream=
     above (``verify_drafts`` gives such); it ends in front of the first entry that does not. ``k_pool`` [..., pages, kv_heads, 64, width]: any number of layers,
     or keys and values, in front, all with one block table; ``v_pool``: more layers, perhaps of another width. A sequence then holds ``past`` + ``lengths`` rows; what lies behind them is left as it was."""
     i32 = torch.int32
-    _cuda(k_pool, v_pool, block_table, past, path, lengths)
-    shape = k_pool.shape
-    _need(k_pool.dim() >= 4 and shape[-2] == 64 and k_pool.dtype in DT, "cache_compact: pools are [..., pages, kv_heads, 64, width], float32 or bfloat16")
-    _need(v_pool is None or v_pool.dim() >= 4 and v_pool.dtype == k_pool.dtype and v_pool.shape[-4:-1] == shape[-4:-1], "cache_compact: v_pool has the pages and heads of k_pool")
-    _need(block_table.dim() == 2 and path.dim() == 2, "cache_compact: block_table is [n, pages], path is [n, places]")
-    n = block_table.shape[0]
-    _need(all(t.dtype == i32 for t in (block_table, past, path, lengths)) and past.numel() >= n and lengths.numel() >= n and path.shape[0] >= n,
-          "cache_compact: block_table, past, path and lengths are int32, one row a sequence")
-    _need(path.shape[1] <= MOST_NODES, f"cache_compact: paths of {path.shape[1]} nodes; at most {MOST_NODES} are taken")
-    size, rows = k_pool.element_size(), shape[-4] * shape[-3] * 64
-    k_row, v_row = shape[-1] * size, 0 if v_pool is None else v_pool.shape[-1] * size
-    _need(k_row > 0 and k_row % 4 == 0 and v_row % 4 == 0, "cache_compact: a row's bytes are a multiple of four")
-    if rows == 0 or path.shape[1] == 0 or n == 0:
+    shape, dt = k_pool.shape, k_pool.dtype
+    _need(len(shape) >= 4 and block_table.dim() == 2 and path.dim() == 2, "cache_compact: pools are [..., pages, kv_heads, 64, width], block_table is [n, pages], path is [n, places]")
+    (n, stride), places, size = block_table.shape, path.shape[1], 2 if dt == torch.bfloat16 else 4
+    pages, kv_heads, page, width = shape[-4:]
+    v_width = 0 if v_pool is None else v_pool.shape[-1]
+    if not (k_pool.is_cuda and k_pool.is_contiguous() and _plain_cuda(v_pool) and block_table.is_cuda and block_table.is_contiguous()
+            and past.is_cuda and past.is_contiguous() and path.is_cuda and path.is_contiguous() and lengths.is_cuda and lengths.is_contiguous()
+            and dt in DT and page == 64 and (v_pool is None or v_pool.dtype == dt and v_pool.dim() >= 4 and v_pool.shape[-4:-1] == shape[-4:-1])
+            and i32 == block_table.dtype == past.dtype == path.dtype == lengths.dtype and past.numel() >= n and lengths.numel() >= n and path.shape[0] >= n
+            and places <= MOST_NODES and width * size % 4 == 0 and v_width * size % 4 == 0):
+        _kept_refusal("cache_compact", dict(k_pool=k_pool, v_pool=v_pool, block_table=block_table, past=past, path=path, lengths=lengths), (
+            (lambda: dt in DT and page == 64, "pools are [..., pages, kv_heads, 64, width], float32 or bfloat16"),
+            (lambda: v_pool is None or v_pool.dtype == dt and v_pool.dim() >= 4 and v_pool.shape[-4:-1] == shape[-4:-1], "v_pool has the type, pages and heads of k_pool"),
+            (lambda: i32 == block_table.dtype == past.dtype == path.dtype == lengths.dtype and past.numel() >= n and lengths.numel() >= n and path.shape[0] >= n,
+             "block_table, past, path and lengths are int32, one row a sequence"),
+            (lambda: places <= MOST_NODES, f"paths of {places} nodes; at most {MOST_NODES} are taken"),
+            (lambda: width * size % 4 == 0 and v_width * size % 4 == 0, "a row's bytes are a multiple of four")))
+    rows = pages * kv_heads * 64
+    if rows == 0 or places == 0 or n == 0 or width == 0:
         return
-    lib().call("slb_cache_compact", _p(k_pool), _p(v_pool), _p(block_table), _p(past), _p(path), _p(lengths), k_pool.numel() // (rows * shape[-1]),
-               0 if v_row == 0 else v_pool.numel() // (rows * v_pool.shape[-1]), shape[-4], block_table.shape[1], n, shape[-3], k_row, v_row, path.shape[1],
-               stream if stream is not None else current_stream())
+    try:
+        call = _COMPACT_CALL.pack(k_pool.data_ptr(), 0 if v_pool is None else v_pool.data_ptr(), block_table.data_ptr(), past.data_ptr(), path.data_ptr(),
+                                  lengths.data_ptr(), stream if stream is not None else current_stream(), k_pool.numel() // (rows * width),
+                                  0 if v_width == 0 else v_pool.numel() // (rows * v_width), pages, stride, n, kv_heads, width * size, v_width * size, places)
+    except struct.error as e:
+        raise ValueError(f"cache_compact: a number is out of range ({e})") from None
+    lib().call("slb_cache_compact", call)
