@@ -18,7 +18,7 @@ constexpr int kTreeThreads = 256, kTreeRows = 16, kTreeKeys = 64;
 
 __host__ __device__ constexpr int tree_pad(int hd) { return (hd + 3) & ~3; }
 __host__ __device__ constexpr int tree_smem(int hd) {
-  return (kTreeKeys * (tree_pad(hd) + 4) + kTreeRows * tree_pad(hd) + kTreeRows * kTreeKeys + 2 * kTreeRows) * 4;
+  return (2 * kTreeKeys * (tree_pad(hd) + 4) + kTreeRows * tree_pad(hd) + kTreeRows * kTreeKeys + 2 * kTreeRows) * 4;
 }
 
 // Scratch of a share: per (share, token, head) hd weighted values, maximum, sum.
@@ -64,7 +64,8 @@ __global__ void __launch_bounds__(kTreeThreads) tree_general_kernel(TreeArgs a) 
   extern __shared__ __align__(16) float smem[];
   const int hd = a.head_dim, hdp = tree_pad(hd);
   float* rows_s = smem;                                  // [64][hdp + 4]
-  float* q_s = rows_s + kTreeKeys * (hdp + 4);           // [16][hdp]
+  float* values_s = rows_s + kTreeKeys * (hdp + 4);      // [64][hdp + 4]
+  float* q_s = values_s + kTreeKeys * (hdp + 4);         // [16][hdp]
   float* p_s = q_s + kTreeRows * hdp;                    // [16][64]
   float* alpha_s = p_s + kTreeRows * kTreeKeys;          // [16]
   float* l_s = alpha_s + kTreeRows;                      // [16]
@@ -98,6 +99,7 @@ __global__ void __launch_bounds__(kTreeThreads) tree_general_kernel(TreeArgs a) 
     const int key0 = first + step * kTreeKeys;
     __syncthreads();
     tree_rows<T>(rows_s, (const T*)a.k_pool, a, table, kh, key0, end);
+    tree_rows<T>(values_s, (const T*)a.v_pool, a, table, kh, key0, end);
     if (tid < kTreeRows) {      // what a row sees of these 64 keys
       const int R = r0 + tid;
       unsigned long long b = 0ull;
@@ -129,7 +131,6 @@ __global__ void __launch_bounds__(kTreeThreads) tree_general_kernel(TreeArgs a) 
       for (int i = 0; i < 4; ++i) p_s[(group * 4 + i) * kTreeKeys + key] = bits_s[group * 4 + i] >> key & 1ull ? sc[i] : -INFINITY;
     }
     __syncthreads();
-    tree_rows<T>(rows_s, (const T*)a.v_pool, a, table, kh, key0, end);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       float* p = p_s + (2 * warp + i) * kTreeKeys;
@@ -153,10 +154,11 @@ __global__ void __launch_bounds__(kTreeThreads) tree_general_kernel(TreeArgs a) 
 #pragma unroll
       for (int k = 0; k < 4; ++k) acc[i][k] *= keep;
       const unsigned long long b = bits_s[r];
+#pragma unroll 4
       for (int j = 0; j < n; ++j) {
         if (!(b >> j & 1ull)) continue;
         const float p = p_s[r * kTreeKeys + j];
-        const float4 v = *reinterpret_cast<const float4*>(rows_s + j * (hdp + 4) + c);
+        const float4 v = *reinterpret_cast<const float4*>(values_s + j * (hdp + 4) + c);
         acc[i][0] = fmaf(p, v.x, acc[i][0]);
         acc[i][1] = fmaf(p, v.y, acc[i][1]);
         acc[i][2] = fmaf(p, v.z, acc[i][2]);
@@ -191,32 +193,54 @@ __global__ void __launch_bounds__(kTreeThreads) tree_general_kernel(TreeArgs a) 
   }
 }
 
-// A warp joins the shares of a (token, head), in their order.
+// A warp joins the shares of a (token, head), in their order: a lane a share's factor, then the lanes along the channels, eight shares on the way at once.
+constexpr int kMostSplits = 64;
 template <typename T>
 __global__ void __launch_bounds__(128) tree_join_kernel(TreeArgs a) {
-  pdl_enter();
-  const int lane = threadIdx.x & 31, seq = blockIdx.y;
-  const TreeSeq s(a, seq);
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, seq = blockIdx.y;
+  const TreeSeq s(a, seq);      // (in front of the wait: what the kernel before this one has waited for is there)
+  const long long row = (long long)blockIdx.x * 4 + warp;
+  pdl_wait();
   if (row >= (long long)s.count * a.heads) return;
+  __shared__ float factor_s[4][kMostSplits];
   const size_t token = s.tok0 + row / a.heads;
   const int head = (int)(row % a.heads), hd = a.head_dim;
-  float top = -INFINITY;
-  for (int i = 0; i < a.splits; ++i) top = fmaxf(top, tree_slot(a, i, token, head)[hd]);
-  const float use = top == -INFINITY ? 0.0f : top;
-  float l = 0.0f;
-  for (int i = 0; i < a.splits; ++i) {
-    const float* slot = tree_slot(a, i, token, head);
-    l += slot[hd + 1] * expf(slot[hd] - use);
-  }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  for (int c = lane; c < hd; c += 32) {
-    float v = 0.0f;
-    for (int i = 0; i < a.splits; ++i) {
+  float m[kMostSplits / 32], l[kMostSplits / 32], top = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < kMostSplits / 32; ++k) {
+    const int i = lane + 32 * k;
+    m[k] = -INFINITY;
+    l[k] = 0.0f;
+    if (i < a.splits) {
       const float* slot = tree_slot(a, i, token, head);
-      v = fmaf(slot[c], expf(slot[hd] - use), v);
+      m[k] = slot[hd];
+      l[k] = slot[hd + 1];
     }
-    ((T*)a.out)[(token * a.heads + head) * hd + c] = from_f32<T>(v * inv);
+    top = fmaxf(top, m[k]);
+  }
+  top = warp_max(top);
+  const float use = top == -INFINITY ? 0.0f : top;
+  float sum = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kMostSplits / 32; ++k) {
+    const float f = l[k] == 0.0f ? 0.0f : expf(m[k] - use);      // (0: a share that saw nothing)
+    factor_s[warp][lane + 32 * k] = f;
+    sum += l[k] * f;
+  }
+  sum = warp_sum(sum);
+  __syncwarp();
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  for (int c = lane; c < hd; c += 32) {
+    float acc = 0.0f;
+    for (int i0 = 0; i0 < a.splits; i0 += 8) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = i0 + i < a.splits ? tree_slot(a, i0 + i, token, head)[c] : 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i0 + i < a.splits && factor_s[warp][i0 + i] != 0.0f) acc = fmaf(v[i], factor_s[warp][i0 + i], acc);
+    }
+    ((T*)a.out)[(token * a.heads + head) * hd + c] = from_f32<T>(acc * inv);
   }
 }
 
@@ -224,7 +248,7 @@ __global__ void __launch_bounds__(128) tree_join_kernel(TreeArgs a) {
 static int general_tree_splits(int n_seqs, int max_count, int heads, int kv_heads, int max_keys) {
   const long long tiles = (long long)n_seqs * kv_heads * (((long long)max_count * (heads / kv_heads) + kTreeRows - 1) / kTreeRows);
   const long long steps = ((long long)max_keys + kTreeKeys - 1) / kTreeKeys + 1, wanted = (4ll * sm_count() + tiles - 1) / tiles;
-  return (int)std::max(1ll, std::min(std::min(steps, wanted), 256ll));
+  return (int)std::max(1ll, std::min(std::min(steps, wanted), (long long)kMostSplits));
 }
 
 static long long general_tree_floats(long long tokens, int n_seqs, int max_count, int heads, int kv_heads, int head_dim, int max_keys) {
@@ -243,7 +267,7 @@ static int launch_tree_general(TreeArgs a, cudaStream_t s) {
   launch(tree_general_kernel<T>, dim3(a.splits, (unsigned)tiles, a.n_seqs), dim3(kTreeThreads), (size_t)tree_smem(a.head_dim), s, a);
   const int rc = check_launch("attention_tree");
   if (rc || a.splits == 1) return rc;
-  launch(tree_join_kernel<T>, dim3((unsigned)(((long long)a.max_count * a.heads + 3) / 4), a.n_seqs), dim3(128), 0, s, a);
+  launch_prefetching(tree_join_kernel<T>, dim3((unsigned)(((long long)a.max_count * a.heads + 3) / 4), a.n_seqs), dim3(128), 0, s, a);
   return check_launch("attention_tree (joined)");
 }
 
