@@ -10,6 +10,7 @@ Importing the package needs no GPU; loading a model does.
 from .config import ConfigError, Qwen3Config, parse_config, register_architecture
 from .cache.keep import KeepPolicy
 from .sampling.config import SamplingConfig
+from .sampling.drafts import DraftPolicy
 
 __version__ = "0.1.0"
 
@@ -29,5 +30,5 @@ def write_random_model(*args, **kwargs):
     return _w(*args, **kwargs)
 
 
-__all__ = ["ConfigError", "Qwen3Config", "parse_config", "register_architecture", "KeepPolicy", "SamplingConfig", "load",
+__all__ = ["ConfigError", "Qwen3Config", "parse_config", "register_architecture", "KeepPolicy", "SamplingConfig", "DraftPolicy", "load",
            "generate", "write_random_model", "__version__"]

@@ -245,6 +245,17 @@ class CacheBook:
                         row[lo:keep_from] = -1
                         g.first_page[s] = keep_from
 
+    def settle(self, slots, new_lengths) -> None:
+        """After a step whose rows are not all kept (drafted tokens): ``commit``, and pages behind the last row go back."""
+        if self.budget:
+            raise CacheMisuse("rows of a cache with a budget are not taken back")
+        self.commit(slots, new_lengths)
+        for s, n in zip(slots, new_lengths):
+            for g in self.groups:
+                behind = g.table[s][pages_for(n):]
+                g.pool.give(behind[behind >= 0].tolist())
+                behind[:] = -1
+
     def tables_for(self, slots, pages: int | None = None) -> list[np.ndarray]:
         """Per group the block-table rows of ``slots`` [n, stride] (or their first ``pages`` entries)."""
         idx = np.asarray(slots, dtype=np.int64)

@@ -13,7 +13,7 @@ takes comma- or space-separated token ids (several prompts separated by ``;`` ru
 the new ids are printed. ``--prompt`` works when the model folder has a ``tokenizer.json`` and the
 ``tokenizers``-free byte-level BPE reader is given by the user through ``--tokenizer``; otherwise it
 explains what to pass instead. Options of the reference that belong to parts this library does not
-have (``--step``, ``--draft*``, ``--keep-quantized``, ``--chat``) are not offered.
+have (``--step``, drafting models, ``--keep-quantized``, ``--chat``) are not offered; ``--draft-tokens`` here drafts from the text itself.
 """
 
 from __future__ import annotations
@@ -72,6 +72,10 @@ def build_parser() -> argparse.ArgumentParser:
                    help="the cache keeps N tokens for each key/value head: the first, the latest, and those that were looked at most")
     s.add_argument("--keep-first", type=int, default=4, metavar="N", help="first tokens that stay (default 4)")
     s.add_argument("--keep-recent", type=int, default=None, metavar="N", help="latest tokens that stay under a budget (default: half of it)")
+    s.add_argument("--draft-tokens", type=int, default=0, metavar="N",
+                   help="draft up to N tokens a step from the text so far and judge them at once; the output stays the same (0 = off)")
+    s.add_argument("--draft-branches", type=int, default=None, metavar="N", help="continuations that a step tries (default 1)")
+    s.add_argument("--draft-ngram", type=int, default=None, metavar="N", help="the longest phrase that is looked for in the text (default 3)")
     s.set_defaults(fn=cmd_generate)
 
     r = sub.add_parser("replay", help="feed token traces through a model and write logits (see bin/trace_run)")
@@ -115,6 +119,11 @@ def cmd_generate(a) -> int:
     if a.keep_window or a.keep_budget or a.keep_recent is not None:
         from .cache.keep import KeepPolicy
         keep = KeepPolicy(budget=a.keep_budget, window=a.keep_window, first=a.keep_first, recent=a.keep_recent)
+    drafts = None
+    if a.draft_tokens or a.draft_branches is not None or a.draft_ngram is not None:
+        from .sampling.drafts import DraftPolicy
+        drafts = DraftPolicy(a.draft_tokens, 1 if a.draft_branches is None else a.draft_branches, 3 if a.draft_ngram is None else a.draft_ngram)
+    drafting = {} if drafts is None else {"drafts": drafts}
     per_prompt = keep.rows_for(a.max_seq_len) if keep is not None and keep.budget else a.max_seq_len
     engine = load(a.path, dtype=_dtype_name(a.dtype), max_seq_len=a.max_seq_len, device=device,
                   max_tokens=max(1, len(prompts)) * (-(-per_prompt // 64) * 64 if keep is not None else per_prompt), keep=keep,
@@ -126,16 +135,17 @@ def cmd_generate(a) -> int:
     print(f"[{engine.spec.__class__.__name__} of {type(engine.config).__name__}, {n_params / 1e6:.2f}M params, "
           f"{engine.device}, {str(engine.dtype).replace('torch.', '')}]", file=sys.stderr, flush=True)
     stop_ids = set(a.stop_id) if a.stop_id is not None else None
-    engine.generate([[prompts[0][0]] * 8], 2, sampling, seed=0, cuda_graph=a.cuda_graph)     # warm-up
+    engine.generate([[prompts[0][0]] * 8], 2, sampling, seed=0, cuda_graph=a.cuda_graph, **drafting)     # warm-up
     for i in range(a.samples):
         seed = None if a.seed is None else a.seed + i
-        res = engine.generate(prompts, a.max_new_tokens, sampling, stop_ids=stop_ids, seed=seed, cuda_graph=a.cuda_graph)
+        res = engine.generate(prompts, a.max_new_tokens, sampling, stop_ids=stop_ids, seed=seed, cuda_graph=a.cuda_graph, **drafting)
         for r in res:
             if tok is not None:
                 print(tok[1](r.new_ids), flush=True)
             else:
                 print(" ".join(str(t) for t in r.new_ids), flush=True)
-            mem = f", peak GPU memory {torch.cuda.max_memory_allocated(engine.device) / 2**30:.2f} GiB"
+            drafted = f", drafts {r.stats['drafts_taken']} of {r.stats['drafted']} taken" if drafts is not None else ""
+            mem = f"{drafted}, peak GPU memory {torch.cuda.max_memory_allocated(engine.device) / 2**30:.2f} GiB"
             print(f"[{len(r.new_ids)} tokens, stop: {r.stop_reason}, prompt {len(r.prompt_ids)} tokens in "
                   f"{r.prefill_seconds * 1000:.0f} ms, decode {r.decode_tok_per_s:,.1f} tok/s{mem}]",
                   file=sys.stderr, flush=True)

@@ -54,6 +54,7 @@ class StepBatch:
     tok_rot: torch.Tensor | None = None
     lengths: torch.Tensor | None = None
     seen: torch.Tensor | None = None
+    tree: object | None = None      # a step of drafted tokens (stepper.DraftStep); ``tok_pos`` then speaks of rows of the cache
 
 
 def _round(n: int) -> int:

@@ -27,12 +27,13 @@ from ..config.registry import parse_config
 from ..parts.base import BuildContext
 from ..kernels import ops
 from ..sampling.config import SamplingConfig
+from ..sampling.drafts import DraftPolicy
 from ..sampling.sampler import Sampler
 from ..weights.loader import load_into
 from ..weights.safetensors import Checkpoint
 from .generate import GenerationResult, generate_batches
 from .model import Model
-from .stepper import StepEntry, Stepper
+from .stepper import StepEntry, Stepper, TreeEntry, drafts_refusal
 
 _DTYPES = {"bf16": torch.bfloat16, "bfloat16": torch.bfloat16, "fp32": torch.float32, "float32": torch.float32,
            "auto": torch.bfloat16, None: torch.bfloat16, torch.bfloat16: torch.bfloat16, torch.float32: torch.float32}
@@ -159,7 +160,9 @@ class Engine:
 
     # ------------------------------------------------------------------ stepping ----
     def open(self, n: int) -> list[int]:
-        return self.cache.open(n)
+        slots = self.cache.open(n)
+        self.stepper.forget(slots)
+        return slots
 
     def close(self, slots: Sequence[int]) -> None:
         self.cache.close(slots)
@@ -167,6 +170,14 @@ class Engine:
     def step(self, entries) -> torch.Tensor:
         """entries: ``StepEntry`` objects or ``(slot, tokens, want)`` tuples. See ``Stepper.step``."""
         return self.stepper.step([e if isinstance(e, StepEntry) else StepEntry(*e) for e in entries])
+
+    def step_tree(self, entries) -> torch.Tensor:
+        """entries: ``TreeEntry`` objects or ``(slot, tokens, parents)`` tuples: the newest token of each sequence and drafts behind it. See ``Stepper.step_tree``."""
+        return self.stepper.step_tree([e if isinstance(e, TreeEntry) else TreeEntry(*e) for e in entries])
+
+    def accept(self, slots: Sequence[int], paths) -> None:
+        """Which nodes of each sequence's last ``step_tree`` stay. See ``Stepper.accept``."""
+        self.stepper.accept(slots, paths)
 
     # ---- what the generation loop needs (the ``Backend`` protocol of engine/generate.py) ----
     def prefill(self, slots, prompts):
@@ -214,11 +225,17 @@ class Engine:
     def generate(self, prompts, max_new_tokens: int = 200, sampling: SamplingConfig | None = None, stop_ids=None,
                  vocab_limit: int | None = None, seed: int | None = None,
                  on_token: Callable[[int, int], None] | None = None, cuda_graph: bool = True,
-                 max_batch: int = 64) -> list[GenerationResult]:
+                 max_batch: int = 64, drafts: DraftPolicy | None = None) -> list[GenerationResult]:
         """Generate for a list of prompts (token id lists of unequal lengths).
 
         stop_ids default to the ``eos_token_id`` of ``config.json``. ``cuda_graph=False`` runs every
-        decode step launch by launch."""
+        decode step launch by launch. ``drafts``: steps judge several drafted tokens at once (``sampling/drafts.py``)."""
+        if drafts is not None:
+            if not isinstance(drafts, DraftPolicy):
+                raise TypeError(f"drafts is a DraftPolicy or None, got {type(drafts).__name__}")
+            why = drafts_refusal(self.model, self.cache)
+            if why is not None:
+                raise ValueError(f"drafts: not built for this model: {why}")
         if stop_ids is None:
             stop_ids = set(getattr(self.config, "stop_ids", ()))
         before = self.stepper.use_graphs
@@ -227,7 +244,7 @@ class Engine:
         self.pipelined = len(prompts) <= self.stepper.feed.numel() and max_batch <= self.stepper.feed.numel()
         try:
             results = generate_batches(self, prompts, max_new_tokens, sampling, stop_ids, vocab_limit, seed, on_token,
-                                       max_batch)
+                                       max_batch, drafts)
         finally:
             self.stepper.use_graphs = before
         # every token has been read back, so the device is idle: one look at the status word that the tensor-memory
@@ -248,9 +265,9 @@ def load(path, dtype="bf16", max_seq_len: int = 4096, max_tokens: int | None = N
 def generate(engine: Engine, prompt_ids: Sequence[int], max_new_tokens: int = 200,
              sampling: SamplingConfig | None = None, stop_ids=None, vocab_limit: int | None = None,
              seed: int | None = None, on_token: Callable[[int], None] | None = None,
-             cuda_graph: bool = True) -> GenerationResult:
+             cuda_graph: bool = True, drafts: DraftPolicy | None = None) -> GenerationResult:
     """Generate after one prompt; the counterpart of the reference's ``generate``
     (sleuth/forge/infer/generate.py:50-52), same argument names and meanings."""
     cb = None if on_token is None else (lambda request, tok: on_token(tok))
     return engine.generate([list(prompt_ids)], max_new_tokens, sampling, stop_ids, vocab_limit, seed, cb,
-                           cuda_graph)[0]
+                           cuda_graph, drafts=drafts)[0]

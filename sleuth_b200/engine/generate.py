@@ -24,6 +24,7 @@ from typing import Callable, Protocol, Sequence
 
 from ..cache.book import pages_for
 from ..sampling.config import SamplingConfig
+from ..sampling.drafts import DraftPolicy, NgramDrafter
 from ..sampling.host import NgramBlocker, fresh_seed, recent_window, uniform
 
 
@@ -64,6 +65,8 @@ class Backend(Protocol):
     #   choose_later(logits, cfg, uniforms, vocab_limit) -> callable giving the tokens once they are on the host;
     #       the tokens also stay on the device, row i of them in feed slot i
     #   decode_fed(slots, feed_map) -> logits: sequence i continues with the token in feed slot feed_map[i]
+    # optional, for drafted tokens (sampling/drafts.py):
+    #   step_tree([(slot, tokens, parents)]) -> logits of every node; accept(slots, paths): the nodes of each that stay
 
 
 @dataclass
@@ -73,6 +76,9 @@ class _Live:
     prompt: list[int]
     new: list[int] = field(default_factory=list)
     blocker: NgramBlocker | None = None
+    drafter: NgramDrafter | None = None
+    drafted: int = 0            # drafts that were judged, and those that were right
+    taken: int = 0
 
 
 def plan_batches(prompt_lengths: Sequence[int], max_new_tokens: int, max_len: int, total_pages: int,
@@ -96,7 +102,7 @@ def plan_batches(prompt_lengths: Sequence[int], max_new_tokens: int, max_len: in
 def generate_batches(backend: Backend, prompts: Sequence[Sequence[int]], max_new_tokens: int = 200,
                      sampling: SamplingConfig | None = None, stop_ids=None, vocab_limit: int | None = None,
                      seed: int | None = None, on_token: Callable[[int, int], None] | None = None,
-                     max_batch: int = 64) -> list[GenerationResult]:
+                     max_batch: int = 64, drafts: DraftPolicy | None = None) -> list[GenerationResult]:
     """Generate for every prompt; results come back in the order of ``prompts``.
 
     on_token(request_index, token) is called for each new token as it is produced.
@@ -104,6 +110,8 @@ def generate_batches(backend: Backend, prompts: Sequence[Sequence[int]], max_new
     sampling = sampling or SamplingConfig()
     stop_ids = set(stop_ids or ())
     seed = fresh_seed() if seed is None else int(seed)
+    if drafts is not None and sampling.needs_context:
+        raise ValueError("drafts: not built for repetition_penalty and no_repeat_ngram, which change the logits token by token")
     cleaned = []
     for i, p in enumerate(prompts):
         p = [int(t) for t in p]
@@ -119,6 +127,9 @@ def generate_batches(backend: Backend, prompts: Sequence[Sequence[int]], max_new
     # one step ahead of the host (see _run_batch_pipelined).
     pipelined = getattr(backend, "pipelined", False) and not sampling.needs_context
     run = _run_batch_pipelined if pipelined else _run_batch
+    if drafts is not None:
+        def run(*args):
+            _run_batch_drafted(*args, drafts)
     for batch in plan_batches([len(p) for p in cleaned], max_new_tokens, backend.max_len, backend.total_pages,
                               max_batch, getattr(backend, "max_rows", None)):
         run(backend, batch, cleaned, results, max_new_tokens, sampling, stop_ids, vocab_limit, seed, on_token)
@@ -249,8 +260,110 @@ def _run_batch_pipelined(backend, batch, prompts, results, max_new_tokens, sampl
             backend.close(sorted(held))
 
 
+def _run_batch_drafted(backend, batch, prompts, results, max_new_tokens, sampling, stop_ids, vocab_limit, seed, on_token, drafts):
+    """The same choices as ``_run_batch``, several a step where drafts are right.
+
+    A step brings each sequence's newest token and what its drafter proposes behind it. A token is chosen at every node, with the random number of the node's
+    place in the text; from the newest token on the choices are followed as long as one of them is a draft. What was chosen behind the last of those is the next newest token."""
+    slots = backend.open(len(batch))
+    live = [_Live(r, s, prompts[r], drafter=NgramDrafter(drafts, prompts[r])) for r, s in zip(batch, slots)]
+    held = set(slots)
+
+    def choose(logits, draws):
+        us = None if sampling.greedy else [uniform(seed, q.request, step) for q, step in draws]
+        return backend.choose(logits, sampling, us, vocab_limit, None, None)      # synchronises
+
+    def take(q, tok, length):
+        """One more token of a sequence whose cache holds ``length`` tokens; why it ends, or None."""
+        q.new.append(tok)
+        q.drafter.add(tok)
+        if on_token is not None:
+            on_token(q.request, tok)
+        if tok in stop_ids:
+            return "stop_token"
+        if length >= backend.max_len:
+            return "context_full"
+        return "max_new_tokens" if len(q.new) >= max_new_tokens else None
+
+    try:
+        backend.sync()
+        t0 = time.perf_counter()
+        tokens = choose(backend.prefill([q.slot for q in live], [q.prompt for q in live]), [(q, 0) for q in live])
+        now = t1 = time.perf_counter()
+        keep = []
+        for q, tok in zip(live, tokens):
+            reason = take(q, tok, backend.length(q.slot))
+            if reason is None:
+                keep.append(q)
+            else:
+                _finish(backend, q, reason, results, t0, t1, now, held)
+        live = keep
+        while live:
+            # sequences that would need a page the cache no longer has end here
+            while live and backend.pages_needed([q.slot for q in live], [backend.length(q.slot) + 1 for q in live]) > backend.free_pages():
+                q = max(live, key=lambda q: backend.length(q.slot))
+                live.remove(q)
+                _finish(backend, q, "context_full", results, t0, t1, time.perf_counter(), held)
+            if not live:
+                break
+            # (a draft behind the last token that there is room for would be judged for nothing)
+            rooms = [min(max_new_tokens - len(q.new), backend.max_len - backend.length(q.slot)) - 1 for q in live]
+            trees = []
+            for q, room in zip(live, rooms):
+                more, parents = q.drafter.propose(room)
+                trees.append(([q.new[-1], *more], [-1, *parents]))
+            if any(len(t) > 1 for t, _ in trees):
+                # every sequence brings as many tokens as there may be, so that recorded steps serve the next ones: the last one again and again, which is a draft like any other
+                for (t, p), room in zip(trees, rooms):
+                    for _ in range(min(room, drafts.tokens) + 1 - len(t)):
+                        p.append(len(t) - 1)
+                        t.append(t[-1])
+            if backend.pages_needed([q.slot for q in live], [backend.length(q.slot) + len(t) for q, (t, _) in zip(live, trees)]) > backend.free_pages():
+                trees = [([q.new[-1]], [-1]) for q in live]
+            drafted = any(len(t) > 1 for t, _ in trees)
+            if drafted:
+                logits = backend.step_tree([(q.slot, t, p) for q, (t, p) in zip(live, trees)])
+            else:
+                logits = backend.decode([q.slot for q in live], [t[0] for t, _ in trees])
+            draws = []
+            for q, (t, p) in zip(live, trees):
+                depth = [0] * len(t)
+                for i in range(1, len(t)):
+                    depth[i] = depth[p[i]] + 1
+                draws += [(q, len(q.new) + d) for d in depth]
+            chosen = choose(logits, draws)
+            now = time.perf_counter()
+            keep, paths, base = [], [], 0
+            for q, (t, p) in zip(live, trees):
+                before = backend.length(q.slot) - (0 if drafted else 1)      # tokens in the cache before the step
+                node, path, reason = 0, [0], None
+                q.drafted += len(t) - 1
+                while True:
+                    tok = chosen[base + node]
+                    reason = take(q, tok, before + len(path))
+                    if reason is not None:
+                        break
+                    node = next((i for i in range(node + 1, len(t)) if p[i] == node and t[i] == tok), None)
+                    if node is None:
+                        break
+                    path.append(node)
+                    q.taken += 1
+                base += len(t)
+                if reason is None:
+                    keep.append(q)
+                    paths.append(path)
+                else:
+                    _finish(backend, q, reason, results, t0, t1, now, held)
+            if drafted and keep:
+                backend.accept([q.slot for q in keep], paths)
+            live = keep
+    finally:
+        if held:
+            backend.close(sorted(held))
+
+
 def _finish(backend, q: _Live, reason: str, results, t0, t1, now, held) -> None:
     results[q.request] = GenerationResult(q.prompt, q.new, reason, t1 - t0, now - t1,
-                                          {"slot": q.slot})
+                                          {"slot": q.slot} if q.drafter is None else {"slot": q.slot, "drafted": q.drafted, "drafts_taken": q.taken})
     backend.close([q.slot])
     held.discard(q.slot)

@@ -30,7 +30,9 @@ import torch
 
 from ..cache.book import CacheFull
 from ..kernels import ops
+from ..parts.attention import GQAAttention
 from ..parts.base import Workspace
+from ..parts.ends import TokenEmbedding
 from .batch import MetaStager
 
 
@@ -39,6 +41,37 @@ class StepEntry:
     slot: int
     tokens: object              # sequence of token ids
     want: object = ()           # positions among ``tokens`` whose logits are wanted
+
+
+@dataclass
+class TreeEntry:
+    """A sequence's share of a step of drafted tokens: ``tokens[0]`` is its newest certain token, ``tokens[i]`` a draft behind ``tokens[parents[i]]``
+    (``parents[i]`` < i; ``parents[0]`` is -1)."""
+    slot: int
+    tokens: object
+    parents: object
+
+
+@dataclass
+class DraftStep:
+    """What the attention parts need of such a step."""
+    positions: torch.Tensor         # [tokens] int32, by which rows are rotated
+    seen: list                      # per cache group [tokens, words] int32: the rows of the step that a row sees under the group's window
+
+
+def drafts_refusal(model, cache) -> str | None:
+    """Why steps of drafted tokens are not built for a model, or None."""
+    if cache.book.budget:
+        return "a cache with a budget gives no rows back"
+    if type(model.embedding) is not TokenEmbedding or model.embedding.turns is not None:
+        return "the embedding is more than a table of tokens"
+    mixers = [layer.children.get("mixer") if hasattr(layer, "children") else None for layer in model.layers]
+    if not all(isinstance(m, GQAAttention) and m.takes_drafts for m in mixers):
+        return "every mixer has to be grouped-query attention over a cache entry of its own, without a policy, chunks, sinks, a gate or values of another width"
+    schedule = model.spec.schedule
+    if len({e.cache for e in schedule}) != len(schedule) or any(e.borrow >= 0 for e in schedule):
+        return "layer applications share a cache entry"
+    return None
 
 
 class Stepper:
@@ -63,6 +96,7 @@ class Stepper:
         self._seen_chunk: set = set()
         self._chunk_logits: torch.Tensor | None = None
         self.max_graph_rows = 64        # steps of many tokens are recorded only if they want at most this many rows of logits
+        self.max_draft_rows = 512       # the same for steps of drafted tokens, which want every row's
         self.max_chunk_graphs = 16      # recordings of such steps kept at a time
         self._decode_logits: torch.Tensor | None = None
         self._graph_key = None
@@ -72,6 +106,9 @@ class Stepper:
         self._steps_unseen = 0              # single-token steps since the word was last copied
         self._graph_own: dict = {}          # own kernel launches captured in each graph
         self.graph_kernel_launches = 0      # own kernel launches replayed through graphs so far
+        self._drafted: dict[int, tuple[int, int]] = {}      # slot -> its rows before the last step of drafted tokens, and the rows of that step
+        self._draft_parents: torch.Tensor | None = None     # what a recorded step of drafted tokens reads, at fixed places
+        self._draft_tables: dict = {}
         ops.lib()   # build or load the kernels now; fail here, loudly, if that is impossible
 
     # ------------------------------------------------------------------ public ----
@@ -131,6 +168,102 @@ class Stepper:
             self._run_chunk(entries, slots, toks, chunk, out, out_base)
         self._look_at_status()
         return out
+
+    # ------------------------------------------------------------------ drafted tokens ----
+    def step_tree(self, entries: list[TreeEntry]) -> torch.Tensor:
+        """Run the newest token of each sequence and the drafts behind it, all at once: float32 logits of every node, in the order of the entries and
+        of their tokens. Nothing of it is kept until ``accept`` says which nodes are; a sequence that takes another step before is as it was."""
+        why = drafts_refusal(self.model, self.cache)
+        if why is not None:
+            raise ValueError(f"drafts: not built for this model: {why}")
+        if not entries:
+            return torch.empty((0, self.model.vocab), dtype=torch.float32, device=self.device)
+        self._raise_late_status()
+        book = self.cache.book
+        toks = [np.asarray(e.tokens, dtype=np.int64).reshape(-1) for e in entries]
+        trees = [np.asarray(e.parents, dtype=np.int64).reshape(-1) for e in entries]
+        slots = [int(e.slot) for e in entries]
+        if len(set(slots)) != len(slots):
+            raise ValueError("a step names a slot twice")
+        for s, t, p in zip(slots, toks, trees):
+            if not 1 <= t.size <= ops.MOST_NODES or p.size != t.size:
+                raise ValueError(f"slot {s}: a step of drafted tokens brings 1 to {ops.MOST_NODES} tokens and a parent for each")
+            if t.min() < 0 or t.max() >= self.model.vocab:
+                raise ValueError(f"slot {s}: token ids must lie in [0, {self.model.vocab})")
+            if p[0] != -1 or (t.size > 1 and (p[1:].min() < 0 or (p[1:] >= np.arange(1, t.size)).any())):
+                raise ValueError(f"slot {s}: a draft continues an earlier token of the step, and the first token none (-1)")
+        past = [int(book.lengths[s]) for s in slots]
+        counts = [int(t.size) for t in toks]
+        new_lens = [p + c for p, c in zip(past, counts)]
+        for s, n in zip(slots, new_lens):
+            if n > self.max_len:
+                raise CacheFull(f"slot {s} would hold {n} tokens; the longest sequence allowed is {self.max_len}")
+        T = sum(counts)
+        if T > self.max_step_tokens:
+            raise ValueError(f"a step of drafted tokens brings at most {self.max_step_tokens} tokens, got {T}")
+        book.grow(slots, new_lens)
+        b = self.meta.upload(slots, past, counts, np.concatenate(toks).astype(np.int32), np.arange(T, dtype=np.int32), book.tables_for(slots))
+        b.tree = self._draft_step(b, np.concatenate(trees).astype(np.int32))
+        out = torch.empty((T, self.model.vocab), dtype=torch.float32, device=self.device)
+        if not self._chunk_by_graph(b, T, out, np.arange(T)):
+            self.model.forward(b, self.cache, self.ws, out)
+        for s, p, c in zip(slots, past, counts):
+            self._drafted[s] = (p, c)
+        self._look_at_status()
+        return out
+
+    def _draft_step(self, b, parents: np.ndarray) -> DraftStep:
+        """The step's parents on the device, and the tables that the attention reads, one launch a window."""
+        T, words = b.T, -(-b.max_count // 32)
+        if self._draft_parents is None or self._draft_parents.numel() < T:
+            self._draft_parents = torch.zeros(max(2 * T, 1024), dtype=torch.int32, device=self.device)
+            self._draft_tables.clear()
+            self._graphs.clear()
+        at = self._draft_parents[:T]
+        at.copy_(torch.from_numpy(parents))
+        if words not in self._draft_tables:
+            cap = self._draft_parents.numel()
+            windows = sorted({r.window for r in self.cache.group_requests})
+            self._draft_tables[words] = (torch.zeros(cap, dtype=torch.int32, device=self.device),
+                                         {w: torch.zeros((cap, words), dtype=torch.int32, device=self.device) for w in windows})
+        positions, seen = self._draft_tables[words]
+        for window, table in seen.items():
+            ops.draft_tree(at, b.seq_start, b.past, b.counts, table, positions, b.max_count, window)
+        return DraftStep(positions, [seen[r.window] for r in self.cache.group_requests])
+
+    def forget(self, slots) -> None:
+        """Slots that stand for new sequences: what an earlier one drafted is not theirs to accept."""
+        for s in slots:
+            self._drafted.pop(int(s), None)
+
+    def accept(self, slots, paths) -> None:
+        """Of the last ``step_tree`` of each of ``slots`` the nodes of its path stay (numbers of its tokens, rising, from 0 on); their rows move together in every
+        layer and the others' go."""
+        book = self.cache.book
+        slots = [int(s) for s in slots]
+        paths = [[int(i) for i in p] for p in paths]
+        if len(set(slots)) != len(slots) or len(paths) != len(slots):
+            raise ValueError("accept: one path for each slot, every slot once")
+        for s, p in zip(slots, paths):
+            past, count = self._drafted.get(s, (-1, 0))
+            if past < 0 or past != int(book.lengths[s]):
+                raise ValueError(f"accept: slot {s} has taken no step of drafted tokens, or another one since")
+            if not p or p[0] != 0 or any(a >= b for a, b in zip(p, p[1:])) or p[-1] >= count:
+                raise ValueError(f"accept: slot {s}: a path rises from 0 and stays below the step's {count} tokens")
+        moving = [i for i, p in enumerate(paths) if p != list(range(len(p)))]
+        if moving:
+            width = max(len(paths[i]) for i in moving)
+            host = np.full((len(moving), width + 2), -1, dtype=np.int32)
+            for row, i in zip(host, moving):
+                row[:len(paths[i])] = paths[i]
+                row[width:] = book.lengths[slots[i]], len(paths[i])
+            both = torch.from_numpy(host).to(self.device)
+            path, past, lengths = (both[:, a:z].contiguous() for a, z in ((0, width), (width, width + 1), (width + 1, width + 2)))
+            for pool, rows in zip(self.cache.pools, book.tables_for([slots[i] for i in moving])):
+                ops.cache_compact(pool, torch.from_numpy(np.ascontiguousarray(rows)).to(self.device), past, path, lengths)
+        for s in slots:
+            del self._drafted[s]
+        book.settle(slots, [int(book.lengths[s]) + len(p) for s, p in zip(slots, paths)])
 
     def _cut(self, toks) -> list:
         """The chunks of a step: lists of (entry index, first token, tokens) with at most ``max_step_tokens`` tokens
@@ -235,10 +368,11 @@ class Stepper:
         launches per step, which for short prompts is most of the step's time. Lengths, positions and tables live
         in the device buffer that the upload refreshed, so one recording serves every step of that shape. The logits
         land in a buffer of the stepper's and are copied to ``out``. Returns False if the step was not run."""
-        if not (self.use_graphs and getattr(self.model, "capturable", True) and 0 < W <= self.max_graph_rows):
+        most = self.max_graph_rows if b.tree is None else self.max_draft_rows
+        if not (self.use_graphs and getattr(self.model, "capturable", True) and 0 < W <= most):
             return False
         self._check_graph_key()
-        gkey = ("chunk", b.T, b.n, b.max_count, W, b.fresh)      # parts may treat steps that start at position 0 differently
+        gkey = ("chunk" if b.tree is None else "drafts", b.T, b.n, b.max_count, W, b.fresh)      # parts may treat steps that start at position 0 differently
         graph = self._graphs.get(gkey)
         if graph is None and gkey not in self._seen_chunk:
             self._seen_chunk.add(gkey)

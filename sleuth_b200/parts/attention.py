@@ -255,9 +255,37 @@ class GQAAttention(Part):
                             slots=b.slots, scratch=ws.take((words,), torch.int32) if words else None, max_length=most, stream=b.stream)
         ws.release(mark)
 
+    @property
+    def takes_drafts(self) -> bool:
+        """Whether steps of drafted tokens are built for this attention."""
+        return self.keep is None and not (self.wide or self.spec.sinks or self.spec.unit_sink or self.spec.chunk or self.spec.reads_shared_kv)
+
+    def _forward_drafts(self, h, x, b, view, ws):
+        """A step of drafted tokens: a row sees what lies before the step and the rows that it continues; rows are rotated by their positions."""
+        s, T = self.spec, h.shape[0]
+        mark = ws.mark()
+        table, tree = b.tables[view.group], b.tree
+        tables = self.position.tables()
+        cos, sin = tables if tables is not None else (None, None)
+        qkv = self.qkv.forward(h, ws=ws, stream=b.stream)
+        q = ws.take((T, s.heads, s.head_dim), self.ctx.dtype)
+        ops.qkv_post(qkv, self.bias, self.q_gain, self.k_gain, cos, sin, q, view.k_pool, view.v_pool, b.tok_seq, b.tok_pos, table, s.heads,
+                     s.kv_heads, s.head_dim, self.position.rot_dim, s.qk_norm_eps, b.stream, tok_rot=tree.positions)
+        y = ws.take((T, s.heads * s.head_dim), self.ctx.dtype)
+        # (a recorded step serves later ones of its shape, so sizes go by what the cache may hold, not by what it holds now)
+        floats = ops.attention_tree_scratch_floats(T, b.n, b.max_count, s.heads, s.kv_heads, s.head_dim, 64 * table.shape[1], self.ctx.dtype)
+        scratch = ws.take((floats,), torch.float32) if floats else None
+        ops.attention_tree(q, view.k_pool, view.v_pool, y, b.seq_start, b.past, b.counts, tree.seen[view.group], tree.positions, table, b.max_count, s.heads,
+                           s.kv_heads, s.head_dim, view.window, self.scale, scratch=scratch, stream=b.stream)
+        self.o.forward(y, ws=ws, stream=b.stream, next_read=getattr(b, "next_read", None) if self.ctx.dtype == torch.float32 else None, **result_target(b, x))
+        ws.release(mark)
+
     def forward(self, h, x, b, view, ws):
         if self.keep is not None:
             self._forward_kept(h, x, b, view, ws)
+            return
+        if getattr(b, "tree", None) is not None:
+            self._forward_drafts(h, x, b, view, ws)
             return
         s = self.spec
         T = h.shape[0]
