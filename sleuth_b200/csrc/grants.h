@@ -1,4 +1,4 @@
-// Dynamic shared memory above 48 KB has to be allowed for a kernel, once on every device that runs it.
+// Dynamic shared memory above 48 KB has to be allowed for a kernel, once on every device that runs it; so have clusters of more than eight blocks.
 #pragma once
 
 #include <cuda_runtime_api.h>
@@ -20,5 +20,8 @@ inline cudaError_t allow_shared(const void* kernel, int bytes, std::atomic<unsig
   if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
   return e;
 }
+
+// Lets `kernel` be launched in clusters of more than eight blocks on the current device. A launcher asks when it works out what it may launch on a device, and keeps that by device.
+inline cudaError_t allow_wide_clusters(const void* kernel) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1); }
 
 }  // namespace slb

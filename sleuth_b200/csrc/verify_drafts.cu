@@ -759,7 +759,7 @@ static int wide_clusters() {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaFuncSetAttribute((const void*)verify_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+  if (allow_wide_clusters((const void*)verify_kernel) != cudaSuccess ||
       cudaOccupancyMaxActiveClusters(&clusters, verify_kernel, &cfg) != cudaSuccess) {
     cudaGetLastError();
     clusters = 0;
