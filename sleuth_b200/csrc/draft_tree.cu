@@ -109,6 +109,7 @@ struct CompactArgs {
   long long k_layer, v_layer;             // bytes of a layer
   long long k_pieces, pieces;             // (layer, kv head, piece) of the keys, and of keys and values
   int table_stride, kv_heads, k_row, v_row, path_width;      // bytes of a row
+  long long pages;
 };
 
 constexpr int kCompactThreads = 256;
@@ -127,7 +128,13 @@ __global__ void __launch_bounds__(kCompactThreads) cache_compact_kernel(CompactA
   if (tid < most) {
     const int p = path[tid], before = tid ? path[tid - 1] : -1;
     from_s[tid] = p;
-    if (p <= before || p < 0 || past < 0 || (long long)past + p >= rows) atomicMin(&s_len, tid);      // the path ends in front of it
+    bool good = p > before && p >= 0 && past >= 0 && (long long)past + p < rows;
+    if (good) {
+      const int* table = a.block_table + (size_t)seq * a.table_stride;
+      const int from = table[(past + p) / kPageTokens], to = table[(past + tid) / kPageTokens];
+      good = from >= 0 && from < a.pages && to >= 0 && to < a.pages;
+    }
+    if (!good) atomicMin(&s_len, tid);      // the path ends in front of it
   }
   __syncthreads();
   const int len = s_len;
@@ -181,6 +188,7 @@ extern "C" int slb_cache_compact(const CompactCall* call) {
   if (n_seqs == 0 || layers + v_layers == 0) return 0;
   CompactArgs a{};
   a.k_pool = (char*)k_pool; a.v_pool = (char*)v_pool; a.block_table = c.block_table; a.past = c.past; a.path = c.path; a.lengths = c.lengths;
+  a.pages = pages;
   a.table_stride = table_stride; a.kv_heads = kv_heads; a.k_row = k_row; a.v_row = v_row; a.path_width = path_width;
   a.k_layer = pages * kv_heads * kPageTokens * k_row;
   a.v_layer = pages * kv_heads * kPageTokens * v_row;

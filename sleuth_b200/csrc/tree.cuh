@@ -23,7 +23,7 @@ struct TreeArgs {
   const int* positions;     // [tokens], or null without a window
   const int* block_table;   // [n, table_stride]
   int table_stride, n_seqs, heads, kv_heads, head_dim, window, words, max_count;
-  long long tokens;
+  long long tokens, pool_pages;
   float scale;
   float* scratch;
   int splits, max_keys;
@@ -45,13 +45,15 @@ struct TreeCall {
 };
 static_assert(sizeof(TreeCall) == 13 * 8 + 3 * 8 + 10 * 4 + 4 + 4, "as packed in kernels/ops.py");
 
-// A sequence's share of a step: its rows before it and its nodes, both inside what the call promised.
+// A sequence's share of a step: its rows before it and its nodes, both inside what the call promised and the given tokens.
 struct TreeSeq {
   int past, count, tok0;
   __device__ __forceinline__ TreeSeq(const TreeArgs& a, int seq) {
     tok0 = a.seq_start[seq];
     past = min(max(a.past[seq], 0), a.max_keys);
     count = min(min(max(a.counts[seq], 0), a.max_count), a.max_keys - past);
+    if (tok0 < 0 || tok0 >= a.tokens) count = 0;
+    else if (count > a.tokens - tok0) count = (int)(a.tokens - tok0);
   }
 };
 

@@ -26,7 +26,7 @@ __device__ __forceinline__ float* tree_slot(const TreeArgs& a, int split, size_t
   return a.scratch + (((size_t)split * a.tokens + token) * a.heads + head) * (a.head_dim + 2);
 }
 
-// 64 rows of a pool from row `key0` on as float32 in shared memory, rows of hdp + 4 floats; zeros from row `end` on.
+// 64 rows of a pool from row `key0` on as float32 in shared memory, rows of hdp + 4 floats; zeros from row `end` on, and for pages that the pool has not (as TMA reads them).
 template <typename T>
 __device__ __forceinline__ void tree_rows(float* dst, const T* pool, const TreeArgs& a, const int* table, int kh, int key0, int end) {
   const int hd = a.head_dim, hdp = tree_pad(hd), r0 = threadIdx.x >> 4;
@@ -34,7 +34,8 @@ __device__ __forceinline__ void tree_rows(float* dst, const T* pool, const TreeA
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int key = key0 + r0 + 16 * i;
-    const T* src = key < end ? pool + (((size_t)table[key / kPageTokens] * a.kv_heads + kh) * kPageTokens + key % kPageTokens) * hd : nullptr;
+    const int page = key < end ? table[key / kPageTokens] : -1;
+    const T* src = page >= 0 && page < a.pool_pages ? pool + (((size_t)page * a.kv_heads + kh) * kPageTokens + key % kPageTokens) * hd : nullptr;
     for (int c = 4 * (threadIdx.x & 15); c < hdp; c += 64) {
       float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (src) {
@@ -297,7 +298,7 @@ extern "C" int slb_attention_tree(const TreeCall* call) {
   a.q = c.q; a.k_pool = c.k_pool; a.v_pool = c.v_pool; a.out = c.out; a.seq_start = c.seq_start; a.past = c.past; a.counts = c.counts;
   a.seen = (const uint32_t*)c.seen; a.positions = c.positions; a.block_table = c.block_table; a.table_stride = c.table_stride; a.n_seqs = c.n_seqs;
   a.heads = c.heads; a.kv_heads = c.kv_heads; a.head_dim = c.head_dim; a.window = c.window; a.words = c.words; a.max_count = c.max_count;
-  a.tokens = c.tokens; a.scale = c.scale; a.scratch = c.scratch;
+  a.tokens = c.tokens; a.pool_pages = c.pool_pages; a.scale = c.scale; a.scratch = c.scratch;
   a.max_keys = c.max_keys > 0 && c.max_keys < table_rows ? c.max_keys : (int)table_rows;
   const long long need = slb_attention_tree_scratch(c.tokens, c.n_seqs, c.max_count, c.heads, c.kv_heads, c.head_dim, a.max_keys, c.dtype);
   SLB_REQUIRE(need == 0 || (c.scratch != nullptr && c.scratch_floats >= need), "attention_tree: the step needs %lld floats of scratch, %lld were given", need,

@@ -158,7 +158,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t base = smem_addr(smem);
   if ((base & 1023u) != 0) {
-    if (tid == 0) atomicExch(ta.status, 91);
+    if (tid == 0) atomicExch(ta.status, 111);
     return;
   }
   const uint32_t sK = base + L.k_off, sV = base + L.v_off, bars = base + L.bar_off;
@@ -277,7 +277,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         }
       }
     }
-    if (!ok && lane == 0) atomicExch(ta.status, 92);
+    if (!ok && lane == 0) atomicExch(ta.status, 112);
     // copies under way land before the block goes
     for (int i = 0; i < L.stages; ++i) {
       if (st == 0) { st = L.stages; --lap; }
@@ -293,17 +293,17 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       int st = 0, lap = 0, x = 0;
       for (int seg = 0;; ++seg) {
         const int qb = L.queries == 2 ? seg & 1 : 0, q_lap = L.queries == 2 ? seg >> 1 : seg;
-        if (!mbar_wait(q_full + 8 * qb, q_lap & 1)) { atomicExch(ta.status, 93); break; }
+        if (!mbar_wait(q_full + 8 * qb, q_lap & 1)) { atomicExch(ta.status, 113); break; }
         const int n = desc[qb].n;
         const bool dual = desc[qb].rows > kTtRows;
         if (n == 0) break;
         bool ok = true;
         for (int i = 0; i < n && ok; ++i) {
-          if (!mbar_wait(k_full + 8 * st, lap & 1)) { atomicExch(ta.status, 94); ok = false; break; }
+          if (!mbar_wait(k_full + 8 * st, lap & 1)) { atomicExch(ta.status, 114); ok = false; break; }
           for (int d = 0; d < (dual ? 2 : 1); ++d, ++x) {
             const int g = x & 1, c = x >> 1, b = c & 1;
             // S lands where S and then P of two items ago lay: the product that read that P must be through
-            if (c >= 2 && !mbar_wait(pv_done + 8 * (2 * g + b), ((c >> 1) - 1) & 1)) { atomicExch(ta.status, 95); ok = false; break; }
+            if (c >= 2 && !mbar_wait(pv_done + 8 * (2 * g + b), ((c >> 1) - 1) & 1)) { atomicExch(ta.status, 115); ok = false; break; }
             tc_fence_after();
             const uint32_t q = base + qb * L.q_bytes + (dual ? g * (kTtRows * 128) : 0);
 #pragma unroll
@@ -330,19 +330,19 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       int st = 0, lap = 0, x = 0;
       for (int seg = 0;; ++seg) {
         const int qb = L.queries == 2 ? seg & 1 : 0, q_lap = L.queries == 2 ? seg >> 1 : seg;
-        if (!mbar_wait(q_full + 8 * qb, q_lap & 1)) { atomicExch(ta.status, 96); break; }
+        if (!mbar_wait(q_full + 8 * qb, q_lap & 1)) { atomicExch(ta.status, 116); break; }
         const int n = desc[qb].n;
         const bool dual = desc[qb].rows > kTtRows;
         if (n == 0) break;
         mbar_arrive(q_free + 8 * qb);
-        if (seg > 0 && !mbar_wait(o_free, (seg - 1) & 1)) { atomicExch(ta.status, 96); break; }
+        if (seg > 0 && !mbar_wait(o_free, (seg - 1) & 1)) { atomicExch(ta.status, 116); break; }
         uint32_t fresh = 3u;      // groups without a product in this segment
         bool ok = true;
         for (int i = 0; i < n && ok; ++i) {
-          if (!mbar_wait(v_full + 8 * st, lap & 1)) { atomicExch(ta.status, 97); ok = false; break; }
+          if (!mbar_wait(v_full + 8 * st, lap & 1)) { atomicExch(ta.status, 117); ok = false; break; }
           for (int d = 0; d < (dual ? 2 : 1); ++d, ++x) {
             const int g = x & 1, c = x >> 1, b = c & 1;
-            if (!mbar_wait(p_full + 8 * (2 * g + b), (c >> 1) & 1)) { atomicExch(ta.status, 98); ok = false; break; }
+            if (!mbar_wait(p_full + 8 * (2 * g + b), (c >> 1) & 1)) { atomicExch(ta.status, 118); ok = false; break; }
             tc_fence_after();
 #pragma unroll
             for (int k4 = 0; k4 < 4; ++k4) {
@@ -366,7 +366,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       const int qb = L.queries == 2 ? seg & 1 : 0, q_lap = L.queries == 2 ? seg >> 1 : seg;
       const bool more = run.next(a);
       if (q_lap > 0 && !mbar_wait(q_free + 8 * qb, (q_lap - 1) & 1)) {
-        if (lane == 0) atomicExch(ta.status, 103);
+        if (lane == 0) atomicExch(ta.status, 123);
         break;
       }
       const uint32_t q = base + qb * L.q_bytes;
@@ -429,7 +429,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         __syncwarp();
         asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 11, 512, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(any) : "r"(lost) : "memory");
         if (any) {
-          if (stid == 0) atomicExch(ta.status, 104);
+          if (stid == 0) atomicExch(ta.status, 124);
           break;
         }
       }
@@ -461,7 +461,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         }
         const int c = (dual ? x - 2 + ((x & 1) != g) : x - 1) >> 1, b = c & 1;      // the item's number among the group's
         const int key_page = key_first + i * 64, key0 = key_page + half * 32;
-        wait_warp(s_full + 8 * (2 * g + b), (c >> 1) & 1, 99);
+        wait_warp(s_full + 8 * (2 * g + b), (c >> 1) & 1, 119);
         const bool mixed = key_page + 63 >= past || key_page < lo_most;      // not all rows see all of the page
         uint32_t seen = 0xffffffffu;
         if (warp_live) {
@@ -496,7 +496,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
           const float m_new = fmaxf(m_used, mx * ta.scale_log2);      // the scale is positive
           const bool grow = m_new > m_used + kTtRescale;              // also true for the first finite maximum
           if (done > 0 && __any_sync(0xffffffffu, grow)) {
-            wait_warp(pv_done + 8 * (2 * g + (b ^ 1)), ((c - 1) >> 1) & 1, 100);      // O must hold all of the last product
+            wait_warp(pv_done + 8 * (2 * g + (b ^ 1)), ((c - 1) >> 1) & 1, 120);      // O must hold all of the last product
             tc_fence_after();
             const float alpha = grow ? tt_ex2(m_used - m_new) : 1.0f;
 #pragma unroll 1
@@ -528,7 +528,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         if (mixed) {
           // values that are not finite go; rows that see one remember it. Two groups on one page look together, since what one has taken out the other would miss
           const int st = page_no % L.stages, lap = page_no / L.stages;
-          wait_warp(v_full + 8 * st, lap & 1, 101);
+          wait_warp(v_full + 8 * st, lap & 1, 121);
           const int held = past + w.s.count - key_page;      // rows of the page that belong to the sequence
           uint32_t* odd = dual ? s_odd[2][looked[1]++ & 1] : s_odd[g][looked[0]++ & 1];
           bool wrote = false;
@@ -576,7 +576,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       auto items = [&](int group) { return dual ? n : (n + (((first_item & 1) == group) ? 1 : 0)) / 2; };      // of a group in the segment
       auto wait_done = [&](int group) {      // its last one
         const int last = (x - 1 - (((x - 1) & 1) != group)) >> 1;
-        wait_warp(pv_done + 8 * (2 * group + (last & 1)), (last >> 1) & 1, 102);
+        wait_warp(pv_done + 8 * (2 * group + (last & 1)), (last >> 1) & 1, 122);
       };
       if (live) ml[(g * 2 + half) * kTtRows + r] = make_float4(m_used, l, poisoned ? 1.0f : 0.0f, 0.0f);
       look_sync(true);

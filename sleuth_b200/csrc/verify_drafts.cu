@@ -228,7 +228,7 @@ __device__ __forceinline__ float floor_of(const VerifyArgs& a, size_t t) {
 
 constexpr int kStatsThreads = 256, kStatsStep = 4096;      // tokens that a block holds at once, the next ones on their way
 // A piece of the row of a node that has children: `steps` steps. A thread's sum is relative to its own largest logit, in units of log2 after the temperature.
-__global__ void __launch_bounds__(kStatsThreads) verify_stats_kernel(VerifyArgs a) {
+__global__ void __launch_bounds__(kStatsThreads, 5) verify_stats_kernel(VerifyArgs a) {
   pdl_enter();
   __shared__ float top_s[kStatsThreads / 32];
   __shared__ int best_s[kStatsThreads / 32];
@@ -776,7 +776,7 @@ extern "C" int slb_verify_drafts(const VerifyCall* call) {
   SLB_REQUIRE(c.max_count > 0 && c.max_count <= kMostNodes, "verify_drafts: %d nodes of a sequence; 1 to %d are taken", c.max_count, kMostNodes);
   SLB_REQUIRE(c.path_width >= c.max_count, "verify_drafts: paths of %d places do not hold %d nodes", c.path_width, c.max_count);
   SLB_REQUIRE(c.temperature < INFINITY, "verify_drafts: the temperature must be finite");
-  SLB_REQUIRE(!(c.temperature > 0.0) || c.uniforms != nullptr, "verify_drafts: a temperature needs the random numbers");
+  SLB_REQUIRE(!(c.temperature > 0.0) || c.uniforms != nullptr || c.rows == 0, "verify_drafts: a temperature needs the random numbers");
   if (c.n_seqs == 0) return 0;
   VerifyArgs a{};
   a.logits = c.logits; a.probs = c.probs; a.floors = c.floors; a.uniforms = c.uniforms; a.tokens = c.tokens; a.parents = c.parents; a.seq_start = c.seq_start;

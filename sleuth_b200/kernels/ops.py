@@ -817,7 +817,8 @@ def gemm_tc_check(device) -> None:
                            f"chunk, 63 = loaded chunk, 64 = multiplied chunk, 65 = up values; streamed product: 71 = free slice, 72 = loaded slice, "
                            f"73 = finished sums; attention over a bounded cache, few tokens: 81 = shared memory misaligned, 82 = a free stage, 83 = a "
                            f"loaded stage; its weights: 84 = shared memory misaligned, 85-89 = producer and MMA waits, 90 = finished scores; 99 = the wait "
-                           f"probe of the tests); "
+                           f"probe of the tests; attention of drafted tokens: 111 = shared memory misaligned, 112 = a free stage, 113-118 = MMA "
+                           f"waits, 119-122 = softmax waits, 123 = free queries, 124 = a segment that did not come); "
                            f"its results are not valid")
 
 
@@ -1891,6 +1892,11 @@ _DRAFT_TREE_CALL = struct.Struct("7Qq4i")    # DraftTreeCall in csrc/draft_tree.
 _COMPACT_CALL = struct.Struct("7Q3q6i")      # CompactCall there
 
 
+def _on_current_device(what: str, t) -> None:
+    """A launch goes to the current device, whichever the tensors are on."""
+    _need(t.get_device() == torch._C._cuda_getDevice(), f"{what}: the tensors are on cuda:{t.get_device()}, which is not the current device")
+
+
 def _fits_int(what: str, *values: int) -> None:
     _need(all(-(1 << 31) <= int(v) < 1 << 31 for v in values), f"{what}: a number is out of range")
 
@@ -1917,6 +1923,7 @@ def draft_tree(parents, seq_start, past, counts, seen, positions, max_count: int
             (lambda: 0 < max_count <= MOST_NODES, f"{max_count} nodes of a sequence; 1 to {MOST_NODES} are taken"),
             (lambda: rows >= T and positions.numel() >= T and words * 32 >= max_count, "seen is [tokens, words] with a bit for each of max_count nodes, positions is [tokens]"),
             (lambda: window >= 0, "the window is not negative")))
+    _on_current_device("draft_tree", parents)
     try:
         call = _DRAFT_TREE_CALL.pack(parents.data_ptr(), seq_start.data_ptr(), past.data_ptr(), counts.data_ptr(), seen.data_ptr(), positions.data_ptr(),
                                      stream if stream is not None else current_stream(), T, n, max_count, words, window)
@@ -1947,7 +1954,8 @@ def attention_tree(q, k_pool, v_pool, out, seq_start, past, counts, seen, positi
     ``window`` those above ``positions`` [tokens] - window alone (without one ``positions`` may be None; a position below ``past`` counts as ``past``), and of the step's rows the
     ones whose bit is set in its row of ``seen`` [tokens, words] int32 (``draft_tree`` makes both; any bits are taken). float32 or bfloat16, even
     ``head_dim`` up to 256; softmax and sums in float32. ``max_keys``: a promise that no sequence has more rows after the step (0: as many as its table
-    holds). ``scratch``: ``attention_tree_scratch_floats`` floats. A node that sees nothing gives zeros. Rows that a node does not see never reach its result, whatever they hold."""
+    holds). ``scratch``: ``attention_tree_scratch_floats`` floats. A node that sees nothing gives zeros. Rows that a node does not see never reach its result, whatever they hold;
+    rows of a page that the pool has not read as zeros."""
     dt, i32 = q.dtype, torch.int32
     q_shape, k_shape, t_shape = q.shape, k_pool.shape, block_table.shape
     _need(len(q_shape) == 3 and len(k_shape) == 4 and len(t_shape) == 2 and seen.dim() == 2,
@@ -1980,6 +1988,7 @@ def attention_tree(q, k_pool, v_pool, out, seq_start, past, counts, seen, positi
     status = _TC_STATUS.get(q.device)
     if status is None:
         status = _tc_status(q.device)
+    _on_current_device("attention_tree", q)
     try:
         call = _TREE_CALL.pack(q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), seq_start.data_ptr(), past.data_ptr(), counts.data_ptr(),
                                seen.data_ptr(), 0 if positions is None else positions.data_ptr(), block_table.data_ptr(),
@@ -2041,6 +2050,7 @@ def verify_drafts(logits, limit: int, tokens, parents, seq_start, counts, unifor
             (lambda: uniforms.dtype == f32 and uniforms.numel() >= T if uniforms is not None else temperature <= 0, "uniforms are float32, one a node, and needed above temperature 0"),
             (lambda: floors is None or floors.dtype == f32 and floors.numel() >= T, "floors are float32, one a node"),
             (lambda: scratch is None or scratch.dtype == i32, "scratch is int32")))
+    _on_current_device("verify_drafts", logits)
     try:
         call = _VERIFY_CALL.pack(logits.data_ptr(), 0 if probs is None else probs.data_ptr(), 0 if floors is None else floors.data_ptr(),
                                  0 if uniforms is None else uniforms.data_ptr(), tokens.data_ptr(), parents.data_ptr(), seq_start.data_ptr(), counts.data_ptr(),
@@ -2057,7 +2067,7 @@ def cache_compact(k_pool, block_table, past, path, lengths, v_pool=None, stream=
     """The rows of the nodes that stay move together behind the rows from before the step, in every layer.
 
     For each sequence, i = 0 .. ``lengths`` - 1: the row ``past`` + ``path[i]`` becomes row ``past`` + i. ``path`` [n, places] int32 (at most 256 places) rises, from 0 or
-    above (``verify_drafts`` gives such); it ends in front of the first entry that does not. ``k_pool`` [..., pages, kv_heads, 64, width]: any number of layers,
+    above (``verify_drafts`` gives such); it ends in front of the first entry that does not, or that needs a page that the pool has not. ``k_pool`` [..., pages, kv_heads, 64, width]: any number of layers,
     or keys and values, in front, all with one block table; ``v_pool``: more layers, perhaps of another width. A sequence then holds ``past`` + ``lengths`` rows; what lies behind them is left as it was."""
     i32 = torch.int32
     shape, dt = k_pool.shape, k_pool.dtype
@@ -2080,6 +2090,7 @@ def cache_compact(k_pool, block_table, past, path, lengths, v_pool=None, stream=
     rows = pages * kv_heads * 64
     if rows == 0 or places == 0 or n == 0 or width == 0:
         return
+    _on_current_device("cache_compact", k_pool)
     try:
         call = _COMPACT_CALL.pack(k_pool.data_ptr(), 0 if v_pool is None else v_pool.data_ptr(), block_table.data_ptr(), past.data_ptr(), path.data_ptr(),
                                   lengths.data_ptr(), stream if stream is not None else current_stream(), k_pool.numel() // (rows * width),

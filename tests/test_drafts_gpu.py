@@ -290,6 +290,121 @@ def test_long_window_and_large_positions():
     assert torch.isfinite(out).all() and none.T == step.T
 
 
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim", [HEADS[0], HEADS[5], HEADS[6]], ids=[IDS[i] for i in (0, 5, 6)])
+def test_pages_that_the_pool_has_not_read_as_zeros(dtype, heads, kv_heads, dim):
+    step = Step(dtype, heads, kv_heads, dim, [200, 70], [5, 9], "random", 0, seed=12)
+    for s, i, bad in ((0, 1, -1), (0, 2, 10 ** 6), (1, 0, step.k.shape[0])):
+        page = int(step.table[s, i])
+        step.k[page], step.v[page] = 0, 0
+        step.table[s, i] = bad
+    out = step.run()
+    for s, i in ((0, 1), (0, 2), (1, 0)):      # what the oracle reads there: pages of zeros
+        step.table[s, i] = step.k.shape[0]
+    step.k, step.v = (torch.cat([t, torch.zeros_like(t[:1])]) for t in (step.k, step.v))
+    want, size, slack = step.want()
+    rel = slack[..., None] + ((1 + 2.0 ** -8) ** 2 - 1 if dtype == torch.bfloat16 else 2.0 ** -23)
+    assert bool(((out - want).abs() <= rel * size + 1e-30).all())
+
+
+def test_counts_beyond_the_given_tokens_write_nothing_there():
+    from sleuth_b200.kernels import ops
+    for dtype in (torch.float32, torch.bfloat16):
+        q, pool = torch.randn((6, 2, 64), device=DEV).to(dtype), torch.randn((3, 1, 64, 64), device=DEV).to(dtype)
+        memory = torch.full((9, 128), 7.0, dtype=dtype, device=DEV)
+        seen = torch.full((6, 1), -1, dtype=torch.int32, device=DEV)
+        floats = ops.attention_tree_scratch_floats(6, 3, 8, 2, 1, 64, 64, dtype)
+        scratch = torch.zeros(max(1, floats), device=DEV)
+        ops.attention_tree(q, pool, pool, memory[:6], i32([0, 4, 30]), i32([3, 3, 3]), i32([4, 8, 8]), seen, None, i32([[0], [1], [2]]), 8, 2, 1, 64, 0, 0.1, scratch=scratch)
+        assert bool((memory[6:] == 7.0).all()) and torch.isfinite(memory).all() and not bool((memory[:6] == 7.0).all(1).any())
+
+
+def test_refused_calls():
+    from sleuth_b200.kernels import ops
+    z = lambda *shape, t=torch.int32: torch.zeros(shape, dtype=t, device=DEV)  # noqa: E731
+    bf, f32 = torch.bfloat16, torch.float32
+
+    def attention(error, match, **kw):
+        a = dict(q=z(4, 4, 64, t=bf), k_pool=z(2, 2, 64, 64, t=bf), v_pool=z(2, 2, 64, 64, t=bf), out=z(4, 256, t=bf), seq_start=z(1), past=z(1), counts=z(1), seen=z(4, 1),
+                 positions=z(4), block_table=z(1, 2), max_count=4, heads=4, kv_heads=2, head_dim=64, window=0, scale=0.1, scratch=z(1 << 20, t=f32))
+        a.update(kw)
+        with pytest.raises(error, match=match):
+            ops.attention_tree(**a)
+
+    attention(ValueError, "contiguous", q=z(4, 4, 128, t=bf)[..., ::2])
+    attention(ValueError, "alike", out=z(4, 256, t=f32))
+    attention(ValueError, "pools", v_pool=z(2, 2, 64, 32, t=bf))
+    attention(ValueError, "heads", heads=8)
+    attention(ValueError, "nodes", max_count=257, seen=z(4, 9))
+    attention(ValueError, "bit", max_count=33)
+    attention(ValueError, "int32", counts=z(1, t=torch.int64))
+    attention(ValueError, "positions", window=5, positions=None)
+    attention(ValueError, "window", window=-1)
+    attention(ValueError, "scale", scale=0.0)
+    attention(ValueError, "range", window=2 ** 31)
+    attention(ValueError, "range", max_keys=2 ** 40)
+    attention(RuntimeError, "scratch", scratch=None, max_keys=0, block_table=z(1, 4000))
+    attention(RuntimeError, "heads", q=z(4, 3, 64, t=bf), heads=3, out=z(4, 192, t=bf))
+    attention(RuntimeError, "head_dim", q=z(4, 4, 65, t=f32), k_pool=z(2, 2, 64, 65, t=f32), v_pool=z(2, 2, 64, 65, t=f32), out=z(4, 260, t=f32), head_dim=65)
+    attention(RuntimeError, "aligned", q=z(4 * 4 * 64 + 1, t=bf)[1:].view(4, 4, 64))
+
+    def tree(match, **kw):
+        a = dict(parents=z(4), seq_start=z(2), past=z(1), counts=z(1), seen=z(4, 1), positions=z(4), max_count=4)
+        a.update(kw)
+        with pytest.raises(ValueError, match=match):
+            ops.draft_tree(**a)
+
+    tree("int32", parents=z(4, t=torch.int64))
+    tree("row a sequence", counts=z(2))
+    tree("bit", seen=z(3, 1))
+    tree("bit", max_count=40)
+    tree("nodes", max_count=0)
+    tree("window", window=-3)
+    tree("range", window=2 ** 31)
+    tree("contiguous", seen=z(4, 2)[:, :1])
+
+    def verify(match, error=ValueError, **kw):
+        a = dict(logits=z(4, 50, t=f32), limit=50, tokens=z(4), parents=z(4), seq_start=z(1), counts=z(1), uniforms=z(4, t=f32), temperature=1.0, path=z(1, 4), lengths=z(1), chosen=z(1),
+                 max_count=4, scratch=z(100))
+        a.update(kw)
+        with pytest.raises(error, match=match):
+            ops.verify_drafts(**a)
+
+    verify("limit", limit=51)
+    verify("limit", probs=z(3, 50, t=f32))
+    verify("float32", logits=z(4, 50, t=bf))
+    verify("stride", logits=z(4, 100, t=f32)[:, ::2])
+    verify("temperature", temperature=math.inf)
+    verify("temperature", temperature=math.nan)
+    verify("uniforms", uniforms=None)
+    verify("floors", floors=z(3, t=f32))
+    verify("path", path=z(1, 3))
+    verify("nodes", max_count=300, path=z(1, 300))
+    verify("int32", tokens=z(4, t=torch.int64))
+    verify("value for each", tokens=z(3))
+    verify("scratch", error=RuntimeError, scratch=None)
+
+    def compact(match, **kw):
+        a = dict(k_pool=z(2, 2, 1, 64, 8, t=bf), block_table=z(1, 2), past=z(1), path=z(1, 4), lengths=z(1))
+        a.update(kw)
+        with pytest.raises(ValueError, match=match):
+            ops.cache_compact(**a)
+
+    compact("pools", k_pool=z(2, 1, 32, 8, t=bf))
+    compact("four", k_pool=z(2, 1, 64, 7, t=bf))
+    compact("v_pool", v_pool=z(3, 1, 64, 8, t=bf))
+    compact("at most", path=z(1, 257))
+    compact("int32", past=z(1, t=torch.int64))
+    compact("contiguous", k_pool=z(2, 1, 64, 16, t=bf)[..., :8])
+    # nothing to do is no mistake
+    ops.draft_tree(z(0), z(1), z(0), z(0), z(0, 1), z(0), 1)
+    ops.cache_compact(z(2, 1, 64, 8, t=bf), z(0, 2), z(0), z(0, 4), z(0))
+    ops.verify_drafts(z(0, 50, t=f32), 50, z(0), z(0), z(0), z(0), z(0, t=f32), 1.0, z(0, 4), z(0), z(0), 4)
+    lengths, chosen, path = z(2) + 9, z(2) + 9, z(2, 4) + 9
+    ops.verify_drafts(z(0, 50, t=f32), 50, z(0), z(0), z(3), z(2), z(0, t=f32), 1.0, path, lengths, chosen, 4)
+    assert lengths.tolist() == [0, 0] and chosen.tolist() == [-1, -1] and bool((path == -1).all())
+    ops.attention_tree(z(0, 4, 64, t=bf), z(2, 2, 64, 64, t=bf), z(2, 2, 64, 64, t=bf), z(0, 256, t=bf), z(1), z(0), z(0), z(0, 1), None, z(0, 2), 4, 4, 2, 64, 0, 0.1)
+
+
 # ------------------------------------------------------------------ verification ----
 
 class Judged:
@@ -470,6 +585,14 @@ def test_compaction_ends_where_a_path_does_not_rise():
     got = pool.to(DEV)
     ops.cache_compact(got, table.to(DEV), i32([10, 0, 5]), path.to(DEV), i32([4, 9, 4]))
     plain.compact(pool, table, [10, 0, 5], [[0, 2], [1, 3], [0, 4]])
+    assert torch.equal(got.cpu(), pool)
+    # nor where a row lies on a page that the pool has not
+    pool = torch.randn((2, 3, 1, 64, 8))
+    table = torch.tensor([[0, -1], [1, 3], [2, 0]], dtype=torch.int32)
+    path = torch.tensor([[0, 2, 3, 20], [1, 9, 10, 11], [0, 3, 9, 10]], dtype=torch.int32)
+    got = pool.to(DEV)
+    ops.cache_compact(got, table.to(DEV), i32([60, 57, 60]), path.to(DEV), i32([4, 4, 4]))
+    plain.compact(pool, table, [60, 57, 60], [[0, 2, 3], [1], [0, 3, 9, 10]])
     assert torch.equal(got.cpu(), pool)
 
 
