@@ -26,7 +26,7 @@
 
 namespace slb {
 
-constexpr int kTtRows = 128, kTtTile = 256, kTtThreads = 20 * 32;
+constexpr int kTtRows = 128, kTtTile = 256, kTtThreads = 20 * 32, kTtSoftmax = 4 * 32;      // (the first thread of the softmax)
 constexpr float kTtRescale = 8.0f;      // log2 units by which a maximum may be stale
 
 __device__ __forceinline__ float tt_ex2(float x) {
@@ -170,7 +170,6 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (lane < 12) (&s_odd[0][0][0])[lane] = 0u;
     if (lane < 2) s_lo[lane] = 0;
-    if (!CLUSTER && lane == 0) ta.info[blockIdx.x] = make_int2(0, 0);
   }
   if (warp == 2) {
     __syncwarp();
@@ -178,6 +177,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   pdl_wait();
+  if (!CLUSTER && tid == kTtSoftmax) ta.info[blockIdx.x] = make_int2(0, 0);      // (by the thread that may write it again; the scratch may have been another kernel's until now)
 
   // where this block's run of units begins
   const int G = a.heads / a.kv_heads;
@@ -252,7 +252,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     while (ok && run.next(a)) {
       const int* table = a.block_table + (size_t)run.seq * a.table_stride + run.s.page_lo + run.off;
       for (int i0 = 0; i0 < run.n && ok; i0 += 32) {
-        const int mine = i0 + lane < run.n ? table[i0 + lane] : 0;
+        int mine = i0 + lane < run.n ? table[i0 + lane] : 0;
+        if (mine < 0 || mine >= a.pool_pages) mine = -1;      // (rows in front of the pool: zeros; another page's number times its rows might come back into it)
         for (int i = 0; i < min(32, run.n - i0) && ok; ++i) {
           const int row = (__shfl_sync(0xffffffffu, mine, i) * a.kv_heads + run.kh) * 64;
           if (lap > 0 && !mbar_wait(k_free + 8 * st, (lap - 1) & 1)) { ok = false; break; }
@@ -397,7 +398,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     }
   } else {
     // ---- softmax: tensor-memory lanes 32 (warp % 4) .. + 31 hold the rows; two warps share them, keys 0..31 and 32..63 of a page ----
-    const int quad = warp & 3, g = (warp - 4) >> 3, half = (warp - 4) >> 2 & 1, r = quad * 32 + lane, stid = tid - 128, gtid = stid & 255;
+    const int quad = warp & 3, g = (warp - 4) >> 3, half = (warp - 4) >> 2 & 1, r = quad * 32 + lane, stid = tid - kTtSoftmax, gtid = stid & 255;
     const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16), own = lane_addr + g * 256;
     uint32_t* poison = reinterpret_cast<uint32_t*>(smem + L.poison_off) + (g * kTtRows + r) * WORDS;      // [2 groups][128 rows][WORDS]; of the other group: other_poison words on
     const int other_poison = g ? -kTtRows * WORDS : kTtRows * WORDS;

@@ -389,7 +389,7 @@ struct Verifier {
       const float top = warp_max(mine.top);
       const double z = warp_sum_f64(mine.top > -INFINITY ? mine.z * rough_exp(a, mine.top, top) : 0.0);
       const int best = __reduce_min_sync(0xffffffffu, mine.top == top ? mine.best : 0x7fffffff);
-      if (lane == 0) s.stat[node] = VerifyStat{top, best == 0x7fffffff ? 0 : best, z};
+      if (lane == 0) s.stat[node] = VerifyStat{top, top > -INFINITY ? best : 0, z};
     }
   }
 
@@ -419,7 +419,7 @@ struct Verifier {
       bv = -INFINITY;
       bi = 0x7fffffff;
       for (int r = 0; r < a.team; ++r) better(peer_f32(peer(&s.x.max[flip], r)), __float_as_int(peer_f32(peer(&s.x.best[flip], r))));
-      s.best = bi == 0x7fffffff ? 0 : bi;
+      s.best = bv > -INFINITY ? bi : 0;
     }
     __syncthreads();
     flip ^= 1;

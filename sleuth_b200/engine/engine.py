@@ -218,6 +218,10 @@ class Engine:
         """Tokens of the sequence so far."""
         return int(self.cache.book.seen[slot])
 
+    @property
+    def max_step_tokens(self) -> int:
+        return self.stepper.max_step_tokens
+
     def sync(self) -> None:
         torch.cuda.synchronize(self.device)
 

@@ -66,7 +66,8 @@ class Backend(Protocol):
     #       the tokens also stay on the device, row i of them in feed slot i
     #   decode_fed(slots, feed_map) -> logits: sequence i continues with the token in feed slot feed_map[i]
     # optional, for drafted tokens (sampling/drafts.py):
-    #   step_tree([(slot, tokens, parents)]) -> logits of every node; accept(slots, paths): the nodes of each that stay
+    #   step_tree([(slot, tokens, parents)]) -> logits of every node; accept(slots, paths): the nodes of each that stay;
+    #   max_step_tokens: tokens of such a step, at most
 
 
 @dataclass
@@ -307,7 +308,9 @@ def _run_batch_drafted(backend, batch, prompts, results, max_new_tokens, samplin
             if not live:
                 break
             # (a draft behind the last token that there is room for would be judged for nothing)
-            rooms = [min(max_new_tokens - len(q.new), backend.max_len - backend.length(q.slot)) - 1 for q in live]
+            step = getattr(backend, "max_step_tokens", None)
+            share = drafts.tokens if step is None else step // len(live) - 1
+            rooms = [min(share, min(max_new_tokens - len(q.new), backend.max_len - backend.length(q.slot)) - 1) for q in live]
             trees = []
             for q, room in zip(live, rooms):
                 more, parents = q.drafter.propose(room)

@@ -1901,6 +1901,14 @@ def _fits_int(what: str, *values: int) -> None:
     _need(all(-(1 << 31) <= int(v) < 1 << 31 for v in values), f"{what}: a number is out of range")
 
 
+def _plain_on(t, dev: int) -> bool:
+    return t is None or (t.get_device() == dev and t.is_contiguous())
+
+
+def _one_device(dev: int, *tensors) -> bool:
+    return all(t is None or t.get_device() == dev for t in tensors)
+
+
 def draft_tree(parents, seq_start, past, counts, seen, positions, max_count: int, window: int = 0, stream=None) -> None:
     """What each drafted node sees of its step, and its position, from the nodes' parents.
 
@@ -1912,12 +1920,14 @@ def draft_tree(parents, seq_start, past, counts, seen, positions, max_count: int
     n, T = past.numel(), parents.numel()
     _need(seen.dim() == 2, "draft_tree: seen is [tokens, words]")
     rows, words = seen.shape
-    if not (parents.is_cuda and parents.is_contiguous() and seq_start.is_cuda and seq_start.is_contiguous() and past.is_cuda and past.is_contiguous()
-            and counts.is_cuda and counts.is_contiguous() and seen.is_cuda and seen.is_contiguous() and positions.is_cuda and positions.is_contiguous()
+    dev = parents.get_device()
+    if not (dev >= 0 and parents.is_contiguous() and seq_start.get_device() == dev and seq_start.is_contiguous() and past.get_device() == dev and past.is_contiguous()
+            and counts.get_device() == dev and counts.is_contiguous() and seen.get_device() == dev and seen.is_contiguous() and positions.get_device() == dev and positions.is_contiguous()
             and i32 == parents.dtype == seq_start.dtype == past.dtype == counts.dtype == seen.dtype == positions.dtype
             and seq_start.numel() >= n and counts.numel() == n and rows >= T and positions.numel() >= T and words * 32 >= max_count
             and 0 < max_count <= MOST_NODES and window >= 0):
         _kept_refusal("draft_tree", dict(parents=parents, seq_start=seq_start, past=past, counts=counts, seen=seen, positions=positions), (
+            (lambda: _one_device(dev, seq_start, past, counts, seen, positions), "all tensors are on one device"),
             (lambda: i32 == parents.dtype == seq_start.dtype == past.dtype == counts.dtype == seen.dtype == positions.dtype, "all tensors are int32"),
             (lambda: seq_start.numel() >= n and counts.numel() == n, "seq_start, past and counts have one row a sequence"),
             (lambda: 0 < max_count <= MOST_NODES, f"{max_count} nodes of a sequence; 1 to {MOST_NODES} are taken"),
@@ -1961,10 +1971,11 @@ def attention_tree(q, k_pool, v_pool, out, seq_start, past, counts, seen, positi
     _need(len(q_shape) == 3 and len(k_shape) == 4 and len(t_shape) == 2 and seen.dim() == 2,
           "attention_tree: q is [tokens, heads, head_dim], pools are [pages, kv_heads, 64, head_dim], block_table is [n, pages], seen is [tokens, words]")
     (n, stride), T = t_shape, q_shape[0]
-    if not (q.is_cuda and q.is_contiguous() and k_pool.is_cuda and k_pool.is_contiguous() and v_pool.is_cuda and v_pool.is_contiguous()
-            and out.is_cuda and out.is_contiguous() and seq_start.is_cuda and seq_start.is_contiguous() and past.is_cuda and past.is_contiguous()
-            and counts.is_cuda and counts.is_contiguous() and seen.is_cuda and seen.is_contiguous() and block_table.is_cuda and block_table.is_contiguous()
-            and _plain_cuda(positions) and _plain_cuda(scratch)
+    dev = q.get_device()
+    if not (dev >= 0 and q.is_contiguous() and k_pool.get_device() == dev and k_pool.is_contiguous() and v_pool.get_device() == dev and v_pool.is_contiguous()
+            and out.get_device() == dev and out.is_contiguous() and seq_start.get_device() == dev and seq_start.is_contiguous() and past.get_device() == dev and past.is_contiguous()
+            and counts.get_device() == dev and counts.is_contiguous() and seen.get_device() == dev and seen.is_contiguous() and block_table.get_device() == dev and block_table.is_contiguous()
+            and _plain_on(positions, dev) and _plain_on(scratch, dev)
             and q_shape == (T, heads, head_dim) and out.shape == (T, heads * head_dim) and dt in DT
             and dt == out.dtype == k_pool.dtype == v_pool.dtype and k_shape == (k_shape[0], kv_heads, 64, head_dim) and k_shape == v_pool.shape
             and i32 == block_table.dtype == seq_start.dtype == past.dtype == counts.dtype == seen.dtype
@@ -1974,6 +1985,7 @@ def attention_tree(q, k_pool, v_pool, out, seq_start, past, counts, seen, positi
             and (positions is None and window == 0 or positions is not None and positions.dtype == i32 and positions.numel() >= T)):
         _kept_refusal("attention_tree", dict(q=q, k_pool=k_pool, v_pool=v_pool, out=out, seq_start=seq_start, past=past, counts=counts, seen=seen,
                                              positions=positions, block_table=block_table, scratch=scratch), (
+            (lambda: _one_device(dev, k_pool, v_pool, out, seq_start, past, counts, seen, positions, block_table, scratch), "all tensors are on one device"),
             (lambda: q_shape == (T, heads, head_dim) and out.shape == (T, heads * head_dim), "q is [tokens, heads, head_dim], out [tokens, heads * head_dim]"),
             (lambda: dt in DT and dt == out.dtype == k_pool.dtype == v_pool.dtype, "q, out and the pools are float32 or bfloat16 alike"),
             (lambda: k_shape == (k_shape[0], kv_heads, 64, head_dim) and k_shape == v_pool.shape, "pools are [pages, kv_heads, 64, head_dim]"),
@@ -2026,11 +2038,12 @@ def verify_drafts(logits, limit: int, tokens, parents, seq_start, counts, unifor
     i32, f32 = torch.int32, torch.float32
     _need(logits.dim() == 2 and path.dim() == 2 and (probs is None or probs.dim() == 2), "verify_drafts: logits, probs and path have two dimensions")
     n, (T, vocab), places = counts.numel(), logits.shape, path.shape[1]
-    if not (logits.is_cuda and logits.dtype == f32 and logits.stride(1) == 1 and 0 < limit <= vocab
-            and (probs is None or probs.is_cuda and probs.dtype == f32 and probs.stride(1) == 1 and probs.shape[0] >= T and probs.shape[1] >= limit)
-            and tokens.is_cuda and tokens.is_contiguous() and parents.is_cuda and parents.is_contiguous() and seq_start.is_cuda and seq_start.is_contiguous()
-            and counts.is_cuda and counts.is_contiguous() and path.is_cuda and path.is_contiguous() and lengths.is_cuda and lengths.is_contiguous()
-            and chosen.is_cuda and chosen.is_contiguous() and _plain_cuda(uniforms) and _plain_cuda(floors) and _plain_cuda(scratch)
+    dev = logits.get_device()
+    if not (dev >= 0 and logits.dtype == f32 and logits.stride(1) == 1 and 0 < limit <= vocab
+            and (probs is None or probs.get_device() == dev and probs.dtype == f32 and probs.stride(1) == 1 and probs.shape[0] >= T and probs.shape[1] >= limit)
+            and tokens.get_device() == dev and tokens.is_contiguous() and parents.get_device() == dev and parents.is_contiguous() and seq_start.get_device() == dev and seq_start.is_contiguous()
+            and counts.get_device() == dev and counts.is_contiguous() and path.get_device() == dev and path.is_contiguous() and lengths.get_device() == dev and lengths.is_contiguous()
+            and chosen.get_device() == dev and chosen.is_contiguous() and _plain_on(uniforms, dev) and _plain_on(floors, dev) and _plain_on(scratch, dev)
             and i32 == tokens.dtype == parents.dtype == seq_start.dtype == counts.dtype == path.dtype == lengths.dtype == chosen.dtype
             and tokens.numel() >= T and parents.numel() >= T and seq_start.numel() >= n and lengths.numel() >= n and chosen.numel() >= n
             and path.shape[0] >= n and places >= max_count and 0 < max_count <= MOST_NODES and temperature < math.inf
@@ -2040,6 +2053,7 @@ def verify_drafts(logits, limit: int, tokens, parents, seq_start, counts, unifor
             _need(t is None or t.is_cuda and t.dtype == f32 and t.stride(1) == 1, f"verify_drafts: {name} are float32 CUDA rows of unit column stride")
         _kept_refusal("verify_drafts", dict(tokens=tokens, parents=parents, seq_start=seq_start, counts=counts, path=path, lengths=lengths, chosen=chosen, uniforms=uniforms,
                                             floors=floors, scratch=scratch), (
+            (lambda: _one_device(dev, probs, tokens, parents, seq_start, counts, path, lengths, chosen, uniforms, floors, scratch), "all tensors are on one device"),
             (lambda: 0 < limit <= vocab and (probs is None or probs.shape[0] >= T and probs.shape[1] >= limit), "limit tokens of a row of logits and of probs, one row a node"),
             (lambda: i32 == tokens.dtype == parents.dtype == seq_start.dtype == counts.dtype == path.dtype == lengths.dtype == chosen.dtype, "tables and outputs are int32"),
             (lambda: tokens.numel() >= T and parents.numel() >= T, "tokens and parents have a value for each row of logits"),
@@ -2075,12 +2089,14 @@ def cache_compact(k_pool, block_table, past, path, lengths, v_pool=None, stream=
     (n, stride), places, size = block_table.shape, path.shape[1], 2 if dt == torch.bfloat16 else 4
     pages, kv_heads, page, width = shape[-4:]
     v_width = 0 if v_pool is None else v_pool.shape[-1]
-    if not (k_pool.is_cuda and k_pool.is_contiguous() and _plain_cuda(v_pool) and block_table.is_cuda and block_table.is_contiguous()
-            and past.is_cuda and past.is_contiguous() and path.is_cuda and path.is_contiguous() and lengths.is_cuda and lengths.is_contiguous()
+    dev = k_pool.get_device()
+    if not (dev >= 0 and k_pool.is_contiguous() and _plain_on(v_pool, dev) and block_table.get_device() == dev and block_table.is_contiguous()
+            and past.get_device() == dev and past.is_contiguous() and path.get_device() == dev and path.is_contiguous() and lengths.get_device() == dev and lengths.is_contiguous()
             and dt in DT and page == 64 and (v_pool is None or v_pool.dtype == dt and v_pool.dim() >= 4 and v_pool.shape[-4:-1] == shape[-4:-1])
             and i32 == block_table.dtype == past.dtype == path.dtype == lengths.dtype and past.numel() >= n and lengths.numel() >= n and path.shape[0] >= n
             and places <= MOST_NODES and width * size % 4 == 0 and v_width * size % 4 == 0):
         _kept_refusal("cache_compact", dict(k_pool=k_pool, v_pool=v_pool, block_table=block_table, past=past, path=path, lengths=lengths), (
+            (lambda: _one_device(dev, v_pool, block_table, past, path, lengths), "all tensors are on one device"),
             (lambda: dt in DT and page == 64, "pools are [..., pages, kv_heads, 64, width], float32 or bfloat16"),
             (lambda: v_pool is None or v_pool.dtype == dt and v_pool.dim() >= 4 and v_pool.shape[-4:-1] == shape[-4:-1], "v_pool has the type, pages and heads of k_pool"),
             (lambda: i32 == block_table.dtype == past.dtype == path.dtype == lengths.dtype and past.numel() >= n and lengths.numel() >= n and path.shape[0] >= n,

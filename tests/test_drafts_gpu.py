@@ -306,6 +306,23 @@ def test_pages_that_the_pool_has_not_read_as_zeros(dtype, heads, kv_heads, dim):
     assert bool(((out - want).abs() <= rel * size + 1e-30).all())
 
 
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim", [HEADS[0], HEADS[5], HEADS[6]], ids=[IDS[i] for i in (0, 5, 6)])
+def test_page_numbers_whose_rows_pass_32_bits_read_as_zeros(dtype, heads, kv_heads, dim):
+    """A number of pages that, times the rows of a page, comes round to the pool's own ones in 32 bits."""
+    step = Step(dtype, heads, kv_heads, dim, [200, 70], [5, 9], "random", 0, seed=12)
+    around = 2 ** 26 // (kv_heads & -kv_heads)
+    for s, i in ((0, 1), (1, 0)):
+        page = int(step.table[s, i])
+        step.table[s, i] = page + around
+    out = step.run()
+    for s, i in ((0, 1), (1, 0)):
+        step.table[s, i] = step.k.shape[0]
+    step.k, step.v = (torch.cat([t, torch.zeros_like(t[:1])]) for t in (step.k, step.v))
+    want, size, slack = step.want()
+    rel = slack[..., None] + ((1 + 2.0 ** -8) ** 2 - 1 if dtype == torch.bfloat16 else 2.0 ** -23)
+    assert bool(((out - want).abs() <= rel * size + 1e-30).all())
+
+
 def test_counts_beyond_the_given_tokens_write_nothing_there():
     from sleuth_b200.kernels import ops
     for dtype in (torch.float32, torch.bfloat16):
@@ -318,6 +335,16 @@ def test_counts_beyond_the_given_tokens_write_nothing_there():
         assert bool((memory[6:] == 7.0).all()) and torch.isfinite(memory).all() and not bool((memory[:6] == 7.0).all(1).any())
 
 
+class Elsewhere(torch.Tensor):
+    def get_device(self):
+        return 5
+
+
+def moved(a, moved=None, **kw):
+    a = {**a, **kw}
+    return a if moved is None else {**a, moved: a[moved].as_subclass(Elsewhere)}
+
+
 def test_refused_calls():
     from sleuth_b200.kernels import ops
     z = lambda *shape, t=torch.int32: torch.zeros(shape, dtype=t, device=DEV)  # noqa: E731
@@ -326,9 +353,8 @@ def test_refused_calls():
     def attention(error, match, **kw):
         a = dict(q=z(4, 4, 64, t=bf), k_pool=z(2, 2, 64, 64, t=bf), v_pool=z(2, 2, 64, 64, t=bf), out=z(4, 256, t=bf), seq_start=z(1), past=z(1), counts=z(1), seen=z(4, 1),
                  positions=z(4), block_table=z(1, 2), max_count=4, heads=4, kv_heads=2, head_dim=64, window=0, scale=0.1, scratch=z(1 << 20, t=f32))
-        a.update(kw)
         with pytest.raises(error, match=match):
-            ops.attention_tree(**a)
+            ops.attention_tree(**moved(a, **kw))
 
     attention(ValueError, "contiguous", q=z(4, 4, 128, t=bf)[..., ::2])
     attention(ValueError, "alike", out=z(4, 256, t=f32))
@@ -349,9 +375,8 @@ def test_refused_calls():
 
     def tree(match, **kw):
         a = dict(parents=z(4), seq_start=z(2), past=z(1), counts=z(1), seen=z(4, 1), positions=z(4), max_count=4)
-        a.update(kw)
         with pytest.raises(ValueError, match=match):
-            ops.draft_tree(**a)
+            ops.draft_tree(**moved(a, **kw))
 
     tree("int32", parents=z(4, t=torch.int64))
     tree("row a sequence", counts=z(2))
@@ -365,9 +390,8 @@ def test_refused_calls():
     def verify(match, error=ValueError, **kw):
         a = dict(logits=z(4, 50, t=f32), limit=50, tokens=z(4), parents=z(4), seq_start=z(1), counts=z(1), uniforms=z(4, t=f32), temperature=1.0, path=z(1, 4), lengths=z(1), chosen=z(1),
                  max_count=4, scratch=z(100))
-        a.update(kw)
         with pytest.raises(error, match=match):
-            ops.verify_drafts(**a)
+            ops.verify_drafts(**moved(a, **kw))
 
     verify("limit", limit=51)
     verify("limit", probs=z(3, 50, t=f32))
@@ -385,9 +409,8 @@ def test_refused_calls():
 
     def compact(match, **kw):
         a = dict(k_pool=z(2, 2, 1, 64, 8, t=bf), block_table=z(1, 2), past=z(1), path=z(1, 4), lengths=z(1))
-        a.update(kw)
         with pytest.raises(ValueError, match=match):
-            ops.cache_compact(**a)
+            ops.cache_compact(**moved(a, **kw))
 
     compact("pools", k_pool=z(2, 1, 32, 8, t=bf))
     compact("four", k_pool=z(2, 1, 64, 7, t=bf))
@@ -395,6 +418,15 @@ def test_refused_calls():
     compact("at most", path=z(1, 257))
     compact("int32", past=z(1, t=torch.int64))
     compact("contiguous", k_pool=z(2, 1, 64, 16, t=bf)[..., :8])
+    # one tensor after the other on another device (these say so alone)
+    for name in ("k_pool", "v_pool", "out", "seq_start", "past", "counts", "seen", "positions", "block_table", "scratch"):
+        attention(ValueError, "device", moved=name)
+    for name in ("seq_start", "past", "counts", "seen", "positions"):
+        tree("device", moved=name)
+    for name in ("probs", "tokens", "parents", "seq_start", "counts", "uniforms", "floors", "path", "lengths", "chosen", "scratch"):
+        verify("device", moved=name, probs=z(4, 50, t=f32), floors=z(4, t=f32))
+    for name in ("v_pool", "block_table", "past", "path", "lengths"):
+        compact("device", moved=name, v_pool=z(2, 2, 1, 64, 8, t=bf))
     # nothing to do is no mistake
     ops.draft_tree(z(0), z(1), z(0), z(0), z(0, 1), z(0), 1)
     ops.cache_compact(z(2, 1, 64, 8, t=bf), z(0, 2), z(0), z(0, 4), z(0))
@@ -503,6 +535,16 @@ def test_verification_of_odd_logits(temperature):
     j.tokens[13:15] = torch.tensor([400, -1], dtype=torch.int32)
     path, lengths, chosen = j.check()
     assert int(lengths[0]) >= 2 and int(chosen[1]) == 0 and int(lengths[2]) == 4 and int(lengths[3]) == 1
+
+
+def test_rows_without_a_number_above_minus_infinity_pick_token_0():
+    """Whether the row has children or not, and whatever stands in front of the first -inf."""
+    j = Judged([3, 1, 2], "chain", 300, 300, 0.0, False, seed=9)
+    j.logits[:] = -math.inf
+    j.logits[:, :3] = math.nan
+    j.tokens[:] = 3
+    path, lengths, chosen = j.run()
+    assert chosen.tolist() == [0, 0, 0] and lengths.tolist() == [1, 1, 1]
 
 
 @pytest.mark.parametrize("temperature", [0.0, 0.7])

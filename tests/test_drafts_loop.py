@@ -82,6 +82,17 @@ def test_drafts_change_nothing(policy, temperature, kw, script):
             assert runs[1][2].trees > 0 and sum(r.stats["drafts_taken"] for r in runs[1][0]) > 50
 
 
+@pytest.mark.parametrize("most", [3, 4, 7, 20])
+def test_a_step_brings_no_more_tokens_than_the_backend_takes(most):
+    prompts, runs = [[1, 2, 3] * 5, [4] * 9, [5, 6] * 6], []
+    for drafts in (None, DraftPolicy(8, 2)):
+        be = Drafting(circling, max_len=200, n_pages=64)
+        be.max_step_tokens, step, widest = most, be.step_tree, []
+        be.step_tree = lambda entries: (widest.append(sum(len(t) for _, t, _ in entries)), step(entries))[1]
+        runs.append([r.new_ids for r in generate_batches(be, prompts, 90, SamplingConfig(temperature=0.0), stop_ids={22}, seed=5, max_batch=3, drafts=drafts)])
+    assert runs[0] == runs[1] and max(widest, default=0) <= most and (most < 6 or widest)
+
+
 def test_drafts_and_penalties_do_not_go_together():
     with pytest.raises(ValueError, match="drafts"):
         generate_batches(Drafting(repeating), [[1]], 3, SamplingConfig(repetition_penalty=1.2), drafts=DraftPolicy())
