@@ -15,10 +15,13 @@
 namespace slb {
 
 constexpr int kTreeThreads = 256, kTreeRows = 16, kTreeKeys = 64;
+constexpr int kTreePitch = kTreeRows + 4;      // of a key's weights: 16-byte reads of four rows
 
 __host__ __device__ constexpr int tree_pad(int hd) { return (hd + 3) & ~3; }
+// A row's floats in shared memory: half the banks and a whole number of times all of them, so that two neighbouring keys' pieces of 64 bytes lie in different banks.
+__host__ __device__ constexpr int tree_row(int hd) { return ((hd + 31) & ~31) + 16; }
 __host__ __device__ constexpr int tree_smem(int hd) {
-  return (2 * kTreeKeys * (tree_pad(hd) + 4) + kTreeRows * tree_pad(hd) + kTreeRows * kTreeKeys + 2 * kTreeRows) * 4;
+  return ((2 * kTreeKeys + kTreeRows) * tree_row(hd) + kTreeKeys * kTreePitch + 2 * kTreeRows) * 4;
 }
 
 // Scratch of a share: per (share, token, head) hd weighted values, maximum, sum.
@@ -26,35 +29,53 @@ __device__ __forceinline__ float* tree_slot(const TreeArgs& a, int split, size_t
   return a.scratch + (((size_t)split * a.tokens + token) * a.heads + head) * (a.head_dim + 2);
 }
 
-// 64 rows of a pool from row `key0` on as float32 in shared memory, rows of hdp + 4 floats; zeros from row `end` on, and for pages that the pool has not (as TMA reads them).
+// Four channels of a row from channel c on, zeros behind the last one.
 template <typename T>
-__device__ __forceinline__ void tree_rows(float* dst, const T* pool, const TreeArgs& a, const int* table, int kh, int key0, int end) {
-  const int hd = a.head_dim, hdp = tree_pad(hd), r0 = threadIdx.x >> 4;
-  const bool whole = hd % 4 == 0 && (reinterpret_cast<uintptr_t>(pool) & (4 * sizeof(T) - 1)) == 0;
+__device__ __forceinline__ float4 tree_load(const T* src, int c, int hd, bool whole) {
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (whole) {
+    if constexpr (sizeof(T) == 4) {
+      v = *reinterpret_cast<const float4*>(src + c);
+    } else {
+      const uint2 p = *reinterpret_cast<const uint2*>(src + c);
+      const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&p.x)), y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&p.y));
+      v = make_float4(x.x, x.y, y.x, y.y);
+    }
+  } else {
+    v.x = to_f32(src[c]);
+    if (c + 1 < hd) v.y = to_f32(src[c + 1]);
+    if (c + 2 < hd) v.z = to_f32(src[c + 2]);
+    if (c + 3 < hd) v.w = to_f32(src[c + 3]);
+  }
+  return v;
+}
+
+// The page of rows key0 .. key0 + 63, keys and values, as float32 in shared memory: 64 channels of eight rows of each on their way at once. Zeros from row `end` on, and for a page that the
+// pool has not (as TMA reads them).
+template <typename T>
+__device__ __forceinline__ void tree_rows(float* ks, float* vs, const TreeArgs& a, const int* table, int kh, int key0, int end) {
+  const int hd = a.head_dim, hdp = tree_pad(hd), pitch = tree_row(hd), r0 = threadIdx.x >> 4;
+  const int page = table[key0 / kPageTokens];
+  const bool there = page >= 0 && page < a.pool_pages;
+  const size_t at = there ? ((size_t)page * a.kv_heads + kh) * kPageTokens * hd : 0;
+  const T *kp = (const T*)a.k_pool + at, *vp = (const T*)a.v_pool + at;
+  const bool whole = hd % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.k_pool) | reinterpret_cast<uintptr_t>(a.v_pool)) & (4 * sizeof(T) - 1)) == 0;
+#pragma unroll 1
+  for (int c = 4 * (threadIdx.x & 15); c < hdp; c += 64) {
+    float4 k[4], v[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int key = key0 + r0 + 16 * i;
-    const int page = key < end ? table[key / kPageTokens] : -1;
-    const T* src = page >= 0 && page < a.pool_pages ? pool + (((size_t)page * a.kv_heads + kh) * kPageTokens + key % kPageTokens) * hd : nullptr;
-    for (int c = 4 * (threadIdx.x & 15); c < hdp; c += 64) {
-      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (src) {
-        if (whole) {
-          if constexpr (sizeof(T) == 4) {
-            v = *reinterpret_cast<const float4*>(src + c);
-          } else {
-            const uint2 p = *reinterpret_cast<const uint2*>(src + c);
-            const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&p.x)), y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&p.y));
-            v = make_float4(x.x, x.y, y.x, y.y);
-          }
-        } else {
-          v.x = to_f32(src[c]);
-          if (c + 1 < hd) v.y = to_f32(src[c + 1]);
-          if (c + 2 < hd) v.z = to_f32(src[c + 2]);
-          if (c + 3 < hd) v.w = to_f32(src[c + 3]);
-        }
+    for (int i = 0; i < 4; ++i) {
+      const int r = r0 + 16 * i;
+      k[i] = v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (there && key0 + r < end) {
+        k[i] = tree_load(kp + (size_t)r * hd, c, hd, whole);
+        v[i] = tree_load(vp + (size_t)r * hd, c, hd, whole);
       }
-      *reinterpret_cast<float4*>(dst + (r0 + 16 * i) * (hdp + 4) + c) = v;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      *reinterpret_cast<float4*>(ks + (r0 + 16 * i) * pitch + c) = k[i];
+      *reinterpret_cast<float4*>(vs + (r0 + 16 * i) * pitch + c) = v[i];
     }
   }
 }
@@ -63,12 +84,12 @@ template <typename T>
 __global__ void __launch_bounds__(kTreeThreads) tree_general_kernel(TreeArgs a) {
   pdl_enter();
   extern __shared__ __align__(16) float smem[];
-  const int hd = a.head_dim, hdp = tree_pad(hd);
-  float* rows_s = smem;                                  // [64][hdp + 4]
-  float* values_s = rows_s + kTreeKeys * (hdp + 4);      // [64][hdp + 4]
-  float* q_s = values_s + kTreeKeys * (hdp + 4);         // [16][hdp]
-  float* p_s = q_s + kTreeRows * hdp;                    // [16][64]
-  float* alpha_s = p_s + kTreeRows * kTreeKeys;          // [16]
+  const int hd = a.head_dim, hdp = tree_pad(hd), pitch = tree_row(hd);
+  float* rows_s = smem;                                  // [64][pitch]
+  float* values_s = rows_s + kTreeKeys * pitch;          // [64][pitch]
+  float* q_s = values_s + kTreeKeys * pitch;             // [16][pitch]
+  float* p_s = q_s + kTreeRows * pitch;                  // [64][20]: a score, then a weight; below zero where the row does not see the key
+  float* alpha_s = p_s + kTreeKeys * kTreePitch;         // [16]
   float* l_s = alpha_s + kTreeRows;                      // [16]
   __shared__ unsigned long long bits_s[kTreeRows];
   __shared__ int lo_s[kTreeRows];
@@ -81,7 +102,7 @@ __global__ void __launch_bounds__(kTreeThreads) tree_general_kernel(TreeArgs a) 
   if (tid < kTreeRows) lo_s[tid] = r0 + tid < rows_total ? tree_lo(a, s.tok0 + (r0 + tid) / G, s.past) : s.past;
   for (int e = tid; e < kTreeRows * hdp; e += kTreeThreads) {
     const int r = e / hdp, c = e % hdp, R = r0 + r;
-    q_s[e] = R < rows_total && c < hd ? to_f32(((const T*)a.q)[((size_t)(s.tok0 + R / G) * a.heads + kh * G + R % G) * hd + c]) * a.scale : 0.0f;
+    q_s[r * pitch + c] = R < rows_total && c < hd ? to_f32(((const T*)a.q)[((size_t)(s.tok0 + R / G) * a.heads + kh * G + R % G) * hd + c]) * a.scale : 0.0f;
   }
   __syncthreads();
   int first = s.past;
@@ -91,16 +112,15 @@ __global__ void __launch_bounds__(kTreeThreads) tree_general_kernel(TreeArgs a) 
   const int step0 = min(steps, split * per), step1 = min(steps, step0 + per);
 
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};        // rows 2 warp, 2 warp + 1
-  constexpr int kQuads = kTreeRows * 256 / 4 / kTreeThreads;       // row and four channels: kTreeRows * hdp / 4 of them
-  float acc[kQuads][4];
+  // values: a thread has four rows, four channels and every `parts`-th key
+  const int quads = hdp / 4, parts = min(8, kTreeThreads / (4 * quads)), part = tid / (4 * quads), vrow = tid % (4 * quads) / quads * 4, vc = tid % quads * 4;
+  float acc[4][4];
 #pragma unroll
-  for (int i = 0; i < kQuads; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
-  const int quads = hdp / 4;
+  for (int i = 0; i < 4; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
+#pragma unroll 1
   for (int step = step0; step < step1; ++step) {
     const int key0 = first + step * kTreeKeys;
     __syncthreads();
-    tree_rows<T>(rows_s, (const T*)a.k_pool, a, table, kh, key0, end);
-    tree_rows<T>(values_s, (const T*)a.v_pool, a, table, kh, key0, end);
     if (tid < kTreeRows) {      // what a row sees of these 64 keys
       const int R = r0 + tid;
       unsigned long long b = 0ull;
@@ -112,62 +132,99 @@ __global__ void __launch_bounds__(kTreeThreads) tree_general_kernel(TreeArgs a) 
       }
       bits_s[tid] = b;
     }
+    tree_rows<T>(rows_s, values_s, a, table, kh, key0, end);
     __syncthreads();
     {
-      const int key = tid & 63, group = tid >> 6;
-      float sc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      const float* k = rows_s + key * (hdp + 4);
-      for (int c = 0; c < hdp; c += 4) {
-        const float4 kv = *reinterpret_cast<const float4*>(k + c);
+      // scores: a thread has four keys, sixteen apart, four rows and every fourth piece of four channels; its neighbours the other pieces
+      const int piece = tid & 3, key = tid >> 2 & 15, row = (tid >> 6) * 4;
+      float sc[4][4];      // [key][row]
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sc[k][0] = sc[k][1] = sc[k][2] = sc[k][3] = 0.0f;
+#pragma unroll 2
+      for (int c = 4 * piece; c < hdp; c += 16) {
+        float4 kv[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) kv[k] = *reinterpret_cast<const float4*>(rows_s + (key + 16 * k) * pitch + c);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float4 q = *reinterpret_cast<const float4*>(q_s + (group * 4 + i) * hdp + c);
-          sc[i] = fmaf(q.x, kv.x, sc[i]);
-          sc[i] = fmaf(q.y, kv.y, sc[i]);
-          sc[i] = fmaf(q.z, kv.z, sc[i]);
-          sc[i] = fmaf(q.w, kv.w, sc[i]);
+          const float4 q = *reinterpret_cast<const float4*>(q_s + (row + i) * pitch + c);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            sc[k][i] = fmaf(q.x, kv[k].x, sc[k][i]);
+            sc[k][i] = fmaf(q.y, kv[k].y, sc[k][i]);
+            sc[k][i] = fmaf(q.z, kv[k].z, sc[k][i]);
+            sc[k][i] = fmaf(q.w, kv[k].w, sc[k][i]);
+          }
         }
       }
+      // the neighbours' sums come together: lane `piece` ends with key + 16 piece
+      float two[2][4], one[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p_s[(group * 4 + i) * kTreeKeys + key] = bits_s[group * 4 + i] >> key & 1ull ? sc[i] : -INFINITY;
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float other = __shfl_xor_sync(0xffffffffu, piece & 2 ? sc[k][i] : sc[k + 2][i], 2);
+          two[k][i] = (piece & 2 ? sc[k + 2][i] : sc[k][i]) + other;
+        }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float other = __shfl_xor_sync(0xffffffffu, piece & 1 ? two[0][i] : two[1][i], 1);
+        const float mine = (piece & 1 ? two[1][i] : two[0][i]) + other;
+        one[i] = bits_s[row + i] >> (key + 16 * piece) & 1ull ? mine : -INFINITY;
+      }
+      *reinterpret_cast<float4*>(p_s + (key + 16 * piece) * kTreePitch + row) = make_float4(one[0], one[1], one[2], one[3]);
     }
     __syncthreads();
+    {
+      float2* at0 = reinterpret_cast<float2*>(p_s + lane * kTreePitch + 2 * warp);
+      float2* at1 = reinterpret_cast<float2*>(p_s + (lane + 32) * kTreePitch + 2 * warp);
+      const float2 s0 = *at0, s1 = *at1;
+      float2 w0, w1;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float* p = p_s + (2 * warp + i) * kTreeKeys;
-      const float s0 = p[lane], s1 = p[lane + 32], top = fmaxf(m[i], warp_max(fmaxf(s0, s1)));
-      const float use = top == -INFINITY ? 0.0f : top, keep = expf(m[i] - use);
-      const unsigned long long b = bits_s[2 * warp + i];
-      const float p0 = b >> lane & 1ull ? expf(s0 - use) : 0.0f, p1 = b >> (lane + 32) & 1ull ? expf(s1 - use) : 0.0f;
-      p[lane] = p0;
-      p[lane + 32] = p1;
-      l[i] = l[i] * keep + warp_sum(p0 + p1);
-      m[i] = top;
-      if (lane == 0) alpha_s[2 * warp + i] = keep;
+      for (int i = 0; i < 2; ++i) {
+        const float x0 = i ? s0.y : s0.x, x1 = i ? s1.y : s1.x, top = fmaxf(m[i], warp_max(fmaxf(x0, x1)));
+        const float use = top == -INFINITY ? 0.0f : top, keep = expf(m[i] - use);
+        const unsigned long long b = bits_s[2 * warp + i];
+        const bool sees0 = b >> lane & 1ull, sees1 = b >> (lane + 32) & 1ull;
+        const float p0 = expf(x0 - use), p1 = expf(x1 - use);
+        l[i] = l[i] * keep + warp_sum((sees0 ? p0 : 0.0f) + (sees1 ? p1 : 0.0f));
+        m[i] = top;
+        (i ? w0.y : w0.x) = sees0 ? p0 : -1.0f;
+        (i ? w1.y : w1.x) = sees1 ? p1 : -1.0f;
+        if (lane == 0) alpha_s[2 * warp + i] = keep;
+      }
+      *at0 = w0;
+      *at1 = w1;
     }
     __syncthreads();
-    const int n = min(kTreeKeys, end - key0);
+    if (part < parts) {
+      const int n = min(kTreeKeys, end - key0);
 #pragma unroll
-    for (int i = 0; i < kQuads; ++i) {
-      const int e = tid + i * kTreeThreads, r = e / quads, c = e % quads * 4;
-      if (r >= kTreeRows) continue;
-      const float keep = alpha_s[r];
+      for (int i = 0; i < 4; ++i) {
+        const float keep = alpha_s[vrow + i];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) acc[i][k] *= keep;
-      const unsigned long long b = bits_s[r];
+        for (int k = 0; k < 4; ++k) acc[i][k] *= keep;
+      }
 #pragma unroll 4
-      for (int j = 0; j < n; ++j) {
-        if (!(b >> j & 1ull)) continue;
-        const float p = p_s[r * kTreeKeys + j];
-        const float4 v = *reinterpret_cast<const float4*>(values_s + j * (hdp + 4) + c);
-        acc[i][0] = fmaf(p, v.x, acc[i][0]);
-        acc[i][1] = fmaf(p, v.y, acc[i][1]);
-        acc[i][2] = fmaf(p, v.z, acc[i][2]);
-        acc[i][3] = fmaf(p, v.w, acc[i][3]);
+      for (int j = part; j < n; j += parts) {
+        const float4 v = *reinterpret_cast<const float4*>(values_s + j * pitch + vc), w = *reinterpret_cast<const float4*>(p_s + j * kTreePitch + vrow);
+        const float p[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!(p[i] < 0.0f)) {      // (a weight that is no number is one that was seen)
+            acc[i][0] = fmaf(p[i], v.x, acc[i][0]);
+            acc[i][1] = fmaf(p[i], v.y, acc[i][1]);
+            acc[i][2] = fmaf(p[i], v.z, acc[i][2]);
+            acc[i][3] = fmaf(p[i], v.w, acc[i][3]);
+          }
       }
     }
   }
   __syncthreads();
+  float* sums_s = rows_s;      // [parts][16][hdp], where keys and values lay
+  if (part < parts)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(sums_s + (part * kTreeRows + vrow + i) * hdp + vc) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int R = r0 + 2 * warp + i;
@@ -180,17 +237,15 @@ __global__ void __launch_bounds__(kTreeThreads) tree_general_kernel(TreeArgs a) 
     }
   }
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kQuads; ++i) {
-    const int e = tid + i * kTreeThreads, r = e / quads, c = e % quads * 4, R = r0 + r;
-    if (r >= kTreeRows || R >= rows_total) continue;
+  for (int e = tid; e < kTreeRows * hdp; e += kTreeThreads) {
+    const int r = e / hdp, c = e % hdp, R = r0 + r;
+    if (R >= rows_total || c >= hd) continue;
+    float v = 0.0f;
+    for (int k = 0; k < parts; ++k) v += sums_s[(k * kTreeRows + r) * hdp + c];
     const size_t token = s.tok0 + R / G;
     const int head = kh * G + R % G;
-    const float inv = l_s[r] == 0.0f ? 0.0f : 1.0f / l_s[r];
-    for (int k = 0; k < 4 && c + k < hd; ++k) {
-      if (a.splits > 1) tree_slot(a, split, token, head)[c + k] = acc[i][k];
-      else ((T*)a.out)[(token * a.heads + head) * hd + c + k] = from_f32<T>(acc[i][k] * inv);
-    }
+    if (a.splits > 1) tree_slot(a, split, token, head)[c] = v;
+    else ((T*)a.out)[(token * a.heads + head) * hd + c] = from_f32<T>(l_s[r] == 0.0f ? 0.0f : v / l_s[r]);
   }
 }
 
