@@ -2,10 +2,13 @@
 //
 //   out = sum_j softmax_j(scale q . k_j) v_j over the rows j that the node sees; zeros where it sees none
 //
-// A block takes 16 rows of queries of a (sequence, kv head) (row r is node r / G, query head r % G of the group) and a share of the keys, 64 at a
-// time: keys as float32 in shared memory, a thread a key and four rows; then the values the same way, with a running maximum and sum a row. A key
-// that a row does not see is left out of its sum, not multiplied by zero, so what lies in such a row of the pool (infinities, NaN) never
+// A block takes 16 rows of queries of a (sequence, kv head) (row r is node r / G, query head r % G of the group) and a share of the keys, a page of 64 at a
+// time, keys and values as float32 in shared memory. Scores: a thread has four keys by four rows of every fourth piece of four channels, and four neighbours meet by shuffles (eight 16-byte reads of shared memory for 64
+// FMAs; with a key and four rows a thread it was five for 16). Then the running maximum and sum, two rows a warp; then the values, four rows by four channels a thread, the keys dealt to as many groups of threads as there
+// are, whose sums meet at the end. A key that a row does not see is left out of its sum, not multiplied by zero, so what lies in such a row of the pool (infinities, NaN) never
 // reaches it. Shares are joined by a second kernel, in their order: no two blocks add to the same place.
+// Measured (one B200, device): five sequences of 33 to 700 rows in float32, 8 / 4 heads of 64 under a window of 256, 17 us, two dependent launches of a page a block. 64 sequences of 150 to 4,096 rows in float32, 32 / 8 heads of
+// 128: 772 us, FMA pipe 43 %, issue 67 %, shared memory 53 % (the one key a thread 2,018); eight trees of 40 to 64 nodes 1,354 (3,550). bfloat16 with heads of 80, eight sequences: 68 (155).
 #include <math.h>
 
 #include <algorithm>
@@ -332,7 +335,7 @@ __global__ void __launch_bounds__(128) tree_join_kernel(TreeArgs a) {
   }
 }
 
-// Shares of the keys: as many as give every SM four blocks, of at least 64 keys.
+// Shares of the keys: as many as give every SM four blocks (at heads of 128 two run at a time; a share's sums cross memory once more), of at least 64 keys.
 static int general_tree_splits(int n_seqs, int max_count, int heads, int kv_heads, int max_keys) {
   const long long tiles = (long long)n_seqs * kv_heads * (((long long)max_count * (heads / kv_heads) + kTreeRows - 1) / kTreeRows);
   const long long steps = ((long long)max_keys + kTreeKeys - 1) / kTreeKeys + 1, wanted = (4ll * sm_count() + tiles - 1) / tiles;

@@ -10,6 +10,12 @@
 //   warps 4..19  the softmax: two groups of 256 threads, two threads a row (32 keys of a page each), that take the pages in turn where the tile has up to 128 rows (each with a maximum, a sum
 //                and an accumulator of its own, joined at the segment's end), or every page for 128 rows each where it has more. P is rounded to bfloat16 (the instruction takes no wider one
 //                beside bfloat16 values), the sum is of the unrounded weights, in 32 bits.
+// What bounds it, measured on one B200 (calls back to back in a graph): 64 sequences of 150 to 4,096 rows, 8 nodes each, 32 / 8 heads of 128: 104 us, 5.0 TB/s, where a copy reads 6.57; four of 9,000 to 30,000
+// rows 84 us, 5.1 TB/s. A block walks a page in 0.64 to 0.68 us (32 KB: 7 TB/s over all) and pays 4 to 5 us a segment, the last product, the results and the next queries' wait: that is the rest. Eight trees of 40 to 64
+// nodes on 1,000 to 8,192 rows: 64 us where the bytes take 22; a page of 256 rows is 16,384 powers of two (1,024 cycles of their unit) and takes 0.93 us, 31 of the 64; the way in, the shares' 37 MB and the joining are the
+// rest. One chat, 5 tokens in a row on 2,000 rows, 16 / 8 heads, in clusters: 12.6 us, a chain of latencies around four pages a block.
+// The layouts before this one, in the same order (batch, trees): two blocks an SM 155 and 81 us, one with a thread a row 140 and 78, two threads a row 111 and 70, and with segments weighed (kTtEntry) and shares joined from
+// a list 100 and 64. The next page's scores asked for before this one's weights leave spill registers (batch 112, trees 71); sums of the rounded weights instead of the exact ones cost 5 % and gain nothing (2.2e-3 against 2.3e-3).
 // Where the sequences are few (tt_cluster) the blocks of a cluster share one (sequence, kv head, tile) instead: the shares meet in distributed shared memory, and there is neither a second
 // kernel nor scratch.
 // Rows are row r = node r / G, query head r % G of the group. Fewer than 128 rows leave the instruction's other rows to whatever lies behind the queries in shared memory: a row of
@@ -75,7 +81,7 @@ struct TtArgs {
 };
 
 // The pages of a sequence that some node may see: those from the window of a node at `past` on. A (sequence, kv head, tile) counts kTtEntry units more than it has
-// pages: what a segment's beginning and end cost (runs of equal pages left blocks with many short segments behind: 64 sequences of 150 to 4,096 rows, of 148 blocks the median 99 us, the last 136).
+// pages: what a segment's beginning and end cost (runs of equal pages left blocks with many short segments behind: 64 sequences of 150 to 4,096 rows, of 148 blocks the median 99 us, the last 136; with it the call takes 104).
 constexpr int kTtEntry = 5;
 struct TtSeq {
   int past, count, tok0, page_lo, pages, tiles, units;
@@ -790,7 +796,7 @@ bool tree_tc_takes(int n_seqs, int max_count, int heads, int kv_heads, int head_
   return dtype == kBF16 && (head_dim == 64 || head_dim == 128) && n_seqs * tiles * kv_heads * (max_keys / 64 + 2ll + kTtEntry) < (1ll << 31);
 }
 
-// Whether blocks of a cluster share each (sequence, kv head, tile), and how many. A cluster waits for its longest sequence alone, so only where all clusters run at once (128 of the 148 blocks:
+// Whether blocks of a cluster share each (sequence, kv head, tile), and how many: one chat (5 tokens on 2,000 rows, 16 / 8 heads) takes 12.5 us so and 20.6 by runs of units and a second kernel. A cluster waits for its longest sequence alone, so only where all clusters run at once (128 of the 148 blocks:
 // clusters of eight lie within one of the GPU's partitions each) and no block takes more than ten pages.
 static int tt_cluster(int n_seqs, int kv_heads, int tiles, int max_count, int max_keys, int window) {
   long long pages = ((long long)max_keys + 63) / 64;

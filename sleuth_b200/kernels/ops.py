@@ -1965,7 +1965,7 @@ def attention_tree(q, k_pool, v_pool, out, seq_start, past, counts, seen, positi
     ones whose bit is set in its row of ``seen`` [tokens, words] int32 (``draft_tree`` makes both; any bits are taken). float32 or bfloat16, even
     ``head_dim`` up to 256; softmax and sums in float32. ``max_keys``: a promise that no sequence has more rows after the step (0: as many as its table
     holds). ``scratch``: ``attention_tree_scratch_floats`` floats. A node that sees nothing gives zeros. Rows that a node does not see never reach its result, whatever they hold;
-    rows of a page that the pool has not read as zeros."""
+    rows of a page that the pool has not read as zeros. bfloat16 tensors with heads of 64 or 128 start at 16-byte boundaries."""
     dt, i32 = q.dtype, torch.int32
     q_shape, k_shape, t_shape = q.shape, k_pool.shape, block_table.shape
     _need(len(q_shape) == 3 and len(k_shape) == 4 and len(t_shape) == 2 and seen.dim() == 2,
