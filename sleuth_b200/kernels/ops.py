@@ -1892,9 +1892,12 @@ _DRAFT_TREE_CALL = struct.Struct("7Qq4i")    # DraftTreeCall in csrc/draft_tree.
 _COMPACT_CALL = struct.Struct("7Q3q6i")      # CompactCall there
 
 
-def _on_current_device(what: str, t) -> None:
-    """A launch goes to the current device, whichever the tensors are on."""
-    _need(t.get_device() == torch._C._cuda_getDevice(), f"{what}: the tensors are on cuda:{t.get_device()}, which is not the current device")
+def _stream_on(what: str, dev: int) -> int:
+    """The current stream, for tensors on device ``dev``: a launch goes to the current device, whichever the tensors are on."""
+    current = torch._C._cuda_getDevice()
+    if dev != current:
+        raise ValueError(f"{what}: the tensors are on cuda:{dev}, which is not the current device")
+    return torch._C._cuda_getCurrentRawStream(current)
 
 
 def _fits_int(what: str, *values: int) -> None:
@@ -1933,10 +1936,10 @@ def draft_tree(parents, seq_start, past, counts, seen, positions, max_count: int
             (lambda: 0 < max_count <= MOST_NODES, f"{max_count} nodes of a sequence; 1 to {MOST_NODES} are taken"),
             (lambda: rows >= T and positions.numel() >= T and words * 32 >= max_count, "seen is [tokens, words] with a bit for each of max_count nodes, positions is [tokens]"),
             (lambda: window >= 0, "the window is not negative")))
-    _on_current_device("draft_tree", parents)
+    current = _stream_on("draft_tree", dev)
     try:
         call = _DRAFT_TREE_CALL.pack(parents.data_ptr(), seq_start.data_ptr(), past.data_ptr(), counts.data_ptr(), seen.data_ptr(), positions.data_ptr(),
-                                     stream if stream is not None else current_stream(), T, n, max_count, words, window)
+                                     current if stream is None else stream, T, n, max_count, words, window)
     except struct.error as e:
         raise ValueError(f"draft_tree: a number is out of range ({e})") from None
     lib().call("slb_draft_tree", call)
@@ -2000,11 +2003,11 @@ def attention_tree(q, k_pool, v_pool, out, seq_start, past, counts, seen, positi
     status = _TC_STATUS.get(q.device)
     if status is None:
         status = _tc_status(q.device)
-    _on_current_device("attention_tree", q)
+    current = _stream_on("attention_tree", dev)
     try:
         call = _TREE_CALL.pack(q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), out.data_ptr(), seq_start.data_ptr(), past.data_ptr(), counts.data_ptr(),
                                seen.data_ptr(), 0 if positions is None else positions.data_ptr(), block_table.data_ptr(),
-                               0 if scratch is None else scratch.data_ptr(), status.data_ptr(), stream if stream is not None else current_stream(),
+                               0 if scratch is None else scratch.data_ptr(), status.data_ptr(), current if stream is None else stream,
                                T, 0 if scratch is None else scratch.numel(), k_shape[0], stride, n, max_count, max_keys, heads, kv_heads, head_dim,
                                window, seen.shape[1], DT[dt], scale)
     except struct.error as e:
@@ -2064,12 +2067,12 @@ def verify_drafts(logits, limit: int, tokens, parents, seq_start, counts, unifor
             (lambda: uniforms.dtype == f32 and uniforms.numel() >= T if uniforms is not None else temperature <= 0, "uniforms are float32, one a node, and needed above temperature 0"),
             (lambda: floors is None or floors.dtype == f32 and floors.numel() >= T, "floors are float32, one a node"),
             (lambda: scratch is None or scratch.dtype == i32, "scratch is int32")))
-    _on_current_device("verify_drafts", logits)
+    current = _stream_on("verify_drafts", dev)
     try:
         call = _VERIFY_CALL.pack(logits.data_ptr(), 0 if probs is None else probs.data_ptr(), 0 if floors is None else floors.data_ptr(),
                                  0 if uniforms is None else uniforms.data_ptr(), tokens.data_ptr(), parents.data_ptr(), seq_start.data_ptr(), counts.data_ptr(),
                                  path.data_ptr(), lengths.data_ptr(), chosen.data_ptr(), 0 if scratch is None else scratch.data_ptr(),
-                                 stream if stream is not None else current_stream(), T, logits.stride(0) if T > 1 else vocab,
+                                 current if stream is None else stream, T, logits.stride(0) if T > 1 else vocab,
                                  0 if probs is None else probs.stride(0) if probs.shape[0] > 1 else probs.shape[1], 0 if scratch is None else scratch.numel(),
                                  temperature, n, limit, max_count, places)
     except struct.error as e:
@@ -2106,10 +2109,10 @@ def cache_compact(k_pool, block_table, past, path, lengths, v_pool=None, stream=
     rows = pages * kv_heads * 64
     if rows == 0 or places == 0 or n == 0 or width == 0:
         return
-    _on_current_device("cache_compact", k_pool)
+    current = _stream_on("cache_compact", dev)
     try:
         call = _COMPACT_CALL.pack(k_pool.data_ptr(), 0 if v_pool is None else v_pool.data_ptr(), block_table.data_ptr(), past.data_ptr(), path.data_ptr(),
-                                  lengths.data_ptr(), stream if stream is not None else current_stream(), k_pool.numel() // (rows * width),
+                                  lengths.data_ptr(), current if stream is None else stream, k_pool.numel() // (rows * width),
                                   0 if v_width == 0 else v_pool.numel() // (rows * v_width), pages, stride, n, kv_heads, width * size, v_width * size, places)
     except struct.error as e:
         raise ValueError(f"cache_compact: a number is out of range ({e})") from None
