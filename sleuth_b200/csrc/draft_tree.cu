@@ -11,7 +11,8 @@ namespace slb {
 //   A_{k+1}(i) = A_k(i) u A_k(J_k(i)),   J_{k+1}(i) = J_k(J_k(i)),
 // eight rounds for 256 nodes, where walking up a chain would take 256 dependent reads. Under a window of w positions a node sees the first w nodes of its
 // way: the union of A_k over the binary digits of w, each from where the digit before ended. Depth: nodes on the whole way, less one.
-// All latency: a block a sequence, a thread a node, ways of 256 bits in registers and shared memory. One B200, device: one tree of 8 nodes 1.7 us, 64 of 17 to 250 nodes 3.9; a call takes the host 7.
+// All latency: a block a sequence, a thread a node, ways of 256 bits in registers and shared memory. One B200, device: one tree of 8 nodes 1.7 us, 64 of 17 to 250
+// nodes 3.9; a call takes the host 7.
 struct DraftTreeArgs {
   const int *parents, *seq_start, *past, *counts;
   uint32_t* seen;
@@ -102,8 +103,9 @@ extern "C" int slb_draft_tree(const DraftTreeCall* call) {
 // ---- the cache after the step ----
 // For every sequence, layer and kv head, for i = 0 .. lengths - 1 in this order: row past + i <- row past + path[i]. path rises, so path[i] >= i: a row
 // that is written is never read afterwards, and a thread that takes the same 16 bytes of all rows, eight reads before eight writes, needs no barrier.
-// All layers in one launch: a step's compaction is a few rows of each, 2 KB of a layer and row at 8 heads of 128. One B200, device: 28 layers of 8 heads of 128, one sequence with up to four rows 2.6 us, 24 sequences with up to
-// seven 4.9 (12 MB read and written, in L2 mostly): three dependent reads (table, path, row) and the launch, and the host has 7.4 us a call.
+// All layers in one launch: a step's compaction is a few rows of each, 2 KB of a layer and row at 8 heads of 128. One B200, device: 28 layers of 8 heads of 128, one
+// sequence with up to four rows 2.6 us, 24 sequences with up to seven 4.9 (12 MB read and written, in L2 mostly): three dependent reads (table, path, row) and the
+// launch, and the host has 7.4 us a call.
 struct CompactArgs {
   char *k_pool, *v_pool;                  // [layers, pages, kv_heads, 64, bytes]
   const int *block_table, *past, *path, *lengths;

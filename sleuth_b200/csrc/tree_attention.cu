@@ -2,13 +2,15 @@
 //
 //   out = sum_j softmax_j(scale q . k_j) v_j over the rows j that the node sees; zeros where it sees none
 //
-// A block takes 16 rows of queries of a (sequence, kv head) (row r is node r / G, query head r % G of the group) and a share of the keys, a page of 64 at a
-// time, keys and values as float32 in shared memory. Scores: a thread has four keys by four rows of every fourth piece of four channels, and four neighbours meet by shuffles (eight 16-byte reads of shared memory for 64
-// FMAs; with a key and four rows a thread it was five for 16). Then the running maximum and sum, two rows a warp; then the values, four rows by four channels a thread, the keys dealt to as many groups of threads as there
-// are, whose sums meet at the end. A key that a row does not see is left out of its sum, not multiplied by zero, so what lies in such a row of the pool (infinities, NaN) never
-// reaches it. Shares are joined by a second kernel, in their order: no two blocks add to the same place.
-// Measured (one B200, device): five sequences of 33 to 700 rows in float32, 8 / 4 heads of 64 under a window of 256, 17 us, two dependent launches of a page a block. 64 sequences of 150 to 4,096 rows in float32, 32 / 8 heads of
-// 128: 772 us, FMA pipe 43 %, issue 67 %, shared memory 53 % (the one key a thread 2,018); eight trees of 40 to 64 nodes 1,354 (3,550). bfloat16 with heads of 80, eight sequences: 68 (155).
+// A block takes 16 rows of queries of a (sequence, kv head) (row r is node r / G, query head r % G of the group) and a share of the keys, a page of 64 at a time,
+// keys and values as float32 in shared memory. Scores: a thread has four keys by four rows of every fourth piece of four channels, and four neighbours meet by
+// shuffles (eight 16-byte reads of shared memory for 64 FMAs; with a key and four rows a thread it was five for 16). Then the running maximum and sum, two rows a
+// warp; then the values, four rows by four channels a thread, the keys dealt to as many groups of threads as there are, whose sums meet at the end. A key that a row
+// does not see is left out of its sum, not multiplied by zero, so what lies in such a row of the pool (infinities, NaN) never reaches it. Shares are joined by a
+// second kernel, in their order: no two blocks add to the same place.
+// Measured (one B200, device): five sequences of 33 to 700 rows in float32, 8 / 4 heads of 64 under a window of 256, 17 us, two dependent launches of a page a
+// block. 64 sequences of 150 to 4,096 rows in float32, 32 / 8 heads of 128: 772 us, FMA pipe 43 %, issue 67 %, shared memory 53 % (the one key a thread 2,018);
+// eight trees of 40 to 64 nodes 1,354 (3,550). bfloat16 with heads of 80, eight sequences: 68 (155).
 #include <math.h>
 
 #include <algorithm>
@@ -53,8 +55,8 @@ __device__ __forceinline__ float4 tree_load(const T* src, int c, int hd, bool wh
   return v;
 }
 
-// The page of rows key0 .. key0 + 63, keys and values, as float32 in shared memory: 64 channels of eight rows of each on their way at once. Zeros from row `end` on, and for a page that the
-// pool has not (as TMA reads them).
+// The page of rows key0 .. key0 + 63, keys and values, as float32 in shared memory: 64 channels of eight rows of each on their way at once. Zeros from row `end` on,
+// and for a page that the pool has not (as TMA reads them).
 template <typename T>
 __device__ __forceinline__ void tree_rows(float* ks, float* vs, const TreeArgs& a, const int* table, int kh, int key0, int end) {
   const int hd = a.head_dim, hdp = tree_pad(hd), pitch = tree_row(hd), r0 = threadIdx.x >> 4;
@@ -137,8 +139,9 @@ __global__ void __launch_bounds__(kTreeThreads) tree_general_kernel(TreeArgs a) 
   float acc[4][4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.0f;
-  // Where the copies can be asynchronous the next page's keys come while this one's scores become weights and results, its values while the next scores form (64 sequences of 150 to 4,096 rows
-  // 843 us without, 772 so); a share of one page has nothing to gain and the longer way in (five sequences under a window of 256: 16.7 us without, 17.8 so).
+  // Where the copies can be asynchronous the next page's keys come while this one's scores become weights and results, its values while the next scores form (64
+  // sequences of 150 to 4,096 rows 843 us without, 772 so); a share of one page has nothing to gain and the longer way in (five sequences under a window of 256:
+  // 16.7 us without, 17.8 so).
   const bool ahead = sizeof(T) == 4 && step1 - step0 > 1 && hd % 4 == 0 && ((reinterpret_cast<uintptr_t>(a.k_pool) | reinterpret_cast<uintptr_t>(a.v_pool)) & 15) == 0;
   if (ahead) {
     tree_rows_async(rows_s, (const float*)a.k_pool, a, table, kh, first + step0 * kTreeKeys, end, true);

@@ -1,8 +1,9 @@
 // Attention of drafted nodes (tree.cuh) on the tcgen05 tensor cores: bfloat16, heads of 64 and 128, any number of query heads a key/value head.
 //
-// What such a step costs is the read of the keys and values (up to 256 rows of queries meet each: 512 FLOP a byte at most), so the work is the pages: every sequence has
-// (kv head, tile of 256 rows, page) units, and each block, one an SM, takes an equal run of the list of all units, whatever the sequences' lengths. What a run holds of one (sequence, kv head,
-// tile) is a segment. A (sequence, kv head, tile) that is one segment is finished by its block; the others' shares wait in scratch for a second kernel that joins them in their order.
+// What such a step costs is the read of the keys and values (up to 256 rows of queries meet each: 512 FLOP a byte at most), so the work is the pages: every sequence
+// has (kv head, tile of 256 rows, page) units, and each block, one an SM, takes an equal run of the list of all units, whatever the sequences' lengths. What a run
+// holds of one (sequence, kv head, tile) is a segment. A (sequence, kv head, tile) that is one segment is finished by its block; the others' shares wait in scratch
+// for a second kernel that joins them in their order.
 //   warp 0       asks TMA for the pages of the run, keys and values, each into a ring of its own (128 KB on the way at most: 43 KB an SM hide a microsecond of latency, and it is more under load);
 //   warp 1       S = Q K^T, 128 x 64, ahead of the softmax; two score buffers a group in tensor memory;
 //   warp 2       O += P V as soon as P is written, P read from tensor memory where S was;
@@ -10,18 +11,21 @@
 //   warps 4..19  the softmax: two groups of 256 threads, two threads a row (32 keys of a page each), that take the pages in turn where the tile has up to 128 rows (each with a maximum, a sum
 //                and an accumulator of its own, joined at the segment's end), or every page for 128 rows each where it has more. P is rounded to bfloat16 (the instruction takes no wider one
 //                beside bfloat16 values), the sum is of the unrounded weights, in 32 bits.
-// What bounds it, measured on one B200 (calls back to back in a graph): 64 sequences of 150 to 4,096 rows, 8 nodes each, 32 / 8 heads of 128: 104 us, 5.0 TB/s, where a copy reads 6.57; four of 9,000 to 30,000
-// rows 84 us, 5.1 TB/s. A block walks a page in 0.64 to 0.68 us (32 KB: 7 TB/s over all) and pays 4 to 5 us a segment, the last product, the results and the next queries' wait: that is the rest. Eight trees of 40 to 64
-// nodes on 1,000 to 8,192 rows: 64 us where the bytes take 22; a page of 256 rows is 16,384 powers of two (1,024 cycles of their unit) and takes 0.93 us, 31 of the 64; the way in, the shares' 37 MB and the joining are the
-// rest. One chat, 5 tokens in a row on 2,000 rows, 16 / 8 heads, in clusters: 12.6 us, a chain of latencies around four pages a block.
-// The layouts before this one, in the same order (batch, trees): two blocks an SM 155 and 81 us, one with a thread a row 140 and 78, two threads a row 111 and 70, and with segments weighed (kTtEntry) and shares joined from
-// a list 100 and 64. The next page's scores asked for before this one's weights leave spill registers (batch 112, trees 71); sums of the rounded weights instead of the exact ones cost 5 % and gain nothing (2.2e-3 against 2.3e-3).
-// Where the sequences are few (tt_cluster) the blocks of a cluster share one (sequence, kv head, tile) instead: the shares meet in distributed shared memory, and there is neither a second
-// kernel nor scratch.
-// Rows are row r = node r / G, query head r % G of the group. Fewer than 128 rows leave the instruction's other rows to whatever lies behind the queries in shared memory: a row of
-// A reaches that row of the result alone, and nobody reads it.
-// Rows that a node does not see are masked by a bit each. Their values meet a zero weight in the product, which an infinity or a NaN among them would survive: so in pages that
-// not all rows see alike (the step's own and those at a window's edge) values that are not finite are taken out in shared memory, and nodes that do see them get them back at the end, a bit pair for each (row, channel).
+// What bounds it, measured on one B200 (calls back to back in a graph): 64 sequences of 150 to 4,096 rows, 8 nodes each, 32 / 8 heads of 128: 104 us, 5.0 TB/s,
+// where a copy reads 6.57; four of 9,000 to 30,000 rows 84 us, 5.1 TB/s. A block walks a page in 0.64 to 0.68 us (32 KB: 7 TB/s over all) and pays 4 to 5 us a
+// segment, the last product, the results and the next queries' wait: that is the rest. Eight trees of 40 to 64 nodes on 1,000 to 8,192 rows: 64 us where the bytes
+// take 22; a page of 256 rows is 16,384 powers of two (1,024 cycles of their unit) and takes 0.93 us, 31 of the 64; the way in, the shares' 37 MB and the joining
+// are the rest. One chat, 5 tokens in a row on 2,000 rows, 16 / 8 heads, in clusters: 12.6 us, a chain of latencies around four pages a block.
+// The layouts before this one, in the same order (batch, trees): two blocks an SM 155 and 81 us, one with a thread a row 140 and 78, two threads a row 111 and 70,
+// and with segments weighed (kTtEntry) and shares joined from a list 100 and 64. The next page's scores asked for before this one's weights leave spill registers
+// (batch 112, trees 71); sums of the rounded weights instead of the exact ones cost 5 % and gain nothing (2.2e-3 against 2.3e-3).
+// Where the sequences are few (tt_cluster) the blocks of a cluster share one (sequence, kv head, tile) instead: the shares meet in distributed shared memory, and
+// there is neither a second kernel nor scratch.
+// Rows are row r = node r / G, query head r % G of the group. Fewer than 128 rows leave the instruction's other rows to whatever lies behind the queries in shared
+// memory: a row of A reaches that row of the result alone, and nobody reads it.
+// Rows that a node does not see are masked by a bit each. Their values meet a zero weight in the product, which an infinity or a NaN among them would survive: so in
+// pages that not all rows see alike (the step's own and those at a window's edge) values that are not finite are taken out in shared memory, and nodes that do see
+// them get them back at the end, a bit pair for each (row, channel).
 #include <math.h>
 
 #include <algorithm>
@@ -81,7 +85,8 @@ struct TtArgs {
 };
 
 // The pages of a sequence that some node may see: those from the window of a node at `past` on. A (sequence, kv head, tile) counts kTtEntry units more than it has
-// pages: what a segment's beginning and end cost (runs of equal pages left blocks with many short segments behind: 64 sequences of 150 to 4,096 rows, of 148 blocks the median 99 us, the last 136; with it the call takes 104).
+// pages: what a segment's beginning and end cost (runs of equal pages left blocks with many short segments behind: 64 sequences of 150 to 4,096 rows, of 148 blocks
+// the median 99 us, the last 136; with it the call takes 104).
 constexpr int kTtEntry = 5;
 struct TtSeq {
   int past, count, tok0, page_lo, pages, tiles, units;
@@ -720,8 +725,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   }
 }
 
-// Joins the shares of what no block finished alone, of each block of the kernel before at most one (sequence, kv head, tile): the blocks make a list of them and go over its pieces of
-// 256 (row, four channels), a thread each, eight shares on the way at once.
+// Joins the shares of what no block finished alone, of each block of the kernel before at most one (sequence, kv head, tile): the blocks make a list of them and go
+// over its pieces of 256 (row, four channels), a thread each, eight shares on the way at once.
 constexpr int kTtMostBlocks = 256;
 template <int HD>
 __global__ void __launch_bounds__(256) tree_tc_join_kernel(TtArgs ta, int blocks) {
@@ -796,7 +801,8 @@ bool tree_tc_takes(int n_seqs, int max_count, int heads, int kv_heads, int head_
   return dtype == kBF16 && (head_dim == 64 || head_dim == 128) && n_seqs * tiles * kv_heads * (max_keys / 64 + 2ll + kTtEntry) < (1ll << 31);
 }
 
-// Whether blocks of a cluster share each (sequence, kv head, tile), and how many: one chat (5 tokens on 2,000 rows, 16 / 8 heads) takes 12.5 us so and 20.6 by runs of units and a second kernel. A cluster waits for its longest sequence alone, so only where all clusters run at once (128 of the 148 blocks:
+// Whether blocks of a cluster share each (sequence, kv head, tile), and how many: one chat (5 tokens on 2,000 rows, 16 / 8 heads) takes 12.5 us so and 20.6 by runs
+// of units and a second kernel. A cluster waits for its longest sequence alone, so only where all clusters run at once (128 of the 148 blocks:
 // clusters of eight lie within one of the GPU's partitions each) and no block takes more than ten pages.
 static int tt_cluster(int n_seqs, int kv_heads, int tiles, int max_count, int max_keys, int window) {
   long long pages = ((long long)max_keys + 63) / 64;

@@ -1,25 +1,29 @@
 // Which drafted tokens the target's probabilities accept, and the token behind the last of them.
 //
-// Every sequence brings a tree: node 0 is its newest certain token, row t of `logits` what the target says behind node t. With l the logits of the node
-// reached, p(i) = exp(l_i / T) / Z over i < limit with l_i >= floor, q the distribution that its children were drawn from, independently, the children x are tried in their order: x is
-// accepted with probability min(1, p(x) / q(x)); after a refusal p becomes max(p - q, 0) over its sum. Refusals in a row stay in one family:
+// Every sequence brings a tree: node 0 is its newest certain token, row t of `logits` what the target says behind node t. With l the logits of the node reached,
+// p(i) = exp(l_i / T) / Z over i < limit with l_i >= floor, q the distribution that its children were drawn from, independently, the children x are tried in their
+// order: x is accepted with probability min(1, p(x) / q(x)); after a refusal p becomes max(p - q, 0) over its sum. Refusals in a row stay in one family:
 //   p after k refusals = max(p - c_k q, 0) / F_k,   F_k = sum max(p - c_k q, 0),   c_0 = 0, F_0 = 1, c_{k+1} = c_k + F_k,
 // because max(max(p - c q, 0) / F - q, 0) = max(p - (c + F) q, 0) / F. So child x with the number u goes through iff p(x) > (c + u F) q(x), and a refusal costs one
 // sum over the row. Certain drafts are point masses: p(x) > u (1 - R), R the probability of the distinct tokens refused before. Where no child is left the next token is
 // drawn from what p has become: the first token, in the order of their numbers, where the running sum passes u of the whole. Temperature 0: the child that is
 // the row's first largest logit, and in the end that token.
 //
-// Two kernels: the first leaves the largest logit and the sum Z of every node that has children, the whole GPU over all of them; the second walks the sequences' ways,
-// a cluster of up to sixteen blocks each, a run of the row a warp, and reads whole rows only where a draft is refused or the next token is drawn. (Where the rows of all nodes would be too much
-// to read, kMostStatsBytes, the second finds Z by itself, row by row.) Results are whole numbers and have to be the definition's: what decides about a child (Z, p) comes from
-// 32-bit powers summed in 64 bits, off by some 1e-8, which is the chance that a random number falls between; but a draw compares one number with 150,000 running sums, so sums
-// for draws and refusals are of powers in pairs of 32-bit numbers, off by some 1e-12 (a table of 64 and four terms of the series; in 64 bits, of which an SM does 16 operations a clock, a pass over a row
-// took 7.5 us in eight blocks, four fifths of them waiting for that unit). A refusal takes one pass: the sums of exp, and of exp and of q over the tokens where exp / Z > c q as far as 32 bits tell, make
-// both the exact Z and F (a token on the wrong side is off by 1e-7 of itself, and one in a million is).
-// Measured (one B200, device, 151,936 tokens): one sequence of five drafts with distributions 21 us, 64 sequences of two to five 75 (the first kernel 32 for 137 MB, 4.3 TB/s; the second 48 in clusters of two, one pass of some 60
-// instructions a token and one of 300 tokens by the block that draws), eight trees of 15 to 23 certain drafts 36 (19 and 23). Steps before: every row by the blocks of its sequence, in 64 bits 45, 128 and 27; sums of all nodes first, 64-bit
-// powers 27, 91 and 45; pairs of 32-bit numbers, clusters of sixteen blocks of 512 threads 18, 86 and 38; of 1,024 threads 21, 75 and 37, which is kept: a batch has fewer blocks a sequence and gains most.
-// Sums first or row by row: eight trees 36 against 27 before, whose ways are short and whose trees wide, but chats and batches 21 against 45 and 75 against 128, and which it is depends on what is accepted, which no rule can know.
+// Two kernels: the first leaves the largest logit and the sum Z of every node that has children, the whole GPU over all of them; the second walks the sequences'
+// ways, a cluster of up to sixteen blocks each, a run of the row a warp, and reads whole rows only where a draft is refused or the next token is drawn. (Where the
+// rows of all nodes would be too much to read, kMostStatsBytes, the second finds Z by itself, row by row.) Results are whole numbers and have to be the
+// definition's: what decides about a child (Z, p) comes from 32-bit powers summed in 64 bits, off by some 1e-8, which is the chance that a random number falls
+// between; but a draw compares one number with 150,000 running sums, so sums for draws and refusals are of powers in pairs of 32-bit numbers, off by some 1e-12 (a
+// table of 64 and four terms of the series; in 64 bits, of which an SM does 16 operations a clock, a pass over a row took 7.5 us in eight blocks, four fifths of
+// them waiting for that unit). A refusal takes one pass: the sums of exp, and of exp and of q over the tokens where exp / Z > c q as far as 32 bits tell, make both
+// the exact Z and F (a token on the wrong side is off by 1e-7 of itself, and one in a million is).
+// Measured (one B200, device, 151,936 tokens): one sequence of five drafts with distributions 21 us, 64 sequences of two to five 75 (the first kernel 32 for 137 MB,
+// 4.3 TB/s; the second 48 in clusters of two, one pass of some 60 instructions a token and one of 300 tokens by the block that draws), eight trees of 15 to 23
+// certain drafts 36 (19 and 23). Steps before: every row by the blocks of its sequence, in 64 bits 45, 128 and 27; sums of all nodes first, 64-bit powers 27, 91 and
+// 45; pairs of 32-bit numbers, clusters of sixteen blocks of 512 threads 18, 86 and 38; of 1,024 threads 21, 75 and 37, which is kept: a batch has fewer blocks a
+// sequence and gains most.
+// Sums first or row by row: eight trees 36 against 27 before, whose ways are short and whose trees wide, but chats and batches 21 against 45 and 75 against 128, and
+// which it is depends on what is accepted, which no rule can know.
 #include <float.h>
 #include <math.h>
 
@@ -114,9 +118,9 @@ struct PairSum {
   __device__ __forceinline__ double value() const { return ((double)hi - 4.0) + (double)lo; }
 };
 
-// 2^y scaled so that the row's largest logit has between 1/2 and 1, y = l * log2 e / T in two parts (the product's error is an FMA away): y = m + j / 64 + r with |r| <= 1 / 128, 2^r = 1 + a + b with
-// a = r ln 2 rounded and b its error and the series' other terms up to the fourth, 2^(j / 64) from the table in two parts. Off by 1e-12 or less. Logits are counted from `base`: 0, or the
-// largest where its y is beyond 1,000 (all that counts then lies so near that the difference is exact).
+// 2^y scaled so that the row's largest logit has between 1/2 and 1, y = l * log2 e / T in two parts (the product's error is an FMA away): y = m + j / 64 + r with
+// |r| <= 1 / 128, 2^r = 1 + a + b with a = r ln 2 rounded and b its error and the series' other terms up to the fourth, 2^(j / 64) from the table in two parts. Off
+// by 1e-12 or less. Logits are counted from `base`: 0, or the largest where its y is beyond 1,000 (all that counts then lies so near that the difference is exact).
 struct PairPower {
   float scale_hi, scale_lo, base, cap, least;      // below `least` nothing counts; from `base` no logit lies further up than `cap`
   int bias;                                   // what makes a power of two of the whole part
@@ -156,8 +160,9 @@ struct PairPower {
   }
 };
 
-// f(token, logit, q) for tokens lo .. hi - 1 of a row of logits and, if there is one, a row of q (else 0), by the lanes of a warp; `vec`: 16-byte reads, lo a multiple of 4. The next
-// eight tokens of a lane are on their way while f works on four: loops that fetch their instructions once (unrolled twice as far every pass waited for instructions more than for anything else).
+// f(token, logit, q) for tokens lo .. hi - 1 of a row of logits and, if there is one, a row of q (else 0), by the lanes of a warp; `vec`: 16-byte reads, lo a
+// multiple of 4. The next eight tokens of a lane are on their way while f works on four: loops that fetch their instructions once (unrolled twice as far every pass
+// waited for instructions more than for anything else).
 template <bool PAIR, typename F>
 __device__ __forceinline__ void each_logit(const float* row, const float* other, int lo, int hi, int lane, bool vec, F f) {
   if (vec) {
@@ -731,8 +736,8 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(VerifyArgs a) {
   cluster_sync_all();      // the others may still be reading this block's sums
 }
 
-// 32-bit words of scratch that slb_verify_drafts takes.
-// Pieces of a row in the first kernel: small ones where the rows are few, else as many blocks as run at once twice over.
+// Pieces of a row in the first kernel: small ones where the rows are few, else as many blocks as run at once three times over, of which those of nodes without
+// children leave at once (a batch of 64: 73 to 77 us with 740 to 4,736 blocks, 83 with 500, 79 with 7,000; eight trees 36 to 37, 41, 42).
 static int stats_steps(long long rows, int limit) {
   const long long steps = ((long long)limit + kStatsStep - 1) / kStatsStep, pieces = 2368 / rows + 1;
   return (int)(pieces >= steps ? 1 : (steps + pieces - 1) / pieces);
@@ -742,6 +747,7 @@ static int stats_pieces(long long rows, int limit) {
   return (int)((limit + piece - 1) / piece);
 }
 static bool stats_first(long long rows, int limit) { return rows * limit * 4 <= kMostStatsBytes; }
+// 32-bit words of scratch that slb_verify_drafts takes.
 extern "C" long long slb_verify_drafts_scratch(int n_seqs, long long rows, int limit, int drawn) {
   return n_seqs > 0 && n_seqs < 65536 && rows > 0 && limit > 0 && stats_first(rows, limit) ? rows * stats_pieces(rows, limit) * (long long)(sizeof(VerifyStat) / 4) : 0;
 }
