@@ -181,6 +181,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (lane < 12) (&s_odd[0][0][0])[lane] = 0u;
     if (lane < 2) s_lo[lane] = 0;
+    if (CLUSTER)      // (of a block without pages nothing else becomes)
+      for (int r = lane; r < kTtTile; r += 32) s_ml[r] = make_float2(-INFINITY, 0.0f);
   }
   if (warp == 2) {
     __syncwarp();
@@ -672,19 +674,17 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     }
   }
   tc_fence_before();
-  __syncthreads();
-  if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  if constexpr (!CLUSTER) __syncthreads();
   if constexpr (CLUSTER) {
     // the shares meet: every block adds up its part of the (row, four channels)
     const int kh = s_run.kh, tile = s_run.tile, rank = (int)cluster_ctarank();
     const TtSeq& s = s_run.s;
     const int rows = min(kTtTile, s.count * G - tile * kTtTile);
-    if (s_run.u >= s_run.u_hi)      // (a block without pages)
-      for (int r = tid; r < kTtTile; r += kTtThreads) s_ml[r] = make_float2(-INFINITY, 0.0f);
-    __syncthreads();
+    __syncwarp();
     cluster_sync_all();
     const uint32_t ml_at = smem_addr(s_ml), part_at = base + L.k_off;
-    for (int e = rank * kTtThreads + tid; e < L.rows * (HD / 4); e += ta.cluster * kTtThreads) {
+    // (dealt to the blocks by the warp: what a block's reads of the others can bring is what this waits for)
+    for (int e = (warp * ta.cluster + rank) * 32 + lane; e < L.rows * (HD / 4); e += ta.cluster * kTtThreads) {
       const int r = e % L.rows, c0 = e / L.rows * 4;
       if (r >= rows) continue;
       float2 p[8];
@@ -720,8 +720,12 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       const int R = tile * kTtTile + r;
       *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + ((size_t)(s.tok0 + R / G) * a.heads + kh * G + R % G) * HD + c0) = make_uint2(w[0], w[1]);
     }
-    __syncthreads();
+    __syncwarp();
     cluster_sync_all();      // the others may still be reading this block's share
+  }
+  if (warp == 2) {
+    __syncwarp();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
   }
 }
 
