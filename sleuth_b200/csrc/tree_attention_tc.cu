@@ -15,7 +15,7 @@
 // where a copy reads 6.57; four of 9,000 to 30,000 rows 84 us, 5.1 TB/s. A block walks a page in 0.64 to 0.68 us (32 KB: 7 TB/s over all) and pays 4 to 5 us a
 // segment, the last product, the results and the next queries' wait: that is the rest. Eight trees of 40 to 64 nodes on 1,000 to 8,192 rows: 64 us where the bytes
 // take 22; a page of 256 rows is 16,384 powers of two (1,024 cycles of their unit) and takes 0.93 us, 31 of the 64; the way in, the shares' 37 MB and the joining
-// are the rest. One chat, 5 tokens in a row on 2,000 rows, 16 / 8 heads, in clusters: 12.6 us, a chain of latencies around four pages a block.
+// are the rest. One chat, 5 tokens in a row on 2,000 rows, 16 / 8 heads, in clusters: 12.2 us, a chain of latencies around four pages a block.
 // The layouts before this one, in the same order (batch, trees): two blocks an SM 155 and 81 us, one with a thread a row 140 and 78, two threads a row 111 and 70,
 // and with segments weighed (kTtEntry) and shares joined from a list 100 and 64. The next page's scores asked for before this one's weights leave spill registers
 // (batch 112, trees 71); sums of the rounded weights instead of the exact ones cost 5 % and gain nothing (2.2e-3 against 2.3e-3).
@@ -805,7 +805,7 @@ bool tree_tc_takes(int n_seqs, int max_count, int heads, int kv_heads, int head_
   return dtype == kBF16 && (head_dim == 64 || head_dim == 128) && n_seqs * tiles * kv_heads * (max_keys / 64 + 2ll + kTtEntry) < (1ll << 31);
 }
 
-// Whether blocks of a cluster share each (sequence, kv head, tile), and how many: one chat (5 tokens on 2,000 rows, 16 / 8 heads) takes 12.5 us so and 20.6 by runs
+// Whether blocks of a cluster share each (sequence, kv head, tile), and how many: one chat (5 tokens on 2,000 rows, 16 / 8 heads) takes 12.2 us so and 20.6 by runs
 // of units and a second kernel. A cluster waits for its longest sequence alone, so only where all clusters run at once (128 of the 148 blocks:
 // clusters of eight lie within one of the GPU's partitions each) and no block takes more than ten pages.
 static int tt_cluster(int n_seqs, int kv_heads, int tiles, int max_count, int max_keys, int window) {
@@ -859,11 +859,12 @@ static int launch_tree_tc(const CUtensorMap& mq, const CUtensorMap& mk, const CU
   static std::atomic<unsigned long long> allowed, allowed_clusters;
   cudaError_t e = ta.cluster ? allow_shared((const void*)tree_tc_kernel<HD, true>, 224 * 1024, allowed_clusters) : allow_shared((const void*)tree_tc_kernel<HD, false>, 224 * 1024, allowed);
   if (e != cudaSuccess) return fail(2, "attention_tree: cannot reserve shared memory: %s", cudaGetErrorString(e));
+  // (both may begin early: barriers and tensor memory are made while the kernel before ends. One chat, call after call: 12.2 us so, 14.4 one after the other)
   if (ta.cluster) {
-    launch_clusters(pdl_mode() == 1, (unsigned)ta.cluster, tree_tc_kernel<HD, true>, dim3(ta.cluster * ta.t.kv_heads * ta.tiles * ta.t.n_seqs), dim3(kTtThreads), (size_t)ta.lay.total, s, mq, mk, mv, ta);
+    launch_clusters(pdl_mode() != 0, (unsigned)ta.cluster, tree_tc_kernel<HD, true>, dim3(ta.cluster * ta.t.kv_heads * ta.tiles * ta.t.n_seqs), dim3(kTtThreads), (size_t)ta.lay.total, s, mq, mk, mv, ta);
     return check_launch("attention_tree (tensor cores, clusters)");
   }
-  launch(tree_tc_kernel<HD, false>, dim3(blocks), dim3(kTtThreads), (size_t)ta.lay.total, s, mq, mk, mv, ta);
+  launch_prefetching(tree_tc_kernel<HD, false>, dim3(blocks), dim3(kTtThreads), (size_t)ta.lay.total, s, mq, mk, mv, ta);
   const int rc = check_launch("attention_tree (tensor cores)");
   if (rc) return rc;
   if (blocks == 1) return 0;

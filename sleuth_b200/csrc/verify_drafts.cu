@@ -815,7 +815,8 @@ extern "C" int slb_verify_drafts(const VerifyCall* call) {
   }
   if (need > 0) {
     a.stats = reinterpret_cast<VerifyStat*>(c.scratch);
-    launch(verify_stats_kernel, dim3(a.pieces, c.n_seqs, c.max_count), dim3(kStatsThreads), 0, (cudaStream_t)c.stream, a);
+    // (begins early, call after call: one chat 21.9 us, 23.2 otherwise: a launch is on its way while the kernel before ends)
+    launch_prefetching(verify_stats_kernel, dim3(a.pieces, c.n_seqs, c.max_count), dim3(kStatsThreads), 0, (cudaStream_t)c.stream, a);
     const int rc = check_launch("verify_drafts (sums)");
     if (rc) return rc;
   }
