@@ -437,6 +437,18 @@ def test_refused_calls():
     ops.attention_tree(z(0, 4, 64, t=bf), z(2, 2, 64, 64, t=bf), z(2, 2, 64, 64, t=bf), z(0, 256, t=bf), z(1), z(0), z(0), z(0, 1), None, z(0, 2), 4, 4, 2, 64, 0, 0.1)
 
 
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim", HEADS, ids=IDS)
+@pytest.mark.parametrize("past,counts", [([0, 10, 60], [3, 6, 5]), ([700, 70], [4, 9]), ([0, 40] * 40, [2, 5] * 40), ([90, 5], [130, 140])], ids=["few", "long", "many", "broad"])
+def test_results_are_off_by_their_own_rounding(dtype, heads, kv_heads, dim, past, counts):
+    """In bfloat16 a result is rounded once, by half a step (2^-8 of it); weights are off by 2^-15 at most, beside what 32-bit sums leave (the oracle's slack)."""
+    step = Step(dtype, heads, kv_heads, dim, past, counts, "random", 0, seed=30)
+    out = step.run()
+    want, size, slack = step.want()
+    own, weights = (2.0 ** -8, 2.0 ** -15) if dtype == torch.bfloat16 else (2.0 ** -24, 2.0 ** -23)
+    err, allowed = (out - want).abs(), (slack[..., None] + weights) * size
+    assert bool((err <= allowed * (1 + own) + own * want.abs() + 1e-30).all()), float((err / (allowed + own * want.abs() + 1e-30)).max())
+
+
 # ------------------------------------------------------------------ verification ----
 
 class Judged:
