@@ -39,6 +39,11 @@ namespace slb {
 
 constexpr int kTtRows = 128, kTtTile = 256, kTtThreads = 20 * 32, kTtSoftmax = 4 * 32;      // (the first thread of the softmax)
 constexpr float kTtRescale = 8.0f;      // log2 units by which a maximum may be stale
+// A row's maximum m serves its weights as 2^(score scale - m), one FMA each, and is off by up to half a step of 32 bits, a factor that all of them share; from 2^31 on
+// that factor alone would be below the least number. So a maximum of 2^29 and more is kept as the score times the power of two at or above the scale, which is exact,
+// and its weights are 2^((score - maximum) scale). Two such scores lie 32 units apart or are equal, so it does not matter that their distance looks up to twice as long.
+constexpr float kTtFar = 536870912.0f;
+__device__ __forceinline__ bool tt_far(float m) { return fabsf(m) >= kTtFar && fabsf(m) < INFINITY; }
 
 __device__ __forceinline__ float tt_ex2(float x) {
   float y;
@@ -60,21 +65,21 @@ static TtLayout tt_layout(int HD, int rows) {
   l.rows = std::min(kTtTile, (rows + 31) & ~31);
   l.queries = l.rows <= kTtRows ? 2 : 1;
   l.q_bytes = l.rows * HD * 2;
-  const int page = 64 * HD * 2, rest = 2 * kTtRows * HD / 4 + 2 * 2 * kTtRows * 16 + 2 * 2 * 2 * kTtRows * 2 + 64 * 8;
+  const int page = 64 * HD * 2, rest = 2 * kTtRows * HD / 4 + 2 * 2 * kTtRows * 16 + 2 * 2 * 2 * kTtRows * 4 + 64 * 8;
   l.stages = std::min(8, (223 * 1024 - l.queries * l.q_bytes - rest) / (2 * page));      // (227 KB a block, up to 3 KB of it static)
   l.k_off = l.queries * l.q_bytes;
   l.v_off = l.k_off + l.stages * page;
   l.poison_off = l.v_off + l.stages * page;
   l.ml_off = l.poison_off + 2 * kTtRows * HD / 4;
   l.xch_off = l.ml_off + 2 * 2 * kTtRows * 16;
-  l.bar_off = l.xch_off + 2 * 2 * 2 * kTtRows * 2;
+  l.bar_off = l.xch_off + 2 * 2 * 2 * kTtRows * 4;
   l.total = l.bar_off + 64 * 8;
   return l;
 }
 
 struct TtArgs {
   TreeArgs t;
-  float scale_log2;
+  float scale_log2, far_scale, far_back;      // far_scale: the power of two at or above scale_log2, far_back: one over it
   float* part;          // [blocks][2][HD][rows] weighted values
   float2* part_ml;      // [blocks][2][rows] maximum (log2 units) and sum
   int2* info;           // [blocks] the (sequence, kv head, tile) whose first pages this block has and whose last ones it has not, and the blocks that share it (0: none)
@@ -418,7 +423,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     uint32_t* poison = reinterpret_cast<uint32_t*>(smem + L.poison_off) + (g * kTtRows + r) * WORDS;      // [2 groups][128 rows][WORDS]; of the other group: other_poison words on
     const int other_poison = g ? -kTtRows * WORDS : kTtRows * WORDS;
     float4* ml = reinterpret_cast<float4*>(smem + L.ml_off);                  // [2 groups][2 halves][128 rows] maximum, sum, whether there is poison
-    unsigned short* xch = reinterpret_cast<unsigned short*>(smem + L.xch_off) + g * 512 + r;      // [2 groups][2 buffers][2 halves][128 rows]
+    float* xch = reinterpret_cast<float*>(smem + L.xch_off) + g * 512 + r;      // [2 groups][2 buffers][2 halves][128 rows]
     // A wait that gives up ends nothing here: the warp notes it and walks on to the segment's end, because others meet it at barriers; the status word says so.
     bool ok = true;
     auto wait_warp = [&](uint32_t bar, uint32_t parity, int code) {
@@ -499,18 +504,17 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             mx = tt_max3(mx, __uint_as_float(sr[k]), __uint_as_float(sr[k + 1]));
             mx1 = tt_max3(mx1, __uint_as_float(sr[k + 2]), __uint_as_float(sr[k + 3]));
           }
-          // The row's maximum is the larger of the two halves'. They are exchanged rounded up to 16 bits (any common reference at or above the maximum serves a
-          // softmax), so both threads of a row take the same decisions.
+          // The row's maximum is the larger of the two halves', so that both threads of a row take the same decisions, and it is exchanged as it is: rounded up to 16
+          // bits it lies up to 2^-7 of itself too high, 126 units of log2 where scores pass 10^4, and no weight is left beside it.
           {
-            const uint32_t bits = __float_as_uint(fmaxf(mx, mx1));
-            const unsigned short up = (unsigned short)(((bits & 0x80000000u) ? bits : bits + 0xffffu) >> 16);
-            xch[b * 256 + half * 128] = up;      // (a place per buffer: the partner passes the barrier of the next item only after reading this one)
+            const float own_max = fmaxf(mx, mx1);
+            xch[b * 256 + half * 128] = own_max;      // (a place per buffer: the partner passes the barrier of the next item only after reading this one)
             pair_sync();
-            const unsigned short other = xch[b * 256 + (half ^ 1) * 128];
-            mx = fmaxf(__uint_as_float((uint32_t)up << 16), __uint_as_float((uint32_t)other << 16));
+            mx = fmaxf(own_max, xch[b * 256 + (half ^ 1) * 128]);
           }
-          const float m_new = fmaxf(m_used, mx * ta.scale_log2);      // the scale is positive
-          const bool grow = m_new > m_used + kTtRescale;              // also true for the first finite maximum
+          mx = fabsf(mx * ta.scale_log2) >= kTtFar ? mx * ta.far_scale : mx * ta.scale_log2;      // the scale is positive
+          const float m_new = fmaxf(m_used, mx);
+          const bool grow = m_new > m_used + kTtRescale;      // also true for the first finite maximum
           if (done > 0 && __any_sync(0xffffffffu, grow)) {
             wait_warp(pv_done + 8 * (2 * g + (b ^ 1)), ((c - 1) >> 1) & 1, 120);      // O must hold all of the last product
             tc_fence_after();
@@ -526,7 +530,13 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             l *= alpha;
           }
           if (grow) m_used = m_new;
-          const f32x2 refs = both(m_used == -INFINITY ? 0.0f : -m_used), scales = both(ta.scale_log2);
+          const bool far = tt_far(m_used);
+          if (__any_sync(0xffffffffu, far)) {
+            const float ref = far ? m_used * ta.far_back : 0.0f;
+#pragma unroll
+            for (int k = 0; k < 32; ++k) sr[k] = __float_as_uint(__uint_as_float(sr[k]) - ref);
+          }
+          const f32x2 refs = both(m_used == -INFINITY || far ? 0.0f : -m_used), scales = both(ta.scale_log2);
           f32x2 sums = 0ull;
           uint32_t pk[16], rest[16];      // the weights' upper 16 bits, and those of what is left of them
 #pragma unroll
@@ -891,6 +901,10 @@ int tree_tc(const TreeArgs& a, long long pool_pages, int* status, cudaStream_t s
   TtArgs ta{};
   ta.t = a;
   ta.scale_log2 = a.scale * 1.4426950408889634f;
+  int exponent = 0;
+  const float fraction = frexpf(ta.scale_log2, &exponent);
+  ta.far_scale = ldexpf(1.0f, fraction == 0.5f ? exponent - 1 : exponent);
+  ta.far_back = 1.0f / ta.far_scale;
   if (!f.cluster) {
     ta.part = a.scratch + f.part;
     ta.part_ml = reinterpret_cast<float2*>(a.scratch + f.part_ml);

@@ -449,6 +449,48 @@ def test_results_are_off_by_their_own_rounding(dtype, heads, kv_heads, dim, past
     assert bool((err <= allowed * (1 + own) + own * want.abs() + 1e-30).all()), float((err / (allowed + own * want.abs() + 1e-30)).max())
 
 
+def _scores(step, q0, k0, k1, twins):
+    """Every node sees the rows before the step, whose scores lie far below, and of the step's own rows itself (with ``twins`` the node beside it too); its score
+    there is q0 k0 + k1."""
+    step.q.zero_()
+    step.q[..., 0], step.q[..., 1] = q0, 1.0
+    rows = torch.isfinite(step.k)
+    step.k[rows] = 0.0
+    for s, (p, c) in enumerate(zip(step.past, step.counts)):
+        for r in range(p + c):
+            page, at = step.place(s, r)
+            step.k[page, :, at, 0] = k0 if r >= p else 2 * k0 if k0 < 0 else k0 / 2
+            step.k[page, :, at, 1] = k1 if r >= p else 0.0
+    want = torch.zeros((step.T, step.heads, step.dim), dtype=torch.float64)
+    for s, (p, c) in enumerate(zip(step.past, step.counts)):
+        for i in range(c):
+            seen = [i, i ^ 1] if twins and i ^ 1 < c else [i]
+            word = torch.zeros(step.words * 32, dtype=torch.int64)
+            word[seen] = 1
+            word = (word.view(-1, 32) << torch.arange(32)).sum(1)
+            step.seen[step.starts[s] + i] = torch.where(word >= 1 << 31, word - (1 << 32), word).to(torch.int32)
+            values = [step.v[step.place(s, p + b)[0], :, step.place(s, p + b)[1]].double() for b in seen]
+            want[step.starts[s] + i] = (sum(values) / len(values)).repeat_interleave(step.heads // step.kv_heads, 0)
+    return want
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim", [HEADS[2], HEADS[5], HEADS[6], HEADS[9]], ids=[IDS[i] for i in (2, 5, 6, 9)])
+@pytest.mark.parametrize("past,counts", [([0, 30, 200], [3, 6, 5]), ([3000, 70], [4, 9]), ([0, 100] * 40, [2, 5] * 40), ([90, 5], [130, 140])],
+                         ids=["few", "long", "many", "broad"])
+@pytest.mark.parametrize("q0,k0,k1", [(512.0, 256.0, 1.0), (512.0, -256.0, -1020.0), (2048.0, 128.0, 56.0), (2.0 ** 20, 2.0 ** 12, 255 * 2.0 ** 17), (2.0 ** 20, -2.0 ** 12, -255 * 2.0 ** 17),
+                                      (2.0 ** 30, 2.0 ** 30, 255 * 2.0 ** 45), (2.0 ** 30, -2.0 ** 30, -255 * 2.0 ** 45)])
+def test_large_scores(dtype, heads, kv_heads, dim, past, counts, q0, k0, k1):
+    """Scores of 10^4 to 10^17, of both signs, just above and just below what 16 bits hold: a node that sees one key of such a score gives that key's value as it
+    is; two of the same score, their mean."""
+    step = Step(dtype, heads, kv_heads, dim, past, counts, "star", 0, seed=31)
+    want = _scores(step, q0, k0, k1, False)
+    assert torch.equal(step.run(), want)
+    want = _scores(step, q0, k0, k1, True)
+    # half a step of the result; a float32 sum's and quotient's, weights' parts (2^-15 of a weight, the same for both)
+    rounding = 2.0 ** -8 + 2.0 ** -14 if dtype == torch.bfloat16 else 2.0 ** -23
+    assert bool(((step.run() - want).abs() <= rounding * want.abs() + 1e-30).all())
+
+
 # ------------------------------------------------------------------ verification ----
 
 class Judged:
