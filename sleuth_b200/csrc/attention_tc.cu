@@ -151,8 +151,8 @@ struct AttnTcLayout {
   static constexpr int SUM_OFF = V_OFF + 2 * KV_BYTES;        // the halves' row sums, float [2 halves][128 rows]
   static constexpr int BAR_OFF = SUM_OFF + 2 * kAtRows * 4;
   static constexpr int N_BARS = 12;
-  static constexpr int XCH_OFF = BAR_OFF + N_BARS * 8 + 16;   // row maxima as 16-bit values, [2 pages][2 halves][128 rows]
-  static constexpr int TOTAL = XCH_OFF + 4 * kAtRows * 2;
+  static constexpr int XCH_OFF = BAR_OFF + N_BARS * 8 + 16;   // row maxima, float [2 pages][2 halves][128 rows]
+  static constexpr int TOTAL = XCH_OFF + 4 * kAtRows * 4;
   static_assert(2 * (TOTAL + 1024) <= 228 * 1024, "two blocks must fit on an SM");
   static constexpr int TMEM_COLS = 256;              // S0, S1 (64 each; P_j takes the first 32 of S_j's) and O (HD <= 128)
 };
@@ -310,7 +310,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     const int pos = R < rows_total ? past + R / G : -1;        // -1: a padding row sees nothing
     const int lo = first_key(pos, a.window);
     const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16);
-    unsigned short* xch = reinterpret_cast<unsigned short*>(smem + L::XCH_OFF);     // [2 pages][2 halves][128 rows]
+    float* xch = reinterpret_cast<float*>(smem + L::XCH_OFF);     // [2 pages][2 halves][128 rows]
     float m_used = -INFINITY, l = 0.0f;
     // KEPT: the sum of the weights as they are rounded for the product, by which the result is divided: what rounds the one key that a peaked row looks at
     // then cancels (error against 64 bits 2.2e-3 to 2.3e-3 -> 2.1e-3 to 2.2e-3 for 2 to 4 per cent of the time); the denominator that others get is the sum of the weights themselves
@@ -374,17 +374,15 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       float mx = -INFINITY;
 #pragma unroll
       for (int c = 0; c < 32; c += 2) mx = max3(mx, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
-      // The row's maximum is the larger of the two halves'. They are exchanged rounded up to 16 bits (any common
-      // reference at or above the maximum serves a softmax), so both threads of a row take the same decisions.
+      // The row's maximum is the larger of the two halves', so both threads of a row take the same decisions. It is
+      // exchanged whole: a reference rounded up to 16 bits lies above all scores by up to 2^-7 of them, which is 126
+      // units of log2 where scores pass 10^4, and leaves no weight.
       {
-        const uint32_t bits = __float_as_uint(mx);
-        const unsigned short up = (unsigned short)(((bits & 0x80000000u) ? bits : bits + 0xffffu) >> 16);
         // a place per page parity: when this is written again two pages on, the partner has passed the barrier of
         // the page between, which it reaches only after reading this one
-        xch[b * 256 + half * 128 + r] = up;
+        xch[b * 256 + half * 128 + r] = mx;
         pair_sync();
-        const unsigned short other = xch[b * 256 + (half ^ 1) * 128 + r];
-        mx = fmaxf(__uint_as_float((uint32_t)up << 16), __uint_as_float((uint32_t)other << 16));
+        mx = fmaxf(mx, xch[b * 256 + (half ^ 1) * 128 + r]);
       }
       const float m_new = fmaxf(m_used, mx * sl2);               // the scale is positive
       const bool grow = m_new > m_used + kRescaleStep;      // also true for the first finite maximum
@@ -503,8 +501,8 @@ struct AttnWideLayout {
   static constexpr int SUM_OFF = V_OFF + 2 * STAGE_BYTES;        // the parts' row sums, float [4 parts][128 rows]
   static constexpr int BAR_OFF = SUM_OFF + 4 * kAtRows * 4;
   static constexpr int N_BARS = 12;
-  static constexpr int XCH_OFF = BAR_OFF + N_BARS * 8 + 16;      // row maxima as 16-bit values, [2 steps][4 parts][128 rows]
-  static constexpr int TOTAL = XCH_OFF + 2 * 4 * kAtRows * 2;
+  static constexpr int XCH_OFF = BAR_OFF + N_BARS * 8 + 16;      // row maxima, float [2 steps][4 parts][128 rows]
+  static constexpr int TOTAL = XCH_OFF + 2 * 4 * kAtRows * 4;
   static_assert(TOTAL + 1024 <= 227 * 1024, "the block must fit on an SM");
   static constexpr int TMEM_COLS = 512;                  // S0, S1 (128 each; P takes the first 64 of its S) and O (HD <= 128)
 };
@@ -673,7 +671,7 @@ attn_tc_wide_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
     const int pos = R < rows_total ? past + R / G : -1;        // -1: a padding row sees nothing
     const int lo = first_key(pos, a.window);
     const uint32_t lane_addr = tmem + ((uint32_t)(quad * 32) << 16);
-    unsigned short* xch = reinterpret_cast<unsigned short*>(smem + L::XCH_OFF);     // [2 steps][4 parts][128 rows]
+    float* xch = reinterpret_cast<float*>(smem + L::XCH_OFF);     // [2 steps][4 parts][128 rows]
     float m_used = -INFINITY, l = 0.0f;
     // KEPT: the sum of the weights as they are rounded for the product, by which the result is divided: what rounds the one key that a peaked row looks at
     // then cancels (error against 64 bits 2.2e-3 to 2.3e-3 -> 2.1e-3 to 2.2e-3 for 2 to 4 per cent of the time); the denominator that others get is the sum of the weights themselves
@@ -735,13 +733,10 @@ attn_tc_wide_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
 #pragma unroll
       for (int c = 0; c < 32; c += 2) mx = max3(mx, __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
       {
-        const uint32_t bits = __float_as_uint(mx);
-        const unsigned short up = (unsigned short)(((bits & 0x80000000u) ? bits : bits + 0xffffu) >> 16);
-        unsigned short* x = xch + b * 512 + r;
-        x[part * 128] = up;
+        float* x = xch + b * 512 + r;
+        x[part * 128] = mx;
         row_sync();
-        mx = fmaxf(fmaxf(__uint_as_float((uint32_t)x[0] << 16), __uint_as_float((uint32_t)x[128] << 16)),
-                   fmaxf(__uint_as_float((uint32_t)x[256] << 16), __uint_as_float((uint32_t)x[384] << 16)));
+        mx = fmaxf(fmaxf(x[0], x[128]), fmaxf(x[256], x[384]));
       }
       const float m_new = fmaxf(m_used, mx * sl2);               // the scale is positive
       const bool grow = m_new > m_used + kRescaleStep;      // also true for the first finite maximum
