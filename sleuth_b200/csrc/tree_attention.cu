@@ -292,9 +292,9 @@ constexpr int kMostSplits = 64;
 template <typename T>
 __global__ void __launch_bounds__(128) tree_join_kernel(TreeArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, seq = blockIdx.y;
-  const TreeSeq s(a, seq);      // (in front of the wait: what the kernel before this one has waited for is there)
   const long long row = (long long)blockIdx.x * 4 + warp;
-  pdl_wait();
+  pdl_wait();      // (the kernel before this one lets it begin before it has waited itself: the tables may still be on their way)
+  const TreeSeq s(a, seq);
   if (row >= (long long)s.count * a.heads) return;
   __shared__ float factor_s[4][kMostSplits];
   const size_t token = s.tok0 + row / a.heads;

@@ -491,6 +491,55 @@ def test_large_scores(dtype, heads, kv_heads, dim, past, counts, q0, k0, k1):
     assert bool(((step.run() - want).abs() <= rounding * want.abs() + 1e-30).all())
 
 
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim", [HEADS[0], HEADS[2], HEADS[5], HEADS[6], HEADS[9]], ids=[IDS[i] for i in (0, 2, 5, 6, 9)])
+def test_tables_that_the_kernel_in_front_writes(dtype, heads, kv_heads, dim):
+    """The numbers of rows and nodes come from a judgement right in front of the attention, which lets it begin early: always the new ones count."""
+    from sleuth_b200.kernels import ops
+    vocab, n, most = 4000, 6, 6
+    past, counts = [700, 300, 5, 0, 64, 1000], [6, 5, 4, 3, 2, 1]
+    step = Step(dtype, heads, kv_heads, dim, past, counts, "chain", 0, seed=32)
+    t = [x.to(DEV) for x in (step.q, step.k, step.v)]
+    starts, seen, table = i32(step.starts), step.seen.to(DEV), step.table.to(DEV)
+    floats = ops.attention_tree_scratch_floats(step.T, n, most, heads, kv_heads, dim, step.stride * 64, dtype)
+    assert floats > 0 or dtype == torch.bfloat16 and dim in (64, 128)
+    scratch = torch.zeros(max(1, floats), device=DEV)
+    # a judgement whose lengths are the counts: greedy chains of which the first counts[s] nodes are right
+    logits = torch.zeros((n * most, vocab), device=DEV)
+    logits[:, 7] = 1.0
+    tokens = torch.full((n, most), 7, dtype=torch.int32)
+    for s, c in enumerate(counts):
+        tokens[s, c:] = 8
+    tokens = tokens.view(-1).to(DEV)
+    parents, verify_starts, sixes = i32([i - 1 for i in range(most)] * n), i32([most * s for s in range(n)]), i32([most] * n)
+    path, lengths, chosen = (torch.zeros(s, dtype=torch.int32, device=DEV) for s in ((n, most), (n,), (n,)))
+    words = torch.zeros(max(1, ops.verify_drafts_scratch_words(n, n * most, vocab, False)), dtype=torch.int32, device=DEV)
+    # and a tree table whose positions are the numbers of rows before the step: trees of single nodes
+    pasts, single, ones = i32([0] * n), i32([-1] * n), i32([1] * n)
+    bits, before = torch.zeros((n, 1), dtype=torch.int32, device=DEV), i32(past)
+    out = torch.empty((step.T, heads * dim), dtype=dtype, device=DEV)
+    wanted = step.run(promise=False).view(step.T, -1)
+
+    def call():
+        ops.verify_drafts(logits, vocab, tokens, parents, verify_starts, sixes, None, 0.0, path, lengths, chosen, most, scratch=words)
+        ops.draft_tree(single, i32_range, before, ones, bits, pasts, 1)
+        ops.attention_tree(t[0], t[1], t[2], out, starts, pasts, lengths, seen, None, table, most, heads, kv_heads, dim, 0, step.scale, scratch=scratch)
+
+    i32_range = i32(list(range(n)))
+    graph = torch.cuda.CUDAGraph()
+    call()
+    torch.cuda.synchronize()
+    assert lengths.tolist() == counts and pasts.tolist() == past
+    with torch.cuda.graph(graph):
+        for _ in range(4):
+            call()
+    for again in range(20):
+        lengths.fill_(again % 3)
+        pasts.fill_(again)
+        out.fill_(7.0)
+        graph.replay() if again % 2 else call()
+        assert torch.equal(out.cpu().double(), wanted), again
+
+
 # ------------------------------------------------------------------ verification ----
 
 class Judged:

@@ -39,3 +39,17 @@ def test_the_next_kernel_starts_only_when_tensor_memory_is_taken():
             assert "bar.arrive" not in kernel[:signal] or "if (" in line, path.name
             seen += 1
     assert seen >= 5
+
+
+def test_tables_are_read_behind_the_wait():
+    """A kernel may begin while any kernel in front of it still runs, for one that begins early itself lets its successor begin at once: so what another
+    kernel may have written, a step's tables among them, is read behind the kernel's own wait."""
+    reads = re.compile(r"\bTreeSeq \w+\(|\.read\(|\.(?:seq_start|past|counts|positions|block_table|seen|lengths|parents|tokens)\s*\[")
+    seen = 0
+    for path in [library.CSRC / name for name in ("tree_attention.cu", "tree_attention_tc.cu", "draft_tree.cu", "verify_drafts.cu")]:
+        for kernel in re.split(r"\n(?=__global__)", path.read_text())[1:]:
+            waits = [at for at in (kernel.find("pdl_wait()"), kernel.find("pdl_enter()")) if at >= 0]
+            assert waits, path.name
+            assert not reads.search(kernel[:min(waits)]), (path.name, reads.search(kernel[:min(waits)]).group())
+            seen += 1
+    assert seen >= 8
