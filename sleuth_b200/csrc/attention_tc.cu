@@ -181,22 +181,6 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   const int pairs = (int)(gridDim.y * gridDim.z);
   const int lin = (int)(blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z));
   const int seq = (lin % pairs) / (int)gridDim.y, kh = (lin % pairs) % (int)gridDim.y;
-  const int G = a.heads / a.kv_heads;
-  const int count = a.counts[seq], past = a.past[seq], tok0 = a.seq_start[seq];
-  const int rows_total = count * G;
-  const int n_tiles = (rows_total + kAtRows - 1) / kAtRows;
-  const int tile = (int)gridDim.x - 1 - lin / pairs;
-  if (tile >= n_tiles) return;
-  const int r0 = tile * kAtRows;
-  const int t_first = r0 / G;
-  const int t_last = min(rows_total - 1, r0 + kAtRows - 1) / G;
-  const int key_lo = first_key(past + t_first, a.window);
-  const int page_hi = (past + t_last) / 64;
-  const TilePages pages(KEPT, key_lo, page_hi, a.first);
-  const int n_pages = pages.count;
-  const int seq_len = past + count;
-  const int* table = a.block_table + (size_t)seq * a.table_stride;
-
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     for (int i = 0; i < 2; ++i) {
@@ -220,8 +204,26 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   const uint32_t tO = tmem + 128;
 
   pdl_launch_dependents();     // only now: a successor that also wants tensor memory must not take it before this block has its own
-  pdl_wait();
+  pdl_wait();      // the step's tables too may come from the kernel in front
   trace.mark(1);
+  const int G = a.heads / a.kv_heads;
+  const int count = a.counts[seq], past = a.past[seq], tok0 = a.seq_start[seq];
+  const int rows_total = count * G;
+  const int n_tiles = (rows_total + kAtRows - 1) / kAtRows;
+  const int tile = (int)gridDim.x - 1 - lin / pairs;
+  if (tile >= n_tiles) {      // the whole block
+    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::TMEM_COLS) : "memory");
+    return;
+  }
+  const int r0 = tile * kAtRows;
+  const int t_first = r0 / G;
+  const int t_last = min(rows_total - 1, r0 + kAtRows - 1) / G;
+  const int key_lo = first_key(past + t_first, a.window);
+  const int page_hi = (past + t_last) / 64;
+  const TilePages pages(KEPT, key_lo, page_hi, a.first);
+  const int n_pages = pages.count;
+  const int seq_len = past + count;
+  const int* table = a.block_table + (size_t)seq * a.table_stride;
 
   if (warp == 0) {
     if (elect_one()) {
@@ -529,23 +531,6 @@ attn_tc_wide_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   const int pairs = (int)(gridDim.y * gridDim.z);
   const int lin = (int)(blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z));
   const int seq = (lin % pairs) / (int)gridDim.y, kh = (lin % pairs) % (int)gridDim.y;
-  const int G = a.heads / a.kv_heads;
-  const int count = a.counts[seq], past = a.past[seq], tok0 = a.seq_start[seq];
-  const int rows_total = count * G;
-  const int n_tiles = (rows_total + kAtRows - 1) / kAtRows;
-  const int tile = (int)gridDim.x - 1 - lin / pairs;     // longest first
-  if (tile >= n_tiles) return;
-  const int r0 = tile * kAtRows;
-  const int t_first = r0 / G;
-  const int t_last = min(rows_total - 1, r0 + kAtRows - 1) / G;
-  const int key_lo = first_key(past + t_first, a.window);
-  const int page_hi = (past + t_last) / 64;
-  const TilePages pages(KEPT, key_lo, page_hi, a.first);
-  const int n_pages = pages.count;
-  const int n_steps = (n_pages + 1) >> 1;
-  const int seq_len = past + count;
-  const int* table = a.block_table + (size_t)seq * a.table_stride;
-
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     for (int i = 0; i < 2; ++i) {
@@ -569,8 +554,27 @@ attn_tc_wide_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_cons
   const uint32_t tO = tmem + 256;
 
   pdl_launch_dependents();     // only now: a successor that also wants tensor memory must not take it before this block has its own
-  pdl_wait();
+  pdl_wait();      // the step's tables too may come from the kernel in front
   trace.mark(1);
+  const int G = a.heads / a.kv_heads;
+  const int count = a.counts[seq], past = a.past[seq], tok0 = a.seq_start[seq];
+  const int rows_total = count * G;
+  const int n_tiles = (rows_total + kAtRows - 1) / kAtRows;
+  const int tile = (int)gridDim.x - 1 - lin / pairs;     // longest first
+  if (tile >= n_tiles) {      // the whole block
+    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::TMEM_COLS) : "memory");
+    return;
+  }
+  const int r0 = tile * kAtRows;
+  const int t_first = r0 / G;
+  const int t_last = min(rows_total - 1, r0 + kAtRows - 1) / G;
+  const int key_lo = first_key(past + t_first, a.window);
+  const int page_hi = (past + t_last) / 64;
+  const TilePages pages(KEPT, key_lo, page_hi, a.first);
+  const int n_pages = pages.count;
+  const int n_steps = (n_pages + 1) >> 1;
+  const int seq_len = past + count;
+  const int* table = a.block_table + (size_t)seq * a.table_stride;
 
   if (warp == 0) {
     if (elect_one()) {
