@@ -12,8 +12,9 @@
 // Two kernels: the first leaves the largest logit and the sum Z of every node that has children, the whole GPU over all of them; the second walks the sequences'
 // ways, a cluster of up to sixteen blocks each, a run of the row a warp, and reads whole rows only where a draft is refused or the next token is drawn. (Where the
 // rows of all nodes would be too much to read, kMostStatsBytes, the second finds Z by itself, row by row.) Results are whole numbers and have to be the
-// definition's: what decides about a child (Z, p) comes from 32-bit powers summed in 64 bits, off by some 1e-8, which is the chance that a random number falls
-// between; but a draw compares one number with 150,000 running sums, so sums for draws and refusals are of powers in pairs of 32-bit numbers, off by some 1e-12 (a
+// definition's. Z comes from 32-bit powers summed in 64 bits, off by some 1e-7 (the power unit's 2^-22, rounded exponents and partial sums, 1e-5 at the very most), and
+// where a child lies nearer to its number than kVerifyDoubt the row's exact sum decides, one pass that one child in 30,000 takes; a draw compares one number with
+// 150,000 running sums. Those sums, and refusals', are of powers in pairs of 32-bit numbers, off by some 1e-12 (1e-11 where logits over temperature pass 1,000; a
 // table of 64 and four terms of the series; in 64 bits, of which an SM does 16 operations a clock, a pass over a row took 7.5 us in eight blocks, four fifths of
 // them waiting for that unit). A refusal takes one pass: the sums of exp, and of exp and of q over the tokens where exp / Z > c q as far as 32 bits tell, make both
 // the exact Z and F (a token on the wrong side is off by 1e-7 of itself, and one in a million is).
@@ -33,6 +34,7 @@
 namespace slb {
 
 constexpr int kVerifyTeam = 16, kVerifyThreads = 1024, kVerifyWarps = kVerifyThreads / 32, kVerifyRuns = kVerifyTeam * kVerifyWarps;
+constexpr double kVerifyDoubt = 0x1p-16;      // of a probability: what the rough sums may be off by, with room
 constexpr long long kMostStatsBytes = 512ll << 20;      // 80 us of reading at most in front of the way; beyond it few rows of many lie on a way
 
 // Of a piece of a row of logits: the largest kept one, its first place, and the sum of exp((l - top) / T).
@@ -60,7 +62,7 @@ struct VerifyArgs {
   int *path, *lengths, *chosen;
   long long rows, ld, ldp;
   double scale, unscale;      // log2 e / T, and one over it; 0: the largest logit alone counts
-  float scale_hi, scale_lo;
+  float scale_hi, scale_lo, least;      // least: a difference of logits whose power is nothing
   VerifyStat* stats;          // [rows, pieces], or null
   int limit, max_count, path_width, run, vec;      // run: tokens of a warp, a multiple of 4
   int team, pieces, steps;    // blocks of a sequence; pieces of a row in the first kernel, and their steps
@@ -299,23 +301,15 @@ __global__ void __launch_bounds__(kStatsThreads, 5) verify_stats_kernel(VerifyAr
         top = high;
       }
       float part = 0.0f;
-      const float ref = top * a.scale_hi;
-      if (fabsf(ref) < 4096.0f) {      // (its rounding is then nothing beside 1)
-        const float shift = ex2_f32(fmaf(top, a.scale_hi, fmaf(top, a.scale_lo, -ref)));      // (the largest logit's own power: near 1)
+      if (fabsf(top) < INFINITY) {
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
-          const float y = ex2_f32(fmaf(v[k], a.scale_hi, fmaf(v[k], a.scale_lo, -ref)));
+          const float y = ex2_f32(fmaxf(v[k] - top, a.least) * a.scale_hi);      // (a difference: nothing is lost where logits over temperature are large)
           part += v[k] > -INFINITY ? y : 0.0f;
         }
-        part /= shift;
-      } else if (top > -INFINITY) {      // (infinite, the type's lowest value, almost no temperature)
-#pragma unroll 1
-        for (int k = 0; k < PER; ++k) {
-          float x = v[0];
+      } else if (top > -INFINITY) {      // infinite: as many of them as there are
 #pragma unroll
-          for (int e = 1; e < PER; ++e) x = e == k ? v[e] : x;
-          part += x > -INFINITY ? rough_exp(a, x, top) : 0.0f;
-        }
+        for (int k = 0; k < PER; ++k) part += v[k] == top ? 1.0f : 0.0f;
       }
       z += part;
     }
@@ -559,6 +553,17 @@ struct Verifier {
     return s.runs[runs - 1];
   }
 
+  // s.p of a node's children from the exact sum of its row, which a refusal of drafts with distributions (`formed`) has left
+  __device__ void exact_children(int node, int count, bool formed) {
+    if (!formed) {
+      const double all = sums(false, 0.0, 0.0f, 0);
+      inv_e = all > 0.0 ? 1.0 / all : 0.0;
+    }
+    __syncthreads();      // (others may still be reading)
+    if (tid > node && tid < count && s.parent[tid] == node) s.p[tid] = s.token[tid] < 0 ? 0.0 : fine(s.logit[tid]) * inv_e;
+    __syncthreads();
+  }
+
   // the token where the running sum passes `target`; in the block that has its run, else -1
   __device__ int draw(double target, bool pair, double c, int n_refused) {
     const int runs = a.team * kVerifyWarps;
@@ -684,14 +689,33 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(VerifyArgs a) {
         }
       }
       double f = 1.0, gone = 0.0;
+      bool exact = false;      // s.p of this node's children are
       for (int j = inner ? node + 1 : count; j < count; ++j) {
         if (s.parent[j] != node) continue;
-        const double p = s.p[j], u = s.u[j];
+        const double u = s.u[j];
         bool again = false;      // a certain draft that was refused before has no probability left
         for (int r = 0; r < n_refused; ++r) again = again || s.refused[r] == s.token[j];
-        if (!again && (a.probs ? p > (c + u * f) * (double)s.prob[j] : p > u * (1.0 - gone))) {
-          taken = j;
-          break;
+        if (!again) {
+          double p = s.p[j], border = a.probs ? (c + u * f) * (double)s.prob[j] : u * (1.0 - gone);
+          if (!exact && p > 0.0 && fabs(p - border) <= kVerifyDoubt * (p + u * gone)) {      // the rough Z does not tell
+            exact = true;
+            if (!set) v.set_top(s.stat[node].top);
+            set = true;
+            v.exact_children(node, count, pair);
+            gone = 0.0;
+            for (int i = node + 1; i < j; ++i) {      // what was refused, every token once
+              if (a.probs || s.parent[i] != node || s.token[i] < 0) continue;
+              bool twice = false;
+              for (int k = node + 1; k < i; ++k) twice = twice || (s.parent[k] == node && s.token[k] == s.token[i]);
+              if (!twice) gone += s.p[i];
+            }
+            p = s.p[j];
+            border = a.probs ? (c + u * f) * (double)s.prob[j] : u * (1.0 - gone);
+          }
+          if (p > border) {
+            taken = j;
+            break;
+          }
         }
         if (a.probs) {
           if (!(z > 0.0)) continue;      // a row without probabilities: nothing to refuse
@@ -703,7 +727,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(VerifyArgs a) {
           __syncthreads();
           if (tid == 0) s.refused[n_refused] = s.token[j];
           ++n_refused;
-          gone += p;
+          gone += s.p[j];
           __syncthreads();
         }
       }
@@ -797,6 +821,7 @@ extern "C" int slb_verify_drafts(const VerifyCall* call) {
     a.unscale = 1.0 / a.scale;
     a.scale_hi = (float)a.scale;
     a.scale_lo = (float)(a.scale - (double)a.scale_hi);
+    a.least = (float)fmax(-200.0 * a.unscale, -(double)FLT_MAX);
   }
   const long long need = slb_verify_drafts_scratch(c.n_seqs, c.rows, c.limit, c.probs != nullptr);
   SLB_REQUIRE(need == 0 || (c.scratch != nullptr && c.scratch_words >= need), "verify_drafts: the call needs %lld words of scratch, %lld were given", need,

@@ -611,6 +611,56 @@ def test_verification(vocab, limit, pad, temperature, kind, drawn, floors):
     Judged([5, 1, 0, 9, 17, 2, 8], kind, vocab, limit, temperature, drawn, floors, seed=vocab + int(10 * temperature), pad=pad).check()
 
 
+def _beside(border):
+    """The nearest float32 numbers below and above, further away than what the sums leave open (1e-11)."""
+    down = torch.tensor(border, dtype=torch.float32)
+    while float(down) > border * (1 - 1e-10):
+        down = torch.nextafter(down, torch.tensor(0.0))
+    up = torch.nextafter(down, torch.tensor(2.0))
+    while float(up) < border * (1 + 1e-10):
+        up = torch.nextafter(up, torch.tensor(2.0))
+    return down, up
+
+
+@pytest.mark.parametrize("drawn", [False, True])
+@pytest.mark.parametrize("temperature", [0.01, 0.02, 0.3, 1.0, 30.0])
+@pytest.mark.parametrize("vocab,wanted", [(40, 0.9), (4100, 0.6), (30000, 0.02)])
+def test_numbers_next_to_a_probability(vocab, wanted, temperature, drawn):
+    """Random numbers that are the nearest float32 below and above a draft's probability (over that of its draw): accepted and refused, as in 64 bits. Where a second
+    child follows, the refused one's probability counts as exactly."""
+    n = 120
+    counts = [3] * n
+    j = Judged(counts, "star", vocab, vocab, temperature, drawn, seed=41)
+    g = torch.Generator().manual_seed(41)
+    T = 3 * n
+    j.logits = 20.0 + 3.0 * temperature * torch.randn((T, vocab), generator=g)
+    if drawn:
+        j.probs = torch.softmax(torch.randn((T, vocab), generator=g), 1)
+    for s in range(n):
+        row = j.logits[3 * s]
+        x, y = s % vocab, (s + 7) % vocab
+        # token x gets about the wanted share of the row, y half of what is left where it is the second child's turn
+        for token, share in ((x, wanted), (y, 0.5 * (1 - wanted) if s % 4 > 1 else 0.1 * wanted)):
+            rest = torch.logsumexp(torch.cat([row[:token], row[token + 1:]]).double() / temperature, 0)
+            row[token] = float((rest + math.log(share / (1 - share))) * temperature)
+        p = torch.softmax(row.double() / temperature, 0)
+        j.tokens[3 * s + 1], j.tokens[3 * s + 2] = x, y
+        if drawn:
+            q = j.probs[3 * s].double()
+            q[x] = min(1.0, float(p[x]) * 1.3)
+            j.probs[3 * s] = q.float()
+        border = float(p[x]) / (float(j.probs[3 * s, x]) if drawn else 1.0)
+        down, up = _beside(border)
+        if s % 4 > 1 and not drawn:      # the first is refused, the second lies at its border
+            j.uniforms[3 * s + 1] = 1.0 - 2.0 ** -24
+            down, up = _beside(float(p[y]) / (1.0 - float(p[x])))
+            j.uniforms[3 * s + 2] = down if s % 2 else up
+        else:
+            j.uniforms[3 * s + 1] = down if s % 2 else up
+            j.uniforms[3 * s + 2] = 0.9
+    j.check()
+
+
 @pytest.mark.parametrize("drawn", [True, False])
 def test_verification_of_a_large_vocabulary(drawn):
     Judged([6, 6, 4, 1], "chain", 151936, 151936, 0.8, drawn, seed=3, sharp=2.5).check()
