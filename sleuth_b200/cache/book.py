@@ -249,6 +249,8 @@ class CacheBook:
         """After a step whose rows are not all kept (drafted tokens): ``commit``, and pages behind the last row go back."""
         if self.budget:
             raise CacheMisuse("rows of a cache with a budget are not taken back")
+        for s in slots:
+            self._check_live(s)
         self.commit(slots, new_lengths)
         for s, n in zip(slots, new_lengths):
             for g in self.groups:

@@ -166,6 +166,7 @@ class Engine:
 
     def close(self, slots: Sequence[int]) -> None:
         self.cache.close(slots)
+        self.stepper.forget(slots)
 
     def step(self, entries) -> torch.Tensor:
         """entries: ``StepEntry`` objects or ``(slot, tokens, want)`` tuples. See ``Stepper.step``."""

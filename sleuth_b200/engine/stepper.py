@@ -232,7 +232,7 @@ class Stepper:
         return DraftStep(positions, [seen[r.window] for r in self.cache.group_requests])
 
     def forget(self, slots) -> None:
-        """Slots that stand for new sequences: what an earlier one drafted is not theirs to accept."""
+        """Slots that were closed, or stand for new sequences: what an earlier one drafted is not theirs to accept."""
         for s in slots:
             self._drafted.pop(int(s), None)
 
