@@ -252,7 +252,11 @@ class CacheBook:
         for s in slots:
             self._check_live(s)
         self.commit(slots, new_lengths)
-        for s, n in zip(slots, new_lengths):
+        self.trim(slots, new_lengths)
+
+    def trim(self, slots, lengths) -> None:
+        """Pages behind the last of ``lengths`` rows go back; nothing else changes."""
+        for s, n in zip(slots, lengths):
             for g in self.groups:
                 behind = g.table[s][pages_for(n):]
                 g.pool.give(behind[behind >= 0].tolist())

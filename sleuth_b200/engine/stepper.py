@@ -172,7 +172,8 @@ class Stepper:
     # ------------------------------------------------------------------ drafted tokens ----
     def step_tree(self, entries: list[TreeEntry]) -> torch.Tensor:
         """Run the newest token of each sequence and the drafts behind it, all at once: float32 logits of every node, in the order of the entries and
-        of their tokens. Nothing of it is kept until ``accept`` says which nodes are; a sequence that takes another step before is as it was."""
+        of their tokens. Nothing of it is kept until ``accept`` says which nodes are; a sequence that takes another step before is as it was,
+        its pages too (until then, or until it is closed, it holds those of the drafts)."""
         why = drafts_refusal(self.model, self.cache)
         if why is not None:
             raise ValueError(f"drafts: not built for this model: {why}")
@@ -202,6 +203,7 @@ class Stepper:
         if T > self.max_step_tokens:
             raise ValueError(f"a step of drafted tokens brings at most {self.max_step_tokens} tokens, got {T}")
         book.grow(slots, new_lens)
+        self._drop_drafts(slots, new_lens)
         b = self.meta.upload(slots, past, counts, np.concatenate(toks).astype(np.int32), np.arange(T, dtype=np.int32), book.tables_for(slots))
         b.tree = self._draft_step(b, np.concatenate(trees).astype(np.int32))
         out = torch.empty((T, self.model.vocab), dtype=torch.float32, device=self.device)
@@ -235,6 +237,13 @@ class Stepper:
         """Slots that were closed, or stand for new sequences: what an earlier one drafted is not theirs to accept."""
         for s in slots:
             self._drafted.pop(int(s), None)
+
+    def _drop_drafts(self, slots, lengths) -> None:
+        """``slots`` take another step, after which they hold ``lengths`` rows: what they drafted goes, and the pages that only drafts had."""
+        if self._drafted:
+            for s, n in zip(slots, lengths):
+                if self._drafted.pop(s, None) is not None:
+                    self.cache.book.trim([s], [n])
 
     def accept(self, slots, paths) -> None:
         """Of the last ``step_tree`` of each of ``slots`` the nodes of its path stay (numbers of its tokens, rising, from 0 on); their rows move together in every
@@ -361,6 +370,7 @@ class Stepper:
         else:
             self.model.forward(b, self.cache, self.ws, out[:0])
         book.commit(c_slots, new_lens)
+        self._drop_drafts(c_slots, new_lens)
 
     def _chunk_by_graph(self, b, W: int, out, dest_a) -> bool:
         """A step of many tokens whose shape (tokens, sequences, longest share, wanted rows) has been seen before is
@@ -475,6 +485,7 @@ class Stepper:
             self.model.forward(b, self.cache, self.ws, logits)
             self._seen_decode.add(gkey)
         book.commit(slots, new_lens)
+        self._drop_drafts(slots, new_lens)
         self._look_at_status(single_tokens=True)
         return logits
 
