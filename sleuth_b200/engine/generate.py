@@ -78,7 +78,7 @@ class _Live:
     new: list[int] = field(default_factory=list)
     blocker: NgramBlocker | None = None
     drafter: NgramDrafter | None = None
-    drafted: int = 0            # drafts that were judged, and those that were right
+    drafted: int = 0            # what its drafter proposed and a step judged, and how much of that was right
     taken: int = 0
 
 
@@ -315,14 +315,15 @@ def _run_batch_drafted(backend, batch, prompts, results, max_new_tokens, samplin
             for q, room in zip(live, rooms):
                 more, parents = q.drafter.propose(room)
                 trees.append(([q.new[-1], *more], [-1, *parents]))
+            proposed = [len(t) - 1 for t, _ in trees]
             if any(len(t) > 1 for t, _ in trees):
-                # every sequence brings as many tokens as there may be, so that recorded steps serve the next ones: the last one again and again, which is a draft like any other
+                # every sequence brings as many tokens as there may be, so that recorded steps serve the next ones: the last one again and again, judged like any draft (and not counted)
                 for (t, p), room in zip(trees, rooms):
                     for _ in range(min(room, drafts.tokens) + 1 - len(t)):
                         p.append(len(t) - 1)
                         t.append(t[-1])
             if backend.pages_needed([q.slot for q in live], [backend.length(q.slot) + len(t) for q, (t, _) in zip(live, trees)]) > backend.free_pages():
-                trees = [([q.new[-1]], [-1]) for q in live]
+                trees, proposed = [([q.new[-1]], [-1]) for q in live], [0] * len(live)
             drafted = any(len(t) > 1 for t, _ in trees)
             if drafted:
                 logits = backend.step_tree([(q.slot, t, p) for q, (t, p) in zip(live, trees)])
@@ -337,10 +338,10 @@ def _run_batch_drafted(backend, batch, prompts, results, max_new_tokens, samplin
             chosen = choose(logits, draws)
             now = time.perf_counter()
             keep, paths, base = [], [], 0
-            for q, (t, p) in zip(live, trees):
+            for q, (t, p), own in zip(live, trees, proposed):
                 before = backend.length(q.slot) - (0 if drafted else 1)      # tokens in the cache before the step
                 node, path, reason = 0, [0], None
-                q.drafted += len(t) - 1
+                q.drafted += own
                 while True:
                     tok = chosen[base + node]
                     reason = take(q, tok, before + len(path))
@@ -350,7 +351,7 @@ def _run_batch_drafted(backend, batch, prompts, results, max_new_tokens, samplin
                     if node is None:
                         break
                     path.append(node)
-                    q.taken += 1
+                    q.taken += node <= own
                 base += len(t)
                 if reason is None:
                     keep.append(q)

@@ -7,7 +7,11 @@ import torch
 
 from sleuth_b200.cache.book import CacheBook, CacheMisuse
 from sleuth_b200.engine.engine import Engine
+from sleuth_b200.engine.generate import generate_batches
 from sleuth_b200.engine.stepper import Stepper
+from sleuth_b200.sampling import DraftPolicy, SamplingConfig
+
+from test_drafts_loop import Drafting
 
 
 def bare_engine(book):
@@ -85,3 +89,12 @@ def test_pages_of_drafts_go_back_with_the_next_step(monkeypatch, step):
     assert s._drafted[b] == (60, 200)
     engine.accept([b], [[0, 1]])
     assert book.pages_in_use() == [2, 2] and int(book.lengths[b]) == 62
+
+
+def test_drafts_that_are_counted():
+    """Proposals count, and those that were right; not the tokens that fill a step up to one width."""
+    # one text repeats itself from the start, the other never, whose steps are filled up
+    be = Drafting(lambda text, u: text[-1] % 4 + 1 if text[0] == 1 else text[-1] + 1, max_len=400, n_pages=64)
+    circling, rising = generate_batches(be, [[1, 2, 3, 4] * 3, [50]], 24, SamplingConfig(temperature=0.0), stop_ids=(), max_batch=2, drafts=DraftPolicy(6))
+    assert rising.stats["drafted"] == rising.stats["drafts_taken"] == 0 and rising.new_ids == list(range(51, 75))
+    assert circling.stats["drafted"] == circling.stats["drafts_taken"] > 10
