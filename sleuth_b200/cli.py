@@ -73,7 +73,7 @@ def build_parser() -> argparse.ArgumentParser:
     s.add_argument("--keep-first", type=int, default=4, metavar="N", help="first tokens that stay (default 4)")
     s.add_argument("--keep-recent", type=int, default=None, metavar="N", help="latest tokens that stay under a budget (default: half of it)")
     s.add_argument("--draft-tokens", type=int, default=0, metavar="N",
-                   help="draft up to N tokens a step from the text so far and judge them at once; the output stays the same (0 = off)")
+                   help="draft up to N tokens a step from the text so far and judge them at once; the same choices up to the rounding of wider steps (0 = off)")
     s.add_argument("--draft-branches", type=int, default=None, metavar="N", help="continuations that a step tries (default 1)")
     s.add_argument("--draft-ngram", type=int, default=None, metavar="N", help="the longest phrase that is looked for in the text (default 3)")
     s.set_defaults(fn=cmd_generate)

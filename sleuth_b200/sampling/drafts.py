@@ -3,8 +3,9 @@
 ``DraftPolicy(tokens=8)``: before each step the latest tokens of a sequence are looked for further up in its text (the longest phrase
 of up to ``ngram`` tokens that occurs there), and what followed it then is drafted: up to ``tokens`` tokens, with ``branches`` > 1 as a
 tree of the continuations of several occurrences. One step then runs the newest token and all drafts; every draft
-that is the token which would have been chosen anyway is one step less. The choices are the same as without drafts, random ones too (a token's
-random number belongs to its place in the text, not to the step); only the sums of a step of several tokens differ from a single token's in their last bits.
+that is the token which would have been chosen anyway is one step less. The choices are made as without drafts, random ones too (a token's
+random number belongs to its place in the text, not to the step), from logits of a step of several tokens: in float32 its sums differ from a single token's in their
+last bits, in bfloat16 its products and its attention round otherwise, so choices between near-equal logits may differ, and the text behind them.
 
 Nothing here touches a GPU; the loop that uses it is ``engine/generate.py``, the step ``engine/stepper.py``. A text that
 repeats itself (code, tables, quotations) gains, another one pays a wider step for little.

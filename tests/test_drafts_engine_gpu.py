@@ -132,3 +132,87 @@ def test_refusals(tmp_path):
     other = Engine.from_config(tiny_rabadra.CONFIGS["A"], dtype="fp32", max_seq_len=64)
     with pytest.raises(ValueError, match="drafts"):
         other.step_tree([(other.open(1)[0], [1], [-1])])
+
+
+@pytest.mark.parametrize("name,dtype", [("A", "fp32"), ("D", "fp32"), ("F", "fp32"), ("G", "bf16")])
+@pytest.mark.parametrize("temperature", [0.0, 0.8])
+def test_drafts_of_another_model(tmp_path, name, dtype, temperature):
+    """The way of a program that drafts with a model of its own: step_tree, verify_drafts on its logits, accept, the chosen token as the next newest one. Every
+    judgement is the definition's on these logits, and at temperature 0 the text is the one that single-token steps choose."""
+    import sleuth_b200 as sb
+    from plain import drafts_plain
+    from sleuth_b200.kernels import ops
+    cfg = _folder(tmp_path, name, std=0.06)
+    vocab, dev = cfg["vocab_size"], "cuda:0"
+    engine = sb.load(tmp_path, dtype=dtype, max_seq_len=128, device=dev)
+    g, rng = torch.Generator().manual_seed(8), np.random.default_rng(8)
+    prompts = [rng.integers(0, vocab, n).tolist() for n in (9, 30, 4)]
+    slots = engine.open(3)
+    newest = engine.step([(s, p, (len(p) - 1,)) for s, p in zip(slots, prompts)]).argmax(1).tolist()
+    texts, taken = [[t] for t in newest], 0
+    tree = [-1, 0, 0, 0, 1, 2, 4]
+    n, c = len(slots), len(tree)
+    T, i32 = n * c, lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    parents, starts, counts = i32(tree * n), i32([c * i for i in range(n)]), i32([c] * n)
+    path, lengths, chosen = (torch.zeros(s, dtype=torch.int32, device=dev) for s in ((n, c), (n,), (n,)))
+    scratch = torch.zeros(max(1, ops.verify_drafts_scratch_words(n, T, vocab, True)), dtype=torch.int32, device=dev)
+    guess = engine.open(n)      # the drafting model: the same one, a token at a time, made to err now and then
+    for s, p in zip(guess, prompts):
+        engine.step([(s, p, ())])
+    for _ in range(8):
+        at = [engine.length(s) for s in guess]
+        likely = engine.step([(s, t[-1:], (0,)) for s, t in zip(guess, texts)]).cpu()
+        q = torch.softmax(2.0 * likely + torch.randn(likely.shape, generator=g), 1)
+        probs = torch.zeros((T, vocab))
+        tokens = torch.randint(0, vocab, (T,), generator=g, dtype=torch.int32)
+        for i in range(n):
+            tokens[c * i] = texts[i][-1]
+            probs[c * i:c * i + c] = torch.softmax(torch.randn((c, vocab), generator=g), 1)
+            probs[c * i] = q[i]
+            tokens[c * i + 1:c * i + 4] = torch.multinomial(q[i], 3, replacement=True, generator=g).to(torch.int32)
+        logits = engine.step_tree([(s, tokens[c * i:c * i + c].tolist(), tree) for i, s in enumerate(slots)])
+        uniforms = torch.rand(T, generator=g)
+        floors = torch.topk(logits, min(20, vocab), dim=1).values[:, -1].contiguous() if temperature else None
+        ops.verify_drafts(logits, vocab, tokens.to(dev), parents, starts, counts, uniforms.to(dev), temperature, path, lengths, chosen, c, probs=probs.to(dev), floors=floors,
+                          scratch=scratch)
+        paths = [p[:k] for p, k in zip(path.tolist(), lengths.tolist())]
+        for i in range(n):
+            rows = slice(c * i, c * i + c)
+            want = drafts_plain.verify(logits[rows].cpu(), tokens[rows], tree, uniforms[rows], temperature, vocab, probs[rows], None if floors is None else floors[rows].cpu())
+            assert (paths[i], int(chosen[i])) == want
+        engine.accept(slots, paths)
+        more = [[int(tokens[c * i + k]) for k in p[1:]] + [int(chosen[i])] for i, p in enumerate(paths)]
+        for s, text, m in zip(guess, texts, more):
+            if len(m) > 1:
+                engine.step([(s, m[:-1], ())])
+            text += m
+        taken += sum(len(m) - 1 for m in more)
+        assert [engine.length(s) for s in guess] == [engine.length(s) for s in slots] == [a + len(m) for a, m in zip(at, more)]
+    assert taken > 0
+    engine.close(slots + guess)
+    if temperature == 0.0 and dtype == "fp32":
+        plainly = engine.generate(prompts, max(map(len, texts)), sb.SamplingConfig(temperature=0.0), stop_ids=())
+        # (float32 sums of several rows and of one agree to some 1e-6 of the logits, and no two logits of these texts lie so near)
+        assert [r.new_ids[:len(t)] for r, t in zip(plainly, texts)] == texts
+
+
+@pytest.mark.parametrize("name", ["A", "E", "G"])
+@pytest.mark.parametrize("policy", [(6, 1, 3), (9, 3, 1)], ids=str)
+def test_bfloat16_choices_with_drafts(tmp_path, name, policy):
+    """In bfloat16 a step of several tokens rounds otherwise than one of a single token: a choice is the plain decoder's wherever its two largest logits lie further
+    apart than both sides' rounding."""
+    import sleuth_b200 as sb
+    cfg = _folder(tmp_path, name)
+    pc, pw = plain.read_model(tmp_path)
+    pw = {k: v.to(torch.bfloat16).float() for k, v in pw.items()}
+    longest = min(cfg["max_position_embeddings"], 200)
+    engine = sb.load(tmp_path, dtype="bf16", max_seq_len=longest, device="cuda:0")
+    rng = np.random.default_rng(5)
+    phrase = rng.integers(0, cfg["vocab_size"], 7).tolist()
+    prompts = [phrase * 4, phrase[:3] * 9 + phrase, rng.integers(0, cfg["vocab_size"], 12).tolist() * 2]
+    res = engine.generate(prompts, 40, sb.SamplingConfig(temperature=0.0), stop_ids=(), drafts=sb.DraftPolicy(*policy))
+    assert sum(r.stats["drafted"] for r in res) > 0
+    for r in res:
+        rows = plain.logits(pc, pw, r.prompt_ids + r.new_ids)[len(r.prompt_ids) - 1:-1].double()
+        short = rows.max(1).values - rows.gather(1, torch.tensor(r.new_ids)[:, None])[:, 0]
+        assert bool((short <= 2 * TOL["bf16"]["atol"]).all()), float(short.max())

@@ -540,6 +540,17 @@ def test_tables_that_the_kernel_in_front_writes(dtype, heads, kv_heads, dim):
         assert torch.equal(out.cpu().double(), wanted), again
 
 
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim", [HEADS[0], HEADS[2], HEADS[5], HEADS[6], HEADS[9]], ids=[IDS[i] for i in (0, 2, 5, 6, 9)])
+@pytest.mark.parametrize("window", [1, 5, 150, 2 ** 31 - 1])
+@pytest.mark.parametrize("far", [0, 3, 140, 2 ** 31])
+def test_positions_far_from_their_rows(dtype, heads, kv_heads, dim, window, far):
+    """Positions up to the last of 32 bits, far beyond the rows: what lies before the step and in the window is what counts, nothing where the window is short."""
+    step = Step(dtype, heads, kv_heads, dim, [200, 3], [6, 20], "random", 0, seed=11)
+    step.window = window
+    step.positions += min(far, 2 ** 31 - 1 - int(step.positions.max()))
+    step.check()
+
+
 # ------------------------------------------------------------------ verification ----
 
 class Judged:
