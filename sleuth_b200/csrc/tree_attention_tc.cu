@@ -10,8 +10,8 @@
 //   warp 3       walks the segments ahead of the others, leaves their descriptions and brings their queries, into the other of two buffers where they fit;
 //   warps 4..19  the softmax: two groups of 256 threads, two threads a row (32 keys of a page each), that take the pages in turn where the tile has up to 128 rows (each with a maximum, a sum
 //                and an accumulator of its own, joined at the segment's end), or every page for 128 rows each where it has more. The instruction takes no weights
-//                wider than bfloat16 beside bfloat16 values, so P goes in two parts, its upper 16 bits and those of the rest, which are multiplied one after the other: a
-//                weight is off by 2^-15 at most. The sum is of the whole weights, in 32 bits.
+//                wider than bfloat16 beside bfloat16 values, so P goes in two parts of 16 bits each, which are multiplied one after the other: a weight is off by 2^-14 at most. The sum is
+//                of the whole weights, in 32 bits.
 // What bounds it, measured on one B200 (calls back to back in a graph): 64 sequences of 150 to 4,096 rows, 8 nodes each, 32 / 8 heads of 128: 104 us, 5.0 TB/s,
 // where a copy reads 6.57; four of 9,000 to 30,000 rows 84 us, 5.1 TB/s. A block walks a page in 0.64 to 0.68 us (32 KB: 7 TB/s over all) and pays 4 to 5 us a
 // segment, the last product, the results and the next queries' wait: that is the rest. Eight trees of 40 to 64 nodes on 1,000 to 8,192 rows: 64 us where the bytes
@@ -538,14 +538,16 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
           }
           const f32x2 refs = both(m_used == -INFINITY || far ? 0.0f : -m_used), scales = both(ta.scale_log2);
           f32x2 sums = 0ull;
-          uint32_t pk[16], rest[16];      // the weights' upper 16 bits, and those of what is left of them
+          // The weights' upper 16 bits, less one in the last place, and the upper 16 bits of what is left: only a weight of nothing has a part that is nothing, so an
+          // infinity that all rows see is not multiplied by zero. What is lost is below 2^-14 of a weight.
+          uint32_t pk[16], rest[16];
 #pragma unroll
           for (int k = 0; k < 32; k += 2) {
             const f32x2 e = fma2(pair_of(__uint_as_float(sr[k]), __uint_as_float(sr[k + 1])), scales, refs);
             const float p0 = tt_ex2(__uint_as_float((uint32_t)e)), p1 = tt_ex2(__uint_as_float((uint32_t)(e >> 32)));
             const f32x2 p = pair_of(p0, p1);
-            pk[k >> 1] = __byte_perm(__float_as_uint(p0), __float_as_uint(p1), 0x7632);
-            const f32x2 low = fma2(pair_of(__uint_as_float(__float_as_uint(p0) & 0xffff0000u), __uint_as_float(__float_as_uint(p1) & 0xffff0000u)), both(-1.0f), p);
+            pk[k >> 1] = __viaddmax_s16x2(__byte_perm(__float_as_uint(p0), __float_as_uint(p1), 0x7632), 0xffffffffu, 0u);
+            const f32x2 low = fma2(pair_of(__uint_as_float(pk[k >> 1] << 16), __uint_as_float(pk[k >> 1] & 0xffff0000u)), both(-1.0f), p);
             rest[k >> 1] = __byte_perm((uint32_t)low, (uint32_t)(low >> 32), 0x7632);
             sums = add2(sums, p);
           }

@@ -440,11 +440,12 @@ def test_refused_calls():
 @pytest.mark.parametrize("dtype,heads,kv_heads,dim", HEADS, ids=IDS)
 @pytest.mark.parametrize("past,counts", [([0, 10, 60], [3, 6, 5]), ([700, 70], [4, 9]), ([0, 40] * 40, [2, 5] * 40), ([90, 5], [130, 140])], ids=["few", "long", "many", "broad"])
 def test_results_are_off_by_their_own_rounding(dtype, heads, kv_heads, dim, past, counts):
-    """In bfloat16 a result is rounded once, by half a step (2^-8 of it); weights are off by 2^-15 at most, beside what 32-bit sums leave (the oracle's slack)."""
+    """In bfloat16 a result is rounded once, by half a step (2^-8 of it); weights are off by 2^-14 at most (two parts of 16 bits, the first up to two steps of 2^-7
+    below the weight, the second cut to eight digits: 2^-6 2^-8), beside what 32-bit sums leave (the oracle's slack)."""
     step = Step(dtype, heads, kv_heads, dim, past, counts, "random", 0, seed=30)
     out = step.run()
     want, size, slack = step.want()
-    own, weights = (2.0 ** -8, 2.0 ** -15) if dtype == torch.bfloat16 else (2.0 ** -24, 2.0 ** -23)
+    own, weights = (2.0 ** -8, 2.0 ** -14) if dtype == torch.bfloat16 else (2.0 ** -24, 2.0 ** -23)
     err, allowed = (out - want).abs(), (slack[..., None] + weights) * size
     assert bool((err <= allowed * (1 + own) + own * want.abs() + 1e-30).all()), float((err / (allowed + own * want.abs() + 1e-30)).max())
 
@@ -486,8 +487,8 @@ def test_large_scores(dtype, heads, kv_heads, dim, past, counts, q0, k0, k1):
     want = _scores(step, q0, k0, k1, False)
     assert torch.equal(step.run(), want)
     want = _scores(step, q0, k0, k1, True)
-    # half a step of the result; a float32 sum's and quotient's, weights' parts (2^-15 of a weight, the same for both)
-    rounding = 2.0 ** -8 + 2.0 ** -14 if dtype == torch.bfloat16 else 2.0 ** -23
+    # half a step of the result; a float32 sum's and quotient's, weights' parts (2^-14 of a weight, the same for both)
+    rounding = 2.0 ** -8 + 2.0 ** -13 if dtype == torch.bfloat16 else 2.0 ** -23
     assert bool(((step.run() - want).abs() <= rounding * want.abs() + 1e-30).all())
 
 
@@ -549,6 +550,23 @@ def test_positions_far_from_their_rows(dtype, heads, kv_heads, dim, window, far)
     step.window = window
     step.positions += min(far, 2 ** 31 - 1 - int(step.positions.max()))
     step.check()
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim", [HEADS[2], HEADS[5], HEADS[6], HEADS[8], HEADS[9]], ids=[IDS[i] for i in (2, 5, 6, 8, 9)])
+@pytest.mark.parametrize("past,counts", [([200], [12]), ([400, 70] * 40, [3, 5] * 40), ([130, 64], [40, 256])], ids=["few", "many", "broad"])
+@pytest.mark.parametrize("sharp", [0.0, 1.5])
+def test_infinite_values_before_the_step(dtype, heads, kv_heads, dim, past, counts, sharp):
+    """An infinity among the values of a row that every node sees comes out in its channel, whatever its weight (where all scores are equal every weight is 1 and has
+    no second part), and leaves the other channels alone."""
+    step = Step(dtype, heads, kv_heads, dim, past, counts, "random", 0, seed=33, sharp=sharp)
+    clean = step.run()
+    for s, p in enumerate(past):
+        for row, channel, value in ((10, 1, math.inf), (p - 1, dim - 1, -math.inf)):
+            page, at = step.place(s, row)
+            step.v[page, :, at, channel] = value
+    out = step.run()
+    assert bool((out[..., 1] == math.inf).all()) and bool((out[..., dim - 1] == -math.inf).all())
+    assert torch.equal(out[..., 2:dim - 1], clean[..., 2:dim - 1]) and torch.equal(out[..., 0], clean[..., 0])
 
 
 # ------------------------------------------------------------------ verification ----
