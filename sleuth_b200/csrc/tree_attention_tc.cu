@@ -12,14 +12,18 @@
 //                and an accumulator of its own, joined at the segment's end), or every page for 128 rows each where it has more. The instruction takes no weights
 //                wider than bfloat16 beside bfloat16 values, so P goes in two parts of 16 bits each, which are multiplied one after the other: a weight is off by 2^-14 at most. The sum is
 //                of the whole weights, in 32 bits.
-// What bounds it, measured on one B200 (calls back to back in a graph): 64 sequences of 150 to 4,096 rows, 8 nodes each, 32 / 8 heads of 128: 104 us, 5.0 TB/s,
-// where a copy reads 6.57; four of 9,000 to 30,000 rows 84 us, 5.1 TB/s. A block walks a page in 0.64 to 0.68 us (32 KB: 7 TB/s over all) and pays 4 to 5 us a
-// segment, the last product, the results and the next queries' wait: that is the rest. Eight trees of 40 to 64 nodes on 1,000 to 8,192 rows: 64 us where the bytes
-// take 22; a page of 256 rows is 16,384 powers of two (1,024 cycles of their unit) and takes 0.93 us, 31 of the 64; the way in, the shares' 37 MB and the joining
-// are the rest. One chat, 5 tokens in a row on 2,000 rows, 16 / 8 heads, in clusters: 12.2 us, a chain of latencies around four pages a block.
-// The layouts before this one, in the same order (batch, trees): two blocks an SM 155 and 81 us, one with a thread a row 140 and 78, two threads a row 111 and 70,
+// What bounds it, measured on one B200 (calls back to back in a graph): 64 sequences of 150 to 4,096 rows, 8 nodes each, 32 / 8 heads of 128: 112 us, 4.7 TB/s,
+// where a copy reads 6.57; four of 9,000 to 30,000 rows 94 us, 4.6 TB/s; eight trees of 40 to 64 nodes on 1,000 to 8,192 rows 70 us where the bytes take 22; one
+// chat, 5 tokens in a row on 2,000 rows, 16 / 8 heads, in clusters, 11.2 us, a chain of latencies around four pages a block. Tensor pipe 46 to 48 % busy, issue 32
+// to 50 %: neither, but a page's chain of scores, softmax and products, which the ring of pages covers while the pages come, and 4 to 5 us of a segment's last
+// product, results and next queries, which nothing covers.
+// The second part of the weights costs 8, 12 and 9 % in the first three (103, 83 and 64 us with one part, nothing in the chat) and takes the error against 64 bits
+// from 2.3e-3 to 1.7e-3, that of the result's own rounding. With one part a block walked a page in 0.64 to 0.68 us (32 KB: 7 TB/s over all), one of 256 rows, 16,384
+// powers of two or 1,024 cycles of their unit, in 0.93; the way in, 37 MB of shares and the joining were the rest of the trees' time.
+// The layouts before this one, with one part (batch, trees): two blocks an SM 155 and 81 us, one with a thread a row 140 and 78, two threads a row 111 and 70,
 // and with segments weighed (kTtEntry) and shares joined from a list 100 and 64. The next page's scores asked for before this one's weights leave spill registers
-// (batch 112, trees 71); sums of the rounded weights instead of the exact ones cost 5 % and gain nothing (2.2e-3 against 2.3e-3).
+// (batch 112, trees 71); references before the scale throughout 106 and 67. With two parts: scores of two pages by one instruction of N = 128 gain nothing (batch 131
+// cold, 131 otherwise; long texts 107, 109), for the pages then wait for one another.
 // Where the sequences are few (tt_cluster) the blocks of a cluster share one (sequence, kv head, tile) instead: the shares meet in distributed shared memory, and
 // there is neither a second kernel nor scratch.
 // Rows are row r = node r / G, query head r % G of the group. Fewer than 128 rows leave the instruction's other rows to whatever lies behind the queries in shared
@@ -822,7 +826,7 @@ bool tree_tc_takes(int n_seqs, int max_count, int heads, int kv_heads, int head_
   return dtype == kBF16 && (head_dim == 64 || head_dim == 128) && n_seqs * tiles * kv_heads * (max_keys / 64 + 2ll + kTtEntry) < (1ll << 31);
 }
 
-// Whether blocks of a cluster share each (sequence, kv head, tile), and how many: one chat (5 tokens on 2,000 rows, 16 / 8 heads) takes 12.2 us so and 20.6 by runs
+// Whether blocks of a cluster share each (sequence, kv head, tile), and how many: one chat (5 tokens on 2,000 rows, 16 / 8 heads) takes 11.2 us so and 20.6 by runs
 // of units and a second kernel. A cluster waits for its longest sequence alone, so only where all clusters run at once (128 of the 148 blocks:
 // clusters of eight lie within one of the GPU's partitions each) and no block takes more than ten pages.
 static int tt_cluster(int n_seqs, int kv_heads, int tiles, int max_count, int max_keys, int window) {
@@ -876,7 +880,7 @@ static int launch_tree_tc(const CUtensorMap& mq, const CUtensorMap& mk, const CU
   static std::atomic<unsigned long long> allowed, allowed_clusters;
   cudaError_t e = ta.cluster ? allow_shared((const void*)tree_tc_kernel<HD, true>, 224 * 1024, allowed_clusters) : allow_shared((const void*)tree_tc_kernel<HD, false>, 224 * 1024, allowed);
   if (e != cudaSuccess) return fail(2, "attention_tree: cannot reserve shared memory: %s", cudaGetErrorString(e));
-  // (both may begin early: barriers and tensor memory are made while the kernel before ends. One chat, call after call: 12.2 us so, 14.4 one after the other)
+  // (both may begin early: barriers and tensor memory are made while the kernel before ends. One chat, call after call: 11.2 us so, two more one after the other)
   if (ta.cluster) {
     launch_clusters(pdl_mode() != 0, (unsigned)ta.cluster, tree_tc_kernel<HD, true>, dim3(ta.cluster * ta.t.kv_heads * ta.tiles * ta.t.n_seqs), dim3(kTtThreads), (size_t)ta.lay.total, s, mq, mk, mv, ta);
     return check_launch("attention_tree (tensor cores, clusters)");

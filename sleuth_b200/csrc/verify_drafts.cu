@@ -18,13 +18,15 @@
 // table of 64 and four terms of the series; in 64 bits, of which an SM does 16 operations a clock, a pass over a row took 7.5 us in eight blocks, four fifths of
 // them waiting for that unit). A refusal takes one pass: the sums of exp, and of exp and of q over the tokens where exp / Z > c q as far as 32 bits tell, make both
 // the exact Z and F (a token on the wrong side is off by 1e-7 of itself, and one in a million is).
-// Measured (one B200, device, 151,936 tokens): one sequence of five drafts with distributions 21 us, 64 sequences of two to five 75 (the first kernel 32 for 137 MB,
-// 4.3 TB/s; the second 48 in clusters of two, one pass of some 60 instructions a token and one of 300 tokens by the block that draws), eight trees of 15 to 23
+// Measured (one B200, device, 151,936 tokens): one sequence of five drafts with distributions 21 us, 64 sequences of two to five 77 (the first kernel 32 for 137 MB,
+// 4.2 TB/s; the second 50 in clusters of two, one pass of some 60 instructions a token and one of 300 tokens by the block that draws), eight trees of 15 to 23
 // certain drafts 36 (19 and 23). Steps before: every row by the blocks of its sequence, in 64 bits 45, 128 and 27; sums of all nodes first, 64-bit powers 27, 91 and
 // 45; pairs of 32-bit numbers, clusters of sixteen blocks of 512 threads 18, 86 and 38; of 1,024 threads 21, 75 and 37, which is kept: a batch has fewer blocks a
 // sequence and gains most.
-// Sums first or row by row: eight trees 36 against 27 before, whose ways are short and whose trees wide, but chats and batches 21 against 45 and 75 against 128, and
-// which it is depends on what is accepted, which no rule can know.
+// Sums first or row by row, both in the present form, drafts certain (which need no pass for a refusal): eight trees whose first draft is refused 36 and 37 us, whose
+// first drafts are right 43 and 108; 64 chains 62 and 85, 80 and 193; at temperature 0 the trees 28 and 18, 33 and 62, the chains 36 and 45, 56 and 106. Row by row
+// gains 10 us where a greedy tree is refused at once and loses 30 to 110 where drafts are right; what will be accepted is not known before, so sums come first, with
+// distributions and without.
 #include <float.h>
 #include <math.h>
 

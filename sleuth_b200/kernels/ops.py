@@ -2016,7 +2016,7 @@ def attention_tree(q, k_pool, v_pool, out, seq_start, past, counts, seen, positi
 
 
 def verify_drafts_scratch_words(n_seqs: int, tokens: int, limit: int, drawn: bool) -> int:
-    """int32 words of scratch that ``verify_drafts`` takes; ``drawn``: with ``probs``."""
+    """int32 words of scratch that ``verify_drafts`` takes; ``drawn``: with ``probs`` (the words are the same without)."""
     fn = lib().dll.slb_verify_drafts_scratch
     fn.argtypes, fn.restype = [ctypes.c_int, ctypes.c_longlong, ctypes.c_int, ctypes.c_int], ctypes.c_longlong
     _fits_int("verify_drafts", n_seqs, limit)
